@@ -24,7 +24,11 @@ EXPORTS = ("hb_abi_version", "hb_last_error", "hb_kernel_launch_count", "hb_set_
            "hb_norm_scan", "hb_norm_scan_noalloc", "hb_merge_topk", "hb_pair_costs_workspace", "hb_pair_costs", "hb_restricted_ot_workspace",
            "hb_restricted_ot_solve", "hb_filter_new_pairs_workspace", "hb_filter_new_pairs",
            "hb_prune_select_workspace", "hb_prune_select", "hb_norm_scan_ex", "hb_norm_topk_ex",
-           "hb_pair_costs_ex", "hb_l2sq_last_rescans")
+           "hb_pair_costs_ex", "hb_l2sq_last_rescans", "hb_index_sort_workspace", "hb_index_sort",
+           "hb_route_dispatch", "hb_route_combine", "hb_route_combine_grad", "hb_embedding_lookup",
+           "hb_embedding_grad_workspace", "hb_embedding_grad", "hb_clip_workspace", "hb_grad_norm",
+           "hb_clip_grad_norm")
+FLOAT_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # HB_F32, HB_F16, HB_BF16
 
 
 class HBError(RuntimeError):
@@ -135,6 +139,30 @@ def load_library(path: Path | str = LIB_PATH):
     lib.hb_restricted_ot_solve.argtypes = [P, P, P, c_int64, P, c_int64, c_int64, P, P, POINTER(PdlpControls), P, P,
                                            POINTER(PdlpInfo), POINTER(PdlpTraceRow), c_int32, POINTER(c_int32), P,
                                            c_size_t, P]
+    lib.hb_index_sort_workspace.restype = c_size_t
+    lib.hb_index_sort_workspace.argtypes = [c_int64, c_int64]
+    lib.hb_index_sort.restype = c_int
+    lib.hb_index_sort.argtypes = [P, c_int, c_int64, c_int64, P, P, P, P, c_size_t, P]
+    lib.hb_route_dispatch.restype = c_int
+    lib.hb_route_dispatch.argtypes = [c_int, P, c_int64, c_int64, c_int64, c_int64, P, P, P, P]
+    lib.hb_route_combine.restype = c_int
+    lib.hb_route_combine.argtypes = [c_int, P, c_int64, c_int64, c_int64, c_int64, P, P, P, c_int, P, P]
+    lib.hb_route_combine_grad.restype = c_int
+    lib.hb_route_combine_grad.argtypes = [c_int, P, c_int64, P, c_int64, c_int64, c_int64, c_int64, P, P, P, c_int, P,
+                                          P, P]
+    lib.hb_embedding_lookup.restype = c_int
+    lib.hb_embedding_lookup.argtypes = [c_int, P, c_int64, c_int64, c_int64, P, c_int, c_int64, c_double, P, P]
+    lib.hb_embedding_grad_workspace.restype = c_size_t
+    lib.hb_embedding_grad_workspace.argtypes = [c_int64, c_int64, c_int64]
+    lib.hb_embedding_grad.restype = c_int
+    lib.hb_embedding_grad.argtypes = [c_int, P, c_int64, P, c_int, c_int64, c_int64, c_int64, c_double, c_int, P, c_int,
+                                      P, c_size_t, P]
+    lib.hb_clip_workspace.restype = c_size_t
+    lib.hb_clip_workspace.argtypes = [c_int64]
+    lib.hb_grad_norm.restype = c_int
+    lib.hb_grad_norm.argtypes = [c_int64, P, P, P, P, P, c_size_t, P]
+    lib.hb_clip_grad_norm.restype = c_int
+    lib.hb_clip_grad_norm.argtypes = [c_int64, P, P, P, P, P, c_double, P, P, c_size_t, P]
     if lib.hb_abi_version() != ABI_VERSION:
         raise HBError(HB_BAD_ARGUMENT, f"libhello_b200 ABI {lib.hb_abi_version()} != {ABI_VERSION}; rebuild")
     _LIB = lib
@@ -179,6 +207,59 @@ def ptr(t) -> int | None:
 
 def stream_handle(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def on_device(what: str, *tensors):
+    """The loaded library, after checking that all tensors are on one CUDA device."""
+    device = tensors[0].get_device()
+    for t in tensors:
+        if not t.is_cuda:
+            lib()  # without CUDA: the library's own error
+            raise ValueError(f"{what}: expected CUDA tensors")
+        if t.get_device() != device:
+            raise ValueError(f"{what}: tensors on different devices")
+    return _LIB or load_library()
+
+
+class current:
+    """``with current(t) as stream``: t's device made current, and its current stream's handle."""
+
+    __slots__ = ("device", "before")
+
+    def __init__(self, t):
+        self.device = t.get_device()
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.device:
+            torch.cuda.set_device(self.device)
+        return torch._C._cuda_getCurrentRawStream(self.device)
+
+    def __exit__(self, *_):
+        if self.before != self.device:
+            torch.cuda.set_device(self.before)
+
+
+def feature_rows(t, what: str):
+    """(t, row stride in elements) of a 2-D tensor of features whose rows are contiguous; a copy where they are not."""
+    if t.dim() != 2:
+        raise ValueError(f"{what} must be 2-D (rows x features), got {tuple(t.shape)}")
+    if t.dtype not in FLOAT_TYPES:
+        raise ValueError(f"{what} must be float32, float16 or bfloat16, got {t.dtype}")
+    rows, stride = t.shape[0], t.stride()
+    if t.shape[1] > 1 and stride[1] != 1:
+        t = t.contiguous()
+        return t, t.shape[1]
+    return t, stride[0] if rows > 1 else t.shape[1]
+
+
+def index_bytes(t, what: str) -> int:
+    """4 or 8 for an int32 or int64 tensor."""
+    if t.dtype == torch.int64:
+        return 8
+    if t.dtype == torch.int32:
+        return 4
+    raise ValueError(f"{what} must be int32 or int64, got {t.dtype}")
 
 
 class Workspace:

@@ -1,0 +1,302 @@
+// The global norm of many gradients, and the gradients scaled down to a limit.
+//
+//   norm = sqrt(sum over all tensors of g^2),  f = min(1, limit / (norm + 1e-6)),  out = f g
+//
+// Two launches over one list of chunks: the first leaves one fp64 sum of squares a
+// block, the second adds those in order in every block, so nothing waits on an
+// atomic and the result does not depend on the launch.  Bound by HBM: g is read
+// twice and written once.  The second launch goes through the chunks backwards, so
+// that it finds in L2 what the first read last.
+//
+// Squares are added in fp32 over at most 32 values and in fp64 from there on.  A
+// group whose fp32 sum is so small or so large that squares were lost or overflowed
+// is added again in fp64, so the norm of finite gradients is finite wherever fp32
+// can hold it.
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+#include "internal.h"
+#include "rows.cuh"
+
+namespace hb {
+namespace clip {
+
+constexpr int kThreads = 256;
+constexpr int64_t kChunk = 8192;  // elements
+constexpr int kMostBlocks = 148 * 8;
+constexpr double kEps = 1e-6;
+
+// A list of tensors in the kernel's parameters: no copy to the device.
+template <int MOST>
+struct List {
+    const void* in[MOST];
+    void* out[MOST];
+    int64_t size[MOST];
+    int32_t first[MOST + 1];  // first chunk of each tensor
+    uint8_t type[MOST], out_type[MOST];
+    int count;
+};
+constexpr int kFew = 64, kMany = 1024;  // 1.9 KB and 30 KB of parameters (32 KB is the most)
+
+template <int MOST>
+__device__ __forceinline__ int tensor_of(const List<MOST>& l, int chunk) {
+    int lo = 0, hi = l.count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (l.first[mid] <= chunk) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ double block_sum(double v) {
+    __shared__ double part[kThreads / 32];
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    double r = 0.0;
+#pragma unroll
+    for (int i = 0; i < kThreads / 32; ++i) r += part[i];
+    return r;
+}
+
+// Sum of squares of n values: fp32, or fp64 where fp32 would lose them.
+template <int N>
+__device__ __forceinline__ double squares(const float (&f)[N]) {
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) s = fmaf(f[i], f[i], s);
+    if (s >= 1e-24f && s <= 3e38f) return (double)s;
+    double d = 0.0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) d = fma((double)f[i], (double)f[i], d);
+    return d;
+}
+
+template <typename T>
+__device__ __forceinline__ double chunk_squares(const T* p, int n) {
+    using V = rows::Vec<T, 16>;
+    constexpr int U = 4;
+    double sum = 0.0;
+    int done = 0;
+    if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+        const int whole = n / V::N;
+        for (int i = threadIdx.x; i < whole; i += kThreads * U) {
+            V v[U];
+            float f[U * V::N];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (i + u * kThreads < whole) v[u].load(p + (int64_t)(i + u * kThreads) * V::N);
+                else v[u].zero();
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int j = 0; j < V::N; ++j) f[u * V::N + j] = rows::to_float(v[u].v[j]);
+            sum += squares(f);
+        }
+        done = whole * V::N;
+    }
+    for (int i = done + threadIdx.x; i < n; i += kThreads) {
+        const float f[1] = {rows::to_float(p[i])};
+        sum += squares(f);
+    }
+    return sum;
+}
+
+template <int MOST>
+__global__ void __launch_bounds__(kThreads) square_kernel(const __grid_constant__ List<MOST> l, double* __restrict__ partial) {
+    double sum = 0.0;
+    for (int chunk = blockIdx.x; chunk < l.first[l.count]; chunk += gridDim.x) {
+        const int t = tensor_of(l, chunk);
+        const int64_t at = (int64_t)(chunk - l.first[t]) * kChunk;
+        const int n = (int)min(kChunk, l.size[t] - at);
+        if (l.type[t] == HB_F32) sum += chunk_squares(static_cast<const float*>(l.in[t]) + at, n);
+        else if (l.type[t] == HB_F16) sum += chunk_squares(static_cast<const __half*>(l.in[t]) + at, n);
+        else sum += chunk_squares(static_cast<const __nv_bfloat16*>(l.in[t]) + at, n);
+    }
+    sum = block_sum(sum);
+    if (threadIdx.x == 0) partial[blockIdx.x] = sum;
+}
+
+__device__ __forceinline__ double total_norm(const double* partial, int partials) {
+    double s = 0.0;
+    for (int i = threadIdx.x; i < partials; i += kThreads) s += partial[i];
+    return sqrt(block_sum(s));
+}
+
+__global__ void __launch_bounds__(kThreads) norm_kernel(const double* __restrict__ partial, int partials,
+                                                        float* __restrict__ norm) {
+    const double n = total_norm(partial, partials);
+    if (threadIdx.x == 0) *norm = (float)n;
+}
+
+template <typename T, typename TO>
+__device__ __forceinline__ void scale_chunk(const T* p, TO* out, int n, float f) {
+    constexpr int N = 16 / (int)sizeof(T), kPieces = N * (int)sizeof(TO) / 16;
+    using V = rows::Vec<T, 16>;
+    using O = rows::Vec<TO, 16>;
+    constexpr int U = 4;
+    int done = 0;
+    if (((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(out)) & 15) == 0) {
+        const int whole = n / N;
+        for (int i = threadIdx.x; i < whole; i += kThreads * U) {
+            V v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (i + u * kThreads < whole) v[u].raw = *reinterpret_cast<const uint4*>(p + (int64_t)(i + u * kThreads) * N);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (i + u * kThreads < whole) {
+#pragma unroll
+                    for (int q = 0; q < kPieces; ++q) {
+                        O o;
+#pragma unroll
+                        for (int j = 0; j < O::N; ++j)
+                            o.v[j] = rows::from_float<TO>(f * rows::to_float(v[u].v[q * O::N + j]));
+                        o.store(out + (int64_t)(i + u * kThreads) * N + q * O::N);
+                    }
+                }
+        }
+        done = whole * N;
+    }
+    for (int i = done + threadIdx.x; i < n; i += kThreads) out[i] = rows::from_float<TO>(f * rows::to_float(p[i]));
+}
+
+template <int MOST>
+__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ List<MOST> l,
+                                                         const double* __restrict__ partial, int partials, double limit,
+                                                         float* __restrict__ norm) {
+    const double n = total_norm(partial, partials);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
+    const double r = limit / (n + kEps);
+    const float f = r >= 1.0 ? 1.0f : (float)r;  // a NaN stays
+    for (int c = blockIdx.x; c < l.first[l.count]; c += gridDim.x) {
+        const int chunk = l.first[l.count] - 1 - c;
+        const int t = tensor_of(l, chunk);
+        if (f == 1.0f && l.in[t] == l.out[t]) continue;
+        const int64_t at = (int64_t)(chunk - l.first[t]) * kChunk;
+        const int m = (int)min(kChunk, l.size[t] - at);
+        const int type = l.type[t], to = l.out_type[t];
+        if (type == HB_F32) {
+            scale_chunk(static_cast<const float*>(l.in[t]) + at, static_cast<float*>(l.out[t]) + at, m, f);
+        } else if (type == HB_F16) {
+            const __half* p = static_cast<const __half*>(l.in[t]) + at;
+            if (to == HB_F32) scale_chunk(p, static_cast<float*>(l.out[t]) + at, m, f);
+            else scale_chunk(p, static_cast<__half*>(l.out[t]) + at, m, f);
+        } else {
+            const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(l.in[t]) + at;
+            if (to == HB_F32) scale_chunk(p, static_cast<float*>(l.out[t]) + at, m, f);
+            else scale_chunk(p, static_cast<__nv_bfloat16*>(l.out[t]) + at, m, f);
+        }
+    }
+}
+
+// The tensors from..to of the caller's list that hold elements.
+template <int MOST>
+int fill(List<MOST>& l, int64_t from, int64_t to, const void* const* in, const int64_t* size, const int32_t* type,
+         void* const* out, const int32_t* out_type) {
+    l.count = 0;
+    int64_t chunks = 0;
+    for (int64_t i = from; i < to; ++i) {
+        if (size[i] == 0) continue;
+        const int t = l.count++;
+        l.in[t] = in[i];
+        l.out[t] = out ? out[i] : nullptr;
+        l.size[t] = size[i];
+        l.type[t] = (uint8_t)type[i];
+        l.out_type[t] = (uint8_t)(out ? out_type[i] : type[i]);
+        l.first[t] = (int32_t)chunks;
+        chunks += (size[i] + kChunk - 1) / kChunk;
+    }
+    l.first[l.count] = (int32_t)chunks;
+    return (int)chunks;
+}
+
+inline int blocks_of(int chunks) { return std::max(1, std::min(chunks, kMostBlocks)); }
+
+template <int MOST>
+cudaError_t run(int64_t count, const void* const* in, const int64_t* size, const int32_t* type, void* const* out,
+                const int32_t* out_type, double limit, float* norm, double* partial, cudaStream_t st) {
+    List<MOST> l;
+    int partials = 0;
+    for (int64_t from = 0; from < count || from == 0; from += MOST) {
+        const int blocks = blocks_of(fill(l, from, std::min(count, from + MOST), in, size, type, out, out_type));
+        square_kernel<MOST><<<blocks, kThreads, 0, st>>>(l, partial + partials);
+        count_launches(1);
+        partials += blocks;
+    }
+    if (!out) {
+        norm_kernel<<<1, kThreads, 0, st>>>(partial, partials, norm);
+        count_launches(1);
+        return cudaGetLastError();
+    }
+    for (int64_t from = 0; from < count || from == 0; from += MOST) {
+        if (count > MOST) fill(l, from, std::min(count, from + MOST), in, size, type, out, out_type);
+        scale_kernel<MOST><<<blocks_of(l.first[l.count]), kThreads, 0, st>>>(l, partial, partials, limit, norm);
+        count_launches(1);
+    }
+    return cudaGetLastError();
+}
+
+int check(int64_t count, const void* const* in, const int64_t* size, const int32_t* type, const float* norm,
+          const void* ws, size_t ws_bytes) {
+    if (count < 0 || count > INT32_MAX) return abi_fail(HB_BAD_ARGUMENT, "gradient norm: number of tensors out of range");
+    if (!norm || !ws || (count > 0 && (!in || !size || !type)))
+        return abi_fail(HB_BAD_ARGUMENT, "gradient norm: null pointer");
+    int64_t chunks = 0;
+    for (int64_t i = 0; i < count; ++i) {
+        if (size[i] < 0 || !rows::valid_type(type[i]) || (size[i] > 0 && !in[i]))
+            return abi_fail(HB_BAD_ARGUMENT, "gradient norm: size, type or pointer of a tensor");
+        if (size[i] > INT32_MAX * kChunk || (chunks += (size[i] + kChunk - 1) / kChunk) > INT32_MAX)
+            return abi_fail(HB_BAD_ARGUMENT, "gradient norm: too many elements");
+    }
+    if (ws_bytes < hb_clip_workspace(count)) return abi_fail(HB_WORKSPACE, "workspace smaller than hb_clip_workspace()");
+    return HB_OK;
+}
+
+int start(int64_t count, const void* const* in, const int64_t* size, const int32_t* type, void* const* out,
+          const int32_t* out_type, double limit, float* norm, void* ws, void* stream) {
+    const auto st = static_cast<cudaStream_t>(stream);
+    double* partial = static_cast<double*>(ws);
+    const cudaError_t e = count <= kFew ? run<kFew>(count, in, size, type, out, out_type, limit, norm, partial, st)
+                                        : run<kMany>(count, in, size, type, out, out_type, limit, norm, partial, st);
+    return e == cudaSuccess ? HB_OK : abi_fail(HB_LAUNCH, std::string("gradient norm: ") + cudaGetErrorString(e));
+}
+
+}  // namespace clip
+}  // namespace hb
+
+using namespace hb;
+using namespace hb::clip;
+
+extern "C" size_t hb_clip_workspace(int64_t count) {
+    if (count < 0) return 0;
+    return sizeof(double) * kMostBlocks * (size_t)std::max<int64_t>(1, (count + kMany - 1) / kMany);
+}
+
+extern "C" int hb_grad_norm(int64_t count, const void* const* grads, const int64_t* sizes, const int32_t* types,
+                            float* norm, void* workspace, size_t workspace_bytes, void* stream) {
+    const int rc = check(count, grads, sizes, types, norm, workspace, workspace_bytes);
+    if (rc) return rc;
+    return start(count, grads, sizes, types, nullptr, nullptr, 0.0, norm, workspace, stream);
+}
+
+extern "C" int hb_clip_grad_norm(int64_t count, const void* const* grads, const int64_t* sizes, const int32_t* types,
+                                 void* const* outs, const int32_t* out_types, double limit, float* norm,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
+    const int rc = check(count, grads, sizes, types, norm, workspace, workspace_bytes);
+    if (rc) return rc;
+    if (!(limit >= 0.0)) return abi_fail(HB_BAD_ARGUMENT, "gradient clipping: the limit must be a number >= 0");
+    if (count > 0 && (!outs || !out_types)) return abi_fail(HB_BAD_ARGUMENT, "gradient clipping: null pointer");
+    for (int64_t i = 0; i < count; ++i)
+        if (sizes[i] > 0 && (!outs[i] || (out_types[i] != types[i] && out_types[i] != HB_F32)))
+            return abi_fail(HB_BAD_ARGUMENT, "gradient clipping: an output has its gradient's type or is fp32");
+    static void* const none[1] = {nullptr};
+    static const int32_t any[1] = {HB_F32};
+    return start(count, grads, sizes, types, count > 0 ? outs : none, count > 0 ? out_types : any, limit, norm, workspace,
+                 stream);
+}

@@ -355,6 +355,72 @@ int hb_prune_select(const int32_t* rows, const int32_t* cols, const double* cost
                     int64_t n_target, int32_t current_inner_iter, int64_t num_to_remove, int32_t* positions,
                     int64_t* removable_count, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Routed layers: an assignment of tokens to experts (a transport plan between
+ * tokens and experts, or a router's choice) applied to rows of features, rows of
+ * a table looked up by index, and the norm of the gradients of it all.  No
+ * counterpart in the reference, which stops at the plan.
+ *
+ * These entry points only enqueue work on `stream`: they neither synchronise nor
+ * keep anything between calls, and can be captured in a graph.  Element types
+ * are HB_F32, HB_F16 and HB_BF16; arithmetic and sums are fp32 or wider and a
+ * result is rounded once.  Rows are `width` contiguous elements, `*_stride`
+ * elements apart; row arrays without a stride argument are dense.  Results do
+ * not depend on launch order (no floating-point atomics).
+ * ------------------------------------------------------------------------- */
+enum { HB_F32 = 0, HB_F16 = 1, HB_BF16 = 2 };
+
+/* Stable sort of entries by expert.  index: `entries` int32 or int64 (index_bytes
+ * 4 or 8) values; one outside 0..bins-1 has no expert.  order (entries): the entry
+ * of each place, those without an expert last; position (entries): its inverse;
+ * offsets (bins + 1): first place of each expert, offsets[bins] = entries that have
+ * an expert. */
+size_t hb_index_sort_workspace(int64_t entries, int64_t bins);
+int hb_index_sort(const void* index, int index_bytes, int64_t entries, int64_t bins, int32_t* order,
+                  int32_t* position, int32_t* offsets, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Moves between tokens and sorted entries.  Entry t * slots + k belongs to token t;
+ * position as hb_index_sort gives it; kept (device): how many places have an expert
+ * (its offsets[bins]).  `sorted`, z and dz hold tokens * slots rows.
+ *   dispatch      sorted[position[t,k]] = x[t], zero rows from place `kept` on
+ *   combine       out[t] = sum_k weights[t,k] z[position[t,k]] over places below kept;
+ *                 weights null: all 1 (this is also dispatch's gradient)
+ *   combine_grad  dz[position[t,k]] = weights[t,k] dy[t], zero from `kept` on;
+ *                 dweights[t,k] = <dy[t], z[position[t,k]]>, 0 from `kept` on (null: not computed)
+ * weights and dweights (tokens x slots, dense) are of weight_type.  Rows of z at or
+ * above place `kept` are not read.  A position outside 0..tokens*slots-1 is skipped. */
+int hb_route_dispatch(int type, const void* x, int64_t x_stride, int64_t tokens, int64_t slots, int64_t width,
+                      const int32_t* position, const int32_t* kept, void* sorted, void* stream);
+int hb_route_combine(int type, const void* z, int64_t z_stride, int64_t tokens, int64_t slots, int64_t width,
+                     const int32_t* position, const int32_t* kept, const void* weights, int weight_type, void* out,
+                     void* stream);
+int hb_route_combine_grad(int type, const void* dy, int64_t dy_stride, const void* z, int64_t z_stride, int64_t tokens,
+                          int64_t slots, int64_t width, const int32_t* position, const int32_t* kept,
+                          const void* weights, int weight_type, void* dz, void* dweights, void* stream);
+
+/* out[i] = scale * table[ids[i]], a zero row for an id outside 0..rows-1.  ids: int32 or
+ * int64 (id_bytes).  The gradient is dense: out[v] = scale * sum of dy[i] over ids[i] = v,
+ * of dy's type or fp32; accumulate != 0 adds to out instead and leaves other rows alone. */
+int hb_embedding_lookup(int type, const void* table, int64_t table_stride, int64_t rows, int64_t width, const void* ids,
+                        int id_bytes, int64_t n, double scale, void* out, void* stream);
+size_t hb_embedding_grad_workspace(int64_t n, int64_t rows, int64_t width);
+int hb_embedding_grad(int type, const void* dy, int64_t dy_stride, const void* ids, int id_bytes, int64_t n,
+                      int64_t rows, int64_t width, double scale, int out_type, void* out, int accumulate,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* Global norm of `count` tensors: norm = sqrt(sum of squares of all their elements),
+ * one fp32 on the device.  grads, sizes, types, outs and out_types are HOST arrays
+ * (device pointers, element counts, element types).  clip writes
+ * outs[i] = grads[i] * min(1, limit / (norm + 1e-6)), outs[i] == grads[i] for in place,
+ * of the gradient's type or fp32; a NaN norm makes every output NaN.  Tensors must not
+ * overlap one another. */
+size_t hb_clip_workspace(int64_t count);
+int hb_grad_norm(int64_t count, const void* const* grads, const int64_t* sizes, const int32_t* types, float* norm,
+                 void* workspace, size_t workspace_bytes, void* stream);
+int hb_clip_grad_norm(int64_t count, const void* const* grads, const int64_t* sizes, const int32_t* types,
+                      void* const* outs, const int32_t* out_types, double limit, float* norm, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
