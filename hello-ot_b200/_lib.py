@@ -28,6 +28,8 @@ EXPORTS = ("hb_abi_version", "hb_last_error", "hb_kernel_launch_count", "hb_set_
            "hb_route_dispatch", "hb_route_combine", "hb_route_combine_grad", "hb_embedding_lookup",
            "hb_embedding_grad_workspace", "hb_embedding_grad", "hb_clip_workspace", "hb_grad_norm",
            "hb_clip_grad_norm")
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
 FLOAT_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # HB_F32, HB_F16, HB_BF16
 
 
@@ -209,35 +211,25 @@ def stream_handle(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def on_device(what: str, *tensors):
-    """The loaded library, after checking that all tensors are on one CUDA device."""
+def device_of(what: str, *tensors) -> int:
+    """The one CUDA device of all tensors, by index."""
     device = tensors[0].get_device()
     for t in tensors:
-        if not t.is_cuda:
+        if t.get_device() != device or device < 0:
             lib()  # without CUDA: the library's own error
-            raise ValueError(f"{what}: expected CUDA tensors")
-        if t.get_device() != device:
-            raise ValueError(f"{what}: tensors on different devices")
-    return _LIB or load_library()
+            raise ValueError(f"{what}: expected CUDA tensors on one device, got {[str(t.device) for t in tensors]}")
+    return device
 
 
-class current:
-    """``with current(t) as stream``: t's device made current, and its current stream's handle."""
-
-    __slots__ = ("device", "before")
-
-    def __init__(self, t):
-        self.device = t.get_device()
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.device:
-            torch.cuda.set_device(self.device)
-        return torch._C._cuda_getCurrentRawStream(self.device)
-
-    def __exit__(self, *_):
-        if self.before != self.device:
-            torch.cuda.set_device(self.before)
+def call(device: int, function, *args) -> None:
+    """function(*args, stream) on the device's current stream, with the device current."""
+    if torch.cuda.current_device() == device:
+        rc = function(*args, _raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = function(*args, _raw_stream(device))
+    if rc:
+        check(rc)
 
 
 def feature_rows(t, what: str):

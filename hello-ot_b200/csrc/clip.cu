@@ -6,7 +6,9 @@
 // block, the second adds those in order in every block, so nothing waits on an
 // atomic and the result does not depend on the launch.  Bound by HBM: g is read
 // twice and written once.  The second launch goes through the chunks backwards, so
-// that it finds in L2 what the first read last.
+// that it finds in L2 what the first read last.  Up to a million elements the time
+// is launches: one cluster of blocks does both steps in one, with its hardware
+// barrier between them.
 //
 // Squares are added in fp32 over at most 32 values and in fp64 from there on.  A
 // group whose fp32 sum is so small or so large that squares were lost or overflowed
@@ -16,6 +18,8 @@
 #include <cmath>
 #include <string>
 
+#include <cooperative_groups.h>
+
 #include "internal.h"
 #include "rows.cuh"
 
@@ -23,7 +27,9 @@ namespace hb {
 namespace clip {
 
 constexpr int kThreads = 256;
-constexpr int64_t kChunk = 8192;  // elements
+constexpr int64_t kChunk = 8192, kSmallChunk = 2048;  // elements
+constexpr int64_t kSmallMost = 1 << 20;               // elements of the one-launch form
+constexpr int kCluster = 16;
 constexpr int kMostBlocks = 148 * 8;
 constexpr double kEps = 1e-6;
 
@@ -35,7 +41,7 @@ struct List {
     int64_t size[MOST];
     int32_t first[MOST + 1];  // first chunk of each tensor
     uint8_t type[MOST], out_type[MOST];
-    int count;
+    int count, chunk;  // tensors, elements a chunk
 };
 constexpr int kFew = 64, kMany = 1024;  // 1.9 KB and 30 KB of parameters (32 KB is the most)
 
@@ -107,18 +113,24 @@ __device__ __forceinline__ double chunk_squares(const T* p, int n) {
     return sum;
 }
 
+// This block's sum of squares.
 template <int MOST>
-__global__ void __launch_bounds__(kThreads) square_kernel(const __grid_constant__ List<MOST> l, double* __restrict__ partial) {
+__device__ __forceinline__ double list_squares(const List<MOST>& l) {
     double sum = 0.0;
     for (int chunk = blockIdx.x; chunk < l.first[l.count]; chunk += gridDim.x) {
         const int t = tensor_of(l, chunk);
-        const int64_t at = (int64_t)(chunk - l.first[t]) * kChunk;
-        const int n = (int)min(kChunk, l.size[t] - at);
+        const int64_t at = (int64_t)(chunk - l.first[t]) * l.chunk;
+        const int n = (int)min((int64_t)l.chunk, l.size[t] - at);
         if (l.type[t] == HB_F32) sum += chunk_squares(static_cast<const float*>(l.in[t]) + at, n);
         else if (l.type[t] == HB_F16) sum += chunk_squares(static_cast<const __half*>(l.in[t]) + at, n);
         else sum += chunk_squares(static_cast<const __nv_bfloat16*>(l.in[t]) + at, n);
     }
-    sum = block_sum(sum);
+    return block_sum(sum);
+}
+
+template <int MOST>
+__global__ void __launch_bounds__(kThreads) square_kernel(const __grid_constant__ List<MOST> l, double* __restrict__ partial) {
+    const double sum = list_squares(l);
     if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
 
@@ -166,20 +178,19 @@ __device__ __forceinline__ void scale_chunk(const T* p, TO* out, int n, float f)
     for (int i = done + threadIdx.x; i < n; i += kThreads) out[i] = rows::from_float<TO>(f * rows::to_float(p[i]));
 }
 
+__device__ __forceinline__ float factor_of(double norm, double limit) {
+    const double r = limit / (norm + kEps);
+    return r >= 1.0 ? 1.0f : (float)r;  // a NaN stays
+}
+
 template <int MOST>
-__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ List<MOST> l,
-                                                         const double* __restrict__ partial, int partials, double limit,
-                                                         float* __restrict__ norm) {
-    const double n = total_norm(partial, partials);
-    if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
-    const double r = limit / (n + kEps);
-    const float f = r >= 1.0 ? 1.0f : (float)r;  // a NaN stays
+__device__ __forceinline__ void scale_list(const List<MOST>& l, float f) {
     for (int c = blockIdx.x; c < l.first[l.count]; c += gridDim.x) {
         const int chunk = l.first[l.count] - 1 - c;
         const int t = tensor_of(l, chunk);
         if (f == 1.0f && l.in[t] == l.out[t]) continue;
-        const int64_t at = (int64_t)(chunk - l.first[t]) * kChunk;
-        const int m = (int)min(kChunk, l.size[t] - at);
+        const int64_t at = (int64_t)(chunk - l.first[t]) * l.chunk;
+        const int m = (int)min((int64_t)l.chunk, l.size[t] - at);
         const int type = l.type[t], to = l.out_type[t];
         if (type == HB_F32) {
             scale_chunk(static_cast<const float*>(l.in[t]) + at, static_cast<float*>(l.out[t]) + at, m, f);
@@ -195,11 +206,38 @@ __global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__
     }
 }
 
+template <int MOST>
+__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ List<MOST> l,
+                                                         const double* __restrict__ partial, int partials, double limit,
+                                                         float* __restrict__ norm) {
+    const double n = total_norm(partial, partials);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
+    scale_list(l, factor_of(n, limit));
+}
+
+// Both steps in one cluster.  A block takes the same chunks in both, and no other block's.
+__global__ void __launch_bounds__(kThreads) clip_small_kernel(const __grid_constant__ List<kFew> l, int scale, double limit,
+                                                              float* __restrict__ norm) {
+    namespace cg = cooperative_groups;
+    __shared__ double mine;
+    cg::cluster_group cluster = cg::this_cluster();
+    const double sum = list_squares(l);
+    if (threadIdx.x == 0) mine = sum;
+    cluster.sync();
+    double s = 0.0;
+    for (int b = 0; b < (int)cluster.num_blocks(); ++b) s += *cluster.map_shared_rank(&mine, b);
+    const double n = sqrt(s);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
+    if (scale) scale_list(l, factor_of(n, limit));
+    cluster.sync();  // a block stays until the others have read its sum
+}
+
 // The tensors from..to of the caller's list that hold elements.
 template <int MOST>
-int fill(List<MOST>& l, int64_t from, int64_t to, const void* const* in, const int64_t* size, const int32_t* type,
-         void* const* out, const int32_t* out_type) {
+int fill(List<MOST>& l, int64_t chunk, int64_t from, int64_t to, const void* const* in, const int64_t* size,
+         const int32_t* type, void* const* out, const int32_t* out_type) {
     l.count = 0;
+    l.chunk = (int)chunk;
     int64_t chunks = 0;
     for (int64_t i = from; i < to; ++i) {
         if (size[i] == 0) continue;
@@ -210,7 +248,7 @@ int fill(List<MOST>& l, int64_t from, int64_t to, const void* const* in, const i
         l.type[t] = (uint8_t)type[i];
         l.out_type[t] = (uint8_t)(out ? out_type[i] : type[i]);
         l.first[t] = (int32_t)chunks;
-        chunks += (size[i] + kChunk - 1) / kChunk;
+        chunks += (size[i] + chunk - 1) / chunk;
     }
     l.first[l.count] = (int32_t)chunks;
     return (int)chunks;
@@ -224,7 +262,7 @@ cudaError_t run(int64_t count, const void* const* in, const int64_t* size, const
     List<MOST> l;
     int partials = 0;
     for (int64_t from = 0; from < count || from == 0; from += MOST) {
-        const int blocks = blocks_of(fill(l, from, std::min(count, from + MOST), in, size, type, out, out_type));
+        const int blocks = blocks_of(fill(l, kChunk, from, std::min(count, from + MOST), in, size, type, out, out_type));
         square_kernel<MOST><<<blocks, kThreads, 0, st>>>(l, partial + partials);
         count_launches(1);
         partials += blocks;
@@ -235,7 +273,7 @@ cudaError_t run(int64_t count, const void* const* in, const int64_t* size, const
         return cudaGetLastError();
     }
     for (int64_t from = 0; from < count || from == 0; from += MOST) {
-        if (count > MOST) fill(l, from, std::min(count, from + MOST), in, size, type, out, out_type);
+        if (count > MOST) fill(l, kChunk, from, std::min(count, from + MOST), in, size, type, out, out_type);
         scale_kernel<MOST><<<blocks_of(l.first[l.count]), kThreads, 0, st>>>(l, partial, partials, limit, norm);
         count_launches(1);
     }
@@ -254,6 +292,7 @@ int check(int64_t count, const void* const* in, const int64_t* size, const int32
         if (size[i] > INT32_MAX * kChunk || (chunks += (size[i] + kChunk - 1) / kChunk) > INT32_MAX)
             return abi_fail(HB_BAD_ARGUMENT, "gradient norm: too many elements");
     }
+    if (rows::address_bits(ws) % 256) return abi_fail(HB_BAD_ARGUMENT, "gradient norm: the workspace must be 256-byte aligned");
     if (ws_bytes < hb_clip_workspace(count)) return abi_fail(HB_WORKSPACE, "workspace smaller than hb_clip_workspace()");
     return HB_OK;
 }
@@ -262,8 +301,29 @@ int start(int64_t count, const void* const* in, const int64_t* size, const int32
           const int32_t* out_type, double limit, float* norm, void* ws, void* stream) {
     const auto st = static_cast<cudaStream_t>(stream);
     double* partial = static_cast<double*>(ws);
-    const cudaError_t e = count <= kFew ? run<kFew>(count, in, size, type, out, out_type, limit, norm, partial, st)
-                                        : run<kMany>(count, in, size, type, out, out_type, limit, norm, partial, st);
+    int64_t total = 0;
+    for (int64_t i = 0; i < count; ++i) total += size[i];
+    cudaError_t e = cudaSuccess;
+    if (count <= kFew && total <= kSmallMost) {
+        List<kFew> l;
+        fill(l, kSmallChunk, 0, count, in, size, type, out, out_type);
+        e = cudaFuncSetAttribute(clip_small_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = kCluster;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cudaLaunchConfig_t config{};
+        config.gridDim = dim3(kCluster);
+        config.blockDim = dim3(kThreads);
+        config.stream = st;
+        config.attrs = &attr;
+        config.numAttrs = 1;
+        if (e == cudaSuccess) e = cudaLaunchKernelEx(&config, clip_small_kernel, l, out != nullptr ? 1 : 0, limit, norm);
+        count_launches(1);
+        return e == cudaSuccess ? HB_OK : abi_fail(HB_LAUNCH, std::string("gradient norm: ") + cudaGetErrorString(e));
+    }
+    e = count <= kFew ? run<kFew>(count, in, size, type, out, out_type, limit, norm, partial, st)
+                      : run<kMany>(count, in, size, type, out, out_type, limit, norm, partial, st);
     return e == cudaSuccess ? HB_OK : abi_fail(HB_LAUNCH, std::string("gradient norm: ") + cudaGetErrorString(e));
 }
 

@@ -10,9 +10,11 @@
 // wildly in how often they occur, so the work is cut by sorted places, not by
 // rows: a group of threads sums a chunk of places in fp32 registers and writes the
 // rows that begin and end inside it.  A row that crosses chunks leaves one fp32
-// partial a chunk, and a second launch adds them in chunk order.  No atomics: the
-// result does not depend on the launch.  Blocks behind the chunks write the zeros
-// of the rows that no token names.
+// partial a chunk; the group that leaves the last of 16 chunks' (a counter says so,
+// nobody waits) adds those up in order, and the last of these groups their sums, so
+// a row that holds most of the batch is joined by many, and the result does not
+// depend on the launch.
+// Blocks behind the chunks write the zeros of the rows that no token names.
 #include <string>
 
 #include "index_sort.cuh"
@@ -42,6 +44,16 @@ struct Values {
             for (int i = 0; i < V::N; ++i) f[j * V::N + i] = rows::to_float(v.v[i]);
         }
     }
+    // what other blocks have written in this launch
+    static __device__ __forceinline__ void load_l2(const TO* p, float (&f)[N]) {
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j) {
+            V v;
+            v.raw = __ldcg(reinterpret_cast<const typename V::Raw*>(p + j * V::N));
+#pragma unroll
+            for (int i = 0; i < V::N; ++i) f[j * V::N + i] = rows::to_float(v.v[i]);
+        }
+    }
     static __device__ __forceinline__ void store(TO* p, const float (&f)[N]) {
 #pragma unroll
         for (int j = 0; j < kPieces; ++j) {
@@ -53,34 +65,38 @@ struct Values {
     }
 };
 
-template <typename T, int VB>
+// A group of threads serves M rows, U column steps at a time: M * U vectors a thread in flight.
+template <typename T, int VB, int M, int U>
 __global__ void __launch_bounds__(256) lookup_kernel(const T* __restrict__ table, int64_t stride, int64_t rows_,
                                                      int64_t width, const void* __restrict__ ids, int id_bytes, int64_t n,
                                                      float scale, T* __restrict__ out) {
     using V = Vec<T, VB>;
-    constexpr int U = 4;
-    const int g = blockDim.x;
-    const int64_t i = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-    if (i >= n) return;
-    const int64_t id = load_id(ids, id_bytes, i);
-    const bool there = id >= 0 && id < rows_;
-    const T* row = table + (there ? id : 0) * stride;
-    T* to = out + i * width;
-    for (int64_t c0 = threadIdx.x * V::N; c0 < width; c0 += (int64_t)g * V::N * U) {
-        V v[U];
+    const int64_t first = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * M;
+    const int64_t step = (int64_t)blockDim.x * V::N;
+    int64_t id[M];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (c0 + u * g * V::N < width && there) v[u].load(row + c0 + u * g * V::N);
+    for (int m = 0; m < M; ++m) {
+        id[m] = first + m < n ? load_id(ids, id_bytes, first + m) : -1;
+        if (id[m] >= rows_) id[m] = -1;
+    }
+    for (int64_t c = threadIdx.x * V::N; c < width; c += step * U) {
+        V v[M][U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t c = c0 + u * g * V::N;
-            if (c < width) {
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (id[m] >= 0 && c + u * step < width) v[m][u].load(table + id[m] * stride + c + u * step);
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (first + m >= n || c + u * step >= width) break;
+                V r;
 #pragma unroll
                 for (int j = 0; j < V::N; ++j)
-                    v[u].v[j] = rows::from_float<T>(there ? scale * rows::to_float(v[u].v[j]) : 0.0f);
-                v[u].store(to + c);
+                    r.v[j] = rows::from_float<T>(id[m] >= 0 ? scale * rows::to_float(v[m][u].v[j]) : 0.0f);
+                r.store(out + (first + m) * width + c + u * step);
             }
-        }
     }
 }
 
@@ -95,6 +111,7 @@ struct Grad {
     int64_t chunks;
     int tiles;               // column tiles
     float* partial;          // [chunks][2][width]: the row that a chunk continues, the row that it leaves open
+    uint32_t* arrived;       // [chunks][3][tiles], zero: what join_run counts
     TO* out;
     int accumulate;
     int64_t sum_blocks;
@@ -116,50 +133,221 @@ __device__ __forceinline__ void write_row(const Grad<T, TO>& g, uint32_t key, in
     Values<TO, N>::store(to, r);
 }
 
+// The chunks of a row that crosses them: the last one that `key` reaches from chunk c, which it leaves open,
+// and the first one from chunk c, which it is continued in.  Doubling steps, then halving ones.
+template <typename G>
+__device__ __forceinline__ int64_t last_chunk(const G& g, uint32_t key, int64_t c) {
+    int64_t e = c + 1, step = 1;
+    while (e + step < g.chunks && g.keys[(e + step) * g.chunk] == key) e += step, step <<= 1;
+    for (; step; step >>= 1)
+        if (e + step < g.chunks && g.keys[(e + step) * g.chunk] == key) e += step;
+    return e;
+}
+template <typename G>
+__device__ __forceinline__ int64_t first_chunk(const G& g, uint32_t key, int64_t c) {
+    int64_t s = c - 1, step = 1;
+    while (s - step >= 0 && g.keys[(s - step + 1) * g.chunk - 1] == key) s -= step, step <<= 1;
+    for (; step; step >>= 1)
+        if (s - step >= 0 && g.keys[(s - step + 1) * g.chunk - 1] == key) s -= step;
+    return s;
+}
+
+// All threads of a group (a part of a warp, or whole warps).
+__device__ __forceinline__ unsigned group_lanes() {
+    const int n = blockDim.x;
+    return n >= 32 ? 0xffffffffu : ((1u << n) - 1u) << ((threadIdx.y * n) & 31);
+}
+__device__ __forceinline__ void group_sync() {
+    if (blockDim.x <= 32) __syncwarp(group_lanes());
+    else asm volatile("bar.sync %0, %1;" ::"r"(threadIdx.y + 1), "r"(blockDim.x) : "memory");
+}
+
+// sum of `count` partials at part + i * step, in order
+template <int N>
+__device__ __forceinline__ void add_partials(const float* part, int64_t step, int count, float (&sum)[N]) {
+    constexpr int U = N > 4 ? 4 : 8;
+    for (int q = 0; q < count; q += U) {
+        float v[U][N];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (q + u < count) Values<float, N>::load_l2(part + (q + u) * step, v[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (q + u < count) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) sum[i] += v[u][i];
+            }
+    }
+}
+
+// Called by a group whose partial, of chunk `chunk` of the row `key` that reaches from chunk `first` to `last`,
+// is stored: counts it in, and joins what that completes.  Partial 1 of a row's first chunk holds what it
+// begins with, partial 0 of each later chunk what continues it.  Chunks go by blocks of kJoin: the sum of a
+// block's partials takes the place of its first one.
+constexpr int kJoin = 16;
+template <typename T, typename TO, int N>
+__device__ void join_run(const Grad<T, TO>& g, uint32_t key, int64_t first, int64_t last, int64_t chunk, int tile, int64_t c,
+                         bool mine, int32_t* completes) {
+    const int64_t block = chunk / kJoin, from = max(first, block * kJoin), to = min(last, block * kJoin + kJoin - 1);
+    const int opens = from == first;  // which partial and which counter
+    auto counted = [&](int64_t at, int which, int64_t most) {  // whether this group is the last of most + 1
+        __threadfence();
+        group_sync();
+        if (threadIdx.x == 0) {
+            *completes = atomicAdd(g.arrived + (at * 3 + which) * g.tiles + tile, 1u) == (uint32_t)most;
+            __threadfence();
+        }
+        group_sync();
+        const bool yes = *completes != 0;
+        group_sync();
+        return yes;
+    };
+    if (!counted(from, opens, to - from)) return;
+    const bool whole = first / kJoin == last / kJoin;
+    float* place = g.partial + (from * 2 + opens) * g.width + c;
+    float sum[N];
+    if (mine) {
+        Values<float, N>::load_l2(place, sum);
+        add_partials<N>(g.partial + (from + 1) * 2 * g.width + c, 2 * g.width, (int)(to - from), sum);
+        if (whole) write_row<T, TO, N>(g, key, c, sum);
+        else Values<float, N>::store(place, sum);
+    }
+    if (whole || !counted(first, 2, last / kJoin - first / kJoin) || !mine) return;
+    Values<float, N>::load_l2(g.partial + (first * 2 + 1) * g.width + c, sum);
+    const int64_t next = (first / kJoin + 1) * kJoin;
+    add_partials<N>(g.partial + next * 2 * g.width + c, 2 * kJoin * g.width, (int)(last / kJoin - first / kJoin), sum);
+    write_row<T, TO, N>(g, key, c, sum);
+}
+
+__device__ __forceinline__ void add_pair(float& a, float& b, float x, float y) {
+    asm("{\n\t.reg .b64 s, v;\n\tmov.b64 s, {%0, %1};\n\tmov.b64 v, {%2, %3};\n\tadd.rn.f32x2 s, s, v;\n\t"
+        "mov.b64 {%0, %1}, s;\n\t}"
+        : "+f"(a), "+f"(b)
+        : "f"(x), "f"(y));
+}
+template <typename T, int VB>
+__device__ __forceinline__ void add_vector(float (&sum)[Vec<T, VB>::N], const Vec<T, VB>& v) {
+    constexpr int N = Vec<T, VB>::N;
+#pragma unroll
+    for (int i = 0; i + 1 < N; i += 2) add_pair(sum[i], sum[i + 1], rows::to_float(v.v[i]), rows::to_float(v.v[i + 1]));
+    if (N % 2) sum[N - 1] += rows::to_float(v.v[N - 1]);
+}
+
+// 8 consecutive words of an array that is padded to whole 32-byte groups.
+__device__ __forceinline__ void load8(const void* array, int64_t at, uint32_t (&w)[8]) {
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint32_t*>(array) + at);
+    const uint4 a = __ldg(p), b = __ldg(p + 1);
+    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+}
+
+// Sums a chunk.  Each thread has its own ring of 8 vectors in shared memory, one a sorted place, filled ahead by
+// asynchronous copies: 8 rows are in flight while the sums hold few registers, and no thread waits for another.
+// The loop goes by 8 places (chunks are multiples of 8), whose rows and tokens come in whole vectors, since its
+// instructions are the next bound after the bytes.
 template <typename T, typename TO, int VB>
 __device__ __forceinline__ void sum_chunk(const Grad<T, TO>& g, int64_t block) {
     using V = Vec<T, VB>;
-    constexpr int N = V::N, U = 8;
+    constexpr int N = V::N, D = 8;
+    __shared__ int32_t completes[256];  // a group
+    __shared__ __align__(16) typename V::Raw ring[D * 256];
     const int tile = (int)(block % g.tiles);
     const int64_t c = ((int64_t)tile * blockDim.x + threadIdx.x) * N;
     const int64_t chunk = block / g.tiles * blockDim.y + threadIdx.y;
-    if (chunk >= g.chunks || c >= g.width) return;
-    const int64_t p0 = chunk * g.chunk, p1 = min(g.n, p0 + g.chunk);
-    uint32_t key = g.keys[p0];
-    bool head = p0 > 0 && g.keys[p0 - 1] == key;
+    if (chunk >= g.chunks) return;  // the whole group
+    const bool mine = c < g.width;
+    const uint32_t none = (uint32_t)g.rows;
+    const int64_t p0 = chunk * g.chunk;
+    const int count = (int)min((int64_t)g.chunk, g.n - p0);
+    const uint32_t first_key = g.keys[p0];
+    if (first_key >= none) return;
+    typename V::Raw* slots = ring + threadIdx.y * blockDim.x + threadIdx.x;
+    const int step = blockDim.x * blockDim.y;
+    const char* column = reinterpret_cast<const char*>(g.dy + (mine ? c : 0));
+    const uint32_t stride = (uint32_t)(g.dy_stride * (int64_t)sizeof(T));  // bytes, below 2^32
+    auto fetch = [&](int j, uint32_t token, bool there) {  // into slot j
+        const char* p = column + (uint64_t)token * stride;
+        if constexpr (VB >= 4) {
+            const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(slots + j * step));
+            if (there) {
+                if constexpr (VB == 16)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(p) : "memory");
+                else
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(p), "n"(VB) : "memory");
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+    };
+    uint32_t keys[D], tokens[D], after[D];
+    load8(g.order, p0, tokens);
+#pragma unroll
+    for (int j = 0; j < D; ++j) fetch(j, tokens[j], mine && j < count);
+    load8(g.keys, p0, after);
+    const bool continues = p0 > 0 && g.keys[p0 - 1] == first_key;
+    uint32_t key = first_key;
+    bool head = continues;
     float sum[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) sum[i] = 0.0f;
-    for (int64_t p = p0; p < p1; p += U) {
-        V v[U];
-        uint32_t k[U];
+    auto flush = [&]() {
+        if (mine) {
+            if (head) Values<float, N>::store(g.partial + (chunk * 2) * g.width + c, sum);
+            else write_row<T, TO, N>(g, key, c, sum);
+        }
+    };
+    for (int i = 0; i < count; i += D) {
+        const bool more = i + D < count;
+        typename V::Raw raw[VB >= 4 ? 1 : D];
+        if constexpr (VB < 4) {  // no asynchronous copy of 2 bytes: 8 loads by way of registers
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            k[u] = p + u < p1 ? g.keys[p + u] : (uint32_t)g.rows;
-            if (k[u] < (uint32_t)g.rows) v[u].load_once(g.dy + (int64_t)g.order[p + u] * g.dy_stride + c);
+            for (int j = 0; j < D; ++j)
+                if (mine && i + j < count)
+                    raw[j] = __ldcs(reinterpret_cast<const typename V::Raw*>(column + (uint64_t)tokens[j] * stride));
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (p + u >= p1) break;
-            if (k[u] != key) {
-                if (head) Values<float, N>::store(g.partial + (chunk * 2) * g.width + c, sum);
-                else write_row<T, TO, N>(g, key, c, sum);
+        for (int j = 0; j < D; ++j) keys[j] = i + j < count ? after[j] : none;
+        if (more) {
+            load8(g.order, p0 + i + D, tokens);
+            load8(g.keys, p0 + i + D, after);
+        }
 #pragma unroll
-                for (int i = 0; i < N; ++i) sum[i] = 0.0f;
-                key = k[u];
+        for (int j = 0; j < D; ++j) {
+            if (keys[j] != key) {
+                flush();
+#pragma unroll
+                for (int q = 0; q < N; ++q) sum[q] = 0.0f;
+                key = keys[j];
                 head = false;
+                if (key >= none) break;
             }
-            if (key < (uint32_t)g.rows) {
-#pragma unroll
-                for (int i = 0; i < N; ++i) sum[i] += rows::to_float(v[u].v[i]);
+            V v;
+            if constexpr (VB >= 4) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
+                v.raw = slots[j * step];
+            } else {
+                v.raw = raw[j];
             }
+            add_vector<T, VB>(sum, v);
+            fetch(j, tokens[j], mine && more && i + D + j < count);
+        }
+        if (key >= none) break;
+    }
+    if constexpr (VB >= 4) asm volatile("cp.async.wait_all;" ::: "memory");
+    const int64_t p1 = p0 + count;
+    const bool open = key < none && p1 < g.n && g.keys[p1] == key;
+    if (key < none) {
+        if (!head && open) {
+            if (mine) Values<float, N>::store(g.partial + (chunk * 2 + 1) * g.width + c, sum);
+        } else {
+            flush();
         }
     }
-    if (key >= (uint32_t)g.rows) return;
-    const bool open = p1 < g.n && g.keys[p1] == key;
-    if (head) Values<float, N>::store(g.partial + (chunk * 2) * g.width + c, sum);
-    else if (open) Values<float, N>::store(g.partial + (chunk * 2 + 1) * g.width + c, sum);
-    else write_row<T, TO, N>(g, key, c, sum);
+    if (continues) {
+        const int64_t to = head && open ? last_chunk(g, first_key, chunk) : chunk;
+        join_run<T, TO, N>(g, first_key, first_chunk(g, first_key, chunk), to, chunk, tile, c, mine,
+                           completes + threadIdx.y);
+    }
+    if (open && !head)
+        join_run<T, TO, N>(g, key, chunk, last_chunk(g, key, chunk), chunk, tile, c, mine, completes + threadIdx.y);
 }
 
 // Zeros of the rows that no sorted place holds: a lane searches a row, then the warp writes.
@@ -198,41 +386,6 @@ __global__ void __launch_bounds__(256) grad_kernel(const Grad<T, TO> g) {
     else zero_rows(g, blockIdx.x - g.sum_blocks);
 }
 
-// The rows that cross chunks: the group of the chunk that a row begins in adds its partials in chunk order.
-template <typename T, typename TO, int VB>
-__global__ void __launch_bounds__(256) join_kernel(const Grad<T, TO> g) {
-    constexpr int N = Vec<T, VB>::N, U = 4;
-    const int tile = (int)(blockIdx.x % g.tiles);
-    const int64_t c = ((int64_t)tile * blockDim.x + threadIdx.x) * N;
-    const int64_t chunk = (int64_t)(blockIdx.x / g.tiles) * blockDim.y + threadIdx.y;
-    if (chunk + 1 >= g.chunks || c >= g.width) return;
-    const int64_t p0 = chunk * g.chunk, p1 = p0 + g.chunk;
-    const uint32_t key = g.keys[p1 - 1];
-    if (key >= (uint32_t)g.rows || g.keys[p1] != key || (p0 > 0 && g.keys[p0 - 1] == key)) return;
-    int64_t lo = p1, hi = g.n;  // first place above the row's
-    while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (g.keys[mid] <= key) lo = mid + 1;
-        else hi = mid;
-    }
-    const int64_t last = (lo - 1) / g.chunk;
-    float sum[N];
-    Values<float, N>::load(g.partial + (chunk * 2 + 1) * g.width + c, sum);
-    for (int64_t q = chunk + 1; q <= last; q += U) {
-        float v[U][N];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (q + u <= last) Values<float, N>::load(g.partial + ((q + u) * 2) * g.width + c, v[u]);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (q + u <= last) {
-#pragma unroll
-                for (int i = 0; i < N; ++i) sum[i] += v[u][i];
-            }
-    }
-    write_row<T, TO, N>(g, key, c, sum);
-}
-
 // Threads a row: a power of two up to 32 vectors, else whole warps, at most 256 a column tile.
 struct Shape {
     int group, groups, tiles;
@@ -250,22 +403,27 @@ inline Shape shape_of(int64_t vectors) {
     return s;
 }
 
-// Places a chunk: 64 when there are plenty, fewer (at least 8) to have 64 warps of work an SM.
+// Places a chunk, a multiple of 8 as sum_chunk needs.  A chunk costs some microseconds of its own (its first
+// loads, its join), so up to 128 while that leaves 16 warps of work an SM; at least 16.  Measured with chunks of
+// 16 / 32 / 64 / 128: 131072 x 2048 bf16 236 / 186 / 174 / 166 us, 20000 x 2048 f16 45 / 37 / 34 / 37 us,
+// 1000 x 129 f32 16 / 18 / 21 / 28 us.
 inline int chunk_of(int64_t n, const Shape& s) {
-    const int64_t warps = n * s.tiles * s.group / 32;
-    const int64_t c = warps / (148 * 64);
-    return (int)(c < 8 ? 8 : c > 64 ? 64 : c);
+    const int64_t c = n * s.tiles * s.group / 32 / (148 * 16);
+    return (int)(c < 16 ? 16 : c > 128 ? 128 : c / 8 * 8);
 }
 
 struct Layout {
     uint32_t* keys;
     int32_t* order;
     float* partial;
+    uint32_t* arrived;
+    int64_t arrivals;
     void* sort;
     size_t sort_bytes, bytes;
 };
-// The chunk depends on the vector size, which a workspace query does not give: the partials are sized
-// for the fewest vectors a row can have (16 bytes of a 16-bit type), which makes the shortest chunk.
+// The chunk and the column tiles depend on the vector size, which a workspace query does not give: the
+// partials are sized for the fewest vectors a row can have (16 bytes of a 16-bit type), which makes the
+// shortest chunk, the counters for that chunk and the most tiles (an element a vector).
 inline Layout layout(void* ws, int64_t n, int64_t rows_, int64_t width) {
     Layout l{};
     char* base = static_cast<char*>(ws);
@@ -279,7 +437,10 @@ inline Layout layout(void* ws, int64_t n, int64_t rows_, int64_t width) {
     l.sort_bytes = index_sort_bytes(n, rows_);
     l.sort = take(l.sort_bytes);
     const int chunk = chunk_of(n, shape_of((width + 7) / 8));
-    l.partial = reinterpret_cast<float*>(take(sizeof(float) * 2 * width * ((n + chunk - 1) / chunk)));
+    const int64_t chunks = (n + chunk - 1) / chunk;
+    l.partial = reinterpret_cast<float*>(take(sizeof(float) * 2 * width * chunks));
+    l.arrivals = chunks * 3 * shape_of(width).tiles;
+    l.arrived = reinterpret_cast<uint32_t*>(take(sizeof(uint32_t) * l.arrivals));
     return l;
 }
 
@@ -300,10 +461,6 @@ cudaError_t run_grad(Grad<T, TO> g, cudaStream_t st) {
     }
     grad_kernel<T, TO, VB><<<(unsigned)(g.sum_blocks + zero_blocks), block, 0, st>>>(g);
     count_launches(1);
-    if (g.chunks > 1) {
-        join_kernel<T, TO, VB><<<(unsigned)g.sum_blocks, block, 0, st>>>(g);
-        count_launches(1);
-    }
     return cudaGetLastError();
 }
 
@@ -324,14 +481,18 @@ extern "C" int hb_embedding_lookup(int type, const void* table, int64_t table_st
     const int size = rows::type_bytes(type);
     const int vb = rows::vector_bytes(rows::address_bits(table) | rows::address_bits(out) |
                                       (uint64_t)(table_stride * size) | (uint64_t)(width * size), type);
-    // a warp a row; a block when the rows are too few to fill the SMs with warps
+    // few rows: a thread a vector, so that every load starts at once.  Enough rows for 16 blocks an SM: 4
+    // vectors in flight a thread, of 4 rows, or of one where a row has more than 128.
     const int64_t vectors = width * size / vb;
-    Shape s = shape_of(vectors < 32 ? vectors : 32);
-    if (n < 148 * 8 && vectors > 32) s = shape_of(256);
-    const unsigned blocks = (unsigned)((n + s.groups - 1) / s.groups);
+    const bool many = n * (vectors < 256 ? vectors : 256) >= (int64_t)148 * 16 * 256, wide = many && vectors > 128;
+    const int group = (int)(wide ? 32 : vectors < 256 ? vectors : 256), groups = 256 / group;
+    const int64_t per = groups * (many && !wide ? 4 : 1);
+    const unsigned blocks = (unsigned)((n + per - 1) / per);
     rows::for_type(type, vb, [&](auto t, auto b) {
         using T = decltype(t);
-        lookup_kernel<T, decltype(b)::value><<<blocks, dim3(s.group, s.groups), 0, static_cast<cudaStream_t>(stream)>>>(
+        constexpr int VB = decltype(b)::value;
+        const auto kernel = wide ? lookup_kernel<T, VB, 1, 4> : many ? lookup_kernel<T, VB, 4, 1> : lookup_kernel<T, VB, 1, 1>;
+        kernel<<<blocks, dim3(group, groups), 0, static_cast<cudaStream_t>(stream)>>>(
             static_cast<const T*>(table), table_stride, rows_, width, ids, id_bytes, n, (float)scale,
             static_cast<T*>(out));
     });
@@ -352,6 +513,8 @@ extern "C" int hb_embedding_grad(int type, const void* dy, int64_t dy_stride, co
         return abi_fail(HB_BAD_ARGUMENT, "embedding gradient: the gradient has dy's type or is fp32, ids are 32 or 64 bits");
     if (rows_ < 1 || rows_ >= INT32_MAX || width < 0 || width > INT32_MAX || n < 0 || n > INT32_MAX)
         return abi_fail(HB_BAD_ARGUMENT, "embedding gradient: sizes out of range");
+    if (dy_stride < 0 || dy_stride > UINT32_MAX / rows::type_bytes(type))
+        return abi_fail(HB_BAD_ARGUMENT, "embedding gradient: rows of dy must start less than 2^32 bytes apart");
     if (width == 0) return HB_OK;
     if (!out || (n > 0 && (!dy || !ids || !workspace))) return abi_fail(HB_BAD_ARGUMENT, "embedding gradient: null pointer");
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -361,10 +524,13 @@ extern "C" int hb_embedding_grad(int type, const void* dy, int64_t dy_stride, co
         if (!accumulate) e = cudaMemsetAsync(out, 0, (size_t)rows_ * width * out_size, st);
         return e == cudaSuccess ? HB_OK : abi_fail(HB_CUDA, std::string("embedding gradient: ") + cudaGetErrorString(e));
     }
+    if (rows::address_bits(workspace) % 256)
+        return abi_fail(HB_BAD_ARGUMENT, "embedding gradient: the workspace must be 256-byte aligned");
     const Layout l = layout(workspace, n, rows_, width);
     if (workspace_bytes < l.bytes)
         return abi_fail(HB_WORKSPACE, "workspace smaller than hb_embedding_grad_workspace()");
-    const int rc = index_sort(ids, id_bytes, n, rows_, l.order, nullptr, l.keys, nullptr, l.sort, l.sort_bytes, st);
+    const int rc = index_sort(ids, id_bytes, n, rows_, l.order, nullptr, l.keys, nullptr, l.sort, l.sort_bytes, st,
+                              l.arrived, l.arrivals);
     if (rc) return rc;
     int vb = rows::vector_bytes(rows::address_bits(dy) | (uint64_t)(dy_stride * size) | (uint64_t)(width * size), type);
     while (vb > size) {
@@ -387,6 +553,7 @@ extern "C" int hb_embedding_grad(int type, const void* dy, int64_t dy_stride, co
             g.order = l.order;
             g.keys = l.keys;
             g.partial = l.partial;
+            g.arrived = l.arrived;
             g.out = static_cast<TO*>(out);
             g.accumulate = accumulate;
             e = run_grad<T, TO, VB>(g, st);

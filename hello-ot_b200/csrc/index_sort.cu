@@ -1,13 +1,26 @@
 // Stable counting sort of entries by expert (or by row of a table).
 //
 // Least significant digit first, digits of up to 11 bits, so one pass for up to
-// 2047 bins and two for up to 4 million.  A pass counts each tile's digits, scans
-// the counts over the tiles of a digit (a warp a digit), and places the entries:
-// a warp ranks 32 entries at a time with a match over its lanes on top of its own
-// shared-memory counters, so equal digits keep their order and nothing depends on
-// the order of atomics.  Up to 4096 entries sort in one block with the entries in
-// shared memory: one launch, which is what counts for single tokens.
+// 2047 bins and two for up to 4 million.  A pass counts digits block by block, and
+// places the entries: a warp ranks 32 entries at a time by ballots over its lanes
+// on top of its own shared-memory counters, so equal digits keep their order and
+// nothing depends on the order of atomics.
+//
+// Such a sort moves little (a megabyte at 131072 entries), so its time is launches,
+// barriers and the single sector a cycle at which an SM scatters 4-byte stores.
+//   up to 32768 entries  one launch of one cluster of up to 16 blocks: the entries
+//                        stay in the blocks' shared memory over all passes, the
+//                        blocks read each other's counts and write each other's
+//                        entries there, and the hardware's cluster barrier stands
+//                        between the steps
+//   up to 524288         tiles over all SMs, a launch for the first pass's counts
+//                        and one a pass: a block adds up the counts of all tiles
+//                        itself, and counts the next pass's digits as it places
+//   above                tiles of 8192 and three launches a pass, the counts scanned
+//                        over the tiles by a launch of their own
 #include <string>
+
+#include <cooperative_groups.h>
 
 #include "../../include/hello_b200.h"
 #include "index_sort.cuh"
@@ -16,9 +29,13 @@
 namespace hb {
 namespace isort {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kSmallRounds = 8, kSmallMost = kThreads * kSmallRounds;
+constexpr int kThreads = 1024, kWarps = kThreads / 32;     // a tile's block
+constexpr int kBlock = 1024, kBlockWarps = kBlock / 32;     // a cluster's block
+constexpr int kRounds = 2;                                  // entries a thread of a cluster
+constexpr int kMostClusters = 16;
+constexpr int64_t kClusterMost = (int64_t)kMostClusters * kBlock * kRounds;
 constexpr int kMaxDigitBits = 11;
+constexpr int kMostTiles = 64;                              // that every block adds up itself
 
 // The keys of a pass: the caller's index (first pass) or the keys of the pass before.
 struct Source {
@@ -32,10 +49,16 @@ struct Source {
     }
 };
 
-// Rank of every lane's digit among the equal digits its warp has seen, in order.
-__device__ __forceinline__ uint32_t warp_rank(uint16_t* counts, uint32_t digit, bool valid, uint32_t none) {
+// Rank of every lane's digit among the equal digits its warp has seen, in order.  The lanes with an
+// equal digit come from a ballot a bit of it.
+__device__ __forceinline__ uint32_t warp_rank(uint16_t* counts, uint32_t digit, bool valid, int bits) {
     const uint32_t lane = threadIdx.x & 31;
-    const uint32_t same = __match_any_sync(0xffffffffu, valid ? digit : none);
+    uint32_t same = __ballot_sync(0xffffffffu, valid);
+#pragma unroll 4
+    for (int b = 0; b < bits; ++b) {
+        const uint32_t set = __ballot_sync(0xffffffffu, (digit >> b) & 1u);
+        same &= (digit >> b) & 1u ? set : ~set;
+    }
     const uint32_t before = valid ? counts[digit] : 0;
     __syncwarp();
     if (valid && (same >> lane) == 1u) counts[digit] = (uint16_t)(before + __popc(same));
@@ -44,11 +67,12 @@ __device__ __forceinline__ uint32_t warp_rank(uint16_t* counts, uint32_t digit, 
 }
 
 // counts[warp][digit] -> digits before this warp's in the block; total[digit] the block's.
+template <int WARPS>
 __device__ __forceinline__ void scan_warps(uint16_t* counts, uint32_t* total, int digits) {
-    for (int d = threadIdx.x; d < digits; d += kThreads) {
+    for (int d = threadIdx.x; d < digits; d += WARPS * 32) {
         uint32_t sum = 0;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
+        for (int w = 0; w < WARPS; ++w) {
             const uint32_t c = counts[w * digits + d];
             counts[w * digits + d] = (uint16_t)sum;
             sum += c;
@@ -58,9 +82,10 @@ __device__ __forceinline__ void scan_warps(uint16_t* counts, uint32_t* total, in
 }
 
 // Exclusive scan of v[0..digits) in place by the whole block.
+template <int WARPS>
 __device__ __forceinline__ void block_scan(uint32_t* v, int digits) {
-    __shared__ uint32_t sums[kWarps];
-    const int per = (digits + kThreads - 1) / kThreads;
+    __shared__ uint32_t sums[WARPS];
+    const int per = (digits + WARPS * 32 - 1) / (WARPS * 32);
     const int lo = min(digits, (int)threadIdx.x * per), hi = min(digits, lo + per);
     uint32_t mine = 0;
     for (int d = lo; d < hi; ++d) mine += v[d];
@@ -72,8 +97,9 @@ __device__ __forceinline__ void block_scan(uint32_t* v, int digits) {
     }
     if ((threadIdx.x & 31) == 31) sums[threadIdx.x >> 5] = incl;
     __syncthreads();
-    uint32_t base = incl - mine;
-    for (int w = 0; w < (int)(threadIdx.x >> 5); ++w) base += sums[w];
+    // every warp adds up the warps before it: lane w has warp w's sum
+    uint32_t base = (threadIdx.x & 31) < min((int)(threadIdx.x >> 5), WARPS) ? sums[threadIdx.x & 31] : 0;
+    base = __reduce_add_sync(0xffffffffu, base) + incl - mine;
     for (int d = lo; d < hi; ++d) {
         const uint32_t c = v[d];
         v[d] = base;
@@ -82,20 +108,31 @@ __device__ __forceinline__ void block_scan(uint32_t* v, int digits) {
     __syncthreads();
 }
 
-__global__ void __launch_bounds__(kThreads) sort_small(Source src, int n, int passes, int digit_bits, int digits,
-                                                       int32_t* __restrict__ order, int32_t* __restrict__ position,
-                                                       uint32_t* __restrict__ keys_out, int32_t* __restrict__ offsets) {
-    extern __shared__ uint32_t smem[];
-    uint32_t* key_at = smem;                              // kSmallMost
-    uint16_t* val_at = reinterpret_cast<uint16_t*>(key_at + (passes > 1 ? kSmallMost : 0));
-    uint32_t* total = smem + (passes > 1 ? kSmallMost + kSmallMost / 2 : 0);  // digits
-    uint16_t* counts = reinterpret_cast<uint16_t*>(total + digits);           // kWarps x digits
+// All of a sort in one cluster.  Block b holds entries b * rounds * 1024 and on; a thread of warp w its
+// entries w * rounds * 32 + r * 32 + lane, so the order of (block, warp, round, lane) is the entries'.
+__global__ void __launch_bounds__(kBlock, 1) sort_cluster(Source src, int n, int rounds, int passes, int digit_bits,
+                                                          int digits, int32_t* __restrict__ order,
+                                                          int32_t* __restrict__ position, uint32_t* __restrict__ keys_out,
+                                                          int32_t* __restrict__ offsets, uint32_t* __restrict__ zero,
+                                                          int64_t zeros) {
+    namespace cg = cooperative_groups;
+    extern __shared__ __align__(16) uint32_t smem[];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int blocks = (int)cluster.num_blocks(), me = (int)cluster.block_rank();
+    const int mine = rounds * kBlock;                      // entries a block
+    uint32_t* total = smem;                                // digits: this block's counts, read by the others
+    uint32_t* base = total + digits;                       // digits: first place of this block's
+    uint32_t* before = base + digits;                      // digits: those of the blocks before
+    uint2* entry_at = reinterpret_cast<uint2*>(smem + (3 * digits + 1) / 2 * 2);  // (key, entry) between passes
+    uint16_t* counts = reinterpret_cast<uint16_t*>(entry_at + (passes > 1 ? mine : 0));  // kBlockWarps x digits
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rounds = (n + kThreads - 1) / kThreads;
-    const int first = warp * 32 * rounds + lane;
-    uint32_t key[kSmallRounds], val[kSmallRounds], rank[kSmallRounds];
+    const int within = warp * 32 * rounds + lane;
+    const int first = me * mine + within;
+    for (int64_t i = (int64_t)me * kBlock + threadIdx.x; i < zeros; i += blocks * kBlock) zero[i] = 0;
+    uint32_t key[kRounds], rank[kRounds];
+    int32_t val[kRounds];
 #pragma unroll
-    for (int r = 0; r < kSmallRounds; ++r) {
+    for (int r = 0; r < kRounds; ++r) {
         const int i = first + r * 32;
         if (r < rounds && i < n) key[r] = src.key(i);
         val[r] = i;
@@ -103,62 +140,88 @@ __global__ void __launch_bounds__(kThreads) sort_small(Source src, int n, int pa
     const uint32_t mask = (1u << digit_bits) - 1u;
     for (int pass = 0; pass < passes; ++pass) {
         const int shift = pass * digit_bits;
-        for (int i = threadIdx.x; i < kWarps * digits; i += kThreads) counts[i] = 0;
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < kSmallRounds; ++r)
-            if (r < rounds)
-                rank[r] = warp_rank(counts + warp * digits, (key[r] >> shift) & mask, first + r * 32 < n, digits);
-        __syncthreads();
-        scan_warps(counts, total, digits);
-        __syncthreads();
-        block_scan(total, digits);
         const bool last = pass + 1 == passes;
+        for (int i = threadIdx.x; i < kBlockWarps * digits / 2; i += kBlock) reinterpret_cast<uint32_t*>(counts)[i] = 0;
+        __syncthreads();
 #pragma unroll
-        for (int r = 0; r < kSmallRounds; ++r) {
+        for (int r = 0; r < kRounds; ++r)
+            if (r < rounds)
+                rank[r] = warp_rank(counts + warp * digits, (key[r] >> shift) & mask, first + r * 32 < n, digit_bits);
+        __syncthreads();
+        scan_warps<kBlockWarps>(counts, total, digits);
+        cluster.sync();
+        for (int d = threadIdx.x; d < digits; d += kBlock) {
+            uint32_t all = 0, lower = 0;
+#pragma unroll
+            for (int b = 0; b < kMostClusters; ++b) {
+                const uint32_t c = b < blocks ? *cluster.map_shared_rank(total + d, b) : 0;
+                if (b < me) lower += c;
+                all += c;
+            }
+            base[d] = all;
+            before[d] = lower;
+        }
+        __syncthreads();
+        block_scan<kBlockWarps>(base, digits);
+        if (offsets && passes == 1 && me == 0)
+            for (int d = threadIdx.x; d < digits; d += kBlock) offsets[d] = (int32_t)base[d];
+        // all counts are read: a block may leave, or count again
+        if (last) cluster.sync();
+#pragma unroll
+        for (int r = 0; r < kRounds; ++r) {
             if (r < rounds && first + r * 32 < n) {
                 const uint32_t d = (key[r] >> shift) & mask;
-                const uint32_t p = total[d] + counts[warp * digits + d] + rank[r];
+                const uint32_t p = base[d] + before[d] + counts[warp * digits + d] + rank[r];
                 if (last) {
-                    if (order) order[p] = (int32_t)val[r];
+                    if (order) order[p] = val[r];
                     if (position) position[val[r]] = (int32_t)p;
                     if (keys_out) keys_out[p] = key[r];
                 } else {
-                    key_at[p] = key[r];
-                    val_at[p] = (uint16_t)val[r];
+                    const uint32_t to = p / (uint32_t)mine, at = p - to * (uint32_t)mine;
+                    *cluster.map_shared_rank(entry_at + at, to) = make_uint2(key[r], (uint32_t)val[r]);
                 }
             }
         }
         if (!last) {
-            __syncthreads();
+            cluster.sync();
 #pragma unroll
-            for (int r = 0; r < kSmallRounds; ++r) {
-                const int i = first + r * 32;
-                if (r < rounds && i < n) {
-                    key[r] = key_at[i];
-                    val[r] = val_at[i];
+            for (int r = 0; r < kRounds; ++r) {
+                if (r < rounds && first + r * 32 < n) {
+                    const uint2 v = entry_at[within + r * 32];
+                    key[r] = v.x;
+                    val[r] = (int32_t)v.y;
                 }
             }
         }
     }
-    if (offsets && passes == 1)
-        for (int d = threadIdx.x; d < digits; d += kThreads) offsets[d] = (int32_t)total[d];
 }
 
-template <int ROUNDS>
+// A tile's digits: counts[digit][tile] for scan_tiles (SCANNED), else 16 bits each, two to a word,
+// counts[tile][digit / 2].  Clears `next` and `zero` too.
+template <int ROUNDS, bool SCANNED>
 __global__ void __launch_bounds__(kThreads) tile_counts(Source src, int64_t n, int shift, uint32_t mask, int digits,
-                                                        int tiles, uint32_t* __restrict__ counts) {
+                                                        int tiles, uint32_t* __restrict__ counts,
+                                                        uint32_t* __restrict__ next, int64_t nexts,
+                                                        uint32_t* __restrict__ zero, int64_t zeros) {
     extern __shared__ uint32_t smem[];
-    for (int d = threadIdx.x; d < digits; d += kThreads) smem[d] = 0;
+    const int64_t thread = (int64_t)blockIdx.x * kThreads + threadIdx.x, threads = (int64_t)tiles * kThreads;
+    for (int64_t i = thread; i < nexts; i += threads) next[i] = 0;
+    for (int64_t i = thread; i < zeros; i += threads) zero[i] = 0;
+    const int words = SCANNED ? digits : (digits + 1) / 2;
+    for (int d = threadIdx.x; d < words; d += kThreads) smem[d] = 0;
     __syncthreads();
     const int64_t base = (int64_t)blockIdx.x * (kThreads * ROUNDS);
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
         const int64_t i = base + r * kThreads + threadIdx.x;
-        if (i < n) atomicAdd(&smem[(src.key(i) >> shift) & mask], 1u);
+        if (i < n) {
+            const uint32_t d = (src.key(i) >> shift) & mask;
+            atomicAdd(&smem[SCANNED ? d : d / 2], SCANNED ? 1u : 1u << (d % 2 * 16));
+        }
     }
     __syncthreads();
-    for (int d = threadIdx.x; d < digits; d += kThreads) counts[(int64_t)d * tiles + blockIdx.x] = smem[d];
+    for (int d = threadIdx.x; d < words; d += kThreads)
+        counts[SCANNED ? (int64_t)d * tiles + blockIdx.x : (int64_t)blockIdx.x * words + d] = smem[d];
 }
 
 // A warp a digit: its counts become exclusive sums over the tiles, its total goes to totals.
@@ -183,16 +246,20 @@ __global__ void __launch_bounds__(256) scan_tiles(uint32_t* __restrict__ counts,
     if (lane == 0) totals[d] = run;
 }
 
-template <int ROUNDS>
+// Places a tile's entries.  SCANNED: counts and totals as scan_tiles leaves them; else the tiles' packed counts,
+// and the digits of the next pass are counted into `next` (cleared before), tile by tile of where entries go.
+template <int ROUNDS, bool SCANNED>
 __global__ void __launch_bounds__(kThreads) tile_place(Source src, const int32_t* __restrict__ vals, int64_t n, int shift,
                                                        uint32_t mask, int digits, int tiles,
                                                        const uint32_t* __restrict__ counts,
-                                                       const uint32_t* __restrict__ totals, int32_t* __restrict__ order,
+                                                       const uint32_t* __restrict__ totals, uint32_t* __restrict__ next,
+                                                       int next_shift, int32_t* __restrict__ order,
                                                        int32_t* __restrict__ position, uint32_t* __restrict__ keys_out,
                                                        int32_t* __restrict__ offsets) {
     extern __shared__ uint32_t smem[];
-    uint32_t* base = smem;                                            // digits
-    uint32_t* total = base + digits;                                  // digits
+    uint32_t* base = smem;                                            // digits: of all entries
+    uint32_t* before = base + digits;                                 // digits: of the tiles before
+    uint32_t* total = before + digits;                                // digits
     uint16_t* mine = reinterpret_cast<uint16_t*>(total + digits);     // kWarps x digits
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t first = (int64_t)blockIdx.x * (kThreads * ROUNDS) + warp * (32 * ROUNDS) + lane;
@@ -204,25 +271,54 @@ __global__ void __launch_bounds__(kThreads) tile_place(Source src, const int32_t
         key[r] = i < n ? src.key(i) : 0;
         val[r] = i < n ? (vals ? vals[i] : (int32_t)i) : 0;
     }
-    for (int d = threadIdx.x; d < digits; d += kThreads) base[d] = totals[d];
+    for (int d = threadIdx.x; d < digits; d += kThreads) {
+        base[d] = SCANNED ? totals[d] : 0;
+        before[d] = SCANNED ? counts[(int64_t)d * tiles + blockIdx.x] : 0;
+    }
     for (int i = threadIdx.x; i < kWarps * digits; i += kThreads) mine[i] = 0;
     __syncthreads();
+    const int words = (digits + 1) / 2;
+    if (!SCANNED) {  // as many threads a word of counts as there are, each every slices-th tile
+        const int slices = max(1, kThreads / words);
+        for (int j = threadIdx.x; j < words * slices; j += kThreads) {
+            const int w = j % words;
+            uint32_t all[2] = {0, 0}, lower[2] = {0, 0};
+#pragma unroll 16
+            for (int t = j / words; t < tiles; t += slices) {
+                const uint32_t c = counts[(int64_t)t * words + w];
+                const uint32_t low = t < (int)blockIdx.x ? c : 0;
+                all[0] += c & 0xffffu, all[1] += c >> 16;
+                lower[0] += low & 0xffffu, lower[1] += low >> 16;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (w * 2 + h < digits) {
+                    atomicAdd(&base[w * 2 + h], all[h]);
+                    atomicAdd(&before[w * 2 + h], lower[h]);
+                }
+        }
+    }
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r)
-        rank[r] = warp_rank(mine + warp * digits, (key[r] >> shift) & mask, first + r * 32 < n, digits);
-    block_scan(base, digits);
+        rank[r] = warp_rank(mine + warp * digits, (key[r] >> shift) & mask, first + r * 32 < n, __popc(mask));
+    __syncthreads();
+    block_scan<kWarps>(base, digits);
     if (offsets && blockIdx.x == 0)
         for (int d = threadIdx.x; d < digits; d += kThreads) offsets[d] = (int32_t)base[d];
-    scan_warps(mine, total, digits);
+    scan_warps<kWarps>(mine, total, digits);
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
         if (first + r * 32 >= n) continue;
         const uint32_t d = (key[r] >> shift) & mask;
-        const uint32_t p = base[d] + counts[(int64_t)d * tiles + blockIdx.x] + mine[warp * digits + d] + rank[r];
+        const uint32_t p = base[d] + before[d] + mine[warp * digits + d] + rank[r];
         if (order) order[p] = val[r];
         if (position) position[val[r]] = (int32_t)p;
         if (keys_out) keys_out[p] = key[r];
+        if (next) {
+            const uint32_t q = (key[r] >> next_shift) & mask;
+            atomicAdd(&next[(int64_t)(p / (kThreads * ROUNDS)) * words + q / 2], 1u << (q % 2 * 16));
+        }
     }
 }
 
@@ -242,10 +338,12 @@ __global__ void __launch_bounds__(256) find_offsets(const uint32_t* __restrict__
 
 struct Plan {
     int passes, digit_bits, digits, rounds, tiles;
+    int cluster;  // blocks of the one-launch sort, 0: tiles
 };
 
-// One pass over bins + 1 digits when they fit, else equal digits of at most 11 bits.  Tiles of 1024
-// entries keep all SMs busy up to half a million entries, tiles of 4096 keep the counts short above.
+// One pass over bins + 1 digits when they fit, else equal digits of at most 11 bits.
+// A cluster has a block for every 1024 entries up to 16 (one for up to 2048); tiles have 2048, 4096 or 8192
+// entries, the least that makes at most 64 tiles, so that a block adds up their counts in a few loads a thread.
 inline Plan plan_of(int64_t n, int64_t bins) {
     Plan p{};
     int bits = 1;
@@ -253,13 +351,22 @@ inline Plan plan_of(int64_t n, int64_t bins) {
     p.passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
     p.digit_bits = (bits + p.passes - 1) / p.passes;
     p.digits = p.passes == 1 ? (int)(bins + 1) : 1 << p.digit_bits;
-    p.rounds = n > (1 << 19) ? 8 : 2;
+    if (n <= kClusterMost) {
+        p.cluster = 1;
+        if (n > kBlock * kRounds)
+            while (p.cluster < kMostClusters && (int64_t)p.cluster * kBlock < n) p.cluster <<= 1;
+        p.rounds = (int)((n + p.cluster * kBlock - 1) / (p.cluster * kBlock));
+        return p;
+    }
+    p.rounds = 2;
+    while (p.rounds < 8 && (int64_t)p.rounds * kThreads * kMostTiles < n) p.rounds <<= 1;
     const int64_t tile = (int64_t)kThreads * p.rounds;
     p.tiles = (int)((n + tile - 1) / tile);
     return p;
 }
+inline bool scanned(const Plan& p) { return p.tiles > kMostTiles; }
 
-// counts and totals of a pass, the keys and entries between passes, and the last
+// Counts (of a pass, or of each) and totals, the keys and entries between passes, and the last
 // pass's keys (searched for the offsets when the caller takes no keys).
 struct Layout {
     uint32_t *counts, *totals, *keys[2], *sorted;
@@ -274,8 +381,9 @@ inline Layout layout(void* ws, int64_t n, const Plan& p) {
         l.bytes += (bytes + 255) / 256 * 256;
         return r;
     };
-    if (n > kSmallMost) {
-        l.counts = reinterpret_cast<uint32_t*>(take(sizeof(uint32_t) * (size_t)p.digits * p.tiles));
+    if (!p.cluster) {
+        l.counts = reinterpret_cast<uint32_t*>(
+            take(sizeof(uint32_t) * p.tiles * (scanned(p) ? (size_t)p.digits : (size_t)(p.digits + 1) / 2 * p.passes)));
         l.totals = reinterpret_cast<uint32_t*>(take(sizeof(uint32_t) * p.digits));
         for (int i = 0; i < 2 && i + 1 < p.passes; ++i) {
             l.keys[i] = reinterpret_cast<uint32_t*>(take(sizeof(uint32_t) * n));
@@ -286,24 +394,48 @@ inline Layout layout(void* ws, int64_t n, const Plan& p) {
     return l;
 }
 
-inline size_t small_smem(const Plan& p) {
-    return (p.passes > 1 ? (size_t)kSmallMost * 6 : 0) + (size_t)p.digits * (4 + 2 * kWarps);
+inline size_t cluster_smem(const Plan& p) {
+    return (size_t)(3 * p.digits + 1) / 2 * 8 + (p.passes > 1 ? (size_t)p.rounds * kBlock * 8 : 0) +
+           (size_t)p.digits * 2 * kBlockWarps;
 }
-inline size_t place_smem(const Plan& p) { return (size_t)p.digits * (8 + 2 * kWarps); }
+inline size_t place_smem(const Plan& p) { return (size_t)p.digits * (12 + 2 * kWarps); }
 
-// Dynamic shared memory above 48 KB has to be allowed once per kernel.
+// Dynamic shared memory above 48 KB has to be allowed for the kernel.
 template <typename K>
 inline cudaError_t allow(K* kernel, size_t bytes) {
     if (bytes <= 48 * 1024) return cudaSuccess;
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
 }
 
-template <int ROUNDS>
+cudaError_t sort_one_launch(const Source& src, int n, const Plan& p, int32_t* order, int32_t* position, uint32_t* keys,
+                            int32_t* offsets, uint32_t* zero, int64_t zeros, cudaStream_t st) {
+    cudaError_t e = allow(sort_cluster, cluster_smem(p));
+    if (e == cudaSuccess && p.cluster > 8)
+        e = cudaFuncSetAttribute(sort_cluster, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = p.cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(p.cluster);
+    config.blockDim = dim3(kBlock);
+    config.dynamicSmemBytes = cluster_smem(p);
+    config.stream = st;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    count_launches(1);
+    return cudaLaunchKernelEx(&config, sort_cluster, src, n, p.rounds, p.passes, p.digit_bits, p.digits, order, position,
+                              keys, offsets, zero, zeros);
+}
+
+template <int ROUNDS, bool SCANNED>
 cudaError_t sort_tiles(const Source& input, int64_t n, const Plan& p, const Layout& l, int32_t* order, int32_t* position,
-                       uint32_t* keys, int32_t* offsets, cudaStream_t st) {
-    cudaError_t e = allow(tile_place<ROUNDS>, place_smem(p));
+                       uint32_t* keys, int32_t* offsets, uint32_t* zero, int64_t zeros, cudaStream_t st) {
+    cudaError_t e = allow(tile_place<ROUNDS, SCANNED>, place_smem(p));
     if (e != cudaSuccess) return e;
     const uint32_t mask = (1u << p.digit_bits) - 1u;
+    const int64_t counted = (int64_t)(p.digits + 1) / 2 * p.tiles;  // words of a pass (SCANNED has one area)
     Source src = input;
     const int32_t* vals = nullptr;
     for (int pass = 0; pass < p.passes; ++pass) {
@@ -311,13 +443,21 @@ cudaError_t sort_tiles(const Source& input, int64_t n, const Plan& p, const Layo
         const bool last = pass + 1 == p.passes;
         uint32_t* to_keys = last ? keys : l.keys[pass & 1];
         int32_t* to_vals = last ? order : l.vals[pass & 1];
-        tile_counts<ROUNDS><<<p.tiles, kThreads, sizeof(uint32_t) * p.digits, st>>>(src, n, shift, mask, p.digits,
-                                                                                    p.tiles, l.counts);
-        scan_tiles<<<(p.digits + 7) / 8, 256, 0, st>>>(l.counts, p.tiles, p.digits, l.totals);
-        tile_place<ROUNDS><<<p.tiles, kThreads, place_smem(p), st>>>(
-            src, vals, n, shift, mask, p.digits, p.tiles, l.counts, l.totals, to_vals, last ? position : nullptr, to_keys,
-            last && p.passes == 1 ? offsets : nullptr);
-        count_launches(3);
+        uint32_t* counts = l.counts + (SCANNED ? 0 : pass * counted);
+        if (SCANNED || pass == 0) {
+            tile_counts<ROUNDS, SCANNED><<<p.tiles, kThreads, sizeof(uint32_t) * p.digits, st>>>(
+                src, n, shift, mask, p.digits, p.tiles, counts, l.counts + counted,
+                SCANNED ? 0 : counted * (p.passes - 1), zero, pass == 0 ? zeros : 0);
+            count_launches(1);
+        }
+        if (SCANNED) {
+            scan_tiles<<<(p.digits + 7) / 8, 256, 0, st>>>(counts, p.tiles, p.digits, l.totals);
+            count_launches(1);
+        }
+        tile_place<ROUNDS, SCANNED><<<p.tiles, kThreads, place_smem(p), st>>>(
+            src, vals, n, shift, mask, p.digits, p.tiles, counts, l.totals, SCANNED || last ? nullptr : counts + counted,
+            shift + p.digit_bits, to_vals, last ? position : nullptr, to_keys, last && p.passes == 1 ? offsets : nullptr);
+        count_launches(1);
         src.data = to_keys;
         src.kind = 0;
         vals = to_vals;
@@ -333,7 +473,8 @@ size_t index_sort_bytes(int64_t n, int64_t bins) {
 }
 
 int index_sort(const void* index, int index_bytes, int64_t n, int64_t bins, int32_t* order, int32_t* position,
-               uint32_t* keys, int32_t* offsets, void* ws, size_t ws_bytes, cudaStream_t st) {
+               uint32_t* keys, int32_t* offsets, void* ws, size_t ws_bytes, cudaStream_t st, uint32_t* zero,
+               int64_t zeros) {
     using namespace isort;
     cudaError_t e = cudaSuccess;
     if (n == 0) {
@@ -342,21 +483,19 @@ int index_sort(const void* index, int index_bytes, int64_t n, int64_t bins, int3
     }
     const Plan p = plan_of(n, bins);
     const Layout l = layout(ws, n, p);
+    if ((uintptr_t)ws % 256) return abi_fail(HB_BAD_ARGUMENT, "index sort: the workspace must be 256-byte aligned");
     if (l.bytes > ws_bytes || (l.bytes > 0 && !ws))
         return abi_fail(HB_WORKSPACE, "workspace too small for the index sort");
     const Source src{index, index_bytes, (uint32_t)bins};
     if (!keys && p.passes > 1 && offsets) keys = l.sorted;
-    if (n <= kSmallMost) {
-        e = allow(sort_small, small_smem(p));
-        if (e == cudaSuccess) {
-            sort_small<<<1, kThreads, small_smem(p), st>>>(src, (int)n, p.passes, p.digit_bits, p.digits, order, position,
-                                                           keys, offsets);
-            count_launches(1);
-            e = cudaGetLastError();
-        }
+    if (p.cluster) {
+        e = sort_one_launch(src, (int)n, p, order, position, keys, offsets, zero, zeros, st);
     } else {
-        e = p.rounds == 8 ? sort_tiles<8>(src, n, p, l, order, position, keys, offsets, st)
-                          : sort_tiles<2>(src, n, p, l, order, position, keys, offsets, st);
+        auto sort = scanned(p) ? sort_tiles<8, true>
+                    : p.rounds == 8 ? sort_tiles<8, false>
+                    : p.rounds == 4 ? sort_tiles<4, false>
+                                    : sort_tiles<2, false>;
+        e = sort(src, n, p, l, order, position, keys, offsets, zero, zeros, st);
     }
     if (e == cudaSuccess && offsets && p.passes > 1) {
         find_offsets<<<(unsigned)((bins + 256) / 256), 256, 0, st>>>(keys, n, bins, offsets);

@@ -10,9 +10,11 @@ namespace hb {
 // otherwise, sorted by key, equal keys in entry order.  Any output may be null:
 // order (n, entry of each place), position (n, place of each entry), keys (n,
 // sorted), offsets (bins + 1, first place of a key not below it; offsets[bins] is
-// the number of entries with a valid index).  Returns 0, or an HB_* code.
+// the number of entries with a valid index).  `zeros` words at `zero` are set to 0 on the
+// way (n > 0).  Returns 0, or an HB_* code.
 size_t index_sort_bytes(int64_t n, int64_t bins);
 int index_sort(const void* index, int index_bytes, int64_t n, int64_t bins, int32_t* order, int32_t* position,
-               uint32_t* keys, int32_t* offsets, void* ws, size_t ws_bytes, cudaStream_t st);
+               uint32_t* keys, int32_t* offsets, void* ws, size_t ws_bytes, cudaStream_t st,
+               uint32_t* zero = nullptr, int64_t zeros = 0);
 
 }  // namespace hb

@@ -9,10 +9,11 @@
 //   combine grad   dz[p] = w[t, k] dy[t] (0 for p >= kept),  dw[t, k] = <dy[t], z[p]>
 //   dispatch grad  dx[t] = combine of dxs without weights
 //
-// Every kernel goes by token: a group of threads holds the columns of one token,
-// so x, dy and y cross HBM once and each sorted row once, which is all they have
-// to.  Bound by HBM.  Sums are fp32 and run over k in order (no atomics): the
-// result does not depend on the launch.
+// Every kernel goes by token: a group of threads holds the columns of a token, so
+// x, dy and y cross HBM once and each sorted row once, which is all they have to.
+// Bound by HBM, so what counts is loads in flight: each thread has 4 vectors of up
+// to 16 bytes under way, of one row or of 4.  Sums are fp32 and run over k in order
+// (no atomics): the result does not depend on the launch.
 #include <string>
 
 #include "index_sort.cuh"
@@ -35,94 +36,164 @@ __device__ __forceinline__ uint32_t kept_entries(const Moves& m) {
     return (uint32_t)min((int64_t)max(*m.kept, 0), m.entries);
 }
 
-template <typename T, int VB, int G>
+// Wide rows: a group holds 4 vectors a thread of one token (8 short ones).  Rows of at most a vector a thread (NARROW): 4
+// tokens, so that as many loads are in flight.
+template <typename T, int VB, int G, bool NARROW>
 __global__ void __launch_bounds__(256) dispatch_kernel(Moves m, const T* __restrict__ x, int64_t x_stride,
                                                        T* __restrict__ out) {
     using V = Vec<T, VB>;
-    constexpr int U = 4;
-    const int64_t token = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    constexpr int U = NARROW || VB >= 8 ? 4 : 8;
+    const int64_t group = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const int64_t token = NARROW ? group * U : group;
     if (token >= m.tokens) return;
     const uint32_t kept = kept_entries(m);
-    const T* row = x + token * x_stride;
-    const int32_t* place = m.position + token * m.slots;
-    for (int64_t c0 = (threadIdx.x % G) * V::N; c0 < m.width; c0 += G * V::N * U) {
+    // vector u: of token + u, or u * G vectors further on in the row
+    for (int64_t c0 = (threadIdx.x % G) * V::N; c0 < m.width; c0 += NARROW ? m.width : G * V::N * U) {
         V v[U];
+        bool there[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (c0 + u * G * V::N < m.width) v[u].load(row + c0 + u * G * V::N);
+        for (int u = 0; u < U; ++u) {
+            there[u] = NARROW ? token + u < m.tokens : c0 + u * G * V::N < m.width;
+            if (there[u]) v[u].load_once(x + (NARROW ? token + u : token) * x_stride + (NARROW ? c0 : c0 + u * G * V::N));
+        }
         for (int k = 0; k < m.slots; ++k) {
-            const uint32_t p = (uint32_t)place[k];
-            if (p >= (uint64_t)m.entries) continue;
-            T* to = out + (int64_t)p * m.width;
-            V w[U];
+            uint32_t p[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                p[u] = there[u] ? (uint32_t)m.position[(NARROW ? token + u : token) * m.slots + k] : ~0u;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int64_t c = c0 + u * G * V::N;
-                if (c < m.width) {
-                    if (p >= kept) {
-                        w[u].zero();
-                        w[u].store(to + c);
-                    } else {
-                        v[u].store(to + c);
-                    }
+                if (!there[u] || p[u] >= (uint64_t)m.entries) continue;
+                T* to = out + (int64_t)p[u] * m.width + (NARROW ? c0 : c0 + u * G * V::N);
+                if (p[u] >= kept) {
+                    V w;
+                    w.zero();
+                    w.store(to);
+                } else {
+                    v[u].store(to);
                 }
             }
         }
     }
 }
 
-template <typename T, int VB, int G>
+// Weights of the entries e0..e0+B-1 (the last entry's beyond it); 1 without weights.
+template <int B>
+__device__ __forceinline__ void load_weights(const Moves& m, const void* weights, int type, int64_t e0, float (&w)[B]) {
+#pragma unroll
+    for (int b = 0; b < B; ++b) w[b] = 1.0f;
+    if (!weights) return;
+    if (type == HB_F32) {
+#pragma unroll
+        for (int b = 0; b < B; ++b) w[b] = static_cast<const float*>(weights)[min(e0 + b, m.entries - 1)];
+    } else {
+#pragma unroll
+        for (int b = 0; b < B; ++b) w[b] = rows::load_weight(weights, type, min(e0 + b, m.entries - 1));
+    }
+}
+
+// SLOTS 1, 2, 4: a group serves 4, 2, 1 tokens, 4 sorted rows in flight; 0: any number of slots, 4 at a time.
+template <typename T, int VB, int G, int SLOTS>
 __global__ void __launch_bounds__(256) combine_kernel(Moves m, const T* __restrict__ z, int64_t z_stride,
                                                       const void* __restrict__ weights, int weight_type,
                                                       T* __restrict__ out) {
     using V = Vec<T, VB>;
-    constexpr int B = 4;  // rows in flight
-    const int64_t token = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    constexpr int B = 4, M = SLOTS ? B / SLOTS : 1, S = B / M;  // rows, tokens, rows of a token in flight
+    constexpr int U = VB >= 8 ? 1 : 4;                          // column steps in flight
+    const int64_t token = ((int64_t)blockIdx.x * (256 / G) + threadIdx.x / G) * M;
     if (token >= m.tokens) return;
-    const uint32_t kept = kept_entries(m);
-    for (int64_t c = (threadIdx.x % G) * V::N; c < m.width; c += G * V::N) {
-        float sum[V::N];
+    const int slots = SLOTS ? SLOTS : m.slots;
+    const int64_t e0 = token * slots, e1 = min(m.entries, e0 + (SLOTS ? B : slots));
+    uint32_t p[B];
+    float w[B];
+    // places first, then weights, then rows: loads that wait for one another only where they must
+    auto places = [&](int64_t e) {
 #pragma unroll
-        for (int i = 0; i < V::N; ++i) sum[i] = 0.0f;
-        for (int k0 = 0; k0 < m.slots; k0 += B) {
-            V v[B];
-            float w[B];
-            bool there[B];
+        for (int b = 0; b < B; ++b) p[b] = (uint32_t)m.position[min(e + b, e1 - 1)];
+        load_weights(m, weights, weight_type, e, w);
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+            if (e + b >= e1) p[b] = ~0u;
+    };
+    if (SLOTS) places(e0);
+    const uint32_t kept = kept_entries(m);
+    for (int64_t c0 = (threadIdx.x % G) * V::N; c0 < m.width; c0 += G * V::N * U) {
+        float sum[U][M][V::N];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int t = 0; t < M; ++t)
+#pragma unroll
+                for (int i = 0; i < V::N; ++i) sum[u][t][i] = 0.0f;
+        for (int64_t e = e0; e < e1; e += B) {
+            if (!SLOTS) places(e);
+            V v[U][B];
 #pragma unroll
             for (int b = 0; b < B; ++b) {
-                const int64_t e = token * m.slots + k0 + b;
-                there[b] = false;
-                if (k0 + b < m.slots) {
-                    const uint32_t p = (uint32_t)m.position[e];
-                    there[b] = p < kept;
-                    if (there[b]) {
-                        v[b].load_once(z + (int64_t)p * z_stride + c);
-                        w[b] = weights ? rows::load_weight(weights, weight_type, e) : 1.0f;
-                    }
-                }
+                const T* row = z + (int64_t)p[b] * z_stride + c0;
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (p[b] < kept && c0 + u * G * V::N < m.width) v[u][b].load_once(row + u * G * V::N);
             }
 #pragma unroll
             for (int b = 0; b < B; ++b)
-                if (there[b]) {
+                if (p[b] < kept) {
 #pragma unroll
-                    for (int i = 0; i < V::N; ++i) sum[i] = fmaf(w[b], rows::to_float(v[b].v[i]), sum[i]);
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int i = 0; i < V::N; ++i)
+                            sum[u][b / S][i] = fmaf(w[b], rows::to_float(v[u][b].v[i]), sum[u][b / S][i]);
                 }
         }
-        V r;
 #pragma unroll
-        for (int i = 0; i < V::N; ++i) r.v[i] = rows::from_float<T>(sum[i]);
-        r.store(out + token * m.width + c);
+        for (int t = 0; t < M; ++t) {
+            if (token + t >= m.tokens) break;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (c0 + u * G * V::N >= m.width) break;
+                V r;
+#pragma unroll
+                for (int i = 0; i < V::N; ++i) r.v[i] = rows::from_float<T>(sum[u][t][i]);
+                r.store(out + (token + t) * m.width + c0 + u * G * V::N);
+            }
+        }
     }
 }
 
+// Sums of B values a thread over the group; every thread has them.
+template <int G, int B>
+__device__ __forceinline__ void group_sum(float (&v)[B]) {
+    constexpr int W = G < 32 ? G : 32;
+    const unsigned lanes = G < 32 ? ((1u << (G & 31)) - 1u) << ((threadIdx.x & 31) / G * G) : 0xffffffffu;
+#pragma unroll
+    for (int s = W / 2; s > 0; s >>= 1)
+#pragma unroll
+        for (int b = 0; b < B; ++b) v[b] += __shfl_xor_sync(lanes, v[b], s);
+    if (G == 256) {
+        __shared__ float part[B][8];
+        __syncthreads();
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+            if ((threadIdx.x & 31) == 0) part[b][threadIdx.x >> 5] = v[b];
+        __syncthreads();
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            v[b] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[b] += part[b][i];
+        }
+    }
+}
+
+// Wide rows: a group goes through a token's entries, 4 vectors a thread (8 short ones) of z and of dy, which
+// is in L1 after the first entry.
 template <typename T, int VB, int G>
 __global__ void __launch_bounds__(256) combine_grad_kernel(Moves m, const T* __restrict__ dy, int64_t dy_stride,
                                                            const T* __restrict__ z, int64_t z_stride,
                                                            const void* __restrict__ weights, int weight_type,
                                                            T* __restrict__ dz, void* __restrict__ dw) {
     using V = Vec<T, VB>;
-    constexpr int U = 4;
-    __shared__ float part[8];
+    constexpr int U = VB >= 8 ? 4 : 8;
     const int64_t token = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
     if (token >= m.tokens) return;  // G = 256: the whole block or none of it
     const uint32_t kept = kept_entries(m);
@@ -134,7 +205,7 @@ __global__ void __launch_bounds__(256) combine_grad_kernel(Moves m, const T* __r
         const float w = weights && there ? rows::load_weight(weights, weight_type, e) : 1.0f;
         const T* zrow = z + (int64_t)p * z_stride;
         T* to = dz + (int64_t)p * m.width;
-        float dot = 0.0f;
+        float dot[1] = {0.0f};
         if (there) {
             for (int64_t c0 = (threadIdx.x % G) * V::N; c0 < m.width; c0 += G * V::N * U) {
                 V g[U], a[U];
@@ -154,7 +225,7 @@ __global__ void __launch_bounds__(256) combine_grad_kernel(Moves m, const T* __r
 #pragma unroll
                         for (int i = 0; i < V::N; ++i) {
                             const float gv = rows::to_float(g[u].v[i]);
-                            if (dw) dot = fmaf(gv, rows::to_float(a[u].v[i]), dot);
+                            if (dw) dot[0] = fmaf(gv, rows::to_float(a[u].v[i]), dot[0]);
                             r.v[i] = rows::from_float<T>(w * gv);
                         }
                         r.store(to + c);
@@ -167,37 +238,81 @@ __global__ void __launch_bounds__(256) combine_grad_kernel(Moves m, const T* __r
             for (int64_t c = (threadIdx.x % G) * V::N; c < m.width; c += G * V::N) r.store(to + c);
         }
         if (dw) {
-            constexpr int W = G < 32 ? G : 32;
-            const unsigned lanes = G < 32 ? ((1u << (G & 31)) - 1u) << ((threadIdx.x & 31) / G * G) : 0xffffffffu;
-#pragma unroll
-            for (int s = W / 2; s > 0; s >>= 1) dot += __shfl_xor_sync(lanes, dot, s);
-            if (G == 256) {
-                if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = dot;
-                __syncthreads();
-                dot = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) dot += part[i];
-                __syncthreads();
-            }
-            if (threadIdx.x % G == 0) rows::store_weight(dw, weight_type, e, dot);
+            group_sum<G>(dot);
+            if (threadIdx.x % G == 0) rows::store_weight(dw, weight_type, e, dot[0]);
         }
     }
 }
 
-// Threads a token: 8 for rows of up to 8 vectors, else a warp; a block when the tokens are too few to
+// Rows of at most a vector a thread: a group serves 4 entries that follow each other.
+template <typename T, int VB, int G>
+__global__ void __launch_bounds__(256) combine_grad_narrow(Moves m, const T* __restrict__ dy, int64_t dy_stride,
+                                                           const T* __restrict__ z, int64_t z_stride,
+                                                           const void* __restrict__ weights, int weight_type,
+                                                           T* __restrict__ dz, void* __restrict__ dw) {
+    using V = Vec<T, VB>;
+    constexpr int B = 4;
+    const int64_t e0 = ((int64_t)blockIdx.x * (256 / G) + threadIdx.x / G) * B;
+    if (e0 >= m.entries) return;
+    const int64_t c = (threadIdx.x % G) * V::N;
+    const bool mine = c < m.width;
+    uint32_t p[B];
+    float w[B], dot[B];
+    V g[B], a[B];
+#pragma unroll
+    for (int b = 0; b < B; ++b) p[b] = (uint32_t)m.position[min(e0 + b, m.entries - 1)];
+    load_weights(m, weights, weight_type, e0, w);
+    const uint32_t kept = kept_entries(m);
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+        if (e0 + b >= m.entries) p[b] = ~0u;
+        if (p[b] < kept && mine) {
+            if (dw) a[b].load_once(z + (int64_t)p[b] * z_stride + c);
+            g[b].load(dy + (int64_t)((uint32_t)(e0 + b) / (uint32_t)m.slots) * dy_stride + c);
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+        dot[b] = 0.0f;
+        if (p[b] >= (uint64_t)m.entries || !mine) continue;
+        V r;
+        if (p[b] < kept) {
+#pragma unroll
+            for (int i = 0; i < V::N; ++i) {
+                const float gv = rows::to_float(g[b].v[i]);
+                if (dw) dot[b] = fmaf(gv, rows::to_float(a[b].v[i]), dot[b]);
+                r.v[i] = rows::from_float<T>(w[b] * gv);
+            }
+        } else {
+            r.zero();
+        }
+        r.store(dz + (int64_t)p[b] * m.width + c);
+    }
+    if (!dw) return;
+    group_sum<G>(dot);
+    if (threadIdx.x % G == 0) {
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+            if (e0 + b < m.entries) rows::store_weight(dw, weight_type, e0 + b, dot[b]);
+    }
+}
+
+// Threads a group: 8 for rows of up to 8 vectors, else a warp; a block when the groups are too few to
 // fill the SMs with warps and a row has more than a warp's vectors.
-inline int group_of(int64_t tokens, int64_t vectors) {
+inline int group_of(int64_t groups, int64_t vectors) {
     if (vectors <= 8) return 8;
-    if (tokens < 148 * 8 && vectors > 32) return 256;
+    if (groups < 148 * 8 && vectors > 32) return 256;
     return 32;
 }
+// Tokens a group of combine_kernel.
+inline int tokens_of(int64_t slots) { return slots == 1 ? 4 : slots == 2 ? 2 : 1; }
 template <typename F>
 inline void for_group(int g, F&& f) {
     if (g == 8) f(rows::Bytes<8>{});
     else if (g == 32) f(rows::Bytes<32>{});
     else f(rows::Bytes<256>{});
 }
-inline unsigned blocks_of(int64_t tokens, int g) { return (unsigned)((tokens + 256 / g - 1) / (256 / g)); }
+inline unsigned blocks_of(int64_t groups, int g) { return (unsigned)((groups + 256 / g - 1) / (256 / g)); }
 
 // Shapes and pointers that every move checks; HB_OK or the failure.
 int check(const char* what, int type, int64_t tokens, int64_t slots, int64_t width, const void* position,
@@ -247,13 +362,23 @@ extern "C" int hb_route_dispatch(int type, const void* x, int64_t x_stride, int6
     const Moves m{tokens, tokens * slots, width, (int)slots, position, kept};
     const int vb = rows::vector_bytes(rows::address_bits(x) | rows::address_bits(sorted) | (uint64_t)(x_stride * size) |
                                       (uint64_t)(width * size), type);
-    const int g = group_of(tokens, width * size / vb);
+    const int64_t vectors = width * size / vb;
+    const int g = group_of(tokens, vectors);
+    const auto st = static_cast<cudaStream_t>(stream);
     rows::for_type(type, vb, [&](auto t, auto b) {
         using T = decltype(t);
         for_group(g, [&](auto gg) {
-            constexpr int G = decltype(gg)::value;
-            dispatch_kernel<T, decltype(b)::value, G><<<blocks_of(tokens, G), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-                m, static_cast<const T*>(x), x_stride, static_cast<T*>(sorted));
+            constexpr int G = decltype(gg)::value, VB = decltype(b)::value;
+            if constexpr (G < 256) {
+                if (vectors <= G) {
+                    dispatch_kernel<T, VB, G, true><<<blocks_of((tokens + 3) / 4, G), 256, 0, st>>>(
+                        m, static_cast<const T*>(x), x_stride, static_cast<T*>(sorted));
+                    return;
+                }
+            }
+            if constexpr (G > 8)  // 8 threads are for rows of up to 8 vectors
+                dispatch_kernel<T, VB, G, false><<<blocks_of(tokens, G), 256, 0, st>>>(
+                    m, static_cast<const T*>(x), x_stride, static_cast<T*>(sorted));
         });
     });
     return launched("route dispatch");
@@ -271,13 +396,21 @@ extern "C" int hb_route_combine(int type, const void* z, int64_t z_stride, int64
     const Moves m{tokens, tokens * slots, width, (int)slots, position, kept};
     const int vb = rows::vector_bytes(rows::address_bits(z) | rows::address_bits(out) | (uint64_t)(z_stride * size) |
                                       (uint64_t)(width * size), type);
-    const int g = group_of(tokens, width * size / vb);
+    const int64_t groups = (tokens + tokens_of(slots) - 1) / tokens_of(slots);
+    const int g = group_of(groups, width * size / vb);
     rows::for_type(type, vb, [&](auto t, auto b) {
         using T = decltype(t);
         for_group(g, [&](auto gg) {
-            constexpr int G = decltype(gg)::value;
-            combine_kernel<T, decltype(b)::value, G><<<blocks_of(tokens, G), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-                m, static_cast<const T*>(z), z_stride, weights, weight_type, static_cast<T*>(out));
+            constexpr int G = decltype(gg)::value, VB = decltype(b)::value;
+            auto launch = [&](auto s) {
+                combine_kernel<T, VB, G, decltype(s)::value>
+                    <<<blocks_of(groups, G), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+                        m, static_cast<const T*>(z), z_stride, weights, weight_type, static_cast<T*>(out));
+            };
+            if (slots == 1) launch(rows::Bytes<1>{});
+            else if (slots == 2) launch(rows::Bytes<2>{});
+            else if (slots == 4) launch(rows::Bytes<4>{});
+            else launch(rows::Bytes<0>{});
         });
     });
     return launched("route combine");
@@ -300,13 +433,23 @@ extern "C" int hb_route_combine_grad(int type, const void* dy, int64_t dy_stride
     uint64_t bits = rows::address_bits(dy) | rows::address_bits(dz) | (uint64_t)(dy_stride * size) | (uint64_t)(width * size);
     if (dweights) bits |= rows::address_bits(z) | (uint64_t)(z_stride * size);
     const int vb = rows::vector_bytes(bits, type);
-    const int g = group_of(tokens, width * size / vb);
+    const int64_t vectors = width * size / vb;
+    const int g = group_of(tokens, vectors);
+    const auto st = static_cast<cudaStream_t>(stream);
     rows::for_type(type, vb, [&](auto t, auto b) {
         using T = decltype(t);
         for_group(g, [&](auto gg) {
-            constexpr int G = decltype(gg)::value;
-            combine_grad_kernel<T, decltype(b)::value, G>
-                <<<blocks_of(tokens, G), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+            constexpr int G = decltype(gg)::value, VB = decltype(b)::value;
+            if constexpr (G < 256) {
+                if (vectors <= G) {
+                    combine_grad_narrow<T, VB, G><<<blocks_of((m.entries + 3) / 4, G), 256, 0, st>>>(
+                        m, static_cast<const T*>(dy), dy_stride, static_cast<const T*>(z), z_stride, weights, weight_type,
+                        static_cast<T*>(dz), dweights);
+                    return;
+                }
+            }
+            if constexpr (G > 8)
+                combine_grad_kernel<T, VB, G><<<blocks_of(tokens, G), 256, 0, st>>>(
                     m, static_cast<const T*>(dy), dy_stride, static_cast<const T*>(z), z_stride, weights, weight_type,
                     static_cast<T*>(dz), dweights);
         });

@@ -9,22 +9,20 @@ from __future__ import annotations
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._lib import FLOAT_TYPES, check, current, feature_rows, index_bytes, on_device
+from ._lib import FLOAT_TYPES, call, device_of, feature_rows, index_bytes, load_library
 
 
 def _lookup(table, ids, scale):
     size = index_bytes(ids, "ids")
     table, stride = feature_rows(table, "table")
-    L = on_device("embedding_lookup", table, ids)
+    device = device_of("embedding_lookup", table, ids)
     ids = ids.contiguous()
     n, (rows, width) = ids.numel(), table.shape
     if n >= 2 ** 31:
         raise ValueError("embedding_lookup: at most 2^31 - 1 ids")
-    out = torch.empty((*ids.shape, width), dtype=table.dtype, device=table.device)
-    with current(table) as stream:
-        rc = L.hb_embedding_lookup(FLOAT_TYPES[table.dtype], table.data_ptr(), stride, rows, width, ids.data_ptr(), size,
-                                   n, scale, out.data_ptr(), stream)
-    check(rc)
+    out = table.new_empty((*ids.shape, width))
+    call(device, load_library().hb_embedding_lookup, FLOAT_TYPES[table.dtype], table.data_ptr(), stride, rows, width,
+         ids.data_ptr(), size, n, scale, out.data_ptr())
     return out
 
 
@@ -43,6 +41,8 @@ def embedding_grad(dy, ids, rows: int, *, scale: float = 1.0, dtype=None, out=No
     if ids.numel() >= 2 ** 31:
         raise ValueError(f"{what}: at most 2^31 - 1 ids")
     dy, stride = feature_rows(dy.reshape(ids.numel(), width), "dy")
+    if stride * dy.element_size() >= 2 ** 32:
+        dy, stride = dy.contiguous(), width
     if dtype is None:
         dtype = dy.dtype if out is None else out.dtype
     if dtype != dy.dtype and dtype != torch.float32:
@@ -50,21 +50,19 @@ def embedding_grad(dy, ids, rows: int, *, scale: float = 1.0, dtype=None, out=No
     if out is None:
         if accumulate:
             raise ValueError(f"{what}: accumulate needs out")
-        L = on_device(what, dy, ids)
-        out = torch.empty((rows, width), dtype=dtype, device=dy.device)
+        device = device_of(what, dy, ids)
+        out = dy.new_empty((rows, width), dtype=dtype)
     else:
-        L = on_device(what, dy, ids, out)
+        device = device_of(what, dy, ids, out)
         if out.dtype != dtype or out.shape != (rows, width) or not out.is_contiguous():
             raise ValueError(f"{what}: out must be a contiguous {dtype} tensor of shape {(rows, width)}")
     ids = ids.contiguous()
     n = ids.numel()
+    L = load_library()
     nbytes = L.hb_embedding_grad_workspace(n, rows, width)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dy.device)
-    with current(dy) as stream:
-        rc = L.hb_embedding_grad(FLOAT_TYPES[dy.dtype], dy.data_ptr(), stride, ids.data_ptr(), size, n, rows, width,
-                                 scale, FLOAT_TYPES[dtype], out.data_ptr(), bool(accumulate), ws.data_ptr(), nbytes,
-                                 stream)
-    check(rc)
+    ws = dy.new_empty(nbytes, dtype=torch.uint8)
+    call(device, L.hb_embedding_grad, FLOAT_TYPES[dy.dtype], dy.data_ptr(), stride, ids.data_ptr(), size, n, rows, width,
+         scale, FLOAT_TYPES[dtype], out.data_ptr(), bool(accumulate), ws.data_ptr(), nbytes)
     return out
 
 

@@ -9,13 +9,11 @@ from array import array
 
 import torch
 
-from ._lib import FLOAT_TYPES, check, current, on_device
+from ._lib import FLOAT_TYPES, call, device_of, load_library
 
 
 def _dense(t) -> bool:
     """Whether t's elements fill one stretch of memory, in any order of its dimensions."""
-    if t.is_contiguous():
-        return True
     size = 1
     for step, length in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
         if step != size:
@@ -25,60 +23,66 @@ def _dense(t) -> bool:
 
 
 def _addresses(tensors, what: str):
-    """Host arrays (addresses, element types) of float tensors, each dense in memory."""
-    for t in tensors:
-        if t.dtype not in FLOAT_TYPES:
-            raise ValueError(f"{what}: gradients are float32, float16 or bfloat16, got {t.dtype}")
-        if not _dense(t):
-            raise ValueError(f"{what}: gradients must be dense in memory, got strides {t.stride()} for {tuple(t.shape)}")
-    addresses = array("Q", [t.data_ptr() for t in tensors])
-    if len({a for a in addresses if a}) != sum(1 for a in addresses if a):
-        raise ValueError(f"{what}: a tensor is listed twice")
-    return addresses, array("i", [FLOAT_TYPES[t.dtype] for t in tensors])
+    """Host arrays (addresses, element types) of float tensors, each dense in memory, and whether all are
+    contiguous."""
+    try:
+        types = array("i", [FLOAT_TYPES[t.dtype] for t in tensors])
+    except KeyError as e:
+        raise ValueError(f"{what}: gradients are float32, float16 or bfloat16, got {e.args[0]}") from None
+    contiguous = all(t.is_contiguous() for t in tensors)
+    if not contiguous:
+        for t in tensors:
+            if not t.is_contiguous() and not _dense(t):
+                raise ValueError(f"{what}: gradients must be dense in memory, got strides {t.stride()} for "
+                                 f"{tuple(t.shape)}")
+    addresses = [t.data_ptr() for t in tensors]
+    if len(set(addresses)) != len(addresses):  # tensors without elements may share an address
+        full = [t.data_ptr() for t in tensors if t.numel()]
+        if len(set(full)) != len(full):
+            raise ValueError(f"{what}: a tensor is listed twice")
+    return array("Q", addresses), types, contiguous
 
 
-def _address(a):
-    return a.buffer_info()[0] if a else None
+def _tensors(v):
+    return [v] if torch.is_tensor(v) else list(v)
 
 
 def _run(grads, limit, out, what):
-    grads = [grads] if torch.is_tensor(grads) else list(grads)
+    grads = _tensors(grads)
     if not grads:
         raise ValueError(f"{what}: no gradients")
-    L = on_device(what, *grads)
-    pointers, types = _addresses(grads, what)
+    device = device_of(what, *grads)
+    pointers, types, contiguous = _addresses(grads, what)
     sizes = array("q", [g.numel() for g in grads])
-    first = grads[0]
-    norm = torch.empty((), dtype=torch.float32, device=first.device)
+    L = load_library()
+    norm = grads[0].new_empty((), dtype=torch.float32)
     nbytes = L.hb_clip_workspace(len(grads))
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=first.device)
-    common = (len(grads), _address(pointers), _address(sizes), _address(types))
+    ws = grads[0].new_empty(nbytes, dtype=torch.uint8)
+    host = [len(grads), pointers.buffer_info()[0], sizes.buffer_info()[0], types.buffer_info()[0]]
     if limit is None:
-        with current(first) as stream:
-            rc = L.hb_grad_norm(*common, norm.data_ptr(), ws.data_ptr(), nbytes, stream)
-    else:
-        limit = float(limit)
-        if not limit >= 0.0:
-            raise ValueError(f"{what}: max_norm must be a number >= 0, got {limit}")
-        to_pointers, to_types = pointers, types
-        if out is not None:
-            out = [out] if torch.is_tensor(out) else list(out)
-            if len(out) != len(grads):
-                raise ValueError(f"{what}: {len(out)} outputs for {len(grads)} gradients")
-            on_device(what, first, *out)
+        call(device, L.hb_grad_norm, *host, norm.data_ptr(), ws.data_ptr(), nbytes)
+        return norm
+    limit = float(limit)
+    if not limit >= 0.0:
+        raise ValueError(f"{what}: max_norm must be a number >= 0, got {limit}")
+    to_pointers, to_types = pointers, types
+    if out is not None:
+        out = _tensors(out)
+        if [g.shape for g in grads] != [o.shape for o in out]:
+            raise ValueError(f"{what}: outputs have their gradients' shapes")
+        if device_of(what, *out) != device:
+            raise ValueError(f"{what}: outputs on another device than their gradients")
+        to_pointers, to_types, to_contiguous = _addresses(out, what)
+        if not (contiguous and to_contiguous) and any(o.stride() != g.stride() for g, o in zip(grads, out)
+                                                      if not (g.is_contiguous() and o.is_contiguous())):
+            raise ValueError(f"{what}: outputs have their gradients' strides")
+        if to_types != types:
             for g, o in zip(grads, out):
-                if o.shape != g.shape or (o.dtype != g.dtype and o.dtype != torch.float32):
-                    raise ValueError(f"{what}: an output has its gradient's shape, and its type or float32; got "
-                                     f"{tuple(o.shape)} {o.dtype} for {tuple(g.shape)} {g.dtype}")
-                if o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()):
-                    raise ValueError(f"{what}: an output has its gradient's strides")
-                if o.dtype != g.dtype and o.data_ptr() == g.data_ptr() and g.numel():
-                    raise ValueError(f"{what}: an output in place has its gradient's type")
-            to_pointers, to_types = _addresses(out, what)
-        with current(first) as stream:
-            rc = L.hb_clip_grad_norm(*common, _address(to_pointers), _address(to_types), limit, norm.data_ptr(),
-                                     ws.data_ptr(), nbytes, stream)
-    check(rc)
+                if o.dtype != g.dtype and (o.dtype != torch.float32 or (g.numel() and o.data_ptr() == g.data_ptr())):
+                    raise ValueError(f"{what}: an output has its gradient's type, or is float32 and not in place; got "
+                                     f"{o.dtype} for {g.dtype}")
+    call(device, L.hb_clip_grad_norm, *host, to_pointers.buffer_info()[0], to_types.buffer_info()[0], limit,
+         norm.data_ptr(), ws.data_ptr(), nbytes)
     return norm
 
 

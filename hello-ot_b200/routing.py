@@ -19,7 +19,7 @@ from typing import NamedTuple
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._lib import FLOAT_TYPES, check, current, feature_rows, index_bytes, on_device
+from ._lib import FLOAT_TYPES, call, device_of, feature_rows, index_bytes, load_library
 
 
 class RoutePlan(NamedTuple):
@@ -62,18 +62,17 @@ def route_plan(index, num_experts: int) -> RoutePlan:
     n = index.numel()
     if n >= 2 ** 31:
         raise ValueError("an assignment holds at most 2^31 - 1 entries")
-    L = on_device("route_plan", index)
+    device = device_of("route_plan", index)
     index = index.contiguous()
-    device = index.device
-    order = torch.empty(n, dtype=torch.int32, device=device)
-    position = torch.empty((index.shape[0], 1 if index.dim() == 1 else index.shape[1]), dtype=torch.int32, device=device)
-    offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=device)
+    L = load_library()
+    int32 = torch.int32
+    order = index.new_empty(n, dtype=int32)
+    position = index.new_empty((index.shape[0], 1 if index.dim() == 1 else index.shape[1]), dtype=int32)
+    offsets = index.new_empty(num_experts + 1, dtype=int32)
     nbytes = L.hb_index_sort_workspace(n, num_experts)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    with current(index) as stream:
-        rc = L.hb_index_sort(index.data_ptr(), size, n, num_experts, order.data_ptr(), position.data_ptr(),
-                             offsets.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, stream)
-    check(rc)
+    ws = index.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    call(device, L.hb_index_sort, index.data_ptr(), size, n, num_experts, order.data_ptr(), position.data_ptr(),
+         offsets.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
     return RoutePlan(order, position, offsets)
 
 
@@ -101,13 +100,11 @@ def _dispatch(x, plan):
     tokens, slots = position.shape
     if x.shape[0] != tokens:
         raise ValueError(f"route_dispatch: x has {x.shape[0]} rows for {tokens} tokens")
-    L = on_device("route_dispatch", x, position, plan.offsets)
+    device = device_of("route_dispatch", x, position, plan.offsets)
     width = x.shape[1]
-    out = torch.empty((tokens * slots, width), dtype=x.dtype, device=x.device)
-    with current(x) as stream:
-        rc = L.hb_route_dispatch(FLOAT_TYPES[x.dtype], x.data_ptr(), stride, tokens, slots, width, position.data_ptr(),
-                                 kept, out.data_ptr(), stream)
-    check(rc)
+    out = x.new_empty((tokens * slots, width))
+    call(device, load_library().hb_route_dispatch, FLOAT_TYPES[x.dtype], x.data_ptr(), stride, tokens, slots, width,
+         position.data_ptr(), kept, out.data_ptr())
     return out
 
 
@@ -118,17 +115,15 @@ def _combine(z, plan, weights, what="route_combine"):
     if z.shape[0] != tokens * slots:
         raise ValueError(f"{what}: {z.shape[0]} sorted rows for {tokens} x {slots} entries")
     if weights is None:
-        L, wptr, wtype = on_device(what, z, position, plan.offsets), None, 0
+        device, wptr, wtype = device_of(what, z, position, plan.offsets), None, 0
     else:
         weights = _weights(weights, position, what)
-        L = on_device(what, z, position, plan.offsets, weights)
+        device = device_of(what, z, position, plan.offsets, weights)
         wptr, wtype = weights.data_ptr(), FLOAT_TYPES[weights.dtype]
     width = z.shape[1]
-    out = torch.empty((tokens, width), dtype=z.dtype, device=z.device)
-    with current(z) as stream:
-        rc = L.hb_route_combine(FLOAT_TYPES[z.dtype], z.data_ptr(), stride, tokens, slots, width, position.data_ptr(),
-                                kept, wptr, wtype, out.data_ptr(), stream)
-    check(rc)
+    out = z.new_empty((tokens, width))
+    call(device, load_library().hb_route_combine, FLOAT_TYPES[z.dtype], z.data_ptr(), stride, tokens, slots, width,
+         position.data_ptr(), kept, wptr, wtype, out.data_ptr())
     return out
 
 
@@ -150,19 +145,17 @@ def route_combine_grad(dy, z, plan, weights=None, *, need_weights: bool = True):
                          f"assignment {tuple(position.shape)}")
     dw, wptr, wtype = None, None, 0
     if weights is None:
-        L = on_device(what, dy, z, position, plan.offsets)
+        device = device_of(what, dy, z, position, plan.offsets)
     else:
         weights = _weights(weights, position, what)
-        L = on_device(what, dy, z, position, plan.offsets, weights)
+        device = device_of(what, dy, z, position, plan.offsets, weights)
         wptr, wtype = weights.data_ptr(), FLOAT_TYPES[weights.dtype]
         if need_weights:
             dw = torch.empty_like(weights)
-    dz = torch.empty((tokens * slots, z.shape[1]), dtype=z.dtype, device=z.device)
-    with current(z) as stream:
-        rc = L.hb_route_combine_grad(FLOAT_TYPES[z.dtype], dy.data_ptr(), dy_stride, z.data_ptr(), z_stride, tokens,
-                                     slots, z.shape[1], position.data_ptr(), kept, wptr, wtype, dz.data_ptr(),
-                                     None if dw is None else dw.data_ptr(), stream)
-    check(rc)
+    dz = z.new_empty((tokens * slots, z.shape[1]))
+    call(device, load_library().hb_route_combine_grad, FLOAT_TYPES[z.dtype], dy.data_ptr(), dy_stride, z.data_ptr(),
+         z_stride, tokens, slots, z.shape[1], position.data_ptr(), kept, wptr, wtype, dz.data_ptr(),
+         None if dw is None else dw.data_ptr())
     return dz, dw
 
 

@@ -24,9 +24,10 @@ def _check_plan(plan, index, experts):
 
 @pytest.mark.parametrize("tokens,slots,experts", [
     (1, 1, 1), (1, 2, 16), (31, 1, 2), (33, 3, 5), (511, 8, 64), (512, 8, 255), (513, 8, 256),  # one block, one pass
-    (4096, 1, 2047), (4096, 1, 2048), (1365, 3, 70000),                                     # one block, two and three passes
-    (4097, 1, 7), (5000, 3, 1024), (100, 100, 2047), (4097, 1, 2048), (20000, 2, 100003),       # tiles of 1024
-    (3000, 4, 5_000_000),                                                                       # tiles, three passes
+    (4096, 1, 2047), (4096, 1, 2048), (1365, 3, 70000), (1365, 3, 5_000_000),                   # two and three passes
+    (4097, 1, 7), (5000, 3, 1024), (100, 100, 2047), (8193, 2, 300), (65537, 1, 5), (131072, 1, 2047),  # clusters
+    (4097, 1, 2048), (20000, 2, 100003), (3000, 4, 5_000_000), (65536, 2, 65536),
+    (131073, 1, 1024), (200000, 2, 100003), (140000, 1, 5_000_000),                             # tiles of 1024
     (2 ** 19 + 5, 1, 37), (70001, 8, 1025), (2 ** 19 + 1, 1, 4000)])                            # tiles of 4096
 @pytest.mark.parametrize("dropped", [0.0, 0.2])
 def test_plan_matches_counting(hb, cuda, tokens, slots, experts, dropped):
