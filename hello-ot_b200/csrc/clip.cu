@@ -287,7 +287,8 @@ int check(int64_t count, const void* const* in, const int64_t* size, const int32
         return abi_fail(HB_BAD_ARGUMENT, "gradient norm: null pointer");
     int64_t chunks = 0;
     for (int64_t i = 0; i < count; ++i) {
-        if (size[i] < 0 || !rows::valid_type(type[i]) || (size[i] > 0 && !in[i]))
+        if (size[i] < 0 || !rows::valid_type(type[i]) || (size[i] > 0 && !in[i]) ||
+            rows::address_bits(in[i]) % rows::type_bytes(type[i]))
             return abi_fail(HB_BAD_ARGUMENT, "gradient norm: size, type or pointer of a tensor");
         if (size[i] > INT32_MAX * kChunk || (chunks += (size[i] + kChunk - 1) / kChunk) > INT32_MAX)
             return abi_fail(HB_BAD_ARGUMENT, "gradient norm: too many elements");
@@ -353,7 +354,8 @@ extern "C" int hb_clip_grad_norm(int64_t count, const void* const* grads, const 
     if (!(limit >= 0.0)) return abi_fail(HB_BAD_ARGUMENT, "gradient clipping: the limit must be a number >= 0");
     if (count > 0 && (!outs || !out_types)) return abi_fail(HB_BAD_ARGUMENT, "gradient clipping: null pointer");
     for (int64_t i = 0; i < count; ++i)
-        if (sizes[i] > 0 && (!outs[i] || (out_types[i] != types[i] && out_types[i] != HB_F32)))
+        if (sizes[i] > 0 && (!outs[i] || (out_types[i] != types[i] && out_types[i] != HB_F32) ||
+                             rows::address_bits(outs[i]) % rows::type_bytes(out_types[i])))
             return abi_fail(HB_BAD_ARGUMENT, "gradient clipping: an output has its gradient's type or is fp32");
     static void* const none[1] = {nullptr};
     static const int32_t any[1] = {HB_F32};

@@ -479,6 +479,8 @@ extern "C" int hb_embedding_lookup(int type, const void* table, int64_t table_st
     if (n == 0 || width == 0) return HB_OK;
     if ((rows_ > 0 && !table) || !ids || !out) return abi_fail(HB_BAD_ARGUMENT, "embedding lookup: null pointer");
     const int size = rows::type_bytes(type);
+    if ((rows::address_bits(table) | rows::address_bits(out)) % size || rows::address_bits(ids) % id_bytes)
+        return abi_fail(HB_BAD_ARGUMENT, "embedding lookup: misaligned pointer");
     const int vb = rows::vector_bytes(rows::address_bits(table) | rows::address_bits(out) |
                                       (uint64_t)(table_stride * size) | (uint64_t)(width * size), type);
     // few rows: a thread a vector, so that every load starts at once.  Enough rows for 16 blocks an SM: 4
@@ -524,8 +526,9 @@ extern "C" int hb_embedding_grad(int type, const void* dy, int64_t dy_stride, co
         if (!accumulate) e = cudaMemsetAsync(out, 0, (size_t)rows_ * width * out_size, st);
         return e == cudaSuccess ? HB_OK : abi_fail(HB_CUDA, std::string("embedding gradient: ") + cudaGetErrorString(e));
     }
-    if (rows::address_bits(workspace) % 256)
-        return abi_fail(HB_BAD_ARGUMENT, "embedding gradient: the workspace must be 256-byte aligned");
+    if (rows::address_bits(workspace) % 256 || rows::address_bits(dy) % size || rows::address_bits(out) % out_size ||
+        rows::address_bits(ids) % id_bytes)
+        return abi_fail(HB_BAD_ARGUMENT, "embedding gradient: misaligned pointer, or a workspace that is not 256-byte aligned");
     const Layout l = layout(workspace, n, rows_, width);
     if (workspace_bytes < l.bytes)
         return abi_fail(HB_WORKSPACE, "workspace smaller than hb_embedding_grad_workspace()");

@@ -483,7 +483,8 @@ int index_sort(const void* index, int index_bytes, int64_t n, int64_t bins, int3
     }
     const Plan p = plan_of(n, bins);
     const Layout l = layout(ws, n, p);
-    if ((uintptr_t)ws % 256) return abi_fail(HB_BAD_ARGUMENT, "index sort: the workspace must be 256-byte aligned");
+    if ((uintptr_t)ws % 256 || (uintptr_t)index % index_bytes)
+        return abi_fail(HB_BAD_ARGUMENT, "index sort: misaligned index, or a workspace that is not 256-byte aligned");
     if (l.bytes > ws_bytes || (l.bytes > 0 && !ws))
         return abi_fail(HB_WORKSPACE, "workspace too small for the index sort");
     const Source src{index, index_bytes, (uint32_t)bins};

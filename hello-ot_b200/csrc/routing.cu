@@ -11,9 +11,9 @@
 //
 // Every kernel goes by token: a group of threads holds the columns of a token, so
 // x, dy and y cross HBM once and each sorted row once, which is all they have to.
-// Bound by HBM, so what counts is loads in flight: each thread has 4 vectors of up
-// to 16 bytes under way, of one row or of 4.  Sums are fp32 and run over k in order
-// (no atomics): the result does not depend on the launch.
+// Bound by HBM, so what counts is loads in flight: each thread has 4 vectors of 8 or
+// 16 bytes under way, or 16 shorter ones, of one row or of 4.  Sums are fp32 and run
+// over k in order (no atomics): the result does not depend on the launch.
 #include <string>
 
 #include "index_sort.cuh"
@@ -36,41 +36,47 @@ __device__ __forceinline__ uint32_t kept_entries(const Moves& m) {
     return (uint32_t)min((int64_t)max(*m.kept, 0), m.entries);
 }
 
-// Wide rows: a group holds 4 vectors a thread of one token (8 short ones).  Rows of at most a vector a thread (NARROW): 4
-// tokens, so that as many loads are in flight.
+// Column steps of a narrow row: short vectors (rows off the 16-byte grid) take four to hold as many bytes in
+// flight as one long vector.
+constexpr int steps_of(int vb) { return vb >= 8 ? 1 : 4; }
+
+// A group serves M tokens, U column steps at a time: 4 vectors a thread in flight, 16 short ones.  Wide rows: one
+// token; narrow ones, of at most steps_of(VB) vectors a thread: 4.
 template <typename T, int VB, int G, bool NARROW>
 __global__ void __launch_bounds__(256) dispatch_kernel(Moves m, const T* __restrict__ x, int64_t x_stride,
                                                        T* __restrict__ out) {
     using V = Vec<T, VB>;
-    constexpr int U = NARROW || VB >= 8 ? 4 : 8;
-    const int64_t group = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
-    const int64_t token = NARROW ? group * U : group;
+    constexpr int M = NARROW ? 4 : 1, U = steps_of(VB) * 4 / M;
+    const int64_t token = ((int64_t)blockIdx.x * (256 / G) + threadIdx.x / G) * M;
     if (token >= m.tokens) return;
     const uint32_t kept = kept_entries(m);
-    // vector u: of token + u, or u * G vectors further on in the row
-    for (int64_t c0 = (threadIdx.x % G) * V::N; c0 < m.width; c0 += NARROW ? m.width : G * V::N * U) {
-        V v[U];
-        bool there[U];
+    for (int64_t c0 = (threadIdx.x % G) * V::N; c0 < m.width; c0 += G * V::N * U) {
+        V v[M][U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            there[u] = NARROW ? token + u < m.tokens : c0 + u * G * V::N < m.width;
-            if (there[u]) v[u].load_once(x + (NARROW ? token + u : token) * x_stride + (NARROW ? c0 : c0 + u * G * V::N));
-        }
-        for (int k = 0; k < m.slots; ++k) {
-            uint32_t p[U];
+        for (int t = 0; t < M; ++t)
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                p[u] = there[u] ? (uint32_t)m.position[(NARROW ? token + u : token) * m.slots + k] : ~0u;
+                if (token + t < m.tokens && c0 + u * G * V::N < m.width)
+                    v[t][u].load_once(x + (token + t) * x_stride + c0 + u * G * V::N);
+        for (int k = 0; k < m.slots; ++k) {
+            uint32_t p[M];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (!there[u] || p[u] >= (uint64_t)m.entries) continue;
-                T* to = out + (int64_t)p[u] * m.width + (NARROW ? c0 : c0 + u * G * V::N);
-                if (p[u] >= kept) {
-                    V w;
-                    w.zero();
-                    w.store(to);
-                } else {
-                    v[u].store(to);
+            for (int t = 0; t < M; ++t)
+                p[t] = token + t < m.tokens ? (uint32_t)m.position[(token + t) * m.slots + k] : ~0u;
+#pragma unroll
+            for (int t = 0; t < M; ++t) {
+                if (p[t] >= (uint64_t)m.entries) continue;
+                T* to = out + (int64_t)p[t] * m.width + c0;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (c0 + u * G * V::N >= m.width) break;
+                    if (p[t] >= kept) {
+                        V w;
+                        w.zero();
+                        w.store(to + u * G * V::N);
+                    } else {
+                        v[t][u].store(to + u * G * V::N);
+                    }
                 }
             }
         }
@@ -244,21 +250,20 @@ __global__ void __launch_bounds__(256) combine_grad_kernel(Moves m, const T* __r
     }
 }
 
-// Rows of at most a vector a thread: a group serves 4 entries that follow each other.
+// Narrow rows, of at most steps_of(VB) vectors a thread: a group serves 4 entries that follow each other.
 template <typename T, int VB, int G>
 __global__ void __launch_bounds__(256) combine_grad_narrow(Moves m, const T* __restrict__ dy, int64_t dy_stride,
                                                            const T* __restrict__ z, int64_t z_stride,
                                                            const void* __restrict__ weights, int weight_type,
                                                            T* __restrict__ dz, void* __restrict__ dw) {
     using V = Vec<T, VB>;
-    constexpr int B = 4;
+    constexpr int B = 4, U = steps_of(VB);
     const int64_t e0 = ((int64_t)blockIdx.x * (256 / G) + threadIdx.x / G) * B;
     if (e0 >= m.entries) return;
     const int64_t c = (threadIdx.x % G) * V::N;
-    const bool mine = c < m.width;
     uint32_t p[B];
     float w[B], dot[B];
-    V g[B], a[B];
+    V g[B][U], a[B][U];
 #pragma unroll
     for (int b = 0; b < B; ++b) p[b] = (uint32_t)m.position[min(e0 + b, m.entries - 1)];
     load_weights(m, weights, weight_type, e0, w);
@@ -266,27 +271,35 @@ __global__ void __launch_bounds__(256) combine_grad_narrow(Moves m, const T* __r
 #pragma unroll
     for (int b = 0; b < B; ++b) {
         if (e0 + b >= m.entries) p[b] = ~0u;
-        if (p[b] < kept && mine) {
-            if (dw) a[b].load_once(z + (int64_t)p[b] * z_stride + c);
-            g[b].load(dy + (int64_t)((uint32_t)(e0 + b) / (uint32_t)m.slots) * dy_stride + c);
-        }
+        const T* zrow = z + (int64_t)p[b] * z_stride;
+        const T* grow = dy + (int64_t)((uint32_t)(e0 + b) / (uint32_t)m.slots) * dy_stride;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (p[b] < kept && c + u * G * V::N < m.width) {
+                if (dw) a[b][u].load_once(zrow + c + u * G * V::N);
+                g[b][u].load(grow + c + u * G * V::N);
+            }
     }
 #pragma unroll
     for (int b = 0; b < B; ++b) {
         dot[b] = 0.0f;
-        if (p[b] >= (uint64_t)m.entries || !mine) continue;
-        V r;
-        if (p[b] < kept) {
+        if (p[b] >= (uint64_t)m.entries) continue;
 #pragma unroll
-            for (int i = 0; i < V::N; ++i) {
-                const float gv = rows::to_float(g[b].v[i]);
-                if (dw) dot[b] = fmaf(gv, rows::to_float(a[b].v[i]), dot[b]);
-                r.v[i] = rows::from_float<T>(w[b] * gv);
+        for (int u = 0; u < U; ++u) {
+            if (c + u * G * V::N >= m.width) break;
+            V r;
+            if (p[b] < kept) {
+#pragma unroll
+                for (int i = 0; i < V::N; ++i) {
+                    const float gv = rows::to_float(g[b][u].v[i]);
+                    if (dw) dot[b] = fmaf(gv, rows::to_float(a[b][u].v[i]), dot[b]);
+                    r.v[i] = rows::from_float<T>(w[b] * gv);
+                }
+            } else {
+                r.zero();
             }
-        } else {
-            r.zero();
+            r.store(dz + (int64_t)p[b] * m.width + c + u * G * V::N);
         }
-        r.store(dz + (int64_t)p[b] * m.width + c);
     }
     if (!dw) return;
     group_sum<G>(dot);
@@ -297,10 +310,10 @@ __global__ void __launch_bounds__(256) combine_grad_narrow(Moves m, const T* __r
     }
 }
 
-// Threads a group: 8 for rows of up to 8 vectors, else a warp; a block when the groups are too few to
-// fill the SMs with warps and a row has more than a warp's vectors.
-inline int group_of(int64_t groups, int64_t vectors) {
-    if (vectors <= 8) return 8;
+// Threads a group: 8 for rows that they hold in their column steps, else a warp; a block when the groups are
+// too few to fill the SMs with warps and a row has more than a warp's vectors.
+inline int group_of(int64_t groups, int64_t vectors, int vb) {
+    if (vectors <= 8 * steps_of(vb)) return 8;
     if (groups < 148 * 8 && vectors > 32) return 256;
     return 32;
 }
@@ -360,23 +373,25 @@ extern "C" int hb_route_dispatch(int type, const void* x, int64_t x_stride, int6
     if (!x || !sorted) return abi_fail(HB_BAD_ARGUMENT, "route dispatch: null pointer");
     const int size = rows::type_bytes(type);
     const Moves m{tokens, tokens * slots, width, (int)slots, position, kept};
+    if ((rows::address_bits(x) | rows::address_bits(sorted)) % size)
+        return abi_fail(HB_BAD_ARGUMENT, "route dispatch: misaligned pointer");
     const int vb = rows::vector_bytes(rows::address_bits(x) | rows::address_bits(sorted) | (uint64_t)(x_stride * size) |
                                       (uint64_t)(width * size), type);
     const int64_t vectors = width * size / vb;
-    const int g = group_of(tokens, vectors);
+    const int g = group_of(tokens, vectors, vb);
     const auto st = static_cast<cudaStream_t>(stream);
     rows::for_type(type, vb, [&](auto t, auto b) {
         using T = decltype(t);
         for_group(g, [&](auto gg) {
             constexpr int G = decltype(gg)::value, VB = decltype(b)::value;
             if constexpr (G < 256) {
-                if (vectors <= G) {
+                if (vectors <= G * steps_of(VB)) {
                     dispatch_kernel<T, VB, G, true><<<blocks_of((tokens + 3) / 4, G), 256, 0, st>>>(
                         m, static_cast<const T*>(x), x_stride, static_cast<T*>(sorted));
                     return;
                 }
             }
-            if constexpr (G > 8)  // 8 threads are for rows of up to 8 vectors
+            if constexpr (G > 8)  // 8 threads are for narrow rows
                 dispatch_kernel<T, VB, G, false><<<blocks_of(tokens, G), 256, 0, st>>>(
                     m, static_cast<const T*>(x), x_stride, static_cast<T*>(sorted));
         });
@@ -394,10 +409,12 @@ extern "C" int hb_route_combine(int type, const void* z, int64_t z_stride, int64
     if (!z || !out) return abi_fail(HB_BAD_ARGUMENT, "route combine: null pointer");
     const int size = rows::type_bytes(type);
     const Moves m{tokens, tokens * slots, width, (int)slots, position, kept};
+    if ((rows::address_bits(z) | rows::address_bits(out)) % size)
+        return abi_fail(HB_BAD_ARGUMENT, "route combine: misaligned pointer");
     const int vb = rows::vector_bytes(rows::address_bits(z) | rows::address_bits(out) | (uint64_t)(z_stride * size) |
                                       (uint64_t)(width * size), type);
     const int64_t groups = (tokens + tokens_of(slots) - 1) / tokens_of(slots);
-    const int g = group_of(groups, width * size / vb);
+    const int g = group_of(groups, width * size / vb, vb);
     rows::for_type(type, vb, [&](auto t, auto b) {
         using T = decltype(t);
         for_group(g, [&](auto gg) {
@@ -432,16 +449,17 @@ extern "C" int hb_route_combine_grad(int type, const void* dy, int64_t dy_stride
     const Moves m{tokens, tokens * slots, width, (int)slots, position, kept};
     uint64_t bits = rows::address_bits(dy) | rows::address_bits(dz) | (uint64_t)(dy_stride * size) | (uint64_t)(width * size);
     if (dweights) bits |= rows::address_bits(z) | (uint64_t)(z_stride * size);
+    if (bits % size) return abi_fail(HB_BAD_ARGUMENT, "route combine gradient: misaligned pointer");
     const int vb = rows::vector_bytes(bits, type);
     const int64_t vectors = width * size / vb;
-    const int g = group_of(tokens, vectors);
+    const int g = group_of(tokens, vectors, vb);
     const auto st = static_cast<cudaStream_t>(stream);
     rows::for_type(type, vb, [&](auto t, auto b) {
         using T = decltype(t);
         for_group(g, [&](auto gg) {
             constexpr int G = decltype(gg)::value, VB = decltype(b)::value;
             if constexpr (G < 256) {
-                if (vectors <= G) {
+                if (vectors <= G * steps_of(VB)) {
                     combine_grad_narrow<T, VB, G><<<blocks_of((m.entries + 3) / 4, G), 256, 0, st>>>(
                         m, static_cast<const T*>(dy), dy_stride, static_cast<const T*>(z), z_stride, weights, weight_type,
                         static_cast<T*>(dz), dweights);
