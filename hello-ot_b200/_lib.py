@@ -213,11 +213,11 @@ def stream_handle(device) -> int:
 
 def device_of(what: str, *tensors) -> int:
     """The one CUDA device of all tensors, by index."""
-    device = tensors[0].get_device()
-    for t in tensors:
-        if t.get_device() != device or device < 0:
-            lib()  # without CUDA: the library's own error
-            raise ValueError(f"{what}: expected CUDA tensors on one device, got {[str(t.device) for t in tensors]}")
+    devices = set(map(torch.Tensor.get_device, tensors))
+    device = devices.pop()
+    if devices or device < 0:
+        lib()  # without CUDA: the library's own error
+        raise ValueError(f"{what}: expected CUDA tensors on one device, got {[str(t.device) for t in tensors]}")
     return device
 
 

@@ -6,9 +6,12 @@
 // block, the second adds those in order in every block, so nothing waits on an
 // atomic and the result does not depend on the launch.  Bound by HBM: g is read
 // twice and written once.  The second launch goes through the chunks backwards, so
-// that it finds in L2 what the first read last.  Up to a million elements the time
-// is launches: one cluster of blocks does both steps in one, with its hardware
-// barrier between them.
+// that it finds in L2 what the first read last.  Up to half a million elements the
+// time is launches: one cluster of blocks does both steps in one, with its hardware
+// barrier between them.  Above 8 million the second launch has a block a chunk: blocks
+// that start in the order of memory keep HBM's pages open, where resident blocks that
+// stride through it drift apart (1.6 GB copied and scaled: 464 us against 541).  The
+// norm is then a launch of its own, so that a block begins with its loads.
 //
 // Squares are added in fp32 over at most 32 values and in fp64 from there on.  A
 // group whose fp32 sum is so small or so large that squares were lost or overflowed
@@ -26,10 +29,11 @@
 namespace hb {
 namespace clip {
 
-constexpr int kThreads = 256;
-constexpr int64_t kChunk = 8192, kSmallChunk = 2048;  // elements
-constexpr int64_t kSmallMost = 1 << 20;               // elements of the one-launch form
+constexpr int kThreads = 256, kSmallThreads = 1024;
+constexpr int64_t kChunk = 8192, kSmallChunk = 16384;  // elements; 4 loads a thread of fp32
+constexpr int64_t kSmallMost = 1 << 19;               // elements of the one-launch form
 constexpr int kCluster = 16;
+constexpr int64_t kLargeLeast = 1 << 23;              // elements from which a block scales one chunk
 constexpr int kMostBlocks = 148 * 8;
 constexpr double kEps = 1e-6;
 
@@ -56,8 +60,9 @@ __device__ __forceinline__ int tensor_of(const List<MOST>& l, int chunk) {
     return lo;
 }
 
+template <int THREADS>
 __device__ __forceinline__ double block_sum(double v) {
-    __shared__ double part[kThreads / 32];
+    __shared__ double part[THREADS / 32];
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
     __syncthreads();
@@ -65,7 +70,7 @@ __device__ __forceinline__ double block_sum(double v) {
     __syncthreads();
     double r = 0.0;
 #pragma unroll
-    for (int i = 0; i < kThreads / 32; ++i) r += part[i];
+    for (int i = 0; i < THREADS / 32; ++i) r += part[i];
     return r;
 }
 
@@ -82,7 +87,7 @@ __device__ __forceinline__ double squares(const float (&f)[N]) {
     return d;
 }
 
-template <typename T>
+template <int THREADS, typename T>
 __device__ __forceinline__ double chunk_squares(const T* p, int n) {
     using V = rows::Vec<T, 16>;
     constexpr int U = 4;
@@ -90,12 +95,12 @@ __device__ __forceinline__ double chunk_squares(const T* p, int n) {
     int done = 0;
     if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
         const int whole = n / V::N;
-        for (int i = threadIdx.x; i < whole; i += kThreads * U) {
+        for (int i = threadIdx.x; i < whole; i += THREADS * U) {
             V v[U];
             float f[U * V::N];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (i + u * kThreads < whole) v[u].load(p + (int64_t)(i + u * kThreads) * V::N);
+                if (i + u * THREADS < whole) v[u].load(p + (int64_t)(i + u * THREADS) * V::N);
                 else v[u].zero();
             }
 #pragma unroll
@@ -106,7 +111,7 @@ __device__ __forceinline__ double chunk_squares(const T* p, int n) {
         }
         done = whole * V::N;
     }
-    for (int i = done + threadIdx.x; i < n; i += kThreads) {
+    for (int i = done + threadIdx.x; i < n; i += THREADS) {
         const float f[1] = {rows::to_float(p[i])};
         sum += squares(f);
     }
@@ -114,39 +119,47 @@ __device__ __forceinline__ double chunk_squares(const T* p, int n) {
 }
 
 // This block's sum of squares.
-template <int MOST>
+template <int THREADS, int MOST>
 __device__ __forceinline__ double list_squares(const List<MOST>& l) {
     double sum = 0.0;
     for (int chunk = blockIdx.x; chunk < l.first[l.count]; chunk += gridDim.x) {
         const int t = tensor_of(l, chunk);
         const int64_t at = (int64_t)(chunk - l.first[t]) * l.chunk;
         const int n = (int)min((int64_t)l.chunk, l.size[t] - at);
-        if (l.type[t] == HB_F32) sum += chunk_squares(static_cast<const float*>(l.in[t]) + at, n);
-        else if (l.type[t] == HB_F16) sum += chunk_squares(static_cast<const __half*>(l.in[t]) + at, n);
-        else sum += chunk_squares(static_cast<const __nv_bfloat16*>(l.in[t]) + at, n);
+        if (l.type[t] == HB_F32) sum += chunk_squares<THREADS>(static_cast<const float*>(l.in[t]) + at, n);
+        else if (l.type[t] == HB_F16) sum += chunk_squares<THREADS>(static_cast<const __half*>(l.in[t]) + at, n);
+        else sum += chunk_squares<THREADS>(static_cast<const __nv_bfloat16*>(l.in[t]) + at, n);
     }
-    return block_sum(sum);
+    return block_sum<THREADS>(sum);
 }
 
 template <int MOST>
 __global__ void __launch_bounds__(kThreads) square_kernel(const __grid_constant__ List<MOST> l, double* __restrict__ partial) {
-    const double sum = list_squares(l);
+    const double sum = list_squares<kThreads>(l);
     if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
 
 __device__ __forceinline__ double total_norm(const double* partial, int partials) {
     double s = 0.0;
     for (int i = threadIdx.x; i < partials; i += kThreads) s += partial[i];
-    return sqrt(block_sum(s));
+    return sqrt(block_sum<kThreads>(s));
 }
 
-__global__ void __launch_bounds__(kThreads) norm_kernel(const double* __restrict__ partial, int partials,
-                                                        float* __restrict__ norm) {
+__device__ __forceinline__ float factor_of(double norm, double limit) {
+    const double r = limit / (norm + kEps);
+    return r >= 1.0 ? 1.0f : (float)r;  // a NaN stays
+}
+
+__global__ void __launch_bounds__(kThreads) norm_kernel(const double* __restrict__ partial, int partials, double limit,
+                                                        float* __restrict__ norm, float* __restrict__ factor) {
     const double n = total_norm(partial, partials);
-    if (threadIdx.x == 0) *norm = (float)n;
+    if (threadIdx.x == 0) {
+        *norm = (float)n;
+        *factor = factor_of(n, limit);
+    }
 }
 
-template <typename T, typename TO>
+template <int THREADS, typename T, typename TO>
 __device__ __forceinline__ void scale_chunk(const T* p, TO* out, int n, float f) {
     constexpr int N = 16 / (int)sizeof(T), kPieces = N * (int)sizeof(TO) / 16;
     using V = rows::Vec<T, 16>;
@@ -155,55 +168,54 @@ __device__ __forceinline__ void scale_chunk(const T* p, TO* out, int n, float f)
     int done = 0;
     if (((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(out)) & 15) == 0) {
         const int whole = n / N;
-        for (int i = threadIdx.x; i < whole; i += kThreads * U) {
+        for (int i = threadIdx.x; i < whole; i += THREADS * U) {
             V v[U];
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (i + u * kThreads < whole) v[u].raw = *reinterpret_cast<const uint4*>(p + (int64_t)(i + u * kThreads) * N);
+                if (i + u * THREADS < whole) v[u].raw = *reinterpret_cast<const uint4*>(p + (int64_t)(i + u * THREADS) * N);
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (i + u * kThreads < whole) {
+                if (i + u * THREADS < whole) {
 #pragma unroll
                     for (int q = 0; q < kPieces; ++q) {
                         O o;
 #pragma unroll
                         for (int j = 0; j < O::N; ++j)
                             o.v[j] = rows::from_float<TO>(f * rows::to_float(v[u].v[q * O::N + j]));
-                        o.store(out + (int64_t)(i + u * kThreads) * N + q * O::N);
+                        o.store(out + (int64_t)(i + u * THREADS) * N + q * O::N);
                     }
                 }
         }
         done = whole * N;
     }
-    for (int i = done + threadIdx.x; i < n; i += kThreads) out[i] = rows::from_float<TO>(f * rows::to_float(p[i]));
+    for (int i = done + threadIdx.x; i < n; i += THREADS) out[i] = rows::from_float<TO>(f * rows::to_float(p[i]));
 }
 
-__device__ __forceinline__ float factor_of(double norm, double limit) {
-    const double r = limit / (norm + kEps);
-    return r >= 1.0 ? 1.0f : (float)r;  // a NaN stays
-}
-
-template <int MOST>
-__device__ __forceinline__ void scale_list(const List<MOST>& l, float f) {
-    for (int c = blockIdx.x; c < l.first[l.count]; c += gridDim.x) {
-        const int chunk = l.first[l.count] - 1 - c;
-        const int t = tensor_of(l, chunk);
-        if (f == 1.0f && l.in[t] == l.out[t]) continue;
-        const int64_t at = (int64_t)(chunk - l.first[t]) * l.chunk;
-        const int m = (int)min((int64_t)l.chunk, l.size[t] - at);
-        const int type = l.type[t], to = l.out_type[t];
-        if (type == HB_F32) {
-            scale_chunk(static_cast<const float*>(l.in[t]) + at, static_cast<float*>(l.out[t]) + at, m, f);
-        } else if (type == HB_F16) {
-            const __half* p = static_cast<const __half*>(l.in[t]) + at;
-            if (to == HB_F32) scale_chunk(p, static_cast<float*>(l.out[t]) + at, m, f);
-            else scale_chunk(p, static_cast<__half*>(l.out[t]) + at, m, f);
-        } else {
-            const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(l.in[t]) + at;
-            if (to == HB_F32) scale_chunk(p, static_cast<float*>(l.out[t]) + at, m, f);
-            else scale_chunk(p, static_cast<__nv_bfloat16*>(l.out[t]) + at, m, f);
-        }
+// Chunk c from the end.
+template <int THREADS, int MOST>
+__device__ __forceinline__ void scale_one(const List<MOST>& l, int c, float f) {
+    const int chunk = l.first[l.count] - 1 - c;
+    const int t = tensor_of(l, chunk);
+    if (f == 1.0f && l.in[t] == l.out[t]) return;
+    const int64_t at = (int64_t)(chunk - l.first[t]) * l.chunk;
+    const int m = (int)min((int64_t)l.chunk, l.size[t] - at);
+    const int type = l.type[t], to = l.out_type[t];
+    if (type == HB_F32) {
+        scale_chunk<THREADS>(static_cast<const float*>(l.in[t]) + at, static_cast<float*>(l.out[t]) + at, m, f);
+    } else if (type == HB_F16) {
+        const __half* p = static_cast<const __half*>(l.in[t]) + at;
+        if (to == HB_F32) scale_chunk<THREADS>(p, static_cast<float*>(l.out[t]) + at, m, f);
+        else scale_chunk<THREADS>(p, static_cast<__half*>(l.out[t]) + at, m, f);
+    } else {
+        const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(l.in[t]) + at;
+        if (to == HB_F32) scale_chunk<THREADS>(p, static_cast<float*>(l.out[t]) + at, m, f);
+        else scale_chunk<THREADS>(p, static_cast<__nv_bfloat16*>(l.out[t]) + at, m, f);
     }
+}
+
+template <int THREADS, int MOST>
+__device__ __forceinline__ void scale_list(const List<MOST>& l, float f) {
+    for (int c = blockIdx.x; c < l.first[l.count]; c += gridDim.x) scale_one<THREADS>(l, c, f);
 }
 
 template <int MOST>
@@ -212,24 +224,38 @@ __global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__
                                                          float* __restrict__ norm) {
     const double n = total_norm(partial, partials);
     if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
-    scale_list(l, factor_of(n, limit));
+    scale_list<kThreads>(l, factor_of(n, limit));
+}
+
+// A block a chunk; the factor is norm_kernel's.
+template <int MOST>
+__global__ void __launch_bounds__(kThreads) scale_large_kernel(const __grid_constant__ List<MOST> l,
+                                                               const float* __restrict__ factor) {
+    scale_one<kThreads>(l, blockIdx.x, *factor);
 }
 
 // Both steps in one cluster.  A block takes the same chunks in both, and no other block's.
-__global__ void __launch_bounds__(kThreads) clip_small_kernel(const __grid_constant__ List<kFew> l, int scale, double limit,
+__global__ void __launch_bounds__(kSmallThreads) clip_small_kernel(const __grid_constant__ List<kFew> l, int scale, double limit,
                                                               float* __restrict__ norm) {
     namespace cg = cooperative_groups;
-    __shared__ double mine;
+    __shared__ double mine, all;
     cg::cluster_group cluster = cg::this_cluster();
-    const double sum = list_squares(l);
+    const double sum = list_squares<kSmallThreads>(l);
     if (threadIdx.x == 0) mine = sum;
     cluster.sync();
-    double s = 0.0;
-    for (int b = 0; b < (int)cluster.num_blocks(); ++b) s += *cluster.map_shared_rank(&mine, b);
-    const double n = sqrt(s);
+    if (threadIdx.x < 32) {
+        double s = threadIdx.x < kCluster ? *cluster.map_shared_rank(&mine, threadIdx.x) : 0.0;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+        if (threadIdx.x == 0) all = s;
+    }
+    __syncthreads();
+    // a block stays until the others have read its sum; nothing else is handed over
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    const double n = sqrt(all);
     if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
-    if (scale) scale_list(l, factor_of(n, limit));
-    cluster.sync();  // a block stays until the others have read its sum
+    if (scale) scale_list<kSmallThreads>(l, factor_of(n, limit));
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
 
 // The tensors from..to of the caller's list that hold elements.
@@ -258,7 +284,8 @@ inline int blocks_of(int chunks) { return std::max(1, std::min(chunks, kMostBloc
 
 template <int MOST>
 cudaError_t run(int64_t count, const void* const* in, const int64_t* size, const int32_t* type, void* const* out,
-                const int32_t* out_type, double limit, float* norm, double* partial, cudaStream_t st) {
+                const int32_t* out_type, double limit, bool large, float* norm, float* factor, double* partial,
+                cudaStream_t st) {
     List<MOST> l;
     int partials = 0;
     for (int64_t from = 0; from < count || from == 0; from += MOST) {
@@ -267,14 +294,17 @@ cudaError_t run(int64_t count, const void* const* in, const int64_t* size, const
         count_launches(1);
         partials += blocks;
     }
-    if (!out) {
-        norm_kernel<<<1, kThreads, 0, st>>>(partial, partials, norm);
+    if (!out || large) {
+        norm_kernel<<<1, kThreads, 0, st>>>(partial, partials, limit, norm, factor);
         count_launches(1);
-        return cudaGetLastError();
+        if (!out) return cudaGetLastError();
     }
     for (int64_t from = 0; from < count || from == 0; from += MOST) {
         if (count > MOST) fill(l, kChunk, from, std::min(count, from + MOST), in, size, type, out, out_type);
-        scale_kernel<MOST><<<blocks_of(l.first[l.count]), kThreads, 0, st>>>(l, partial, partials, limit, norm);
+        const int chunks = l.first[l.count];
+        if (chunks == 0 && large) continue;
+        if (large) scale_large_kernel<MOST><<<chunks, kThreads, 0, st>>>(l, factor);
+        else scale_kernel<MOST><<<blocks_of(chunks), kThreads, 0, st>>>(l, partial, partials, limit, norm);
         count_launches(1);
     }
     return cudaGetLastError();
@@ -301,7 +331,7 @@ int check(int64_t count, const void* const* in, const int64_t* size, const int32
 int start(int64_t count, const void* const* in, const int64_t* size, const int32_t* type, void* const* out,
           const int32_t* out_type, double limit, float* norm, void* ws, void* stream) {
     const auto st = static_cast<cudaStream_t>(stream);
-    double* partial = static_cast<double*>(ws);
+    double* partial = static_cast<double*>(ws) + 1;  // after the factor
     int64_t total = 0;
     for (int64_t i = 0; i < count; ++i) total += size[i];
     cudaError_t e = cudaSuccess;
@@ -315,7 +345,7 @@ int start(int64_t count, const void* const* in, const int64_t* size, const int32
         attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
         cudaLaunchConfig_t config{};
         config.gridDim = dim3(kCluster);
-        config.blockDim = dim3(kThreads);
+        config.blockDim = dim3(kSmallThreads);
         config.stream = st;
         config.attrs = &attr;
         config.numAttrs = 1;
@@ -323,8 +353,9 @@ int start(int64_t count, const void* const* in, const int64_t* size, const int32
         count_launches(1);
         return e == cudaSuccess ? HB_OK : abi_fail(HB_LAUNCH, std::string("gradient norm: ") + cudaGetErrorString(e));
     }
-    e = count <= kFew ? run<kFew>(count, in, size, type, out, out_type, limit, norm, partial, st)
-                      : run<kMany>(count, in, size, type, out, out_type, limit, norm, partial, st);
+    const auto go = count <= kFew ? run<kFew> : run<kMany>;
+    float* factor = static_cast<float*>(ws);
+    e = go(count, in, size, type, out, out_type, limit, total >= kLargeLeast, norm, factor, partial, st);
     return e == cudaSuccess ? HB_OK : abi_fail(HB_LAUNCH, std::string("gradient norm: ") + cudaGetErrorString(e));
 }
 
@@ -336,7 +367,7 @@ using namespace hb::clip;
 
 extern "C" size_t hb_clip_workspace(int64_t count) {
     if (count < 0) return 0;
-    return sizeof(double) * kMostBlocks * (size_t)std::max<int64_t>(1, (count + kMany - 1) / kMany);
+    return sizeof(double) * (1 + kMostBlocks * (size_t)std::max<int64_t>(1, (count + kMany - 1) / kMany));
 }
 
 extern "C" int hb_grad_norm(int64_t count, const void* const* grads, const int64_t* sizes, const int32_t* types,

@@ -8,7 +8,11 @@
 //
 // Such a sort moves little (a megabyte at 131072 entries), so its time is launches,
 // barriers and the single sector a cycle at which an SM scatters 4-byte stores.
-//   up to 32768 entries  one launch of one cluster of up to 16 blocks: the entries
+//   up to 2048 entries   one launch of independent blocks: each ranks its 64 entries
+//                        against all keys by comparing, n^2 comparisons in all, which
+//                        at this size are cheaper than any barrier, and as many
+//                        offsets; no passes, whatever the number of bins
+//   up to 32768          one launch of one cluster of up to 16 blocks: the entries
 //                        stay in the blocks' shared memory over all passes, the
 //                        blocks read each other's counts and write each other's
 //                        entries there, and the hardware's cluster barrier stands
@@ -32,6 +36,9 @@ namespace isort {
 constexpr int kThreads = 1024, kWarps = kThreads / 32;     // a tile's block
 constexpr int kBlock = 1024, kBlockWarps = kBlock / 32;     // a cluster's block
 constexpr int kRounds = 2;                                  // entries a thread of a cluster
+constexpr int kRankMost = 2048, kRankThreads = 256;         // sort by comparing
+constexpr int kRankSlices = 4, kRankQueries = kRankThreads / kRankSlices;
+constexpr int64_t kRankBins = 4096;                         // most bins whose offsets it finds
 constexpr int kMostClusters = 16;
 constexpr int64_t kClusterMost = (int64_t)kMostClusters * kBlock * kRounds;
 constexpr int kMaxDigitBits = 11;
@@ -48,6 +55,55 @@ struct Source {
         return v >= 0 && v < (int64_t)bins ? (uint32_t)v : bins;
     }
 };
+
+// Places of the entries, and the offsets, each a count of the keys below: of key k at entry i the keys <= k before
+// i and those < k after it, of offset b the keys < b.  64 queries a block, 4 threads a query, each over a quarter of
+// the keys in shared memory, where a warp reads the same 16 bytes in all its lanes.
+__global__ void __launch_bounds__(kRankThreads) sort_rank(Source src, int n, int entry_blocks, int32_t* __restrict__ order,
+                                                          int32_t* __restrict__ position, uint32_t* __restrict__ keys_out,
+                                                          int32_t* __restrict__ offsets, int bins,
+                                                          uint32_t* __restrict__ zero, int64_t zeros) {
+    __shared__ __align__(16) uint32_t keys[kRankMost];
+    __shared__ uint32_t parts[kRankSlices][kRankQueries];
+    for (int64_t i = (int64_t)blockIdx.x * kRankThreads + threadIdx.x; i < zeros; i += (int64_t)gridDim.x * kRankThreads)
+        zero[i] = 0;
+    const int slice_keys = (n + kRankSlices * 4 - 1) / (kRankSlices * 4) * 4;  // whole vectors
+    for (int i = threadIdx.x; i < slice_keys * kRankSlices; i += kRankThreads) keys[i] = i < n ? src.key(i) : 0xffffffffu;
+    __syncthreads();
+    const int query = threadIdx.x % kRankQueries, slice = threadIdx.x / kRankQueries;
+    const bool entries = (int)blockIdx.x < entry_blocks;
+    const int first = entries ? blockIdx.x * kRankQueries : 0;  // of the block's entries
+    const int i = first + query, b = ((int)blockIdx.x - entry_blocks) * kRankQueries + query;
+    const uint32_t key = entries ? (i < n ? keys[i] : 0) : (uint32_t)b;
+    uint32_t count = 0;
+    auto below = [&](int from, int to, uint32_t limit) {  // whole vectors
+#pragma unroll 4
+        for (int j = from; j < to; j += 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(keys + j);
+            count += (v.x < limit) + (v.y < limit) + (v.z < limit) + (v.w < limit);
+        }
+    };
+    const int lo = slice * slice_keys, hi = lo + slice_keys;
+    if (entries) {
+        below(lo, min(hi, first), key + 1);
+        for (int j = max(lo, first); j < min(hi, first + kRankQueries); ++j) count += keys[j] < key + (j < i);
+        below(max(lo, first + kRankQueries), hi, key);
+    } else {
+        below(lo, hi, key);
+    }
+    parts[slice][query] = count;
+    __syncthreads();
+    if (slice != 0) return;
+#pragma unroll
+    for (int s = 1; s < kRankSlices; ++s) count += parts[s][query];
+    if (!entries) {
+        if (b <= bins) offsets[b] = (int32_t)count;
+    } else if (i < n) {
+        if (order) order[count] = i;
+        if (position) position[i] = (int32_t)count;
+        if (keys_out) keys_out[count] = key;
+    }
+}
 
 // Rank of every lane's digit among the equal digits its warp has seen, in order.  The lanes with an
 // equal digit come from a ballot a bit of it.
@@ -339,13 +395,15 @@ __global__ void __launch_bounds__(256) find_offsets(const uint32_t* __restrict__
 struct Plan {
     int passes, digit_bits, digits, rounds, tiles;
     int cluster;  // blocks of the one-launch sort, 0: tiles
+    bool rank;    // by comparing
 };
 
 // One pass over bins + 1 digits when they fit, else equal digits of at most 11 bits.
-// A cluster has a block for every 1024 entries up to 16 (one for up to 2048); tiles have 2048, 4096 or 8192
+// A cluster has a block for every 1024 entries up to 16; tiles have 2048, 4096 or 8192
 // entries, the least that makes at most 64 tiles, so that a block adds up their counts in a few loads a thread.
 inline Plan plan_of(int64_t n, int64_t bins) {
     Plan p{};
+    p.rank = n <= kRankMost;
     int bits = 1;
     while (bits < 32 && (bins >> bits) != 0) ++bits;
     p.passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
@@ -353,8 +411,7 @@ inline Plan plan_of(int64_t n, int64_t bins) {
     p.digits = p.passes == 1 ? (int)(bins + 1) : 1 << p.digit_bits;
     if (n <= kClusterMost) {
         p.cluster = 1;
-        if (n > kBlock * kRounds)
-            while (p.cluster < kMostClusters && (int64_t)p.cluster * kBlock < n) p.cluster <<= 1;
+        while (p.cluster < kMostClusters && (int64_t)p.cluster * kBlock < n) p.cluster <<= 1;
         p.rounds = (int)((n + p.cluster * kBlock - 1) / (p.cluster * kBlock));
         return p;
     }
@@ -366,14 +423,14 @@ inline Plan plan_of(int64_t n, int64_t bins) {
 }
 inline bool scanned(const Plan& p) { return p.tiles > kMostTiles; }
 
-// Counts (of a pass, or of each) and totals, the keys and entries between passes, and the last
-// pass's keys (searched for the offsets when the caller takes no keys).
+// Counts (of a pass, or of each) and totals, the keys and entries between passes, and the sorted keys
+// (searched for the offsets when the caller takes no keys).
 struct Layout {
     uint32_t *counts, *totals, *keys[2], *sorted;
     int32_t* vals[2];
     size_t bytes;
 };
-inline Layout layout(void* ws, int64_t n, const Plan& p) {
+inline Layout layout(void* ws, int64_t n, int64_t bins, const Plan& p) {
     Layout l{};
     char* base = static_cast<char*>(ws);
     auto take = [&](size_t bytes) {
@@ -390,7 +447,7 @@ inline Layout layout(void* ws, int64_t n, const Plan& p) {
             l.vals[i] = reinterpret_cast<int32_t*>(take(sizeof(int32_t) * n));
         }
     }
-    if (p.passes > 1) l.sorted = reinterpret_cast<uint32_t*>(take(sizeof(uint32_t) * n));
+    if (p.rank ? bins > kRankBins : p.passes > 1) l.sorted = reinterpret_cast<uint32_t*>(take(sizeof(uint32_t) * n));
     return l;
 }
 
@@ -469,7 +526,7 @@ cudaError_t sort_tiles(const Source& input, int64_t n, const Plan& p, const Layo
 
 size_t index_sort_bytes(int64_t n, int64_t bins) {
     if (n <= 0) return 0;
-    return isort::layout(nullptr, n, isort::plan_of(n, bins)).bytes;
+    return isort::layout(nullptr, n, bins, isort::plan_of(n, bins)).bytes;
 }
 
 int index_sort(const void* index, int index_bytes, int64_t n, int64_t bins, int32_t* order, int32_t* position,
@@ -482,14 +539,22 @@ int index_sort(const void* index, int index_bytes, int64_t n, int64_t bins, int3
         return e == cudaSuccess ? HB_OK : abi_fail(HB_CUDA, std::string("index sort: ") + cudaGetErrorString(e));
     }
     const Plan p = plan_of(n, bins);
-    const Layout l = layout(ws, n, p);
+    const Layout l = layout(ws, n, bins, p);
     if ((uintptr_t)ws % 256 || (uintptr_t)index % index_bytes)
         return abi_fail(HB_BAD_ARGUMENT, "index sort: misaligned index, or a workspace that is not 256-byte aligned");
     if (l.bytes > ws_bytes || (l.bytes > 0 && !ws))
         return abi_fail(HB_WORKSPACE, "workspace too small for the index sort");
     const Source src{index, index_bytes, (uint32_t)bins};
-    if (!keys && p.passes > 1 && offsets) keys = l.sorted;
-    if (p.cluster) {
+    const bool search = offsets && (p.rank ? bins > kRankBins : p.passes > 1);  // offsets by searching the sorted keys
+    if (!keys && search) keys = l.sorted;
+    if (p.rank) {
+        const int blocks = (int)((n + kRankQueries - 1) / kRankQueries);
+        const int more = offsets && !search ? (int)(bins / kRankQueries + 1) : 0;
+        sort_rank<<<blocks + more, kRankThreads, 0, st>>>(src, (int)n, blocks, order, position, keys, offsets,
+                                                          (int)bins, zero, zeros);
+        count_launches(1);
+        e = cudaGetLastError();
+    } else if (p.cluster) {
         e = sort_one_launch(src, (int)n, p, order, position, keys, offsets, zero, zeros, st);
     } else {
         auto sort = scanned(p) ? sort_tiles<8, true>
@@ -498,7 +563,7 @@ int index_sort(const void* index, int index_bytes, int64_t n, int64_t bins, int3
                                     : sort_tiles<2, false>;
         e = sort(src, n, p, l, order, position, keys, offsets, zero, zeros, st);
     }
-    if (e == cudaSuccess && offsets && p.passes > 1) {
+    if (e == cudaSuccess && search) {
         find_offsets<<<(unsigned)((bins + 256) / 256), 256, 0, st>>>(keys, n, bins, offsets);
         count_launches(1);
         e = cudaGetLastError();

@@ -29,13 +29,13 @@ def _addresses(tensors, what: str):
         types = array("i", [FLOAT_TYPES[t.dtype] for t in tensors])
     except KeyError as e:
         raise ValueError(f"{what}: gradients are float32, float16 or bfloat16, got {e.args[0]}") from None
-    contiguous = all(t.is_contiguous() for t in tensors)
+    contiguous = all(map(torch.Tensor.is_contiguous, tensors))
     if not contiguous:
         for t in tensors:
             if not t.is_contiguous() and not _dense(t):
                 raise ValueError(f"{what}: gradients must be dense in memory, got strides {t.stride()} for "
                                  f"{tuple(t.shape)}")
-    addresses = [t.data_ptr() for t in tensors]
+    addresses = list(map(torch.Tensor.data_ptr, tensors))
     if len(set(addresses)) != len(addresses):  # tensors without elements may share an address
         full = [t.data_ptr() for t in tensors if t.numel()]
         if len(set(full)) != len(full):
@@ -53,7 +53,7 @@ def _run(grads, limit, out, what):
         raise ValueError(f"{what}: no gradients")
     device = device_of(what, *grads)
     pointers, types, contiguous = _addresses(grads, what)
-    sizes = array("q", [g.numel() for g in grads])
+    sizes = array("q", map(torch.Tensor.numel, grads))
     L = load_library()
     norm = grads[0].new_empty((), dtype=torch.float32)
     nbytes = L.hb_clip_workspace(len(grads))
@@ -68,7 +68,7 @@ def _run(grads, limit, out, what):
     to_pointers, to_types = pointers, types
     if out is not None:
         out = _tensors(out)
-        if [g.shape for g in grads] != [o.shape for o in out]:
+        if len(out) != len(grads) or not all(map(torch.Tensor.is_same_size, grads, out)):
             raise ValueError(f"{what}: outputs have their gradients' shapes")
         if device_of(what, *out) != device:
             raise ValueError(f"{what}: outputs on another device than their gradients")
