@@ -105,8 +105,7 @@ struct Grad {
     const T* dy;
     int64_t dy_stride, n, rows, width;
     float scale;
-    const int32_t* order;    // token of each sorted place
-    const uint32_t* keys;    // row of each sorted place; `rows` for an id outside the table
+    const uint2* pairs;      // (row, token) of each sorted place; row `rows` for an id outside the table
     int chunk;               // places a group
     int64_t chunks;
     int tiles;               // column tiles
@@ -138,17 +137,17 @@ __device__ __forceinline__ void write_row(const Grad<T, TO>& g, uint32_t key, in
 template <typename G>
 __device__ __forceinline__ int64_t last_chunk(const G& g, uint32_t key, int64_t c) {
     int64_t e = c + 1, step = 1;
-    while (e + step < g.chunks && g.keys[(e + step) * g.chunk] == key) e += step, step <<= 1;
+    while (e + step < g.chunks && g.pairs[(e + step) * g.chunk].x == key) e += step, step <<= 1;
     for (; step; step >>= 1)
-        if (e + step < g.chunks && g.keys[(e + step) * g.chunk] == key) e += step;
+        if (e + step < g.chunks && g.pairs[(e + step) * g.chunk].x == key) e += step;
     return e;
 }
 template <typename G>
 __device__ __forceinline__ int64_t first_chunk(const G& g, uint32_t key, int64_t c) {
     int64_t s = c - 1, step = 1;
-    while (s - step >= 0 && g.keys[(s - step + 1) * g.chunk - 1] == key) s -= step, step <<= 1;
+    while (s - step >= 0 && g.pairs[(s - step + 1) * g.chunk - 1].x == key) s -= step, step <<= 1;
     for (; step; step >>= 1)
-        if (s - step >= 0 && g.keys[(s - step + 1) * g.chunk - 1] == key) s -= step;
+        if (s - step >= 0 && g.pairs[(s - step + 1) * g.chunk - 1].x == key) s -= step;
     return s;
 }
 
@@ -233,11 +232,14 @@ __device__ __forceinline__ void add_vector(float (&sum)[Vec<T, VB>::N], const Ve
     if (N % 2) sum[N - 1] += rows::to_float(v.v[N - 1]);
 }
 
-// 8 consecutive words of an array that is padded to whole 32-byte groups.
-__device__ __forceinline__ void load8(const void* array, int64_t at, uint32_t (&w)[8]) {
-    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint32_t*>(array) + at);
-    const uint4 a = __ldg(p), b = __ldg(p + 1);
-    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+// The rows and tokens of 8 consecutive places; the array is padded to whole groups of 8.
+__device__ __forceinline__ void load8(const uint2* pairs, uint32_t (&row)[8], uint32_t (&token)[8]) {
+    const uint4* p = reinterpret_cast<const uint4*>(pairs);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint4 v = __ldg(p + i);
+        row[2 * i] = v.x, token[2 * i] = v.y, row[2 * i + 1] = v.z, token[2 * i + 1] = v.w;
+    }
 }
 
 // Sums a chunk.  Each thread has its own ring of 8 vectors in shared memory, one a sorted place, filled ahead by
@@ -258,7 +260,7 @@ __device__ __forceinline__ void sum_chunk(const Grad<T, TO>& g, int64_t block) {
     const uint32_t none = (uint32_t)g.rows;
     const int64_t p0 = chunk * g.chunk;
     const int count = (int)min((int64_t)g.chunk, g.n - p0);
-    const uint32_t first_key = g.keys[p0];
+    const uint32_t first_key = g.pairs[p0].x;
     if (first_key >= none) return;
     typename V::Raw* slots = ring + threadIdx.y * blockDim.x + threadIdx.x;
     const int step = blockDim.x * blockDim.y;
@@ -278,11 +280,10 @@ __device__ __forceinline__ void sum_chunk(const Grad<T, TO>& g, int64_t block) {
         }
     };
     uint32_t keys[D], tokens[D], after[D];
-    load8(g.order, p0, tokens);
+    load8(g.pairs + p0, after, tokens);
 #pragma unroll
     for (int j = 0; j < D; ++j) fetch(j, tokens[j], mine && j < count);
-    load8(g.keys, p0, after);
-    const bool continues = p0 > 0 && g.keys[p0 - 1] == first_key;
+    const bool continues = p0 > 0 && g.pairs[p0 - 1].x == first_key;
     uint32_t key = first_key;
     bool head = continues;
     float sum[N];
@@ -305,10 +306,7 @@ __device__ __forceinline__ void sum_chunk(const Grad<T, TO>& g, int64_t block) {
         }
 #pragma unroll
         for (int j = 0; j < D; ++j) keys[j] = i + j < count ? after[j] : none;
-        if (more) {
-            load8(g.order, p0 + i + D, tokens);
-            load8(g.keys, p0 + i + D, after);
-        }
+        if (more) load8(g.pairs + p0 + i + D, after, tokens);
 #pragma unroll
         for (int j = 0; j < D; ++j) {
             if (keys[j] != key) {
@@ -333,7 +331,7 @@ __device__ __forceinline__ void sum_chunk(const Grad<T, TO>& g, int64_t block) {
     }
     if constexpr (VB >= 4) asm volatile("cp.async.wait_all;" ::: "memory");
     const int64_t p1 = p0 + count;
-    const bool open = key < none && p1 < g.n && g.keys[p1] == key;
+    const bool open = key < none && p1 < g.n && g.pairs[p1].x == key;
     if (key < none) {
         if (!head && open) {
             if (mine) Values<float, N>::store(g.partial + (chunk * 2 + 1) * g.width + c, sum);
@@ -363,10 +361,10 @@ __device__ __forceinline__ void zero_rows(const Grad<T, TO>& g, int64_t block) {
         int64_t lo = 0, hi = g.n;
         while (lo < hi) {
             const int64_t mid = (lo + hi) >> 1;
-            if (g.keys[mid] < (uint32_t)row) lo = mid + 1;
+            if (g.pairs[mid].x < (uint32_t)row) lo = mid + 1;
             else hi = mid;
         }
-        empty = lo >= g.n || g.keys[lo] != (uint32_t)row;
+        empty = lo >= g.n || g.pairs[lo].x != (uint32_t)row;
     }
     for (unsigned left = __ballot_sync(0xffffffffu, empty); left; left &= left - 1) {
         TO* to = g.out + (first + __ffs(left) - 1) * g.width;
@@ -381,7 +379,8 @@ __device__ __forceinline__ void zero_rows(const Grad<T, TO>& g, int64_t block) {
 }
 
 template <typename T, typename TO, int VB>
-__global__ void __launch_bounds__(256) grad_kernel(const Grad<T, TO> g) {
+__global__ void __launch_bounds__(256, 3) grad_kernel(const Grad<T, TO> g) {
+    after_last();
     if ((int64_t)blockIdx.x < g.sum_blocks) sum_chunk<T, TO, VB>(g, blockIdx.x);
     else zero_rows(g, blockIdx.x - g.sum_blocks);
 }
@@ -413,8 +412,7 @@ inline int chunk_of(int64_t n, const Shape& s) {
 }
 
 struct Layout {
-    uint32_t* keys;
-    int32_t* order;
+    uint2* pairs;
     float* partial;
     uint32_t* arrived;
     int64_t arrivals;
@@ -432,8 +430,7 @@ inline Layout layout(void* ws, int64_t n, int64_t rows_, int64_t width) {
         l.bytes += (bytes + 255) / 256 * 256;
         return r;
     };
-    l.keys = reinterpret_cast<uint32_t*>(take(sizeof(uint32_t) * n));
-    l.order = reinterpret_cast<int32_t*>(take(sizeof(int32_t) * n));
+    l.pairs = reinterpret_cast<uint2*>(take(sizeof(uint2) * n));
     l.sort_bytes = index_sort_bytes(n, rows_);
     l.sort = take(l.sort_bytes);
     const int chunk = chunk_of(n, shape_of((width + 7) / 8));
@@ -459,9 +456,8 @@ cudaError_t run_grad(Grad<T, TO> g, cudaStream_t st) {
         const int warps = s.group * s.groups / 32;
         zero_blocks = (g.rows + (int64_t)g.rows_per_warp * warps - 1) / ((int64_t)g.rows_per_warp * warps);
     }
-    grad_kernel<T, TO, VB><<<(unsigned)(g.sum_blocks + zero_blocks), block, 0, st>>>(g);
     count_launches(1);
-    return cudaGetLastError();
+    return launch_next(grad_kernel<T, TO, VB>, dim3((unsigned)(g.sum_blocks + zero_blocks)), block, 0, st, g);
 }
 
 }  // namespace embedding
@@ -532,7 +528,7 @@ extern "C" int hb_embedding_grad(int type, const void* dy, int64_t dy_stride, co
     const Layout l = layout(workspace, n, rows_, width);
     if (workspace_bytes < l.bytes)
         return abi_fail(HB_WORKSPACE, "workspace smaller than hb_embedding_grad_workspace()");
-    const int rc = index_sort(ids, id_bytes, n, rows_, l.order, nullptr, l.keys, nullptr, l.sort, l.sort_bytes, st,
+    const int rc = index_sort(ids, id_bytes, n, rows_, nullptr, nullptr, l.pairs, nullptr, l.sort, l.sort_bytes, st,
                               l.arrived, l.arrivals);
     if (rc) return rc;
     int vb = rows::vector_bytes(rows::address_bits(dy) | (uint64_t)(dy_stride * size) | (uint64_t)(width * size), type);
@@ -553,8 +549,7 @@ extern "C" int hb_embedding_grad(int type, const void* dy, int64_t dy_stride, co
             g.rows = rows_;
             g.width = width;
             g.scale = (float)scale;
-            g.order = l.order;
-            g.keys = l.keys;
+            g.pairs = l.pairs;
             g.partial = l.partial;
             g.arrived = l.arrived;
             g.out = static_cast<TO*>(out);

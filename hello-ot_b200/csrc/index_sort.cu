@@ -19,8 +19,9 @@
 //                        between the steps
 //   up to 524288         tiles over all SMs, a launch for the first pass's counts
 //                        and one a pass: a block adds up the counts of all tiles
-//                        itself, and counts the next pass's digits as it places
-//   above                tiles of 8192 and three launches a pass, the counts scanned
+//                        itself, and counts the next pass's digits as it places; the
+//                        launches overlap (the first pass ranks while it is counted)
+//   above                tiles of 4096 and three launches a pass, the counts scanned
 //                        over the tiles by a launch of their own
 #include <string>
 
@@ -42,17 +43,17 @@ constexpr int64_t kRankBins = 4096;                         // most bins whose o
 constexpr int kMostClusters = 16;
 constexpr int64_t kClusterMost = (int64_t)kMostClusters * kBlock * kRounds;
 constexpr int kMaxDigitBits = 11;
-constexpr int kMostTiles = 64;                              // that every block adds up itself
+constexpr int kMostTiles = 128;                             // that every block adds up itself
 
-// The keys of a pass: the caller's index (first pass) or the keys of the pass before.
+// What a pass sorts: the caller's index (first pass), or the (key, entry) pairs of the pass before.
 struct Source {
     const void* data;
-    int kind;  // 4: int32 index, 8: int64 index, 0: uint32 keys
+    int kind;  // 4: int32 index, 8: int64 index, 0: pairs
     uint32_t bins;
-    __device__ __forceinline__ uint32_t key(int64_t i) const {
-        if (kind == 0) return static_cast<const uint32_t*>(data)[i];
+    __device__ __forceinline__ uint2 entry(int64_t i) const {
+        if (kind == 0) return static_cast<const uint2*>(data)[i];
         const int64_t v = kind == 8 ? static_cast<const int64_t*>(data)[i] : (int64_t)static_cast<const int32_t*>(data)[i];
-        return v >= 0 && v < (int64_t)bins ? (uint32_t)v : bins;
+        return make_uint2(v >= 0 && v < (int64_t)bins ? (uint32_t)v : bins, (uint32_t)i);
     }
 };
 
@@ -60,15 +61,16 @@ struct Source {
 // i and those < k after it, of offset b the keys < b.  64 queries a block, 4 threads a query, each over a quarter of
 // the keys in shared memory, where a warp reads the same 16 bytes in all its lanes.
 __global__ void __launch_bounds__(kRankThreads) sort_rank(Source src, int n, int entry_blocks, int32_t* __restrict__ order,
-                                                          int32_t* __restrict__ position, uint32_t* __restrict__ keys_out,
+                                                          int32_t* __restrict__ position, uint2* __restrict__ pairs,
                                                           int32_t* __restrict__ offsets, int bins,
                                                           uint32_t* __restrict__ zero, int64_t zeros) {
     __shared__ __align__(16) uint32_t keys[kRankMost];
     __shared__ uint32_t parts[kRankSlices][kRankQueries];
+    allow_next();
     for (int64_t i = (int64_t)blockIdx.x * kRankThreads + threadIdx.x; i < zeros; i += (int64_t)gridDim.x * kRankThreads)
         zero[i] = 0;
     const int slice_keys = (n + kRankSlices * 4 - 1) / (kRankSlices * 4) * 4;  // whole vectors
-    for (int i = threadIdx.x; i < slice_keys * kRankSlices; i += kRankThreads) keys[i] = i < n ? src.key(i) : 0xffffffffu;
+    for (int i = threadIdx.x; i < slice_keys * kRankSlices; i += kRankThreads) keys[i] = i < n ? src.entry(i).x : 0xffffffffu;
     __syncthreads();
     const int query = threadIdx.x % kRankQueries, slice = threadIdx.x / kRankQueries;
     const bool entries = (int)blockIdx.x < entry_blocks;
@@ -101,37 +103,58 @@ __global__ void __launch_bounds__(kRankThreads) sort_rank(Source src, int n, int
     } else if (i < n) {
         if (order) order[count] = i;
         if (position) position[i] = (int32_t)count;
-        if (keys_out) keys_out[count] = key;
+        if (pairs) pairs[count] = make_uint2(key, (uint32_t)i);
     }
 }
 
-// Rank of every lane's digit among the equal digits its warp has seen, in order.  The lanes with an
-// equal digit come from a ballot a bit of it.
-__device__ __forceinline__ uint32_t warp_rank(uint16_t* counts, uint32_t digit, bool valid, int bits) {
-    const uint32_t lane = threadIdx.x & 31;
+// The lanes whose digit equals this lane's, from a ballot a bit of it.
+__device__ __forceinline__ uint32_t equal_lanes(uint32_t digit, bool valid, int bits) {
     uint32_t same = __ballot_sync(0xffffffffu, valid);
 #pragma unroll 4
     for (int b = 0; b < bits; ++b) {
         const uint32_t set = __ballot_sync(0xffffffffu, (digit >> b) & 1u);
         same &= (digit >> b) & 1u ? set : ~set;
     }
-    const uint32_t before = valid ? counts[digit] : 0;
-    __syncwarp();
-    if (valid && (same >> lane) == 1u) counts[digit] = (uint16_t)(before + __popc(same));
-    __syncwarp();
-    return before + __popc(same & ((1u << lane) - 1u));
+    return same;
+}
+// Ranks of a thread's digits among the equal ones that its warp has seen, in order.  left: entries from this
+// lane's first to the last.
+template <int ROUNDS, typename D>
+__device__ __forceinline__ void warp_ranks(uint16_t* counts, D&& digit, int rounds, int64_t left, int bits,
+                                           uint32_t (&rank)[ROUNDS]) {
+    const uint32_t lane = threadIdx.x & 31;
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r)
+        if (r < rounds) rank[r] = equal_lanes(digit(r), r * 32 < left, bits);
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        if (r >= rounds) break;
+        const uint32_t same = rank[r], d = digit(r);
+        const bool valid = r * 32 < left;
+        const uint32_t before = valid ? counts[d] : 0;
+        __syncwarp();
+        if (valid && (same >> lane) == 1u) counts[d] = (uint16_t)(before + __popc(same));
+        __syncwarp();
+        rank[r] = before + __popc(same & ((1u << lane) - 1u));
+    }
 }
 
 // counts[warp][digit] -> digits before this warp's in the block; total[digit] the block's.
 template <int WARPS>
 __device__ __forceinline__ void scan_warps(uint16_t* counts, uint32_t* total, int digits) {
     for (int d = threadIdx.x; d < digits; d += WARPS * 32) {
+        constexpr int B = 8;  // loads before stores
         uint32_t sum = 0;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            const uint32_t c = counts[w * digits + d];
-            counts[w * digits + d] = (uint16_t)sum;
-            sum += c;
+        for (int w0 = 0; w0 < WARPS; w0 += B) {
+            uint32_t c[B];
+#pragma unroll
+            for (int w = 0; w < B; ++w) c[w] = counts[(w0 + w) * digits + d];
+#pragma unroll
+            for (int w = 0; w < B; ++w) {
+                counts[(w0 + w) * digits + d] = (uint16_t)sum;
+                sum += c[w];
+            }
         }
         total[d] = sum;
     }
@@ -168,11 +191,12 @@ __device__ __forceinline__ void block_scan(uint32_t* v, int digits) {
 // entries w * rounds * 32 + r * 32 + lane, so the order of (block, warp, round, lane) is the entries'.
 __global__ void __launch_bounds__(kBlock, 1) sort_cluster(Source src, int n, int rounds, int passes, int digit_bits,
                                                           int digits, int32_t* __restrict__ order,
-                                                          int32_t* __restrict__ position, uint32_t* __restrict__ keys_out,
+                                                          int32_t* __restrict__ position, uint2* __restrict__ pairs,
                                                           int32_t* __restrict__ offsets, uint32_t* __restrict__ zero,
                                                           int64_t zeros) {
     namespace cg = cooperative_groups;
     extern __shared__ __align__(16) uint32_t smem[];
+    allow_next();
     cg::cluster_group cluster = cg::this_cluster();
     const int blocks = (int)cluster.num_blocks(), me = (int)cluster.block_rank();
     const int mine = rounds * kBlock;                      // entries a block
@@ -185,24 +209,20 @@ __global__ void __launch_bounds__(kBlock, 1) sort_cluster(Source src, int n, int
     const int within = warp * 32 * rounds + lane;
     const int first = me * mine + within;
     for (int64_t i = (int64_t)me * kBlock + threadIdx.x; i < zeros; i += blocks * kBlock) zero[i] = 0;
-    uint32_t key[kRounds], rank[kRounds];
-    int32_t val[kRounds];
+    uint2 entry[kRounds];  // (key, entry)
+    uint32_t rank[kRounds];
 #pragma unroll
-    for (int r = 0; r < kRounds; ++r) {
-        const int i = first + r * 32;
-        if (r < rounds && i < n) key[r] = src.key(i);
-        val[r] = i;
-    }
+    for (int r = 0; r < kRounds; ++r)
+        if (r < rounds && first + r * 32 < n) entry[r] = src.entry(first + r * 32);
+        else entry[r] = make_uint2(0, 0);
     const uint32_t mask = (1u << digit_bits) - 1u;
     for (int pass = 0; pass < passes; ++pass) {
         const int shift = pass * digit_bits;
         const bool last = pass + 1 == passes;
         for (int i = threadIdx.x; i < kBlockWarps * digits / 2; i += kBlock) reinterpret_cast<uint32_t*>(counts)[i] = 0;
         __syncthreads();
-#pragma unroll
-        for (int r = 0; r < kRounds; ++r)
-            if (r < rounds)
-                rank[r] = warp_rank(counts + warp * digits, (key[r] >> shift) & mask, first + r * 32 < n, digit_bits);
+        auto digit = [&](int r) { return (entry[r].x >> shift) & mask; };
+        warp_ranks(counts + warp * digits, digit, rounds, n - first, digit_bits, rank);
         __syncthreads();
         scan_warps<kBlockWarps>(counts, total, digits);
         cluster.sync();
@@ -226,44 +246,43 @@ __global__ void __launch_bounds__(kBlock, 1) sort_cluster(Source src, int n, int
 #pragma unroll
         for (int r = 0; r < kRounds; ++r) {
             if (r < rounds && first + r * 32 < n) {
-                const uint32_t d = (key[r] >> shift) & mask;
+                const uint32_t d = digit(r);
                 const uint32_t p = base[d] + before[d] + counts[warp * digits + d] + rank[r];
                 if (last) {
-                    if (order) order[p] = val[r];
-                    if (position) position[val[r]] = (int32_t)p;
-                    if (keys_out) keys_out[p] = key[r];
+                    if (order) order[p] = (int32_t)entry[r].y;
+                    if (position) position[entry[r].y] = (int32_t)p;
+                    if (pairs) pairs[p] = entry[r];
                 } else {
                     const uint32_t to = p / (uint32_t)mine, at = p - to * (uint32_t)mine;
-                    *cluster.map_shared_rank(entry_at + at, to) = make_uint2(key[r], (uint32_t)val[r]);
+                    *cluster.map_shared_rank(entry_at + at, to) = entry[r];
                 }
             }
         }
         if (!last) {
             cluster.sync();
 #pragma unroll
-            for (int r = 0; r < kRounds; ++r) {
-                if (r < rounds && first + r * 32 < n) {
-                    const uint2 v = entry_at[within + r * 32];
-                    key[r] = v.x;
-                    val[r] = (int32_t)v.y;
-                }
-            }
+            for (int r = 0; r < kRounds; ++r)
+                if (r < rounds && first + r * 32 < n) entry[r] = entry_at[within + r * 32];
         }
     }
 }
 
-// A tile's digits: counts[digit][tile] for scan_tiles (SCANNED), else 16 bits each, two to a word,
-// counts[tile][digit / 2].  Clears `next` and `zero` too.
+// Words of a tile's packed counts: 16 bits a digit, in whole 16-byte vectors.
+__host__ __device__ inline int words_of(int digits) { return (digits + 7) / 8 * 4; }
+
+// A tile's digits: counts[digit][tile] for scan_tiles (SCANNED), else packed, counts[tile][words_of].  Clears
+// `next` and `zero` too.
 template <int ROUNDS, bool SCANNED>
 __global__ void __launch_bounds__(kThreads) tile_counts(Source src, int64_t n, int shift, uint32_t mask, int digits,
                                                         int tiles, uint32_t* __restrict__ counts,
                                                         uint32_t* __restrict__ next, int64_t nexts,
                                                         uint32_t* __restrict__ zero, int64_t zeros) {
     extern __shared__ uint32_t smem[];
+    allow_next();
     const int64_t thread = (int64_t)blockIdx.x * kThreads + threadIdx.x, threads = (int64_t)tiles * kThreads;
     for (int64_t i = thread; i < nexts; i += threads) next[i] = 0;
     for (int64_t i = thread; i < zeros; i += threads) zero[i] = 0;
-    const int words = SCANNED ? digits : (digits + 1) / 2;
+    const int words = SCANNED ? digits : words_of(digits);
     for (int d = threadIdx.x; d < words; d += kThreads) smem[d] = 0;
     __syncthreads();
     const int64_t base = (int64_t)blockIdx.x * (kThreads * ROUNDS);
@@ -271,7 +290,7 @@ __global__ void __launch_bounds__(kThreads) tile_counts(Source src, int64_t n, i
     for (int r = 0; r < ROUNDS; ++r) {
         const int64_t i = base + r * kThreads + threadIdx.x;
         if (i < n) {
-            const uint32_t d = (src.key(i) >> shift) & mask;
+            const uint32_t d = (src.entry(i).x >> shift) & mask;
             atomicAdd(&smem[SCANNED ? d : d / 2], SCANNED ? 1u : 1u << (d % 2 * 16));
         }
     }
@@ -304,13 +323,13 @@ __global__ void __launch_bounds__(256) scan_tiles(uint32_t* __restrict__ counts,
 
 // Places a tile's entries.  SCANNED: counts and totals as scan_tiles leaves them; else the tiles' packed counts,
 // and the digits of the next pass are counted into `next` (cleared before), tile by tile of where entries go.
-template <int ROUNDS, bool SCANNED>
-__global__ void __launch_bounds__(kThreads) tile_place(Source src, const int32_t* __restrict__ vals, int64_t n, int shift,
-                                                       uint32_t mask, int digits, int tiles,
-                                                       const uint32_t* __restrict__ counts,
+// FIRST: the first pass, whose keys are the caller's: the block ranks them while the counts are still being made.
+template <int ROUNDS, bool SCANNED, bool FIRST>
+__global__ void __launch_bounds__(kThreads) tile_place(Source src, int64_t n, int shift, uint32_t mask, int digits,
+                                                       int tiles, const uint32_t* __restrict__ counts,
                                                        const uint32_t* __restrict__ totals, uint32_t* __restrict__ next,
                                                        int next_shift, int32_t* __restrict__ order,
-                                                       int32_t* __restrict__ position, uint32_t* __restrict__ keys_out,
+                                                       int32_t* __restrict__ position, uint2* __restrict__ pairs,
                                                        int32_t* __restrict__ offsets) {
     extern __shared__ uint32_t smem[];
     uint32_t* base = smem;                                            // digits: of all entries
@@ -319,74 +338,82 @@ __global__ void __launch_bounds__(kThreads) tile_place(Source src, const int32_t
     uint16_t* mine = reinterpret_cast<uint16_t*>(total + digits);     // kWarps x digits
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t first = (int64_t)blockIdx.x * (kThreads * ROUNDS) + warp * (32 * ROUNDS) + lane;
-    uint32_t key[ROUNDS], rank[ROUNDS];
-    int32_t val[ROUNDS];
+    uint2 entry[ROUNDS];  // (key, entry)
+    uint32_t rank[ROUNDS];
+    auto digit = [&](int r) { return (entry[r].x >> shift) & mask; };
+    allow_next();
+    for (int d = threadIdx.x; d < digits; d += kThreads) base[d] = before[d] = 0;
+    for (int i = threadIdx.x; i < kWarps * digits / 2; i += kThreads) reinterpret_cast<uint32_t*>(mine)[i] = 0;
+    if (!FIRST) after_last();
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
-        const int64_t i = first + r * 32;
-        key[r] = i < n ? src.key(i) : 0;
-        val[r] = i < n ? (vals ? vals[i] : (int32_t)i) : 0;
+        entry[r] = make_uint2(0, 0);
+        if (first + r * 32 < n) entry[r] = src.entry(first + r * 32);
     }
-    for (int d = threadIdx.x; d < digits; d += kThreads) {
-        base[d] = SCANNED ? totals[d] : 0;
-        before[d] = SCANNED ? counts[(int64_t)d * tiles + blockIdx.x] : 0;
-    }
-    for (int i = threadIdx.x; i < kWarps * digits; i += kThreads) mine[i] = 0;
     __syncthreads();
-    const int words = (digits + 1) / 2;
-    if (!SCANNED) {  // as many threads a word of counts as there are, each every slices-th tile
-        const int slices = max(1, kThreads / words);
-        for (int j = threadIdx.x; j < words * slices; j += kThreads) {
-            const int w = j % words;
-            uint32_t all[2] = {0, 0}, lower[2] = {0, 0};
-#pragma unroll 16
-            for (int t = j / words; t < tiles; t += slices) {
-                const uint32_t c = counts[(int64_t)t * words + w];
-                const uint32_t low = t < (int)blockIdx.x ? c : 0;
-                all[0] += c & 0xffffu, all[1] += c >> 16;
-                lower[0] += low & 0xffffu, lower[1] += low >> 16;
+    warp_ranks(mine + warp * digits, digit, ROUNDS, n - first, __popc(mask), rank);
+    __syncthreads();
+    scan_warps<kWarps>(mine, total, digits);
+    if (FIRST) after_last();
+    const int words = words_of(digits);
+    if (SCANNED) {
+        for (int d = threadIdx.x; d < digits; d += kThreads) {
+            base[d] = totals[d];
+            before[d] = counts[(int64_t)d * tiles + blockIdx.x];
+        }
+    } else {  // a vector of 8 digits a thread, as many threads a vector as there are, each every slices-th tile
+        const int vectors = words / 4, slices = kThreads / vectors;
+        const int v = threadIdx.x % vectors, slice = threadIdx.x / vectors;
+        if (slice < slices) {
+            uint32_t all[8] = {}, lower[8] = {};
+#pragma unroll 4
+            for (int t = slice; t < tiles; t += slices) {
+                const uint4 c = reinterpret_cast<const uint4*>(counts + (int64_t)t * words)[v];
+                const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+                const uint32_t own = t < (int)blockIdx.x ? ~0u : 0u;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    all[2 * i] += w[i] & 0xffffu, all[2 * i + 1] += w[i] >> 16;
+                    lower[2 * i] += w[i] & 0xffffu & own, lower[2 * i + 1] += w[i] >> 16 & own;
+                }
             }
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                if (w * 2 + h < digits) {
-                    atomicAdd(&base[w * 2 + h], all[h]);
-                    atomicAdd(&before[w * 2 + h], lower[h]);
+            for (int i = 0; i < 8; ++i)
+                if (v * 8 + i < digits) {
+                    atomicAdd(&base[v * 8 + i], all[i]);
+                    atomicAdd(&before[v * 8 + i], lower[i]);
                 }
         }
     }
-#pragma unroll
-    for (int r = 0; r < ROUNDS; ++r)
-        rank[r] = warp_rank(mine + warp * digits, (key[r] >> shift) & mask, first + r * 32 < n, __popc(mask));
     __syncthreads();
     block_scan<kWarps>(base, digits);
     if (offsets && blockIdx.x == 0)
         for (int d = threadIdx.x; d < digits; d += kThreads) offsets[d] = (int32_t)base[d];
-    scan_warps<kWarps>(mine, total, digits);
-    __syncthreads();
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
         if (first + r * 32 >= n) continue;
-        const uint32_t d = (key[r] >> shift) & mask;
+        const uint32_t d = digit(r), e = FIRST ? (uint32_t)(first + r * 32) : entry[r].y;
         const uint32_t p = base[d] + before[d] + mine[warp * digits + d] + rank[r];
-        if (order) order[p] = val[r];
-        if (position) position[val[r]] = (int32_t)p;
-        if (keys_out) keys_out[p] = key[r];
+        if (order) order[p] = (int32_t)e;
+        if (position) position[e] = (int32_t)p;
+        if (pairs) pairs[p] = make_uint2(entry[r].x, e);
         if (next) {
-            const uint32_t q = (key[r] >> next_shift) & mask;
+            const uint32_t q = (entry[r].x >> next_shift) & mask;
             atomicAdd(&next[(int64_t)(p / (kThreads * ROUNDS)) * words + q / 2], 1u << (q % 2 * 16));
         }
     }
 }
 
 // offsets[b] = first place whose key is not below b.
-__global__ void __launch_bounds__(256) find_offsets(const uint32_t* __restrict__ keys, int64_t n, int64_t bins,
+__global__ void __launch_bounds__(256) find_offsets(const uint2* __restrict__ pairs, int64_t n, int64_t bins,
                                                     int32_t* __restrict__ offsets) {
     const int64_t b = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    after_last();
     if (b > bins) return;
     int64_t lo = 0, hi = n;
     while (lo < hi) {
         const int64_t mid = (lo + hi) >> 1;
-        if (keys[mid] < (uint32_t)b) lo = mid + 1;
+        if (pairs[mid].x < (uint32_t)b) lo = mid + 1;
         else hi = mid;
     }
     offsets[b] = (int32_t)lo;
@@ -399,8 +426,8 @@ struct Plan {
 };
 
 // One pass over bins + 1 digits when they fit, else equal digits of at most 11 bits.
-// A cluster has a block for every 1024 entries up to 16; tiles have 2048, 4096 or 8192
-// entries, the least that makes at most 64 tiles, so that a block adds up their counts in a few loads a thread.
+// A cluster has a block for every 1024 entries up to 16; tiles have 1024, 2048 or 4096
+// entries, the least that makes at most 128 tiles, so that a block adds up their counts in a few loads a thread.
 inline Plan plan_of(int64_t n, int64_t bins) {
     Plan p{};
     p.rank = n <= kRankMost;
@@ -415,19 +442,19 @@ inline Plan plan_of(int64_t n, int64_t bins) {
         p.rounds = (int)((n + p.cluster * kBlock - 1) / (p.cluster * kBlock));
         return p;
     }
-    p.rounds = 2;
-    while (p.rounds < 8 && (int64_t)p.rounds * kThreads * kMostTiles < n) p.rounds <<= 1;
+    p.rounds = 1;
+    while (p.rounds < 4 && (int64_t)p.rounds * kThreads * kMostTiles < n) p.rounds <<= 1;
     const int64_t tile = (int64_t)kThreads * p.rounds;
     p.tiles = (int)((n + tile - 1) / tile);
     return p;
 }
 inline bool scanned(const Plan& p) { return p.tiles > kMostTiles; }
 
-// Counts (of a pass, or of each) and totals, the keys and entries between passes, and the sorted keys
-// (searched for the offsets when the caller takes no keys).
+// Counts (of a pass, or of each) and totals, the pairs between passes, and the sorted pairs (searched for the
+// offsets when the caller takes none).
 struct Layout {
-    uint32_t *counts, *totals, *keys[2], *sorted;
-    int32_t* vals[2];
+    uint32_t *counts, *totals;
+    uint2 *pairs[2], *sorted;
     size_t bytes;
 };
 inline Layout layout(void* ws, int64_t n, int64_t bins, const Plan& p) {
@@ -440,14 +467,11 @@ inline Layout layout(void* ws, int64_t n, int64_t bins, const Plan& p) {
     };
     if (!p.cluster) {
         l.counts = reinterpret_cast<uint32_t*>(
-            take(sizeof(uint32_t) * p.tiles * (scanned(p) ? (size_t)p.digits : (size_t)(p.digits + 1) / 2 * p.passes)));
+            take(sizeof(uint32_t) * p.tiles * (scanned(p) ? (size_t)p.digits : (size_t)words_of(p.digits) * p.passes)));
         l.totals = reinterpret_cast<uint32_t*>(take(sizeof(uint32_t) * p.digits));
-        for (int i = 0; i < 2 && i + 1 < p.passes; ++i) {
-            l.keys[i] = reinterpret_cast<uint32_t*>(take(sizeof(uint32_t) * n));
-            l.vals[i] = reinterpret_cast<int32_t*>(take(sizeof(int32_t) * n));
-        }
+        for (int i = 0; i < 2 && i + 1 < p.passes; ++i) l.pairs[i] = reinterpret_cast<uint2*>(take(sizeof(uint2) * n));
     }
-    if (p.rank ? bins > kRankBins : p.passes > 1) l.sorted = reinterpret_cast<uint32_t*>(take(sizeof(uint32_t) * n));
+    if (p.rank ? bins > kRankBins : p.passes > 1) l.sorted = reinterpret_cast<uint2*>(take(sizeof(uint2) * n));
     return l;
 }
 
@@ -464,7 +488,7 @@ inline cudaError_t allow(K* kernel, size_t bytes) {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
 }
 
-cudaError_t sort_one_launch(const Source& src, int n, const Plan& p, int32_t* order, int32_t* position, uint32_t* keys,
+cudaError_t sort_one_launch(const Source& src, int n, const Plan& p, int32_t* order, int32_t* position, uint2* pairs,
                             int32_t* offsets, uint32_t* zero, int64_t zeros, cudaStream_t st) {
     cudaError_t e = allow(sort_cluster, cluster_smem(p));
     if (e == cudaSuccess && p.cluster > 8)
@@ -483,26 +507,26 @@ cudaError_t sort_one_launch(const Source& src, int n, const Plan& p, int32_t* or
     config.numAttrs = 1;
     count_launches(1);
     return cudaLaunchKernelEx(&config, sort_cluster, src, n, p.rounds, p.passes, p.digit_bits, p.digits, order, position,
-                              keys, offsets, zero, zeros);
+                              pairs, offsets, zero, zeros);
 }
 
 template <int ROUNDS, bool SCANNED>
 cudaError_t sort_tiles(const Source& input, int64_t n, const Plan& p, const Layout& l, int32_t* order, int32_t* position,
-                       uint32_t* keys, int32_t* offsets, uint32_t* zero, int64_t zeros, cudaStream_t st) {
-    cudaError_t e = allow(tile_place<ROUNDS, SCANNED>, place_smem(p));
+                       uint2* pairs, int32_t* offsets, uint32_t* zero, int64_t zeros, cudaStream_t st) {
+    cudaError_t e = allow(tile_place<ROUNDS, SCANNED, true>, place_smem(p));
+    if (e == cudaSuccess) e = allow(tile_place<ROUNDS, SCANNED, false>, place_smem(p));
     if (e != cudaSuccess) return e;
     const uint32_t mask = (1u << p.digit_bits) - 1u;
-    const int64_t counted = (int64_t)(p.digits + 1) / 2 * p.tiles;  // words of a pass (SCANNED has one area)
+    const int64_t counted = (int64_t)words_of(p.digits) * p.tiles;  // words of a pass (SCANNED has one area)
     Source src = input;
-    const int32_t* vals = nullptr;
     for (int pass = 0; pass < p.passes; ++pass) {
         const int shift = pass * p.digit_bits;
         const bool last = pass + 1 == p.passes;
-        uint32_t* to_keys = last ? keys : l.keys[pass & 1];
-        int32_t* to_vals = last ? order : l.vals[pass & 1];
+        uint2* to = last ? pairs : l.pairs[pass & 1];
         uint32_t* counts = l.counts + (SCANNED ? 0 : pass * counted);
         if (SCANNED || pass == 0) {
-            tile_counts<ROUNDS, SCANNED><<<p.tiles, kThreads, sizeof(uint32_t) * p.digits, st>>>(
+            const size_t smem = sizeof(uint32_t) * (SCANNED ? p.digits : words_of(p.digits));
+            tile_counts<ROUNDS, SCANNED><<<p.tiles, kThreads, smem, st>>>(
                 src, n, shift, mask, p.digits, p.tiles, counts, l.counts + counted,
                 SCANNED ? 0 : counted * (p.passes - 1), zero, pass == 0 ? zeros : 0);
             count_launches(1);
@@ -511,13 +535,15 @@ cudaError_t sort_tiles(const Source& input, int64_t n, const Plan& p, const Layo
             scan_tiles<<<(p.digits + 7) / 8, 256, 0, st>>>(counts, p.tiles, p.digits, l.totals);
             count_launches(1);
         }
-        tile_place<ROUNDS, SCANNED><<<p.tiles, kThreads, place_smem(p), st>>>(
-            src, vals, n, shift, mask, p.digits, p.tiles, counts, l.totals, SCANNED || last ? nullptr : counts + counted,
-            shift + p.digit_bits, to_vals, last ? position : nullptr, to_keys, last && p.passes == 1 ? offsets : nullptr);
+        const auto place = pass == 0 ? tile_place<ROUNDS, SCANNED, true> : tile_place<ROUNDS, SCANNED, false>;
+        e = launch_next(place, p.tiles, kThreads, place_smem(p), st, src, n, shift, mask, p.digits, p.tiles, counts,
+                        l.totals, SCANNED || last ? nullptr : counts + counted, shift + p.digit_bits,
+                        last ? order : nullptr, last ? position : nullptr, to,
+                        last && p.passes == 1 ? offsets : nullptr);
+        if (e != cudaSuccess) return e;
         count_launches(1);
-        src.data = to_keys;
+        src.data = to;
         src.kind = 0;
-        vals = to_vals;
     }
     return cudaGetLastError();
 }
@@ -530,7 +556,7 @@ size_t index_sort_bytes(int64_t n, int64_t bins) {
 }
 
 int index_sort(const void* index, int index_bytes, int64_t n, int64_t bins, int32_t* order, int32_t* position,
-               uint32_t* keys, int32_t* offsets, void* ws, size_t ws_bytes, cudaStream_t st, uint32_t* zero,
+               uint2* pairs, int32_t* offsets, void* ws, size_t ws_bytes, cudaStream_t st, uint32_t* zero,
                int64_t zeros) {
     using namespace isort;
     cudaError_t e = cudaSuccess;
@@ -545,28 +571,27 @@ int index_sort(const void* index, int index_bytes, int64_t n, int64_t bins, int3
     if (l.bytes > ws_bytes || (l.bytes > 0 && !ws))
         return abi_fail(HB_WORKSPACE, "workspace too small for the index sort");
     const Source src{index, index_bytes, (uint32_t)bins};
-    const bool search = offsets && (p.rank ? bins > kRankBins : p.passes > 1);  // offsets by searching the sorted keys
-    if (!keys && search) keys = l.sorted;
+    const bool search = offsets && (p.rank ? bins > kRankBins : p.passes > 1);  // offsets by searching the sorted pairs
+    if (!pairs && search) pairs = l.sorted;
     if (p.rank) {
         const int blocks = (int)((n + kRankQueries - 1) / kRankQueries);
         const int more = offsets && !search ? (int)(bins / kRankQueries + 1) : 0;
-        sort_rank<<<blocks + more, kRankThreads, 0, st>>>(src, (int)n, blocks, order, position, keys, offsets,
+        sort_rank<<<blocks + more, kRankThreads, 0, st>>>(src, (int)n, blocks, order, position, pairs, offsets,
                                                           (int)bins, zero, zeros);
         count_launches(1);
         e = cudaGetLastError();
     } else if (p.cluster) {
-        e = sort_one_launch(src, (int)n, p, order, position, keys, offsets, zero, zeros, st);
+        e = sort_one_launch(src, (int)n, p, order, position, pairs, offsets, zero, zeros, st);
     } else {
-        auto sort = scanned(p) ? sort_tiles<8, true>
-                    : p.rounds == 8 ? sort_tiles<8, false>
+        auto sort = scanned(p) ? sort_tiles<4, true>
                     : p.rounds == 4 ? sort_tiles<4, false>
-                                    : sort_tiles<2, false>;
-        e = sort(src, n, p, l, order, position, keys, offsets, zero, zeros, st);
+                    : p.rounds == 2 ? sort_tiles<2, false>
+                                    : sort_tiles<1, false>;
+        e = sort(src, n, p, l, order, position, pairs, offsets, zero, zeros, st);
     }
     if (e == cudaSuccess && search) {
-        find_offsets<<<(unsigned)((bins + 256) / 256), 256, 0, st>>>(keys, n, bins, offsets);
+        e = launch_next(find_offsets, dim3((unsigned)((bins + 256) / 256)), 256, 0, st, pairs, n, bins, offsets);
         count_launches(1);
-        e = cudaGetLastError();
     }
     return e == cudaSuccess ? HB_OK : abi_fail(HB_LAUNCH, std::string("index sort: ") + cudaGetErrorString(e));
 }

@@ -19,11 +19,11 @@ def f64(t):
 
 
 def plan(index, experts):
-    """(order, position, offsets) by counting, entry by entry in order."""
+    """(order, position, offsets) of a stable sort by expert."""
     index = np.asarray(index)
     flat = index.reshape(-1)
     key = np.where((flat >= 0) & (flat < experts), flat, experts)
-    order = np.concatenate([np.nonzero(key == e)[0] for e in np.unique(key)] or [np.zeros(0, int)]).astype(np.int64)
+    order = np.argsort(key, kind="stable")
     position = np.empty_like(order)
     position[order] = np.arange(order.size)
     count = np.bincount(key, minlength=experts + 1)[:experts]

@@ -28,7 +28,7 @@ def _check_plan(plan, index, experts):
     (4097, 1, 7), (5000, 3, 1024), (100, 100, 2047), (8193, 2, 300), (65537, 1, 5), (131072, 1, 2047),  # clusters
     (4097, 1, 2048), (20000, 2, 100003), (3000, 4, 5_000_000), (65536, 2, 65536),
     (131073, 1, 1024), (200000, 2, 100003), (140000, 1, 5_000_000),                             # tiles of 1024
-    (2 ** 19 + 5, 1, 37), (70001, 8, 1025), (2 ** 19 + 1, 1, 4000)])                            # tiles of 4096
+    (2 ** 19 + 5, 1, 37), (70001, 8, 1025), (2 ** 19 + 1, 1, 4000), (2 ** 18 + 3, 2, 200), (2 ** 19, 1, 300)])                            # tiles of 4096
 @pytest.mark.parametrize("dropped", [0.0, 0.2])
 def test_plan_matches_counting(hb, cuda, tokens, slots, experts, dropped):
     rng = np.random.default_rng(tokens + slots)
