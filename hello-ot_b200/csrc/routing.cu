@@ -124,16 +124,8 @@ __global__ void __launch_bounds__(256) combine_kernel(Moves m, const T* __restri
     if (SLOTS) places(e0);
     const uint32_t kept = kept_entries(m);
     for (int64_t c0 = (threadIdx.x % G) * V::N; c0 < m.width; c0 += G * V::N * U) {
-        float sum[U][M][V::N];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int t = 0; t < M; ++t)
-#pragma unroll
-                for (int i = 0; i < V::N; ++i) sum[u][t][i] = 0.0f;
-        for (int64_t e = e0; e < e1; e += B) {
-            if (!SLOTS) places(e);
-            V v[U][B];
+        V v[U][B];
+        auto load = [&]() {
 #pragma unroll
             for (int b = 0; b < B; ++b) {
                 const T* row = z + (int64_t)p[b] * z_stride + c0;
@@ -141,27 +133,43 @@ __global__ void __launch_bounds__(256) combine_kernel(Moves m, const T* __restri
                 for (int u = 0; u < U; ++u)
                     if (p[b] < kept && c0 + u * G * V::N < m.width) v[u][b].load_once(row + u * G * V::N);
             }
+        };
+        auto add = [&](int b, int u, float (&sum)[V::N]) {
+            if (p[b] < kept) {
 #pragma unroll
-            for (int b = 0; b < B; ++b)
-                if (p[b] < kept) {
-#pragma unroll
-                    for (int u = 0; u < U; ++u)
-#pragma unroll
-                        for (int i = 0; i < V::N; ++i)
-                            sum[u][b / S][i] = fmaf(w[b], rows::to_float(v[u][b].v[i]), sum[u][b / S][i]);
-                }
-        }
-#pragma unroll
-        for (int t = 0; t < M; ++t) {
-            if (token + t >= m.tokens) break;
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (c0 + u * G * V::N >= m.width) break;
-                V r;
-#pragma unroll
-                for (int i = 0; i < V::N; ++i) r.v[i] = rows::from_float<T>(sum[u][t][i]);
-                r.store(out + (token + t) * m.width + c0 + u * G * V::N);
+                for (int i = 0; i < V::N; ++i) sum[i] = fmaf(w[b], rows::to_float(v[u][b].v[i]), sum[i]);
             }
+        };
+        auto store = [&](int64_t t, int u, const float (&sum)[V::N]) {
+            if (t >= m.tokens || c0 + u * G * V::N >= m.width) return;
+            V r;
+#pragma unroll
+            for (int i = 0; i < V::N; ++i) r.v[i] = rows::from_float<T>(sum[i]);
+            r.store(out + t * m.width + c0 + u * G * V::N);
+        };
+        if (SLOTS) {  // all rows of the tokens at once; one token's sum at a time
+            load();
+#pragma unroll
+            for (int t = 0; t < M; ++t)
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    float sum[V::N] = {};
+#pragma unroll
+                    for (int k = 0; k < S; ++k) add(t * S + k, u, sum);
+                    store(token + t, u, sum);
+                }
+        } else {
+            float sum[U][V::N] = {};
+            for (int64_t e = e0; e < e1; e += B) {
+                places(e);
+                load();
+#pragma unroll
+                for (int b = 0; b < B; ++b)
+#pragma unroll
+                    for (int u = 0; u < U; ++u) add(b, u, sum[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) store(token, u, sum[u]);
         }
     }
 }
