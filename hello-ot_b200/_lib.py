@@ -28,6 +28,8 @@ EXPORTS = ("hb_abi_version", "hb_last_error", "hb_kernel_launch_count", "hb_set_
            "hb_route_dispatch", "hb_route_combine", "hb_route_combine_grad", "hb_embedding_lookup",
            "hb_embedding_grad_workspace", "hb_embedding_grad", "hb_clip_workspace", "hb_grad_norm",
            "hb_clip_grad_norm")
+# the current device and stream handle without torch.cuda's wrappers (2 us a call), where torch has them
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda device: torch.cuda.current_stream(device).cuda_stream)
 FLOAT_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # HB_F32, HB_F16, HB_BF16
@@ -213,9 +215,8 @@ def stream_handle(device) -> int:
 
 def device_of(what: str, *tensors) -> int:
     """The one CUDA device of all tensors, by index."""
-    devices = set(map(torch.Tensor.get_device, tensors))
-    device = devices.pop()
-    if devices or device < 0:
+    device = tensors[0].get_device()  # -1 on the CPU
+    if device < 0 or any([t.get_device() != device for t in tensors]):
         lib()  # without CUDA: the library's own error
         raise ValueError(f"{what}: expected CUDA tensors on one device, got {[str(t.device) for t in tensors]}")
     return device
@@ -223,7 +224,7 @@ def device_of(what: str, *tensors) -> int:
 
 def call(device: int, function, *args) -> None:
     """function(*args, stream) on the device's current stream, with the device current."""
-    if torch.cuda.current_device() == device:
+    if _current_device() == device:
         rc = function(*args, _raw_stream(device))
     else:
         with torch.cuda.device(device):
@@ -238,11 +239,13 @@ def feature_rows(t, what: str):
         raise ValueError(f"{what} must be 2-D (rows x features), got {tuple(t.shape)}")
     if t.dtype not in FLOAT_TYPES:
         raise ValueError(f"{what} must be float32, float16 or bfloat16, got {t.dtype}")
-    rows, stride = t.shape[0], t.stride()
-    if t.shape[1] > 1 and stride[1] != 1:
-        t = t.contiguous()
-        return t, t.shape[1]
-    return t, stride[0] if rows > 1 else t.shape[1]
+    rows, width = t.shape
+    if t.is_contiguous():
+        return t, width
+    stride = t.stride()
+    if width > 1 and stride[1] != 1:
+        return t.contiguous(), width
+    return t, stride[0] if rows > 1 else width
 
 
 def index_bytes(t, what: str) -> int:

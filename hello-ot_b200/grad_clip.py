@@ -29,7 +29,7 @@ def _addresses(tensors, what: str):
         types = array("i", [FLOAT_TYPES[t.dtype] for t in tensors])
     except KeyError as e:
         raise ValueError(f"{what}: gradients are float32, float16 or bfloat16, got {e.args[0]}") from None
-    contiguous = all(map(torch.Tensor.is_contiguous, tensors))
+    contiguous = False not in map(torch.Tensor.is_contiguous, tensors)
     if not contiguous:
         for t in tensors:
             if not t.is_contiguous() and not _dense(t):
@@ -51,13 +51,14 @@ def _run(grads, limit, out, what):
     grads = _tensors(grads)
     if not grads:
         raise ValueError(f"{what}: no gradients")
+    first = grads[0]
     device = device_of(what, *grads)
     pointers, types, contiguous = _addresses(grads, what)
     sizes = array("q", map(torch.Tensor.numel, grads))
     L = load_library()
-    norm = grads[0].new_empty((), dtype=torch.float32)
+    norm = first.new_empty((), dtype=torch.float32)
     nbytes = L.hb_clip_workspace(len(grads))
-    ws = grads[0].new_empty(nbytes, dtype=torch.uint8)
+    ws = first.new_empty(nbytes, dtype=torch.uint8)
     host = [len(grads), pointers.buffer_info()[0], sizes.buffer_info()[0], types.buffer_info()[0]]
     if limit is None:
         call(device, L.hb_grad_norm, *host, norm.data_ptr(), ws.data_ptr(), nbytes)
@@ -68,10 +69,9 @@ def _run(grads, limit, out, what):
     to_pointers, to_types = pointers, types
     if out is not None:
         out = _tensors(out)
-        if len(out) != len(grads) or not all(map(torch.Tensor.is_same_size, grads, out)):
+        if [g.shape for g in grads] != [o.shape for o in out]:
             raise ValueError(f"{what}: outputs have their gradients' shapes")
-        if device_of(what, *out) != device:
-            raise ValueError(f"{what}: outputs on another device than their gradients")
+        device_of(what, first, *out)
         to_pointers, to_types, to_contiguous = _addresses(out, what)
         if not (contiguous and to_contiguous) and any(o.stride() != g.stride() for g, o in zip(grads, out)
                                                       if not (g.is_contiguous() and o.is_contiguous())):

@@ -78,18 +78,20 @@ def route_plan(index, num_experts: int) -> RoutePlan:
 
 def _places(plan, what: str):
     """(position, address of the number of entries with an expert) of a checked plan."""
-    position, offsets = plan.position, plan.offsets
-    if position.dtype != torch.int32 or offsets.dtype != torch.int32 or position.dim() != 2 or offsets.dim() != 1:
+    _, position, offsets = plan
+    int32 = torch.int32
+    if position.dtype != int32 or offsets.dtype != int32 or position.dim() != 2 or offsets.dim() != 1:
         raise ValueError(f"{what}: a plan holds int32 position [tokens, slots] and offsets [num_experts + 1]")
-    if not position.is_contiguous() or not offsets.is_contiguous() or offsets.numel() < 2 or position.shape[1] < 1:
+    ends = offsets.numel()
+    if not position.is_contiguous() or not offsets.is_contiguous() or ends < 2 or position.size(1) < 1:
         raise ValueError(f"{what}: a plan's tensors are contiguous, with at least one slot and one expert")
-    return position, offsets.data_ptr() + 4 * (offsets.numel() - 1)
+    return position, offsets.data_ptr() + 4 * (ends - 1)
 
 
 def _weights(weights, position, what: str):
     if weights.dtype not in FLOAT_TYPES:
         raise ValueError(f"{what}: weights must be float32, float16 or bfloat16, got {weights.dtype}")
-    if weights.numel() != position.numel() or weights.shape[0] != position.shape[0] or weights.dim() > 2:
+    if weights.shape != position.shape and (weights.shape != position.shape[:1] or position.size(1) != 1):
         raise ValueError(f"{what}: weights {tuple(weights.shape)} do not fit an assignment {tuple(position.shape)}")
     return weights.contiguous()
 
