@@ -12,8 +12,8 @@
 // Every kernel goes by token: a group of threads holds the columns of a token, so
 // x, dy and y cross HBM once and each sorted row once, which is all they have to.
 // Bound by HBM, so what counts is loads in flight: each thread has 4 vectors of 8 or
-// 16 bytes under way, or 16 shorter ones, of one row or of 4.  Sums are fp32 and run
-// over k in order (no atomics): the result does not depend on the launch.
+// 16 bytes under way, or 16 and more shorter ones, of one row or of 4.  Sums are fp32
+// and run over k in order (no atomics): the result does not depend on the launch.
 #include <string>
 
 #include "index_sort.cuh"
@@ -40,13 +40,13 @@ __device__ __forceinline__ uint32_t kept_entries(const Moves& m) {
 // flight as one long vector.
 constexpr int steps_of(int vb) { return vb >= 8 ? 1 : 4; }
 
-// A group serves M tokens, U column steps at a time: 4 vectors a thread in flight, 16 short ones.  Wide rows: one
-// token; narrow ones, of at most steps_of(VB) vectors a thread: 4.
+// A group serves M tokens, U column steps at a time: 4 vectors a thread in flight, 16 of 4 bytes, 32 of 2.  Wide
+// rows: one token; narrow ones, of at most steps_of(VB) vectors a thread: 4.
 template <typename T, int VB, int G, bool NARROW>
 __global__ void __launch_bounds__(256) dispatch_kernel(Moves m, const T* __restrict__ x, int64_t x_stride,
                                                        T* __restrict__ out) {
     using V = Vec<T, VB>;
-    constexpr int M = NARROW ? 4 : 1, U = steps_of(VB) * 4 / M;
+    constexpr int M = NARROW ? 4 : 1, U = NARROW ? steps_of(VB) : VB >= 8 ? 4 : VB == 4 ? 16 : 32;
     const int64_t token = ((int64_t)blockIdx.x * (256 / G) + threadIdx.x / G) * M;
     if (token >= m.tokens) return;
     const uint32_t kept = kept_entries(m);
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(256) combine_kernel(Moves m, const T* __restri
                                                       T* __restrict__ out) {
     using V = Vec<T, VB>;
     constexpr int B = 4, M = SLOTS ? B / SLOTS : 1, S = B / M;  // rows, tokens, rows of a token in flight
-    constexpr int U = VB >= 8 ? 1 : 4;                          // column steps in flight
+    constexpr int U = VB >= 8 ? 1 : VB == 4 ? 4 : 8;            // column steps in flight
     const int64_t token = ((int64_t)blockIdx.x * (256 / G) + threadIdx.x / G) * M;
     if (token >= m.tokens) return;
     const int slots = SLOTS ? SLOTS : m.slots;
@@ -199,15 +199,15 @@ __device__ __forceinline__ void group_sum(float (&v)[B]) {
     }
 }
 
-// Wide rows: a group goes through a token's entries, 4 vectors a thread (8 short ones) of z and of dy, which
-// is in L1 after the first entry.
+// Wide rows: a group goes through a token's entries, 4 vectors a thread (8 of 4 bytes, 16 of 2) of z and of dy,
+// which is in L1 after the first entry.
 template <typename T, int VB, int G>
 __global__ void __launch_bounds__(256) combine_grad_kernel(Moves m, const T* __restrict__ dy, int64_t dy_stride,
                                                            const T* __restrict__ z, int64_t z_stride,
                                                            const void* __restrict__ weights, int weight_type,
                                                            T* __restrict__ dz, void* __restrict__ dw) {
     using V = Vec<T, VB>;
-    constexpr int U = VB >= 8 ? 4 : 8;
+    constexpr int U = VB >= 8 ? 4 : VB == 4 ? 8 : 16;
     const int64_t token = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
     if (token >= m.tokens) return;  // G = 256: the whole block or none of it
     const uint32_t kept = kept_entries(m);
