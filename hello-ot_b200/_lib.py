@@ -28,11 +28,6 @@ EXPORTS = ("hb_abi_version", "hb_last_error", "hb_kernel_launch_count", "hb_set_
            "hb_route_dispatch", "hb_route_combine", "hb_route_combine_grad", "hb_embedding_lookup",
            "hb_embedding_grad_workspace", "hb_embedding_grad", "hb_clip_workspace", "hb_grad_norm",
            "hb_clip_grad_norm")
-# the current device and stream handle without torch.cuda's wrappers (2 us a call), where torch has them
-_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
-    lambda device: torch.cuda.current_stream(device).cuda_stream)
-FLOAT_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # HB_F32, HB_F16, HB_BF16
 
 
 class HBError(RuntimeError):
@@ -73,6 +68,7 @@ class PdlpTraceRow(ctypes.Structure):
 
 
 _LIB = None
+_HOST = None
 
 
 def load_library(path: Path | str = LIB_PATH):
@@ -213,48 +209,16 @@ def stream_handle(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def device_of(what: str, *tensors) -> int:
-    """The one CUDA device of all tensors, by index."""
-    device = tensors[0].get_device()  # -1 on the CPU
-    if device < 0 or any([t.get_device() != device for t in tensors]):
-        lib()  # without CUDA: the library's own error
-        raise ValueError(f"{what}: expected CUDA tensors on one device, got {[str(t.device) for t in tensors]}")
-    return device
-
-
-def call(device: int, function, *args) -> None:
-    """function(*args, stream) on the device's current stream, with the device current."""
-    if _current_device() == device:
-        rc = function(*args, _raw_stream(device))
-    else:
-        with torch.cuda.device(device):
-            rc = function(*args, _raw_stream(device))
-    if rc:
-        check(rc)
-
-
-def feature_rows(t, what: str):
-    """(t, row stride in elements) of a 2-D tensor of features whose rows are contiguous; a copy where they are not."""
-    if t.dim() != 2:
-        raise ValueError(f"{what} must be 2-D (rows x features), got {tuple(t.shape)}")
-    if t.dtype not in FLOAT_TYPES:
-        raise ValueError(f"{what} must be float32, float16 or bfloat16, got {t.dtype}")
-    rows, width = t.shape
-    if t.is_contiguous():
-        return t, width
-    stride = t.stride()
-    if width > 1 and stride[1] != 1:
-        return t.contiguous(), width
-    return t, stride[0] if rows > 1 else width
-
-
-def index_bytes(t, what: str) -> int:
-    """4 or 8 for an int32 or int64 tensor."""
-    if t.dtype == torch.int64:
-        return 8
-    if t.dtype == torch.int32:
-        return 4
-    raise ValueError(f"{what} must be int32 or int64, got {t.dtype}")
+def host():
+    """The compiled host path of the routing, lookup and clipping calls (csrc/host.cpp)."""
+    global _HOST
+    if _HOST is None:
+        load_library()
+        if not (HERE / "_host.so").exists():
+            raise HBError(HB_CUDA, "_host.so is not built; run __graft_entry__.build() (python hello-ot_b200/build.py)")
+        from . import _host
+        _HOST = _host
+    return _HOST
 
 
 class Workspace:

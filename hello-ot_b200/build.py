@@ -4,7 +4,9 @@
 
 Each CUDA source compiles to an object under hello-ot_b200/_build/ (in
 parallel) and the objects link into hello-ot_b200/libhello_b200.so with the
-CUDA runtime linked statically.  pdlp.cu is compiled without fma contraction
+CUDA runtime linked statically.  host.cpp, the host path of the routing, lookup
+and clipping calls, compiles with g++ against the installed torch into the
+extension module hello-ot_b200/_host.so, which links to the library.  pdlp.cu is compiled without fma contraction
 so the PDHG update arithmetic matches the reference operation by operation;
 exact.cu likewise, so its fp64 scores round like the written expressions.
 """
@@ -14,13 +16,16 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
+from importlib import metadata
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 BUILD = HERE / "_build"
 LIB = HERE / "libhello_b200.so"
+HOST = HERE / "_host.so"
 INCLUDE = HERE.parent / "include"
 SOURCES = ["abi.cu", "scan_l2sq.cu", "scan_norm.cu", "pairs.cu", "pdlp.cu", "support.cu", "exact.cu", "index_sort.cu",
            "routing.cu", "embedding.cu", "clip.cu"]
@@ -42,6 +47,30 @@ def _stale(target: Path, deps) -> bool:
         return True
     t = target.stat().st_mtime
     return any(Path(d).stat().st_mtime > t for d in deps)
+
+
+def build_host(force: bool = False, verbose: bool = False) -> Path:
+    """_host.so, again when its source, the C ABI or the installed torch changed."""
+    stamp = BUILD / "host.torch"
+    built_for = stamp.read_text() if stamp.exists() else ""
+    version = f"{metadata.version('torch')} python {sysconfig.get_python_version()}"
+    if not force and built_for == version and not _stale(HOST, [CSRC / "host.cpp", *INCLUDE.glob("*.h"), Path(__file__)]):
+        return HOST
+    import torch
+    where = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parent.parent / "include"
+    include = [where / "include", where / "include/torch/csrc/api/include", cuda, sysconfig.get_path("include")]
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", *(f"-I{d}" for d in include),
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", str(CSRC / "host.cpp"), "-o", str(HOST),
+           f"-L{where / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
+           f"-L{HERE}", "-l:" + LIB.name, "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("g++ failed:\n" + r.stdout + r.stderr)
+    stamp.write_text(version)
+    return HOST
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
@@ -78,6 +107,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError("link failed:\n" + r.stdout + r.stderr)
+    build_host(force, verbose)
     return LIB
 
 

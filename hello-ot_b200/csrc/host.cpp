@@ -1,0 +1,391 @@
+// Host path of the routing, lookup and clipping calls: argument checks, output allocation and the call of
+// the C ABI, as a Python extension module (hello_ot_b200._host).
+//
+// The kernels of a small call take 2 to 8 us, so what a user waits for is the host: through ctypes and
+// Python-level checks a call took 10 to 13 us, 3 of them the launch itself.  The functions here take the
+// tensors themselves and do the same in compiled code.  They hold no state; tensors and workspaces come
+// from torch's allocator on the current stream.  Shapes and types are refused with ValueError; errors of
+// the C ABI are raised by hello_ot_b200._lib.check.
+#include <algorithm>
+#include <initializer_list>
+#include <vector>
+
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/object_ptr.h>
+
+#include "../../include/hello_b200.h"
+
+namespace {
+
+using at::Tensor;
+
+// ---------------------------------------------------------------- arguments
+const Tensor& tensor(PyObject* o, const char* name) {
+    TORCH_CHECK_VALUE(THPVariable_Check(o), name, " must be a tensor");
+    return THPVariable_Unpack(o);
+}
+int64_t integer(PyObject* o) {
+    const int64_t v = PyLong_AsLongLong(o);
+    if (v == -1 && PyErr_Occurred()) throw python_error();
+    return v;
+}
+double number(PyObject* o) {
+    const double v = PyFloat_AsDouble(o);
+    if (v == -1.0 && PyErr_Occurred()) throw python_error();
+    return v;
+}
+void expect(Py_ssize_t got, Py_ssize_t want, const char* what) {
+    TORCH_CHECK_TYPE(got == want, what, " takes ", want, " arguments, got ", got);
+}
+PyObject* wrap(const Tensor& t) { return THPVariable_Wrap(t); }
+
+// A function of hello_ot_b200._lib, for the error paths alone.
+void call_lib(const char* name, PyObject* arg) {
+    THPObjectPtr module(PyImport_ImportModule("hello_ot_b200._lib"));
+    if (!module) throw python_error();
+    THPObjectPtr result(arg ? PyObject_CallMethod(module, name, "O", arg) : PyObject_CallMethod(module, name, nullptr));
+    if (!result) throw python_error();
+}
+void check(int rc) {
+    if (rc == HB_OK) return;
+    THPObjectPtr code(PyLong_FromLong(rc));
+    call_lib("check", code);
+}
+
+int type_or(at::ScalarType t, int otherwise) {
+    return t == at::kFloat ? HB_F32 : t == at::kHalf ? HB_F16 : t == at::kBFloat16 ? HB_BF16 : otherwise;
+}
+int type_of(const Tensor& t, const char* name) {
+    const int type = type_or(t.scalar_type(), -1);
+    TORCH_CHECK_VALUE(type >= 0, name, " must be float32, float16 or bfloat16, got ", t.scalar_type());
+    return type;
+}
+int index_bytes(const Tensor& t, const char* name) {
+    TORCH_CHECK_VALUE(t.scalar_type() == at::kLong || t.scalar_type() == at::kInt, name, " must be int32 or int64, got ",
+                      t.scalar_type());
+    return t.scalar_type() == at::kLong ? 8 : 4;
+}
+// The one CUDA device of all tensors.
+c10::Device device_of(const char* what, std::initializer_list<const Tensor*> tensors) {
+    const c10::Device device = (*tensors.begin())->device();
+    for (const Tensor* t : tensors)
+        if (!t->is_cuda() || t->device() != device) {
+            call_lib("lib", nullptr);  // without CUDA: the library's own error
+            TORCH_CHECK_VALUE(false, what, ": expected CUDA tensors on one device, got ", device, " and ", t->device());
+        }
+    return device;
+}
+
+// Features whose rows are contiguous (a copy where they are not) and the rows' distance in elements.
+struct Rows {
+    Tensor t;
+    int64_t stride;
+    int type;
+};
+Rows feature_rows(const Tensor& t, const char* name) {
+    TORCH_CHECK_VALUE(t.dim() == 2, name, " must be 2-D (rows x features), got ", t.sizes());
+    const int type = type_of(t, name);
+    const int64_t width = t.size(1);
+    if (t.is_contiguous()) return {t, width, type};
+    if (width > 1 && t.stride(1) != 1) return {t.contiguous(), width, type};
+    return {t, t.size(0) > 1 ? t.stride(0) : width, type};
+}
+
+// The device made current, its current stream, and a workspace on it.
+struct Launch {
+    c10::cuda::CUDAGuard guard;
+    void* stream;
+    explicit Launch(c10::Device d) : guard(d), stream(c10::cuda::getCurrentCUDAStream(d.index()).stream()) {}
+};
+Tensor workspace(size_t bytes, c10::Device device) {
+    return at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(device));
+}
+
+// ---------------------------------------------------------------- routing
+struct Places {
+    const Tensor &position, &offsets;
+    int64_t tokens, slots;
+    const int32_t* at() const { return position.const_data_ptr<int32_t>(); }
+    const int32_t* kept() const { return offsets.const_data_ptr<int32_t>() + offsets.numel() - 1; }
+};
+Places places(PyObject* position, PyObject* offsets, const char* what) {
+    const Tensor &p = tensor(position, "position"), &o = tensor(offsets, "offsets");
+    TORCH_CHECK_VALUE(p.scalar_type() == at::kInt && o.scalar_type() == at::kInt && p.dim() == 2 && o.dim() == 1, what,
+                      ": a plan holds int32 position [tokens, slots] and offsets [num_experts + 1]");
+    TORCH_CHECK_VALUE(p.is_contiguous() && o.is_contiguous() && o.numel() >= 2 && p.size(1) >= 1, what,
+                      ": a plan's tensors are contiguous, with at least one slot and one expert");
+    return {p, o, p.size(0), p.size(1)};
+}
+Tensor weights_of(PyObject* w, const Places& p, const char* what) {
+    const Tensor& t = tensor(w, "weights");
+    type_of(t, "weights");
+    TORCH_CHECK_VALUE(t.sizes() == p.position.sizes() || (t.dim() == 1 && p.slots == 1 && t.size(0) == p.tokens), what,
+                      ": weights ", t.sizes(), " do not fit an assignment ", p.position.sizes());
+    return t.contiguous();
+}
+
+// route_plan(index, num_experts) -> (order, position, offsets)
+PyObject* route_plan(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 2, "route_plan");
+    const Tensor& given = tensor(args[0], "index");
+    TORCH_CHECK_VALUE(given.dim() == 1 || (given.dim() == 2 && given.size(1) >= 1),
+                      "index must be [tokens] or [tokens, slots], got ", given.sizes());
+    const int bytes = index_bytes(given, "index");
+    const int64_t experts = integer(args[1]), entries = given.numel();
+    TORCH_CHECK_VALUE(experts >= 1 && experts < INT32_MAX, "num_experts must be positive and below 2^31 - 1");
+    TORCH_CHECK_VALUE(entries <= INT32_MAX, "an assignment holds at most 2^31 - 1 entries");
+    const c10::Device device = device_of("route_plan", {&given});
+    const Tensor index = given.contiguous();
+    const auto options = at::TensorOptions().dtype(at::kInt).device(device);
+    Tensor order = at::empty({entries}, options), offsets = at::empty({experts + 1}, options);
+    Tensor position = at::empty({index.size(0), index.dim() == 2 ? index.size(1) : 1}, options);
+    const size_t size = hb_index_sort_workspace(entries, experts);
+    Tensor ws;
+    if (size) ws = workspace(size, device);
+    const Launch on(device);
+    check(hb_index_sort(index.const_data_ptr(), bytes, entries, experts, order.data_ptr<int32_t>(),
+                        position.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(), size ? ws.data_ptr() : nullptr, size,
+                        on.stream));
+    THPObjectPtr result(PyTuple_New(3));
+    if (!result) throw python_error();
+    PyTuple_SET_ITEM(result.get(), 0, wrap(order));
+    PyTuple_SET_ITEM(result.get(), 1, wrap(position));
+    PyTuple_SET_ITEM(result.get(), 2, wrap(offsets));
+    return result.release();
+    END_HANDLE_TH_ERRORS
+}
+
+// route_dispatch(x, position, offsets) -> sorted
+PyObject* route_dispatch(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 3, "route_dispatch");
+    const Rows x = feature_rows(tensor(args[0], "x"), "x");
+    const Places p = places(args[1], args[2], "route_dispatch");
+    TORCH_CHECK_VALUE(x.t.size(0) == p.tokens, "route_dispatch: x has ", x.t.size(0), " rows for ", p.tokens, " tokens");
+    const c10::Device device = device_of("route_dispatch", {&x.t, &p.position, &p.offsets});
+    Tensor out = at::empty({p.tokens * p.slots, x.t.size(1)}, x.t.options());
+    const Launch on(device);
+    check(hb_route_dispatch(x.type, x.t.const_data_ptr(), x.stride, p.tokens, p.slots, x.t.size(1), p.at(), p.kept(),
+                            out.data_ptr(), on.stream));
+    return wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// route_combine(z, position, offsets, weights or None, name) -> combined
+PyObject* route_combine(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 5, "route_combine");
+    const char* what = PyUnicode_AsUTF8(args[4]);
+    if (!what) throw python_error();
+    const Rows z = feature_rows(tensor(args[0], "z"), "z");
+    const Places p = places(args[1], args[2], what);
+    TORCH_CHECK_VALUE(z.t.size(0) == p.tokens * p.slots, what, ": ", z.t.size(0), " sorted rows for ", p.tokens, " x ",
+                      p.slots, " entries");
+    Tensor weights;
+    if (args[3] != Py_None) weights = weights_of(args[3], p, what);
+    const bool weighted = weights.defined();
+    const c10::Device device = device_of(what, {&z.t, &p.position, &p.offsets, weighted ? &weights : &z.t});
+    Tensor out = at::empty({p.tokens, z.t.size(1)}, z.t.options());
+    const Launch on(device);
+    check(hb_route_combine(z.type, z.t.const_data_ptr(), z.stride, p.tokens, p.slots, z.t.size(1), p.at(), p.kept(),
+                           weighted ? weights.const_data_ptr() : nullptr, weighted ? type_of(weights, "weights") : 0,
+                           out.data_ptr(), on.stream));
+    return wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// route_combine_grad(dy, z, position, offsets, weights or None, need_weights) -> (dz, dweights or None)
+PyObject* route_combine_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const char* what = "route_combine_grad";
+    expect(n, 6, what);
+    const Rows dy = feature_rows(tensor(args[0], "dy"), "dy"), z = feature_rows(tensor(args[1], "z"), "z");
+    const Places p = places(args[2], args[3], what);
+    const int64_t width = z.t.size(1);
+    TORCH_CHECK_VALUE(dy.t.size(0) == p.tokens && dy.t.size(1) == width && z.t.size(0) == p.tokens * p.slots &&
+                          dy.type == z.type,
+                      what, ": dy ", dy.t.sizes(), " ", dy.t.scalar_type(), " and z ", z.t.sizes(), " ", z.t.scalar_type(),
+                      " do not fit an assignment ", p.position.sizes());
+    Tensor weights, dw;
+    if (args[4] != Py_None) weights = weights_of(args[4], p, what);
+    const bool weighted = weights.defined();
+    const c10::Device device = device_of(what, {&z.t, &dy.t, &p.position, &p.offsets, weighted ? &weights : &z.t});
+    if (weighted && args[5] == Py_True) dw = at::empty_like(weights);
+    Tensor dz = at::empty({p.tokens * p.slots, width}, z.t.options());
+    const Launch on(device);
+    check(hb_route_combine_grad(z.type, dy.t.const_data_ptr(), dy.stride, z.t.const_data_ptr(), z.stride, p.tokens, p.slots,
+                                width, p.at(), p.kept(), weighted ? weights.const_data_ptr() : nullptr,
+                                weighted ? type_of(weights, "weights") : 0, dz.data_ptr(),
+                                dw.defined() ? dw.data_ptr() : nullptr, on.stream));
+    THPObjectPtr result(PyTuple_New(2));
+    if (!result) throw python_error();
+    PyTuple_SET_ITEM(result.get(), 0, wrap(dz));
+    PyTuple_SET_ITEM(result.get(), 1, wrap(dw));  // None when undefined
+    return result.release();
+    END_HANDLE_TH_ERRORS
+}
+
+// ---------------------------------------------------------------- embedding
+// embedding_lookup(table, ids, scale) -> rows
+PyObject* embedding_lookup(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 3, "embedding_lookup");
+    const Tensor& given = tensor(args[1], "ids");
+    const int bytes = index_bytes(given, "ids");
+    const Rows table = feature_rows(tensor(args[0], "table"), "table");
+    const c10::Device device = device_of("embedding_lookup", {&table.t, &given});
+    TORCH_CHECK_VALUE(given.numel() <= INT32_MAX, "embedding_lookup: at most 2^31 - 1 ids");
+    const Tensor ids = given.contiguous();
+    c10::SmallVector<int64_t, 8> shape(ids.sizes().begin(), ids.sizes().end());
+    shape.push_back(table.t.size(1));
+    Tensor out = at::empty(shape, table.t.options());
+    const Launch on(device);
+    check(hb_embedding_lookup(table.type, table.t.const_data_ptr(), table.stride, table.t.size(0), table.t.size(1),
+                              ids.const_data_ptr(), bytes, ids.numel(), number(args[2]), out.data_ptr(), on.stream));
+    return wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// embedding_grad(dy, ids, rows, scale, dtype or None, out or None, accumulate) -> gradient
+PyObject* embedding_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const char* what = "embedding_grad";
+    expect(n, 7, what);
+    const Tensor &dy_given = tensor(args[0], "dy"), &given = tensor(args[1], "ids");
+    const int bytes = index_bytes(given, "ids");
+    const int64_t count = given.numel(), rows = integer(args[2]);
+    TORCH_CHECK_VALUE(dy_given.dim() >= 1 && dy_given.sizes().slice(0, dy_given.dim() - 1) == given.sizes(), what, ": dy ",
+                      dy_given.sizes(), " does not fit ids ", given.sizes());
+    const int64_t width = dy_given.size(-1);
+    TORCH_CHECK_VALUE(rows >= 1 && rows < INT32_MAX, what, ": rows must be positive and below 2^31 - 1");
+    TORCH_CHECK_VALUE(count <= INT32_MAX, what, ": at most 2^31 - 1 ids");
+    Rows dy = feature_rows(dy_given.dim() == 2 ? dy_given : dy_given.reshape({count, width}), "dy");
+    if (dy.stride * dy.t.element_size() > (int64_t)UINT32_MAX) dy = {dy.t.contiguous(), width, dy.type};
+    const bool accumulate = args[6] == Py_True;
+    Tensor out;
+    if (args[5] != Py_None) out = tensor(args[5], "out");
+    at::ScalarType type = out.defined() ? out.scalar_type() : dy.t.scalar_type();
+    if (args[4] != Py_None) {
+        TORCH_CHECK_VALUE(THPDtype_Check(args[4]), what, ": dtype must be a torch.dtype");
+        type = reinterpret_cast<THPDtype*>(args[4])->scalar_type;
+    }
+    TORCH_CHECK_VALUE(type == dy.t.scalar_type() || type == at::kFloat, what, ": the gradient of ", dy.t.scalar_type(),
+                      " rows is ", dy.t.scalar_type(), " or float32, not ", type);
+    TORCH_CHECK_VALUE(out.defined() || !accumulate, what, ": accumulate needs out");
+    const c10::Device device = device_of(what, {&dy.t, &given, out.defined() ? &out : &dy.t});
+    if (!out.defined())
+        out = at::empty({rows, width}, dy.t.options().dtype(type));
+    else
+        TORCH_CHECK_VALUE(out.scalar_type() == type && out.dim() == 2 && out.size(0) == rows && out.size(1) == width &&
+                              out.is_contiguous(),
+                          what, ": out must be a contiguous ", type, " tensor of shape [", rows, ", ", width, "]");
+    const Tensor ids = given.contiguous();
+    const size_t size = hb_embedding_grad_workspace(count, rows, width);
+    Tensor ws = workspace(size, device);
+    const Launch on(device);
+    check(hb_embedding_grad(dy.type, dy.t.const_data_ptr(), dy.stride, ids.const_data_ptr(), bytes, count, rows, width,
+                            number(args[3]), type_or(type, HB_F32), out.data_ptr(), accumulate, ws.data_ptr(), size,
+                            on.stream));
+    return wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// ---------------------------------------------------------------- clipping
+struct List {
+    std::vector<Tensor> tensors;
+    std::vector<void*> address;
+    std::vector<int64_t> size;
+    std::vector<int32_t> type;
+};
+// A list of float tensors on one device, each dense in memory and listed once.
+List list_of(PyObject* o, const char* what, c10::Device* device) {
+    THPObjectPtr items(PySequence_Fast(o, "gradients must be a list of tensors"));
+    if (!items) throw python_error();
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(items.get());
+    List l;
+    l.tensors.reserve(n), l.address.reserve(n), l.size.reserve(n), l.type.reserve(n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        const Tensor& t = tensor(PySequence_Fast_GET_ITEM(items.get(), i), "a gradient");
+        if (i == 0 && !device->is_cuda()) *device = device_of(what, {&t});
+        if (t.device() != *device) device_of(what, {&t, i > 0 ? &l.tensors[0] : &t});
+        TORCH_CHECK_VALUE(t.device() == *device, what, ": outputs on another device than their gradients");
+        l.type.push_back(type_of(t, "gradients"));
+        TORCH_CHECK_VALUE(t.is_contiguous() || t.is_non_overlapping_and_dense(), what,
+                          ": gradients must be dense in memory, got strides ", t.strides(), " for ", t.sizes());
+        l.tensors.push_back(t);
+        l.size.push_back(t.numel());
+        l.address.push_back(t.numel() ? t.data_ptr() : nullptr);
+    }
+    std::vector<void*> sorted(l.address);
+    std::sort(sorted.begin(), sorted.end());
+    for (size_t i = 1; i < sorted.size(); ++i)
+        TORCH_CHECK_VALUE(!sorted[i] || sorted[i] != sorted[i - 1], what, ": a tensor is listed twice");
+    return l;
+}
+
+// clip(gradients, limit or None, outputs or None, name) -> norm
+PyObject* clip(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 4, "clip");
+    const char* what = PyUnicode_AsUTF8(args[3]);
+    if (!what) throw python_error();
+    c10::Device device(c10::kCPU);
+    const List grads = list_of(args[0], what, &device);
+    const int64_t count = (int64_t)grads.tensors.size();
+    TORCH_CHECK_VALUE(count > 0, what, ": no gradients");
+    const bool scale = args[1] != Py_None;
+    const double limit = scale ? number(args[1]) : 0.0;
+    TORCH_CHECK_VALUE(limit >= 0.0, what, ": max_norm must be a number >= 0, got ", limit);
+    List outs;
+    const List* to = &grads;
+    if (args[2] != Py_None) {
+        outs = list_of(args[2], what, &device);
+        to = &outs;
+        TORCH_CHECK_VALUE(outs.tensors.size() == grads.tensors.size(), what, ": ", outs.tensors.size(), " outputs for ",
+                          count, " gradients");
+        for (int64_t i = 0; i < count; ++i) {
+            const Tensor &g = grads.tensors[i], &o = outs.tensors[i];
+            TORCH_CHECK_VALUE(o.sizes() == g.sizes(), what, ": outputs have their gradients' shapes, got ", o.sizes(), " for ",
+                              g.sizes());
+            TORCH_CHECK_VALUE((o.is_contiguous() && g.is_contiguous()) || o.strides() == g.strides(), what,
+                              ": outputs have their gradients' strides");
+            TORCH_CHECK_VALUE(outs.type[i] == grads.type[i] ||
+                                  (outs.type[i] == HB_F32 && (!outs.address[i] || outs.address[i] != grads.address[i])),
+                              what, ": an output has its gradient's type, or is float32 and not in place; got ",
+                              o.scalar_type(), " for ", g.scalar_type());
+        }
+    }
+    Tensor norm = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(device));
+    const size_t size = hb_clip_workspace(count);
+    Tensor ws = workspace(size, device);
+    const Launch on(device);
+    if (scale)
+        check(hb_clip_grad_norm(count, grads.address.data(), grads.size.data(), grads.type.data(), to->address.data(),
+                                to->type.data(), limit, norm.data_ptr<float>(), ws.data_ptr(), size, on.stream));
+    else
+        check(hb_grad_norm(count, grads.address.data(), grads.size.data(), grads.type.data(), norm.data_ptr<float>(),
+                           ws.data_ptr(), size, on.stream));
+    return wrap(norm);
+    END_HANDLE_TH_ERRORS
+}
+
+PyMethodDef methods[] = {
+    {"route_plan", reinterpret_cast<PyCFunction>(route_plan), METH_FASTCALL, nullptr},
+    {"route_dispatch", reinterpret_cast<PyCFunction>(route_dispatch), METH_FASTCALL, nullptr},
+    {"route_combine", reinterpret_cast<PyCFunction>(route_combine), METH_FASTCALL, nullptr},
+    {"route_combine_grad", reinterpret_cast<PyCFunction>(route_combine_grad), METH_FASTCALL, nullptr},
+    {"embedding_lookup", reinterpret_cast<PyCFunction>(embedding_lookup), METH_FASTCALL, nullptr},
+    {"embedding_grad", reinterpret_cast<PyCFunction>(embedding_grad), METH_FASTCALL, nullptr},
+    {"clip", reinterpret_cast<PyCFunction>(clip), METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr}};
+PyModuleDef definition = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__host() { return PyModule_Create(&definition); }

@@ -19,7 +19,7 @@ from typing import NamedTuple
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._lib import FLOAT_TYPES, call, device_of, feature_rows, index_bytes, load_library
+from ._lib import host
 
 
 class RoutePlan(NamedTuple):
@@ -53,119 +53,25 @@ class RoutePlan(NamedTuple):
 
 def route_plan(index, num_experts: int) -> RoutePlan:
     """Stable sort of an assignment ``index`` ([tokens] or [tokens, slots], int32 or int64) by expert."""
-    if index.dim() not in (1, 2) or (index.dim() == 2 and index.shape[1] < 1):
-        raise ValueError(f"index must be [tokens] or [tokens, slots], got {tuple(index.shape)}")
-    size = index_bytes(index, "index")
-    num_experts = int(num_experts)
-    if not 1 <= num_experts < 2 ** 31 - 1:
-        raise ValueError("num_experts must be positive and below 2^31 - 1")
-    n = index.numel()
-    if n >= 2 ** 31:
-        raise ValueError("an assignment holds at most 2^31 - 1 entries")
-    device = device_of("route_plan", index)
-    index = index.contiguous()
-    L = load_library()
-    int32 = torch.int32
-    order = index.new_empty(n, dtype=int32)
-    position = index.new_empty((index.shape[0], 1 if index.dim() == 1 else index.shape[1]), dtype=int32)
-    offsets = index.new_empty(num_experts + 1, dtype=int32)
-    nbytes = L.hb_index_sort_workspace(n, num_experts)
-    ws = index.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    call(device, L.hb_index_sort, index.data_ptr(), size, n, num_experts, order.data_ptr(), position.data_ptr(),
-         offsets.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
-    return RoutePlan(order, position, offsets)
-
-
-def _places(plan, what: str):
-    """(position, address of the number of entries with an expert) of a checked plan."""
-    _, position, offsets = plan
-    int32 = torch.int32
-    if position.dtype != int32 or offsets.dtype != int32 or position.dim() != 2 or offsets.dim() != 1:
-        raise ValueError(f"{what}: a plan holds int32 position [tokens, slots] and offsets [num_experts + 1]")
-    ends = offsets.numel()
-    if not position.is_contiguous() or not offsets.is_contiguous() or ends < 2 or position.size(1) < 1:
-        raise ValueError(f"{what}: a plan's tensors are contiguous, with at least one slot and one expert")
-    return position, offsets.data_ptr() + 4 * (ends - 1)
-
-
-def _weights(weights, position, what: str):
-    if weights.dtype not in FLOAT_TYPES:
-        raise ValueError(f"{what}: weights must be float32, float16 or bfloat16, got {weights.dtype}")
-    if weights.shape != position.shape and (weights.shape != position.shape[:1] or position.size(1) != 1):
-        raise ValueError(f"{what}: weights {tuple(weights.shape)} do not fit an assignment {tuple(position.shape)}")
-    return weights.contiguous()
-
-
-def _dispatch(x, plan):
-    x, stride = feature_rows(x, "x")
-    position, kept = _places(plan, "route_dispatch")
-    tokens, slots = position.shape
-    if x.shape[0] != tokens:
-        raise ValueError(f"route_dispatch: x has {x.shape[0]} rows for {tokens} tokens")
-    device = device_of("route_dispatch", x, position, plan.offsets)
-    width = x.shape[1]
-    out = x.new_empty((tokens * slots, width))
-    call(device, load_library().hb_route_dispatch, FLOAT_TYPES[x.dtype], x.data_ptr(), stride, tokens, slots, width,
-         position.data_ptr(), kept, out.data_ptr())
-    return out
-
-
-def _combine(z, plan, weights, what="route_combine"):
-    z, stride = feature_rows(z, "z")
-    position, kept = _places(plan, what)
-    tokens, slots = position.shape
-    if z.shape[0] != tokens * slots:
-        raise ValueError(f"{what}: {z.shape[0]} sorted rows for {tokens} x {slots} entries")
-    if weights is None:
-        device, wptr, wtype = device_of(what, z, position, plan.offsets), None, 0
-    else:
-        weights = _weights(weights, position, what)
-        device = device_of(what, z, position, plan.offsets, weights)
-        wptr, wtype = weights.data_ptr(), FLOAT_TYPES[weights.dtype]
-    width = z.shape[1]
-    out = z.new_empty((tokens, width))
-    call(device, load_library().hb_route_combine, FLOAT_TYPES[z.dtype], z.data_ptr(), stride, tokens, slots, width,
-         position.data_ptr(), kept, wptr, wtype, out.data_ptr())
-    return out
+    return RoutePlan(*host().route_plan(index, num_experts))
 
 
 def route_dispatch_grad(dsorted, plan):
     """Gradient of ``route_dispatch`` with respect to x: each token's sorted rows added up."""
-    return _combine(dsorted, plan, None, "route_dispatch_grad")
+    return host().route_combine(dsorted, plan[1], plan[2], None, "route_dispatch_grad")
 
 
 def route_combine_grad(dy, z, plan, weights=None, *, need_weights: bool = True):
     """Gradients of ``route_combine`` with respect to z and weights, as (dz, dweights); dweights is None
     without weights or with ``need_weights=False``."""
-    what = "route_combine_grad"
-    dy, dy_stride = feature_rows(dy, "dy")
-    z, z_stride = feature_rows(z, "z")
-    position, kept = _places(plan, what)
-    tokens, slots = position.shape
-    if dy.shape != (tokens, z.shape[1]) or z.shape[0] != tokens * slots or dy.dtype != z.dtype:
-        raise ValueError(f"{what}: dy {tuple(dy.shape)} {dy.dtype} and z {tuple(z.shape)} {z.dtype} do not fit an "
-                         f"assignment {tuple(position.shape)}")
-    dw, wptr, wtype = None, None, 0
-    if weights is None:
-        device = device_of(what, dy, z, position, plan.offsets)
-    else:
-        weights = _weights(weights, position, what)
-        device = device_of(what, dy, z, position, plan.offsets, weights)
-        wptr, wtype = weights.data_ptr(), FLOAT_TYPES[weights.dtype]
-        if need_weights:
-            dw = torch.empty_like(weights)
-    dz = z.new_empty((tokens * slots, z.shape[1]))
-    call(device, load_library().hb_route_combine_grad, FLOAT_TYPES[z.dtype], dy.data_ptr(), dy_stride, z.data_ptr(),
-         z_stride, tokens, slots, z.shape[1], position.data_ptr(), kept, wptr, wtype, dz.data_ptr(),
-         None if dw is None else dw.data_ptr())
-    return dz, dw
+    return host().route_combine_grad(dy, z, plan[1], plan[2], weights, bool(need_weights))
 
 
 class _Dispatch(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, plan):
         ctx.plan = plan
-        return _dispatch(x, plan)
+        return host().route_dispatch(x, plan[1], plan[2])
 
     @staticmethod
     @once_differentiable
@@ -178,7 +84,7 @@ class _Combine(torch.autograd.Function):
     def forward(ctx, z, plan, weights):
         ctx.plan = plan
         ctx.save_for_backward(z, weights)
-        return _combine(z, plan, weights)
+        return host().route_combine(z, plan[1], plan[2], weights, "route_combine")
 
     @staticmethod
     @once_differentiable
@@ -193,7 +99,7 @@ def route_dispatch(x, plan):
     an expert.  Differentiable in x."""
     if x.requires_grad and torch.is_grad_enabled():
         return _Dispatch.apply(x, plan)
-    return _dispatch(x, plan)
+    return host().route_dispatch(x, plan[1], plan[2])
 
 
 def route_combine(z, plan, weights=None):
@@ -201,7 +107,7 @@ def route_combine(z, plan, weights=None):
     when there are none.  Differentiable in z and weights."""
     if torch.is_grad_enabled() and (z.requires_grad or (weights is not None and weights.requires_grad)):
         return _Combine.apply(z, plan, weights)
-    return _combine(z, plan, weights)
+    return host().route_combine(z, plan[1], plan[2], weights, "route_combine")
 
 
 def assignment_of_plan(rows, cols, mass, tokens: int, *, tolerance: float = 0.0, device=None):
