@@ -200,19 +200,21 @@ __device__ __forceinline__ void group_sum(float (&v)[B]) {
 }
 
 // Wide rows: a group goes through a token's entries, 4 vectors a thread (8 of 4 bytes, 16 of 2) of z and of dy,
-// which is in L1 after the first entry.
+// which is in L1 after the first entry.  ways: groups a token, 1, or one an entry when tokens are few.
 template <typename T, int VB, int G>
-__global__ void __launch_bounds__(256) combine_grad_kernel(Moves m, const T* __restrict__ dy, int64_t dy_stride,
+__global__ void __launch_bounds__(256) combine_grad_kernel(Moves m, int ways, const T* __restrict__ dy, int64_t dy_stride,
                                                            const T* __restrict__ z, int64_t z_stride,
                                                            const void* __restrict__ weights, int weight_type,
                                                            T* __restrict__ dz, void* __restrict__ dw) {
     using V = Vec<T, VB>;
     constexpr int U = VB >= 8 ? 4 : VB == 4 ? 8 : 16;
-    const int64_t token = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const int64_t group = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const int64_t token = ways == 1 ? group : group / ways;
     if (token >= m.tokens) return;  // G = 256: the whole block or none of it
     const uint32_t kept = kept_entries(m);
     const T* grow = dy + token * dy_stride;
-    for (int k = 0; k < m.slots; ++k) {
+    const int first = ways == 1 ? 0 : (int)(group % ways), last = ways == 1 ? m.slots : first + 1;
+    for (int k = first; k < last; ++k) {
         const int64_t e = token * m.slots + k;
         const uint32_t p = (uint32_t)m.position[e];
         const bool there = p < kept;
@@ -460,7 +462,9 @@ extern "C" int hb_route_combine_grad(int type, const void* dy, int64_t dy_stride
     if (bits % size) return abi_fail(HB_BAD_ARGUMENT, "route combine gradient: misaligned pointer");
     const int vb = rows::vector_bytes(bits, type);
     const int64_t vectors = width * size / vb;
-    const int g = group_of(tokens, vectors, vb);
+    // too few tokens to fill the SMs with a warp each: a group an entry
+    const int ways = tokens < 148 * 32 ? (int)slots : 1;
+    const int g = group_of(tokens * ways, vectors, vb);
     const auto st = static_cast<cudaStream_t>(stream);
     rows::for_type(type, vb, [&](auto t, auto b) {
         using T = decltype(t);
@@ -475,8 +479,8 @@ extern "C" int hb_route_combine_grad(int type, const void* dy, int64_t dy_stride
                 }
             }
             if constexpr (G > 8)
-                combine_grad_kernel<T, VB, G><<<blocks_of(tokens, G), 256, 0, st>>>(
-                    m, static_cast<const T*>(dy), dy_stride, static_cast<const T*>(z), z_stride, weights, weight_type,
+                combine_grad_kernel<T, VB, G><<<blocks_of(tokens * ways, G), 256, 0, st>>>(
+                    m, ways, static_cast<const T*>(dy), dy_stride, static_cast<const T*>(z), z_stride, weights, weight_type,
                     static_cast<T*>(dz), dweights);
         });
     });
