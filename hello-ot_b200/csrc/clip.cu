@@ -29,8 +29,8 @@
 namespace hb {
 namespace clip {
 
-constexpr int kThreads = 256, kSmallThreads = 1024;
-constexpr int64_t kChunk = 8192, kSmallChunk = 16384;  // elements; 4 loads a thread of fp32
+constexpr int kThreads = 256, kSmallThreads = 512;
+constexpr int64_t kChunk = 8192, kSmallChunk = 8192;  // elements; small: 4 loads a thread of fp32
 constexpr int64_t kSmallMost = 1 << 19;               // elements of the one-launch form
 constexpr int kCluster = 16;
 constexpr int64_t kLargeLeast = 1 << 23;              // elements from which a block scales one chunk

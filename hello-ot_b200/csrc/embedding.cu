@@ -348,23 +348,31 @@ __device__ __forceinline__ void sum_chunk(const Grad<T, TO>& g, int64_t block) {
         join_run<T, TO, N>(g, key, chunk, last_chunk(g, key, chunk), chunk, tile, c, mine, completes + threadIdx.y);
 }
 
-// Zeros of the rows that no sorted place holds: a lane searches a row, then the warp writes.
+// Zeros of the rows that no sorted place holds: a lane searches a row, then the warp writes.  The search is in
+// shared memory where the places fit there: its steps wait for one another, and from L2 they take most of the
+// time of a small call.
+constexpr int kStaged = 2048;
 template <typename T, typename TO>
 __device__ __forceinline__ void zero_rows(const Grad<T, TO>& g, int64_t block) {
-    const int t = threadIdx.y * blockDim.x + threadIdx.x, lane = t & 31;
-    const int warps = (blockDim.x * blockDim.y) >> 5;
-    if ((t >> 5) >= warps) return;
-    const int64_t first = (block * warps + (t >> 5)) * g.rows_per_warp;
+    __shared__ uint32_t staged[kStaged];
+    const int threads = blockDim.x * blockDim.y, t = threadIdx.y * blockDim.x + threadIdx.x, lane = t & 31;
+    const int64_t first = (block * (threads >> 5) + (t >> 5)) * g.rows_per_warp;
     const int64_t row = first + lane;
+    const bool small = g.n <= kStaged;
+    if (small) {
+#pragma unroll 4
+        for (int i = t; i < g.n; i += threads) staged[i] = g.pairs[i].x;
+        __syncthreads();
+    }
     bool empty = lane < g.rows_per_warp && row < g.rows;
     if (empty) {
         int64_t lo = 0, hi = g.n;
         while (lo < hi) {
             const int64_t mid = (lo + hi) >> 1;
-            if (g.pairs[mid].x < (uint32_t)row) lo = mid + 1;
+            if ((small ? staged[mid] : g.pairs[mid].x) < (uint32_t)row) lo = mid + 1;
             else hi = mid;
         }
-        empty = lo >= g.n || g.pairs[lo].x != (uint32_t)row;
+        empty = lo >= g.n || (small ? staged[lo] : g.pairs[lo].x) != (uint32_t)row;
     }
     for (unsigned left = __ballot_sync(0xffffffffu, empty); left; left &= left - 1) {
         TO* to = g.out + (first + __ffs(left) - 1) * g.width;
@@ -385,15 +393,16 @@ __global__ void __launch_bounds__(256, 3) grad_kernel(const Grad<T, TO> g) {
     else zero_rows(g, blockIdx.x - g.sum_blocks);
 }
 
-// Threads a row: a power of two up to 32 vectors, else whole warps, at most 256 a column tile.
+// Threads a row: a power of two up to 32 vectors, else whole warps, at most 256 a column tile.  Up to 32768
+// tokens a warp at least: groups that share a warp take their turns wherever their rows end differently.
 struct Shape {
     int group, groups, tiles;
 };
-inline Shape shape_of(int64_t vectors) {
+inline Shape shape_of(int64_t n, int64_t vectors) {
     Shape s{};
     s.tiles = (int)((vectors + 255) / 256);
     if (vectors <= 32) {
-        s.group = 1;
+        s.group = n <= 32768 ? 32 : 1;
         while (s.group < vectors) s.group <<= 1;
     } else {
         s.group = (int)(((vectors + s.tiles - 1) / s.tiles + 31) / 32 * 32);
@@ -433,17 +442,17 @@ inline Layout layout(void* ws, int64_t n, int64_t rows_, int64_t width) {
     l.pairs = reinterpret_cast<uint2*>(take(sizeof(uint2) * n));
     l.sort_bytes = index_sort_bytes(n, rows_);
     l.sort = take(l.sort_bytes);
-    const int chunk = chunk_of(n, shape_of((width + 7) / 8));
+    const int chunk = chunk_of(n, shape_of(n, (width + 7) / 8));
     const int64_t chunks = (n + chunk - 1) / chunk;
     l.partial = reinterpret_cast<float*>(take(sizeof(float) * 2 * width * chunks));
-    l.arrivals = chunks * 3 * shape_of(width).tiles;
+    l.arrivals = chunks * 3 * shape_of(n, width).tiles;
     l.arrived = reinterpret_cast<uint32_t*>(take(sizeof(uint32_t) * l.arrivals));
     return l;
 }
 
 template <typename T, typename TO, int VB>
 cudaError_t run_grad(Grad<T, TO> g, cudaStream_t st) {
-    const Shape s = shape_of(g.width * (int64_t)sizeof(T) / VB);
+    const Shape s = shape_of(g.n, g.width * (int64_t)sizeof(T) / VB);
     const dim3 block(s.group, s.groups);
     g.tiles = s.tiles;
     g.chunk = chunk_of(g.n, s);

@@ -37,8 +37,8 @@ namespace isort {
 constexpr int kThreads = 1024, kWarps = kThreads / 32;     // a tile's block
 constexpr int kBlock = 1024, kBlockWarps = kBlock / 32;     // a cluster's block
 constexpr int kRounds = 2;                                  // entries a thread of a cluster
-constexpr int kRankMost = 2048, kRankThreads = 256;         // sort by comparing
-constexpr int kRankSlices = 4, kRankQueries = kRankThreads / kRankSlices;
+constexpr int kRankMost = 2048, kRankThreads = 512;         // sort by comparing
+constexpr int kRankSlices = 8, kRankQueries = kRankThreads / kRankSlices;
 constexpr int64_t kRankBins = 4096;                         // most bins whose offsets it finds
 constexpr int kMostClusters = 16;
 constexpr int64_t kClusterMost = (int64_t)kMostClusters * kBlock * kRounds;
@@ -58,7 +58,7 @@ struct Source {
 };
 
 // Places of the entries, and the offsets, each a count of the keys below: of key k at entry i the keys <= k before
-// i and those < k after it, of offset b the keys < b.  64 queries a block, 4 threads a query, each over a quarter of
+// i and those < k after it, of offset b the keys < b.  64 queries a block, 8 threads a query, each over an eighth of
 // the keys in shared memory, where a warp reads the same 16 bytes in all its lanes.
 __global__ void __launch_bounds__(kRankThreads) sort_rank(Source src, int n, int entry_blocks, int32_t* __restrict__ order,
                                                           int32_t* __restrict__ position, uint2* __restrict__ pairs,
@@ -70,7 +70,17 @@ __global__ void __launch_bounds__(kRankThreads) sort_rank(Source src, int n, int
     for (int64_t i = (int64_t)blockIdx.x * kRankThreads + threadIdx.x; i < zeros; i += (int64_t)gridDim.x * kRankThreads)
         zero[i] = 0;
     const int slice_keys = (n + kRankSlices * 4 - 1) / (kRankSlices * 4) * 4;  // whole vectors
-    for (int i = threadIdx.x; i < slice_keys * kRankSlices; i += kRankThreads) keys[i] = i < n ? src.entry(i).x : 0xffffffffu;
+    uint32_t own[kRankMost / kRankThreads];  // all loads before the first store
+#pragma unroll
+    for (int r = 0; r < kRankMost / kRankThreads; ++r) {
+        const int i = r * kRankThreads + threadIdx.x;
+        own[r] = i < n ? src.entry(i).x : 0xffffffffu;
+    }
+#pragma unroll
+    for (int r = 0; r < kRankMost / kRankThreads; ++r) {
+        const int i = r * kRankThreads + threadIdx.x;
+        if (i < slice_keys * kRankSlices) keys[i] = own[r];
+    }
     __syncthreads();
     const int query = threadIdx.x % kRankQueries, slice = threadIdx.x / kRankQueries;
     const bool entries = (int)blockIdx.x < entry_blocks;
