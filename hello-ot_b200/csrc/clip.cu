@@ -10,8 +10,11 @@
 // time is launches: one cluster of blocks does both steps in one, with its hardware
 // barrier between them.  Above 8 million the second launch has a block a chunk: blocks
 // that start in the order of memory keep HBM's pages open, where resident blocks that
-// stride through it drift apart (1.6 GB copied and scaled: 464 us against 541).  The
+// stride through it drift apart (1.6 GB copied and scaled: 471 us against 541).  The
 // norm is then a launch of its own, so that a block begins with its loads.
+//
+// Measured on a B200: 800 million bf16 values 705 us (2 reads and a write: 6.8 TB/s), their
+// norm alone 233 us (6.9 TB/s); 200 thousand f32 values in one tensor 6 us.
 //
 // Squares are added in fp32 over at most 32 values and in fp64 from there on.  A
 // group whose fp32 sum is so small or so large that squares were lost or overflowed

@@ -23,6 +23,10 @@
 //                        launches overlap (the first pass ranks while it is counted)
 //   above                tiles of 4096 and three launches a pass, the counts scanned
 //                        over the tiles by a launch of their own
+//
+// Measured on a B200 (us): 2 entries 1.8, 3111 by 37 experts 5.1, 131072 by 64 7.6, 262144
+// by 1024 14.5, 524288 by 128 12.9; 131072 ids by 65536 rows in two passes 20.  What is left
+// is latency: a launch, a barrier or an L2 access for every step of a pass.
 #include <string>
 
 #include <cooperative_groups.h>
