@@ -87,13 +87,19 @@ struct Rows {
     int64_t stride;
     int type;
 };
-Rows feature_rows(const Tensor& t, const char* name) {
-    TORCH_CHECK_VALUE(t.dim() == 2, name, " must be 2-D (rows x features), got ", t.sizes());
-    const int type = type_of(t, name);
+Rows feature_rows(const Tensor& given, const char* name) {
+    TORCH_CHECK_VALUE(given.dim() == 2, name, " must be 2-D (rows x features), got ", given.sizes());
+    const int type = type_of(given, name);
+    const Tensor t = given.is_neg() ? given.resolve_neg() : given;  // a lazily negated view: its memory has the other sign
     const int64_t width = t.size(1);
     if (t.is_contiguous()) return {t, width, type};
     if (width > 1 && t.stride(1) != 1) return {t.contiguous(), width, type};
     return {t, t.size(0) > 1 ? t.stride(0) : width, type};
+}
+
+// Tells autograd that a tensor of the caller's was written.
+void written(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 // The device made current, its current stream, and a workspace on it.
@@ -122,7 +128,7 @@ Places places(PyObject* position, PyObject* offsets, const char* what) {
     return {p, o, p.size(0), p.size(1)};
 }
 Tensor weights_of(PyObject* w, const Places& p, const char* what) {
-    const Tensor& t = tensor(w, "weights");
+    const Tensor t = tensor(w, "weights").resolve_neg();
     type_of(t, "weights");
     TORCH_CHECK_VALUE(t.sizes() == p.position.sizes() || (t.dim() == 1 && p.slots == 1 && t.size(0) == p.tokens), what,
                       ": weights ", t.sizes(), " do not fit an assignment ", p.position.sizes());
@@ -283,11 +289,12 @@ PyObject* embedding_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
         out = at::empty({rows, width}, dy.t.options().dtype(type));
     else
         TORCH_CHECK_VALUE(out.scalar_type() == type && out.dim() == 2 && out.size(0) == rows && out.size(1) == width &&
-                              out.is_contiguous(),
+                              out.is_contiguous() && !out.is_neg(),
                           what, ": out must be a contiguous ", type, " tensor of shape [", rows, ", ", width, "]");
     const Tensor ids = given.contiguous();
     const size_t size = hb_embedding_grad_workspace(count, rows, width);
     Tensor ws = workspace(size, device);
+    if (args[5] != Py_None) written(out);
     const Launch on(device);
     check(hb_embedding_grad(dy.type, dy.t.const_data_ptr(), dy.stride, ids.const_data_ptr(), bytes, count, rows, width,
                             number(args[3]), type_or(type, HB_F32), out.data_ptr(), accumulate, ws.data_ptr(), size,
@@ -316,6 +323,7 @@ List list_of(PyObject* o, const char* what, c10::Device* device) {
         if (t.device() != *device) device_of(what, {&t, i > 0 ? &l.tensors[0] : &t});
         TORCH_CHECK_VALUE(t.device() == *device, what, ": outputs on another device than their gradients");
         l.type.push_back(type_of(t, "gradients"));
+        TORCH_CHECK_VALUE(!t.is_neg(), what, ": gradients must not be lazily negated views");
         TORCH_CHECK_VALUE(t.is_contiguous() || t.is_non_overlapping_and_dense(), what,
                           ": gradients must be dense in memory, got strides ", t.strides(), " for ", t.sizes());
         l.tensors.push_back(t);
@@ -365,6 +373,8 @@ PyObject* clip(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const size_t size = hb_clip_workspace(count);
     Tensor ws = workspace(size, device);
     const Launch on(device);
+    if (scale)
+        for (const Tensor& t : to->tensors) written(t);
     if (scale)
         check(hb_clip_grad_norm(count, grads.address.data(), grads.size.data(), grads.type.data(), to->address.data(),
                                 to->type.data(), limit, norm.data_ptr<float>(), ws.data_ptr(), size, on.stream));

@@ -28,6 +28,18 @@ def test_lookup_matches_64_bits(hb, cuda, dtype, n, rows, width):
     assert np.array_equal(ref.f64(plain), want)
 
 
+@pytest.mark.parametrize("dtype", ref.DTYPES)
+@pytest.mark.parametrize("n,rows,width", [(20_000, 500, 2048), (30_000, 3000, 256), (100_000, 700, 33),
+                                          (200_000, 100, 8)])
+def test_lookup_of_many_rows(hb, cuda, dtype, n, rows, width):
+    """Scaled by 2, which is exact: equal to indexing, bit for bit."""
+    gen = torch.Generator(device=cuda).manual_seed(n)
+    table = torch.randn((rows, width), generator=gen, device=cuda).to(dtype)
+    ids = torch.randint(-1, rows, (n,), generator=gen, device=cuda)
+    want = torch.where((ids >= 0).unsqueeze(1), 2 * table[ids.clamp(min=0)], torch.zeros((), dtype=dtype, device=cuda))
+    assert torch.equal(hb.embedding_lookup(table, ids, scale=2), want)
+
+
 def _grad_reference(dy, ids, rows, scale):
     want, mag, count = (np.zeros((rows, dy.shape[1])) for _ in range(3))
     live = (ids >= 0) & (ids < rows)
@@ -75,12 +87,12 @@ def test_grad_matches_64_bits(hb, cuda, dtype, kind, n, rows, width):
         assert torch.equal(total[untouched], base[untouched])
 
 
-def test_grad_of_long_runs_and_large_batches(hb, cuda):
+@pytest.mark.parametrize("n,rows,width", [(150_000, 5000, 256), (600_000, 70_000, 8), (40_000, 200, 16), (300_000, 3, 4)])
+def test_grad_of_long_runs_and_large_batches(hb, cuda, n, rows, width):
     """Enough tokens for long chunks and several sort tiles; one row takes a third of them."""
     gen = torch.Generator(device=cuda).manual_seed(4)
-    n, rows, width = 150_000, 5000, 256
     ids = torch.randint(0, rows, (n,), generator=gen, device=cuda)
-    ids[torch.rand(n, generator=gen, device=cuda) < 1 / 3] = 77
+    ids[torch.rand(n, generator=gen, device=cuda) < 1 / 3] = 2
     dy = torch.randn((n, width), generator=gen, device=cuda).to(torch.bfloat16)
     got = hb.embedding_grad(dy, ids, rows, dtype=torch.float32)
     want = torch.zeros((rows, width), dtype=torch.float64, device=cuda).index_add_(0, ids, dy.double())
@@ -144,6 +156,13 @@ def test_autograd_and_differences(hb, cuda):
         along = float((table.grad.double() * v.double()).sum())
         scale = float(np.abs(ref.f64(table)).max() + 4) * float(r.abs().sum())
         assert abs(along - change) <= 2.0 ** -22 * scale
+
+
+def test_written_gradients_count_as_changed(hb, cuda):
+    out = torch.zeros((5, 4), device=cuda)
+    before = out._version
+    hb.embedding_grad(torch.ones((3, 4), device=cuda), torch.tensor([0, 1, 1], device=cuda), 5, out=out)
+    assert out._version > before
 
 
 def test_refusals(hb, cuda):

@@ -38,7 +38,7 @@ def _check_clipped(got, grads, limit):
 
 SIZES = {"one": [1], "tail": [8191, 8192, 8193, 3], "empty among": [0, 5, 0, 70000, 0], "few": [1000 + 37 * i for i in range(14)],
          "most of the short list": [17 + i for i in range(64)], "long list": [1 + i % 9 for i in range(65)],
-         "several lists": [1 + i % 40 for i in range(2500)], "large": [20_000_003, 5_000_000]}
+         "several lists": [1 + i % 40 for i in range(2500)], "large": [20_000_003, 5_000_000], "large in several lists": [8001 - i % 3 for i in range(1100)]}
 
 
 @pytest.mark.parametrize("sizes", SIZES)
@@ -115,6 +115,15 @@ def test_graph_and_stream(hb, cuda):
     again = [torch.empty_like(g) for g in grads]
     assert torch.equal(norm, hb.clip_grad_norm(grads, 0.5, out=again))
     assert all(torch.equal(a, b) for a, b in zip(out, again))
+
+
+def test_clipped_gradients_count_as_changed(hb, cuda):
+    g = torch.ones(10, device=cuda)
+    before = g._version
+    hb.grad_norm([g])
+    assert g._version == before
+    hb.clip_grad_norm([g], 1.0)
+    assert g._version > before
 
 
 def test_refusals(hb, cuda):

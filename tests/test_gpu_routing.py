@@ -55,6 +55,7 @@ def test_plan_edges(hb, cuda):
 
 CASES = [  # tokens, slots, experts, width, dropped
     (1, 2, 16, 2048, 0.0), (1, 1, 1, 1, 0.0), (5, 3, 4, 7, 0.3), (37, 3, 11, 1000, 0.2), (130, 5, 8, 257, 0.1),
+    (1400, 3, 6, 1024, 0.1), (1300, 1, 6, 2048, 0.0), (1250, 2, 6, 1032, 0.1), (5000, 3, 9, 264, 0.1), (5000, 2, 9, 301, 0.1),
     (64, 9, 3, 40, 0.5), (2000, 2, 16, 128, 0.1), (1300, 4, 5, 516, 0.1), (3, 40, 64, 4104, 0.1), (17, 1, 4, 9000, 0.0)]
 
 
@@ -160,6 +161,22 @@ def test_autograd_and_differences(hb, cuda):
             change = (loss64(*move[0]) - loss64(*move[1])) / (2 * h)
             # fp32 gradients: about 2^-22 of the summed magnitudes; differences: h^2 and 2^-53 / h
             assert abs(float((ref.f64(grad) * v).sum()) - change) <= 2.0 ** -18 * np.abs(ref.f64(grad) * v).sum() + 1e-7
+
+
+def test_autograd_without_weights(hb, cuda):
+    index = torch.tensor([[0, 1], [1, -1], [0, 0]], device=cuda)
+    plan = hb.route_plan(index, 2)
+    z = torch.randn((6, 5), device=cuda).requires_grad_()
+    hb.route_combine(z, plan).sum().backward()
+    assert torch.equal(z.grad, torch.tensor([1.0, 1, 1, 1, 1, 0], device=cuda).unsqueeze(1).expand(6, 5))
+
+
+def test_lazily_negated_rows(hb, cuda):
+    """The imaginary part of a conjugate is a view whose memory has the other sign."""
+    rows = torch.randn((4, 3), dtype=torch.complex64, device=cuda).conj().imag
+    assert rows.is_neg()
+    plan = hb.route_plan(torch.tensor([1, 0, 1, 0], device=cuda), 2)
+    assert torch.equal(hb.route_dispatch(rows, plan), rows.resolve_neg()[plan.order.long()])
 
 
 def test_other_stream_and_graph(hb, cuda):
