@@ -36,7 +36,7 @@ constexpr int kThreads = 256, kSmallThreads = 512;
 constexpr int64_t kChunk = 8192, kSmallChunk = 8192;  // elements; small: 4 loads a thread of fp32
 constexpr int64_t kSmallMost = 1 << 19;               // elements of the one-launch form
 constexpr int kCluster = 16;
-constexpr int64_t kLargeLeast = 1 << 23;              // elements from which a block scales one chunk
+constexpr int64_t kLargeLeast = 1 << 23, kLargeChunk = 16384;  // elements from which a block scales one chunk
 constexpr int kMostBlocks = 148 * 8;
 constexpr double kEps = 1e-6;
 
@@ -290,9 +290,10 @@ cudaError_t run(int64_t count, const void* const* in, const int64_t* size, const
                 const int32_t* out_type, double limit, bool large, float* norm, float* factor, double* partial,
                 cudaStream_t st) {
     List<MOST> l;
+    const int64_t chunk = large ? kLargeChunk : kChunk;
     int partials = 0;
     for (int64_t from = 0; from < count || from == 0; from += MOST) {
-        const int blocks = blocks_of(fill(l, kChunk, from, std::min(count, from + MOST), in, size, type, out, out_type));
+        const int blocks = blocks_of(fill(l, chunk, from, std::min(count, from + MOST), in, size, type, out, out_type));
         square_kernel<MOST><<<blocks, kThreads, 0, st>>>(l, partial + partials);
         count_launches(1);
         partials += blocks;
@@ -303,7 +304,7 @@ cudaError_t run(int64_t count, const void* const* in, const int64_t* size, const
         if (!out) return cudaGetLastError();
     }
     for (int64_t from = 0; from < count || from == 0; from += MOST) {
-        if (count > MOST) fill(l, kChunk, from, std::min(count, from + MOST), in, size, type, out, out_type);
+        if (count > MOST) fill(l, chunk, from, std::min(count, from + MOST), in, size, type, out, out_type);
         const int chunks = l.first[l.count];
         if (chunks == 0 && large) continue;
         if (large) scale_large_kernel<MOST><<<chunks, kThreads, 0, st>>>(l, factor);
