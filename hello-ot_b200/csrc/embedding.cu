@@ -122,11 +122,33 @@ struct Grad {
     int rows_per_warp;
 };
 
+// Adds N values to fp32 ones in memory without waiting for them.  An element gets one addition a call, so the
+// order of a launch's additions does not matter.
+template <int N>
+__device__ __forceinline__ void add_in_memory(float* p, const float (&v)[N]) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4)
+            atomicAdd(reinterpret_cast<float4*>(p + i), make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
+    } else if constexpr (N == 2) {
+        atomicAdd(reinterpret_cast<float2*>(p), make_float2(v[0], v[1]));
+    } else {
+        static_assert(N == 1, "vectors have 1, 2, 4 or 8 elements");
+        atomicAdd(p, v[0]);
+    }
+}
+
 template <typename T, typename TO, int N>
 __device__ __forceinline__ void write_row(const Grad<T, TO>& g, uint32_t key, int64_t c, const float (&sum)[N]) {
     TO* to = g.out + (int64_t)key * g.width + c;
     float r[N];
     if (g.accumulate) {
+        if constexpr (sizeof(TO) == 4) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) r[i] = g.scale * sum[i];
+            add_in_memory<N>(to, r);
+            return;
+        }
         Values<TO, N>::load(to, r);
 #pragma unroll
         for (int i = 0; i < N; ++i) r[i] = fmaf(g.scale, sum[i], r[i]);
@@ -379,15 +401,18 @@ __device__ __forceinline__ void zero_rows(const Grad<T, TO>& g, int64_t block) {
         }
         empty = lo >= g.n || (small ? staged[lo] : g.pairs[lo].x) != (uint32_t)row;
     }
-    for (unsigned left = __ballot_sync(0xffffffffu, empty); left; left &= left - 1) {
-        TO* to = g.out + (first + __ffs(left) - 1) * g.width;
-        // bytes up to the first 16-byte boundary, whole vectors, the rest
-        const int64_t lead = min(g.width, (int64_t)((16 - (reinterpret_cast<uintptr_t>(to) & 15)) & 15) / (int)sizeof(TO));
-        const int64_t whole = (g.width - lead) * (int)sizeof(TO) / 16;
+    for (unsigned left = __ballot_sync(0xffffffffu, empty); left;) {  // by runs of empty rows
+        const int from = __ffs(left) - 1, run = __ffs(~(left >> from)) - 1, rows_ = run < 0 ? 32 : run;
+        left &= ~((rows_ == 32 ? ~0u : (1u << rows_) - 1u) << from);
+        TO* to = g.out + (first + from) * g.width;
+        const int64_t elements = rows_ * g.width;
+        // single elements up to the first 16-byte boundary, whole vectors, the rest
+        const int64_t lead = min(elements, (int64_t)((16 - (reinterpret_cast<uintptr_t>(to) & 15)) & 15) / (int)sizeof(TO));
+        const int64_t whole = (elements - lead) * (int)sizeof(TO) / 16;
         const int64_t done = lead + whole * (16 / (int)sizeof(TO));
         if (lane < lead) to[lane] = rows::from_float<TO>(0.0f);
         for (int64_t i = lane; i < whole; i += 32) reinterpret_cast<uint4*>(to + lead)[i] = make_uint4(0, 0, 0, 0);
-        if (done + lane < g.width) to[done + lane] = rows::from_float<TO>(0.0f);
+        if (done + lane < elements) to[done + lane] = rows::from_float<TO>(0.0f);
     }
 }
 
