@@ -115,7 +115,8 @@ struct Grad {
     int64_t chunks;
     int tiles;               // column tiles
     float* partial;          // [chunks][2][width]: the row that a chunk continues, the row that it leaves open
-    uint32_t* arrived;       // [chunks][3][tiles], zero: what join_run counts
+    uint32_t* arrived;       // [chunks][3][tiles], zero: a block's partials of a row that it continues, of one that
+                             // begins in it, and the sums there are of a row's blocks
     TO* out;
     int accumulate;
     int64_t sum_blocks;
@@ -159,23 +160,19 @@ __device__ __forceinline__ void write_row(const Grad<T, TO>& g, uint32_t key, in
     Values<TO, N>::store(to, r);
 }
 
-// The chunks of a row that crosses them: the last one that `key` reaches from chunk c, which it leaves open,
-// and the first one from chunk c, which it is continued in.  Doubling steps, then halving ones.
+// The far chunk of a row `key` that crosses chunks: the first one of a row that chunk c continues (down), or the
+// last one of a row that chunk c leaves open.  Doubling steps, then halving ones.
 template <typename G>
-__device__ __forceinline__ int64_t last_chunk(const G& g, uint32_t key, int64_t c) {
-    int64_t e = c + 1, step = 1;
-    while (e + step < g.chunks && g.pairs[(e + step) * g.chunk].x == key) e += step, step <<= 1;
+__device__ __forceinline__ int64_t far_chunk(const G& g, uint32_t key, int64_t c, bool down) {
+    const int64_t way = down ? -1 : 1;
+    int64_t x = c + way, step = 1;
+    auto holds = [&](int64_t chunk) {  // its last place, or its first
+        return chunk >= 0 && chunk < g.chunks && g.pairs[down ? (chunk + 1) * g.chunk - 1 : chunk * g.chunk].x == key;
+    };
+    while (holds(x + way * step)) x += way * step, step <<= 1;
     for (; step; step >>= 1)
-        if (e + step < g.chunks && g.pairs[(e + step) * g.chunk].x == key) e += step;
-    return e;
-}
-template <typename G>
-__device__ __forceinline__ int64_t first_chunk(const G& g, uint32_t key, int64_t c) {
-    int64_t s = c - 1, step = 1;
-    while (s - step >= 0 && g.pairs[(s - step + 1) * g.chunk - 1].x == key) s -= step, step <<= 1;
-    for (; step; step >>= 1)
-        if (s - step >= 0 && g.pairs[(s - step + 1) * g.chunk - 1].x == key) s -= step;
-    return s;
+        if (holds(x + way * step)) x += way * step;
+    return x;
 }
 
 // All threads of a group (a part of a warp, or whole warps).
@@ -206,31 +203,28 @@ __device__ __forceinline__ void add_partials(const float* part, int64_t step, in
     }
 }
 
-// Called by a group whose partial, of chunk `chunk` of the row `key` that reaches from chunk `first` to `last`,
-// is stored: counts it in, and joins what that completes.  Partial 1 of a row's first chunk holds what it
-// begins with, partial 0 of each later chunk what continues it.  Chunks go by blocks of kJoin: the sum of a
-// block's partials takes the place of its first one.
+// Partial 1 of a row's first chunk holds what the row begins with, partial 0 of each later chunk what continues it.
+// Chunks go by blocks of kJoin: whoever leaves the last partial of a block adds them up, in the place of the
+// block's first one, and whoever leaves the last block's sum adds those.
 constexpr int kJoin = 16;
+struct Join {
+    int32_t first, last, complete;  // chunks of a row; whether this group left its block's last partial
+};
+// How many of a row's partials a chunk's block has beside one, and their counter.
+template <typename T, typename TO>
+__device__ __forceinline__ uint32_t* block_counter(const Grad<T, TO>& g, int64_t first, int64_t last, int64_t chunk, int tile,
+                                                   uint32_t* others) {
+    const int64_t from = max(first, chunk / kJoin * kJoin), to = min(last, chunk / kJoin * kJoin + kJoin - 1);
+    *others = (uint32_t)(to - from);
+    return g.arrived + (from * 3 + (from == first)) * g.tiles + tile;
+}
+// Called by a group that left the last partial of chunk `chunk`'s block of the row.
 template <typename T, typename TO, int N>
-__device__ void join_run(const Grad<T, TO>& g, uint32_t key, int64_t first, int64_t last, int64_t chunk, int tile, int64_t c,
-                         bool mine, int32_t* completes) {
-    const int64_t block = chunk / kJoin, from = max(first, block * kJoin), to = min(last, block * kJoin + kJoin - 1);
-    const int opens = from == first;  // which partial and which counter
-    auto counted = [&](int64_t at, int which, int64_t most) {  // whether this group is the last of most + 1
-        __threadfence();
-        group_sync();
-        if (threadIdx.x == 0) {
-            *completes = atomicAdd(g.arrived + (at * 3 + which) * g.tiles + tile, 1u) == (uint32_t)most;
-            __threadfence();
-        }
-        group_sync();
-        const bool yes = *completes != 0;
-        group_sync();
-        return yes;
-    };
-    if (!counted(from, opens, to - from)) return;
+__device__ void join_row(const Grad<T, TO>& g, uint32_t key, int64_t first, int64_t last, int64_t chunk, int tile, int64_t c,
+                         bool mine, int32_t* complete) {
+    const int64_t from = max(first, chunk / kJoin * kJoin), to = min(last, chunk / kJoin * kJoin + kJoin - 1);
     const bool whole = first / kJoin == last / kJoin;
-    float* place = g.partial + (from * 2 + opens) * g.width + c;
+    float* place = g.partial + (from * 2 + (from == first)) * g.width + c;
     float sum[N];
     if (mine) {
         Values<float, N>::load_l2(place, sum);
@@ -238,7 +232,15 @@ __device__ void join_run(const Grad<T, TO>& g, uint32_t key, int64_t first, int6
         if (whole) write_row<T, TO, N>(g, key, c, sum);
         else Values<float, N>::store(place, sum);
     }
-    if (whole || !counted(first, 2, last / kJoin - first / kJoin) || !mine) return;
+    if (whole) return;
+    __threadfence();
+    group_sync();
+    if (threadIdx.x == 0) {
+        *complete = atomicAdd(g.arrived + (first * 3 + 2) * g.tiles + tile, 1u) == (uint32_t)(last / kJoin - first / kJoin);
+        __threadfence();
+    }
+    group_sync();
+    if (!*complete || !mine) return;
     Values<float, N>::load_l2(g.partial + (first * 2 + 1) * g.width + c, sum);
     const int64_t next = (first / kJoin + 1) * kJoin;
     add_partials<N>(g.partial + next * 2 * g.width + c, 2 * kJoin * g.width, (int)(last / kJoin - first / kJoin), sum);
@@ -277,7 +279,7 @@ template <typename T, typename TO, int VB>
 __device__ __forceinline__ void sum_chunk(const Grad<T, TO>& g, int64_t block) {
     using V = Vec<T, VB>;
     constexpr int N = V::N, D = 8;
-    __shared__ int32_t completes[256];  // a group
+    __shared__ Join joins[64][2];  // a group: of the row that its chunk continues, of the row that it leaves open
     __shared__ __align__(16) typename V::Raw ring[D * 256];
     const int tile = (int)(block % g.tiles);
     const int64_t c = ((int64_t)tile * blockDim.x + threadIdx.x) * N;
@@ -310,7 +312,15 @@ __device__ __forceinline__ void sum_chunk(const Grad<T, TO>& g, int64_t block) {
     load8(g.pairs + p0, after, tokens);
 #pragma unroll
     for (int j = 0; j < D; ++j) fetch(j, tokens[j], mine && j < count);
+    // The rows that cross the chunk's ends, and their far chunks: a thread for each search, while the rows come.
+    const int64_t p1 = p0 + count;
+    const uint32_t last_key = g.pairs[p1 - 1].x;
     const bool continues = p0 > 0 && g.pairs[p0 - 1].x == first_key;
+    const bool open = last_key < none && p1 < g.n && g.pairs[p1].x == last_key;
+    const bool through = continues && open && first_key == last_key;
+    int64_t far = chunk;
+    if (threadIdx.x == 0 ? continues : threadIdx.x == 1 ? through : threadIdx.x == 2 && open && !through)
+        far = far_chunk(g, threadIdx.x < 2 ? first_key : last_key, chunk, threadIdx.x == 0);
     uint32_t key = first_key;
     bool head = continues;
     float sum[N];
@@ -357,8 +367,6 @@ __device__ __forceinline__ void sum_chunk(const Grad<T, TO>& g, int64_t block) {
         if (key >= none) break;
     }
     if constexpr (VB >= 4) asm volatile("cp.async.wait_all;" ::: "memory");
-    const int64_t p1 = p0 + count;
-    const bool open = key < none && p1 < g.n && g.pairs[p1].x == key;
     if (key < none) {
         if (!head && open) {
             if (mine) Values<float, N>::store(g.partial + (chunk * 2 + 1) * g.width + c, sum);
@@ -366,13 +374,30 @@ __device__ __forceinline__ void sum_chunk(const Grad<T, TO>& g, int64_t block) {
             flush();
         }
     }
-    if (continues) {
-        const int64_t to = head && open ? last_chunk(g, first_key, chunk) : chunk;
-        join_run<T, TO, N>(g, first_key, first_chunk(g, first_key, chunk), to, chunk, tile, c, mine,
-                           completes + threadIdx.y);
+    const bool starts = open && !through;
+    if (!continues && !starts) return;
+    // this group's partials are out: count them in, and join the rows whose last one that was
+    __threadfence();
+    group_sync();
+    Join* join = joins[threadIdx.y];
+    if (threadIdx.x < 32) {
+        const unsigned lanes = blockDim.x < 32 ? group_lanes() : 0xffffffffu;
+        const int base = blockDim.x < 32 ? (threadIdx.y * blockDim.x) & 31 : 0;
+        const int64_t last = __shfl_sync(lanes, far, base + 1);  // of the row that goes on to this chunk
+        const bool second = threadIdx.x == 2;
+        if (threadIdx.x == 0 ? continues : second && starts) {
+            const int64_t from = second ? chunk : far, to = second ? far : last;
+            uint32_t others;
+            uint32_t* counter = block_counter(g, from, to, chunk, tile, &others);
+            join[second] = {(int32_t)from, (int32_t)to, atomicAdd(counter, 1u) == others};
+            __threadfence();
+        }
     }
-    if (open && !head)
-        join_run<T, TO, N>(g, key, chunk, last_chunk(g, key, chunk), chunk, tile, c, mine, completes + threadIdx.y);
+    group_sync();
+    if (continues && join[0].complete)
+        join_row<T, TO, N>(g, first_key, join[0].first, join[0].last, chunk, tile, c, mine, &join[0].complete);
+    if (starts && join[1].complete)
+        join_row<T, TO, N>(g, last_key, join[1].first, join[1].last, chunk, tile, c, mine, &join[1].complete);
 }
 
 // Zeros of the rows that no sorted place holds: a lane searches a row, then the warp writes.  The search is in
@@ -423,8 +448,8 @@ __global__ void __launch_bounds__(256, 3) grad_kernel(const Grad<T, TO> g) {
     else zero_rows(g, blockIdx.x - g.sum_blocks);
 }
 
-// Threads a row: a power of two up to 32 vectors, else whole warps, at most 256 a column tile.  Up to 32768
-// tokens a warp at least: groups that share a warp take their turns wherever their rows end differently.
+// Threads a row: a power of two from 4 up to 32 vectors, else whole warps, at most 256 a column tile.  Up to
+// 32768 tokens a warp at least: groups that share a warp take their turns wherever their rows end differently.
 struct Shape {
     int group, groups, tiles;
 };
@@ -432,7 +457,7 @@ inline Shape shape_of(int64_t n, int64_t vectors) {
     Shape s{};
     s.tiles = (int)((vectors + 255) / 256);
     if (vectors <= 32) {
-        s.group = n <= 32768 ? 32 : 1;
+        s.group = n <= 32768 ? 32 : 4;
         while (s.group < vectors) s.group <<= 1;
     } else {
         s.group = (int)(((vectors + s.tiles - 1) / s.tiles + 31) / 32 * 32);
