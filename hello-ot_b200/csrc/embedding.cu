@@ -17,8 +17,8 @@
 // Blocks behind the chunks write the zeros of the rows that no token names.
 //
 // Measured on a B200: 32768 rows of 2048 bf16 looked up in 36 us (187 MB, 5.2 TB/s); the
-// gradient of 131072 tokens into 65536 x 2048 bf16 160 us, 137 of them here (806 MB, 5.9
-// TB/s) and the rest the sort; 1000 tokens into 5003 x 129 f32 12 us, which is the chain of
+// gradient of 131072 tokens into 65536 x 2048 bf16 157 us, 134 of them here (806 MB, 6.0
+// TB/s) and the rest the sort; 1000 tokens into 5003 x 129 f32 11 us, which is the chain of
 // dependent accesses (places, rows, counter, join), not bytes.
 #include <string>
 
@@ -468,8 +468,8 @@ inline Shape shape_of(int64_t n, int64_t vectors) {
 
 // Places a chunk, a multiple of 8 as sum_chunk needs.  A chunk costs some microseconds of its own (its first
 // loads, its join), so up to 128 while that leaves 16 warps of work an SM; at least 16.  Measured with chunks of
-// 16 / 32 / 64 / 128: 131072 x 2048 bf16 236 / 186 / 174 / 166 us, 20000 x 2048 f16 45 / 37 / 34 / 37 us,
-// 1000 x 129 f32 16 / 18 / 21 / 28 us.
+// 16 / 32 / 64 / 128: 131072 x 2048 bf16 212 / 173 / 162 / 156 us, 20000 x 2048 f16 37 / 32 / 28 / 32 us,
+// 1000 x 129 f32 11 / 13 / 16 / 25 us.
 inline int chunk_of(int64_t n, const Shape& s) {
     const int64_t c = n * s.tiles * s.group / 32 / (148 * 16);
     return (int)(c < 16 ? 16 : c > 128 ? 128 : c / 8 * 8);
