@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(256) lookup_kernel(const T* __restrict__ table
 #pragma unroll
                 for (int j = 0; j < V::N; ++j)
                     r.v[j] = rows::from_float<T>(id[m] >= 0 ? scale * rows::to_float(v[m][u].v[j]) : 0.0f);
-                r.store(out + (first + m) * width + c + u * step);
+                r.store_once(out + (first + m) * width + c + u * step);
             }
     }
 }

@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(256) dispatch_kernel(Moves m, const T* __restr
                         w.zero();
                         w.store(to + u * G * V::N);
                     } else {
-                        v[t][u].store(to + u * G * V::N);
+                        v[t][u].store_once(to + u * G * V::N);
                     }
                 }
             }
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(256) combine_kernel(Moves m, const T* __restri
             V r;
 #pragma unroll
             for (int i = 0; i < V::N; ++i) r.v[i] = rows::from_float<T>(sum[i]);
-            r.store(out + t * m.width + c0 + u * G * V::N);
+            r.store_once(out + t * m.width + c0 + u * G * V::N);
         };
         if (SLOTS) {  // all rows of the tokens at once; one token's sum at a time
             load();
@@ -250,7 +250,8 @@ __global__ void __launch_bounds__(256) combine_grad_kernel(Moves m, int ways, co
                             if (dw) dot[0] = fmaf(gv, rows::to_float(a[u].v[i]), dot[0]);
                             r.v[i] = rows::from_float<T>(w * gv);
                         }
-                        r.store(to + c);
+                        if (VB >= 8) r.store_once(to + c);
+                        else r.store(to + c);  // sectors of short ones are written in two parts: kept until whole
                     }
                 }
             }

@@ -41,6 +41,8 @@ struct Vec {
     __device__ __forceinline__ void load(const T* p) { raw = __ldg(reinterpret_cast<const Raw*>(p)); }
     __device__ __forceinline__ void load_once(const T* p) { raw = __ldcs(reinterpret_cast<const Raw*>(p)); }
     __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Raw*>(p) = raw; }
+    // first to leave L2: rows that nothing of this kernel reads again, so that those it does read stay
+    __device__ __forceinline__ void store_once(T* p) const { __stcs(reinterpret_cast<Raw*>(p), raw); }
     __device__ __forceinline__ void zero() {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = from_float<T>(0.0f);
