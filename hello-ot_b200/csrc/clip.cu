@@ -185,7 +185,7 @@ __device__ __forceinline__ void scale_chunk(const T* p, TO* out, int n, float f)
 #pragma unroll
                         for (int j = 0; j < O::N; ++j)
                             o.v[j] = rows::from_float<TO>(f * rows::to_float(v[u].v[q * O::N + j]));
-                        o.store(out + (int64_t)(i + u * THREADS) * N + q * O::N);
+                        o.store_once(out + (int64_t)(i + u * THREADS) * N + q * O::N);
                     }
                 }
         }

@@ -16,9 +16,9 @@
 // and run over k in order (no atomics): the result does not depend on the launch.
 //
 // Measured on a B200, us and TB/s of the bytes above: 32768 tokens x 4 of 2048 bf16
-// dispatch 110 (6.1), combine 111 (6.0), its gradient 193 (6.2); 65536 x 8: 390 (6.2), 384
-// (6.3), 714 (6.4).  262144 x 1 of 128 f32: 44, 48, 64.  Rows off the 16-byte grid stay at
-// 60 % of that (30000 x 2 of 1001 bf16: 44, 48, 79): 2-byte loads hold too few bytes in
+// dispatch 110 (6.1), combine 110 (6.1), its gradient 194 (6.2); 65536 x 8: 389 (6.2), 380
+// (6.4), 710 (6.4).  262144 x 1 of 128 f32: 43, 43, 64.  Rows off the 16-byte grid stay at
+// 60 % of that (30000 x 2 of 1001 bf16: 42, 46, 79): 2-byte loads hold too few bytes in
 // flight, and shifting aligned words together costs more registers than it saves.
 #include <string>
 
