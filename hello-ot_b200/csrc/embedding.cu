@@ -332,18 +332,25 @@ __device__ __forceinline__ void sum_chunk(const Grad<T, TO>& g, int64_t block) {
             else write_row<T, TO, N>(g, key, c, sum);
         }
     };
+    // no asynchronous copy of 2 bytes: 8 rows ahead by way of registers
+    typename V::Raw ahead[VB >= 4 ? 1 : D], raw[VB >= 4 ? 1 : D];
+    auto load_ahead = [&](int i) {
+#pragma unroll
+        for (int j = 0; j < D; ++j)
+            if (mine && i + j < count)
+                ahead[j] = __ldcs(reinterpret_cast<const typename V::Raw*>(column + (uint64_t)tokens[j] * stride));
+    };
+    if constexpr (VB < 4) load_ahead(0);
     for (int i = 0; i < count; i += D) {
         const bool more = i + D < count;
-        typename V::Raw raw[VB >= 4 ? 1 : D];
-        if constexpr (VB < 4) {  // no asynchronous copy of 2 bytes: 8 loads by way of registers
-#pragma unroll
-            for (int j = 0; j < D; ++j)
-                if (mine && i + j < count)
-                    raw[j] = __ldcs(reinterpret_cast<const typename V::Raw*>(column + (uint64_t)tokens[j] * stride));
-        }
 #pragma unroll
         for (int j = 0; j < D; ++j) keys[j] = i + j < count ? after[j] : none;
         if (more) load8(g.pairs + p0 + i + D, after, tokens);
+        if constexpr (VB < 4) {
+#pragma unroll
+            for (int j = 0; j < D; ++j) raw[j] = ahead[j];
+            load_ahead(i + D);
+        }
 #pragma unroll
         for (int j = 0; j < D; ++j) {
             if (keys[j] != key) {
