@@ -273,14 +273,17 @@ __device__ __forceinline__ void load8(const uint2* pairs, uint32_t (&row)[8], ui
 
 // Sums a chunk.  Each thread has its own ring of 8 vectors in shared memory, one a sorted place, filled ahead by
 // asynchronous copies: 8 rows are in flight while the sums hold few registers, and no thread waits for another.
-// The loop goes by 8 places (chunks are multiples of 8), whose rows and tokens come in whole vectors, since its
-// instructions are the next bound after the bytes.
+// Vectors of 4 and 2 bytes are loaded 8 rows ahead into registers instead: they fit there, and the ring's
+// instructions a row weigh more the fewer bytes a row has (92503 tokens into 105992 x 369 f32 98 us against 102,
+// 40000 into 30000 x 1002 f16 60 against 65; vectors of 8 bytes 51.5 in the ring against 53.7).  The loop goes by 8
+// places (chunks are multiples of 8), whose rows and tokens come in whole vectors, since its instructions are the
+// next bound after the bytes.
 template <typename T, typename TO, int VB>
 __device__ __forceinline__ void sum_chunk(const Grad<T, TO>& g, int64_t block) {
     using V = Vec<T, VB>;
     constexpr int N = V::N, D = 8;
     __shared__ Join joins[64][2];  // a group: of the row that its chunk continues, of the row that it leaves open
-    __shared__ __align__(16) typename V::Raw ring[D * 256];
+    __shared__ __align__(16) typename V::Raw ring[VB >= 8 ? D * 256 : 1];
     const int tile = (int)(block % g.tiles);
     const int64_t c = ((int64_t)tile * blockDim.x + threadIdx.x) * N;
     const int64_t chunk = block / g.tiles * blockDim.y + threadIdx.y;
@@ -297,13 +300,13 @@ __device__ __forceinline__ void sum_chunk(const Grad<T, TO>& g, int64_t block) {
     const uint32_t stride = (uint32_t)(g.dy_stride * (int64_t)sizeof(T));  // bytes, below 2^32
     auto fetch = [&](int j, uint32_t token, bool there) {  // into slot j
         const char* p = column + (uint64_t)token * stride;
-        if constexpr (VB >= 4) {
+        if constexpr (VB >= 8) {
             const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(slots + j * step));
             if (there) {
                 if constexpr (VB == 16)
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(p) : "memory");
                 else
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(p), "n"(VB) : "memory");
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(p) : "memory");
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
@@ -332,21 +335,21 @@ __device__ __forceinline__ void sum_chunk(const Grad<T, TO>& g, int64_t block) {
             else write_row<T, TO, N>(g, key, c, sum);
         }
     };
-    // no asynchronous copy of 2 bytes: 8 rows ahead by way of registers
-    typename V::Raw ahead[VB >= 4 ? 1 : D], raw[VB >= 4 ? 1 : D];
+    // short vectors: 8 rows ahead in registers
+    typename V::Raw ahead[VB >= 8 ? 1 : D], raw[VB >= 8 ? 1 : D];
     auto load_ahead = [&](int i) {
 #pragma unroll
         for (int j = 0; j < D; ++j)
             if (mine && i + j < count)
                 ahead[j] = __ldcs(reinterpret_cast<const typename V::Raw*>(column + (uint64_t)tokens[j] * stride));
     };
-    if constexpr (VB < 4) load_ahead(0);
+    if constexpr (VB < 8) load_ahead(0);
     for (int i = 0; i < count; i += D) {
         const bool more = i + D < count;
 #pragma unroll
         for (int j = 0; j < D; ++j) keys[j] = i + j < count ? after[j] : none;
         if (more) load8(g.pairs + p0 + i + D, after, tokens);
-        if constexpr (VB < 4) {
+        if constexpr (VB < 8) {
 #pragma unroll
             for (int j = 0; j < D; ++j) raw[j] = ahead[j];
             load_ahead(i + D);
@@ -362,7 +365,7 @@ __device__ __forceinline__ void sum_chunk(const Grad<T, TO>& g, int64_t block) {
                 if (key >= none) break;
             }
             V v;
-            if constexpr (VB >= 4) {
+            if constexpr (VB >= 8) {
                 asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
                 v.raw = slots[j * step];
             } else {
@@ -373,7 +376,7 @@ __device__ __forceinline__ void sum_chunk(const Grad<T, TO>& g, int64_t block) {
         }
         if (key >= none) break;
     }
-    if constexpr (VB >= 4) asm volatile("cp.async.wait_all;" ::: "memory");
+    if constexpr (VB >= 8) asm volatile("cp.async.wait_all;" ::: "memory");
     if (key < none) {
         if (!head && open) {
             if (mine) Values<float, N>::store(g.partial + (chunk * 2 + 1) * g.width + c, sum);
