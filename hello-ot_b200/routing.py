@@ -69,36 +69,35 @@ def route_combine_grad(dy, z, plan, weights=None, *, need_weights: bool = True):
 
 class _Dispatch(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, plan):
-        ctx.plan = plan
-        return host().route_dispatch(x, plan[1], plan[2])
+    def forward(ctx, x, position, offsets):
+        ctx.save_for_backward(position, offsets)
+        return host().route_dispatch(x, position, offsets)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dsorted):
-        return route_dispatch_grad(dsorted, ctx.plan), None
+        return route_dispatch_grad(dsorted, (None, *ctx.saved_tensors)), None, None
 
 
 class _Combine(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, z, plan, weights):
-        ctx.plan = plan
-        ctx.save_for_backward(z, weights)
-        return host().route_combine(z, plan[1], plan[2], weights, "route_combine")
+    def forward(ctx, z, position, offsets, weights):
+        ctx.save_for_backward(z, position, offsets, weights)
+        return host().route_combine(z, position, offsets, weights, "route_combine")
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        z, weights = ctx.saved_tensors
-        dz, dw = route_combine_grad(dy, z, ctx.plan, weights, need_weights=ctx.needs_input_grad[2])
-        return dz, None, dw
+        z, position, offsets, weights = ctx.saved_tensors
+        dz, dw = route_combine_grad(dy, z, (None, position, offsets), weights, need_weights=ctx.needs_input_grad[3])
+        return dz, None, None, dw
 
 
 def route_dispatch(x, plan):
     """x's rows [tokens, width] in the plan's order, [tokens * slots, width]; zero rows for entries without
     an expert.  Differentiable in x."""
     if x.requires_grad and torch.is_grad_enabled():
-        return _Dispatch.apply(x, plan)
+        return _Dispatch.apply(x, plan[1], plan[2])
     return host().route_dispatch(x, plan[1], plan[2])
 
 
@@ -106,7 +105,7 @@ def route_combine(z, plan, weights=None):
     """sum_k weights[t, k] z[position[t, k]] over the entries with an expert, [tokens, width]; weights of 1
     when there are none.  Differentiable in z and weights."""
     if torch.is_grad_enabled() and (z.requires_grad or (weights is not None and weights.requires_grad)):
-        return _Combine.apply(z, plan, weights)
+        return _Combine.apply(z, plan[1], plan[2], weights)
     return host().route_combine(z, plan[1], plan[2], weights, "route_combine")
 
 
