@@ -11,6 +11,7 @@
 #include <vector>
 
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -25,9 +26,13 @@ namespace {
 using at::Tensor;
 
 // ---------------------------------------------------------------- arguments
+// Whether a tensor carries a forward-mode tangent; inside an autograd function, whose tangents go their own way, none does.
+bool has_tangent(const Tensor& t) { return t._fw_grad(0).defined(); }
 const Tensor& tensor(PyObject* o, const char* name) {
     TORCH_CHECK_VALUE(THPVariable_Check(o), name, " must be a tensor");
-    return THPVariable_Unpack(o);
+    const Tensor& t = THPVariable_Unpack(o);
+    TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(t), name, " carries a forward-mode tangent, and this call has no derivative");
+    return t;
 }
 int64_t integer(PyObject* o) {
     const int64_t v = PyLong_AsLongLong(o);
@@ -81,6 +86,12 @@ c10::Device device_of(const char* what, std::initializer_list<const Tensor*> ten
     return device;
 }
 
+// A tensor whose memory holds its values: a lazily negated view's has the other sign, zeros of a tangent have none.
+Tensor resolved(const Tensor& t) {
+    if (t._is_zerotensor()) return at::zeros(t.sizes(), at::TensorOptions().dtype(t.scalar_type()).device(t.device()));
+    return t.is_neg() ? t.resolve_neg() : t;
+}
+
 // Features whose rows are contiguous (a copy where they are not) and the rows' distance in elements.
 struct Rows {
     Tensor t;
@@ -90,7 +101,7 @@ struct Rows {
 Rows feature_rows(const Tensor& given, const char* name) {
     TORCH_CHECK_VALUE(given.dim() == 2, name, " must be 2-D (rows x features), got ", given.sizes());
     const int type = type_of(given, name);
-    const Tensor t = given.is_neg() ? given.resolve_neg() : given;  // a lazily negated view: its memory has the other sign
+    const Tensor t = resolved(given);
     const int64_t width = t.size(1);
     if (t.is_contiguous()) return {t, width, type};
     if (width > 1 && t.stride(1) != 1) return {t.contiguous(), width, type};
@@ -112,6 +123,18 @@ Tensor workspace(size_t bytes, c10::Device device) {
     return at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(device));
 }
 
+// differentiates(tensor or None, ...) -> whether a derivative is taken through any of them
+PyObject* differentiates(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        if (!THPVariable_Check(args[i])) continue;
+        const Tensor& t = THPVariable_Unpack(args[i]);
+        if (has_tangent(t) || (t.requires_grad() && c10::GradMode::is_enabled())) Py_RETURN_TRUE;
+    }
+    Py_RETURN_FALSE;
+    END_HANDLE_TH_ERRORS
+}
+
 // ---------------------------------------------------------------- routing
 struct Places {
     const Tensor &position, &offsets;
@@ -128,7 +151,7 @@ Places places(PyObject* position, PyObject* offsets, const char* what) {
     return {p, o, p.size(0), p.size(1)};
 }
 Tensor weights_of(PyObject* w, const Places& p, const char* what) {
-    const Tensor t = tensor(w, "weights").resolve_neg();
+    const Tensor t = resolved(tensor(w, "weights"));
     type_of(t, "weights");
     TORCH_CHECK_VALUE(t.sizes() == p.position.sizes() || (t.dim() == 1 && p.slots == 1 && t.size(0) == p.tokens), what,
                       ": weights ", t.sizes(), " do not fit an assignment ", p.position.sizes());
@@ -386,6 +409,7 @@ PyObject* clip(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 PyMethodDef methods[] = {
+    {"differentiates", reinterpret_cast<PyCFunction>(differentiates), METH_FASTCALL, nullptr},
     {"route_plan", reinterpret_cast<PyCFunction>(route_plan), METH_FASTCALL, nullptr},
     {"route_dispatch", reinterpret_cast<PyCFunction>(route_dispatch), METH_FASTCALL, nullptr},
     {"route_combine", reinterpret_cast<PyCFunction>(route_combine), METH_FASTCALL, nullptr},

@@ -15,7 +15,8 @@ from ._lib import host
 def embedding_grad(dy, ids, rows: int, *, scale: float = 1.0, dtype=None, out=None, accumulate: bool = False):
     """Gradient of ``embedding_lookup`` with respect to its table: [rows, width], row v the sum of scale * dy
     over ids == v, summed in fp32 and rounded once to ``dtype`` (dy's, or float32).  ``out`` receives it;
-    ``accumulate=True`` adds it to what ``out`` holds and leaves the rows that no id names untouched."""
+    ``accumulate=True`` adds it to what ``out`` holds and leaves the rows that no id names untouched.  The result
+    has no history."""
     return host().embedding_grad(dy, ids, rows, scale, dtype, out, bool(accumulate))
 
 
@@ -24,6 +25,7 @@ class _Lookup(torch.autograd.Function):
     def forward(ctx, table, ids, scale):
         ctx.rows, ctx.scale = table.shape[0], scale
         ctx.save_for_backward(ids)
+        ctx.save_for_forward(ids)
         return host().embedding_lookup(table, ids, scale)
 
     @staticmethod
@@ -32,10 +34,16 @@ class _Lookup(torch.autograd.Function):
         ids, = ctx.saved_tensors
         return embedding_grad(dy, ids, ctx.rows, scale=ctx.scale), None, None
 
+    @staticmethod
+    def jvp(ctx, dtable, _ids, _scale):
+        ids, = ctx.saved_tensors
+        return embedding_lookup(dtable, ids, scale=ctx.scale)
+
 
 def embedding_lookup(table, ids, *, scale: float = 1.0):
     """scale * table[ids], [*ids.shape, width], in fp32 and rounded once to the table's type.  ids: int32 or
-    int64 of any shape.  Differentiable in the table (a dense gradient)."""
-    if table.requires_grad and torch.is_grad_enabled():
+    int64 of any shape.  Differentiable in the table, backward (a dense
+    gradient) and forward."""
+    if host().differentiates(table):
         return _Lookup.apply(table, ids, scale)
     return host().embedding_lookup(table, ids, scale)

@@ -15,7 +15,8 @@ def _list(v):
 
 
 def grad_norm(grads):
-    """sqrt of the sum of squares of all elements of a list of tensors (float32 scalar on the device)."""
+    """sqrt of the sum of squares of all elements of a list of tensors (float32 scalar on the device, without
+    history)."""
     return host().clip(_list(grads), None, None, "grad_norm")
 
 

@@ -5,7 +5,7 @@ transport plan between tokens and experts, see ``assignment_of_plan``) by expert
 ``route_dispatch`` brings the tokens' rows into that order for the experts, and
 ``route_combine`` brings the experts' rows back to their tokens, weighted.  Both are
 differentiable; ``route_dispatch_grad`` and ``route_combine_grad`` are their
-gradients by themselves.  Entries without an expert (an index outside
+gradients by themselves, whose results have no history.  Entries without an expert (an index outside
 0..num_experts-1) are sorted last, receive zero rows and add nothing.
 
 The calls enqueue work on the current stream and never wait for the device, so the
@@ -71,6 +71,7 @@ class _Dispatch(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, position, offsets):
         ctx.save_for_backward(position, offsets)
+        ctx.save_for_forward(position, offsets)
         return host().route_dispatch(x, position, offsets)
 
     @staticmethod
@@ -78,33 +79,52 @@ class _Dispatch(torch.autograd.Function):
     def backward(ctx, dsorted):
         return route_dispatch_grad(dsorted, (None, *ctx.saved_tensors)), None, None
 
+    @staticmethod
+    def jvp(ctx, dx, _position, _offsets):
+        return route_dispatch(dx, (None, *ctx.saved_tensors))
+
 
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, z, position, offsets, weights):
+        ctx.set_materialize_grads(False)  # a tangent that is not there is None
         ctx.save_for_backward(z, position, offsets, weights)
+        ctx.save_for_forward(z, position, offsets, weights)
         return host().route_combine(z, position, offsets, weights, "route_combine")
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        if dy is None:
+            return None, None, None, None
         z, position, offsets, weights = ctx.saved_tensors
         dz, dw = route_combine_grad(dy, z, (None, position, offsets), weights, need_weights=ctx.needs_input_grad[3])
         return dz, None, None, dw
 
+    @staticmethod
+    def jvp(ctx, dz, _position, _offsets, dw):
+        z, position, offsets, weights = ctx.saved_tensors
+        plan = None, position, offsets
+        if dw is None:
+            return route_combine(dz, plan, weights)
+        if dz is None:
+            return route_combine(z, plan, dw)
+        # both sums in fp32, so that theirs is rounded once
+        return (route_combine(dz.float(), plan, weights) + route_combine(z.float(), plan, dw)).to(z.dtype)
+
 
 def route_dispatch(x, plan):
     """x's rows [tokens, width] in the plan's order, [tokens * slots, width]; zero rows for entries without
-    an expert.  Differentiable in x."""
-    if x.requires_grad and torch.is_grad_enabled():
+    an expert.  Differentiable in x, backward and forward."""
+    if host().differentiates(x):
         return _Dispatch.apply(x, plan[1], plan[2])
     return host().route_dispatch(x, plan[1], plan[2])
 
 
 def route_combine(z, plan, weights=None):
     """sum_k weights[t, k] z[position[t, k]] over the entries with an expert, [tokens, width]; weights of 1
-    when there are none.  Differentiable in z and weights."""
-    if torch.is_grad_enabled() and (z.requires_grad or (weights is not None and weights.requires_grad)):
+    when there are none.  Differentiable in z and weights, backward and forward."""
+    if host().differentiates(z, weights):
         return _Combine.apply(z, plan[1], plan[2], weights)
     return host().route_combine(z, plan[1], plan[2], weights, "route_combine")
 

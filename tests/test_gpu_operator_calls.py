@@ -1,6 +1,10 @@
 """What the routing, lookup and clipping calls keep to beside their results on ordinary arguments."""
+import numpy as np
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
+
+import rows_reference as ref
 
 pytestmark = pytest.mark.gpu
 
@@ -22,3 +26,77 @@ def test_plan_changed_before_backward(hb, cuda):
             part.add_(0)
             with pytest.raises(RuntimeError, match="modified by an inplace operation"):
                 y.sum().backward()
+
+
+def test_forward_mode_of_the_linear_calls(hb, cuda):
+    """Dispatch and lookup are linear: the tangent goes the values' way, bit for bit, with or without grad mode."""
+    gen = torch.Generator(device=cuda).manual_seed(2)
+    plan = _plan(hb, cuda, gen)
+    ids = torch.randint(-1, 40, (3, 7), generator=gen, device=cuda)
+    for dtype in ref.DTYPES:
+        x, t = (torch.randn((40, 24), generator=gen, device=cuda).to(dtype) for _ in range(2))
+        for call in (lambda v: hb.route_dispatch(v, plan), lambda v: hb.embedding_lookup(v, ids, scale=1.5)):
+            for mode in (True, False):
+                with torch.set_grad_enabled(mode), fw.dual_level():
+                    value, tangent = fw.unpack_dual(call(fw.make_dual(x, t)))
+                    assert torch.equal(value, call(x)) and torch.equal(tangent, call(t))
+
+
+@pytest.mark.parametrize("dtype", ref.DTYPES)
+def test_forward_mode_of_combine(hb, cuda, dtype):
+    """The tangent of sum w z is sum (w dz + dw z), 2 slots products in fp32 rounded once."""
+    rng = np.random.default_rng(3)
+    gen = torch.Generator(device=cuda).manual_seed(3)
+    tokens, slots, width = 40, 3, 24
+    plan = _plan(hb, cuda, gen, tokens, slots)
+    position, kept = plan.position.cpu().numpy(), int(plan.offsets[-1])
+    z, dz = (torch.as_tensor(rng.normal(size=(tokens * slots, width)), device=cuda).to(dtype) for _ in range(2))
+    w, dw = (torch.as_tensor(rng.random((tokens, slots)), device=cuda).to(dtype) for _ in range(2))
+    u, floor = ref.U[dtype], ref.FLOOR[dtype]
+    for with_z, with_w in ((True, False), (False, True), (True, True)):
+        want, mag = np.zeros((tokens, width)), np.zeros((tokens, width))
+        for on, rows, weights in ((with_z, dz, w), (with_w, z, dw)):
+            if on:
+                part = ref.combine(ref.f64(rows), position, kept, ref.f64(weights))
+                want, mag = want + part[0], mag + part[1]
+        with fw.dual_level():
+            value, tangent = fw.unpack_dual(hb.route_combine(fw.make_dual(z, dz) if with_z else z, plan,
+                                                             fw.make_dual(w, dw) if with_w else w))
+        assert torch.equal(value, hb.route_combine(z, plan, w))
+        ref.assert_within(tangent, want, 2 * slots * ref.E32 * mag * (1 + u) + u * np.abs(want) + floor)
+    with fw.dual_level():
+        tangent = fw.unpack_dual(hb.route_combine(fw.make_dual(z, dz), plan)).tangent
+    assert torch.equal(tangent, hb.route_combine(dz, plan))
+    # a derivative along z of the derivative along w, whose graph goes through the tangent
+    z = z.clone().requires_grad_()
+    with fw.dual_level():
+        fw.unpack_dual(hb.route_combine(z, plan, fw.make_dual(w, dw))).tangent.sum().backward()
+    assert torch.equal(z.grad, hb.route_combine_grad(torch.ones((tokens, width), dtype=dtype, device=cuda), z.detach(),
+                                                     plan, dw)[0])
+
+
+def test_tangents_are_not_dropped(hb, cuda):
+    """Calls without a derivative of their own refuse a tensor that carries a tangent."""
+    gen = torch.Generator(device=cuda).manual_seed(4)
+    plan = _plan(hb, cuda, gen)
+    ids = torch.randint(0, 9, (40,), generator=gen, device=cuda)
+    x, z, w = (torch.randn(s, generator=gen, device=cuda) for s in ((40, 8), (80, 8), (40, 2)))
+    with fw.dual_level():
+        dx, dz, dw = (fw.make_dual(v, torch.ones_like(v)) for v in (x, z, w))
+        for call in (lambda: hb.route_dispatch_grad(dz, plan), lambda: hb.route_combine_grad(dx, z, plan, w),
+                     lambda: hb.route_combine_grad(x, dz, plan, w), lambda: hb.route_combine_grad(x, z, plan, dw),
+                     lambda: hb.embedding_grad(dx, ids, 9), lambda: hb.grad_norm([x, dx]),
+                     lambda: hb.clip_grad_norm([dx], 1.0), lambda: hb.clip_grad_norm([x], 1.0, out=[dx])):
+            with pytest.raises(NotImplementedError, match="tangent"):
+                call()
+
+
+def test_zeros_without_memory(hb, cuda):
+    """Tangents can be zeros that have no memory, rows and weights alike."""
+    gen = torch.Generator(device=cuda).manual_seed(7)
+    plan = _plan(hb, cuda, gen)
+    z, w = torch.randn((80, 8), generator=gen, device=cuda), torch.rand((40, 2), generator=gen, device=cuda)
+    none = {shape: torch._efficientzerotensor(shape, device=cuda) for shape in ((40, 8), (80, 8), (40, 2))}
+    for got in (hb.route_dispatch(none[40, 8], plan), hb.route_combine(none[80, 8], plan, w),
+                hb.route_combine(z, plan, none[40, 2]), hb.embedding_lookup(none[40, 8], torch.arange(5, device=cuda))):
+        assert not got._is_zerotensor() and not got.any()
