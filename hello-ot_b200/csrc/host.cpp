@@ -7,10 +7,12 @@
 // from torch's allocator on the current stream.  Shapes and types are refused with ValueError; errors of
 // the C ABI are raised by hello_ot_b200._lib.check.
 #include <algorithm>
+#include <cstring>
 #include <initializer_list>
 #include <vector>
 
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -123,9 +125,16 @@ Tensor workspace(size_t bytes, c10::Device device) {
     return at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(device));
 }
 
-// differentiates(tensor or None, ...) -> whether a derivative is taken through any of them
-PyObject* differentiates(PyObject*, PyObject* const* args, Py_ssize_t n) {
+// A trace records torch's operations and autograd functions: of a call that is neither it would keep the empty output.
+void untraced(const char* what) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!at::tracer::impl::is_dispatch_enabled(), what, " cannot be recorded in a trace");
+}
+
+// recorded(tensor or None, ...) -> whether a call on them has to go through its autograd function: a derivative is
+// taken through one of them, or a trace is made
+PyObject* recorded(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
+    if (at::tracer::impl::is_dispatch_enabled()) Py_RETURN_TRUE;
     for (Py_ssize_t i = 0; i < n; ++i) {
         if (!THPVariable_Check(args[i])) continue;
         const Tensor& t = THPVariable_Unpack(args[i]);
@@ -162,6 +171,7 @@ Tensor weights_of(PyObject* w, const Places& p, const char* what) {
 PyObject* route_plan(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     expect(n, 2, "route_plan");
+    untraced("route_plan");
     const Tensor& given = tensor(args[0], "index");
     TORCH_CHECK_VALUE(given.dim() == 1 || (given.dim() == 2 && given.size(1) >= 1),
                       "index must be [tokens] or [tokens, slots], got ", given.sizes());
@@ -212,6 +222,7 @@ PyObject* route_combine(PyObject*, PyObject* const* args, Py_ssize_t n) {
     expect(n, 5, "route_combine");
     const char* what = PyUnicode_AsUTF8(args[4]);
     if (!what) throw python_error();
+    if (std::strcmp(what, "route_combine") != 0) untraced(what);  // by the name of another call it has no function of its own
     const Rows z = feature_rows(tensor(args[0], "z"), "z");
     const Places p = places(args[1], args[2], what);
     TORCH_CHECK_VALUE(z.t.size(0) == p.tokens * p.slots, what, ": ", z.t.size(0), " sorted rows for ", p.tokens, " x ",
@@ -234,6 +245,7 @@ PyObject* route_combine_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     const char* what = "route_combine_grad";
     expect(n, 6, what);
+    untraced(what);
     const Rows dy = feature_rows(tensor(args[0], "dy"), "dy"), z = feature_rows(tensor(args[1], "z"), "z");
     const Places p = places(args[2], args[3], what);
     const int64_t width = z.t.size(1);
@@ -286,6 +298,7 @@ PyObject* embedding_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     const char* what = "embedding_grad";
     expect(n, 7, what);
+    untraced(what);
     const Tensor &dy_given = tensor(args[0], "dy"), &given = tensor(args[1], "ids");
     const int bytes = index_bytes(given, "ids");
     const int64_t count = given.numel(), rows = integer(args[2]);
@@ -366,6 +379,7 @@ PyObject* clip(PyObject*, PyObject* const* args, Py_ssize_t n) {
     expect(n, 4, "clip");
     const char* what = PyUnicode_AsUTF8(args[3]);
     if (!what) throw python_error();
+    untraced(what);
     c10::Device device(c10::kCPU);
     const List grads = list_of(args[0], what, &device);
     const int64_t count = (int64_t)grads.tensors.size();
@@ -409,7 +423,7 @@ PyObject* clip(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 PyMethodDef methods[] = {
-    {"differentiates", reinterpret_cast<PyCFunction>(differentiates), METH_FASTCALL, nullptr},
+    {"recorded", reinterpret_cast<PyCFunction>(recorded), METH_FASTCALL, nullptr},
     {"route_plan", reinterpret_cast<PyCFunction>(route_plan), METH_FASTCALL, nullptr},
     {"route_dispatch", reinterpret_cast<PyCFunction>(route_dispatch), METH_FASTCALL, nullptr},
     {"route_combine", reinterpret_cast<PyCFunction>(route_combine), METH_FASTCALL, nullptr},

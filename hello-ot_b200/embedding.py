@@ -44,6 +44,6 @@ def embedding_lookup(table, ids, *, scale: float = 1.0):
     """scale * table[ids], [*ids.shape, width], in fp32 and rounded once to the table's type.  ids: int32 or
     int64 of any shape.  Differentiable in the table, backward (a dense
     gradient) and forward."""
-    if host().differentiates(table):
+    if host().recorded(table):
         return _Lookup.apply(table, ids, scale)
     return host().embedding_lookup(table, ids, scale)

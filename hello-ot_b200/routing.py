@@ -116,7 +116,7 @@ class _Combine(torch.autograd.Function):
 def route_dispatch(x, plan):
     """x's rows [tokens, width] in the plan's order, [tokens * slots, width]; zero rows for entries without
     an expert.  Differentiable in x, backward and forward."""
-    if host().differentiates(x):
+    if host().recorded(x):
         return _Dispatch.apply(x, plan[1], plan[2])
     return host().route_dispatch(x, plan[1], plan[2])
 
@@ -124,7 +124,7 @@ def route_dispatch(x, plan):
 def route_combine(z, plan, weights=None):
     """sum_k weights[t, k] z[position[t, k]] over the entries with an expert, [tokens, width]; weights of 1
     when there are none.  Differentiable in z and weights, backward and forward."""
-    if host().differentiates(z, weights):
+    if host().recorded(z, weights):
         return _Combine.apply(z, plan[1], plan[2], weights)
     return host().route_combine(z, plan[1], plan[2], weights, "route_combine")
 

@@ -100,3 +100,43 @@ def test_zeros_without_memory(hb, cuda):
     for got in (hb.route_dispatch(none[40, 8], plan), hb.route_combine(none[80, 8], plan, w),
                 hb.route_combine(z, plan, none[40, 2]), hb.embedding_lookup(none[40, 8], torch.arange(5, device=cuda))):
         assert not got._is_zerotensor() and not got.any()
+
+
+def _traced(call, *inputs):
+    return torch.jit.trace(call, inputs, check_trace=False)
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("grad", [False, True])
+def test_traced_calls_run_again(hb, cuda, grad):
+    """A trace holds the call itself, on new rows and on a new plan."""
+    gen = torch.Generator(device=cuda).manual_seed(5)
+
+    def inputs():
+        x, z = (torch.randn(s, generator=gen, device=cuda).requires_grad_(grad) for s in ((40, 8), (80, 8)))
+        w, ids = torch.rand((40, 2), generator=gen, device=cuda), torch.randint(0, 40, (6,), generator=gen, device=cuda)
+        plan = _plan(hb, cuda, gen)
+        return x, z, w, ids, plan.order, plan.position, plan.offsets
+
+    def layer(x, z, w, ids, order, position, offsets):
+        plan = hb.RoutePlan(order, position, offsets)
+        return (hb.route_dispatch(x, plan), hb.route_combine(z, plan, w), hb.route_combine(z, plan),
+                hb.embedding_lookup(x, ids, scale=2.0))
+
+    traced = _traced(layer, *inputs())
+    other = inputs()
+    for got, want in zip(traced(*other), layer(*other)):
+        assert torch.equal(got, want)
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_calls_that_a_trace_cannot_hold(hb, cuda):
+    gen = torch.Generator(device=cuda).manual_seed(6)
+    plan = _plan(hb, cuda, gen)
+    x, z = (torch.randn(s, generator=gen, device=cuda) for s in ((40, 8), (80, 8)))
+    ids = torch.zeros(40, dtype=torch.int64, device=cuda)
+    for call, at in ((lambda v: hb.route_plan(v, 3).order, ids), (lambda v: hb.route_dispatch_grad(v, plan), z),
+                     (lambda v: hb.route_combine_grad(v, z, plan)[0], x), (lambda v: hb.embedding_grad(v, ids, 4), x),
+                     (lambda v: hb.grad_norm([v]), x), (lambda v: hb.clip_grad_norm([v], 1.0), x)):
+        with pytest.raises(NotImplementedError, match="trace"):
+            _traced(call, at)
