@@ -41,7 +41,15 @@ int64_t integer(PyObject* o) {
     if (v == -1 && PyErr_Occurred()) throw python_error();
     return v;
 }
+// A tensor may stand for a number where no derivative is taken through it: none would come back.
 double number(PyObject* o) {
+    if (THPVariable_Check(o)) {
+        const Tensor& t = THPVariable_Unpack(o);
+        TORCH_CHECK_VALUE(!has_tangent(t) && !(t.requires_grad() && c10::GradMode::is_enabled()),
+                          "a scale or limit is a number, not a tensor that takes a derivative");
+        const Tensor plain = t.detach();
+        return plain.item().toDouble();
+    }
     const double v = PyFloat_AsDouble(o);
     if (v == -1.0 && PyErr_Occurred()) throw python_error();
     return v;
@@ -128,6 +136,14 @@ Tensor workspace(size_t bytes, c10::Device device) {
 // A trace records torch's operations and autograd functions: of a call that is neither it would keep the empty output.
 void untraced(const char* what) {
     TORCH_CHECK_NOT_IMPLEMENTED(!at::tracer::impl::is_dispatch_enabled(), what, " cannot be recorded in a trace");
+}
+
+// number(value) -> the value as a float
+PyObject* number_of(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 1, "number");
+    return PyFloat_FromDouble(number(args[0]));
+    END_HANDLE_TH_ERRORS
 }
 
 // recorded(tensor or None, ...) -> whether a call on them has to go through its autograd function: a derivative is
@@ -423,6 +439,7 @@ PyObject* clip(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 PyMethodDef methods[] = {
+    {"number", reinterpret_cast<PyCFunction>(number_of), METH_FASTCALL, nullptr},
     {"recorded", reinterpret_cast<PyCFunction>(recorded), METH_FASTCALL, nullptr},
     {"route_plan", reinterpret_cast<PyCFunction>(route_plan), METH_FASTCALL, nullptr},
     {"route_dispatch", reinterpret_cast<PyCFunction>(route_dispatch), METH_FASTCALL, nullptr},

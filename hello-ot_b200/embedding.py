@@ -45,5 +45,5 @@ def embedding_lookup(table, ids, *, scale: float = 1.0):
     int64 of any shape.  Differentiable in the table, backward (a dense
     gradient) and forward."""
     if host().recorded(table):
-        return _Lookup.apply(table, ids, scale)
+        return _Lookup.apply(table, ids, host().number(scale))
     return host().embedding_lookup(table, ids, scale)

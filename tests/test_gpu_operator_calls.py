@@ -140,3 +140,16 @@ def test_calls_that_a_trace_cannot_hold(hb, cuda):
                      (lambda v: hb.grad_norm([v]), x), (lambda v: hb.clip_grad_norm([v], 1.0), x)):
         with pytest.raises(NotImplementedError, match="trace"):
             _traced(call, at)
+
+
+def test_numbers_carry_no_gradient(hb, cuda):
+    table, ids = torch.ones((4, 3), device=cuda), torch.zeros(2, dtype=torch.int64, device=cuda)
+    scale = torch.tensor(2.0, requires_grad=True)
+    assert torch.equal(hb.embedding_lookup(table, ids, scale=scale.detach()), 2 * table[:2])
+    with torch.no_grad():
+        hb.embedding_lookup(table, ids, scale=scale)
+    for call in (lambda: hb.embedding_lookup(table, ids, scale=scale), lambda: hb.embedding_grad(table[:2], ids, 4, scale=scale),
+                 lambda: hb.embedding_lookup(table.clone().requires_grad_(), ids, scale=scale),
+                 lambda: hb.clip_grad_norm([table], scale)):
+        with pytest.raises(ValueError, match="number"):
+            call()
