@@ -153,3 +153,11 @@ def test_numbers_carry_no_gradient(hb, cuda):
                  lambda: hb.clip_grad_norm([table], scale)):
         with pytest.raises(ValueError, match="number"):
             call()
+
+
+def test_clipping_needs_a_limit(hb, cuda):
+    g = torch.full((4,), 3.0, device=cuda)
+    out = torch.full_like(g, 7.0)
+    for kwargs in ({}, {"out": [out]}):
+        with pytest.raises((TypeError, ValueError)):
+            hb.clip_grad_norm([g], None, **kwargs)
