@@ -32,6 +32,8 @@ class _Lookup(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         ids, = ctx.saved_tensors
+        if ctx.rows == 0:
+            return dy.new_zeros((0, dy.shape[-1])), None, None
         return embedding_grad(dy, ids, ctx.rows, scale=ctx.scale), None, None
 
     @staticmethod

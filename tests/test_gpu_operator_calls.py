@@ -161,3 +161,11 @@ def test_clipping_needs_a_limit(hb, cuda):
     for kwargs in ({}, {"out": [out]}):
         with pytest.raises((TypeError, ValueError)):
             hb.clip_grad_norm([g], None, **kwargs)
+
+
+def test_lookup_of_an_empty_table_has_a_gradient(hb, cuda):
+    table = torch.empty((0, 8), device=cuda).requires_grad_()
+    y = hb.embedding_lookup(table, torch.tensor([0, -1, 3], device=cuda))
+    assert y.shape == (3, 8) and not y.any()
+    y.sum().backward()
+    assert table.grad.shape == (0, 8)
