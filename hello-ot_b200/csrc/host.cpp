@@ -356,8 +356,13 @@ PyObject* embedding_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // ---------------------------------------------------------------- clipping
+struct Extent {  // the memory of a list's tensor
+    const char *begin, *end;
+    int64_t index;
+};
 struct List {
     std::vector<Tensor> tensors;
+    std::vector<Extent> extents;  // by address, of the tensors that hold elements
     std::vector<void*> address;
     std::vector<int64_t> size;
     std::vector<int32_t> type;
@@ -368,7 +373,7 @@ List list_of(PyObject* o, const char* what, c10::Device* device) {
     if (!items) throw python_error();
     const Py_ssize_t n = PySequence_Fast_GET_SIZE(items.get());
     List l;
-    l.tensors.reserve(n), l.address.reserve(n), l.size.reserve(n), l.type.reserve(n);
+    l.tensors.reserve(n), l.extents.reserve(n), l.address.reserve(n), l.size.reserve(n), l.type.reserve(n);
     for (Py_ssize_t i = 0; i < n; ++i) {
         const Tensor& t = tensor(PySequence_Fast_GET_ITEM(items.get(), i), "a gradient");
         if (i == 0 && !device->is_cuda()) *device = device_of(what, {&t});
@@ -381,12 +386,29 @@ List list_of(PyObject* o, const char* what, c10::Device* device) {
         l.tensors.push_back(t);
         l.size.push_back(t.numel());
         l.address.push_back(t.numel() ? t.data_ptr() : nullptr);
+        if (t.numel()) {
+            const char* begin = static_cast<const char*>(l.address.back());
+            l.extents.push_back({begin, begin + t.nbytes(), i});
+        }
     }
-    std::vector<void*> sorted(l.address);
-    std::sort(sorted.begin(), sorted.end());
-    for (size_t i = 1; i < sorted.size(); ++i)
-        TORCH_CHECK_VALUE(!sorted[i] || sorted[i] != sorted[i - 1], what, ": a tensor is listed twice");
+    std::sort(l.extents.begin(), l.extents.end(), [](const Extent& a, const Extent& b) { return a.begin < b.begin; });
+    for (size_t i = 1; i < l.extents.size(); ++i)
+        TORCH_CHECK_VALUE(l.extents[i].begin != l.extents[i - 1].begin, what, ": a tensor is listed twice");
     return l;
+}
+// Blocks write the outputs while others still read the gradients: outputs share no memory with one another, nor with a
+// gradient unless it is their own and they are in place.
+void check_shared(const List& grads, const List& outs, const char* what) {
+    const std::vector<Extent>& to = outs.extents;
+    for (size_t i = 1; i < to.size(); ++i)
+        TORCH_CHECK_VALUE(to[i].begin >= to[i - 1].end, what, ": tensors that are written overlap in memory");
+    if (&grads == &outs) return;
+    for (const Extent& g : grads.extents) {
+        auto o = std::upper_bound(to.begin(), to.end(), g.begin, [](const char* p, const Extent& e) { return p < e.end; });
+        for (; o != to.end() && o->begin < g.end; ++o)
+            TORCH_CHECK_VALUE(o->index == g.index && o->begin == g.begin && o->end == g.end, what,
+                              ": an output overlaps a gradient in memory and is not in its place");
+    }
 }
 
 // clip(gradients, limit or None, outputs or None, name) -> norm
@@ -422,6 +444,7 @@ PyObject* clip(PyObject*, PyObject* const* args, Py_ssize_t n) {
                               o.scalar_type(), " for ", g.scalar_type());
         }
     }
+    if (scale) check_shared(grads, *to, what);
     Tensor norm = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(device));
     const size_t size = hb_clip_workspace(count);
     Tensor ws = workspace(size, device);

@@ -169,3 +169,38 @@ def test_lookup_of_an_empty_table_has_a_gradient(hb, cuda):
     assert y.shape == (3, 8) and not y.any()
     y.sum().backward()
     assert table.grad.shape == (0, 8)
+
+
+def test_clipping_refuses_shared_memory(hb, cuda):
+    """Outputs that overlap one another, or a gradient that is not their own, would be written while they are read."""
+    flat = torch.arange(1.0, 65.0, device=cuda)
+    a, b = flat[:16], flat[16:32]
+    half = torch.ones(32, dtype=torch.bfloat16, device=cuda)
+    kept = flat.clone()
+    for grads, out in (([a, b], [b, a]), ([a, b], [torch.empty_like(a), a]), ([flat, flat[10:20]], None), ([flat[10:20], flat], None),
+                       ([a, b], [flat[1:17], flat[32:48]]), ([a], [flat[15:31]]), ([b], [flat[1:17]]),
+                       ([kept[:16], kept[16:32]], [flat[:16], flat[15:31]]), ([half[:16]], [half.view(torch.float32)[:16]]),
+                       ([half[:8], half[8:16]], [torch.empty(8, device=cuda), half.view(torch.float32)[:8]])):
+        with pytest.raises(ValueError, match="overlap|in place"):
+            hb.clip_grad_norm(grads, 1.0, out=out)
+    assert torch.equal(flat, kept) and bool((half == 1).all())
+
+
+def test_clipping_takes_neighbours_in_memory(hb, cuda):
+    """Slices of one buffer, in place and beside it; gradients that are only read may overlap."""
+    flat = torch.arange(1.0, 65.0, device=cuda)
+    norm = hb.grad_norm([flat[:20], flat[10:30]])
+    want = torch.cat([flat[:20], flat[10:30]]).double().norm()
+    assert abs(float(norm) - float(want)) <= 17 * ref.E32 * float(want)
+    out = torch.empty(40, device=cuda)
+    assert torch.equal(hb.clip_grad_norm([flat[:20], flat[10:30]], 1.0, out=[out[20:], out[:20]]), norm)
+    factor = 1.0 / (float(want) + 1e-6)
+    for got, g in ((out[20:], flat[:20]), (out[:20], flat[10:30])):
+        assert bool(((got.double() - g.double() * factor).abs() <= 21 * ref.E32 * g.double() * factor).all())
+    both = flat.clone()
+    hb.clip_grad_norm([both[:10], both[10:64]], 1.0, out=[both[:10], both[10:64]])
+    alone = flat.clone()
+    hb.clip_grad_norm([alone[:10], alone[10:64]], 1.0)
+    assert torch.equal(both, alone) and not torch.equal(both, flat)
+    empty = flat[5:5]
+    hb.clip_grad_norm([alone, empty], 1.0, out=[both, empty])
