@@ -118,6 +118,17 @@ Rows feature_rows(const Tensor& given, const char* name) {
     return {t, t.size(0) > 1 ? t.stride(0) : width, type};
 }
 
+// Whether rows share memory with a contiguous tensor.
+bool meet(const Rows& r, const Tensor& t) {
+    if (r.t.numel() == 0 || t.numel() == 0) return false;
+    const int64_t size = r.t.element_size(), step = r.stride * size, row = r.t.size(1) * size;
+    const int64_t begin = reinterpret_cast<const char*>(t.const_data_ptr()) - reinterpret_cast<const char*>(r.t.const_data_ptr());
+    const int64_t end = begin + (int64_t)t.nbytes();  // both counted from the first row
+    if (begin < row || step == 0) return begin < row && end > 0;  // a row at step 0 is the first one again
+    const int64_t i = (begin - row) / step + 1;  // the first row that ends behind the tensor's begin
+    return i < r.t.size(0) && i * step < end;
+}
+
 // Tells autograd that a tensor of the caller's was written.
 void written(const Tensor& t) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
@@ -343,6 +354,7 @@ PyObject* embedding_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
         TORCH_CHECK_VALUE(out.scalar_type() == type && out.dim() == 2 && out.size(0) == rows && out.size(1) == width &&
                               out.is_contiguous() && !out.is_neg(),
                           what, ": out must be a contiguous ", type, " tensor of shape [", rows, ", ", width, "]");
+    TORCH_CHECK_VALUE(args[5] == Py_None || !meet(dy, out), what, ": out overlaps dy in memory");
     const Tensor ids = given.contiguous();
     const size_t size = hb_embedding_grad_workspace(count, rows, width);
     Tensor ws = workspace(size, device);

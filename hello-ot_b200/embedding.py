@@ -15,8 +15,8 @@ from ._lib import host
 def embedding_grad(dy, ids, rows: int, *, scale: float = 1.0, dtype=None, out=None, accumulate: bool = False):
     """Gradient of ``embedding_lookup`` with respect to its table: [rows, width], row v the sum of scale * dy
     over ids == v, summed in fp32 and rounded once to ``dtype`` (dy's, or float32).  ``out`` receives it;
-    ``accumulate=True`` adds it to what ``out`` holds and leaves the rows that no id names untouched.  The result
-    has no history."""
+    ``accumulate=True`` adds it to what ``out`` holds and leaves the rows that no id names untouched;
+    it shares no memory with dy.  The result has no history."""
     return host().embedding_grad(dy, ids, rows, scale, dtype, out, bool(accumulate))
 
 

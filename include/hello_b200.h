@@ -401,7 +401,7 @@ int hb_route_combine_grad(int type, const void* dy, int64_t dy_stride, const voi
 /* out[i] = scale * table[ids[i]], a zero row for an id outside 0..rows-1.  ids: int32 or
  * int64 (id_bytes).  The gradient is dense: out[v] = scale * sum of dy[i] over ids[i] = v,
  * of dy's type or fp32; accumulate != 0 adds to out instead and leaves other rows alone.
- * dy's rows start less than 2^32 bytes apart. */
+ * dy's rows start less than 2^32 bytes apart, and share no memory with out. */
 int hb_embedding_lookup(int type, const void* table, int64_t table_stride, int64_t rows, int64_t width, const void* ids,
                         int id_bytes, int64_t n, double scale, void* out, void* stream);
 size_t hb_embedding_grad_workspace(int64_t n, int64_t rows, int64_t width);

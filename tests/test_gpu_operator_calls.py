@@ -204,3 +204,27 @@ def test_clipping_takes_neighbours_in_memory(hb, cuda):
     assert torch.equal(both, alone) and not torch.equal(both, flat)
     empty = flat[5:5]
     hb.clip_grad_norm([alone, empty], 1.0, out=[both, empty])
+
+
+def test_table_gradient_refuses_to_write_its_rows(hb, cuda):
+    """out is written while dy is read: they may lie in one buffer, between rows too, but share nothing."""
+    gen = torch.Generator(device=cuda).manual_seed(8)
+    flat = torch.randn(400, generator=gen, device=cuda)
+    kept = flat.clone()
+    ids = torch.tensor([2, 0, 2, 1, -1], device=cuda)
+    dy = flat[100:200].view(5, 20)[:, :8]  # rows of 8 at 100, 120, 140, 160, 180
+    for start, rows in ((100, 5), (93, 1), (107, 1), (60, 6), (112, 2), (185, 3), (90, 20), (181, 1)):
+        out = flat[start:start + rows * 8].view(rows, 8)
+        for accumulate in (False, True):
+            with pytest.raises(ValueError, match="overlap"):
+                hb.embedding_grad(dy, ids, rows, out=out, accumulate=accumulate)
+    with pytest.raises(ValueError, match="overlap"):
+        hb.embedding_grad(flat[:8].expand(5, 8), ids, 3, out=flat[4:28].view(3, 8))
+    assert torch.equal(flat, kept)
+    for start, rows in ((76, 3), (188, 3), (108, 1), (112, 1), (170, 1)):
+        out = flat[start:start + rows * 8].view(rows, 8)
+        assert torch.equal(hb.embedding_grad(dy, ids, rows, out=out), hb.embedding_grad(kept[100:200].view(5, 20)[:, :8], ids, rows))
+        flat.copy_(kept)
+    t = flat[:40].view(8, 5).t()  # copied before it is read
+    want = hb.embedding_grad(t.contiguous(), ids, 3)
+    assert torch.equal(hb.embedding_grad(t, ids, 3, out=flat[:24].view(3, 8)), want)
