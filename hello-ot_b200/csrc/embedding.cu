@@ -123,33 +123,14 @@ struct Grad {
     int rows_per_warp;
 };
 
-// Adds N values to fp32 ones in memory without waiting for them.  An element gets one addition a call, so the
-// order of a launch's additions does not matter.
-template <int N>
-__device__ __forceinline__ void add_in_memory(float* p, const float (&v)[N]) {
-    if constexpr (N % 4 == 0) {
-#pragma unroll
-        for (int i = 0; i < N; i += 4)
-            atomicAdd(reinterpret_cast<float4*>(p + i), make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
-    } else if constexpr (N == 2) {
-        atomicAdd(reinterpret_cast<float2*>(p), make_float2(v[0], v[1]));
-    } else {
-        static_assert(N == 1, "vectors have 1, 2, 4 or 8 elements");
-        atomicAdd(p, v[0]);
-    }
-}
-
+// A row is written by one group alone, so adding to what is there needs no atomics.  Atomic additions would not wait for
+// the old values (92503 tokens added into 105992 x 368 f32 75 us against 99, x 369 97 against 142), but round the sum
+// before they add it and, on fp32 in global memory, may flush subnormal values to zero.
 template <typename T, typename TO, int N>
 __device__ __forceinline__ void write_row(const Grad<T, TO>& g, uint32_t key, int64_t c, const float (&sum)[N]) {
     TO* to = g.out + (int64_t)key * g.width + c;
     float r[N];
     if (g.accumulate) {
-        if constexpr (sizeof(TO) == 4) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) r[i] = g.scale * sum[i];
-            add_in_memory<N>(to, r);
-            return;
-        }
         Values<TO, N>::load(to, r);
 #pragma unroll
         for (int i = 0; i < N; ++i) r[i] = fmaf(g.scale, sum[i], r[i]);

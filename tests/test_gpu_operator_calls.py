@@ -228,3 +228,23 @@ def test_table_gradient_refuses_to_write_its_rows(hb, cuda):
     t = flat[:40].view(8, 5).t()  # copied before it is read
     want = hb.embedding_grad(t.contiguous(), ids, 3)
     assert torch.equal(hb.embedding_grad(t, ids, 3, out=flat[:24].view(3, 8)), want)
+
+
+@pytest.mark.parametrize("dtype", ref.DTYPES)
+@pytest.mark.parametrize("width", [64, 2, 1])
+def test_accumulated_subnormals(hb, cuda, dtype, width):
+    """Values below fp32's least normal number are added like any other, and a sum is rounded once: with rows of
+    one token the result is scale * dy + out in 64 bits, rounded to fp32 at the end."""
+    rng = np.random.default_rng(width)
+    n, rows = 50, 60
+    tiny = 2.0 ** -140
+    scale = 0.75 if dtype == torch.float32 else 2.0 ** -130  # of fp16's range, products below it
+    size = tiny if dtype == torch.float32 else 1.0
+    dy = torch.as_tensor(rng.normal(size=(n, width)) * size, device=cuda).to(dtype)
+    ids = torch.as_tensor(rng.permutation(rows)[:n], device=cuda)
+    base = torch.as_tensor(rng.normal(size=(rows, width)) * tiny, device=cuda).to(torch.float32)
+    out = base.clone()
+    hb.embedding_grad(dy, ids, rows, scale=scale, out=out, accumulate=True)
+    want = ref.f64(base)
+    want[ids.cpu().numpy()] += ref.f64(dy) * scale
+    assert np.array_equal(ref.f64(out), want.astype(np.float32).astype(np.float64))
