@@ -489,22 +489,26 @@ inline Layout layout(void* ws, int64_t n, int64_t bins, const Plan& p) {
     return l;
 }
 
-inline size_t cluster_smem(const Plan& p) {
-    return (size_t)(3 * p.digits + 1) / 2 * 8 + (p.passes > 1 ? (size_t)p.rounds * kBlock * 8 : 0) +
-           (size_t)p.digits * 2 * kBlockWarps;
+constexpr size_t cluster_smem(int digits, int passes, int rounds) {
+    return (size_t)(3 * digits + 1) / 2 * 8 + (passes > 1 ? (size_t)rounds * kBlock * 8 : 0) +
+           (size_t)digits * 2 * kBlockWarps;
 }
-inline size_t place_smem(const Plan& p) { return (size_t)p.digits * (12 + 2 * kWarps); }
+constexpr size_t place_smem(int digits) { return (size_t)digits * (12 + 2 * kWarps); }
 
-// Dynamic shared memory above 48 KB has to be allowed for the kernel.
+// Dynamic shared memory above 48 KB has to be allowed for the kernel, a setting that the process's calls share: always
+// the most that any plan takes (plan_of: at most 2^kMaxDigitBits digits), so that no thread's call lowers another's.
+constexpr size_t kClusterSmem = cluster_smem(1 << kMaxDigitBits, 2, kRounds), kPlaceSmem = place_smem(1 << kMaxDigitBits);
+static_assert(kClusterSmem <= 227 * 1024 && kPlaceSmem <= 227 * 1024, "shared memory of a block");
 template <typename K>
-inline cudaError_t allow(K* kernel, size_t bytes) {
+inline cudaError_t allow(K* kernel, size_t bytes, size_t most) {
     if (bytes <= 48 * 1024) return cudaSuccess;
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
 }
 
 cudaError_t sort_one_launch(const Source& src, int n, const Plan& p, int32_t* order, int32_t* position, uint2* pairs,
                             int32_t* offsets, uint32_t* zero, int64_t zeros, cudaStream_t st) {
-    cudaError_t e = allow(sort_cluster, cluster_smem(p));
+    const size_t smem = cluster_smem(p.digits, p.passes, p.rounds);
+    cudaError_t e = allow(sort_cluster, smem, kClusterSmem);
     if (e == cudaSuccess && p.cluster > 8)
         e = cudaFuncSetAttribute(sort_cluster, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
@@ -515,7 +519,7 @@ cudaError_t sort_one_launch(const Source& src, int n, const Plan& p, int32_t* or
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(p.cluster);
     config.blockDim = dim3(kBlock);
-    config.dynamicSmemBytes = cluster_smem(p);
+    config.dynamicSmemBytes = smem;
     config.stream = st;
     config.attrs = &attr;
     config.numAttrs = 1;
@@ -527,8 +531,9 @@ cudaError_t sort_one_launch(const Source& src, int n, const Plan& p, int32_t* or
 template <int ROUNDS, bool SCANNED>
 cudaError_t sort_tiles(const Source& input, int64_t n, const Plan& p, const Layout& l, int32_t* order, int32_t* position,
                        uint2* pairs, int32_t* offsets, uint32_t* zero, int64_t zeros, cudaStream_t st) {
-    cudaError_t e = allow(tile_place<ROUNDS, SCANNED, true>, place_smem(p));
-    if (e == cudaSuccess) e = allow(tile_place<ROUNDS, SCANNED, false>, place_smem(p));
+    const size_t smem = place_smem(p.digits);
+    cudaError_t e = allow(tile_place<ROUNDS, SCANNED, true>, smem, kPlaceSmem);
+    if (e == cudaSuccess) e = allow(tile_place<ROUNDS, SCANNED, false>, smem, kPlaceSmem);
     if (e != cudaSuccess) return e;
     const uint32_t mask = (1u << p.digit_bits) - 1u;
     const int64_t counted = (int64_t)words_of(p.digits) * p.tiles;  // words of a pass (SCANNED has one area)
@@ -539,8 +544,8 @@ cudaError_t sort_tiles(const Source& input, int64_t n, const Plan& p, const Layo
         uint2* to = last ? pairs : l.pairs[pass & 1];
         uint32_t* counts = l.counts + (SCANNED ? 0 : pass * counted);
         if (SCANNED || pass == 0) {
-            const size_t smem = sizeof(uint32_t) * (SCANNED ? p.digits : words_of(p.digits));
-            tile_counts<ROUNDS, SCANNED><<<p.tiles, kThreads, smem, st>>>(
+            const size_t counted_smem = sizeof(uint32_t) * (SCANNED ? p.digits : words_of(p.digits));
+            tile_counts<ROUNDS, SCANNED><<<p.tiles, kThreads, counted_smem, st>>>(
                 src, n, shift, mask, p.digits, p.tiles, counts, l.counts + counted,
                 SCANNED ? 0 : counted * (p.passes - 1), zero, pass == 0 ? zeros : 0);
             count_launches(1);
@@ -550,7 +555,7 @@ cudaError_t sort_tiles(const Source& input, int64_t n, const Plan& p, const Layo
             count_launches(1);
         }
         const auto place = pass == 0 ? tile_place<ROUNDS, SCANNED, true> : tile_place<ROUNDS, SCANNED, false>;
-        e = launch_next(place, p.tiles, kThreads, place_smem(p), st, src, n, shift, mask, p.digits, p.tiles, counts,
+        e = launch_next(place, p.tiles, kThreads, smem, st, src, n, shift, mask, p.digits, p.tiles, counts,
                         l.totals, SCANNED || last ? nullptr : counts + counted, shift + p.digit_bits,
                         last ? order : nullptr, last ? position : nullptr, to,
                         last && p.passes == 1 ? offsets : nullptr);

@@ -1,4 +1,6 @@
 """What the routing, lookup and clipping calls keep to beside their results on ordinary arguments."""
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -248,3 +250,40 @@ def test_accumulated_subnormals(hb, cuda, dtype, width):
     want = ref.f64(base)
     want[ids.cpu().numpy()] += ref.f64(dy) * scale
     assert np.array_equal(ref.f64(out), want.astype(np.float32).astype(np.float64))
+
+
+def test_sorts_from_two_threads(hb, cuda):
+    """The C entries share nothing between calls: two host threads sort by different numbers of bins, whose kernels
+    differ in shared memory."""
+    lib, n = hb.load_library(), 30_000
+    gen = torch.Generator(device=cuda).manual_seed(9)
+    failed = []
+
+    def work(n, bins, stream):
+        index = torch.randint(0, bins, (n,), generator=gen, device=cuda, dtype=torch.int32)
+        order, position = (torch.empty(n, dtype=torch.int32, device=cuda) for _ in range(2))
+        offsets = torch.empty(bins + 1, dtype=torch.int32, device=cuda)
+        size = lib.hb_index_sort_workspace(n, bins)
+        ws = torch.empty(max(size, 1), dtype=torch.uint8, device=cuda)
+        torch.cuda.synchronize()
+
+        def loop():
+            for _ in range(400):
+                rc = lib.hb_index_sort(index.data_ptr(), 4, n, bins, order.data_ptr(), position.data_ptr(),
+                                       offsets.data_ptr(), ws.data_ptr(), size, stream.cuda_stream)
+                if rc:
+                    failed.append((bins, rc, lib.hb_last_error()))
+                    return
+        return loop, index, order
+
+    for n in (30_000, 100_000):
+        jobs = [work(n, bins, torch.cuda.Stream()) for bins in (2000, 900)]
+        threads = [threading.Thread(target=job[0]) for job in jobs]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        assert not failed, failed
+        for _, index, order in jobs:
+            assert torch.equal(order.long(), torch.sort(index, stable=True).indices)
