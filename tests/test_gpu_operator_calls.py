@@ -287,3 +287,21 @@ def test_sorts_from_two_threads(hb, cuda):
         assert not failed, failed
         for _, index, order in jobs:
             assert torch.equal(order.long(), torch.sort(index, stable=True).indices)
+
+
+@pytest.mark.parametrize("sizes", [[1 << 19], [8000 - i for i in range(64)], [100_000, 8192 * 20 + 5, 3], [8193] * 31])
+def test_clipping_in_place_in_one_launch(hb, cuda, sizes):
+    """More chunks than the cluster has blocks: in place the same values as beside, and those within the bounds."""
+    gen = torch.Generator(device=cuda).manual_seed(len(sizes))
+    for dtype in ref.DTYPES:
+        grads = [torch.randn(n, generator=gen, device=cuda).to(dtype) for n in sizes]
+        norm = float(torch.stack([g.double().square().sum() for g in grads]).sum().sqrt())
+        out = [torch.empty_like(g) for g in grads]
+        got = hb.clip_grad_norm(grads, 0.5 * norm, out=out)
+        assert abs(float(got) - norm) <= 17 * ref.E32 * norm
+        factor = 0.5 * norm / (norm + 1e-6)
+        for g, o in zip(grads, out):
+            want = ref.f64(g) * factor
+            ref.assert_within(o, want, (20 * ref.E32 * (1 + ref.U[dtype]) + ref.U[dtype]) * np.abs(want) + ref.FLOOR[dtype])
+        assert torch.equal(hb.clip_grad_norm(grads, 0.5 * norm), got)
+        assert all(torch.equal(g, o) for g, o in zip(grads, out))
