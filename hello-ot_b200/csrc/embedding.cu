@@ -242,12 +242,13 @@ __device__ __forceinline__ void add_vector(float (&sum)[Vec<T, VB>::N], const Ve
     if (N % 2) sum[N - 1] += rows::to_float(v.v[N - 1]);
 }
 
-// The rows and tokens of 8 consecutive places; the array is padded to whole groups of 8.
+// The rows and tokens of 8 consecutive places; the array is padded to whole groups of 8.  Plain loads: the sort may
+// still be writing them when this kernel starts (after_last), which rules out the read-only path.
 __device__ __forceinline__ void load8(const uint2* pairs, uint32_t (&row)[8], uint32_t (&token)[8]) {
     const uint4* p = reinterpret_cast<const uint4*>(pairs);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint4 v = __ldg(p + i);
+        const uint4 v = p[i];
         row[2 * i] = v.x, token[2 * i] = v.y, row[2 * i + 1] = v.z, token[2 * i + 1] = v.w;
     }
 }

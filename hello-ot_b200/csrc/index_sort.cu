@@ -338,10 +338,12 @@ __global__ void __launch_bounds__(256) scan_tiles(uint32_t* __restrict__ counts,
 // Places a tile's entries.  SCANNED: counts and totals as scan_tiles leaves them; else the tiles' packed counts,
 // and the digits of the next pass are counted into `next` (cleared before), tile by tile of where entries go.
 // FIRST: the first pass, whose keys are the caller's: the block ranks them while the counts are still being made.
+// counts and totals are written while this kernel may already run, so they are not declared unaliased: the compiler
+// could read them before after_last(), or through the read-only path.
 template <int ROUNDS, bool SCANNED, bool FIRST>
 __global__ void __launch_bounds__(kThreads) tile_place(Source src, int64_t n, int shift, uint32_t mask, int digits,
-                                                       int tiles, const uint32_t* __restrict__ counts,
-                                                       const uint32_t* __restrict__ totals, uint32_t* __restrict__ next,
+                                                       int tiles, const uint32_t* counts, const uint32_t* totals,
+                                                       uint32_t* __restrict__ next,
                                                        int next_shift, int32_t* __restrict__ order,
                                                        int32_t* __restrict__ position, uint2* __restrict__ pairs,
                                                        int32_t* __restrict__ offsets) {
@@ -419,7 +421,7 @@ __global__ void __launch_bounds__(kThreads) tile_place(Source src, int64_t n, in
 }
 
 // offsets[b] = first place whose key is not below b.
-__global__ void __launch_bounds__(256) find_offsets(const uint2* __restrict__ pairs, int64_t n, int64_t bins,
+__global__ void __launch_bounds__(256) find_offsets(const uint2* pairs, int64_t n, int64_t bins,
                                                     int32_t* __restrict__ offsets) {
     const int64_t b = (int64_t)blockIdx.x * 256 + threadIdx.x;
     after_last();

@@ -10,7 +10,8 @@ namespace hb {
 // lets the next one of the row start with allow_next(), and calls after_last() before it reads what earlier ones
 // of the row wrote, or writes what they read; after_last() returns when the kernel before has ended and its
 // writes are there, and that one waited for its own.  The first kernel of a row is launched plainly, so
-// before after_last() everything older than the row is done.
+// before after_last() everything older than the row is done.  What a row's earlier kernels write is read by plain loads
+// from pointers without __restrict__: it is not constant for the whole of a later kernel.
 __device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void after_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 template <typename... P, typename... A>

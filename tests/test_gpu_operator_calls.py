@@ -305,3 +305,80 @@ def test_clipping_in_place_in_one_launch(hb, cuda, sizes):
             ref.assert_within(o, want, (20 * ref.E32 * (1 + ref.U[dtype]) + ref.U[dtype]) * np.abs(want) + ref.FLOOR[dtype])
         assert torch.equal(hb.clip_grad_norm(grads, 0.5 * norm), got)
         assert all(torch.equal(g, o) for g, o in zip(grads, out))
+
+
+# ------------------------------------------------------------------ launches that overlap
+@pytest.mark.parametrize("n,bins", [(1500, 9000), (30_000, 70), (30_000, 90_000), (200_000, 1024), (200_000, 100_003),
+                                    (600_000, 37), (600_000, 5000)])
+def test_captured_sorts(hb, cuda, n, bins):
+    """Every form of the sort, captured and replayed on new entries back to back; a launch of the row may start while
+    the one before ends."""
+    gen = torch.Generator(device=cuda).manual_seed(n + bins)
+    index = torch.empty(n, dtype=torch.int64, device=cuda)
+    index.random_(-1, bins, generator=gen)
+    hb.route_plan(index, bins)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan = hb.route_plan(index, bins)
+    for _ in range(20):
+        index.random_(-1, bins, generator=gen)
+        graph.replay()
+        got = [t.clone() for t in plan]
+        key = torch.where(index >= 0, index, bins)
+        keys, order = torch.sort(key, stable=True)
+        assert torch.equal(got[0].long(), order)
+        assert torch.equal(got[1].view(-1)[order].long(), torch.arange(n, device=cuda))
+        assert torch.equal(got[2].long(), torch.searchsorted(keys, torch.arange(bins + 1, device=cuda)))
+
+
+@pytest.mark.parametrize("n,rows,width", [(1000, 5003, 129), (30_000, 700, 64), (150_000, 5000, 32), (150_000, 900, 9)])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_captured_table_gradients(hb, cuda, n, rows, width, accumulate):
+    """The gradient starts while its sort ends: captured and replayed on new tokens, equal to the call, bit for bit."""
+    gen = torch.Generator(device=cuda).manual_seed(n)
+    ids = torch.empty(n, dtype=torch.int32, device=cuda)
+    dy = torch.empty((n, width), dtype=torch.bfloat16, device=cuda)
+    out = torch.zeros((rows, width), device=cuda)
+
+    def fill():
+        ids.random_(-1, rows, generator=gen)
+        dy.normal_(generator=gen)
+
+    fill()
+    hb.embedding_grad(dy, ids, rows, out=out, accumulate=accumulate)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        hb.embedding_grad(dy, ids, rows, out=out, accumulate=accumulate)
+    for _ in range(10):
+        fill()
+        want = out.clone()
+        graph.replay()
+        assert torch.equal(out, hb.embedding_grad(dy, ids, rows, out=want, accumulate=accumulate))
+
+
+def test_two_streams_at_once(hb, cuda):
+    """Calls with workspaces on two streams overlap and share nothing."""
+    gen = torch.Generator(device=cuda).manual_seed(11)
+    n, rows, width = 60_000, 3000, 96
+    jobs = [(torch.randn((n, width), generator=gen, device=cuda), torch.randint(-1, rows, (n, 2), generator=gen, device=cuda),
+             torch.randn(3_000_000, generator=gen, device=cuda)) for _ in range(2)]
+
+    def work(x, index, g):
+        plan = hb.route_plan(index, rows)
+        y = hb.route_combine(hb.route_dispatch(x, plan), plan)
+        out = torch.empty_like(g)
+        norm = hb.clip_grad_norm([g], 1.0, out=[out])
+        return [*plan, y, hb.embedding_grad(x, index[:, 0], rows), out, norm]
+
+    want = [work(*job) for job in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    for _ in range(8):
+        got = []
+        for stream, job in zip(streams, jobs):
+            with torch.cuda.stream(stream):
+                got.append(work(*job))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
