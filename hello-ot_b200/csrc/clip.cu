@@ -321,6 +321,7 @@ int check(int64_t count, const void* const* in, const int64_t* size, const int32
     if (count < 0 || count > INT32_MAX) return abi_fail(HB_BAD_ARGUMENT, "gradient norm: number of tensors out of range");
     if (!norm || !ws || (count > 0 && (!in || !size || !type)))
         return abi_fail(HB_BAD_ARGUMENT, "gradient norm: null pointer");
+    if (rows::address_bits(norm) % sizeof(float)) return abi_fail(HB_BAD_ARGUMENT, "gradient norm: misaligned pointer");
     int64_t chunks = 0;
     for (int64_t i = 0; i < count; ++i) {
         if (size[i] < 0 || !rows::valid_type(type[i]) || (size[i] > 0 && !in[i]) ||

@@ -352,8 +352,11 @@ int check(const char* what, int type, int64_t tokens, int64_t slots, int64_t wid
         return abi_fail(HB_BAD_ARGUMENT, std::string(what) + ": sizes out of range");
     if (tokens > 0 && width > 0 && (!position || !kept))
         return abi_fail(HB_BAD_ARGUMENT, std::string(what) + ": null pointer");
+    if ((rows::address_bits(position) | rows::address_bits(kept)) % sizeof(int32_t))
+        return abi_fail(HB_BAD_ARGUMENT, std::string(what) + ": misaligned pointer");
     return HB_OK;
 }
+inline bool misaligned(const void* weights, int type) { return rows::address_bits(weights) % rows::type_bytes(type) != 0; }
 int launched(const char* what) {
     count_launches(1);
     const cudaError_t e = cudaGetLastError();
@@ -378,6 +381,8 @@ extern "C" int hb_index_sort(const void* index, int index_bytes, int64_t entries
         return abi_fail(HB_BAD_ARGUMENT, "index sort: sizes out of range");
     if (!offsets || (entries > 0 && (!index || !order || !position)))
         return abi_fail(HB_BAD_ARGUMENT, "index sort: null pointer");
+    if ((rows::address_bits(order) | rows::address_bits(position) | rows::address_bits(offsets)) % sizeof(int32_t))
+        return abi_fail(HB_BAD_ARGUMENT, "index sort: misaligned pointer");
     return index_sort(index, index_bytes, entries, bins, order, position, nullptr, offsets, workspace, workspace_bytes,
                       static_cast<cudaStream_t>(stream));
 }
@@ -426,7 +431,7 @@ extern "C" int hb_route_combine(int type, const void* z, int64_t z_stride, int64
     if (!z || !out) return abi_fail(HB_BAD_ARGUMENT, "route combine: null pointer");
     const int size = rows::type_bytes(type);
     const Moves m{tokens, tokens * slots, width, (int)slots, position, kept};
-    if ((rows::address_bits(z) | rows::address_bits(out)) % size)
+    if ((rows::address_bits(z) | rows::address_bits(out)) % size || (weights && misaligned(weights, weight_type)))
         return abi_fail(HB_BAD_ARGUMENT, "route combine: misaligned pointer");
     const int vb = rows::vector_bytes(rows::address_bits(z) | rows::address_bits(out) | (uint64_t)(z_stride * size) |
                                       (uint64_t)(width * size), type);
@@ -466,7 +471,8 @@ extern "C" int hb_route_combine_grad(int type, const void* dy, int64_t dy_stride
     const Moves m{tokens, tokens * slots, width, (int)slots, position, kept};
     uint64_t bits = rows::address_bits(dy) | rows::address_bits(dz) | (uint64_t)(dy_stride * size) | (uint64_t)(width * size);
     if (dweights) bits |= rows::address_bits(z) | (uint64_t)(z_stride * size);
-    if (bits % size) return abi_fail(HB_BAD_ARGUMENT, "route combine gradient: misaligned pointer");
+    if (bits % size || (weights && misaligned(weights, weight_type)) || (dweights && misaligned(dweights, weight_type)))
+        return abi_fail(HB_BAD_ARGUMENT, "route combine gradient: misaligned pointer");
     const int vb = rows::vector_bytes(bits, type);
     const int64_t vectors = width * size / vb;
     // too few tokens to fill the SMs with a warp each: a group an entry
