@@ -216,10 +216,14 @@ def noise(src, tgt, sigma, seed, mode, coeffs):
     return float(sigma) * v.astype(np.float64)
 
 
+class ReferenceNotBuilt(RuntimeError):
+    """The reference's CPU backend is not there; its sources are not in this repository."""
+
+
 def load_ref(kind: str):
     """The reference's compiled CPU module ``hello_ot_cpp._scan`` / ``._lp``."""
     if not (REF_DIR / "hello_ot_cpp" / "__init__.py").exists():
-        raise RuntimeError("reference CPU backend not built: run `make -C oracle ref`")
+        raise ReferenceNotBuilt("reference CPU backend not built: run `make -C oracle ref`")
     if str(REF_DIR) not in sys.path:
         sys.path.insert(0, str(REF_DIR))
     return importlib.import_module(f"hello_ot_cpp._{kind}")
