@@ -59,17 +59,30 @@ void expect(Py_ssize_t got, Py_ssize_t want, const char* what) {
 }
 PyObject* wrap(const Tensor& t) { return THPVariable_Wrap(t); }
 
-// A function of hello_ot_b200._lib, for the error paths alone.
-void call_lib(const char* name, PyObject* arg) {
+// The interpreter let go, as torch's own calls do: an allocation or a launch can wait for the device, and a full launch
+// queue for work that another Python thread has to do.
+struct Unlocked {
+    PyThreadState* const state = PyEval_SaveThread();
+    Unlocked() = default;
+    Unlocked(const Unlocked&) = delete;
+    ~Unlocked() { PyEval_RestoreThread(state); }
+};
+template <typename F>
+auto unlocked(F&& work) {
+    const Unlocked now;
+    return work();
+}
+
+// A function of hello_ot_b200._lib, for the error paths alone; called while the interpreter is let go.
+void call_lib(const char* name, int arg, bool with_arg) {
+    pybind11::gil_scoped_acquire held;
     THPObjectPtr module(PyImport_ImportModule("hello_ot_b200._lib"));
     if (!module) throw python_error();
-    THPObjectPtr result(arg ? PyObject_CallMethod(module, name, "O", arg) : PyObject_CallMethod(module, name, nullptr));
+    THPObjectPtr result(with_arg ? PyObject_CallMethod(module, name, "i", arg) : PyObject_CallMethod(module, name, nullptr));
     if (!result) throw python_error();
 }
 void check(int rc) {
-    if (rc == HB_OK) return;
-    THPObjectPtr code(PyLong_FromLong(rc));
-    call_lib("check", code);
+    if (rc != HB_OK) call_lib("check", rc, true);
 }
 
 int type_or(at::ScalarType t, int otherwise) {
@@ -90,7 +103,7 @@ c10::Device device_of(const char* what, std::initializer_list<const Tensor*> ten
     const c10::Device device = (*tensors.begin())->device();
     for (const Tensor* t : tensors)
         if (!t->is_cuda() || t->device() != device) {
-            call_lib("lib", nullptr);  // without CUDA: the library's own error
+            call_lib("lib", 0, false);  // without CUDA: the library's own error
             TORCH_CHECK_VALUE(false, what, ": expected CUDA tensors on one device, got ", device, " and ", t->device());
         }
     return device;
@@ -178,21 +191,23 @@ struct Places {
     const int32_t* at() const { return position.const_data_ptr<int32_t>(); }
     const int32_t* kept() const { return offsets.const_data_ptr<int32_t>() + offsets.numel() - 1; }
 };
-Places places(PyObject* position, PyObject* offsets, const char* what) {
-    const Tensor &p = tensor(position, "position"), &o = tensor(offsets, "offsets");
+Places places(const Tensor& p, const Tensor& o, const char* what) {
     TORCH_CHECK_VALUE(p.scalar_type() == at::kInt && o.scalar_type() == at::kInt && p.dim() == 2 && o.dim() == 1, what,
                       ": a plan holds int32 position [tokens, slots] and offsets [num_experts + 1]");
     TORCH_CHECK_VALUE(p.is_contiguous() && o.is_contiguous() && o.numel() >= 2 && p.size(1) >= 1, what,
                       ": a plan's tensors are contiguous, with at least one slot and one expert");
     return {p, o, p.size(0), p.size(1)};
 }
-Tensor weights_of(PyObject* w, const Places& p, const char* what) {
-    const Tensor t = resolved(tensor(w, "weights"));
+Tensor weights_of(const Tensor& given, const Places& p, const char* what) {
+    const Tensor t = resolved(given);
     type_of(t, "weights");
     TORCH_CHECK_VALUE(t.sizes() == p.position.sizes() || (t.dim() == 1 && p.slots == 1 && t.size(0) == p.tokens), what,
                       ": weights ", t.sizes(), " do not fit an assignment ", p.position.sizes());
     return t.contiguous();
 }
+
+// A tensor, or an undefined one for None.
+Tensor tensor_or_none(PyObject* o, const char* name) { return o == Py_None ? Tensor() : tensor(o, name); }
 
 // route_plan(index, num_experts) -> (order, position, offsets)
 PyObject* route_plan(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -200,24 +215,28 @@ PyObject* route_plan(PyObject*, PyObject* const* args, Py_ssize_t n) {
     expect(n, 2, "route_plan");
     untraced("route_plan");
     const Tensor& given = tensor(args[0], "index");
-    TORCH_CHECK_VALUE(given.dim() == 1 || (given.dim() == 2 && given.size(1) >= 1),
-                      "index must be [tokens] or [tokens, slots], got ", given.sizes());
-    const int bytes = index_bytes(given, "index");
-    const int64_t experts = integer(args[1]), entries = given.numel();
-    TORCH_CHECK_VALUE(experts >= 1 && experts < INT32_MAX, "num_experts must be positive and below 2^31 - 1");
-    TORCH_CHECK_VALUE(entries <= INT32_MAX, "an assignment holds at most 2^31 - 1 entries");
-    const c10::Device device = device_of("route_plan", {&given});
-    const Tensor index = given.contiguous();
-    const auto options = at::TensorOptions().dtype(at::kInt).device(device);
-    Tensor order = at::empty({entries}, options), offsets = at::empty({experts + 1}, options);
-    Tensor position = at::empty({index.size(0), index.dim() == 2 ? index.size(1) : 1}, options);
-    const size_t size = hb_index_sort_workspace(entries, experts);
-    Tensor ws;
-    if (size) ws = workspace(size, device);
-    const Launch on(device);
-    check(hb_index_sort(index.const_data_ptr(), bytes, entries, experts, order.data_ptr<int32_t>(),
-                        position.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(), size ? ws.data_ptr() : nullptr, size,
-                        on.stream));
+    const int64_t experts = integer(args[1]);
+    Tensor order, position, offsets;
+    unlocked([&] {
+        TORCH_CHECK_VALUE(given.dim() == 1 || (given.dim() == 2 && given.size(1) >= 1),
+                          "index must be [tokens] or [tokens, slots], got ", given.sizes());
+        const int bytes = index_bytes(given, "index");
+        const int64_t entries = given.numel();
+        TORCH_CHECK_VALUE(experts >= 1 && experts < INT32_MAX, "num_experts must be positive and below 2^31 - 1");
+        TORCH_CHECK_VALUE(entries <= INT32_MAX, "an assignment holds at most 2^31 - 1 entries");
+        const c10::Device device = device_of("route_plan", {&given});
+        const Tensor index = given.contiguous();
+        const auto options = at::TensorOptions().dtype(at::kInt).device(device);
+        order = at::empty({entries}, options), offsets = at::empty({experts + 1}, options);
+        position = at::empty({index.size(0), index.dim() == 2 ? index.size(1) : 1}, options);
+        const size_t size = hb_index_sort_workspace(entries, experts);
+        Tensor ws;
+        if (size) ws = workspace(size, device);
+        const Launch on(device);
+        check(hb_index_sort(index.const_data_ptr(), bytes, entries, experts, order.data_ptr<int32_t>(),
+                            position.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(), size ? ws.data_ptr() : nullptr, size,
+                            on.stream));
+    });
     THPObjectPtr result(PyTuple_New(3));
     if (!result) throw python_error();
     PyTuple_SET_ITEM(result.get(), 0, wrap(order));
@@ -231,15 +250,18 @@ PyObject* route_plan(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* route_dispatch(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     expect(n, 3, "route_dispatch");
-    const Rows x = feature_rows(tensor(args[0], "x"), "x");
-    const Places p = places(args[1], args[2], "route_dispatch");
-    TORCH_CHECK_VALUE(x.t.size(0) == p.tokens, "route_dispatch: x has ", x.t.size(0), " rows for ", p.tokens, " tokens");
-    const c10::Device device = device_of("route_dispatch", {&x.t, &p.position, &p.offsets});
-    Tensor out = at::empty({p.tokens * p.slots, x.t.size(1)}, x.t.options());
-    const Launch on(device);
-    check(hb_route_dispatch(x.type, x.t.const_data_ptr(), x.stride, p.tokens, p.slots, x.t.size(1), p.at(), p.kept(),
-                            out.data_ptr(), on.stream));
-    return wrap(out);
+    const Tensor &given = tensor(args[0], "x"), &position = tensor(args[1], "position"), &offsets = tensor(args[2], "offsets");
+    return wrap(unlocked([&] {
+        const Rows x = feature_rows(given, "x");
+        const Places p = places(position, offsets, "route_dispatch");
+        TORCH_CHECK_VALUE(x.t.size(0) == p.tokens, "route_dispatch: x has ", x.t.size(0), " rows for ", p.tokens, " tokens");
+        const c10::Device device = device_of("route_dispatch", {&x.t, &p.position, &p.offsets});
+        Tensor out = at::empty({p.tokens * p.slots, x.t.size(1)}, x.t.options());
+        const Launch on(device);
+        check(hb_route_dispatch(x.type, x.t.const_data_ptr(), x.stride, p.tokens, p.slots, x.t.size(1), p.at(), p.kept(),
+                                out.data_ptr(), on.stream));
+        return out;
+    }));
     END_HANDLE_TH_ERRORS
 }
 
@@ -250,20 +272,24 @@ PyObject* route_combine(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const char* what = PyUnicode_AsUTF8(args[4]);
     if (!what) throw python_error();
     if (std::strcmp(what, "route_combine") != 0) untraced(what);  // by the name of another call it has no function of its own
-    const Rows z = feature_rows(tensor(args[0], "z"), "z");
-    const Places p = places(args[1], args[2], what);
-    TORCH_CHECK_VALUE(z.t.size(0) == p.tokens * p.slots, what, ": ", z.t.size(0), " sorted rows for ", p.tokens, " x ",
-                      p.slots, " entries");
-    Tensor weights;
-    if (args[3] != Py_None) weights = weights_of(args[3], p, what);
-    const bool weighted = weights.defined();
-    const c10::Device device = device_of(what, {&z.t, &p.position, &p.offsets, weighted ? &weights : &z.t});
-    Tensor out = at::empty({p.tokens, z.t.size(1)}, z.t.options());
-    const Launch on(device);
-    check(hb_route_combine(z.type, z.t.const_data_ptr(), z.stride, p.tokens, p.slots, z.t.size(1), p.at(), p.kept(),
-                           weighted ? weights.const_data_ptr() : nullptr, weighted ? type_of(weights, "weights") : 0,
-                           out.data_ptr(), on.stream));
-    return wrap(out);
+    const Tensor &given = tensor(args[0], "z"), &position = tensor(args[1], "position"), &offsets = tensor(args[2], "offsets");
+    const Tensor given_weights = tensor_or_none(args[3], "weights");
+    return wrap(unlocked([&] {
+        const Rows z = feature_rows(given, "z");
+        const Places p = places(position, offsets, what);
+        TORCH_CHECK_VALUE(z.t.size(0) == p.tokens * p.slots, what, ": ", z.t.size(0), " sorted rows for ", p.tokens, " x ",
+                          p.slots, " entries");
+        const bool weighted = given_weights.defined();
+        Tensor weights;
+        if (weighted) weights = weights_of(given_weights, p, what);
+        const c10::Device device = device_of(what, {&z.t, &p.position, &p.offsets, weighted ? &weights : &z.t});
+        Tensor out = at::empty({p.tokens, z.t.size(1)}, z.t.options());
+        const Launch on(device);
+        check(hb_route_combine(z.type, z.t.const_data_ptr(), z.stride, p.tokens, p.slots, z.t.size(1), p.at(), p.kept(),
+                               weighted ? weights.const_data_ptr() : nullptr, weighted ? type_of(weights, "weights") : 0,
+                               out.data_ptr(), on.stream));
+        return out;
+    }));
     END_HANDLE_TH_ERRORS
 }
 
@@ -273,24 +299,31 @@ PyObject* route_combine_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const char* what = "route_combine_grad";
     expect(n, 6, what);
     untraced(what);
-    const Rows dy = feature_rows(tensor(args[0], "dy"), "dy"), z = feature_rows(tensor(args[1], "z"), "z");
-    const Places p = places(args[2], args[3], what);
-    const int64_t width = z.t.size(1);
-    TORCH_CHECK_VALUE(dy.t.size(0) == p.tokens && dy.t.size(1) == width && z.t.size(0) == p.tokens * p.slots &&
-                          dy.type == z.type,
-                      what, ": dy ", dy.t.sizes(), " ", dy.t.scalar_type(), " and z ", z.t.sizes(), " ", z.t.scalar_type(),
-                      " do not fit an assignment ", p.position.sizes());
-    Tensor weights, dw;
-    if (args[4] != Py_None) weights = weights_of(args[4], p, what);
-    const bool weighted = weights.defined();
-    const c10::Device device = device_of(what, {&z.t, &dy.t, &p.position, &p.offsets, weighted ? &weights : &z.t});
-    if (weighted && args[5] == Py_True) dw = at::empty_like(weights);
-    Tensor dz = at::empty({p.tokens * p.slots, width}, z.t.options());
-    const Launch on(device);
-    check(hb_route_combine_grad(z.type, dy.t.const_data_ptr(), dy.stride, z.t.const_data_ptr(), z.stride, p.tokens, p.slots,
-                                width, p.at(), p.kept(), weighted ? weights.const_data_ptr() : nullptr,
-                                weighted ? type_of(weights, "weights") : 0, dz.data_ptr(),
-                                dw.defined() ? dw.data_ptr() : nullptr, on.stream));
+    const Tensor &given_dy = tensor(args[0], "dy"), &given_z = tensor(args[1], "z");
+    const Tensor &position = tensor(args[2], "position"), &offsets = tensor(args[3], "offsets");
+    const Tensor given_weights = tensor_or_none(args[4], "weights");
+    const bool need_weights = args[5] == Py_True;
+    Tensor dz, dw;
+    unlocked([&] {
+        const Rows dy = feature_rows(given_dy, "dy"), z = feature_rows(given_z, "z");
+        const Places p = places(position, offsets, what);
+        const int64_t width = z.t.size(1);
+        TORCH_CHECK_VALUE(dy.t.size(0) == p.tokens && dy.t.size(1) == width && z.t.size(0) == p.tokens * p.slots &&
+                              dy.type == z.type,
+                          what, ": dy ", dy.t.sizes(), " ", dy.t.scalar_type(), " and z ", z.t.sizes(), " ",
+                          z.t.scalar_type(), " do not fit an assignment ", p.position.sizes());
+        const bool weighted = given_weights.defined();
+        Tensor weights;
+        if (weighted) weights = weights_of(given_weights, p, what);
+        const c10::Device device = device_of(what, {&z.t, &dy.t, &p.position, &p.offsets, weighted ? &weights : &z.t});
+        if (weighted && need_weights) dw = at::empty_like(weights);
+        dz = at::empty({p.tokens * p.slots, width}, z.t.options());
+        const Launch on(device);
+        check(hb_route_combine_grad(z.type, dy.t.const_data_ptr(), dy.stride, z.t.const_data_ptr(), z.stride, p.tokens,
+                                    p.slots, width, p.at(), p.kept(), weighted ? weights.const_data_ptr() : nullptr,
+                                    weighted ? type_of(weights, "weights") : 0, dz.data_ptr(),
+                                    dw.defined() ? dw.data_ptr() : nullptr, on.stream));
+    });
     THPObjectPtr result(PyTuple_New(2));
     if (!result) throw python_error();
     PyTuple_SET_ITEM(result.get(), 0, wrap(dz));
@@ -304,19 +337,22 @@ PyObject* route_combine_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* embedding_lookup(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     expect(n, 3, "embedding_lookup");
-    const Tensor& given = tensor(args[1], "ids");
-    const int bytes = index_bytes(given, "ids");
-    const Rows table = feature_rows(tensor(args[0], "table"), "table");
-    const c10::Device device = device_of("embedding_lookup", {&table.t, &given});
-    TORCH_CHECK_VALUE(given.numel() <= INT32_MAX, "embedding_lookup: at most 2^31 - 1 ids");
-    const Tensor ids = given.contiguous();
-    c10::SmallVector<int64_t, 8> shape(ids.sizes().begin(), ids.sizes().end());
-    shape.push_back(table.t.size(1));
-    Tensor out = at::empty(shape, table.t.options());
-    const Launch on(device);
-    check(hb_embedding_lookup(table.type, table.t.const_data_ptr(), table.stride, table.t.size(0), table.t.size(1),
-                              ids.const_data_ptr(), bytes, ids.numel(), number(args[2]), out.data_ptr(), on.stream));
-    return wrap(out);
+    const Tensor &given = tensor(args[1], "ids"), &given_table = tensor(args[0], "table");
+    const double scale = number(args[2]);
+    return wrap(unlocked([&] {
+        const int bytes = index_bytes(given, "ids");
+        const Rows table = feature_rows(given_table, "table");
+        const c10::Device device = device_of("embedding_lookup", {&table.t, &given});
+        TORCH_CHECK_VALUE(given.numel() <= INT32_MAX, "embedding_lookup: at most 2^31 - 1 ids");
+        const Tensor ids = given.contiguous();
+        c10::SmallVector<int64_t, 8> shape(ids.sizes().begin(), ids.sizes().end());
+        shape.push_back(table.t.size(1));
+        Tensor out = at::empty(shape, table.t.options());
+        const Launch on(device);
+        check(hb_embedding_lookup(table.type, table.t.const_data_ptr(), table.stride, table.t.size(0), table.t.size(1),
+                                  ids.const_data_ptr(), bytes, ids.numel(), scale, out.data_ptr(), on.stream));
+        return out;
+    }));
     END_HANDLE_TH_ERRORS
 }
 
@@ -327,43 +363,45 @@ PyObject* embedding_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
     expect(n, 7, what);
     untraced(what);
     const Tensor &dy_given = tensor(args[0], "dy"), &given = tensor(args[1], "ids");
-    const int bytes = index_bytes(given, "ids");
-    const int64_t count = given.numel(), rows = integer(args[2]);
-    TORCH_CHECK_VALUE(dy_given.dim() >= 1 && dy_given.sizes().slice(0, dy_given.dim() - 1) == given.sizes(), what, ": dy ",
-                      dy_given.sizes(), " does not fit ids ", given.sizes());
-    const int64_t width = dy_given.size(-1);
-    TORCH_CHECK_VALUE(rows >= 1 && rows < INT32_MAX, what, ": rows must be positive and below 2^31 - 1");
-    TORCH_CHECK_VALUE(count <= INT32_MAX, what, ": at most 2^31 - 1 ids");
-    Rows dy = feature_rows(dy_given.dim() == 2 ? dy_given : dy_given.reshape({count, width}), "dy");
-    if (dy.stride * dy.t.element_size() > (int64_t)UINT32_MAX) dy = {dy.t.contiguous(), width, dy.type};
+    const int64_t rows = integer(args[2]);
+    const double scale = number(args[3]);
+    TORCH_CHECK_VALUE(args[4] == Py_None || THPDtype_Check(args[4]), what, ": dtype must be a torch.dtype");
+    const Tensor given_out = tensor_or_none(args[5], "out");
+    at::ScalarType type = given_out.defined() ? given_out.scalar_type() : dy_given.scalar_type();
+    if (args[4] != Py_None) type = reinterpret_cast<THPDtype*>(args[4])->scalar_type;
     const bool accumulate = args[6] == Py_True;
-    Tensor out;
-    if (args[5] != Py_None) out = tensor(args[5], "out");
-    at::ScalarType type = out.defined() ? out.scalar_type() : dy.t.scalar_type();
-    if (args[4] != Py_None) {
-        TORCH_CHECK_VALUE(THPDtype_Check(args[4]), what, ": dtype must be a torch.dtype");
-        type = reinterpret_cast<THPDtype*>(args[4])->scalar_type;
-    }
-    TORCH_CHECK_VALUE(type == dy.t.scalar_type() || type == at::kFloat, what, ": the gradient of ", dy.t.scalar_type(),
-                      " rows is ", dy.t.scalar_type(), " or float32, not ", type);
-    TORCH_CHECK_VALUE(out.defined() || !accumulate, what, ": accumulate needs out");
-    const c10::Device device = device_of(what, {&dy.t, &given, out.defined() ? &out : &dy.t});
-    if (!out.defined())
-        out = at::empty({rows, width}, dy.t.options().dtype(type));
-    else
-        TORCH_CHECK_VALUE(out.scalar_type() == type && out.dim() == 2 && out.size(0) == rows && out.size(1) == width &&
-                              out.is_contiguous() && !out.is_neg(),
-                          what, ": out must be a contiguous ", type, " tensor of shape [", rows, ", ", width, "]");
-    TORCH_CHECK_VALUE(args[5] == Py_None || !meet(dy, out), what, ": out overlaps dy in memory");
-    const Tensor ids = given.contiguous();
-    const size_t size = hb_embedding_grad_workspace(count, rows, width);
-    Tensor ws = workspace(size, device);
-    if (args[5] != Py_None) written(out);
-    const Launch on(device);
-    check(hb_embedding_grad(dy.type, dy.t.const_data_ptr(), dy.stride, ids.const_data_ptr(), bytes, count, rows, width,
-                            number(args[3]), type_or(type, HB_F32), out.data_ptr(), accumulate, ws.data_ptr(), size,
-                            on.stream));
-    return wrap(out);
+    return wrap(unlocked([&] {
+        const int bytes = index_bytes(given, "ids");
+        const int64_t count = given.numel();
+        TORCH_CHECK_VALUE(dy_given.dim() >= 1 && dy_given.sizes().slice(0, dy_given.dim() - 1) == given.sizes(), what,
+                          ": dy ", dy_given.sizes(), " does not fit ids ", given.sizes());
+        const int64_t width = dy_given.size(-1);
+        TORCH_CHECK_VALUE(rows >= 1 && rows < INT32_MAX, what, ": rows must be positive and below 2^31 - 1");
+        TORCH_CHECK_VALUE(count <= INT32_MAX, what, ": at most 2^31 - 1 ids");
+        Rows dy = feature_rows(dy_given.dim() == 2 ? dy_given : dy_given.reshape({count, width}), "dy");
+        if (dy.stride * dy.t.element_size() > (int64_t)UINT32_MAX) dy = {dy.t.contiguous(), width, dy.type};
+        TORCH_CHECK_VALUE(type == dy.t.scalar_type() || type == at::kFloat, what, ": the gradient of ", dy.t.scalar_type(),
+                          " rows is ", dy.t.scalar_type(), " or float32, not ", type);
+        Tensor out = given_out;
+        const bool given_one = out.defined();
+        TORCH_CHECK_VALUE(given_one || !accumulate, what, ": accumulate needs out");
+        const c10::Device device = device_of(what, {&dy.t, &given, given_one ? &out : &dy.t});
+        if (!given_one)
+            out = at::empty({rows, width}, dy.t.options().dtype(type));
+        else
+            TORCH_CHECK_VALUE(out.scalar_type() == type && out.dim() == 2 && out.size(0) == rows && out.size(1) == width &&
+                                  out.is_contiguous() && !out.is_neg(),
+                              what, ": out must be a contiguous ", type, " tensor of shape [", rows, ", ", width, "]");
+        TORCH_CHECK_VALUE(!given_one || !meet(dy, out), what, ": out overlaps dy in memory");
+        const Tensor ids = given.contiguous();
+        const size_t size = hb_embedding_grad_workspace(count, rows, width);
+        Tensor ws = workspace(size, device);
+        if (given_one) written(out);
+        const Launch on(device);
+        check(hb_embedding_grad(dy.type, dy.t.const_data_ptr(), dy.stride, ids.const_data_ptr(), bytes, count, rows, width,
+                                scale, type_or(type, HB_F32), out.data_ptr(), accumulate, ws.data_ptr(), size, on.stream));
+        return out;
+    }));
     END_HANDLE_TH_ERRORS
 }
 
@@ -457,19 +495,21 @@ PyObject* clip(PyObject*, PyObject* const* args, Py_ssize_t n) {
         }
     }
     if (scale) check_shared(grads, *to, what);
-    Tensor norm = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(device));
-    const size_t size = hb_clip_workspace(count);
-    Tensor ws = workspace(size, device);
-    const Launch on(device);
-    if (scale)
-        for (const Tensor& t : to->tensors) written(t);
-    if (scale)
-        check(hb_clip_grad_norm(count, grads.address.data(), grads.size.data(), grads.type.data(), to->address.data(),
-                                to->type.data(), limit, norm.data_ptr<float>(), ws.data_ptr(), size, on.stream));
-    else
-        check(hb_grad_norm(count, grads.address.data(), grads.size.data(), grads.type.data(), norm.data_ptr<float>(),
-                           ws.data_ptr(), size, on.stream));
-    return wrap(norm);
+    return wrap(unlocked([&] {
+        Tensor norm = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(device));
+        const size_t size = hb_clip_workspace(count);
+        Tensor ws = workspace(size, device);
+        const Launch on(device);
+        if (scale) {
+            for (const Tensor& t : to->tensors) written(t);
+            check(hb_clip_grad_norm(count, grads.address.data(), grads.size.data(), grads.type.data(), to->address.data(),
+                                    to->type.data(), limit, norm.data_ptr<float>(), ws.data_ptr(), size, on.stream));
+        } else {
+            check(hb_grad_norm(count, grads.address.data(), grads.size.data(), grads.type.data(), norm.data_ptr<float>(),
+                               ws.data_ptr(), size, on.stream));
+        }
+        return norm;
+    }));
     END_HANDLE_TH_ERRORS
 }
 

@@ -1,5 +1,6 @@
 """What the routing, lookup and clipping calls keep to beside their results on ordinary arguments."""
 import threading
+import time
 
 import numpy as np
 import pytest
@@ -382,3 +383,37 @@ def test_two_streams_at_once(hb, cuda):
                 got.append(work(*job))
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+
+
+def test_other_threads_go_on_while_the_launch_queue_is_full(hb, cuda):
+    """A launch waits when the device is a thousand launches behind; other Python threads do not wait with it."""
+    gen = torch.Generator(device=cuda).manual_seed(12)
+    plan = _plan(hb, cuda, gen)
+    x, z = torch.randn((40, 8), generator=gen, device=cuda), torch.randn((80, 8), generator=gen, device=cuda)
+    ids = torch.zeros(40, dtype=torch.int64, device=cuda)
+    calls = (lambda: hb.route_dispatch(x, plan), lambda: hb.route_combine(z, plan), lambda: hb.embedding_lookup(x, ids),
+             lambda: hb.grad_norm([x]), lambda: hb.route_plan(ids, 3), lambda: hb.embedding_grad(x, ids, 3),
+             lambda: hb.route_combine_grad(x, z, plan))
+    for call in calls:
+        call()
+        torch.cuda.synchronize()
+        seen, done = [], threading.Event()
+
+        def watch():
+            while not done.is_set():
+                seen.append(time.perf_counter())
+                time.sleep(0.002)
+
+        watcher = threading.Thread(target=watch)
+        watcher.start()
+        torch.cuda._sleep(800_000_000)  # some 0.4 s
+        start = time.perf_counter()
+        for _ in range(2500):
+            call()
+        took = time.perf_counter() - start
+        done.set()
+        watcher.join()
+        torch.cuda.synchronize()
+        assert took > 0.2, "the queue was not full"
+        longest = max(b - a for a, b in zip(seen, seen[1:]))
+        assert longest < took / 2
