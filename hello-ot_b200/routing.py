@@ -140,10 +140,14 @@ def assignment_of_plan(rows, cols, mass, tokens: int, *, tolerance: float = 0.0,
     m = torch.as_tensor(mass, device=dev).to(torch.float64).view(-1)
     if not r.numel() == c.numel() == m.numel():
         raise ValueError("rows, cols and mass must have equal lengths")
+    if not bool(torch.isfinite(m).all()):
+        raise ValueError("a mass of the plan is not finite")
     live = m > tolerance
     r, c, m = r[live], c[live], m[live]
     if r.numel() and (int(r.min()) < 0 or int(r.max()) >= tokens):
         raise ValueError("a row of the plan is outside the tokens")
+    if c.numel() and (int(c.min()) < 0 or int(c.max()) >= 2 ** 31 - 1):
+        raise ValueError("a column of the plan is no expert: negative, or 2^31 - 1 and above")
     by = torch.argsort(c, stable=True)
     by = by[torch.argsort(m[by], descending=True, stable=True)]
     by = by[torch.argsort(r[by], stable=True)]

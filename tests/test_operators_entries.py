@@ -1,6 +1,8 @@
-"""Refusals of the C entries of the routing, lookup and clipping operators that need no GPU (addresses are made up
-and never read)."""
+"""Refusals of the C entries of the routing, lookup and clipping operators, and of what else of them needs no GPU
+(addresses are made up and never read)."""
 from array import array
+
+import pytest
 
 A = 1 << 20  # an aligned address
 
@@ -32,3 +34,15 @@ def test_misaligned_arrays(hb):
         room = lib.hb_clip_workspace(1)
         assert lib.hb_grad_norm(1, *host, A + off, A, room, None) == bad
         assert lib.hb_clip_grad_norm(1, *host, host[0], host[2], 1.0, A + off, A, room, None) == bad
+
+
+def test_plans_that_are_no_assignment(hb):
+    """A mass that is no number, or an expert that is none, is refused, where it was left out of the token's shares."""
+    inf, nan = float("inf"), float("nan")
+    for rows, cols, mass in (([0, 1], [-1, 0], [0.5, 0.5]), ([0, 1], [0, 2 ** 31], [0.5, 0.5]), ([0, 1], [0, 2 ** 32], [0.5, 0.5]),
+                             ([0, 0], [0, 1], [0.5, nan]), ([0, 0], [0, 1], [0.5, inf])):
+        with pytest.raises(ValueError):
+            hb.assignment_of_plan(rows, cols, mass, 2, device="cpu")
+    # an edge without mass is no entry, whatever its ends
+    index, weights = hb.assignment_of_plan([0, -1, 1], [0, -1, 2 ** 40], [0.5, 0.0, 0.0], 2, device="cpu")
+    assert index.tolist() == [[0], [-1]] and weights.tolist() == [[1], [0]]
