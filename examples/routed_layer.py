@@ -38,7 +38,7 @@ def balanced_assignment(hb, x, centres, tolerance=1e-6):
 
 def experts_forward(rows, weight, offsets):
     """Each expert's product on its sorted rows; rows without an expert stay zero."""
-    ends = offsets.tolist()
+    ends = offsets.tolist()  # waits for the device: here the experts' rows are sizes of plain products
     out = [rows[a:b] @ w.t() for a, b, w in zip(ends, ends[1:], weight)]
     return torch.cat([*out, rows[ends[-1]:]])
 

@@ -366,7 +366,9 @@ int hb_prune_select(const int32_t* rows, const int32_t* cols, const double* cost
  * are HB_F32, HB_F16 and HB_BF16; arithmetic and sums are fp32 or wider and a
  * result is rounded once.  Rows are `width` contiguous elements, `*_stride`
  * elements apart; row arrays without a stride argument are dense.  Results do
- * not depend on launch order (no floating-point sum is made by atomics).
+ * not depend on launch order (no floating-point sum is made by atomics).  Small
+ * sorts and norms run in one cluster of up to 16 blocks: a partition of a GPU that
+ * cannot place one returns HB_LAUNCH.
  * ------------------------------------------------------------------------- */
 enum { HB_F32 = 0, HB_F16 = 1, HB_BF16 = 2 };
 
