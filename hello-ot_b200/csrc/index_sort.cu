@@ -43,7 +43,9 @@ constexpr int kBlock = 1024, kBlockWarps = kBlock / 32;     // a cluster's block
 constexpr int kRounds = 2;                                  // entries a thread of a cluster
 constexpr int kRankMost = 2048, kRankThreads = 512;         // sort by comparing
 constexpr int kRankSlices = 8, kRankQueries = kRankThreads / kRankSlices;
-constexpr int64_t kRankBins = 4096;                         // most bins whose offsets it finds
+// Most bins whose offsets it finds; above, they are searched in the sorted pairs.  Found / searched (us): 1000 entries by
+// 4000 bins 3.5 / 6.6, 2000 by 4000 4.7 / 8.1, by 16000 7.0 / 8.2, by 32000 12.0 / 8.2.
+constexpr int64_t kRankBins = 4096;
 constexpr int kMostClusters = 16;
 constexpr int64_t kClusterMost = (int64_t)kMostClusters * kBlock * kRounds;
 constexpr int kMaxDigitBits = 11;
