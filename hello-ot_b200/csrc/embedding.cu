@@ -442,7 +442,8 @@ __global__ void __launch_bounds__(256, 3) grad_kernel(const Grad<T, TO> g) {
 
 // Threads a row: a power of two from 4 up to 32 vectors, else whole warps, at most 256 a column tile.  Up to
 // 32768 tokens a warp at least: groups that share a warp take their turns wherever their rows end differently.  A warp
-// against less (us, bf16): 2000 into 1000 x 32 12.3 / 14.7, 32768 into 5000 x 64 24.1 / 23.2, 131072 into 100000 x 64 41.7 / 35.9.
+// against less (us, bf16): 2000 into 1000 x 32 12.3 / 14.7, 32768 into 5000 x 64 24.1 / 23.2, 131072 into 100000 x 64
+// 41.7 / 35.9.
 struct Shape {
     int group, groups, tiles;
 };

@@ -328,10 +328,11 @@ __global__ void __launch_bounds__(256) combine_grad_narrow(Moves m, const T* __r
 }
 
 // Threads a group: 8 for rows that they hold in their column steps, else a warp; a block when the groups are
-// too few to fill the SMs with warps and a row has more than a warp's vectors.  A warp against 8 threads (us): 262144 x 1
-// entries of 64 bf16 dispatch 16.3 / 8.1, combine 27.5 / 8.8, gradient 46 / 14.6; 2000 x 2 the same.  Warps against blocks (us, rows of 2048
-// bf16): combine of 64 x 2 entries 5.2 / 2.3, 1000 x 8 10.6 / 6.3; dispatch of 1180 x 2 3.4 / 3.3, 4000 x 2 7.6 / 7.2; the
-// gradient, by an entry, of 300 x 2 3.7 / 4.0, 600 x 2 4.5 / 5.6, 2000 x 2 6.0 / 13.
+// too few to fill the SMs with warps and a row has more than a warp's vectors.
+// A warp against 8 threads (us): 262144 x 1 entries of 64 bf16 dispatch 16.3 / 8.1, combine 27.5 / 8.8, gradient
+// 46 / 14.6; 2000 x 2 the same.  Warps against blocks (us, rows of 2048 bf16): combine of 64 x 2 entries 5.2 / 2.3,
+// 1000 x 8 10.6 / 6.3; dispatch of 1180 x 2 3.4 / 3.3, 4000 x 2 7.6 / 7.2; the gradient, by an entry, of 300 x 2
+// 3.7 / 4.0, 600 x 2 4.5 / 5.6, 2000 x 2 6.0 / 13.
 inline int group_of(int64_t groups, int64_t vectors, int vb) {
     if (vectors <= 8 * steps_of(vb)) return 8;
     if (groups < 148 * 8 && vectors > 32) return 256;
