@@ -2,7 +2,8 @@
 
 Pricing scan (tensor-core ℓ2², CUDA-core ℓ1/ℓ∞/ℓ2), active-support pair costs
 and the restricted-OT Halpern-PDHG, and the operators that apply an assignment to
-features and train them (routing by expert, table lookups, gradient clipping), as hand-written sm_100a CUDA kernels
+features and train them (routing by expert, the experts' products, table lookups, row
+norms, gradient clipping, the optimizer step), as hand-written sm_100a CUDA kernels
 behind the C ABI of libhello_b200.so (include/hello_b200.h), with host code
 that mirrors the reference's scan / pair-cost / PDLP interfaces.
 
@@ -22,6 +23,9 @@ from .routing import (RoutePlan, assignment_of_plan, route_combine, route_combin
                       route_dispatch_grad, route_plan)
 from .embedding import embedding_grad, embedding_lookup  # noqa: F401
 from .grad_clip import clip_grad_norm, grad_norm  # noqa: F401
+from .experts import expert_gated, expert_gated_grad, expert_product, expert_product_grad  # noqa: F401
+from .norm import Rows8, rms_norm, rms_norm_8bit, rms_norm_grad, rows_of_8bit  # noqa: F401
+from .adamw import AdamWState, adamw_moments, adamw_state, adamw_step  # noqa: F401
 from . import generic_scan, perturb  # noqa: F401
 
 __version__ = "0.1.0"

@@ -27,7 +27,10 @@ EXPORTS = ("hb_abi_version", "hb_last_error", "hb_kernel_launch_count", "hb_set_
            "hb_pair_costs_ex", "hb_l2sq_last_rescans", "hb_index_sort_workspace", "hb_index_sort",
            "hb_route_dispatch", "hb_route_combine", "hb_route_combine_grad", "hb_embedding_lookup",
            "hb_embedding_grad_workspace", "hb_embedding_grad", "hb_clip_workspace", "hb_grad_norm",
-           "hb_clip_grad_norm")
+           "hb_clip_grad_norm", "hb_expert_product", "hb_expert_gated", "hb_expert_product_grad_workspace",
+           "hb_expert_product_grad", "hb_expert_gated_grad_workspace", "hb_expert_gated_grad", "hb_rms_norm",
+           "hb_rows_of_8bit", "hb_rms_norm_grad_workspace", "hb_rms_norm_grad", "hb_adamw_workspace", "hb_adamw_step",
+           "hb_adamw_moments")
 
 
 class HBError(RuntimeError):
@@ -65,6 +68,20 @@ class PdlpTraceRow(ctypes.Structure):
     _fields_ = [("iteration", c_double), ("primal_objective", c_double), ("dual_objective", c_double),
                 ("rel_primal", c_double), ("rel_dual", c_double), ("rel_gap", c_double),
                 ("primal_weight", c_double)]
+
+
+class ExpertShape(ctypes.Structure):
+    _fields_ = [("rows", c_int64), ("width", c_int64), ("hidden", c_int64), ("experts", c_int64), ("type", c_int32),
+                ("activation", c_int32)]
+
+
+class ExpertWeight(ctypes.Structure):
+    _fields_ = [("data", c_void_p), ("row_stride", c_int64), ("expert_stride", c_int64)]
+
+
+class AdamWRule(ctypes.Structure):
+    _fields_ = [("lr", c_double), ("beta1", c_double), ("beta2", c_double), ("eps", c_double), ("decay", c_double),
+                ("max_norm", c_double), ("rate", c_void_p), ("norm", c_void_p)]
 
 
 _LIB = None
@@ -163,6 +180,34 @@ def load_library(path: Path | str = LIB_PATH):
     lib.hb_grad_norm.argtypes = [c_int64, P, P, P, P, P, c_size_t, P]
     lib.hb_clip_grad_norm.restype = c_int
     lib.hb_clip_grad_norm.argtypes = [c_int64, P, P, P, P, P, c_double, P, P, c_size_t, P]
+    S, W = POINTER(ExpertShape), POINTER(ExpertWeight)
+    lib.hb_expert_product.restype = c_int
+    lib.hb_expert_product.argtypes = [S, P, c_int64, P, W, P, P]
+    lib.hb_expert_gated.restype = c_int
+    lib.hb_expert_gated.argtypes = [S, P, c_int64, P, W, W, P, P]
+    lib.hb_expert_product_grad_workspace.restype = c_size_t
+    lib.hb_expert_product_grad_workspace.argtypes = [S]
+    lib.hb_expert_product_grad.restype = c_int
+    lib.hb_expert_product_grad.argtypes = [S, P, c_int64, P, c_int64, P, W, P, P, P, c_size_t, P]
+    lib.hb_expert_gated_grad_workspace.restype = c_size_t
+    lib.hb_expert_gated_grad_workspace.argtypes = [S]
+    lib.hb_expert_gated_grad.restype = c_int
+    lib.hb_expert_gated_grad.argtypes = [S, P, c_int64, P, c_int64, P, W, W, P, P, P, P, c_size_t, P]
+    lib.hb_rms_norm.restype = c_int
+    lib.hb_rms_norm.argtypes = [c_int, P, c_int64, P, c_int64, c_int64, c_int64, P, c_int, c_double, P, P, P, P, P]
+    lib.hb_rows_of_8bit.restype = c_int
+    lib.hb_rows_of_8bit.argtypes = [P, P, c_int64, c_int64, c_int, P, P]
+    lib.hb_rms_norm_grad_workspace.restype = c_size_t
+    lib.hb_rms_norm_grad_workspace.argtypes = [c_int64, c_int64]
+    lib.hb_rms_norm_grad.restype = c_int
+    lib.hb_rms_norm_grad.argtypes = [c_int, P, c_int64, P, c_int64, P, c_int64, c_int64, c_int64, P, c_int, c_double, P, P, P,
+                                     c_size_t, P]
+    lib.hb_adamw_workspace.restype = c_size_t
+    lib.hb_adamw_workspace.argtypes = []
+    lib.hb_adamw_step.restype = c_int
+    lib.hb_adamw_step.argtypes = [c_int64, P, P, P, P, P, P, P, P, P, P, c_int, POINTER(AdamWRule), P, P, c_size_t, P]
+    lib.hb_adamw_moments.restype = c_int
+    lib.hb_adamw_moments.argtypes = [c_int64, P, P, P, P, P, P, P, P]
     if lib.hb_abi_version() != ABI_VERSION:
         raise HBError(HB_BAD_ARGUMENT, f"libhello_b200 ABI {lib.hb_abi_version()} != {ABI_VERSION}; rebuild")
     _LIB = lib
@@ -210,7 +255,7 @@ def stream_handle(device) -> int:
 
 
 def host():
-    """The compiled host path of the routing, lookup and clipping calls (csrc/host.cpp)."""
+    """The compiled host path of the calls around and in a routed layer (csrc/host.cpp)."""
     global _HOST
     if _HOST is None:
         load_library()

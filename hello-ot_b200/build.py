@@ -4,8 +4,8 @@
 
 Each CUDA source compiles to an object under hello-ot_b200/_build/ (in
 parallel) and the objects link into hello-ot_b200/libhello_b200.so with the
-CUDA runtime linked statically.  host.cpp, the host path of the routing, lookup
-and clipping calls, compiles with g++ against the installed torch into the
+CUDA runtime linked statically.  host.cpp, the host path of the calls
+around and in a routed layer, compiles with g++ against the installed torch into the
 extension module hello-ot_b200/_host.so, which links to the library.  pdlp.cu is compiled without fma contraction
 so the PDHG update arithmetic matches the reference operation by operation;
 exact.cu likewise, so its fp64 scores round like the written expressions.
@@ -28,7 +28,7 @@ LIB = HERE / "libhello_b200.so"
 HOST = HERE / "_host.so"
 INCLUDE = HERE.parent / "include"
 SOURCES = ["abi.cu", "scan_l2sq.cu", "scan_norm.cu", "pairs.cu", "pdlp.cu", "support.cu", "exact.cu", "index_sort.cu",
-           "routing.cu", "embedding.cu", "clip.cu"]
+           "routing.cu", "embedding.cu", "clip.cu", "experts.cu", "experts_simt.cu", "norm.cu", "adamw.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
          "-I" + str(INCLUDE), "-Xptxas", "-warn-spills"]

@@ -1,0 +1,871 @@
+// Products of rows sorted by expert with each expert's weight, on the tensor cores (fp16, bf16).
+//
+//   product   y[r] = x[r] W[e]^T                        e the expert of row r
+//   gated     h[r] = act(x[r] Wg[e]^T) * (x[r] Wu[e]^T)
+//   backward  dx[r] = dy[r] W[e],  dW[e] = sum over the expert's rows of dy[r]^T x[r]; of the gated form
+//             dg = dh u act'(g), du = dh act(g), dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x
+//
+// One persistent kernel per product: a TMA producer, one thread that issues tcgen05.mma, eight warps that
+// read the accumulators.  A CTA pair (cta_group::2) takes a tile of 256 x 256 of the output, each CTA with
+// its own 128 rows of one operand and 128 of the other's 256, 64 of the summed length a stage, six stages;
+// the accumulators are fp32 in TMEM, twice, so that a tile is written while the next one is summed.  In the
+// gated forms the even CTA brings 128 rows of Wg and the odd one the same rows of Wu: columns 0-127 of the
+// accumulator are g, 128-255 are u, and one thread holds both of a place, so g and u never leave the chip.
+// The gradients compute g and u again: it costs 2 of 6 products, and saves two arrays of rows x hidden that,
+// kept in 16 bits, would put two more roundings into every gradient.
+//
+// The rows of an expert begin anywhere: TMA boxes may (only the innermost coordinate has to lie on 16
+// bytes), rows of the next expert that a tile's box brings along are summed and not written.  In the sum
+// over an expert's rows (dW) they have to be zeros instead, of both operands (0 * NaN): the box that holds
+// the expert's end completes on a barrier of its own CTA, the producer's warp zeroes the foreign rows and
+// hands the stage on.
+#include <algorithm>
+#include <string>
+#include <type_traits>
+
+#include "common.cuh"
+#include "experts.cuh"
+#include "internal.h"
+
+namespace hb {
+namespace experts {
+
+constexpr int BK = 64, kStages = 6, kEpiWarps = 8, kThreads = 64 + 32 * kEpiWarps;
+constexpr int kTileBytes = 128 * BK * 2, kStageBytes = 2 * kTileBytes;
+constexpr int kBand = 8;  // row tiles that share a weight tile while it is in L2
+
+struct Params {
+    CUtensorMap a[2], b[2];
+    const int32_t* offsets;
+    int groups, rows, n, k, segments, activation;
+    int col_tiles, row_tiles;  // row_tiles: kWeights alone
+    int splits;                // kWeights
+    float* partial;
+    const void* dh;
+    int64_t dh_row;
+    void* out[2];
+    int64_t out_row;  // distance of the outputs' rows in elements
+};
+
+struct __align__(1024) Smem {
+    uint8_t stage[kStages][kStageBytes];
+    __align__(16) uint8_t out[kEpiWarps][32 * 64];  // a warp's 32 x 32 chunk on its way out
+    int start[kMostGroups + 2], tile[kMostGroups + 2];
+    uint64_t full[kStages], empty[kStages], tfull[2], tempty[2], tail;
+    uint32_t tmem_base;
+    int abort, status;
+};
+constexpr size_t kSmemBytes = sizeof(Smem) + 1024;
+static_assert(kSmemBytes <= 227 * 1024, "dynamic shared memory above the 227 KB a CTA may use");
+
+// ---------------------------------------------------------------- instructions
+__device__ __forceinline__ void load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
+    tma_load_2d(dst, map, bar, c0, c1);
+}
+__device__ __forceinline__ void load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
+__device__ __forceinline__ void load_3d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(smem_u32(dst)), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
+// Arrive, with bytes to come, on an mbarrier of either CTA of the cluster (address from peer_smem).
+__device__ __forceinline__ void arrive_expect_cluster(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// A bounded wait on a barrier that the other CTA arrives on as well.
+template <bool PAIR>
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Smem& s) {
+    if constexpr (!PAIR) return mbar_wait(bar, parity, &s.abort, &s.status);
+    else for (int it = 0; it < 4000; ++it) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.b32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u) : "memory");
+        if (ok) return true;
+        if (*(volatile int*)&s.abort) return false;
+    }
+    s.abort = 1;
+    atomicOr(&s.status, kErrWaitTimeout);
+    return false;
+}
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// A tile stored with the 128-byte swizzle whose rows are the summed length (K rows of 64 columns of the output
+// dimension, 128 bytes): 8 rows are 1024 bytes, the next 64 columns are a box of BK rows further.
+__device__ __forceinline__ uint64_t desc_columns(uint32_t saddr) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr >> 4) & 0x3FFF);
+    d |= (uint64_t)((BK * 128) >> 4) << 16;  // leading byte offset: the next 64 columns
+    d |= (uint64_t)(1024 >> 4) << 32;        // stride byte offset: the next 8 rows
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+// Instruction descriptor of kind::f16: fp32 accumulators, both operands bf16 or both fp16, each read along the summed
+// length or (columns) across it.
+__host__ __device__ constexpr uint32_t idesc(bool bf16, bool a_columns, bool b_columns, int m, int n) {
+    return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((a_columns ? 1u : 0u) << 15) |
+           ((b_columns ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+// ---------------------------------------------------------------- tiles
+template <int FORM, bool PAIR>
+struct Shape {
+    static constexpr bool kHalves = FORM == kGated || FORM == kGatedGrad;  // the accumulator is [g | u]
+    static constexpr bool kAColumns = FORM == kWeights, kBColumns = FORM == kWeights || FORM == kBack;
+    static constexpr int M = PAIR ? 256 : 128, N = PAIR ? 256 : 128;  // of the accumulator, over the pair
+    static constexpr int kCols = kHalves ? N / 2 : N;                 // output columns
+    static constexpr uint32_t kTmemCols = 2 * N;
+};
+
+struct Tile {
+    int group, row, rows;  // group; first row of this CTA in the output; rows of the group from there (may be <= 0)
+    int col;               // first column
+    int part, split;       // kWeights: which product, which part of the rows
+    int begin, length;     // kWeights: the rows to sum over
+    int blocks;            // stages; 0: the output is zeros
+};
+
+template <int FORM, bool PAIR>
+__device__ __forceinline__ int tiles_of(const Params& p, const Smem& s) {
+    if (FORM == kWeights) return p.splits * p.segments * p.groups * p.row_tiles * p.col_tiles;
+    return s.tile[p.groups + 1] * p.col_tiles;
+}
+
+template <int FORM, bool PAIR>
+__device__ __forceinline__ Tile tile_at(const Params& p, const Smem& s, int u, int rank) {
+    using S = Shape<FORM, PAIR>;
+    Tile t;
+    int local, row_tiles;
+    if (FORM == kWeights) {
+        row_tiles = p.row_tiles;
+        const int per = row_tiles * p.col_tiles;
+        t.group = u / per;
+        local = u - t.group * per;
+        t.part = t.group % p.segments;
+        t.group /= p.segments;
+        t.split = t.group % p.splits;
+        t.group /= p.splits;
+        int end;
+        split_rows(s.start[t.group + 1] - s.start[t.group], p.splits, t.split, t.begin, end);
+        t.length = end - t.begin;
+        t.begin += s.start[t.group];
+        t.blocks = (t.length + BK - 1) / BK;
+    } else {
+        t.group = group_of(s.tile, p.groups, u / p.col_tiles);
+        row_tiles = s.tile[t.group + 1] - s.tile[t.group];
+        local = u - s.tile[t.group] * p.col_tiles;
+        t.part = t.split = t.begin = t.length = 0;
+        t.blocks = t.group == p.groups ? 0 : p.segments * ((p.k + BK - 1) / BK);
+    }
+    const int band = local / (kBand * p.col_tiles), in_band = local - band * kBand * p.col_tiles;
+    const int deep = min(kBand, row_tiles - band * kBand);
+    const int row = (band * kBand + in_band % deep) * S::M + (PAIR ? rank * 128 : 0);
+    t.col = in_band / deep * S::kCols;
+    if (FORM == kWeights) {
+        t.row = row;
+        t.rows = p.n - row;
+    } else {
+        t.row = s.start[t.group] + row;
+        t.rows = s.start[t.group + 1] - t.row;
+    }
+    return t;
+}
+
+// ---------------------------------------------------------------- roles
+// Lane 0 waits for its warp, which goes on or gives up as one.
+template <bool PAIR>
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, Smem& s) {
+    bool ok = true;
+    if ((threadIdx.x & 31) == 0) ok = wait<PAIR>(bar, parity, s);
+    return __shfl_sync(0xffffffffu, ok, 0);
+}
+
+// The producer's warp; lane 0 issues the loads.  Every stage brings 128 rows of each operand for this CTA.  With pairs
+// the completions of both CTAs count on the even one's barrier.
+template <int FORM, bool PAIR>
+__device__ __forceinline__ void produce(const Params& p, Smem& s, int rank) {
+    using S = Shape<FORM, PAIR>;
+    const int lane = threadIdx.x & 31;
+    uint32_t stage = 0, phase = 0, tails = 0;
+    const int units = tiles_of<FORM, PAIR>(p, s);
+    const int per_segment = (p.k + BK - 1) / BK;
+    for (int u = blockIdx.x / (PAIR ? 2 : 1); u < units; u += gridDim.x / (PAIR ? 2 : 1)) {
+        const Tile t = tile_at<FORM, PAIR>(p, s, u, rank);
+        for (int kb = 0; kb < t.blocks; ++kb) {
+            if (!warp_wait<PAIR>(&s.empty[stage], phase ^ 1, s)) return;
+            uint8_t *a = s.stage[stage], *b = a + kTileBytes;
+            const uint32_t full = PAIR ? peer_smem(&s.full[stage], 0) : 0u;
+            if (FORM == kWeights) {
+                const int row = t.begin + kb * BK, left = t.length - kb * BK;
+                const int bcol = t.col + (PAIR ? rank * 128 : 0);
+                const CUtensorMap* am = &p.a[t.part];
+                if (left >= BK) {
+                    if (lane == 0) {
+                        if (PAIR) {
+                            arrive_expect_cluster(full, kStageBytes);
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                tma_load_2d_pair(a + i * BK * 128, am, full, t.row + i * 64, row);
+                                tma_load_2d_pair(b + i * BK * 128, &p.b[0], full, bcol + i * 64, row);
+                            }
+                        } else {
+                            mbar_arrive_expect_tx(&s.full[stage], kStageBytes);
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                load_2d(a + i * BK * 128, am, &s.full[stage], t.row + i * 64, row);
+                                load_2d(b + i * BK * 128, &p.b[0], &s.full[stage], bcol + i * 64, row);
+                            }
+                        }
+                    }
+                } else {  // rows of the next expert are in the box: zero them once it is there
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&s.tail, kStageBytes);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            load_2d(a + i * BK * 128, am, &s.tail, t.row + i * 64, row);
+                            load_2d(b + i * BK * 128, &p.b[0], &s.tail, bcol + i * 64, row);
+                        }
+                    }
+                    if (!warp_wait<false>(&s.tail, tails & 1, s)) return;
+                    ++tails;
+                    const int words = (BK - left) * 8;  // 16 bytes each, of every box
+                    for (int i = lane; i < words; i += 32)
+#pragma unroll
+                        for (int box = 0; box < 4; ++box)
+                            *reinterpret_cast<uint4*>(a + box * BK * 128 + left * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+                    fence_async_shared();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (PAIR) mbar_arrive_remote(full);
+                        else mbar_arrive(&s.full[stage]);
+                    }
+                }
+            } else if (lane == 0) {
+                const int seg = FORM == kBack ? kb / per_segment : 0;
+                const int k0 = (kb - seg * per_segment) * BK;
+                if (PAIR) {
+                    arrive_expect_cluster(full, kStageBytes);
+                    tma_load_2d_pair(a, &p.a[seg], full, k0, t.row);
+                    if (FORM == kBack) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            load_3d_pair(b + i * BK * 128, &p.b[seg], full, t.col + rank * 128 + i * 64, k0, t.group);
+                    } else if (S::kHalves) {
+                        load_3d_pair(b, &p.b[rank], full, k0, t.col, t.group);
+                    } else {
+                        load_3d_pair(b, &p.b[0], full, k0, t.col + rank * 128, t.group);
+                    }
+                } else {
+                    uint64_t* bar = &s.full[stage];
+                    mbar_arrive_expect_tx(bar, kStageBytes);
+                    load_2d(a, &p.a[seg], bar, k0, t.row);
+                    if (FORM == kBack) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) load_3d(b + i * BK * 128, &p.b[seg], bar, t.col + i * 64, k0, t.group);
+                    } else if (S::kHalves) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) load_3d(b + i * 64 * 128, &p.b[i], bar, k0, t.col, t.group);
+                    } else {
+                        load_3d(b, &p.b[0], bar, k0, t.col, t.group);
+                    }
+                }
+            }
+            if (++stage == kStages) stage = 0, phase ^= 1;
+        }
+    }
+}
+
+// One thread (of the even CTA) issues the products; commits release the stages and hand over the accumulator.
+template <int FORM, bool PAIR, bool BF16>
+__device__ __forceinline__ void multiply(const Params& p, Smem& s, uint32_t tmem) {
+    using S = Shape<FORM, PAIR>;
+    constexpr uint32_t ID = idesc(BF16, S::kAColumns, S::kBColumns, S::M, S::N);
+    auto commit = [](uint64_t* bar) {
+        if (PAIR) mma_commit_pair(bar);
+        else mma_commit(bar);
+    };
+    uint32_t stage = 0, phase = 0, done = 0;
+    const int units = tiles_of<FORM, PAIR>(p, s);
+    for (int u = blockIdx.x / (PAIR ? 2 : 1); u < units; u += gridDim.x / (PAIR ? 2 : 1)) {
+        const int blocks = tile_at<FORM, PAIR>(p, s, u, 0).blocks;
+        if (blocks == 0) continue;
+        const uint32_t buf = done & 1;
+        if (!wait<PAIR>(&s.tempty[buf], ((done >> 1) & 1) ^ 1, s)) return;
+        tc_fence_after();
+        const uint32_t d = tmem + buf * S::N;
+        for (int kb = 0; kb < blocks; ++kb) {
+            if (!wait<PAIR>(&s.full[stage], phase, s)) return;
+            tc_fence_after();
+            const uint32_t a = smem_u32(s.stage[stage]), b = a + kTileBytes;
+#pragma unroll
+            for (int kk = 0; kk < BK / 16; ++kk) {
+                const uint64_t ad = S::kAColumns ? desc_columns(a + kk * 16 * 128) : smem_desc_sw128(a + kk * 32);
+                const uint64_t bd = S::kBColumns ? desc_columns(b + kk * 16 * 128) : smem_desc_sw128(b + kk * 32);
+                if (PAIR) mma_f16_pair(d, ad, bd, ID, (kb | kk) != 0);
+                else mma_f16(d, ad, bd, ID, (kb | kk) != 0);
+            }
+            commit(&s.empty[stage]);
+            if (++stage == kStages) stage = 0, phase ^= 1;
+        }
+        commit(&s.tfull[buf]);
+        ++done;
+    }
+}
+
+// Writes a warp's chunk of 32 rows x 32 columns (thread: its row's 32 values) through shared memory, so that rows leave
+// in whole sectors: `out` its first element, `stride` the rows' distance, `rows` and `cols` how many there are.
+// Rows pass in pieces of 64 bytes; the swizzle keeps 8 rows' 16-byte words in different banks.
+template <typename T>
+__device__ __forceinline__ void write_chunk(uint8_t* buf, const float (&v)[32], T* out, int64_t stride, int rows, int cols,
+                                            bool vectors, int lane) {
+    constexpr int N = 64 / (int)sizeof(T), V = 16 / (int)sizeof(T);  // values of a piece, of a word
+#pragma unroll
+    for (int piece = 0; piece < 32 / N; ++piece) {
+        union {
+            uint4 raw[4];
+            T t[N];
+        } r;
+#pragma unroll
+        for (int i = 0; i < N; ++i) r.t[i] = rows::from_float<T>(v[piece * N + i]);
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = r.raw[j];
+        __syncwarp();
+        T* to = out + piece * N;
+        const int left = cols - piece * N;
+        if (vectors) {
+            const int j = lane & 3;
+            if (j * V < left) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = i * 8 + (lane >> 2);
+                    if (row < rows)
+                        *reinterpret_cast<uint4*>(to + row * stride + j * V) =
+                            *reinterpret_cast<const uint4*>(buf + row * 64 + ((j ^ ((row >> 1) & 3)) << 4));
+                }
+            }
+        } else {
+            const int c = lane % N, j = c / V, in = c % V * (int)sizeof(T);
+            for (int row = lane / N; row < rows; row += 32 / N)
+                if (c < left) to[row * stride + c] = *reinterpret_cast<const T*>(buf + row * 64 + ((j ^ ((row >> 1) & 3)) << 4) + in);
+        }
+    }
+}
+
+// A thread's 32 values of a row.
+template <typename T>
+__device__ __forceinline__ void read_row(float (&v)[32], const T* at, int cols, bool vectors) {
+    if (vectors) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            rows::Vec<T, 16> w;
+            if (j * 8 < cols) w.load(at + j * 8);
+            else w.zero();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[j * 8 + i] = rows::to_float(w.v[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = i < cols ? rows::to_float(at[i]) : 0.0f;
+    }
+}
+
+// Two warps a TMEM lane quarter, each on half of the output's columns.  A wait that gave up leaves NaN.
+template <int FORM, bool PAIR, typename T>
+__device__ __forceinline__ void write_out(const Params& p, Smem& s, uint32_t tmem, int rank) {
+    using S = Shape<FORM, PAIR>;
+    constexpr int kSlice = S::kCols / 2;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int quarter = warp & 3, slice = (warp - 2) >> 2;
+    uint8_t* buf = s.out[warp - 2];
+    const uint32_t tempty = PAIR ? peer_smem(&s.tempty[0], 0) : 0u;
+    const int width = FORM == kWeights ? p.k : p.n;
+    const bool vectors = p.out_row % 8 == 0 && ((reinterpret_cast<uintptr_t>(p.out[0]) | reinterpret_cast<uintptr_t>(p.out[1])) & 15) == 0;
+    const bool dh_vectors = p.dh_row % 8 == 0 && width % 8 == 0 && (reinterpret_cast<uintptr_t>(p.dh) & 15) == 0;
+    uint32_t done = 0;
+    bool good = true;
+    const int units = tiles_of<FORM, PAIR>(p, s);
+    for (int u = blockIdx.x / (PAIR ? 2 : 1); u < units; u += gridDim.x / (PAIR ? 2 : 1)) {
+        const Tile t = tile_at<FORM, PAIR>(p, s, u, rank);
+        const uint32_t acc = done & 1;
+        const bool summed = t.blocks != 0;
+        if (summed) {
+            good = __all_sync(0xffffffffu, good && wait<PAIR>(&s.tfull[acc], (done >> 1) & 1, s));  // a warp goes on as one
+            tc_fence_after();
+        }
+        const int row0 = quarter * 32, col0 = t.col + slice * kSlice;
+        const int rows = min(32, t.rows - row0);  // of this warp; may be <= 0
+        T* out = static_cast<T*>(p.out[FORM == kWeights ? t.part : 0]);
+        float* partial = nullptr;
+        if (FORM == kWeights) {
+            out += (int64_t)t.group * p.n * p.out_row;
+            if (p.splits > 1) partial = p.partial + (((int64_t)t.split * p.segments + t.part) * p.groups + t.group) * p.n * p.k;
+        }
+        const int64_t at = (int64_t)(t.row + row0) * p.out_row + col0;
+        const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16) + acc * S::N + slice * kSlice;
+        for (int c = 0; c < kSlice; c += 32) {
+            const int cols = min(32, width - col0 - c);
+            if (rows <= 0 || cols <= 0) break;  // the same for the whole warp
+            float v[32];
+            if (!summed || !good) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = good ? 0.0f : __int_as_float(0x7fc00000);
+                if (FORM == kWeights && partial) {
+                    write_chunk<float>(buf, v, partial + at + c, p.k, rows, cols, p.k % 4 == 0, lane);
+                    continue;
+                }
+                write_chunk<T>(buf, v, out + at + c, p.out_row, rows, cols, vectors, lane);
+                if (FORM == kGatedGrad)
+                    write_chunk<T>(buf, v, static_cast<T*>(p.out[1]) + at + c, p.out_row, rows, cols, vectors, lane);
+                continue;
+            }
+            if constexpr (S::kHalves) {
+                float w[32], d[32];
+                if (FORM == kGatedGrad) {
+                    const int r = min(lane, rows - 1);
+                    read_row<T>(d, static_cast<const T*>(p.dh) + (int64_t)(t.row + row0 + r) * p.dh_row + col0 + c, cols, dh_vectors);
+                }
+                tmem_ld32(taddr + c, v);
+                tmem_ld32(taddr + S::N / 2 + c, w);
+                tmem_wait_ld(v);
+                tmem_wait_ld(w);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    float slope;
+                    const float a = activate<false, FORM == kGatedGrad>(p.activation, v[i], slope);
+                    if (FORM == kGated) {
+                        v[i] = a * w[i];
+                    } else {
+                        v[i] = d[i] * w[i] * slope;
+                        w[i] = d[i] * a;
+                    }
+                }
+                write_chunk<T>(buf, v, out + at + c, p.out_row, rows, cols, vectors, lane);
+                if (FORM == kGatedGrad)
+                    write_chunk<T>(buf, w, static_cast<T*>(p.out[1]) + at + c, p.out_row, rows, cols, vectors, lane);
+            } else {
+                tmem_ld32(taddr + c, v);
+                tmem_wait_ld(v);
+                if (FORM == kWeights && partial)
+                    write_chunk<float>(buf, v, partial + at + c, p.k, rows, cols, p.k % 4 == 0, lane);
+                else
+                    write_chunk<T>(buf, v, out + at + c, p.out_row, rows, cols, vectors, lane);
+            }
+        }
+        if (summed) {
+            tc_fence_before();
+            if (PAIR && rank != 0) mbar_arrive_remote(tempty + acc * (uint32_t)sizeof(uint64_t));
+            else mbar_arrive(&s.tempty[acc]);
+            ++done;
+        }
+    }
+}
+
+// With pairs both CTAs allocate TMEM together, meet after the barriers are ready and before they leave; every role
+// returns to the end, after a wait that gave up too.
+template <int FORM, bool PAIR, typename T>
+__global__ void __launch_bounds__(kThreads, 1) expert_kernel(const __grid_constant__ Params p) {
+    using S = Shape<FORM, PAIR>;
+    constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+    extern __shared__ uint8_t smem_raw[];
+    Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = PAIR ? (int)cluster_rank() : 0;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; ++i) mbar_init(&s.full[i], PAIR ? 2 : 1), mbar_init(&s.empty[i], 1);
+        for (int i = 0; i < 2; ++i) mbar_init(&s.tfull[i], 1), mbar_init(&s.tempty[i], 32 * kEpiWarps * (PAIR ? 2 : 1));
+        mbar_init(&s.tail, 1);
+        s.abort = s.status = 0;
+        fence_barrier_init();
+    }
+    if (warp == 0 && lane < 2) prefetch_tmap(&p.a[lane]), prefetch_tmap(&p.b[lane]);
+    if (warp == 1) {
+        if (PAIR) tmem_alloc_pair(&s.tmem_base, S::kTmemCols), tmem_relinquish_pair();
+        else tmem_alloc(&s.tmem_base, S::kTmemCols), tmem_relinquish();
+    }
+    read_groups(p.offsets, p.groups, p.rows, S::M, s.start, s.tile);
+    tc_fence_before();
+    __syncthreads();
+    if (PAIR) cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = s.tmem_base;
+    if (warp == 0) {
+        produce<FORM, PAIR>(p, s, rank);
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) multiply<FORM, PAIR, BF16>(p, s, tmem);
+    } else {
+        write_out<FORM, PAIR, T>(p, s, tmem, rank);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (PAIR) cluster_sync();
+    if (warp == 1) {
+        tc_fence_after();
+        if (PAIR) tmem_dealloc_pair(tmem, S::kTmemCols);
+        else tmem_dealloc(tmem, S::kTmemCols);
+    }
+}
+
+// ---------------------------------------------------------------- host
+namespace {
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled find_encode() {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+        return reinterpret_cast<EncodeTiled>(ptr);
+    cudaGetLastError();
+    return nullptr;
+}
+
+// Map of [groups][rows][cols] (groups 0: two dimensions) in boxes of 64 columns (128 bytes) x box_rows, 128-byte swizzle;
+// what lies outside is read as zeros.
+bool encode(CUtensorMap* m, const Operand& o, int type, int64_t cols, int64_t rows, int64_t groups, int box_rows) {
+    static const EncodeTiled enc = find_encode();
+    if (!enc) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)std::max<int64_t>(groups, 1)};
+    const cuuint64_t strides[2] = {(cuuint64_t)o.row * 2, (cuuint64_t)o.group * 2};
+    const cuuint32_t box[3] = {BK, (cuuint32_t)box_rows, 1}, step[3] = {1, 1, 1};
+    return enc(m, type == HB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, groups ? 3 : 2,
+               const_cast<void*>(o.p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int FORM, bool PAIR, typename T>
+cudaError_t launch(const Params& p, int64_t tiles, cudaStream_t st) {
+    const auto fn = expert_kernel<FORM, PAIR, T>;
+    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
+    int device = 0, sms = 0;
+    if (e == cudaSuccess) e = cudaGetDevice(&device);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    if (e != cudaSuccess) return e;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = PAIR ? 2 : 1;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)std::min<int64_t>(PAIR ? sms / 2 * 2 : sms, tiles * (PAIR ? 2 : 1)));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmemBytes;
+    cfg.stream = st;
+    cfg.attrs = at;
+    cfg.numAttrs = PAIR ? 1 : 0;
+    e = cudaLaunchKernelEx(&cfg, fn, p);
+    count_launches(1);
+    return e;
+}
+
+template <int FORM, bool PAIR>
+int run_form(const Job& job, cudaStream_t st) {
+    using S = Shape<FORM, PAIR>;
+    Params p{};
+    p.offsets = job.offsets;
+    p.groups = job.groups;
+    p.rows = job.rows;
+    p.n = job.n;
+    p.k = job.k;
+    p.segments = FORM == kBack || FORM == kWeights ? job.segments : 1;
+    p.activation = job.activation;
+    p.dh = job.dh.p;
+    p.dh_row = job.dh.row;
+    p.out[0] = job.out[0];
+    p.out[1] = job.out[1];
+    const int width = FORM == kWeights ? job.k : job.n;
+    p.out_row = job.out_row;
+    p.splits = FORM == kWeights ? job.splits : 1;
+    p.partial = job.partial;
+    p.col_tiles = (width + S::kCols - 1) / S::kCols;
+    p.row_tiles = FORM == kWeights ? (job.n + S::M - 1) / S::M : 0;
+    const int64_t most = FORM == kWeights ? (int64_t)p.splits * p.segments * job.groups * p.row_tiles * p.col_tiles
+                                          : ((int64_t)job.rows / S::M + job.groups + 1) * p.col_tiles;
+    if (most > INT32_MAX) return abi_fail(HB_BAD_ARGUMENT, "expert product: too many tiles");
+    bool ok = true;
+    const int maps = S::kHalves ? 2 : p.segments;
+    for (int i = 0; i < maps && ok; ++i) {
+        if (FORM == kWeights) {
+            ok = encode(&p.a[i], job.a[i], job.type, job.n, job.rows, 0, BK);
+            if (i == 0) ok = ok && encode(&p.b[0], job.b[0], job.type, job.k, job.rows, 0, BK);
+        } else {
+            if (!S::kHalves || i == 0) ok = encode(&p.a[i], job.a[i], job.type, job.k, job.rows, 0, 128);
+            if (FORM == kBack) ok = ok && encode(&p.b[i], job.b[i], job.type, job.n, job.k, job.groups, BK);
+            else ok = ok && encode(&p.b[i], job.b[i], job.type, job.k, job.n, job.groups, S::kHalves && !PAIR ? 64 : 128);
+        }
+    }
+    if (!ok) return abi_fail(HB_TENSOR_MAP, "expert product: cuTensorMapEncodeTiled failed");
+    if (maps == 1 || FORM == kWeights) p.b[1] = p.b[0];
+    if (maps == 1 || S::kHalves) p.a[1] = p.a[0];
+    const cudaError_t e = job.type == HB_BF16 ? launch<FORM, PAIR, __nv_bfloat16>(p, most, st) : launch<FORM, PAIR, __half>(p, most, st);
+    return e == cudaSuccess ? HB_OK : abi_fail(HB_LAUNCH, std::string("expert product: ") + cudaGetErrorString(e));
+}
+
+// CTA pairs where their tiles are filled: by an expert's rows, or by the weight's two sides.
+bool use_pairs(const Job& job) {
+    return job.form == kWeights ? job.n > 128 && job.k > 128 : job.rows > 128 * (int64_t)job.groups;
+}
+// kWeights: parts of the rows, where the tiles alone leave most of the device idle and experts have many stages.
+constexpr int kSlots = 148, kLeastStages = 16;
+int splits_of(const Job& job) {
+    const bool pair = job.type != HB_F32 && use_pairs(job);
+    const int64_t side = pair ? 256 : 128, slots = pair ? kSlots / 2 : kSlots;
+    const int64_t tiles = job.segments * (int64_t)job.groups * ((job.n + side - 1) / side) * ((job.k + side - 1) / side);
+    const int64_t stages = (job.rows / job.groups + 63) / 64;
+    return (int)std::max<int64_t>(1, std::min(slots / tiles, stages / kLeastStages));
+}
+size_t partial_bytes(const Job& job, int splits) {
+    return splits > 1 ? (size_t)splits * job.segments * job.groups * job.n * job.k * sizeof(float) : 0;
+}
+
+template <int FORM>
+int run_pairs(const Job& job, cudaStream_t st) {
+    return use_pairs(job) ? run_form<FORM, true>(job, st) : run_form<FORM, false>(job, st);
+}
+
+int run(const Job& job, cudaStream_t st) {
+    const bool row_form = job.form == kProduct || job.form == kGated;
+    cudaError_t e = cudaSuccess;
+    if (row_form && job.rows <= kFewRows) e = few_rows(job, st);
+    else if (job.type == HB_F32) e = product_f32(job, st);
+    else {
+        int rc;
+        switch (job.form) {
+            case kProduct: rc = run_pairs<kProduct>(job, st); break;
+            case kGated: rc = run_pairs<kGated>(job, st); break;
+            case kGatedGrad: rc = run_pairs<kGatedGrad>(job, st); break;
+            case kBack: rc = run_pairs<kBack>(job, st); break;
+            default: rc = run_pairs<kWeights>(job, st);
+        }
+        if (rc) return rc;
+    }
+    if (e == cudaSuccess && job.form == kWeights && job.splits > 1) e = join_parts(job, st);
+    return e == cudaSuccess ? HB_OK : abi_fail(HB_LAUNCH, std::string("expert product: ") + cudaGetErrorString(e));
+}
+
+// ---------------------------------------------------------------- checks of the C entries
+bool fits(const Operand& o, int type, int64_t cols, int64_t rows, bool weights, int64_t groups, bool grid) {
+    const uint64_t size = rows::type_bytes(type), unit = grid && type != HB_F32 ? 16 : size;
+    if (!o.p || rows::address_bits(o.p) % unit || o.row < 0 || o.row > INT32_MAX) return false;
+    if (rows > 1 && ((uint64_t)o.row * size % unit || ((weights || unit == 16) && o.row < cols))) return false;
+    if (weights && groups > 1 && (o.group < 0 || o.group >= ((int64_t)1 << 38) || (uint64_t)o.group * size % unit)) return false;
+    return true;
+}
+// Distances that are never stepped over, in the form that a tensor map takes.
+Operand tidy(Operand o, int64_t cols, int64_t rows, int64_t groups) {
+    if (rows <= 1) o.row = (cols + 7) / 8 * 8;
+    if (groups <= 1) o.group = o.row * std::max<int64_t>(rows, 1);
+    return o;
+}
+int check(const hb_expert_shape* s, const int32_t* offsets, const char* what) {
+    const std::string at = std::string(what) + ": ";
+    if (!s) return abi_fail(HB_BAD_ARGUMENT, at + "null shape");
+    if (!rows::valid_type(s->type)) return abi_fail(HB_BAD_ARGUMENT, at + "element type");
+    if (s->rows < 0 || s->rows > INT32_MAX - 1024 || s->width < 1 || s->hidden < 1 || s->width > (1 << 28) || s->hidden > (1 << 28))
+        return abi_fail(HB_BAD_ARGUMENT, at + "rows, width or hidden out of range");
+    if (s->experts < 1 || s->experts > kMostGroups || (!offsets && s->experts != 1))
+        return abi_fail(HB_BAD_ARGUMENT, at + "1 to 2048 experts, and one without offsets");
+    if (rows::address_bits(offsets) % 4) return abi_fail(HB_BAD_ARGUMENT, at + "misaligned offsets");
+    if (s->activation != HB_SILU && s->activation != HB_GELU) return abi_fail(HB_BAD_ARGUMENT, at + "activation");
+    return HB_OK;
+}
+Job job_of(const hb_expert_shape* s, const int32_t* offsets, int form, int64_t n, int64_t k) {
+    Job j{};
+    j.type = s->type;
+    j.form = form;
+    j.activation = s->activation == HB_GELU ? kGelu : kSilu;
+    j.offsets = offsets;
+    j.groups = (int)s->experts;
+    j.rows = (int)s->rows;
+    j.n = (int)n;
+    j.k = (int)k;
+    j.out_row = n;
+    j.segments = j.splits = 1;
+    return j;
+}
+int64_t padded(int64_t width) { return (width + 7) / 8 * 8; }
+
+}  // namespace
+}  // namespace experts
+}  // namespace hb
+
+using namespace hb;
+using namespace hb::experts;
+
+namespace {
+constexpr const char* kOperand = "an operand is null, off its grid or has a bad stride";
+Operand rows_of(const void* p, int64_t stride) { return {p, stride, 0}; }
+Operand weight_of(const hb_expert_weight* w) { return w ? Operand{w->data, w->row_stride, w->expert_stride} : Operand{nullptr, 0, 0}; }
+bool aligned_out(const void* p, int type) { return rows::address_bits(p) % rows::type_bytes(type) == 0; }
+}  // namespace
+
+extern "C" int hb_expert_product(const hb_expert_shape* s, const void* x, int64_t x_stride, const int32_t* offsets,
+                                 const hb_expert_weight* weight, void* out, void* stream) {
+    const char* what = "hb_expert_product";
+    if (const int rc = check(s, offsets, what)) return rc;
+    if (s->rows == 0) return HB_OK;
+    const bool grid = s->rows > kFewRows;
+    Job j = job_of(s, offsets, kProduct, s->hidden, s->width);
+    j.a[0] = rows_of(x, x_stride);
+    j.b[0] = weight_of(weight);
+    if (!fits(j.a[0], s->type, s->width, s->rows, false, 1, grid) || !fits(j.b[0], s->type, s->width, s->hidden, true, s->experts, grid) ||
+        !out || !aligned_out(out, s->type))
+        return abi_fail(HB_BAD_ARGUMENT, std::string(what) + ": " + kOperand);
+    j.a[0] = tidy(j.a[0], s->width, s->rows, 1);
+    j.b[0] = tidy(j.b[0], s->width, s->hidden, s->experts);
+    j.out[0] = out;
+    return run(j, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int hb_expert_gated(const hb_expert_shape* s, const void* x, int64_t x_stride, const int32_t* offsets,
+                               const hb_expert_weight* gate, const hb_expert_weight* up, void* out, void* stream) {
+    const char* what = "hb_expert_gated";
+    if (const int rc = check(s, offsets, what)) return rc;
+    if (s->rows == 0) return HB_OK;
+    const bool grid = s->rows > kFewRows;
+    Job j = job_of(s, offsets, kGated, s->hidden, s->width);
+    j.a[0] = rows_of(x, x_stride);
+    j.b[0] = weight_of(gate);
+    j.b[1] = weight_of(up);
+    if (!fits(j.a[0], s->type, s->width, s->rows, false, 1, grid) || !fits(j.b[0], s->type, s->width, s->hidden, true, s->experts, grid) ||
+        !fits(j.b[1], s->type, s->width, s->hidden, true, s->experts, grid) || !out || !aligned_out(out, s->type))
+        return abi_fail(HB_BAD_ARGUMENT, std::string(what) + ": " + kOperand);
+    j.a[0] = tidy(j.a[0], s->width, s->rows, 1);
+    for (Operand& b : j.b) b = tidy(b, s->width, s->hidden, s->experts);
+    j.out[0] = out;
+    return run(j, static_cast<cudaStream_t>(stream));
+}
+
+namespace {
+int bad_workspace(const void* ws, size_t bytes, size_t need, const char* what) {
+    if (need == 0) return HB_OK;
+    if (!ws || rows::address_bits(ws) % 256)
+        return abi_fail(HB_BAD_ARGUMENT, std::string(what) + ": the workspace must be 256-byte aligned");
+    return bytes < need ? abi_fail(HB_WORKSPACE, std::string(what) + ": workspace smaller than its query says") : HB_OK;
+}
+// The gradients of weights without rows.
+int zero_weights(const hb_expert_shape* s, void* w, cudaStream_t st, const char* what) {
+    if (!w) return HB_OK;
+    const cudaError_t e = cudaMemsetAsync(w, 0, (size_t)s->experts * s->hidden * s->width * rows::type_bytes(s->type), st);
+    return e == cudaSuccess ? HB_OK : abi_fail(HB_LAUNCH, std::string(what) + ": " + cudaGetErrorString(e));
+}
+// dW of one or two products over the same x.
+Job weights_job(const hb_expert_shape* s, const int32_t* offsets, int segments) {
+    Job j = job_of(s, offsets, kWeights, s->hidden, s->width);
+    j.out_row = s->width;
+    j.segments = segments;
+    j.splits = splits_of(j);
+    return j;
+}
+bool valid(const hb_expert_shape* s) {
+    return s && rows::valid_type(s->type) && s->rows >= 0 && s->rows <= INT32_MAX - 1024 && s->hidden >= 1 && s->width >= 1 &&
+           s->hidden <= (1 << 28) && s->width <= (1 << 28) && s->experts >= 1 && s->experts <= kMostGroups;
+}
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+size_t held_bytes(const hb_expert_shape* s) { return round256((size_t)s->rows * padded(s->hidden) * rows::type_bytes(s->type)); }
+}  // namespace
+
+extern "C" size_t hb_expert_product_grad_workspace(const hb_expert_shape* s) {
+    if (!valid(s)) return 0;
+    const Job j = weights_job(s, nullptr, 1);
+    return partial_bytes(j, j.splits);
+}
+
+extern "C" int hb_expert_product_grad(const hb_expert_shape* s, const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
+                                      const int32_t* offsets, const hb_expert_weight* weight, void* dx, void* dweight,
+                                      void* workspace, size_t workspace_bytes, void* stream) {
+    const char* what = "hb_expert_product_grad";
+    if (const int rc = check(s, offsets, what)) return rc;
+    const auto st = static_cast<cudaStream_t>(stream);
+    const Operand dyo = rows_of(dy, dy_stride), xo = rows_of(x, x_stride), w = weight_of(weight);
+    if ((s->rows > 0 && (!fits(dyo, s->type, s->hidden, s->rows, false, 1, true) ||
+                         (dweight && !fits(xo, s->type, s->width, s->rows, false, 1, true)))) ||
+        (dx && !fits(w, s->type, s->width, s->hidden, true, s->experts, true)) || !aligned_out(dx, s->type) || !aligned_out(dweight, s->type))
+        return abi_fail(HB_BAD_ARGUMENT, std::string(what) + ": " + kOperand);
+    if (s->rows == 0) return zero_weights(s, dweight, st, what);
+    if (dweight)
+        if (const int rc = bad_workspace(workspace, workspace_bytes, hb_expert_product_grad_workspace(s), what)) return rc;
+    if (dx) {
+        Job j = job_of(s, offsets, kBack, s->width, s->hidden);
+        j.a[0] = tidy(dyo, s->hidden, s->rows, 1);
+        j.b[0] = tidy(w, s->width, s->hidden, s->experts);
+        j.out[0] = dx;
+        if (const int rc = run(j, st)) return rc;
+    }
+    if (!dweight) return HB_OK;
+    Job j = weights_job(s, offsets, 1);
+    j.a[0] = tidy(dyo, s->hidden, s->rows, 1);
+    j.b[0] = tidy(xo, s->width, s->rows, 1);
+    j.out[0] = dweight;
+    j.partial = static_cast<float*>(workspace);
+    return run(j, st);
+}
+
+extern "C" size_t hb_expert_gated_grad_workspace(const hb_expert_shape* s) {
+    if (!valid(s)) return 0;
+    size_t most = 0;  // one gradient alone may be cut into more parts than both
+    for (int segments : {1, 2}) {
+        const Job j = weights_job(s, nullptr, segments);
+        most = std::max(most, partial_bytes(j, j.splits));
+    }
+    return 2 * held_bytes(s) + most;
+}
+
+extern "C" int hb_expert_gated_grad(const hb_expert_shape* s, const void* dh, int64_t dh_stride, const void* x, int64_t x_stride,
+                                    const int32_t* offsets, const hb_expert_weight* gate, const hb_expert_weight* up, void* dx,
+                                    void* dgate, void* dup, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* what = "hb_expert_gated_grad";
+    if (const int rc = check(s, offsets, what)) return rc;
+    const auto st = static_cast<cudaStream_t>(stream);
+    const Operand dho = rows_of(dh, dh_stride), xo = rows_of(x, x_stride), g = weight_of(gate), u = weight_of(up);
+    if ((s->rows > 0 && (!fits(dho, s->type, s->hidden, s->rows, false, 1, false) || !fits(xo, s->type, s->width, s->rows, false, 1, true))) ||
+        !fits(g, s->type, s->width, s->hidden, true, s->experts, true) || !fits(u, s->type, s->width, s->hidden, true, s->experts, true) ||
+        !aligned_out(dx, s->type) || !aligned_out(dgate, s->type) || !aligned_out(dup, s->type))
+        return abi_fail(HB_BAD_ARGUMENT, std::string(what) + ": " + kOperand);
+    if (s->rows == 0) {
+        if (const int rc = zero_weights(s, dgate, st, what)) return rc;
+        return zero_weights(s, dup, st, what);
+    }
+    if (const int rc = bad_workspace(workspace, workspace_bytes, hb_expert_gated_grad_workspace(s), what)) return rc;
+    const int64_t held = padded(s->hidden);
+    char* const ws = static_cast<char*>(workspace);
+    void* const part[2] = {ws, ws + held_bytes(s)};
+    Job j = job_of(s, offsets, kGatedGrad, s->hidden, s->width);
+    j.a[0] = tidy(xo, s->width, s->rows, 1);
+    j.b[0] = tidy(g, s->width, s->hidden, s->experts);
+    j.b[1] = tidy(u, s->width, s->hidden, s->experts);
+    j.dh = dho;
+    j.out[0] = part[0];
+    j.out[1] = part[1];
+    j.out_row = held;
+    if (const int rc = run(j, st)) return rc;
+    if (dx) {
+        Job back = job_of(s, offsets, kBack, s->width, s->hidden);
+        back.a[0] = {part[0], held, 0};
+        back.a[1] = {part[1], held, 0};
+        back.b[0] = j.b[0];
+        back.b[1] = j.b[1];
+        back.segments = 2;
+        back.out[0] = dx;
+        if (const int rc = run(back, st)) return rc;
+    }
+    if (!dgate && !dup) return HB_OK;
+    Job w = weights_job(s, offsets, (dgate ? 1 : 0) + (dup ? 1 : 0));
+    for (int i = 0, at = 0; i < 2; ++i) {
+        if (!(i ? dup : dgate)) continue;
+        w.a[at] = {part[i], held, 0};
+        w.out[at++] = i ? dup : dgate;
+    }
+    w.b[0] = j.a[0];
+    w.partial = reinterpret_cast<float*>(ws + 2 * held_bytes(s));
+    return run(w, st);
+}

@@ -1,0 +1,128 @@
+// What the kernels of the experts' products share: the rows of each expert, the
+// activations, and the forms that experts.cu hands to experts_simt.cu.
+#pragma once
+#include <cstdint>
+#include <cuda_runtime.h>
+
+#include "rows.cuh"
+
+namespace hb {
+namespace experts {
+
+// Forms of a product.  Row forms go over the rows of each expert, kWeights over each expert's weight.
+//   kProduct    out = a b^T                    kGated      out = act(a b0^T) * (a b1^T)
+//   kGatedGrad  out0 = dh u act'(g), out1 = dh act(g), g = a b0^T, u = a b1^T
+//   kBack       out = sum over segments a b    kWeights    out = a^T b over the expert's rows
+enum Form { kProduct, kGated, kGatedGrad, kBack, kWeights };
+constexpr int kSilu = 0, kGelu = 1;
+constexpr int kMostGroups = 2048;  // experts of a call: their first rows and tiles lie in shared memory
+
+struct Operand {
+    const void* p;
+    int64_t row, group;  // distance of rows and of experts in elements (group: weights alone)
+};
+
+// One product, types and sizes as the C entry checked them.
+struct Job {
+    int type, form, activation;
+    const int32_t* offsets;  // null: all rows are the only expert's
+    int groups, rows;
+    int n, k;                // columns of the output; summed length (kWeights: n x k columns of a and b: out is [n][k])
+    Operand a[2], b[2];
+    Operand dh;              // kGatedGrad
+    void* out[2];
+    int64_t out_row;         // distance of the outputs' rows in elements
+    int segments;            // kBack: products added up; kWeights: products side by side (a[i], out[i])
+    int splits;              // kWeights: parts of the expert's rows that are summed apart; above 1 they go to `partial`,
+    float* partial;          // fp32 [splits][segments][groups][n][k], and are added in order
+};
+
+// The part `split` of an expert's `length` rows: whole stages of 64.
+__host__ __device__ inline void split_rows(int length, int splits, int split, int& begin, int& end) {
+    const int stages = ((length + 63) / 64 + splits - 1) / splits;
+    begin = (int)(length < (int64_t)split * stages * 64 ? length : (int64_t)split * stages * 64);
+    end = (int)(length < (int64_t)begin + stages * 64 ? length : (int64_t)begin + stages * 64);
+}
+
+// The expert's rows [begin, end): offsets are read as their running maximum inside 0..rows, so that whatever they hold
+// the experts' rows are apart and inside.  Group `groups` is the rows behind the last expert.  Fills start[0..groups+1]
+// and tile[0..groups+1], the number of tiles of TILE rows before each group; called by a whole block.
+__device__ inline void read_groups(const int32_t* offsets, int groups, int rows, int tile_rows, int* start, int* tile) {
+    const int t = threadIdx.x;
+    if (!offsets) {
+        if (t == 0) start[0] = 0, start[1] = start[2] = rows;
+    } else if (t < 32) {  // running maximum, 32 at a time
+        int most = 0;
+        for (int base = 0; base <= groups; base += 32) {
+            const int i = base + t;
+            int v = i == 0 || i > groups ? 0 : min(max(offsets[i], 0), rows);
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int o = __shfl_up_sync(0xffffffffu, v, d);
+                if (t >= d) v = max(v, o);
+            }
+            v = max(v, most);
+            if (i <= groups) start[i] = v;
+            most = __shfl_sync(0xffffffffu, v, 31);
+        }
+        if (t == 0) start[groups + 1] = rows;
+    }
+    __syncthreads();
+    if (t < 32) {  // sums of tiles
+        int before = 0;
+        for (int base = 0; base <= groups; base += 32) {
+            const int i = base + t;
+            const int own = i <= groups ? (start[i + 1] - start[i] + tile_rows - 1) / tile_rows : 0;
+            int v = own;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int o = __shfl_up_sync(0xffffffffu, v, d);
+                if (t >= d) v += o;
+            }
+            if (i <= groups) tile[i] = before + v - own;
+            before += __shfl_sync(0xffffffffu, v, 31);
+        }
+        if (t == 0) tile[groups + 1] = before;
+    }
+    __syncthreads();
+}
+
+// The group of a tile: the last one whose first tile is at or before it and that has tiles.
+__device__ inline int group_of(const int* tile, int groups, int t) {
+    int lo = 0, hi = groups;  // groups + 1 of them
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (tile[mid] <= t) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+// act(g) and, with SLOPE, act'(g).  PRECISE: results that are held in 32 bits; otherwise the fast exponential and
+// quotient (2^-21 relative), 8 bits below the rounding of a 16-bit result.
+template <bool PRECISE>
+__device__ __forceinline__ float sigmoid(float g) {
+    if (PRECISE) return 1.0f / (1.0f + expf(-g));
+    return __fdividef(1.0f, 1.0f + __expf(-g));
+}
+template <bool PRECISE, bool SLOPE>
+__device__ __forceinline__ float activate(int kind, float g, float& slope) {
+    if (kind == kSilu) {
+        const float s = sigmoid<PRECISE>(g);
+        if (SLOPE) slope = s * fmaf(g, 1.0f - s, 1.0f);
+        return g * s;
+    }
+    const float cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
+    if (SLOPE) slope = fmaf(g * 0.39894228040143268f, PRECISE ? expf(-0.5f * g * g) : __expf(-0.5f * g * g), cdf);
+    return g * cdf;
+}
+
+// Up to this many rows the weights are streamed by warps (experts_simt.cu), any type.
+constexpr int kFewRows = HB_EXPERT_FEW_ROWS;
+cudaError_t few_rows(const Job& job, cudaStream_t st);
+cudaError_t product_f32(const Job& job, cudaStream_t st);
+// Adds the parts of kWeights in order and rounds them once.
+cudaError_t join_parts(const Job& job, cudaStream_t st);
+
+}  // namespace experts
+}  // namespace hb

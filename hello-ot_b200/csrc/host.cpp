@@ -1,4 +1,4 @@
-// Host path of the routing, lookup and clipping calls: argument checks, output allocation and the call of
+// Host path of the calls around and in a routed layer (routing, lookup, clipping, experts, norm, optimizer step): argument checks, output allocation and the call of
 // the C ABI, as a Python extension module (hello_ot_b200._host).
 //
 // The kernels of a small call take 2 to 8 us, so what a user waits for is the host: through ctypes and
@@ -513,6 +513,508 @@ PyObject* clip(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------- experts
+int64_t on_eight(int64_t width) { return (width + 7) / 8 * 8; }
+// A copy whose rows begin on 16 bytes, for 16-bit operands off that grid.
+Tensor on_grid(const Tensor& t) {
+    c10::SmallVector<int64_t, 3> shape(t.sizes().begin(), t.sizes().end());
+    const int64_t width = shape.back();
+    shape.back() = on_eight(width);
+    Tensor copy = at::empty(shape, t.options()).narrow(-1, 0, width);
+    copy.copy_(t);
+    return copy;
+}
+bool off(const void* p, size_t unit) { return reinterpret_cast<uintptr_t>(p) % unit != 0; }
+
+// Sorted rows as the products take them; grid: 16-bit rows lie on 16 bytes and apart.
+Rows expert_rows(const Tensor& given, const char* name, bool grid) {
+    Rows r = feature_rows(given, name);
+    if (!grid || r.type == HB_F32 || r.t.numel() == 0) return r;
+    const int64_t width = r.t.size(1);
+    if (off(r.t.const_data_ptr(), 16) || (r.t.size(0) > 1 && (r.stride % 8 != 0 || r.stride < width)) || r.stride > INT32_MAX) {
+        r.t = on_grid(r.t);
+        r.stride = r.t.stride(0);
+    }
+    return r;
+}
+struct Weight {
+    Tensor t;
+    hb_expert_weight w;
+};
+// [experts, hidden, width], or [hidden, width] of one expert, without a copy where its rows are contiguous (and on the grid).
+Weight expert_weight(const Tensor& given, const char* name, bool grid) {
+    TORCH_CHECK_VALUE(given.dim() == 3 || given.dim() == 2, name, " must be [experts, hidden, width], or [hidden, width] of one expert, got ",
+                      given.sizes());
+    const int type = type_of(given, name);
+    Tensor t = resolved(given.dim() == 3 ? given : given.unsqueeze(0));
+    const int64_t experts = t.size(0), hidden = t.size(1), width = t.size(2);
+    TORCH_CHECK_VALUE(hidden >= 1 && width >= 1 && experts >= 1, name, " must have elements, got ", given.sizes());
+    auto plain = [&](const Tensor& v) {
+        return (width == 1 || v.stride(2) == 1) && (hidden == 1 || v.stride(1) >= width) && v.stride(0) < (int64_t(1) << 38) &&
+               v.stride(1) <= INT32_MAX;
+    };
+    if (!plain(t)) t = t.contiguous();
+    if (grid && type != HB_F32 &&
+        (off(t.const_data_ptr(), 16) || (hidden > 1 && t.stride(1) % 8 != 0) || (experts > 1 && t.stride(0) % 8 != 0)))
+        t = on_grid(t);
+    return {t, {t.const_data_ptr(), hidden > 1 ? t.stride(1) : on_eight(width), t.stride(0)}};
+}
+int activation_of(PyObject* o) {
+    const char* name = PyUnicode_Check(o) ? PyUnicode_AsUTF8(o) : "";
+    if (!name) throw python_error();
+    if (std::strcmp(name, "silu") == 0) return HB_SILU;
+    TORCH_CHECK_VALUE(std::strcmp(name, "gelu") == 0, "activation must be 'silu' or 'gelu'");
+    return HB_GELU;
+}
+// The first rows of the experts, null without them.
+const int32_t* first_rows(const Tensor& offsets, int64_t experts, const char* what) {
+    if (!offsets.defined()) {
+        TORCH_CHECK_VALUE(experts == 1, what, ": offsets are needed for ", experts, " experts");
+        return nullptr;
+    }
+    TORCH_CHECK_VALUE(offsets.scalar_type() == at::kInt && offsets.dim() == 1 && offsets.is_contiguous() && offsets.numel() == experts + 1, what,
+                      ": offsets must be int32 [experts + 1], contiguous; got ", offsets.scalar_type(), " ", offsets.sizes(), " for ",
+                      experts, " experts");
+    return offsets.const_data_ptr<int32_t>();
+}
+// Shapes that belong together: x [rows, width], weights [experts, hidden, width], dy [rows, hidden].
+hb_expert_shape shape_of(const Rows& x, std::initializer_list<const Weight*> weights, const Rows* dy, int activation, const char* what) {
+    const Weight& w = **weights.begin();
+    const int64_t experts = w.t.size(0), hidden = w.t.size(1), width = w.t.size(2), rows = x.t.size(0);
+    for (const Weight* v : weights)
+        TORCH_CHECK_VALUE(v->t.sizes() == w.t.sizes() && v->t.scalar_type() == x.t.scalar_type() && width == x.t.size(1), what, ": x ",
+                          x.t.sizes(), " ", x.t.scalar_type(), " and weights ", w.t.sizes(), ", ", v->t.sizes(), " ", v->t.scalar_type(),
+                          " do not fit");
+    TORCH_CHECK_VALUE(!dy || (dy->t.size(0) == rows && dy->t.size(1) == hidden && dy->type == x.type), what,
+                      ": the gradient's rows do not fit x and the weights");
+    TORCH_CHECK_VALUE(experts <= 2048, what, ": at most 2048 experts, got ", experts);
+    TORCH_CHECK_VALUE(rows <= INT32_MAX - 1024, what, ": too many rows");
+    return {rows, width, hidden, experts, x.type, activation};
+}
+
+// expert_product(x, weight, offsets or None) -> y
+PyObject* expert_product(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const char* what = "expert_product";
+    expect(n, 3, what);
+    const Tensor &given = tensor(args[0], "x"), &given_weight = tensor(args[1], "weight");
+    const Tensor offsets = tensor_or_none(args[2], "offsets");
+    return wrap(unlocked([&] {
+        const c10::Device device = device_of(what, {&given, &given_weight, offsets.defined() ? &offsets : &given});
+        const Launch on(device);
+        const bool grid = given.dim() == 2 && given.size(0) > HB_EXPERT_FEW_ROWS;
+        const Rows x = expert_rows(given, "x", grid);
+        const Weight w = expert_weight(given_weight, "weight", grid);
+        const hb_expert_shape shape = shape_of(x, {&w}, nullptr, HB_SILU, what);
+        const int32_t* first = first_rows(offsets, shape.experts, what);
+        Tensor out = at::empty({shape.rows, shape.hidden}, x.t.options());
+        check(hb_expert_product(&shape, x.t.const_data_ptr(), x.stride, first, &w.w, out.data_ptr(), on.stream));
+        return out;
+    }));
+    END_HANDLE_TH_ERRORS
+}
+
+// expert_gated(x, gate, up, offsets or None, activation) -> h
+PyObject* expert_gated(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const char* what = "expert_gated";
+    expect(n, 5, what);
+    const Tensor &given = tensor(args[0], "x"), &given_gate = tensor(args[1], "w_gate"), &given_up = tensor(args[2], "w_up");
+    const Tensor offsets = tensor_or_none(args[3], "offsets");
+    const int activation = activation_of(args[4]);
+    return wrap(unlocked([&] {
+        const c10::Device device = device_of(what, {&given, &given_gate, &given_up, offsets.defined() ? &offsets : &given});
+        const Launch on(device);
+        const bool grid = given.dim() == 2 && given.size(0) > HB_EXPERT_FEW_ROWS;
+        const Rows x = expert_rows(given, "x", grid);
+        const Weight g = expert_weight(given_gate, "w_gate", grid), u = expert_weight(given_up, "w_up", grid);
+        const hb_expert_shape shape = shape_of(x, {&g, &u}, nullptr, activation, what);
+        const int32_t* first = first_rows(offsets, shape.experts, what);
+        Tensor out = at::empty({shape.rows, shape.hidden}, x.t.options());
+        check(hb_expert_gated(&shape, x.t.const_data_ptr(), x.stride, first, &g.w, &u.w, out.data_ptr(), on.stream));
+        return out;
+    }));
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject* tuple_of(std::initializer_list<const Tensor*> tensors) {  // undefined ones are None
+    THPObjectPtr result(PyTuple_New((Py_ssize_t)tensors.size()));
+    if (!result) throw python_error();
+    Py_ssize_t i = 0;
+    for (const Tensor* t : tensors) PyTuple_SET_ITEM(result.get(), i++, wrap(*t));
+    return result.release();
+}
+
+// expert_product_grad(dy, x, weight, offsets or None, need_x, need_weight) -> (dx or None, dweight or None)
+PyObject* expert_product_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const char* what = "expert_product_grad";
+    expect(n, 6, what);
+    untraced(what);
+    const Tensor &given_dy = tensor(args[0], "dy"), &given = tensor(args[1], "x"), &given_weight = tensor(args[2], "weight");
+    const Tensor offsets = tensor_or_none(args[3], "offsets");
+    const bool need_x = args[4] == Py_True, need_w = args[5] == Py_True;
+    Tensor dx, dw;
+    unlocked([&] {
+        const c10::Device device = device_of(what, {&given, &given_dy, &given_weight, offsets.defined() ? &offsets : &given});
+        const Launch on(device);
+        const Rows dy = expert_rows(given_dy, "dy", true), x = expert_rows(given, "x", need_w);
+        const Weight w = expert_weight(given_weight, "weight", need_x);
+        const hb_expert_shape shape = shape_of(x, {&w}, &dy, HB_SILU, what);
+        const int32_t* first = first_rows(offsets, shape.experts, what);
+        if (need_x) dx = at::empty({shape.rows, shape.width}, x.t.options());
+        if (need_w) dw = at::empty(given_weight.sizes(), x.t.options());
+        const size_t size = need_w ? hb_expert_product_grad_workspace(&shape) : 0;
+        Tensor ws;
+        if (size) ws = workspace(size, device);
+        check(hb_expert_product_grad(&shape, dy.t.const_data_ptr(), dy.stride, x.t.const_data_ptr(), x.stride, first, &w.w,
+                                     need_x ? dx.data_ptr() : nullptr, need_w ? dw.data_ptr() : nullptr, size ? ws.data_ptr() : nullptr, size,
+                                     on.stream));
+    });
+    return tuple_of({&dx, &dw});
+    END_HANDLE_TH_ERRORS
+}
+
+// expert_gated_grad(dh, x, gate, up, offsets or None, activation, need_x, need_gate, need_up) -> (dx, dgate, dup), None for those not needed
+PyObject* expert_gated_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const char* what = "expert_gated_grad";
+    expect(n, 9, what);
+    untraced(what);
+    const Tensor &given_dh = tensor(args[0], "dh"), &given = tensor(args[1], "x"), &given_gate = tensor(args[2], "w_gate"),
+                 &given_up = tensor(args[3], "w_up");
+    const Tensor offsets = tensor_or_none(args[4], "offsets");
+    const int activation = activation_of(args[5]);
+    const bool need_x = args[6] == Py_True, need_g = args[7] == Py_True, need_u = args[8] == Py_True;
+    Tensor dx, dg, du;
+    unlocked([&] {
+        const c10::Device device = device_of(what, {&given, &given_dh, &given_gate, &given_up, offsets.defined() ? &offsets : &given});
+        const Launch on(device);
+        const Rows dh = expert_rows(given_dh, "dh", false), x = expert_rows(given, "x", true);
+        const Weight g = expert_weight(given_gate, "w_gate", true), u = expert_weight(given_up, "w_up", true);
+        const hb_expert_shape shape = shape_of(x, {&g, &u}, &dh, activation, what);
+        const int32_t* first = first_rows(offsets, shape.experts, what);
+        if (need_x) dx = at::empty({shape.rows, shape.width}, x.t.options());
+        if (need_g) dg = at::empty(given_gate.sizes(), x.t.options());
+        if (need_u) du = at::empty(given_up.sizes(), x.t.options());
+        if (!need_x && !need_g && !need_u) return;
+        const size_t size = hb_expert_gated_grad_workspace(&shape);
+        Tensor ws = workspace(size, device);
+        check(hb_expert_gated_grad(&shape, dh.t.const_data_ptr(), dh.stride, x.t.const_data_ptr(), x.stride, first, &g.w, &u.w,
+                                   need_x ? dx.data_ptr() : nullptr, need_g ? dg.data_ptr() : nullptr, need_u ? du.data_ptr() : nullptr,
+                                   ws.data_ptr(), size, on.stream));
+    });
+    return tuple_of({&dx, &dg, &du});
+    END_HANDLE_TH_ERRORS
+}
+
+// ---------------------------------------------------------------- norm
+// A tensor [..., width] as rows.
+Rows rows_2d(const Tensor& t, const char* name) {
+    TORCH_CHECK_VALUE(t.dim() >= 1 && t.size(-1) >= 1, name, " must be [..., width] with at least one column, got ", t.sizes());
+    return feature_rows(t.dim() == 2 ? t : t.reshape({t.numel() / t.size(-1), t.size(-1)}), name);
+}
+Tensor norm_weight(const Tensor& given, int64_t width) {
+    type_of(given, "weight");
+    TORCH_CHECK_VALUE(given.dim() == 1 && given.size(0) == width, "weight must be [", width, "], got ", given.sizes());
+    return resolved(given).contiguous();
+}
+
+// rms_norm(x, weight, residual or None, eps, bits8) -> (y or codes, None or scales, total or None)
+PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const char* what = "rms_norm";
+    expect(n, 5, what);
+    const bool bits8 = args[4] == Py_True;
+    if (bits8) untraced("rms_norm_8bit");
+    const Tensor &given = tensor(args[0], "x"), &given_weight = tensor(args[1], "weight");
+    const Tensor given_residual = tensor_or_none(args[2], "residual");
+    const double eps = number(args[3]);
+    Tensor y, scales, total;
+    unlocked([&] {
+        const bool add = given_residual.defined();
+        const c10::Device device = device_of(what, {&given, &given_weight, add ? &given_residual : &given});
+        const Launch on(device);
+        const Rows x = rows_2d(given, "x");
+        const int64_t count = x.t.size(0), width = x.t.size(1);
+        TORCH_CHECK_VALUE(!add || (given_residual.sizes() == given.sizes() && given_residual.scalar_type() == given.scalar_type()), what,
+                          ": the residual has x's shape and type, got ", given_residual.sizes(), " ", given_residual.scalar_type());
+        const Rows residual = add ? rows_2d(given_residual, "residual") : x;
+        const Tensor weight = norm_weight(given_weight, width);
+        if (bits8) {
+            y = at::empty(given.sizes(), x.t.options().dtype(at::kFloat8_e4m3fn));
+            c10::SmallVector<int64_t, 8> shape(given.sizes().begin(), given.sizes().end());
+            shape.back() = (width + 31) / 32;
+            scales = at::empty(shape, x.t.options().dtype(at::kFloat8_e8m0fnu));
+        } else {
+            y = at::empty(given.sizes(), x.t.options());
+        }
+        if (add) total = at::empty(given.sizes(), x.t.options());
+        check(hb_rms_norm(x.type, x.t.const_data_ptr(), x.stride, add ? residual.t.const_data_ptr() : nullptr, residual.stride, count, width,
+                          weight.const_data_ptr(), type_of(weight, "weight"), eps, bits8 ? nullptr : y.data_ptr(),
+                          bits8 ? y.data_ptr() : nullptr, bits8 ? scales.data_ptr() : nullptr, add ? total.data_ptr() : nullptr, on.stream));
+    });
+    return tuple_of({&y, &scales, &total});
+    END_HANDLE_TH_ERRORS
+}
+
+// rows_of_8bit(codes, scales, dtype) -> values
+PyObject* rows_of_8bit(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const char* what = "rows_of_8bit";
+    expect(n, 3, what);
+    untraced(what);
+    const Tensor &given = tensor(args[0], "values"), &given_scales = tensor(args[1], "scales");
+    TORCH_CHECK_VALUE(THPDtype_Check(args[2]), what, ": dtype must be a torch.dtype");
+    const at::ScalarType type = reinterpret_cast<THPDtype*>(args[2])->scalar_type;
+    return wrap(unlocked([&] {
+        const c10::Device device = device_of(what, {&given, &given_scales});
+        const Launch on(device);
+        TORCH_CHECK_VALUE(type_or(type, -1) >= 0, what, ": dtype must be float32, float16 or bfloat16, got ", type);
+        TORCH_CHECK_VALUE(given.scalar_type() == at::kFloat8_e4m3fn && given_scales.scalar_type() == at::kFloat8_e8m0fnu && given.dim() >= 1 &&
+                              given.size(-1) >= 1 && given_scales.dim() == given.dim() && given_scales.size(-1) == (given.size(-1) + 31) / 32 &&
+                              given_scales.sizes().slice(0, given.dim() - 1) == given.sizes().slice(0, given.dim() - 1),
+                          what, ": values e4m3 [..., width] with scales e8m0 [..., ceil(width / 32)], got ", given.sizes(), " and ",
+                          given_scales.sizes());
+        const Tensor codes = given.contiguous(), scales = given_scales.contiguous();
+        Tensor out = at::empty(given.sizes(), given.options().dtype(type));
+        check(hb_rows_of_8bit(codes.const_data_ptr(), scales.const_data_ptr(), codes.numel() / codes.size(-1), codes.size(-1),
+                              type_or(type, HB_F32), out.data_ptr(), on.stream));
+        return out;
+    }));
+    END_HANDLE_TH_ERRORS
+}
+
+// rms_norm_grad(dy, x, weight, dsum or None, eps, need_x, need_weight) -> (dx or None, dweight or None)
+PyObject* rms_norm_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const char* what = "rms_norm_grad";
+    expect(n, 7, what);
+    untraced(what);
+    const Tensor &given_dy = tensor(args[0], "dy"), &given = tensor(args[1], "x"), &given_weight = tensor(args[2], "weight");
+    const Tensor given_dsum = tensor_or_none(args[3], "dsum");
+    const double eps = number(args[4]);
+    const bool need_x = args[5] == Py_True, need_w = args[6] == Py_True;
+    Tensor dx, dw;
+    unlocked([&] {
+        const bool add = given_dsum.defined();
+        const c10::Device device = device_of(what, {&given, &given_dy, &given_weight, add ? &given_dsum : &given});
+        const Launch on(device);
+        TORCH_CHECK_VALUE(given_dy.sizes() == given.sizes() && given_dy.scalar_type() == given.scalar_type() &&
+                              (!add || (given_dsum.sizes() == given.sizes() && given_dsum.scalar_type() == given.scalar_type())),
+                          what, ": gradients have x's shape and type, got ", given_dy.sizes(), " ", given_dy.scalar_type(), " for ",
+                          given.sizes(), " ", given.scalar_type());
+        const Rows x = rows_2d(given, "x"), dy = rows_2d(given_dy, "dy"), dsum = add ? rows_2d(given_dsum, "dsum") : x;
+        const int64_t count = x.t.size(0), width = x.t.size(1);
+        const Tensor weight = norm_weight(given_weight, width);
+        if (need_x) dx = at::empty(given.sizes(), x.t.options());
+        if (need_w) dw = at::empty({width}, weight.options());
+        const size_t size = hb_rms_norm_grad_workspace(count, width);
+        Tensor ws = workspace(size, device);
+        check(hb_rms_norm_grad(x.type, dy.t.const_data_ptr(), dy.stride, x.t.const_data_ptr(), x.stride,
+                               add ? dsum.t.const_data_ptr() : nullptr, dsum.stride, count, width, weight.const_data_ptr(),
+                               type_of(weight, "weight"), eps, need_x ? dx.data_ptr() : nullptr, need_w ? dw.data_ptr() : nullptr,
+                               ws.data_ptr(), size, on.stream));
+    });
+    return tuple_of({&dx, &dw});
+    END_HANDLE_TH_ERRORS
+}
+
+// ---------------------------------------------------------------- optimizer step
+// Lists of a step: tensor i of each belongs to parameter i.
+struct Step {
+    const char* what;
+    c10::Device device{c10::kCPU};
+    std::vector<Tensor> params, changed;
+    std::vector<int64_t> size;
+    std::vector<Extent> written, read;
+    Step(const char* name) : what(name) {}
+    void span(const Tensor& t, std::vector<Extent>& to) {
+        if (t.numel() == 0) return;
+        const char* begin = static_cast<const char*>(t.const_data_ptr());
+        to.push_back({begin, begin + t.nbytes(), 0});
+    }
+    const Tensor& on_device(PyObject* o, const char* name) {
+        const Tensor& t = tensor(o, name);
+        if (!device.is_cuda()) device = device_of(what, {&t});
+        if (t.device() != device) device_of(what, {&t, params.empty() ? &t : &params[0]});
+        TORCH_CHECK_VALUE(t.device() == device, what, ": ", name, " on another device than the parameters");
+        TORCH_CHECK_VALUE(!t.is_neg() && !t._is_zerotensor(), what, ": ", name, " must hold its values in memory");
+        return t;
+    }
+};
+struct Items {  // a list of tensors, or of None
+    THPObjectPtr items;
+    Items(PyObject* o, const char* name, Py_ssize_t want, const char* what) : items(PySequence_Fast(o, "a list of tensors is needed")) {
+        if (!items) throw python_error();
+        TORCH_CHECK_VALUE(want < 0 || size() == want, what, ": ", size(), " ", name, " for ", want, " parameters");
+    }
+    Py_ssize_t size() const { return PySequence_Fast_GET_SIZE(items.get()); }
+    PyObject* operator[](Py_ssize_t i) const { return PySequence_Fast_GET_ITEM(items.get(), i); }
+};
+// The addresses of a list whose tensors lie in memory as the parameters do.
+std::vector<void*> like_params(Step& s, PyObject* o, const char* name, at::ScalarType type, bool gaps, bool writes) {
+    const Py_ssize_t n = (Py_ssize_t)s.params.size();
+    const Items items(o, name, n, s.what);
+    std::vector<void*> at(n, nullptr);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        if (gaps && items[i] == Py_None) continue;
+        const Tensor &t = s.on_device(items[i], name), &p = s.params[i];
+        TORCH_CHECK_VALUE(t.scalar_type() == type, s.what, ": ", name, " must be ", type, ", got ", t.scalar_type());
+        TORCH_CHECK_VALUE(t.sizes() == p.sizes() && ((t.is_contiguous() && p.is_contiguous()) || t.strides() == p.strides()), s.what, ": ", name,
+                          " have their parameters' shapes and strides, got ", t.sizes(), " for ", p.sizes());
+        if (t.numel()) at[i] = t.data_ptr();
+        if (writes) s.span(t, s.written), s.changed.push_back(t);
+    }
+    return at;
+}
+std::vector<float*> scales_of(Step& s, PyObject* o, const char* name, bool writes) {
+    const Py_ssize_t n = (Py_ssize_t)s.size.size();
+    const Items items(o, name, n, s.what);
+    std::vector<float*> at(n, nullptr);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        const Tensor& t = s.on_device(items[i], name);
+        TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat && t.is_contiguous() && t.numel() == (s.size[i] + 255) / 256, s.what, ": ", name,
+                          " must be float32, one for each 256 elements");
+        if (t.numel()) at[i] = static_cast<float*>(t.data_ptr());
+        if (writes) s.span(t, s.written), s.changed.push_back(t);
+    }
+    return at;
+}
+// A float32 number on the device.
+const float* device_number(Step& s, PyObject* o, const char* name) {
+    const Tensor& t = s.on_device(o, name);
+    TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat && t.numel() == 1, s.what, ": ", name, " on the device must be one float32 value");
+    s.span(t, s.read);
+    return static_cast<const float*>(t.const_data_ptr());
+}
+void check_apart(Step& s) {
+    auto before = [](const Extent& a, const Extent& b) { return a.begin < b.begin; };
+    std::sort(s.written.begin(), s.written.end(), before);
+    for (size_t i = 1; i < s.written.size(); ++i)
+        TORCH_CHECK_VALUE(s.written[i].begin >= s.written[i - 1].end, s.what, ": tensors that are written overlap in memory");
+    for (const Extent& r : s.read) {
+        auto w = std::upper_bound(s.written.begin(), s.written.end(), r.begin, [](const char* p, const Extent& e) { return p < e.end; });
+        TORCH_CHECK_VALUE(w == s.written.end() || w->begin >= r.end, s.what, ": a tensor that is written overlaps a gradient or number in memory");
+    }
+}
+
+// adamw_step(params, grads, first, second, first_scale or None, second_scale or None, master or None, step, lr, beta1, beta2, eps,
+//            decay, norm or None, max_norm)
+PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Step s("adamw_step");
+    expect(n, 15, s.what);
+    untraced(s.what);
+    const Items params(args[0], "parameters", -1, s.what);
+    const Py_ssize_t count = params.size();
+    TORCH_CHECK_VALUE(count > 0, s.what, ": no parameters");
+    s.params.reserve(count), s.size.reserve(count), s.written.reserve(6 * count + 1), s.read.reserve(count + 2), s.changed.reserve(6 * count + 1);
+    std::vector<void*> param(count);
+    std::vector<int32_t> type(count), grad_type(count);
+    for (Py_ssize_t i = 0; i < count; ++i) {
+        const Tensor& t = s.on_device(params[i], "a parameter");
+        type[i] = type_of(t, "parameters");
+        TORCH_CHECK_VALUE(t.is_contiguous() || t.is_non_overlapping_and_dense(), s.what, ": parameters must be dense in memory, got strides ",
+                          t.strides(), " for ", t.sizes());
+        param[i] = t.numel() ? t.data_ptr() : nullptr;
+        s.params.push_back(t);
+        s.size.push_back(t.numel());
+        s.span(t, s.written);
+        s.changed.push_back(t);
+    }
+    const Items grads(args[1], "gradients", count, s.what);
+    std::vector<const void*> grad(count);
+    for (Py_ssize_t i = 0; i < count; ++i) {
+        const Tensor &t = s.on_device(grads[i], "a gradient"), &p = s.params[i];
+        grad_type[i] = type_of(t, "gradients");
+        TORCH_CHECK_VALUE(grad_type[i] == type[i] || grad_type[i] == HB_F32, s.what, ": a gradient has its parameter's type or is float32, got ",
+                          t.scalar_type(), " for ", p.scalar_type());
+        TORCH_CHECK_VALUE(t.sizes() == p.sizes() && ((t.is_contiguous() && p.is_contiguous()) || t.strides() == p.strides()), s.what,
+                          ": gradients have their parameters' shapes and strides, got ", t.sizes(), " for ", p.sizes());
+        grad[i] = t.numel() ? t.const_data_ptr() : nullptr;
+        s.span(t, s.read);
+    }
+    const bool bits8 = args[4] != Py_None || args[5] != Py_None;
+    const at::ScalarType held = bits8 ? at::kFloat8_e4m3fn : at::kFloat;
+    const std::vector<void*> first = like_params(s, args[2], "first moments", held, false, true);
+    const std::vector<void*> second = like_params(s, args[3], "second moments", held, false, true);
+    std::vector<float*> first_scale, second_scale;
+    if (bits8) first_scale = scales_of(s, args[4], "scales", true), second_scale = scales_of(s, args[5], "scales", true);
+    std::vector<void*> master;
+    if (args[6] != Py_None) master = like_params(s, args[6], "masters", at::kFloat, true, true);
+    const Tensor& step = s.on_device(args[7], "step");
+    TORCH_CHECK_VALUE(step.scalar_type() == at::kInt && step.numel() == 1, s.what, ": step must be one int32 value on the device");
+    s.span(step, s.written);
+    s.changed.push_back(step);
+    hb_adamw_rule rule{};
+    if (THPVariable_Check(args[8]) && THPVariable_Unpack(args[8]).is_cuda()) rule.rate = device_number(s, args[8], "lr");
+    else rule.lr = number(args[8]);
+    rule.beta1 = number(args[9]), rule.beta2 = number(args[10]), rule.eps = number(args[11]), rule.decay = number(args[12]);
+    if (args[13] != Py_None) {
+        TORCH_CHECK_VALUE(args[14] != Py_None, s.what, ": max_norm is needed with norm");
+        rule.norm = device_number(s, args[13], "norm");
+        rule.max_norm = number(args[14]);
+    }
+    TORCH_CHECK_VALUE(args[13] != Py_None || args[14] == Py_None, s.what, ": norm is needed with max_norm");
+    check_apart(s);
+    unlocked([&] {
+        const Launch on(s.device);
+        const size_t size = hb_adamw_workspace();
+        Tensor ws = workspace(size, s.device);
+        check(hb_adamw_step(count, param.data(), grad.data(), first.data(), second.data(), bits8 ? first_scale.data() : nullptr,
+                            bits8 ? second_scale.data() : nullptr, master.empty() ? nullptr : reinterpret_cast<float* const*>(master.data()),
+                            s.size.data(), type.data(), grad_type.data(), bits8 ? 8 : 32, &rule, static_cast<int32_t*>(step.data_ptr()),
+                            ws.data_ptr(), size, on.stream));
+        for (const Tensor& t : s.changed) written(t);
+    });
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+// adamw_moments(first, second, first_scale, second_scale) -> ([m], [v])
+PyObject* adamw_moments(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Step s("adamw_moments");
+    expect(n, 4, s.what);
+    untraced(s.what);
+    const Items codes(args[0], "first moments", -1, s.what);
+    const Py_ssize_t count = codes.size();
+    TORCH_CHECK_VALUE(count > 0, s.what, ": no moments");
+    for (Py_ssize_t i = 0; i < count; ++i) {
+        const Tensor& t = s.on_device(codes[i], "first moments");
+        TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat8_e4m3fn && (t.is_contiguous() || t.is_non_overlapping_and_dense()), s.what,
+                          ": 8-bit moments must be e4m3 and dense in memory");
+        s.params.push_back(t);
+        s.size.push_back(t.numel());
+    }
+    const std::vector<void*> first = like_params(s, args[0], "first moments", at::kFloat8_e4m3fn, false, false);
+    const std::vector<void*> second = like_params(s, args[1], "second moments", at::kFloat8_e4m3fn, false, false);
+    const std::vector<float*> first_scale = scales_of(s, args[2], "scales", false), second_scale = scales_of(s, args[3], "scales", false);
+    std::vector<Tensor> out[2];
+    unlocked([&] {
+        std::vector<float*> at[2];
+        for (int k = 0; k < 2; ++k)
+            for (const Tensor& t : s.params) {
+                out[k].push_back(at::empty_strided(t.sizes(), t.strides(), t.options().dtype(at::kFloat)));
+                at[k].push_back(t.numel() ? out[k].back().data_ptr<float>() : nullptr);
+            }
+        const Launch on(s.device);
+        check(hb_adamw_moments(count, const_cast<const void* const*>(first.data()), const_cast<const void* const*>(second.data()),
+                               first_scale.data(), second_scale.data(), s.size.data(), at[0].data(), at[1].data(), on.stream));
+    });
+    THPObjectPtr result(PyTuple_New(2));
+    if (!result) throw python_error();
+    for (int k = 0; k < 2; ++k) {
+        PyObject* list = PyList_New(count);
+        if (!list) throw python_error();
+        PyTuple_SET_ITEM(result.get(), k, list);
+        for (Py_ssize_t i = 0; i < count; ++i) PyList_SET_ITEM(list, i, wrap(out[k][i]));
+    }
+    return result.release();
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"number", reinterpret_cast<PyCFunction>(number_of), METH_FASTCALL, nullptr},
     {"recorded", reinterpret_cast<PyCFunction>(recorded), METH_FASTCALL, nullptr},
@@ -523,6 +1025,15 @@ PyMethodDef methods[] = {
     {"embedding_lookup", reinterpret_cast<PyCFunction>(embedding_lookup), METH_FASTCALL, nullptr},
     {"embedding_grad", reinterpret_cast<PyCFunction>(embedding_grad), METH_FASTCALL, nullptr},
     {"clip", reinterpret_cast<PyCFunction>(clip), METH_FASTCALL, nullptr},
+    {"expert_product", reinterpret_cast<PyCFunction>(expert_product), METH_FASTCALL, nullptr},
+    {"expert_gated", reinterpret_cast<PyCFunction>(expert_gated), METH_FASTCALL, nullptr},
+    {"expert_product_grad", reinterpret_cast<PyCFunction>(expert_product_grad), METH_FASTCALL, nullptr},
+    {"expert_gated_grad", reinterpret_cast<PyCFunction>(expert_gated_grad), METH_FASTCALL, nullptr},
+    {"rms_norm", reinterpret_cast<PyCFunction>(rms_norm), METH_FASTCALL, nullptr},
+    {"rows_of_8bit", reinterpret_cast<PyCFunction>(rows_of_8bit), METH_FASTCALL, nullptr},
+    {"rms_norm_grad", reinterpret_cast<PyCFunction>(rms_norm_grad), METH_FASTCALL, nullptr},
+    {"adamw_step", reinterpret_cast<PyCFunction>(adamw_step), METH_FASTCALL, nullptr},
+    {"adamw_moments", reinterpret_cast<PyCFunction>(adamw_moments), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef definition = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

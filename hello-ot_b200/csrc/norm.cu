@@ -1,0 +1,579 @@
+// Root-mean-square norm of rows with the residual's addition, its 8-bit output, and its gradients.
+//
+//   t = x + residual,  r = 1 / sqrt(mean(t^2) + eps),  y = t r w
+//   dx = r w dy - x r^3 mean(w dy x) + dtotal,  dw = sum over rows of dy x r
+//
+// Bound by HBM: each array passes once.  A row is held in the registers of 32, 128 or 512 threads (2 or 4 vectors
+// of 16 bytes each), so its sum and its scaling need one read; rows wider than 512 threads hold are read a second
+// time, from L2.  The gradient of w is summed over a block's rows in registers, every block leaves one row of fp32
+// partial sums, and a second launch adds those in order: no atomics, the result does not depend on the launch.
+//
+// Sums are fp32; t is rounded for the output alone.  In 8 bits 32 columns share a power of two: the exponent is that
+// of the group's largest magnitude by 448, rounded up, so nothing saturates and the group's largest value keeps
+// 4 significant bits.
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+#include <cuda_fp8.h>
+
+#include "internal.h"
+#include "rows.cuh"
+
+namespace hb {
+namespace norm8 {
+
+constexpr int kGroup = 32;  // columns that share a scale
+
+// ---------------------------------------------------------------- 8 bits
+// Exponent byte of the smallest power of two by which a magnitude (its bits) fits 448 = 0.875 * 2^9.
+__device__ __forceinline__ int scale_byte(uint32_t bits) {
+    if (bits >= 0x7f800000u) return 255;
+    if (bits == 0) return 0;
+    const int e = (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u);  // 1.75 * 2^8 fits 2^0
+    return max(e, 1);  // 2^-126: no subnormal scale
+}
+__device__ __forceinline__ float scale_value(int byte) {
+    return byte == 255 ? __int_as_float(0x7fc00000) : byte == 0 ? 0.0f : __uint_as_float((uint32_t)byte << 23);
+}
+__device__ __forceinline__ uint8_t to_code(float v) { return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3); }
+__device__ __forceinline__ float of_code(uint8_t c) {
+    return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+}
+
+// ---------------------------------------------------------------- forward
+struct Forward {
+    const void *x, *residual, *weight;
+    int64_t x_row, residual_row, rows;
+    int width, weight_type;
+    float eps;
+    void *y, *total;
+    uint8_t *codes, *scales;
+};
+
+// Sum over the THREADS threads of a row (a warp, or a whole block).
+template <int THREADS>
+__device__ __forceinline__ float row_sum(float v, float* shared) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    if (THREADS == 32) return v;
+    __syncthreads();  // the last row's sums have been read
+    if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < THREADS / 32; ++i) s += shared[i];
+    return s;
+}
+
+// A vector of the weight's values; V::N of them from column c.
+template <int N>
+__device__ __forceinline__ void load_weights(float (&w)[N], const void* p, int type, int c) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) w[j] = rows::load_weight(p, type, c + j);
+}
+
+// N values of row r from column c in 8 bits; the lanes of a group hold neighbouring vectors.  Called by whole warps;
+// `there` false: columns behind the row.
+template <int N>
+__device__ __forceinline__ void write_8bit(const Forward& p, int64_t r, int c, const float (&y)[N], bool there) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) most = max(most, there ? __float_as_uint(fabsf(y[j])) : 0u);
+#pragma unroll
+    for (int d = 1; d < kGroup / N; d <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+    if (!there) return;
+    const int byte = scale_byte(most);
+    const float inverse = byte == 0 ? 0.0f : byte == 255 ? __int_as_float(0x7fc00000)
+                          : byte == 254 ? 0x1p-127f : __uint_as_float((uint32_t)(254 - byte) << 23);
+    rows::Vec<uint8_t, N> code;
+#pragma unroll
+    for (int j = 0; j < N; ++j) code.v[j] = to_code(y[j] * inverse);
+    code.store(p.codes + r * p.width + c);
+    if (c % kGroup == 0) p.scales[r * ((p.width + kGroup - 1) / kGroup) + c / kGroup] = (uint8_t)byte;
+}
+
+// HELD vectors a thread; THREADS threads a row, a block of max(128, THREADS).  HELD 0: rows wider than that, a block a row,
+// read twice.
+template <typename T, int VB, int THREADS, int HELD, bool BITS8>
+__global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS) forward_kernel(const __grid_constant__ Forward p) {
+    using V = rows::Vec<T, VB>;
+    constexpr int BLOCK = THREADS < 128 ? 128 : THREADS, ROWS = BLOCK / THREADS;
+    __shared__ float shared[THREADS / 32];
+    const int t = threadIdx.x % THREADS;
+    const int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS;
+    if (r >= p.rows) return;  // whole warps; with more than a warp a row there is one row a block
+    const T* x = static_cast<const T*>(p.x) + r * p.x_row;
+    const T* residual = p.residual ? static_cast<const T*>(p.residual) + r * p.residual_row : nullptr;
+    T* y = static_cast<T*>(p.y) + r * p.width;
+    T* total = p.total ? static_cast<T*>(p.total) + r * p.width : nullptr;
+    auto load = [&](float (&f)[V::N], int c) {
+        V a, b;
+        a.load_once(x + c);
+        if (residual) b.load_once(residual + c);
+#pragma unroll
+        for (int j = 0; j < V::N; ++j) f[j] = residual ? rows::to_float(a.v[j]) + rows::to_float(b.v[j]) : rows::to_float(a.v[j]);
+    };
+    auto keep = [&](const float (&f)[V::N], int c) {
+        V o;
+#pragma unroll
+        for (int j = 0; j < V::N; ++j) o.v[j] = rows::from_float<T>(f[j]);
+        o.store_once(total + c);
+    };
+    auto write = [&](const float (&f)[V::N], int c, float scale, bool there) {
+        float w[V::N], out[V::N];
+        if (there) load_weights(w, p.weight, p.weight_type, c);
+#pragma unroll
+        for (int j = 0; j < V::N; ++j) out[j] = there ? f[j] * scale * w[j] : 0.0f;
+        if constexpr (BITS8) {
+            write_8bit<V::N>(p, r, c, out, there);
+        } else if (there) {
+            V o;
+#pragma unroll
+            for (int j = 0; j < V::N; ++j) o.v[j] = rows::from_float<T>(out[j]);
+            o.store_once(y + c);
+        }
+    };
+    float squares = 0.0f;
+    if constexpr (HELD > 0) {
+        float f[HELD][V::N];
+        V a[HELD], b[HELD];
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {  // all loads first
+            const int c = (i * THREADS + t) * V::N;
+            if (c < p.width) {
+                a[i].load_once(x + c);
+                if (residual) b[i].load_once(residual + c);
+            } else {
+                a[i].zero();
+                b[i].zero();
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const int c = (i * THREADS + t) * V::N;
+#pragma unroll
+            for (int j = 0; j < V::N; ++j) {
+                f[i][j] = residual ? rows::to_float(a[i].v[j]) + rows::to_float(b[i].v[j]) : rows::to_float(a[i].v[j]);
+                squares = fmaf(f[i][j], f[i][j], squares);
+            }
+            if (total && c < p.width) keep(f[i], c);
+        }
+        const float scale = 1.0f / sqrtf(row_sum<THREADS>(squares, shared) / (float)p.width + p.eps);
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const int c = (i * THREADS + t) * V::N;
+            if (i * THREADS * V::N < p.width) write(f[i], c, scale, c < p.width);
+        }
+    } else {
+        float f[V::N];
+        for (int c = t * V::N; c < p.width; c += THREADS * V::N) {
+            load(f, c);
+#pragma unroll
+            for (int j = 0; j < V::N; ++j) squares = fmaf(f[j], f[j], squares);
+        }
+        const float scale = 1.0f / sqrtf(row_sum<THREADS>(squares, shared) / (float)p.width + p.eps);
+        for (int from = 0; from < p.width; from += THREADS * V::N) {
+            const int c = from + t * V::N;
+            if (c < p.width) {
+                load(f, c);
+                if (total) keep(f, c);
+            }
+            write(f, c, scale, c < p.width);
+        }
+    }
+}
+
+template <typename T, int VB, int THREADS, int HELD>
+void launch_forward(const Forward& p, cudaStream_t st) {
+    constexpr int BLOCK = THREADS < 128 ? 128 : THREADS, ROWS = BLOCK / THREADS;
+    const unsigned blocks = (unsigned)((p.rows + ROWS - 1) / ROWS);
+    if (p.codes) forward_kernel<T, VB, THREADS, HELD, true><<<blocks, BLOCK, 0, st>>>(p);
+    else forward_kernel<T, VB, THREADS, HELD, false><<<blocks, BLOCK, 0, st>>>(p);
+}
+
+// ---------------------------------------------------------------- reading 8 bits back
+template <typename TO>
+__global__ void __launch_bounds__(256) read_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                                                   int64_t rows, int width, int vector, TO* __restrict__ out) {
+    const int groups = (width + kGroup - 1) / kGroup;
+    const int64_t n = rows * width;
+    if (vector) {  // 16 codes: half a group
+        for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 16; i < n; i += (int64_t)gridDim.x * 256 * 16) {
+            rows::Vec<uint8_t, 16> c;
+            c.load_once(codes + i);
+            const int64_t r = i / width;
+            const float s = scale_value(scales[r * groups + (int)(i - r * width) / kGroup]);
+            constexpr int V = 16 / (int)sizeof(TO);
+#pragma unroll
+            for (int q = 0; q < 16 / V; ++q) {
+                rows::Vec<TO, 16> o;
+#pragma unroll
+                for (int j = 0; j < V; ++j) o.v[j] = rows::from_float<TO>(of_code(c.v[q * V + j]) * s);
+                o.store(out + i + q * V);
+            }
+        }
+        return;
+    }
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / width;
+        out[i] = rows::from_float<TO>(of_code(codes[i]) * scale_value(scales[r * groups + (int)(i - r * width) / kGroup]));
+    }
+}
+
+// ---------------------------------------------------------------- gradients
+struct Backward {
+    const void *dy, *x, *dtotal, *weight;
+    int64_t dy_row, x_row, dtotal_row, rows;
+    int width, weight_type;
+    float eps;
+    void* dx;
+    float *partial, *stats;  // partial: [blocks][width]; stats: [rows][2] of wide rows
+};
+
+// One of w dy x and x^2 summed, two at once.
+template <int THREADS>
+__device__ __forceinline__ float2 row_sums(float a, float b, float2* shared) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+        a += __shfl_xor_sync(0xffffffffu, a, d);
+        b += __shfl_xor_sync(0xffffffffu, b, d);
+    }
+    if (THREADS == 32) return make_float2(a, b);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = make_float2(a, b);
+    __syncthreads();
+    float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < THREADS / 32; ++i) s.x += shared[i].x, s.y += shared[i].y;
+    return s;
+}
+
+// Rows held in registers; a block strides over the rows and keeps its sums for dw.
+template <typename T, int VB, int THREADS, int HELD>
+__global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS) backward_kernel(const __grid_constant__ Backward p) {
+    using V = rows::Vec<T, VB>;
+    constexpr int BLOCK = THREADS < 128 ? 128 : THREADS, ROWS = BLOCK / THREADS;
+    __shared__ float2 shared[THREADS / 32];
+    __shared__ float joined[ROWS > 1 ? THREADS * HELD * V::N : 1];
+    const int t = threadIdx.x % THREADS, mine = threadIdx.x / THREADS;
+    float dw[HELD][V::N];
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+#pragma unroll
+        for (int j = 0; j < V::N; ++j) dw[i][j] = 0.0f;
+    for (int64_t r = (int64_t)blockIdx.x * ROWS + mine; r < p.rows; r += (int64_t)gridDim.x * ROWS) {
+        const T* x = static_cast<const T*>(p.x) + r * p.x_row;
+        const T* dy = static_cast<const T*>(p.dy) + r * p.dy_row;
+        const T* dtotal = p.dtotal ? static_cast<const T*>(p.dtotal) + r * p.dtotal_row : nullptr;
+        V a[HELD], g[HELD], d[HELD];
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const int c = (i * THREADS + t) * V::N;
+            if (c < p.width) {
+                a[i].load_once(x + c);
+                g[i].load_once(dy + c);
+                if (dtotal && p.dx) d[i].load_once(dtotal + c);
+            } else {
+                a[i].zero();
+                g[i].zero();
+            }
+        }
+        float squares = 0.0f, along = 0.0f;
+        float w[HELD][V::N];
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const int c = (i * THREADS + t) * V::N;
+            if (c < p.width) load_weights(w[i], p.weight, p.weight_type, c);
+#pragma unroll
+            for (int j = 0; j < V::N; ++j) {
+                const float xf = rows::to_float(a[i].v[j]);
+                w[i][j] = c < p.width ? w[i][j] * rows::to_float(g[i].v[j]) : 0.0f;
+                squares = fmaf(xf, xf, squares);
+                along = fmaf(w[i][j], xf, along);
+            }
+        }
+        const float2 sums = row_sums<THREADS>(squares, along, shared);
+        const float inverse = 1.0f / sqrtf(sums.x / (float)p.width + p.eps);
+        const float back = inverse * inverse * inverse * (sums.y / (float)p.width);
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const int c = (i * THREADS + t) * V::N;
+            if (c >= p.width) continue;
+            V o;
+#pragma unroll
+            for (int j = 0; j < V::N; ++j) {
+                const float xf = rows::to_float(a[i].v[j]);
+                dw[i][j] = fmaf(rows::to_float(g[i].v[j]) * xf, inverse, dw[i][j]);
+                float v = fmaf(inverse, w[i][j], -xf * back);
+                if (dtotal && p.dx) v += rows::to_float(d[i].v[j]);
+                o.v[j] = rows::from_float<T>(v);
+            }
+            if (p.dx) o.store_once(static_cast<T*>(p.dx) + r * p.width + c);
+        }
+    }
+    if (!p.partial) return;
+    float* to = p.partial + (int64_t)blockIdx.x * p.width;
+    if constexpr (ROWS > 1) {  // the block's rows side by side, added in order
+        for (int turn = 0; turn < ROWS; ++turn) {
+            __syncthreads();
+            if (mine != turn) continue;
+#pragma unroll
+            for (int i = 0; i < HELD; ++i)
+#pragma unroll
+                for (int j = 0; j < V::N; ++j) {
+                    float& s = joined[(i * THREADS + t) * V::N + j];
+                    s = turn == 0 ? dw[i][j] : s + dw[i][j];
+                }
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < p.width; c += BLOCK) to[c] = joined[c];
+    } else {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const int c = (i * THREADS + t) * V::N;
+#pragma unroll
+            for (int j = 0; j < V::N; ++j)
+                if (c + j < p.width) to[c + j] = dw[i][j];
+        }
+    }
+}
+
+// Wide rows: the two sums of each row first, then columns by blocks of 256 vectors over slabs of rows.
+template <typename T, int VB>
+__global__ void __launch_bounds__(512) wide_sums_kernel(const __grid_constant__ Backward p) {
+    using V = rows::Vec<T, VB>;
+    __shared__ float2 shared[16];
+    const int64_t r = blockIdx.x;
+    const T* x = static_cast<const T*>(p.x) + r * p.x_row;
+    const T* dy = static_cast<const T*>(p.dy) + r * p.dy_row;
+    float squares = 0.0f, along = 0.0f;
+    for (int c = threadIdx.x * V::N; c < p.width; c += 512 * V::N) {
+        V a, g;
+        float w[V::N];
+        a.load(x + c);
+        g.load(dy + c);
+        load_weights(w, p.weight, p.weight_type, c);
+#pragma unroll
+        for (int j = 0; j < V::N; ++j) {
+            const float xf = rows::to_float(a.v[j]);
+            squares = fmaf(xf, xf, squares);
+            along = fmaf(w[j] * rows::to_float(g.v[j]), xf, along);
+        }
+    }
+    const float2 sums = row_sums<512>(squares, along, shared);
+    if (threadIdx.x == 0) {
+        const float inverse = 1.0f / sqrtf(sums.x / (float)p.width + p.eps);
+        p.stats[2 * r] = inverse;
+        p.stats[2 * r + 1] = inverse * inverse * inverse * (sums.y / (float)p.width);
+    }
+}
+template <typename T, int VB>
+__global__ void __launch_bounds__(256) wide_kernel(const __grid_constant__ Backward p) {
+    using V = rows::Vec<T, VB>;
+    const int c = (blockIdx.x * 256 + threadIdx.x) * V::N;
+    if (c >= p.width) return;
+    float w[V::N], dw[V::N];
+    load_weights(w, p.weight, p.weight_type, c);
+#pragma unroll
+    for (int j = 0; j < V::N; ++j) dw[j] = 0.0f;
+    for (int64_t r = blockIdx.y; r < p.rows; r += gridDim.y) {
+        const float inverse = p.stats[2 * r], back = p.stats[2 * r + 1];
+        V a, g, d, o;
+        a.load(static_cast<const T*>(p.x) + r * p.x_row + c);
+        g.load(static_cast<const T*>(p.dy) + r * p.dy_row + c);
+        if (p.dtotal) d.load(static_cast<const T*>(p.dtotal) + r * p.dtotal_row + c);
+#pragma unroll
+        for (int j = 0; j < V::N; ++j) {
+            const float xf = rows::to_float(a.v[j]), gf = rows::to_float(g.v[j]);
+            dw[j] = fmaf(gf * xf, inverse, dw[j]);
+            float v = fmaf(inverse, w[j] * gf, -xf * back);
+            if (p.dtotal) v += rows::to_float(d.v[j]);
+            o.v[j] = rows::from_float<T>(v);
+        }
+        if (p.dx) o.store(static_cast<T*>(p.dx) + r * p.width + c);
+    }
+    if (p.partial)
+#pragma unroll
+        for (int j = 0; j < V::N; ++j) p.partial[(int64_t)blockIdx.y * p.width + c + j] = dw[j];
+}
+
+// dw: the blocks' sums added, 8 chains a column in a fixed order.
+__global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ partial, int parts, int width, void* dw, int type) {
+    __shared__ float shared[8][33];
+    const int c = blockIdx.x * 32 + (threadIdx.x & 31), chain = threadIdx.x >> 5;
+    float s = 0.0f;
+    if (c < width)
+#pragma unroll 4
+        for (int i = chain; i < parts; i += 8) s += partial[(int64_t)i * width + c];
+    shared[chain][threadIdx.x & 31] = s;
+    __syncthreads();
+    if (chain == 0 && c < width) {
+#pragma unroll
+        for (int i = 1; i < 8; ++i) s += shared[i][threadIdx.x];
+        rows::store_weight(dw, type, c, s);
+    }
+}
+
+// Threads and vectors a row: the smallest form that holds it.  A warp holds 2 vectors a lane, so that short rows go four
+// to a block; above, 2 and then 4 a thread.
+template <typename F>
+void for_width(int64_t vectors, F&& f) {
+    if (vectors <= 64) f(rows::Bytes<32>{}, rows::Bytes<2>{});
+    else if (vectors <= 256) f(rows::Bytes<128>{}, rows::Bytes<2>{});
+    else if (vectors <= 512) f(rows::Bytes<128>{}, rows::Bytes<4>{});
+    else if (vectors <= 2048) f(rows::Bytes<512>{}, rows::Bytes<4>{});
+    else f(rows::Bytes<512>{}, rows::Bytes<0>{});
+}
+constexpr int64_t kMostHeld = 2048;  // vectors of a row that for_width holds
+constexpr int kParts = 148 * 8;      // most blocks that sum dw
+
+inline int parts_of(int64_t rows, int64_t vectors) {
+    // resident blocks: 8 of 128 threads an SM, 2 of 512; the rows of a block are at least 4
+    const int64_t blocks = vectors <= 512 ? 148 * 8 : 148 * 2, side = vectors <= 64 ? 4 : 1;
+    return (int)std::max<int64_t>(1, std::min(blocks, (rows + 4 * side - 1) / (4 * side)));
+}
+
+inline bool bad_rows(const void* p, int64_t stride, int type) {
+    return !p || rows::address_bits(p) % rows::type_bytes(type) || stride < 0;
+}
+// Vector bytes of all rows together: 16, 4 or an element.
+inline int vector_of(uint64_t bits, int type) {
+    return bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : rows::type_bytes(type);
+}
+template <typename F>
+void for_vectors(int type, int vb, F&& f) {
+    if (type == HB_F32) {
+        if (vb == 16) f(float{}, rows::Bytes<16>{});
+        else f(float{}, rows::Bytes<4>{});
+    } else if (type == HB_F16) {
+        if (vb == 16) f(__half{}, rows::Bytes<16>{});
+        else if (vb == 4) f(__half{}, rows::Bytes<4>{});
+        else f(__half{}, rows::Bytes<2>{});
+    } else {
+        if (vb == 16) f(__nv_bfloat16{}, rows::Bytes<16>{});
+        else if (vb == 4) f(__nv_bfloat16{}, rows::Bytes<4>{});
+        else f(__nv_bfloat16{}, rows::Bytes<2>{});
+    }
+}
+int finish(cudaError_t e, const char* what) {
+    return e == cudaSuccess ? HB_OK : abi_fail(HB_LAUNCH, std::string(what) + ": " + cudaGetErrorString(e));
+}
+
+}  // namespace norm8
+}  // namespace hb
+
+using namespace hb;
+using namespace hb::norm8;
+
+extern "C" int hb_rms_norm(int type, const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, int64_t rows,
+                           int64_t width, const void* weight, int weight_type, double eps, void* y, void* codes, void* scales,
+                           void* total, void* stream) {
+    if (!rows::valid_type(type) || !rows::valid_type(weight_type)) return abi_fail(HB_BAD_ARGUMENT, "hb_rms_norm: element type");
+    if (rows < 0 || rows > INT32_MAX || width < 1 || width > (1 << 30)) return abi_fail(HB_BAD_ARGUMENT, "hb_rms_norm: rows or width out of range");
+    if (!(eps >= 0.0)) return abi_fail(HB_BAD_ARGUMENT, "hb_rms_norm: eps must be a number >= 0");
+    if (rows == 0) return HB_OK;
+    const int size = rows::type_bytes(type);
+    if (bad_rows(x, x_stride, type) || (residual && bad_rows(residual, residual_stride, type)) || !weight ||
+        rows::address_bits(weight) % rows::type_bytes(weight_type) || (codes ? !scales || y : !y) || rows::address_bits(y) % size ||
+        rows::address_bits(total) % size)
+        return abi_fail(HB_BAD_ARGUMENT, "hb_rms_norm: null or misaligned pointer, or bad stride");
+    Forward p{x, residual, weight, x_stride, residual_stride, rows, (int)width, weight_type, (float)eps, y, total,
+              static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales)};
+    uint64_t bits = rows::address_bits(x) | rows::address_bits(residual) | rows::address_bits(y) | rows::address_bits(total) |
+                    (uint64_t)(width | (rows > 1 ? x_stride : 0) | (rows > 1 && residual ? residual_stride : 0)) * size;
+    if (codes) bits |= rows::address_bits(codes) % (16 / size) ? 1 : 0;  // a vector's codes lie on their own size
+    const auto st = static_cast<cudaStream_t>(stream);
+    for_vectors(type, vector_of(bits, type), [&](auto t, auto vb) {
+        using T = decltype(t);
+        constexpr int VB = decltype(vb)::value, N = VB / (int)sizeof(T);
+        for_width((width + N - 1) / N, [&](auto threads, auto held) {
+            launch_forward<T, VB, decltype(threads)::value, decltype(held)::value>(p, st);
+        });
+    });
+    count_launches(1);
+    return finish(cudaGetLastError(), "hb_rms_norm");
+}
+
+extern "C" int hb_rows_of_8bit(const void* codes, const void* scales, int64_t rows, int64_t width, int out_type, void* out, void* stream) {
+    if (!rows::valid_type(out_type)) return abi_fail(HB_BAD_ARGUMENT, "hb_rows_of_8bit: element type");
+    if (rows < 0 || rows > INT32_MAX || width < 1 || width > (1 << 30))
+        return abi_fail(HB_BAD_ARGUMENT, "hb_rows_of_8bit: rows or width out of range");
+    if (rows == 0) return HB_OK;
+    if (!codes || !scales || !out || rows::address_bits(out) % rows::type_bytes(out_type))
+        return abi_fail(HB_BAD_ARGUMENT, "hb_rows_of_8bit: null or misaligned pointer");
+    const bool vector = width % 16 == 0 && ((rows::address_bits(codes) | rows::address_bits(out)) & 15) == 0;
+    const int64_t items = (rows * width + (vector ? 16 : 1) - 1) / (vector ? 16 : 1);
+    const unsigned blocks = (unsigned)std::min<int64_t>((items + 255) / 256, 148 * 16);
+    const auto st = static_cast<cudaStream_t>(stream);
+    const auto *c = static_cast<const uint8_t*>(codes), *s = static_cast<const uint8_t*>(scales);
+    rows::for_type(out_type, 16, [&](auto t, auto) {
+        using T = decltype(t);
+        read_kernel<T><<<blocks, 256, 0, st>>>(c, s, rows, (int)width, vector, static_cast<T*>(out));
+    });
+    count_launches(1);
+    return finish(cudaGetLastError(), "hb_rows_of_8bit");
+}
+
+extern "C" size_t hb_rms_norm_grad_workspace(int64_t rows, int64_t width) {
+    if (rows < 0 || rows > INT32_MAX || width < 1 || width > (1 << 30)) return 0;
+    // the blocks of any vector size, and two sums a row of those that none holds
+    const size_t sums = width > kMostHeld ? (size_t)rows * 2 * sizeof(float) : 0;
+    return (sums + 255) / 256 * 256 + (size_t)std::min<int64_t>(kParts, std::max<int64_t>(rows, 1)) * width * sizeof(float);
+}
+
+extern "C" int hb_rms_norm_grad(int type, const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* dtotal,
+                                int64_t dtotal_stride, int64_t rows, int64_t width, const void* weight, int weight_type, double eps,
+                                void* dx, void* dweight, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* what = "hb_rms_norm_grad";
+    if (!rows::valid_type(type) || !rows::valid_type(weight_type)) return abi_fail(HB_BAD_ARGUMENT, "hb_rms_norm_grad: element type");
+    if (rows < 0 || rows > INT32_MAX || width < 1 || width > (1 << 30))
+        return abi_fail(HB_BAD_ARGUMENT, "hb_rms_norm_grad: rows or width out of range");
+    if (!(eps >= 0.0)) return abi_fail(HB_BAD_ARGUMENT, "hb_rms_norm_grad: eps must be a number >= 0");
+    const int size = rows::type_bytes(type);
+    if (!weight || rows::address_bits(weight) % rows::type_bytes(weight_type) || rows::address_bits(dweight) % rows::type_bytes(weight_type) ||
+        rows::address_bits(dx) % size ||
+        (rows > 0 && (bad_rows(dy, dy_stride, type) || bad_rows(x, x_stride, type) || (dtotal && bad_rows(dtotal, dtotal_stride, type)))))
+        return abi_fail(HB_BAD_ARGUMENT, "hb_rms_norm_grad: null or misaligned pointer, or bad stride");
+    const auto st = static_cast<cudaStream_t>(stream);
+    if (rows == 0)
+        return dweight ? finish(cudaMemsetAsync(dweight, 0, (size_t)width * rows::type_bytes(weight_type), st), what) : HB_OK;
+    if (!dx && !dweight) return HB_OK;
+    if (!workspace || rows::address_bits(workspace) % 256)
+        return abi_fail(HB_BAD_ARGUMENT, "hb_rms_norm_grad: the workspace must be 256-byte aligned");
+    if (workspace_bytes < hb_rms_norm_grad_workspace(rows, width))
+        return abi_fail(HB_WORKSPACE, "workspace smaller than hb_rms_norm_grad_workspace()");
+    const size_t sums = width > kMostHeld ? ((size_t)rows * 2 * sizeof(float) + 255) / 256 * 256 : 0;
+    float* const stats = static_cast<float*>(workspace);
+    float* const partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + sums);
+    Backward p{dy, x, dtotal, weight, dy_stride, x_stride, dtotal_stride, rows, (int)width, weight_type, (float)eps, dx,
+               dweight ? partial : nullptr, stats};
+    uint64_t bits = rows::address_bits(dy) | rows::address_bits(x) | rows::address_bits(dtotal) | rows::address_bits(dx) |
+                    (uint64_t)(width | (rows > 1 ? x_stride | dy_stride : 0) | (rows > 1 && dtotal ? dtotal_stride : 0)) * size;
+    int parts = 0;
+    for_vectors(type, vector_of(bits, type), [&](auto t, auto vb) {
+        using T = decltype(t);
+        constexpr int VB = decltype(vb)::value, N = VB / (int)sizeof(T);
+        const int64_t vectors = (width + N - 1) / N;
+        if (vectors <= kMostHeld) {
+            parts = parts_of(rows, vectors);
+            for_width(vectors, [&](auto threads, auto held) {
+                constexpr int THREADS = decltype(threads)::value, HELD = decltype(held)::value;
+                if constexpr (HELD > 0)
+                    backward_kernel<T, VB, THREADS, HELD><<<parts, THREADS < 128 ? 128 : THREADS, 0, st>>>(p);
+            });
+            count_launches(1);
+            return;
+        }
+        wide_sums_kernel<T, VB><<<(unsigned)rows, 512, 0, st>>>(p);
+        const unsigned columns = (unsigned)((vectors + 255) / 256);
+        parts = (int)std::min<int64_t>(rows, std::max<int64_t>(1, 148 * 8 / columns));
+        wide_kernel<T, VB><<<dim3(columns, parts), 256, 0, st>>>(p);
+        count_launches(2);
+    });
+    if (dweight) {
+        join_kernel<<<(unsigned)((width + 31) / 32), 256, 0, st>>>(partial, parts, (int)width, dweight, weight_type);
+        count_launches(1);
+    }
+    return finish(cudaGetLastError(), what);
+}

@@ -27,6 +27,7 @@ template <> struct Bits<16> { using type = uint4; };
 template <> struct Bits<8> { using type = uint2; };
 template <> struct Bits<4> { using type = uint32_t; };
 template <> struct Bits<2> { using type = uint16_t; };
+template <> struct Bits<1> { using type = uint8_t; };  // 8-bit codes alone
 
 // BYTES of T at an address aligned to BYTES.
 template <typename T, int BYTES>

@@ -424,6 +424,78 @@ int hb_clip_grad_norm(int64_t count, const void* const* grads, const int64_t* si
                       void* const* outs, const int32_t* out_types, double limit, float* norm, void* workspace,
                       size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * The experts of a routed layer: products of rows sorted by expert (hb_index_sort,
+ * hb_route_dispatch) with each expert's weight, hidden x width.
+ *   product  out[r] = x[r] W[e]^T                        gated  out[r] = act(x[r] Wg[e]^T) * (x[r] Wu[e]^T)
+ *   gradients  dx[r] = dy[r] W[e], dW[e] = sum of dy[r]^T x[r] over the expert's rows; of the gated form with
+ *   g = x Wg^T and u = x Wu^T computed again: dg = dh u act'(g) and du = dh act(g) (rounded to the element type),
+ *   dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x.
+ * offsets (device, experts + 1): expert e's rows are offsets[e]..offsets[e+1]-1, from 0 on; it is read as its
+ * running maximum within 0..rows.  Rows behind the last expert's give zero rows and are not read; null: one expert
+ * has all rows.  Sums are fp32, results rounded once.  Outputs are dense; null gradients are not computed.  Above
+ * HB_EXPERT_FEW_ROWS rows, and for gradients, 16-bit operands lie on 16 bytes, their rows (distances, in elements, at
+ * least the row's length) and experts too, but for dh.  Experts: at most 2048.  Nothing waits and nothing is kept. */
+#define HB_EXPERT_FEW_ROWS 16
+enum { HB_SILU = 0, HB_GELU = 1 }; /* g / (1 + exp(-g)); g (1 + erf(g / sqrt 2)) / 2 */
+typedef struct hb_expert_shape {
+    int64_t rows, width, hidden, experts; /* sorted rows; weights [experts][hidden][width] */
+    int32_t type, activation;
+} hb_expert_shape;
+typedef struct hb_expert_weight {
+    const void* data;
+    int64_t row_stride, expert_stride; /* elements */
+} hb_expert_weight;
+int hb_expert_product(const hb_expert_shape* shape, const void* x, int64_t x_stride, const int32_t* offsets,
+                      const hb_expert_weight* weight, void* out, void* stream);
+int hb_expert_gated(const hb_expert_shape* shape, const void* x, int64_t x_stride, const int32_t* offsets,
+                    const hb_expert_weight* gate, const hb_expert_weight* up, void* out, void* stream);
+size_t hb_expert_product_grad_workspace(const hb_expert_shape* shape);
+int hb_expert_product_grad(const hb_expert_shape* shape, const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
+                           const int32_t* offsets, const hb_expert_weight* weight, void* dx, void* dweight, void* workspace,
+                           size_t workspace_bytes, void* stream);
+size_t hb_expert_gated_grad_workspace(const hb_expert_shape* shape);
+int hb_expert_gated_grad(const hb_expert_shape* shape, const void* dh, int64_t dh_stride, const void* x, int64_t x_stride,
+                         const int32_t* offsets, const hb_expert_weight* gate, const hb_expert_weight* up, void* dx,
+                         void* dgate, void* dup, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Root-mean-square norm of rows: t = x + residual (null: x), y = t w / sqrt(mean(t^2) + eps), t in fp32; `total`
+ * receives t, rounded.  weight: width values of weight_type.  codes != null: y in 8 bits instead: e4m3 codes
+ * (rows x width) and, for each 32 columns of a row, the exponent byte E of a scale 2^(E-127) (rows x ceil(width / 32)),
+ * the smallest by which the group's largest magnitude fits 448 (0 in a group of zeros; 255, NaN, where a value is not
+ * finite).  rows_of_8bit reads such rows back.  The gradient: with r = 1 / sqrt(mean(x^2) + eps),
+ * dx = r w dy - x r^3 mean(w dy x) + dtotal (null: none), dweight = sum over the rows of dy x r; either may be null. */
+int hb_rms_norm(int type, const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, int64_t rows,
+                int64_t width, const void* weight, int weight_type, double eps, void* y, void* codes, void* scales,
+                void* total, void* stream);
+int hb_rows_of_8bit(const void* codes, const void* scales, int64_t rows, int64_t width, int out_type, void* out, void* stream);
+size_t hb_rms_norm_grad_workspace(int64_t rows, int64_t width);
+int hb_rms_norm_grad(int type, const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* dtotal,
+                     int64_t dtotal_stride, int64_t rows, int64_t width, const void* weight, int weight_type, double eps,
+                     void* dx, void* dweight, void* workspace, size_t workspace_bytes, void* stream);
+
+/* One AdamW step over `count` tensors (host arrays of device pointers, element counts and types):
+ *   g' = f g, f = min(1, max_norm / (norm + 1e-6)) (norm, device, null: f = 1);  m = b1 m + (1 - b1) g';
+ *   v = b2 v + (1 - b2) g'^2;  p = p (1 - lr decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * with every operation rounded to fp32, t = ++*step (device), and lr read from the device where rate is not null.
+ * master (null: none) holds fp32 parameters, of which params receive the rounded values.  grads are of their
+ * parameter's type or fp32.  bits 32: first and second hold m and v in fp32; bits 8: e4m3 codes of m and of sqrt(v),
+ * each 256 elements with a scale of their own (first_scale, second_scale: fp32, largest magnitude / 448); a v above 0
+ * keeps at least the smallest code.  adamw_moments reads m and v of 8-bit states.  Tensors must not overlap. */
+typedef struct hb_adamw_rule {
+    double lr, beta1, beta2, eps, decay, max_norm;
+    const float* rate; /* device, or null */
+    const float* norm; /* device, or null */
+} hb_adamw_rule;
+size_t hb_adamw_workspace(void);
+int hb_adamw_step(int64_t count, void* const* params, const void* const* grads, void* const* first, void* const* second,
+                  float* const* first_scale, float* const* second_scale, float* const* master, const int64_t* sizes,
+                  const int32_t* types, const int32_t* grad_types, int bits, const hb_adamw_rule* rule, int32_t* step,
+                  void* workspace, size_t workspace_bytes, void* stream);
+int hb_adamw_moments(int64_t count, const void* const* first, const void* const* second, const float* const* first_scale,
+                     const float* const* second_scale, const int64_t* sizes, float* const* out_first,
+                     float* const* out_second, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
