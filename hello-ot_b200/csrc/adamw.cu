@@ -14,8 +14,10 @@
 // Scales are fp32, not powers of two: a block whose values all shrink by the same factor keeps its codes and
 // shrinks its scale, where rounding each value to its old code would stop v's decay of 0.1 % a step.
 //
-// Every operation is rounded to fp32 as it is written (no contraction), so that a step's codes can be
-// computed again bit for bit by any fp32 program.
+// m and v are rounded to fp32 at every operation as it is written, and their codes are those of the correctly rounded
+// quotients, so that any fp32 program computes the same states bit for bit.  The change of p takes the approximate
+// root and quotient (2^-20 of the change): with the exact ones, 3 quotients and a root an element, the kernel was bound
+// by instructions (400 million bf16 parameters, 8 bits: 2.46 ms of 0.86 at the copy rate).
 #include <algorithm>
 #include <cmath>
 #include <string>
@@ -49,7 +51,7 @@ struct NoScales {};
 static_assert(sizeof(List<kMost8>) + sizeof(Scales) < 32000 && sizeof(List<kMost32>) < 32000, "kernel parameters");
 
 struct Shared {  // what all elements share, in device memory
-    float factor, keep, rate, root;
+    float factor, keep, rate, over_root;  // over_root: 1 / sqrt(1 - b2^t)
 };
 struct Fixed {
     float beta1, beta2, less1, less2, eps;
@@ -69,7 +71,7 @@ __global__ void begin_kernel(int* step, const float* norm, const float* rate, do
     shared->factor = (float)f;
     shared->keep = (float)(1.0 - lr * decay);
     shared->rate = (float)(lr / (1.0 - pow(beta1, (double)t)));
-    shared->root = (float)sqrt(1.0 - pow(beta2, (double)t));
+    shared->over_root = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)t)));
 }
 
 template <int MOST>
@@ -128,23 +130,47 @@ __device__ __forceinline__ void read_codes(uint8_t (&c)[8], const uint8_t* p, in
         for (int j = 0; j < 8; ++j) c[j] = j < left ? p[j] : 0;
     }
 }
-__device__ __forceinline__ float of_code(uint8_t c) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3))); }
+__device__ __forceinline__ void of_codes(float (&f)[8], const uint8_t (&c)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c[j] | c[j + 1] << 8), __NV_E4M3);
+        const float2 v = __half22float2(__half2(h));
+        f[j] = v.x, f[j + 1] = v.y;
+    }
+}
+// a / b within 2^-21, for any b >= 0 of the range: __fdividef's divisors end at 2^126.
+__device__ __forceinline__ float quotient(float a, float b) { return b < 0x1p126f ? __fdividef(a, b) : a / b; }
+__device__ __forceinline__ float root_near(float v) {  // within 2^-23 of the root
+    float r;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
 
-// The block's values in 8 bits: the warp's largest magnitude by 448 is the scale (a NaN makes it one).  FLOOR: values
-// above zero keep at least the smallest code.
-template <bool FLOOR>
-__device__ __forceinline__ void hold(const float (&f)[8], uint8_t* codes, float* scale, int left, bool vectors) {
+// The block's values (ROOT: their roots, which are >= 0) in 8 bits: the warp's largest magnitude by 448 is the scale (a NaN
+// makes it one), the codes are those of the correctly rounded root and quotient.  Both are approximated first, to
+// within 2^-22 with the scale's inverse: where the codes a little below and above are the same, that is the code, and
+// only next to a border between two codes (one value in some 10^5) the exact operations are run.  ROOT: values above
+// zero keep at least the smallest code.
+template <bool ROOT>
+__device__ __forceinline__ void hold(const float (&f)[8], const float (&near)[8], uint8_t* codes, float* scale, int left, bool vectors) {
     uint32_t most = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) most = max(most, j < left ? __float_as_uint(fabsf(f[j])) : 0u);
     most = __reduce_max_sync(0xffffffffu, most);
-    const float s = __fdiv_rn(__uint_as_float(most), 448.0f);
-    const float by = s > 0.0f ? s : 1.0f;
+    const float largest = ROOT ? __fsqrt_rn(__uint_as_float(most)) : __uint_as_float(most);
+    const float s = __fdiv_rn(largest, 448.0f);
+    const float by = s > 0.0f ? s : 1.0f, inverse = __fdiv_rn(1.0f, by);
+    const bool plain = by >= 0x1p-100f && by <= 0x1p100f;  // nothing below leaves the normal numbers
     rows::Vec<uint8_t, 8> v;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        v.v[j] = __nv_cvt_float_to_fp8(__fdiv_rn(f[j], by), __NV_SATFINITE, __NV_E4M3);
-        if (FLOOR && f[j] > 0.0f && v.v[j] == 0) v.v[j] = 1;
+        const float q = near[j] * inverse;
+        const uint32_t both = __nv_cvt_float2_to_fp8x2(make_float2(fmaf(q, -0x1p-21f, q), fmaf(q, 0x1p-21f, q)), __NV_SATFINITE, __NV_E4M3);
+        uint32_t code = both & 0xff;
+        if (code != both >> 8 || !plain)
+            code = __nv_cvt_float_to_fp8(__fdiv_rn(ROOT ? __fsqrt_rn(f[j]) : f[j], by), __NV_SATFINITE, __NV_E4M3);
+        if (ROOT && code == 0 && f[j] > 0.0f) code = 1;
+        v.v[j] = (uint8_t)code;
     }
     if (vectors) {
         v.store_once(codes);
@@ -185,21 +211,25 @@ __device__ __forceinline__ void step_block(const List<MOST>& l, const S& scales,
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const volatile Shared* now = shared;
-    const float factor = now->factor, keep = now->keep, rate = now->rate, root_of_bias = now->root;
+    const float factor = now->factor, keep = now->keep, rate = now->rate, over_root = now->over_root;
+    if constexpr (BITS == 8) {
+        of_codes(m, mc);
+        of_codes(v, vc);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            m[j] = __fmul_rn(m[j], ms);
+            v[j] = __fmul_rn(v[j], vs);
+            v[j] = __fmul_rn(v[j], v[j]);
+        }
+    }
+    float root[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        if constexpr (BITS == 8) {
-            m[j] = __fmul_rn(of_code(mc[j]), ms);
-            const float root = __fmul_rn(of_code(vc[j]), vs);
-            v[j] = __fmul_rn(root, root);
-        }
         const float gj = __fmul_rn(g[j], factor);
         m[j] = __fadd_rn(__fmul_rn(m[j], fixed.beta1), __fmul_rn(gj, fixed.less1));
         v[j] = __fadd_rn(__fmul_rn(v[j], fixed.beta2), __fmul_rn(__fmul_rn(gj, gj), fixed.less2));
-        const float root = __fsqrt_rn(v[j]);
-        const float by = __fadd_rn(__fdiv_rn(root, root_of_bias), fixed.eps);
-        p[j] = __fsub_rn(__fmul_rn(p[j], keep), __fmul_rn(__fdiv_rn(m[j], by), rate));
-        if (BITS == 8) v[j] = root;
+        root[j] = root_near(v[j]);
+        p[j] = fmaf(-rate, quotient(m[j], fmaf(root[j], over_root, fixed.eps)), __fmul_rn(p[j], keep));
     }
     if (master) write8(p, master + i, left, vectors);
     write8(p, param + i, left, vectors);
@@ -207,8 +237,8 @@ __device__ __forceinline__ void step_block(const List<MOST>& l, const S& scales,
         write8(m, static_cast<float*>(l.first[t]) + i, left, vectors);
         write8(v, static_cast<float*>(l.second[t]) + i, left, vectors);
     } else {
-        hold<false>(m, static_cast<uint8_t*>(l.first[t]) + i, scales.first[t] + at / kBlock, left, vectors);
-        hold<true>(v, static_cast<uint8_t*>(l.second[t]) + i, scales.second[t] + at / kBlock, left, vectors);
+        hold<false>(m, m, static_cast<uint8_t*>(l.first[t]) + i, scales.first[t] + at / kBlock, left, vectors);
+        hold<true>(v, root, static_cast<uint8_t*>(l.second[t]) + i, scales.second[t] + at / kBlock, left, vectors);
     }
 }
 
@@ -259,11 +289,13 @@ __global__ void __launch_bounds__(kThreads) moments_kernel(const __grid_constant
     read_codes(mc, l.first[lo] + i, left, vectors);
     read_codes(vc, l.second[lo] + i, left, vectors);
     const float ms = l.first_scale[lo][at / kBlock], vs = l.second_scale[lo][at / kBlock];
+    of_codes(m, mc);
+    of_codes(v, vc);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        m[j] = __fmul_rn(of_code(mc[j]), ms);
-        const float root = __fmul_rn(of_code(vc[j]), vs);
-        v[j] = __fmul_rn(root, root);
+        m[j] = __fmul_rn(m[j], ms);
+        v[j] = __fmul_rn(v[j], vs);
+        v[j] = __fmul_rn(v[j], v[j]);
     }
     write8(m, l.out_first[lo] + i, left, vectors);
     write8(v, l.out_second[lo] + i, left, vectors);

@@ -40,6 +40,7 @@ struct Params {
     int groups, rows, n, k, segments, activation;
     int col_tiles, row_tiles;  // row_tiles: kWeights alone
     int splits;                // kWeights
+    int blocked[2];            // operands read across the summed length whose columns are whole boxes of 64: a, b
     float* partial;
     const void* dh;
     int64_t dh_row;
@@ -77,6 +78,16 @@ __device__ __forceinline__ void load_3d_pair(void* dst, const CUtensorMap* map, 
 // (the products of 256-row tiles ran at 700 TFLOP/s with it).
 __device__ __forceinline__ void arrive_expect_cluster(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2, int c3) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+        ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
+}
+__device__ __forceinline__ void load_4d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+        ::"r"(smem_u32(dst)), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
 }
 // A bounded wait on a barrier that the other CTA arrives on as well.
 template <bool PAIR>
@@ -181,6 +192,38 @@ __device__ __forceinline__ Tile tile_at(const Params& p, const Smem& s, int u, i
 }
 
 // ---------------------------------------------------------------- roles
+// 128 columns x 64 rows of the summed length, two boxes of 64 columns.  Blocked: the tensor's 64-column blocks are a
+// dimension of their own and one copy brings both boxes (two copies a stage and operand cost up to a tenth of the rate:
+// 16384 x 8192 x 8192 in dW 1288 -> 1424 TFLOP/s).  `bar` this CTA's barrier, or `full` the pair's.
+template <bool PAIR>
+__device__ __forceinline__ void columns_2d(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, uint32_t full, int col, int row,
+                                           int blocked) {
+    if (blocked) {
+        if (PAIR) load_3d_pair(dst, map, full, 0, row, col >> 6);
+        else load_3d(dst, map, bar, 0, row, col >> 6);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if (PAIR) tma_load_2d_pair(dst + i * BK * 128, map, full, col + i * 64, row);
+        else load_2d(dst + i * BK * 128, map, bar, col + i * 64, row);
+    }
+}
+template <bool PAIR>
+__device__ __forceinline__ void columns_3d(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, uint32_t full, int col, int row,
+                                           int group, int blocked) {
+    if (blocked) {
+        if (PAIR) load_4d_pair(dst, map, full, 0, row, col >> 6, group);
+        else load_4d(dst, map, bar, 0, row, col >> 6, group);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if (PAIR) load_3d_pair(dst + i * BK * 128, map, full, col + i * 64, row, group);
+        else load_3d(dst + i * BK * 128, map, bar, col + i * 64, row, group);
+    }
+}
+
 // Lane 0 waits for its warp, which goes on or gives up as one.
 template <bool PAIR>
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, Smem& s) {
@@ -210,30 +253,16 @@ __device__ __forceinline__ void produce(const Params& p, Smem& s, int rank) {
                 const CUtensorMap* am = &p.a[t.part];
                 if (left >= BK) {
                     if (lane == 0) {
-                        if (PAIR) {
-                            arrive_expect_cluster(full, kStageBytes);
-#pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                tma_load_2d_pair(a + i * BK * 128, am, full, t.row + i * 64, row);
-                                tma_load_2d_pair(b + i * BK * 128, &p.b[0], full, bcol + i * 64, row);
-                            }
-                        } else {
-                            mbar_arrive_expect_tx(&s.full[stage], kStageBytes);
-#pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                load_2d(a + i * BK * 128, am, &s.full[stage], t.row + i * 64, row);
-                                load_2d(b + i * BK * 128, &p.b[0], &s.full[stage], bcol + i * 64, row);
-                            }
-                        }
+                        if (PAIR) arrive_expect_cluster(full, kStageBytes);
+                        else mbar_arrive_expect_tx(&s.full[stage], kStageBytes);
+                        columns_2d<PAIR>(a, am, &s.full[stage], full, t.row, row, p.blocked[0]);
+                        columns_2d<PAIR>(b, &p.b[0], &s.full[stage], full, bcol, row, p.blocked[1]);
                     }
                 } else {  // rows of the next expert are in the box: zero them once it is there
                     if (lane == 0) {
                         mbar_arrive_expect_tx(&s.tail, kStageBytes);
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            load_2d(a + i * BK * 128, am, &s.tail, t.row + i * 64, row);
-                            load_2d(b + i * BK * 128, &p.b[0], &s.tail, bcol + i * 64, row);
-                        }
+                        columns_2d<false>(a, am, &s.tail, 0, t.row, row, p.blocked[0]);
+                        columns_2d<false>(b, &p.b[0], &s.tail, 0, bcol, row, p.blocked[1]);
                     }
                     if (!warp_wait<false>(&s.tail, tails & 1, s)) return;
                     ++tails;
@@ -256,9 +285,7 @@ __device__ __forceinline__ void produce(const Params& p, Smem& s, int rank) {
                     arrive_expect_cluster(full, kStageBytes);
                     tma_load_2d_pair(a, &p.a[seg], full, k0, t.row);
                     if (FORM == kBack) {
-#pragma unroll
-                        for (int i = 0; i < 2; ++i)
-                            load_3d_pair(b + i * BK * 128, &p.b[seg], full, t.col + rank * 128 + i * 64, k0, t.group);
+                        columns_3d<true>(b, &p.b[seg], nullptr, full, t.col + rank * 128, k0, t.group, p.blocked[1]);
                     } else if (S::kHalves) {
                         load_3d_pair(b, &p.b[rank], full, k0, t.col, t.group);
                     } else {
@@ -269,8 +296,7 @@ __device__ __forceinline__ void produce(const Params& p, Smem& s, int rank) {
                     mbar_arrive_expect_tx(bar, kStageBytes);
                     load_2d(a, &p.a[seg], bar, k0, t.row);
                     if (FORM == kBack) {
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) load_3d(b + i * BK * 128, &p.b[seg], bar, t.col + i * 64, k0, t.group);
+                        columns_3d<false>(b, &p.b[seg], bar, 0, t.col, k0, t.group, p.blocked[1]);
                     } else if (S::kHalves) {
 #pragma unroll
                         for (int i = 0; i < 2; ++i) load_3d(b + i * 64 * 128, &p.b[i], bar, k0, t.col, t.group);
@@ -533,16 +559,22 @@ EncodeTiled find_encode() {
 }
 
 // Map of [groups][rows][cols] (groups 0: two dimensions) in boxes of 64 columns (128 bytes) x box_rows, 128-byte swizzle;
-// what lies outside is read as zeros.
-bool encode(CUtensorMap* m, const Operand& o, int type, int64_t cols, int64_t rows, int64_t groups, int box_rows) {
+// what lies outside is read as zeros.  Blocked (whole boxes of columns): two boxes side by side in one copy.
+bool encode(CUtensorMap* m, const Operand& o, int type, int64_t cols, int64_t rows, int64_t groups, int box_rows, bool blocked) {
     static const EncodeTiled enc = find_encode();
     if (!enc) return false;
-    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)std::max<int64_t>(groups, 1)};
-    const cuuint64_t strides[2] = {(cuuint64_t)o.row * 2, (cuuint64_t)o.group * 2};
-    const cuuint32_t box[3] = {BK, (cuuint32_t)box_rows, 1}, step[3] = {1, 1, 1};
-    return enc(m, type == HB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, groups ? 3 : 2,
-               const_cast<void*>(o.p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const cuuint64_t most = (cuuint64_t)std::max<int64_t>(groups, 1), row = (cuuint64_t)o.row * 2, group = (cuuint64_t)o.group * 2;
+    cuuint64_t dims[4] = {(cuuint64_t)cols, (cuuint64_t)rows, most, 1}, strides[3] = {row, group, 0};
+    cuuint32_t box[4] = {BK, (cuuint32_t)box_rows, 1, 1};
+    const cuuint32_t step[4] = {1, 1, 1, 1};
+    if (blocked) {
+        dims[0] = BK, dims[2] = (cuuint64_t)cols / BK, dims[3] = most;
+        strides[1] = BK * 2, strides[2] = group;
+        box[2] = 2;
+    }
+    return enc(m, type == HB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+               (groups ? 3 : 2) + (blocked ? 1 : 0), const_cast<void*>(o.p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int FORM, bool PAIR, typename T>
@@ -593,16 +625,18 @@ int run_form(const Job& job, cudaStream_t st) {
     const int64_t most = FORM == kWeights ? (int64_t)p.splits * p.segments * job.groups * p.row_tiles * p.col_tiles
                                           : ((int64_t)job.rows / S::M + job.groups + 1) * p.col_tiles;
     if (most > INT32_MAX) return abi_fail(HB_BAD_ARGUMENT, "expert product: too many tiles");
+    p.blocked[0] = FORM == kWeights && job.n % BK == 0;
+    p.blocked[1] = (FORM == kWeights || FORM == kBack) && width % BK == 0;
     bool ok = true;
     const int maps = S::kHalves ? 2 : p.segments;
     for (int i = 0; i < maps && ok; ++i) {
         if (FORM == kWeights) {
-            ok = encode(&p.a[i], job.a[i], job.type, job.n, job.rows, 0, BK);
-            if (i == 0) ok = ok && encode(&p.b[0], job.b[0], job.type, job.k, job.rows, 0, BK);
+            ok = encode(&p.a[i], job.a[i], job.type, job.n, job.rows, 0, BK, p.blocked[0]);
+            if (i == 0) ok = ok && encode(&p.b[0], job.b[0], job.type, job.k, job.rows, 0, BK, p.blocked[1]);
         } else {
-            if (!S::kHalves || i == 0) ok = encode(&p.a[i], job.a[i], job.type, job.k, job.rows, 0, 128);
-            if (FORM == kBack) ok = ok && encode(&p.b[i], job.b[i], job.type, job.n, job.k, job.groups, BK);
-            else ok = ok && encode(&p.b[i], job.b[i], job.type, job.k, job.n, job.groups, S::kHalves && !PAIR ? 64 : 128);
+            if (!S::kHalves || i == 0) ok = encode(&p.a[i], job.a[i], job.type, job.k, job.rows, 0, 128, false);
+            if (FORM == kBack) ok = ok && encode(&p.b[i], job.b[i], job.type, job.n, job.k, job.groups, BK, p.blocked[1]);
+            else ok = ok && encode(&p.b[i], job.b[i], job.type, job.k, job.n, job.groups, S::kHalves && !PAIR ? 64 : 128, false);
         }
     }
     if (!ok) return abi_fail(HB_TENSOR_MAP, "expert product: cuTensorMapEncodeTiled failed");

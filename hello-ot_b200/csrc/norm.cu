@@ -45,7 +45,7 @@ __device__ __forceinline__ float of_code(uint8_t c) {
 struct Forward {
     const void *x, *residual, *weight;
     int64_t x_row, residual_row, rows;
-    int width, weight_type;
+    int width, weight_type, weight_whole;
     float eps;
     void *y, *total;
     uint8_t *codes, *scales;
@@ -66,11 +66,28 @@ __device__ __forceinline__ float row_sum(float v, float* shared) {
     return s;
 }
 
-// A vector of the weight's values; V::N of them from column c.
-template <int N>
-__device__ __forceinline__ void load_weights(float (&w)[N], const void* p, int type, int c) {
+// N values of the weight from column c, a multiple of N; whole: the weight begins on 16 bytes.
+template <int N, typename T>
+__device__ __forceinline__ void load_values(float (&w)[N], const T* p, bool whole) {
+    constexpr int BYTES = N * (int)sizeof(T) < 16 ? N * (int)sizeof(T) : 16, M = BYTES / (int)sizeof(T);
+    if (whole) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) w[j] = rows::load_weight(p, type, c + j);
+        for (int q = 0; q < N / M; ++q) {
+            rows::Vec<T, BYTES> v;
+            v.load(p + q * M);
+#pragma unroll
+            for (int j = 0; j < M; ++j) w[q * M + j] = rows::to_float(v.v[j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) w[j] = rows::to_float(p[j]);
+    }
+}
+template <int N, typename P>
+__device__ __forceinline__ void load_weights(float (&w)[N], const P& p, int c) {
+    if (p.weight_type == HB_F32) load_values<N>(w, static_cast<const float*>(p.weight) + c, p.weight_whole);
+    else if (p.weight_type == HB_F16) load_values<N>(w, static_cast<const __half*>(p.weight) + c, p.weight_whole);
+    else load_values<N>(w, static_cast<const __nv_bfloat16*>(p.weight) + c, p.weight_whole);
 }
 
 // N values of row r from column c in 8 bits; the lanes of a group hold neighbouring vectors.  Called by whole warps;
@@ -122,7 +139,7 @@ __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS) forward_kernel(
     };
     auto write = [&](const float (&f)[V::N], int c, float scale, bool there) {
         float w[V::N], out[V::N];
-        if (there) load_weights(w, p.weight, p.weight_type, c);
+        if (there) load_weights(w, p, c);
 #pragma unroll
         for (int j = 0; j < V::N; ++j) out[j] = there ? f[j] * scale * w[j] : 0.0f;
         if constexpr (BITS8) {
@@ -225,7 +242,7 @@ __global__ void __launch_bounds__(256) read_kernel(const uint8_t* __restrict__ c
 struct Backward {
     const void *dy, *x, *dtotal, *weight;
     int64_t dy_row, x_row, dtotal_row, rows;
-    int width, weight_type;
+    int width, weight_type, weight_whole;
     float eps;
     void* dx;
     float *partial, *stats;  // partial: [blocks][width]; stats: [rows][2] of wide rows
@@ -249,23 +266,34 @@ __device__ __forceinline__ float2 row_sums(float a, float b, float2* shared) {
     return s;
 }
 
-// Rows held in registers; a block strides over the rows and keeps its sums for dw.
+// Rows held in registers; a block strides over the rows and keeps its sums for dw.  Up to 16 columns a thread the
+// weight's values are held too, above they come from L1 for each row.
+// Resident blocks an SM: what the registers of a thread's columns leave (102, 170, 128 a thread).
+constexpr int resident(int threads, int columns) { return threads >= 512 ? 1 : columns <= 16 ? 5 : 3; }
 template <typename T, int VB, int THREADS, int HELD>
-__global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS) backward_kernel(const __grid_constant__ Backward p) {
+__global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS, resident(THREADS, HELD * VB / (int)sizeof(T)))
+    backward_kernel(const __grid_constant__ Backward p) {
     using V = rows::Vec<T, VB>;
     constexpr int BLOCK = THREADS < 128 ? 128 : THREADS, ROWS = BLOCK / THREADS;
+    constexpr bool KEEP = HELD * V::N <= 16;
     __shared__ float2 shared[THREADS / 32];
     __shared__ float joined[ROWS > 1 ? THREADS * HELD * V::N : 1];
     const int t = threadIdx.x % THREADS, mine = threadIdx.x / THREADS;
-    float dw[HELD][V::N];
+    float dw[HELD][V::N], kept[KEEP ? HELD : 1][V::N];
 #pragma unroll
-    for (int i = 0; i < HELD; ++i)
+    for (int i = 0; i < HELD; ++i) {
+        const int c = (i * THREADS + t) * V::N;
 #pragma unroll
-        for (int j = 0; j < V::N; ++j) dw[i][j] = 0.0f;
+        for (int j = 0; j < V::N; ++j) {
+            dw[i][j] = 0.0f;
+            if (KEEP) kept[i][j] = 0.0f;
+        }
+        if (KEEP && c < p.width) load_weights(kept[i], p, c);
+    }
     for (int64_t r = (int64_t)blockIdx.x * ROWS + mine; r < p.rows; r += (int64_t)gridDim.x * ROWS) {
         const T* x = static_cast<const T*>(p.x) + r * p.x_row;
         const T* dy = static_cast<const T*>(p.dy) + r * p.dy_row;
-        const T* dtotal = p.dtotal ? static_cast<const T*>(p.dtotal) + r * p.dtotal_row : nullptr;
+        const T* dtotal = p.dtotal && p.dx ? static_cast<const T*>(p.dtotal) + r * p.dtotal_row : nullptr;
         V a[HELD], g[HELD], d[HELD];
 #pragma unroll
         for (int i = 0; i < HELD; ++i) {
@@ -273,24 +301,23 @@ __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS) backward_kernel
             if (c < p.width) {
                 a[i].load_once(x + c);
                 g[i].load_once(dy + c);
-                if (dtotal && p.dx) d[i].load_once(dtotal + c);
+                if (dtotal) d[i].load_once(dtotal + c);
             } else {
                 a[i].zero();
                 g[i].zero();
             }
         }
         float squares = 0.0f, along = 0.0f;
-        float w[HELD][V::N];
 #pragma unroll
         for (int i = 0; i < HELD; ++i) {
             const int c = (i * THREADS + t) * V::N;
-            if (c < p.width) load_weights(w[i], p.weight, p.weight_type, c);
+            float w[V::N];
+            if (!KEEP && c < p.width) load_weights(w, p, c);
 #pragma unroll
             for (int j = 0; j < V::N; ++j) {
-                const float xf = rows::to_float(a[i].v[j]);
-                w[i][j] = c < p.width ? w[i][j] * rows::to_float(g[i].v[j]) : 0.0f;
+                const float xf = rows::to_float(a[i].v[j]), wj = KEEP ? kept[i][j] : c < p.width ? w[j] : 0.0f;
                 squares = fmaf(xf, xf, squares);
-                along = fmaf(w[i][j], xf, along);
+                along = fmaf(wj * rows::to_float(g[i].v[j]), xf, along);
             }
         }
         const float2 sums = row_sums<THREADS>(squares, along, shared);
@@ -300,13 +327,15 @@ __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS) backward_kernel
         for (int i = 0; i < HELD; ++i) {
             const int c = (i * THREADS + t) * V::N;
             if (c >= p.width) continue;
+            float w[V::N];
+            if (!KEEP) load_weights(w, p, c);
             V o;
 #pragma unroll
             for (int j = 0; j < V::N; ++j) {
-                const float xf = rows::to_float(a[i].v[j]);
-                dw[i][j] = fmaf(rows::to_float(g[i].v[j]) * xf, inverse, dw[i][j]);
-                float v = fmaf(inverse, w[i][j], -xf * back);
-                if (dtotal && p.dx) v += rows::to_float(d[i].v[j]);
+                const float xf = rows::to_float(a[i].v[j]), gf = rows::to_float(g[i].v[j]);
+                dw[i][j] = fmaf(gf * xf, inverse, dw[i][j]);
+                float v = fmaf(inverse, (KEEP ? kept[i][j] : w[j]) * gf, -xf * back);
+                if (dtotal) v += rows::to_float(d[i].v[j]);
                 o.v[j] = rows::from_float<T>(v);
             }
             if (p.dx) o.store_once(static_cast<T*>(p.dx) + r * p.width + c);
@@ -353,7 +382,7 @@ __global__ void __launch_bounds__(512) wide_sums_kernel(const __grid_constant__ 
         float w[V::N];
         a.load(x + c);
         g.load(dy + c);
-        load_weights(w, p.weight, p.weight_type, c);
+        load_weights(w, p, c);
 #pragma unroll
         for (int j = 0; j < V::N; ++j) {
             const float xf = rows::to_float(a.v[j]);
@@ -374,7 +403,7 @@ __global__ void __launch_bounds__(256) wide_kernel(const __grid_constant__ Backw
     const int c = (blockIdx.x * 256 + threadIdx.x) * V::N;
     if (c >= p.width) return;
     float w[V::N], dw[V::N];
-    load_weights(w, p.weight, p.weight_type, c);
+    load_weights(w, p, c);
 #pragma unroll
     for (int j = 0; j < V::N; ++j) dw[j] = 0.0f;
     for (int64_t r = blockIdx.y; r < p.rows; r += gridDim.y) {
@@ -428,9 +457,9 @@ void for_width(int64_t vectors, F&& f) {
 constexpr int64_t kMostHeld = 2048;  // vectors of a row that for_width holds
 constexpr int kParts = 148 * 8;      // most blocks that sum dw
 
-inline int parts_of(int64_t rows, int64_t vectors) {
-    // resident blocks: 8 of 128 threads an SM, 2 of 512; the rows of a block are at least 4
-    const int64_t blocks = vectors <= 512 ? 148 * 8 : 148 * 2, side = vectors <= 64 ? 4 : 1;
+// Blocks that sum dw: as many as are resident, each with at least 4 turns.
+inline int parts_of(int64_t rows, int threads, int columns) {
+    const int64_t side = threads < 128 ? 128 / threads : 1, blocks = 148 * resident(threads, columns);
     return (int)std::max<int64_t>(1, std::min(blocks, (rows + 4 * side - 1) / (4 * side)));
 }
 
@@ -478,7 +507,7 @@ extern "C" int hb_rms_norm(int type, const void* x, int64_t x_stride, const void
         rows::address_bits(weight) % rows::type_bytes(weight_type) || (codes ? !scales || y : !y) || rows::address_bits(y) % size ||
         rows::address_bits(total) % size)
         return abi_fail(HB_BAD_ARGUMENT, "hb_rms_norm: null or misaligned pointer, or bad stride");
-    Forward p{x, residual, weight, x_stride, residual_stride, rows, (int)width, weight_type, (float)eps, y, total,
+    Forward p{x, residual, weight, x_stride, residual_stride, rows, (int)width, weight_type, rows::address_bits(weight) % 16 == 0, (float)eps, y, total,
               static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales)};
     uint64_t bits = rows::address_bits(x) | rows::address_bits(residual) | rows::address_bits(y) | rows::address_bits(total) |
                     (uint64_t)(width | (rows > 1 ? x_stride : 0) | (rows > 1 && residual ? residual_stride : 0)) * size;
@@ -546,7 +575,7 @@ extern "C" int hb_rms_norm_grad(int type, const void* dy, int64_t dy_stride, con
     const size_t sums = width > kMostHeld ? ((size_t)rows * 2 * sizeof(float) + 255) / 256 * 256 : 0;
     float* const stats = static_cast<float*>(workspace);
     float* const partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + sums);
-    Backward p{dy, x, dtotal, weight, dy_stride, x_stride, dtotal_stride, rows, (int)width, weight_type, (float)eps, dx,
+    Backward p{dy, x, dtotal, weight, dy_stride, x_stride, dtotal_stride, rows, (int)width, weight_type, rows::address_bits(weight) % 16 == 0, (float)eps, dx,
                dweight ? partial : nullptr, stats};
     uint64_t bits = rows::address_bits(dy) | rows::address_bits(x) | rows::address_bits(dtotal) | rows::address_bits(dx) |
                     (uint64_t)(width | (rows > 1 ? x_stride | dy_stride : 0) | (rows > 1 && dtotal ? dtotal_stride : 0)) * size;
@@ -556,11 +585,12 @@ extern "C" int hb_rms_norm_grad(int type, const void* dy, int64_t dy_stride, con
         constexpr int VB = decltype(vb)::value, N = VB / (int)sizeof(T);
         const int64_t vectors = (width + N - 1) / N;
         if (vectors <= kMostHeld) {
-            parts = parts_of(rows, vectors);
             for_width(vectors, [&](auto threads, auto held) {
                 constexpr int THREADS = decltype(threads)::value, HELD = decltype(held)::value;
-                if constexpr (HELD > 0)
+                if constexpr (HELD > 0) {
+                    parts = parts_of(rows, THREADS, HELD * N);
                     backward_kernel<T, VB, THREADS, HELD><<<parts, THREADS < 128 ? 128 : THREADS, 0, st>>>(p);
+                }
             });
             count_launches(1);
             return;
