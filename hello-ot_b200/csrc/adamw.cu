@@ -4,7 +4,7 @@
 //   p = p (1 - lr decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // Two launches over one list of chunks in the kernel's parameters: one thread counts the step and works out what
-// all elements share (in fp64: t, the bias corrections, f), then warps go through blocks of 256 elements, 8 a lane.
+// all elements share (in fp64: t, the bias corrections, f), then a warp takes a block of 256 elements, 8 a lane.
 // The second launch starts while the first runs and waits for it when its first loads are on their way
 // (programmatic dependent launch).  Bound by HBM: every array passes once.
 //
@@ -17,10 +17,11 @@
 // m and v are rounded to fp32 at every operation as it is written, and their codes are those of the correctly rounded
 // quotients, so that any fp32 program computes the same states bit for bit.  The change of p takes the approximate
 // root and quotient (2^-20 of the change): with the exact ones, 3 quotients and a root an element, the kernel was bound
-// by instructions (400 million bf16 parameters, 8 bits: 2.46 ms of 0.86 at the copy rate).
+// by instructions.
 #include <algorithm>
 #include <cmath>
 #include <string>
+#include <type_traits>
 
 #include <cuda_fp8.h>
 
@@ -30,25 +31,27 @@
 namespace hb {
 namespace adamw {
 
-constexpr int kThreads = 256, kBlock = 256, kChunk = 2048;  // elements: of a scale, of a block of threads (a scale a warp)
-constexpr int kMost8 = 280, kMost32 = 330;                   // tensors of a launch: 32 KB of parameters
+constexpr int kThreads = 256, kBlock = 256;            // kBlock: elements of a scale, a warp's
+constexpr int kChunk = 2048, kLongChunk = 8192;        // elements of a block of threads
+constexpr int64_t kLongLeast = 148 * 8 * (int64_t)kLongChunk;  // elements from which chunks are long
+constexpr float kLeastBy = 0x1p-63f;                   // least divisor of a change: the root of the least normal v
+constexpr int kFew = 24, kMany = 360;                  // tensors of a launch: 2 KB or 31 KB of parameters
 
+struct Entry {  // one tensor; its fields lie together, as a block reads those of one
+    void* param;
+    const void* grad;
+    void *first, *second;
+    float *first_scale, *second_scale, *master;
+    int64_t size;
+    int32_t chunk;                    // its first
+    uint8_t type, grad_type, aligned; // aligned: all of its arrays lie on 16 bytes
+};
 template <int MOST>
 struct List {
-    void* param[MOST];
-    const void* grad[MOST];
-    void *first[MOST], *second[MOST];
-    float* master[MOST];
-    int64_t size[MOST];
-    int32_t chunk[MOST + 1];  // first chunk of each tensor
-    uint8_t type[MOST], grad_type[MOST];
-    int count;
+    Entry e[MOST];
+    int count, chunk;  // tensors, elements a chunk
 };
-struct Scales {  // of a list's tensors; 8-bit states
-    float *first[kMost8], *second[kMost8];
-};
-struct NoScales {};
-static_assert(sizeof(List<kMost8>) + sizeof(Scales) < 32000 && sizeof(List<kMost32>) < 32000, "kernel parameters");
+static_assert(sizeof(List<kMany>) < 32000, "kernel parameters");
 
 struct Shared {  // what all elements share, in device memory
     float factor, keep, rate, over_root;  // over_root: 1 / sqrt(1 - b2^t)
@@ -79,193 +82,315 @@ __device__ __forceinline__ int tensor_of(const List<MOST>& l, int chunk) {
     int lo = 0, hi = l.count - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (l.chunk[mid] <= chunk) lo = mid;
+        if (l.e[mid].chunk <= chunk) lo = mid;
         else hi = mid - 1;
     }
     return lo;
 }
 
-// A lane's 8 values, `left` of them there; VECTORS: all of them, on 16 bytes.
-template <typename T>
-__device__ __forceinline__ void read8(float (&f)[8], const T* p, int left, bool vectors) {
-    if (vectors) {
-        constexpr int N = 16 / (int)sizeof(T);
+// Two fp32 values in one operation, each rounded like the scalar one: half the instructions of the multiply-add pipe.
+union Pair {
+    uint64_t both;
+    float2 f;
+    __device__ __forceinline__ Pair() {}
+    __device__ __forceinline__ explicit Pair(float a) : f{a, a} {}
+    __device__ __forceinline__ Pair(float a, float b) : f{a, b} {}
+};
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.both) : "l"(a.both), "l"(b.both));
+    return r;
+}
+// Scalar: of a product and a sum in pairs the assembler makes one fused operation, .rn or not.
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) { return Pair(__fadd_rn(a.f.x, b.f.x), __fadd_rn(a.f.y, b.f.y)); }
+__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.both) : "l"(a.both), "l"(b.both), "l"(c.both));
+    return r;
+}
+// A lane has 8 values of a block of 256: 4 from lane * 4 on and 4 from 128 further, so that neighbouring lanes' words are
+// neighbours in memory.  Writes 4 of them; WHOLE: all are there, on 16 bytes, else `left`.
+template <typename T, bool WHOLE>
+__device__ __forceinline__ void write4(const Pair* f, T* p, int left) {
+    rows::Vec<T, 4 * (int)sizeof(T)> v;
 #pragma unroll
-        for (int q = 0; q < 8 / N; ++q) {
-            rows::Vec<T, 16> v;
-            v.raw = *reinterpret_cast<const uint4*>(p + q * N);
-#pragma unroll
-            for (int j = 0; j < N; ++j) f[q * N + j] = rows::to_float(v.v[j]);
-        }
+    for (int k = 0; k < 2; ++k) {
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) reinterpret_cast<__nv_bfloat162*>(v.v)[k] = __float22bfloat162_rn(f[k].f);
+        else if constexpr (std::is_same<T, __half>::value) reinterpret_cast<__half2*>(v.v)[k] = __float22half2_rn(f[k].f);
+        else v.v[2 * k] = f[k].f.x, v.v[2 * k + 1] = f[k].f.y;
+    }
+    if (WHOLE) {
+        v.store_once(p);
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = j < left ? rows::to_float(p[j]) : 0.0f;
+        for (int j = 0; j < 4; ++j)
+            if (j < left) p[j] = v.v[j];
     }
 }
-template <typename T>
-__device__ __forceinline__ void write8(const float (&f)[8], T* p, int left, bool vectors) {
-    if (vectors) {
-        constexpr int N = 16 / (int)sizeof(T);
-#pragma unroll
-        for (int q = 0; q < 8 / N; ++q) {
-            rows::Vec<T, 16> v;
-#pragma unroll
-            for (int j = 0; j < N; ++j) v.v[j] = rows::from_float<T>(f[q * N + j]);
-            v.store_once(p + q * N);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (j < left) p[j] = rows::from_float<T>(f[j]);
-    }
+__device__ __forceinline__ Pair of_codes(uint32_t two) {  // the lower two bytes
+    Pair r;
+    r.f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3)));
+    return r;
 }
-__device__ __forceinline__ void read_codes(uint8_t (&c)[8], const uint8_t* p, int left, bool vectors) {
-    if (vectors) {
-        rows::Vec<uint8_t, 8> v;
-        v.raw = *reinterpret_cast<const uint2*>(p);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) c[j] = v.v[j];
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) c[j] = j < left ? p[j] : 0;
-    }
-}
-__device__ __forceinline__ void of_codes(float (&f)[8], const uint8_t (&c)[8]) {
-#pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c[j] | c[j + 1] << 8), __NV_E4M3);
-        const float2 v = __half22float2(__half2(h));
-        f[j] = v.x, f[j + 1] = v.y;
-    }
-}
-// a / b within 2^-21, for any b >= 0 of the range: __fdividef's divisors end at 2^126.
-__device__ __forceinline__ float quotient(float a, float b) { return b < 0x1p126f ? __fdividef(a, b) : a / b; }
-__device__ __forceinline__ float root_near(float v) {  // within 2^-23 of the root
+__device__ __forceinline__ float root_near(float v) {  // within 2^-23 of the root, 0 for v below 2^-126
     float r;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float inverse_near(float v) {  // within 2^-23 of 1 / v, v 0 or a normal number below 2^126
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+// v / 448, correctly rounded: the quotient by the constant's inverse and one correction by its residual, both fused, are
+// exact for every 24-bit significand (a quotient by a constant after Brisebarre, Muller and Raina; all 2^23 were
+// checked), as long as nothing on the way is subnormal.
+__device__ __forceinline__ float by_448(float v) {
+    if (!(v >= 0x1p-80f && v <= 0x1p120f)) return __fdiv_rn(v, 448.0f);
+    const float q = v * (1.0f / 448.0f);
+    return fmaf(fmaf(-448.0f, q, v), 1.0f / 448.0f, q);
+}
+__device__ __forceinline__ float larger(float a, float b) {  // a NaN stays
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
 
 // The block's values (ROOT: their roots, which are >= 0) in 8 bits: the warp's largest magnitude by 448 is the scale (a NaN
-// makes it one), the codes are those of the correctly rounded root and quotient.  Both are approximated first, to
-// within 2^-22 with the scale's inverse: where the codes a little below and above are the same, that is the code, and
-// only next to a border between two codes (one value in some 10^5) the exact operations are run.  ROOT: values above
-// zero keep at least the smallest code.
-template <bool ROOT>
-__device__ __forceinline__ void hold(const float (&f)[8], const float (&near)[8], uint8_t* codes, float* scale, int left, bool vectors) {
-    uint32_t most = 0;
+// makes it one), the codes are those of the correctly rounded root and quotient.  Both are approximated first, to within
+// 2^-21 together with the scale's inverse, once from below and once from above: where the two codes differ, a border
+// between codes is that near (one value in some 10^5), and the exact operations are run.  ROOT: values above
+// zero keep at least the smallest code; so where a code is 0, they are run too.
+template <bool ROOT, bool WHOLE>
+__device__ __forceinline__ void hold(const Pair (&f)[4], uint8_t* codes, float* scale, int left) {
+    float top = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) most = max(most, j < left ? __float_as_uint(fabsf(f[j])) : 0u);
-    most = __reduce_max_sync(0xffffffffu, most);
-    const float largest = ROOT ? __fsqrt_rn(__uint_as_float(most)) : __uint_as_float(most);
-    const float s = __fdiv_rn(largest, 448.0f);
-    const float by = s > 0.0f ? s : 1.0f, inverse = __fdiv_rn(1.0f, by);
-    const bool plain = by >= 0x1p-100f && by <= 0x1p100f;  // nothing below leaves the normal numbers
-    rows::Vec<uint8_t, 8> v;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float q = near[j] * inverse;
-        const uint32_t both = __nv_cvt_float2_to_fp8x2(make_float2(fmaf(q, -0x1p-21f, q), fmaf(q, 0x1p-21f, q)), __NV_SATFINITE, __NV_E4M3);
-        uint32_t code = both & 0xff;
-        if (code != both >> 8 || !plain)
-            code = __nv_cvt_float_to_fp8(__fdiv_rn(ROOT ? __fsqrt_rn(f[j]) : f[j], by), __NV_SATFINITE, __NV_E4M3);
-        if (ROOT && code == 0 && f[j] > 0.0f) code = 1;
-        v.v[j] = (uint8_t)code;
+    for (int k = 0; k < 4; ++k) {
+        const int j = (k >> 1) * 128 + (k & 1) * 2;
+        if (WHOLE || j < left) top = larger(top, fabsf(f[k].f.x));
+        if (WHOLE || j + 1 < left) top = larger(top, fabsf(f[k].f.y));
     }
-    if (vectors) {
-        v.store_once(codes);
-    } else {
+    const float most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+    uint32_t c[4] = {0, 0, 0, 0};
+    const float s = by_448(ROOT ? __fsqrt_rn(most) : most);
+    if (most != 0.0f) {  // the same for the warp
+        const float inverse = inverse_near(s);
+        uint32_t differ = s >= 0x1p-50f && s <= 0x1p100f ? 0 : 1;  // outside, the approximations leave the normal numbers
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (j < left) codes[j] = v.v[j];
+        for (int k = 0; k < 4; ++k) {
+            const Pair near = ROOT ? Pair(root_near(f[k].f.x), root_near(f[k].f.y)) : f[k];
+            const Pair below = near * Pair(inverse * (1.0f - 0x1p-21f)), above = near * Pair(inverse * (1.0f + 0x1p-21f));
+            c[k] = __nv_cvt_float2_to_fp8x2(below.f, __NV_SATFINITE, __NV_E4M3);
+            differ |= c[k] ^ __nv_cvt_float2_to_fp8x2(above.f, __NV_SATFINITE, __NV_E4M3);
+        }
+        if (ROOT) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const uint32_t word = c[2 * q] | c[2 * q + 1] << 16;
+                differ |= (word - 0x01010101u) & ~word & 0x80808080u;  // a byte that is 0
+            }
+        }
+        if (differ) {
+            const float by = s > 0.0f ? s : 1.0f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float2 q = f[k].f;
+                if (ROOT) q = make_float2(__fsqrt_rn(q.x), __fsqrt_rn(q.y));
+                c[k] = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(q.x, by), __fdiv_rn(q.y, by)), __NV_SATFINITE, __NV_E4M3);
+                if (ROOT && (c[k] & 0xff) == 0 && f[k].f.x > 0.0f) c[k] |= 1;
+                if (ROOT && c[k] >> 8 == 0 && f[k].f.y > 0.0f) c[k] |= 0x100;
+            }
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const uint32_t word = c[2 * q] | c[2 * q + 1] << 16;
+        if (WHOLE) {
+            __stcs(reinterpret_cast<uint32_t*>(codes + q * 128), word);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (q * 128 + j < left) codes[q * 128 + j] = (uint8_t)(word >> (8 * j));
+        }
     }
     if ((threadIdx.x & 31) == 0) *scale = s;
 }
 
-// A lane's share of a block of 256 elements that begins at `at`.
-template <int BITS, typename T, typename TG, int MOST, typename S>
-__device__ __forceinline__ void step_block(const List<MOST>& l, const S& scales, int t, int64_t at, const Fixed& fixed,
-                                           const Shared* shared) {
-    const int64_t i = at + (threadIdx.x & 31) * 8;
-    const int left = (int)min((int64_t)8, l.size[t] - i);  // may be <= 0
-    T* param = static_cast<T*>(l.param[t]);
-    const TG* grad = static_cast<const TG*>(l.grad[t]);
-    float* master = l.master[t];
-    const uint64_t bits = reinterpret_cast<uintptr_t>(param) | reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(master) |
-                          reinterpret_cast<uintptr_t>(l.first[t]) | reinterpret_cast<uintptr_t>(l.second[t]);
-    const bool vectors = left == 8 && (bits & 15) == 0;
-    float p[8], g[8], m[8], v[8];
-    uint8_t mc[8], vc[8];
-    float ms = 0.0f, vs = 0.0f;
-    if (master) read8(p, master + i, left, vectors);
-    else read8(p, param + i, left, vectors);
-    read8(g, grad + i, left, vectors);
-    if constexpr (BITS == 32) {
-        read8(m, static_cast<const float*>(l.first[t]) + i, left, vectors);
-        read8(v, static_cast<const float*>(l.second[t]) + i, left, vectors);
-    } else {
-        read_codes(mc, static_cast<const uint8_t*>(l.first[t]) + i, left, vectors);
-        read_codes(vc, static_cast<const uint8_t*>(l.second[t]) + i, left, vectors);
-        ms = scales.first[t][at / kBlock];
-        vs = scales.second[t][at / kBlock];
+// The arrays of a chunk: uniform for a block of threads, who add 32-bit offsets.  TS: what parameters are read from, their
+// own type or the fp32 masters.
+template <typename T, typename TS, typename TG>
+struct Chunk {
+    const TS* source;
+    T* param;
+    float* master;
+    const TG* grad;
+    void *first, *second;
+    float *first_scale, *second_scale;
+};
+
+// What a lane reads of a whole block, raw: the next block's is on its way while this one is computed.
+template <int BITS, typename TS, typename TG>
+struct Lane {
+    template <typename V>
+    using Words = rows::Vec<V, 4 * (int)sizeof(V)>;
+    Words<TS> source[2];
+    Words<TG> grad[2];
+    Words<float> first[BITS == 32 ? 2 : 1], second[BITS == 32 ? 2 : 1];
+    uint32_t first_code[2], second_code[2];
+    float first_scale, second_scale;
+    template <typename V>
+    static __device__ __forceinline__ void words(Words<V>& to, const V* p) {
+        to.raw = *reinterpret_cast<const typename Words<V>::Raw*>(p);
     }
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const volatile Shared* now = shared;
-    const float factor = now->factor, keep = now->keep, rate = now->rate, over_root = now->over_root;
-    if constexpr (BITS == 8) {
-        of_codes(m, mc);
-        of_codes(v, vc);
+    template <typename C>
+    __device__ __forceinline__ void load(const C& c, uint32_t block) {
+        const uint32_t i = block * kBlock + (threadIdx.x & 31) * 4;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            m[j] = __fmul_rn(m[j], ms);
-            v[j] = __fmul_rn(v[j], vs);
-            v[j] = __fmul_rn(v[j], v[j]);
+        for (int q = 0; q < 2; ++q) {
+            words<TS>(source[q], c.source + i + q * 128);
+            words<TG>(grad[q], c.grad + i + q * 128);
+            if constexpr (BITS == 32) {
+                words<float>(first[q], static_cast<const float*>(c.first) + i + q * 128);
+                words<float>(second[q], static_cast<const float*>(c.second) + i + q * 128);
+            } else {
+                first_code[q] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(c.first) + i + q * 128);
+                second_code[q] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(c.second) + i + q * 128);
+            }
+        }
+        if constexpr (BITS == 8) first_scale = c.first_scale[block], second_scale = c.second_scale[block];
+    }
+    // Of a block whose end is the tensor's, or off the 16-byte grid: `left` elements from the lane's first on.
+    template <typename C>
+    __device__ __forceinline__ void load_some(const C& c, uint32_t block, int left) {
+        const uint32_t i = block * kBlock + (threadIdx.x & 31) * 4;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            if constexpr (BITS == 8) first_code[q] = second_code[q] = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool there = q * 128 + j < left;
+                const uint32_t at = i + q * 128 + j;
+                source[q].v[j] = there ? c.source[at] : rows::from_float<TS>(0.0f);
+                grad[q].v[j] = there ? c.grad[at] : rows::from_float<TG>(0.0f);
+                if constexpr (BITS == 32) {
+                    first[q].v[j] = there ? static_cast<const float*>(c.first)[at] : 0.0f;
+                    second[q].v[j] = there ? static_cast<const float*>(c.second)[at] : 0.0f;
+                } else if (there) {
+                    first_code[q] |= (uint32_t)static_cast<const uint8_t*>(c.first)[at] << (8 * j);
+                    second_code[q] |= (uint32_t)static_cast<const uint8_t*>(c.second)[at] << (8 * j);
+                }
+            }
+        }
+        if constexpr (BITS == 8) first_scale = c.first_scale[block], second_scale = c.second_scale[block];
+    }
+};
+template <typename V>
+__device__ __forceinline__ Pair pair_of(const V& words, int k) {
+    return Pair(rows::to_float(words.v[2 * k]), rows::to_float(words.v[2 * k + 1]));
+}
+
+// The step of a lane's 8 values of a block, 4 at a time up to the states.
+template <int BITS, bool WHOLE, typename T, typename TS, typename TG>
+__device__ __forceinline__ void advance(const Chunk<T, TS, TG>& c, uint32_t block, int left, const Lane<BITS, TS, TG>& lane,
+                                        const Fixed& fixed, const Shared& now) {
+    const uint32_t i = block * kBlock + (threadIdx.x & 31) * 4;
+    Pair m[4], v[4];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        Pair p[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            Pair &mk = m[q * 2 + k], &vk = v[q * 2 + k];
+            if constexpr (BITS == 8) {
+                mk = of_codes(lane.first_code[q] >> (16 * k)) * Pair(lane.first_scale);
+                vk = of_codes(lane.second_code[q] >> (16 * k)) * Pair(lane.second_scale);
+                vk = vk * vk;
+            } else {
+                mk = pair_of(lane.first[q], k);
+                vk = pair_of(lane.second[q], k);
+            }
+            const Pair g = pair_of(lane.grad[q], k) * Pair(now.factor);
+            mk = mk * Pair(fixed.beta1) + g * Pair(fixed.less1);
+            vk = vk * Pair(fixed.beta2) + (g * g) * Pair(fixed.less2);
+            const Pair root(root_near(vk.f.x), root_near(vk.f.y));
+            Pair by = fma(root, Pair(now.over_root), Pair(fixed.eps));
+            by = Pair(larger(by.f.x, kLeastBy), larger(by.f.y, kLeastBy));
+            p[k] = fma(Pair(-now.rate), mk * Pair(inverse_near(by.f.x), inverse_near(by.f.y)), pair_of(lane.source[q], k) * Pair(now.keep));
+        }
+        if (c.master) write4<float, WHOLE>(p, c.master + i + q * 128, left - q * 128);
+        write4<T, WHOLE>(p, c.param + i + q * 128, left - q * 128);
+        if constexpr (BITS == 32) {
+            write4<float, WHOLE>(m + q * 2, static_cast<float*>(c.first) + i + q * 128, left - q * 128);
+            write4<float, WHOLE>(v + q * 2, static_cast<float*>(c.second) + i + q * 128, left - q * 128);
         }
     }
-    float root[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float gj = __fmul_rn(g[j], factor);
-        m[j] = __fadd_rn(__fmul_rn(m[j], fixed.beta1), __fmul_rn(gj, fixed.less1));
-        v[j] = __fadd_rn(__fmul_rn(v[j], fixed.beta2), __fmul_rn(__fmul_rn(gj, gj), fixed.less2));
-        root[j] = root_near(v[j]);
-        p[j] = fmaf(-rate, quotient(m[j], fmaf(root[j], over_root, fixed.eps)), __fmul_rn(p[j], keep));
-    }
-    if (master) write8(p, master + i, left, vectors);
-    write8(p, param + i, left, vectors);
-    if constexpr (BITS == 32) {
-        write8(m, static_cast<float*>(l.first[t]) + i, left, vectors);
-        write8(v, static_cast<float*>(l.second[t]) + i, left, vectors);
-    } else {
-        hold<false>(m, m, static_cast<uint8_t*>(l.first[t]) + i, scales.first[t] + at / kBlock, left, vectors);
-        hold<true>(v, root, static_cast<uint8_t*>(l.second[t]) + i, scales.second[t] + at / kBlock, left, vectors);
+    if constexpr (BITS == 8) {
+        hold<false, WHOLE>(m, static_cast<uint8_t*>(c.first) + i, c.first_scale + block, left);
+        hold<true, WHOLE>(v, static_cast<uint8_t*>(c.second) + i, c.second_scale + block, left);
     }
 }
 
-template <int BITS, int MOST, typename S>
-__global__ void __launch_bounds__(kThreads) step_kernel(const __grid_constant__ List<MOST> l, const __grid_constant__ S scales,
-                                                        const Fixed fixed, const Shared* shared) {
-    const int t = tensor_of(l, blockIdx.x);
-    const int64_t at = (int64_t)(blockIdx.x - l.chunk[t]) * kChunk + (threadIdx.x >> 5) * kBlock;
-    if (at >= l.size[t]) {  // the launch does not end before the one it overlaps
-        asm volatile("griddepcontrol.wait;" ::: "memory");
-        return;
+// A warp's blocks of the chunk [from, to).
+template <int BITS, typename T, typename TS, typename TG>
+__device__ __forceinline__ void step_chunk(const Entry& e, int64_t from, int64_t to, const Fixed& fixed, const Shared* shared) {
+    constexpr uint32_t kWarps = kThreads / 32;
+    T* const param = static_cast<T*>(e.param) + from;
+    float* const master = e.master ? e.master + from : nullptr;
+    Chunk<T, TS, TG> c{};
+    if constexpr (std::is_same<T, TS>::value) c.source = param;
+    else c.source = master;
+    c.param = param;
+    c.master = master;
+    c.grad = static_cast<const TG*>(e.grad) + from;
+    c.first = static_cast<char*>(e.first) + from * (BITS / 8);
+    c.second = static_cast<char*>(e.second) + from * (BITS / 8);
+    if constexpr (BITS == 8) c.first_scale = e.first_scale + from / kBlock, c.second_scale = e.second_scale + from / kBlock;
+    const uint32_t length = (uint32_t)(to - from), whole = e.aligned ? length / kBlock : 0, blocks = (length + kBlock - 1) / kBlock;
+    Lane<BITS, TS, TG> here, next;
+    uint32_t block = threadIdx.x >> 5;
+    if (block < whole) here.load(c, block);
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // also where no block is left: not to end before the launch it overlaps
+    const volatile Shared* const written = shared;
+    const Shared now{written->factor, written->keep, written->rate, written->over_root};
+    for (; block < whole; block += kWarps) {
+        if (block + kWarps < whole) next.load(c, block + kWarps);
+        advance<BITS, true>(c, block, kBlock, here, fixed, now);
+        here = next;
     }
-    const int type = l.type[t], grad = l.grad_type[t];
-    if (type == HB_F32) step_block<BITS, float, float>(l, scales, t, at, fixed, shared);
-    else if (type == HB_F16 && grad == HB_F16) step_block<BITS, __half, __half>(l, scales, t, at, fixed, shared);
-    else if (type == HB_F16) step_block<BITS, __half, float>(l, scales, t, at, fixed, shared);
-    else if (grad == HB_BF16) step_block<BITS, __nv_bfloat16, __nv_bfloat16>(l, scales, t, at, fixed, shared);
-    else step_block<BITS, __nv_bfloat16, float>(l, scales, t, at, fixed, shared);
+    for (; block < blocks; block += kWarps) {
+        const int left = (int)(length - block * kBlock) - (int)(threadIdx.x & 31) * 4;  // may be <= 0
+        here.load_some(c, block, left);
+        advance<BITS, false>(c, block, left, here, fixed, now);
+    }
+}
+template <int BITS, typename T>
+__device__ __forceinline__ void step_typed(const Entry& e, int64_t from, int64_t to, const Fixed& fixed, const Shared* shared) {
+    if (e.grad_type == HB_F32) {
+        if (e.master) step_chunk<BITS, T, float, float>(e, from, to, fixed, shared);
+        else step_chunk<BITS, T, T, float>(e, from, to, fixed, shared);
+    } else {
+        if (e.master) step_chunk<BITS, T, float, T>(e, from, to, fixed, shared);
+        else step_chunk<BITS, T, T, T>(e, from, to, fixed, shared);
+    }
+}
+
+template <int BITS, int MOST>
+__global__ void __launch_bounds__(kThreads, BITS == 8 ? 3 : 2) step_kernel(const __grid_constant__ List<MOST> l, const Fixed fixed, const Shared* shared) {
+    const Entry& e = l.e[tensor_of(l, blockIdx.x)];
+    const int64_t from = (int64_t)((int)blockIdx.x - e.chunk) * l.chunk, to = min(e.size, from + l.chunk);
+    if (e.type == HB_F32) step_chunk<BITS, float, float, float>(e, from, to, fixed, shared);
+    else if (e.type == HB_F16) step_typed<BITS, __half>(e, from, to, fixed, shared);
+    else step_typed<BITS, __nv_bfloat16>(e, from, to, fixed, shared);
 }
 
 // ---------------------------------------------------------------- m and v of 8-bit states
+constexpr int kHeld = 400;
 struct Held {
-    const uint8_t *first[kMost8], *second[kMost8];
-    const float *first_scale[kMost8], *second_scale[kMost8];
-    float *out_first[kMost8], *out_second[kMost8];
-    int64_t size[kMost8];
-    int32_t chunk[kMost8 + 1];
+    const uint8_t *first[kHeld], *second[kHeld];
+    const float *first_scale[kHeld], *second_scale[kHeld];
+    float *out_first[kHeld], *out_second[kHeld];
+    int64_t size[kHeld];
+    int32_t chunk[kHeld];
     int count;
 };
 static_assert(sizeof(Held) < 32000, "kernel parameters");
@@ -279,59 +404,73 @@ __global__ void __launch_bounds__(kThreads) moments_kernel(const __grid_constant
     }
     const int64_t at = (int64_t)(blockIdx.x - l.chunk[lo]) * kChunk + (threadIdx.x >> 5) * kBlock;
     if (at >= l.size[lo]) return;
-    const int64_t i = at + (threadIdx.x & 31) * 8;
-    const int left = (int)min((int64_t)8, l.size[lo] - i);
+    const int64_t i = at + (threadIdx.x & 31) * 4;
+    const int left = (int)min((int64_t)kBlock, l.size[lo] - i);
     const uint64_t bits = reinterpret_cast<uintptr_t>(l.first[lo]) | reinterpret_cast<uintptr_t>(l.second[lo]) |
                           reinterpret_cast<uintptr_t>(l.out_first[lo]) | reinterpret_cast<uintptr_t>(l.out_second[lo]);
-    const bool vectors = left == 8 && (bits & 15) == 0;
-    uint8_t mc[8], vc[8];
-    float m[8], v[8];
-    read_codes(mc, l.first[lo] + i, left, vectors);
-    read_codes(vc, l.second[lo] + i, left, vectors);
     const float ms = l.first_scale[lo][at / kBlock], vs = l.second_scale[lo][at / kBlock];
-    of_codes(m, mc);
-    of_codes(v, vc);
+    auto go = [&](auto whole) {
+        constexpr bool WHOLE = decltype(whole)::value != 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        m[j] = __fmul_rn(m[j], ms);
-        v[j] = __fmul_rn(v[j], vs);
-        v[j] = __fmul_rn(v[j], v[j]);
-    }
-    write8(m, l.out_first[lo] + i, left, vectors);
-    write8(v, l.out_second[lo] + i, left, vectors);
+        for (int q = 0; q < 2; ++q) {
+            uint32_t mc = 0, vc = 0;
+            const uint8_t *first = l.first[lo] + i + q * 128, *second = l.second[lo] + i + q * 128;
+            if (WHOLE) {
+                mc = *reinterpret_cast<const uint32_t*>(first);
+                vc = *reinterpret_cast<const uint32_t*>(second);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (q * 128 + j < left) mc |= (uint32_t)first[j] << (8 * j), vc |= (uint32_t)second[j] << (8 * j);
+            }
+            Pair m[2], v[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                m[k] = of_codes(mc >> (16 * k)) * Pair(ms);
+                v[k] = of_codes(vc >> (16 * k)) * Pair(vs);
+                v[k] = v[k] * v[k];
+            }
+            write4<float, WHOLE>(m, l.out_first[lo] + i + q * 128, left - q * 128);
+            write4<float, WHOLE>(v, l.out_second[lo] + i + q * 128, left - q * 128);
+        }
+    };
+    if (at + kBlock <= l.size[lo] && (bits & 15) == 0) go(rows::Bytes<1>{});
+    else go(rows::Bytes<0>{});
 }
 
 int finish(cudaError_t e, const char* what) {
     return e == cudaSuccess ? HB_OK : abi_fail(HB_LAUNCH, std::string(what) + ": " + cudaGetErrorString(e));
 }
 
-template <int BITS, int MOST, typename S>
+template <int BITS, int MOST>
 cudaError_t run(int64_t count, void* const* params, const void* const* grads, void* const* first, void* const* second,
                 float* const* first_scale, float* const* second_scale, float* const* master, const int64_t* sizes,
-                const int32_t* types, const int32_t* grad_types, const Fixed& fixed, const Shared* shared, cudaStream_t st) {
+                const int32_t* types, const int32_t* grad_types, int chunk, const Fixed& fixed, const Shared* shared, cudaStream_t st) {
     List<MOST> l;
-    S scales;
+    l.chunk = chunk;
     bool overlap = true;  // the first launch follows begin_kernel, the others a launch that writes
     for (int64_t from = 0; from < count; from += MOST) {
         l.count = 0;
         int64_t chunks = 0;
         for (int64_t i = from; i < std::min(count, from + MOST); ++i) {
             if (sizes[i] == 0) continue;
-            const int t = l.count++;
-            l.param[t] = params[i];
-            l.grad[t] = grads[i];
-            l.first[t] = first[i];
-            l.second[t] = second[i];
-            l.master[t] = master ? master[i] : nullptr;
-            if constexpr (BITS == 8) scales.first[t] = first_scale[i], scales.second[t] = second_scale[i];
-            l.size[t] = sizes[i];
-            l.type[t] = (uint8_t)types[i];
-            l.grad_type[t] = (uint8_t)grad_types[i];
-            l.chunk[t] = (int32_t)chunks;
-            chunks += (sizes[i] + kChunk - 1) / kChunk;
+            Entry& e = l.e[l.count++];
+            e.param = params[i];
+            e.grad = grads[i];
+            e.first = first[i];
+            e.second = second[i];
+            e.first_scale = BITS == 8 ? first_scale[i] : nullptr;
+            e.second_scale = BITS == 8 ? second_scale[i] : nullptr;
+            e.master = master ? master[i] : nullptr;
+            e.size = sizes[i];
+            e.chunk = (int32_t)chunks;
+            e.type = (uint8_t)types[i];
+            e.grad_type = (uint8_t)grad_types[i];
+            e.aligned = ((rows::address_bits(e.param) | rows::address_bits(e.grad) | rows::address_bits(e.first) |
+                          rows::address_bits(e.second) | rows::address_bits(e.master)) & 15) == 0;
+            chunks += (sizes[i] + chunk - 1) / chunk;
         }
         if (l.count == 0) continue;
-        l.chunk[l.count] = (int32_t)chunks;
         cudaLaunchAttribute attr{};
         attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr.val.programmaticStreamSerializationAllowed = 1;
@@ -342,7 +481,7 @@ cudaError_t run(int64_t count, void* const* params, const void* const* grads, vo
         config.attrs = &attr;
         config.numAttrs = overlap ? 1 : 0;
         overlap = false;
-        const cudaError_t e = cudaLaunchKernelEx(&config, step_kernel<BITS, MOST, S>, l, scales, fixed, shared);
+        const cudaError_t e = cudaLaunchKernelEx(&config, step_kernel<BITS, MOST>, l, fixed, shared);
         count_launches(1);
         if (e != cudaSuccess) return e;
     }
@@ -368,9 +507,9 @@ extern "C" int hb_adamw_step(int64_t count, void* const* params, const void* con
     if (!rule || bad(step, 4) || (count > 0 && (!params || !grads || !first || !second || !sizes || !types || !grad_types ||
                                                 (bits == 8 && (!first_scale || !second_scale)))))
         return abi_fail(HB_BAD_ARGUMENT, "hb_adamw_step: null pointer, or misaligned step");
-    if (!(rule->beta1 >= 0.0 && rule->beta1 < 1.0 && rule->beta2 >= 0.0 && rule->beta2 < 1.0) || !(rule->eps >= 0.0) ||
+    if (!(rule->beta1 >= 0.0 && rule->beta1 < 1.0 && rule->beta2 >= 0.0 && rule->beta2 < 1.0) || !(rule->eps >= 0.0 && rule->eps <= 1e30) ||
         !(rule->decay >= 0.0) || (!rule->rate && !(rule->lr >= 0.0)) || (rule->norm && !(rule->max_norm >= 0.0)))
-        return abi_fail(HB_BAD_ARGUMENT, "hb_adamw_step: betas in [0, 1), the other numbers >= 0");
+        return abi_fail(HB_BAD_ARGUMENT, "hb_adamw_step: betas in [0, 1), eps in [0, 1e30], the other numbers >= 0");
     if ((rule->rate && bad(rule->rate, 4)) || (rule->norm && bad(rule->norm, 4)))
         return abi_fail(HB_BAD_ARGUMENT, "hb_adamw_step: misaligned rate or norm");
     int64_t chunks = 0;
@@ -393,11 +532,12 @@ extern "C" int hb_adamw_step(int64_t count, void* const* params, const void* con
     count_launches(1);
     cudaError_t e = cudaGetLastError();
     const Fixed fixed{(float)rule->beta1, (float)rule->beta2, (float)(1.0 - rule->beta1), (float)(1.0 - rule->beta2), (float)rule->eps};
+    int64_t total = 0;
+    for (int64_t i = 0; i < count; ++i) total += sizes[i];
+    const auto go = bits == 8 ? (count <= kFew ? run<8, kFew> : run<8, kMany>) : (count <= kFew ? run<32, kFew> : run<32, kMany>);
     if (e == cudaSuccess)
-        e = bits == 8 ? run<8, kMost8, Scales>(count, params, grads, first, second, first_scale, second_scale, master, sizes, types,
-                                               grad_types, fixed, shared, st)
-                      : run<32, kMost32, NoScales>(count, params, grads, first, second, first_scale, second_scale, master, sizes, types,
-                                                   grad_types, fixed, shared, st);
+        e = go(count, params, grads, first, second, first_scale, second_scale, master, sizes, types, grad_types,
+               total >= kLongLeast ? kLongChunk : kChunk, fixed, shared, st);
     return finish(e, what);
 }
 
@@ -417,11 +557,11 @@ extern "C" int hb_adamw_moments(int64_t count, const void* const* first, const v
             return abi_fail(HB_BAD_ARGUMENT, "hb_adamw_moments: null or misaligned pointer of a tensor");
     }
     const auto st = static_cast<cudaStream_t>(stream);
-    for (int64_t from = 0; from < count; from += kMost8) {
+    for (int64_t from = 0; from < count; from += kHeld) {
         Held l;
         l.count = 0;
         int32_t at = 0;
-        for (int64_t i = from; i < std::min(count, from + kMost8); ++i) {
+        for (int64_t i = from; i < std::min(count, from + kHeld); ++i) {
             if (sizes[i] == 0) continue;
             const int t = l.count++;
             l.first[t] = static_cast<const uint8_t*>(first[i]);
@@ -435,7 +575,6 @@ extern "C" int hb_adamw_moments(int64_t count, const void* const* first, const v
             at += (int32_t)((sizes[i] + kChunk - 1) / kChunk);
         }
         if (l.count == 0) continue;
-        l.chunk[l.count] = at;
         moments_kernel<<<(unsigned)at, kThreads, 0, st>>>(l);
         count_launches(1);
     }

@@ -3,9 +3,9 @@
 //   t = x + residual,  r = 1 / sqrt(mean(t^2) + eps),  y = t r w
 //   dx = r w dy - x r^3 mean(w dy x) + dtotal,  dw = sum over rows of dy x r
 //
-// Bound by HBM: each array passes once.  A row is held in the registers of 32, 128 or 512 threads (2 or 4 vectors
-// of 16 bytes each), so its sum and its scaling need one read; rows wider than 512 threads hold are read a second
-// time, from L2.  The gradient of w is summed over a block's rows in registers, every block leaves one row of fp32
+// Bound by HBM: each array passes once.  A row is held in the registers of 8 to 512 threads, 16 columns each (32 above
+// 8192), so its sum and its scaling need one read, and the next row comes meanwhile; rows of more than 16384 columns
+// are read a second time, from L2.  The gradient of w is summed over a block's rows in registers, every block leaves one row of fp32
 // partial sums, and a second launch adds those in order: no atomics, the result does not depend on the launch.
 //
 // Sums are fp32; t is rounded for the output alone.  In 8 bits 32 columns share a power of two: the exponent is that
@@ -48,15 +48,16 @@ struct Forward {
     int width, weight_type, weight_whole;
     float eps;
     void *y, *total;
+    int turns;
     uint8_t *codes, *scales;
 };
 
-// Sum over the THREADS threads of a row (a warp, or a whole block).
+// Sum over the THREADS threads of a row: a part of a warp, a warp, or a whole block.
 template <int THREADS>
 __device__ __forceinline__ float row_sum(float v, float* shared) {
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-    if (THREADS == 32) return v;
+    for (int d = (THREADS < 32 ? THREADS : 32) / 2; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    if (THREADS <= 32) return v;
     __syncthreads();  // the last row's sums have been read
     if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
     __syncthreads();
@@ -97,8 +98,12 @@ __device__ __forceinline__ void write_8bit(const Forward& p, int64_t r, int c, c
     uint32_t most = 0;
 #pragma unroll
     for (int j = 0; j < N; ++j) most = max(most, there ? __float_as_uint(fabsf(y[j])) : 0u);
+    if (N == 1) {
+        most = __reduce_max_sync(0xffffffffu, most);
+    } else {
 #pragma unroll
-    for (int d = 1; d < kGroup / N; d <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+        for (int d = 1; d < kGroup / N; d <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+    }
     if (!there) return;
     const int byte = scale_byte(most);
     const float inverse = byte == 0 ? 0.0f : byte == 255 ? __int_as_float(0x7fc00000)
@@ -110,131 +115,180 @@ __device__ __forceinline__ void write_8bit(const Forward& p, int64_t r, int c, c
     if (c % kGroup == 0) p.scales[r * ((p.width + kGroup - 1) / kGroup) + c / kGroup] = (uint8_t)byte;
 }
 
-// HELD vectors a thread; THREADS threads a row, a block of max(128, THREADS).  HELD 0: rows wider than that, a block a row,
-// read twice.
-template <typename T, int VB, int THREADS, int HELD, bool BITS8>
-__global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS) forward_kernel(const __grid_constant__ Forward p) {
+// A row's raw values, COLUMNS of each thread; the next row's come while this one is summed.
+template <typename T, int VB, int THREADS, int COLUMNS>
+struct Raw {
     using V = rows::Vec<T, VB>;
-    constexpr int BLOCK = THREADS < 128 ? 128 : THREADS, ROWS = BLOCK / THREADS;
-    __shared__ float shared[THREADS / 32];
-    const int t = threadIdx.x % THREADS;
-    const int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS;
-    if (r >= p.rows) return;  // whole warps; with more than a warp a row there is one row a block
-    const T* x = static_cast<const T*>(p.x) + r * p.x_row;
-    const T* residual = p.residual ? static_cast<const T*>(p.residual) + r * p.residual_row : nullptr;
-    T* y = static_cast<T*>(p.y) + r * p.width;
-    T* total = p.total ? static_cast<T*>(p.total) + r * p.width : nullptr;
-    auto load = [&](float (&f)[V::N], int c) {
-        V a, b;
-        a.load_once(x + c);
-        if (residual) b.load_once(residual + c);
-#pragma unroll
-        for (int j = 0; j < V::N; ++j) f[j] = residual ? rows::to_float(a.v[j]) + rows::to_float(b.v[j]) : rows::to_float(a.v[j]);
-    };
-    auto keep = [&](const float (&f)[V::N], int c) {
-        V o;
-#pragma unroll
-        for (int j = 0; j < V::N; ++j) o.v[j] = rows::from_float<T>(f[j]);
-        o.store_once(total + c);
-    };
-    auto write = [&](const float (&f)[V::N], int c, float scale, bool there) {
-        float w[V::N], out[V::N];
-        if (there) load_weights(w, p, c);
-#pragma unroll
-        for (int j = 0; j < V::N; ++j) out[j] = there ? f[j] * scale * w[j] : 0.0f;
-        if constexpr (BITS8) {
-            write_8bit<V::N>(p, r, c, out, there);
-        } else if (there) {
-            V o;
-#pragma unroll
-            for (int j = 0; j < V::N; ++j) o.v[j] = rows::from_float<T>(out[j]);
-            o.store_once(y + c);
-        }
-    };
-    float squares = 0.0f;
-    if constexpr (HELD > 0) {
-        float f[HELD][V::N];
-        V a[HELD], b[HELD];
-#pragma unroll
-        for (int i = 0; i < HELD; ++i) {  // all loads first
-            const int c = (i * THREADS + t) * V::N;
-            if (c < p.width) {
-                a[i].load_once(x + c);
-                if (residual) b[i].load_once(residual + c);
-            } else {
-                a[i].zero();
-                b[i].zero();
-            }
-        }
+    static constexpr int HELD = COLUMNS / V::N;
+    V v[HELD];
+    __device__ __forceinline__ void load(const T* row, int width, bool there) {
 #pragma unroll
         for (int i = 0; i < HELD; ++i) {
-            const int c = (i * THREADS + t) * V::N;
+            const int c = (i * THREADS + (int)threadIdx.x % THREADS) * V::N;
+            if (there && c < width) v[i].load_once(row + c);
+            else v[i].zero();
+        }
+    }
+};
+
+constexpr int block_of(int threads) { return threads < 128 ? 128 : threads; }
+
+// THREADS threads hold a row, COLUMNS each; a block takes some rows in order (`turns`).
+template <typename T, int VB, int THREADS, int COLUMNS, bool ADD, bool BITS8>
+__global__ void __launch_bounds__(block_of(THREADS)) forward_kernel(const __grid_constant__ Forward p) {
+    using R = Raw<T, VB, THREADS, COLUMNS>;
+    using V = typename R::V;
+    constexpr int ROWS = block_of(THREADS) / THREADS;
+    __shared__ float shared[THREADS < 32 ? 1 : THREADS / 32];
+    const int t = threadIdx.x % THREADS;
+    const int64_t step = ROWS;
+    const int64_t base = (int64_t)blockIdx.x * ROWS * p.turns;
+    const int64_t end = min(p.rows, base + ROWS * p.turns);
+    const T *x = static_cast<const T*>(p.x), *residual = static_cast<const T*>(p.residual);
+    R a, b;
+    int64_t r = base + threadIdx.x / THREADS;
+    a.load(x + r * p.x_row, p.width, r < end);
+    if (ADD) b.load(residual + r * p.residual_row, p.width, r < end);
+    // every thread of a block makes the same turns: the rows of a warp or block are summed together
+    for (int64_t first = base; first < end; first += step, r += step) {
+        const bool there = r < end;
+        float f[R::HELD][V::N], squares = 0.0f;
+#pragma unroll
+        for (int i = 0; i < R::HELD; ++i)
 #pragma unroll
             for (int j = 0; j < V::N; ++j) {
-                f[i][j] = residual ? rows::to_float(a[i].v[j]) + rows::to_float(b[i].v[j]) : rows::to_float(a[i].v[j]);
+                f[i][j] = rows::to_float(a.v[i].v[j]);
+                if (ADD) f[i][j] += rows::to_float(b.v[i].v[j]);
                 squares = fmaf(f[i][j], f[i][j], squares);
             }
-            if (total && c < p.width) keep(f[i], c);
-        }
-        const float scale = 1.0f / sqrtf(row_sum<THREADS>(squares, shared) / (float)p.width + p.eps);
+        const int64_t next = r + step;
+        a.load(x + next * p.x_row, p.width, next < end);
+        if (ADD) b.load(residual + next * p.residual_row, p.width, next < end);
+        if (ADD && p.total && there) {
 #pragma unroll
-        for (int i = 0; i < HELD; ++i) {
-            const int c = (i * THREADS + t) * V::N;
-            if (i * THREADS * V::N < p.width) write(f[i], c, scale, c < p.width);
-        }
-    } else {
-        float f[V::N];
-        for (int c = t * V::N; c < p.width; c += THREADS * V::N) {
-            load(f, c);
+            for (int i = 0; i < R::HELD; ++i) {
+                const int c = (i * THREADS + t) * V::N;
+                V o;
 #pragma unroll
-            for (int j = 0; j < V::N; ++j) squares = fmaf(f[j], f[j], squares);
-        }
-        const float scale = 1.0f / sqrtf(row_sum<THREADS>(squares, shared) / (float)p.width + p.eps);
-        for (int from = 0; from < p.width; from += THREADS * V::N) {
-            const int c = from + t * V::N;
-            if (c < p.width) {
-                load(f, c);
-                if (total) keep(f, c);
+                for (int j = 0; j < V::N; ++j) o.v[j] = rows::from_float<T>(f[i][j]);
+                if (c < p.width) o.store_once(static_cast<T*>(p.total) + r * p.width + c);
             }
-            write(f, c, scale, c < p.width);
+        }
+        const float scale = 1.0f / sqrtf(row_sum<THREADS>(squares, shared) / (float)p.width + p.eps);
+#pragma unroll
+        for (int i = 0; i < R::HELD; ++i) {
+            const int c = (i * THREADS + t) * V::N;
+            if (i * THREADS * V::N >= p.width) break;  // the same for all
+            const bool inside = there && c < p.width;
+            float w[V::N];
+            if (inside) load_weights(w, p, c);
+#pragma unroll
+            for (int j = 0; j < V::N; ++j) f[i][j] = inside ? f[i][j] * scale * w[j] : 0.0f;
+            if constexpr (BITS8) {
+                write_8bit<V::N>(p, r, c, f[i], inside);
+            } else if (inside) {
+                V o;
+#pragma unroll
+                for (int j = 0; j < V::N; ++j) o.v[j] = rows::from_float<T>(f[i][j]);
+                o.store_once(static_cast<T*>(p.y) + r * p.width + c);
+            }
         }
     }
 }
 
-template <typename T, int VB, int THREADS, int HELD>
+// Rows wider than 512 threads hold: a block a row, read twice.
+template <typename T, int VB, bool BITS8>
+__global__ void __launch_bounds__(512) wide_forward_kernel(const __grid_constant__ Forward p) {
+    using V = rows::Vec<T, VB>;
+    __shared__ float shared[16];
+    const int64_t r = blockIdx.x;
+    const T* x = static_cast<const T*>(p.x) + r * p.x_row;
+    const T* residual = p.residual ? static_cast<const T*>(p.residual) + r * p.residual_row : nullptr;
+    auto load = [&](float (&f)[V::N], int c) {
+        V a, b;
+        a.load(x + c);
+        if (residual) b.load(residual + c);
+#pragma unroll
+        for (int j = 0; j < V::N; ++j) f[j] = residual ? rows::to_float(a.v[j]) + rows::to_float(b.v[j]) : rows::to_float(a.v[j]);
+    };
+    float squares = 0.0f, f[V::N];
+    for (int c = threadIdx.x * V::N; c < p.width; c += 512 * V::N) {
+        load(f, c);
+#pragma unroll
+        for (int j = 0; j < V::N; ++j) squares = fmaf(f[j], f[j], squares);
+    }
+    const float scale = 1.0f / sqrtf(row_sum<512>(squares, shared) / (float)p.width + p.eps);
+    for (int from = 0; from < p.width; from += 512 * V::N) {
+        const int c = from + threadIdx.x * V::N;
+        const bool inside = c < p.width;
+        V o;
+        float w[V::N];
+        if (inside) {
+            load(f, c);
+            load_weights(w, p, c);
+#pragma unroll
+            for (int j = 0; j < V::N; ++j) o.v[j] = rows::from_float<T>(f[j]);
+            if (p.total) o.store_once(static_cast<T*>(p.total) + r * p.width + c);
+        }
+#pragma unroll
+        for (int j = 0; j < V::N; ++j) f[j] = inside ? f[j] * scale * w[j] : 0.0f;
+        if constexpr (BITS8) {
+            write_8bit<V::N>(p, r, c, f, inside);
+        } else if (inside) {
+#pragma unroll
+            for (int j = 0; j < V::N; ++j) o.v[j] = rows::from_float<T>(f[j]);
+            o.store_once(static_cast<T*>(p.y) + r * p.width + c);
+        }
+    }
+}
+
+template <typename T, int VB, int THREADS, int COLUMNS, bool BITS8>
 void launch_forward(const Forward& p, cudaStream_t st) {
-    constexpr int BLOCK = THREADS < 128 ? 128 : THREADS, ROWS = BLOCK / THREADS;
-    const unsigned blocks = (unsigned)((p.rows + ROWS - 1) / ROWS);
-    if (p.codes) forward_kernel<T, VB, THREADS, HELD, true><<<blocks, BLOCK, 0, st>>>(p);
-    else forward_kernel<T, VB, THREADS, HELD, false><<<blocks, BLOCK, 0, st>>>(p);
+    constexpr int BLOCK = block_of(THREADS), ROWS = BLOCK / THREADS;
+    if constexpr (COLUMNS == 0) {
+        wide_forward_kernel<T, VB, BITS8><<<(unsigned)p.rows, 512, 0, st>>>(p);
+    } else {
+        // A block's rows come one after the other in memory: enough to hide its start, few enough that blocks which start
+        // in order keep HBM's pages open (65536 x 2048 bf16 with residual 172 us at 1, 160 at 2, 164 at 4, 183 where
+        // resident blocks stride; without residual 103, 95, 92 and 93; 32768 x 2048 fp32 157, 161, 162 and 171).
+        Forward q = p;
+        q.turns = sizeof(T) == 4 ? 1 : p.residual ? 2 : 4;
+        while (q.turns > 1 && p.rows < (int64_t)ROWS * q.turns * 148 * 8) q.turns /= 2;  // few rows: all SMs first
+        const unsigned blocks = (unsigned)((p.rows + ROWS * q.turns - 1) / (ROWS * q.turns));
+        if (p.residual) forward_kernel<T, VB, THREADS, COLUMNS, true, BITS8><<<blocks, BLOCK, 0, st>>>(q);
+        else forward_kernel<T, VB, THREADS, COLUMNS, false, BITS8><<<blocks, BLOCK, 0, st>>>(q);
+    }
 }
 
 // ---------------------------------------------------------------- reading 8 bits back
-template <typename TO>
+// A warp a row: 16 columns a lane where rows lie on 16 bytes, else one.
+template <typename TO, bool VECTORS>
 __global__ void __launch_bounds__(256) read_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                                                   int64_t rows, int width, int vector, TO* __restrict__ out) {
-    const int groups = (width + kGroup - 1) / kGroup;
-    const int64_t n = rows * width;
-    if (vector) {  // 16 codes: half a group
-        for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 16; i < n; i += (int64_t)gridDim.x * 256 * 16) {
-            rows::Vec<uint8_t, 16> c;
-            c.load_once(codes + i);
-            const int64_t r = i / width;
-            const float s = scale_value(scales[r * groups + (int)(i - r * width) / kGroup]);
-            constexpr int V = 16 / (int)sizeof(TO);
+                                                   int64_t rows, int width, TO* __restrict__ out) {
+    const int groups = (width + kGroup - 1) / kGroup, lane = threadIdx.x & 31;
+    const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (r >= rows) return;
+    codes += r * width;
+    scales += r * groups;
+    out += r * width;
+    if (VECTORS) {
+        constexpr int V = 16 / (int)sizeof(TO);
+#pragma unroll 2
+        for (int c = lane * 16; c < width; c += 512) {
+            rows::Vec<uint8_t, 16> in;
+            in.load_once(codes + c);
+            const float s = scale_value(scales[c / kGroup]);
 #pragma unroll
             for (int q = 0; q < 16 / V; ++q) {
                 rows::Vec<TO, 16> o;
 #pragma unroll
-                for (int j = 0; j < V; ++j) o.v[j] = rows::from_float<TO>(of_code(c.v[q * V + j]) * s);
-                o.store(out + i + q * V);
+                for (int j = 0; j < V; ++j) o.v[j] = rows::from_float<TO>(of_code(in.v[q * V + j]) * s);
+                o.store(out + c + q * V);
             }
         }
-        return;
-    }
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / width;
-        out[i] = rows::from_float<TO>(of_code(codes[i]) * scale_value(scales[r * groups + (int)(i - r * width) / kGroup]));
+    } else {
+#pragma unroll 4
+        for (int c = lane; c < width; c += 32) out[c] = rows::from_float<TO>(of_code(codes[c]) * scale_value(scales[c / kGroup]));
     }
 }
 
@@ -248,15 +302,15 @@ struct Backward {
     float *partial, *stats;  // partial: [blocks][width]; stats: [rows][2] of wide rows
 };
 
-// One of w dy x and x^2 summed, two at once.
+// Sums of w dy x and x^2 at once.
 template <int THREADS>
 __device__ __forceinline__ float2 row_sums(float a, float b, float2* shared) {
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
+    for (int d = (THREADS < 32 ? THREADS : 32) / 2; d > 0; d >>= 1) {
         a += __shfl_xor_sync(0xffffffffu, a, d);
         b += __shfl_xor_sync(0xffffffffu, b, d);
     }
-    if (THREADS == 32) return make_float2(a, b);
+    if (THREADS <= 32) return make_float2(a, b);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = make_float2(a, b);
     __syncthreads();
@@ -266,18 +320,20 @@ __device__ __forceinline__ float2 row_sums(float a, float b, float2* shared) {
     return s;
 }
 
+// Resident blocks an SM: what the registers of a thread's columns leave (128 a thread).
+constexpr int resident(int threads) { return threads >= 512 ? 1 : threads == 256 ? 2 : 4; }
+
 // Rows held in registers; a block strides over the rows and keeps its sums for dw.  Up to 16 columns a thread the
-// weight's values are held too, above they come from L1 for each row.
-// Resident blocks an SM: what the registers of a thread's columns leave (102, 170, 128 a thread).
-constexpr int resident(int threads, int columns) { return threads >= 512 ? 1 : columns <= 16 ? 5 : 3; }
-template <typename T, int VB, int THREADS, int HELD>
-__global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS, resident(THREADS, HELD * VB / (int)sizeof(T)))
-    backward_kernel(const __grid_constant__ Backward p) {
-    using V = rows::Vec<T, VB>;
-    constexpr int BLOCK = THREADS < 128 ? 128 : THREADS, ROWS = BLOCK / THREADS;
-    constexpr bool KEEP = HELD * V::N <= 16;
-    __shared__ float2 shared[THREADS / 32];
-    __shared__ float joined[ROWS > 1 ? THREADS * HELD * V::N : 1];
+// weight's values are held too, and rows of 16-byte vectors of 16-bit values, which take half the registers, come while
+// the row before is summed (65536 x 2048 bf16 219 -> 186 us; in fp32 it spills, 208 -> 225).
+template <typename T, int VB, int THREADS, int COLUMNS>
+__global__ void __launch_bounds__(block_of(THREADS), resident(THREADS)) backward_kernel(const __grid_constant__ Backward p) {
+    using R = Raw<T, VB, THREADS, COLUMNS>;
+    using V = typename R::V;
+    constexpr int ROWS = block_of(THREADS) / THREADS, HELD = R::HELD;
+    constexpr bool KEEP = COLUMNS <= 16, AHEAD = KEEP && VB == 16 && sizeof(T) == 2;
+    __shared__ float2 shared[THREADS < 32 ? 1 : THREADS / 32];
+    __shared__ float joined[ROWS > 1 ? THREADS * COLUMNS : 1];
     const int t = threadIdx.x % THREADS, mine = threadIdx.x / THREADS;
     float dw[HELD][V::N], kept[KEEP ? HELD : 1][V::N];
 #pragma unroll
@@ -290,23 +346,22 @@ __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS, resident(THREAD
         }
         if (KEEP && c < p.width) load_weights(kept[i], p, c);
     }
-    for (int64_t r = (int64_t)blockIdx.x * ROWS + mine; r < p.rows; r += (int64_t)gridDim.x * ROWS) {
-        const T* x = static_cast<const T*>(p.x) + r * p.x_row;
-        const T* dy = static_cast<const T*>(p.dy) + r * p.dy_row;
-        const T* dtotal = p.dtotal && p.dx ? static_cast<const T*>(p.dtotal) + r * p.dtotal_row : nullptr;
-        V a[HELD], g[HELD], d[HELD];
-#pragma unroll
-        for (int i = 0; i < HELD; ++i) {
-            const int c = (i * THREADS + t) * V::N;
-            if (c < p.width) {
-                a[i].load_once(x + c);
-                g[i].load_once(dy + c);
-                if (dtotal) d[i].load_once(dtotal + c);
-            } else {
-                a[i].zero();
-                g[i].zero();
-            }
-        }
+    const T *x = static_cast<const T*>(p.x), *dy = static_cast<const T*>(p.dy);
+    const T* dtotal = p.dx ? static_cast<const T*>(p.dtotal) : nullptr;
+    R a, g, d;
+    const int64_t step = (int64_t)gridDim.x * ROWS;
+    int64_t r = (int64_t)blockIdx.x * ROWS + mine;
+    auto fetch = [&](R& ra, R& rg, R& rd, int64_t at) {
+        const bool there = at < p.rows;
+        ra.load(x + at * p.x_row, p.width, there);
+        rg.load(dy + at * p.dy_row, p.width, there);
+        if (dtotal) rd.load(dtotal + at * p.dtotal_row, p.width, there);
+    };
+    if (AHEAD) fetch(a, g, d, r);
+    for (int64_t first = (int64_t)blockIdx.x * ROWS; first < p.rows; first += step, r += step) {
+        R a_next, g_next, d_next;
+        if (AHEAD) fetch(a_next, g_next, d_next, r + step);
+        else fetch(a, g, d, r);
         float squares = 0.0f, along = 0.0f;
 #pragma unroll
         for (int i = 0; i < HELD; ++i) {
@@ -315,31 +370,34 @@ __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS, resident(THREAD
             if (!KEEP && c < p.width) load_weights(w, p, c);
 #pragma unroll
             for (int j = 0; j < V::N; ++j) {
-                const float xf = rows::to_float(a[i].v[j]), wj = KEEP ? kept[i][j] : c < p.width ? w[j] : 0.0f;
+                const float xf = rows::to_float(a.v[i].v[j]), wj = KEEP ? kept[i][j] : c < p.width ? w[j] : 0.0f;
                 squares = fmaf(xf, xf, squares);
-                along = fmaf(wj * rows::to_float(g[i].v[j]), xf, along);
+                along = fmaf(wj * rows::to_float(g.v[i].v[j]), xf, along);
             }
         }
-        const float2 sums = row_sums<THREADS>(squares, along, shared);
-        const float inverse = 1.0f / sqrtf(sums.x / (float)p.width + p.eps);
-        const float back = inverse * inverse * inverse * (sums.y / (float)p.width);
+        const float2 sums = row_sums<THREADS>(along, squares, shared);
+        const float inverse = 1.0f / sqrtf(sums.y / (float)p.width + p.eps);
+        const float back = inverse * inverse * inverse * (sums.x / (float)p.width);
+        if (r < p.rows) {
 #pragma unroll
-        for (int i = 0; i < HELD; ++i) {
-            const int c = (i * THREADS + t) * V::N;
-            if (c >= p.width) continue;
-            float w[V::N];
-            if (!KEEP) load_weights(w, p, c);
-            V o;
+            for (int i = 0; i < HELD; ++i) {
+                const int c = (i * THREADS + t) * V::N;
+                if (c >= p.width) continue;
+                float w[V::N];
+                if (!KEEP) load_weights(w, p, c);
+                V o;
 #pragma unroll
-            for (int j = 0; j < V::N; ++j) {
-                const float xf = rows::to_float(a[i].v[j]), gf = rows::to_float(g[i].v[j]);
-                dw[i][j] = fmaf(gf * xf, inverse, dw[i][j]);
-                float v = fmaf(inverse, (KEEP ? kept[i][j] : w[j]) * gf, -xf * back);
-                if (dtotal) v += rows::to_float(d[i].v[j]);
-                o.v[j] = rows::from_float<T>(v);
+                for (int j = 0; j < V::N; ++j) {
+                    const float xf = rows::to_float(a.v[i].v[j]), gf = rows::to_float(g.v[i].v[j]);
+                    dw[i][j] = fmaf(gf * xf, inverse, dw[i][j]);
+                    float v = fmaf(inverse, (KEEP ? kept[i][j] : w[j]) * gf, -xf * back);
+                    if (dtotal) v += rows::to_float(d.v[i].v[j]);
+                    o.v[j] = rows::from_float<T>(v);
+                }
+                if (p.dx) o.store_once(static_cast<T*>(p.dx) + r * p.width + c);
             }
-            if (p.dx) o.store_once(static_cast<T*>(p.dx) + r * p.width + c);
         }
+        if (AHEAD) a = a_next, g = g_next, d = d_next;
     }
     if (!p.partial) return;
     float* to = p.partial + (int64_t)blockIdx.x * p.width;
@@ -356,7 +414,7 @@ __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS, resident(THREAD
                 }
         }
         __syncthreads();
-        for (int c = threadIdx.x; c < p.width; c += BLOCK) to[c] = joined[c];
+        for (int c = threadIdx.x; c < p.width; c += block_of(THREADS)) to[c] = joined[c];
     } else {
 #pragma unroll
         for (int i = 0; i < HELD; ++i) {
@@ -444,22 +502,24 @@ __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ par
     }
 }
 
-// Threads and vectors a row: the smallest form that holds it.  A warp holds 2 vectors a lane, so that short rows go four
-// to a block; above, 2 and then 4 a thread.
-template <typename F>
-void for_width(int64_t vectors, F&& f) {
-    if (vectors <= 64) f(rows::Bytes<32>{}, rows::Bytes<2>{});
-    else if (vectors <= 256) f(rows::Bytes<128>{}, rows::Bytes<2>{});
-    else if (vectors <= 512) f(rows::Bytes<128>{}, rows::Bytes<4>{});
-    else if (vectors <= 2048) f(rows::Bytes<512>{}, rows::Bytes<4>{});
+// Threads a row and columns a thread: the smallest form that holds the row.  Rows of up to 128 columns lie 16 to a
+// block, where a vector is a quarter of a scale's group at least.
+template <int N, typename F>
+void for_width(int64_t width, F&& f) {
+    if (N >= 4 && width <= 128) f(rows::Bytes<N >= 4 ? 8 : 32>{}, rows::Bytes<16>{});
+    else if (width <= 512) f(rows::Bytes<32>{}, rows::Bytes<16>{});
+    else if (width <= 2048) f(rows::Bytes<128>{}, rows::Bytes<16>{});
+    else if (width <= 4096) f(rows::Bytes<256>{}, rows::Bytes<16>{});
+    else if (width <= 8192) f(rows::Bytes<512>{}, rows::Bytes<16>{});
+    else if (width <= 16384) f(rows::Bytes<512>{}, rows::Bytes<32>{});
     else f(rows::Bytes<512>{}, rows::Bytes<0>{});
 }
-constexpr int64_t kMostHeld = 2048;  // vectors of a row that for_width holds
-constexpr int kParts = 148 * 8;      // most blocks that sum dw
+constexpr int64_t kMostHeld = 16384;  // columns of a row that for_width holds
+constexpr int kParts = 148 * 8;       // most blocks that sum dw
 
 // Blocks that sum dw: as many as are resident, each with at least 4 turns.
-inline int parts_of(int64_t rows, int threads, int columns) {
-    const int64_t side = threads < 128 ? 128 / threads : 1, blocks = 148 * resident(threads, columns);
+inline int parts_of(int64_t rows, int threads) {
+    const int64_t side = block_of(threads) / threads, blocks = 148 * resident(threads);
     return (int)std::max<int64_t>(1, std::min(blocks, (rows + 4 * side - 1) / (4 * side)));
 }
 
@@ -507,7 +567,7 @@ extern "C" int hb_rms_norm(int type, const void* x, int64_t x_stride, const void
         rows::address_bits(weight) % rows::type_bytes(weight_type) || (codes ? !scales || y : !y) || rows::address_bits(y) % size ||
         rows::address_bits(total) % size)
         return abi_fail(HB_BAD_ARGUMENT, "hb_rms_norm: null or misaligned pointer, or bad stride");
-    Forward p{x, residual, weight, x_stride, residual_stride, rows, (int)width, weight_type, rows::address_bits(weight) % 16 == 0, (float)eps, y, total,
+    Forward p{x, residual, weight, x_stride, residual_stride, rows, (int)width, weight_type, rows::address_bits(weight) % 16 == 0, (float)eps, y, total, 1,
               static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales)};
     uint64_t bits = rows::address_bits(x) | rows::address_bits(residual) | rows::address_bits(y) | rows::address_bits(total) |
                     (uint64_t)(width | (rows > 1 ? x_stride : 0) | (rows > 1 && residual ? residual_stride : 0)) * size;
@@ -516,8 +576,10 @@ extern "C" int hb_rms_norm(int type, const void* x, int64_t x_stride, const void
     for_vectors(type, vector_of(bits, type), [&](auto t, auto vb) {
         using T = decltype(t);
         constexpr int VB = decltype(vb)::value, N = VB / (int)sizeof(T);
-        for_width((width + N - 1) / N, [&](auto threads, auto held) {
-            launch_forward<T, VB, decltype(threads)::value, decltype(held)::value>(p, st);
+        for_width<N>(width, [&](auto threads, auto columns) {
+            constexpr int THREADS = decltype(threads)::value, COLUMNS = decltype(columns)::value;
+            if (p.codes) launch_forward<T, VB, THREADS, COLUMNS, true>(p, st);
+            else launch_forward<T, VB, THREADS, COLUMNS, false>(p, st);
         });
     });
     count_launches(1);
@@ -532,13 +594,13 @@ extern "C" int hb_rows_of_8bit(const void* codes, const void* scales, int64_t ro
     if (!codes || !scales || !out || rows::address_bits(out) % rows::type_bytes(out_type))
         return abi_fail(HB_BAD_ARGUMENT, "hb_rows_of_8bit: null or misaligned pointer");
     const bool vector = width % 16 == 0 && ((rows::address_bits(codes) | rows::address_bits(out)) & 15) == 0;
-    const int64_t items = (rows * width + (vector ? 16 : 1) - 1) / (vector ? 16 : 1);
-    const unsigned blocks = (unsigned)std::min<int64_t>((items + 255) / 256, 148 * 16);
+    const unsigned blocks = (unsigned)((rows + 7) / 8);
     const auto st = static_cast<cudaStream_t>(stream);
     const auto *c = static_cast<const uint8_t*>(codes), *s = static_cast<const uint8_t*>(scales);
     rows::for_type(out_type, 16, [&](auto t, auto) {
         using T = decltype(t);
-        read_kernel<T><<<blocks, 256, 0, st>>>(c, s, rows, (int)width, vector, static_cast<T*>(out));
+        if (vector) read_kernel<T, true><<<blocks, 256, 0, st>>>(c, s, rows, (int)width, static_cast<T*>(out));
+        else read_kernel<T, false><<<blocks, 256, 0, st>>>(c, s, rows, (int)width, static_cast<T*>(out));
     });
     count_launches(1);
     return finish(cudaGetLastError(), "hb_rows_of_8bit");
@@ -546,7 +608,7 @@ extern "C" int hb_rows_of_8bit(const void* codes, const void* scales, int64_t ro
 
 extern "C" size_t hb_rms_norm_grad_workspace(int64_t rows, int64_t width) {
     if (rows < 0 || rows > INT32_MAX || width < 1 || width > (1 << 30)) return 0;
-    // the blocks of any vector size, and two sums a row of those that none holds
+    // the blocks' sums, and two sums a row of those that no block holds
     const size_t sums = width > kMostHeld ? (size_t)rows * 2 * sizeof(float) : 0;
     return (sums + 255) / 256 * 256 + (size_t)std::min<int64_t>(kParts, std::max<int64_t>(rows, 1)) * width * sizeof(float);
 }
@@ -583,20 +645,19 @@ extern "C" int hb_rms_norm_grad(int type, const void* dy, int64_t dy_stride, con
     for_vectors(type, vector_of(bits, type), [&](auto t, auto vb) {
         using T = decltype(t);
         constexpr int VB = decltype(vb)::value, N = VB / (int)sizeof(T);
-        const int64_t vectors = (width + N - 1) / N;
-        if (vectors <= kMostHeld) {
-            for_width(vectors, [&](auto threads, auto held) {
-                constexpr int THREADS = decltype(threads)::value, HELD = decltype(held)::value;
-                if constexpr (HELD > 0) {
-                    parts = parts_of(rows, THREADS, HELD * N);
-                    backward_kernel<T, VB, THREADS, HELD><<<parts, THREADS < 128 ? 128 : THREADS, 0, st>>>(p);
+        if (width <= kMostHeld) {
+            for_width<N>(width, [&](auto threads, auto columns) {
+                constexpr int THREADS = decltype(threads)::value, COLUMNS = decltype(columns)::value;
+                if constexpr (COLUMNS > 0) {
+                    parts = parts_of(rows, THREADS);
+                    backward_kernel<T, VB, THREADS, COLUMNS><<<parts, block_of(THREADS), 0, st>>>(p);
                 }
             });
             count_launches(1);
             return;
         }
         wide_sums_kernel<T, VB><<<(unsigned)rows, 512, 0, st>>>(p);
-        const unsigned columns = (unsigned)((vectors + 255) / 256);
+        const unsigned columns = (unsigned)((width + 256 * N - 1) / (256 * N));
         parts = (int)std::min<int64_t>(rows, std::max<int64_t>(1, 148 * 8 / columns));
         wide_kernel<T, VB><<<dim3(columns, parts), 256, 0, st>>>(p);
         count_launches(2);
