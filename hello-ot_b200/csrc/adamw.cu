@@ -6,13 +6,18 @@
 // Two launches over one list of chunks in the kernel's parameters: one thread counts the step and works out what
 // all elements share (in fp64: t, the bias corrections, f), then a warp takes a block of 256 elements, 8 a lane.
 // The second launch starts while the first runs and waits for it when its first loads are on their way
-// (programmatic dependent launch).  Bound by HBM: every array passes once.
+// (programmatic dependent launch).  Bound by HBM: every array passes once.  On a B200 400 million bf16 parameters with
+// masters and 8-bit states take 981 us (6.5 TB/s), 200 million in fp32 with fp32 states 818 us (6.8 TB/s).
 //
 // 8 bits: e4m3 codes of m and of sqrt(v) with a scale for each 256 elements (largest magnitude / 448).  The root
 // halves v's range of exponents, so e4m3's 2^17 between the largest and the smallest code are 2^34 of v; a v above
 // zero keeps at least the smallest code, so that no later step divides an m that was kept by a v that was lost.
 // Scales are fp32, not powers of two: a block whose values all shrink by the same factor keeps its codes and
 // shrinks its scale, where rounding each value to its old code would stop v's decay of 0.1 % a step.
+//
+// With 8-bit states a warp computes for longer than its loads take, at 51 instructions an element; loads held in registers
+// for the next block left too few warps (3 blocks of threads an SM, 1.55 ms).  So bulk copies bring the next stages
+// into a ring of three in shared memory.  fp32 states compute less: there the next block in registers suffices.
 //
 // m and v are rounded to fp32 at every operation as it is written, and their codes are those of the correctly rounded
 // quotients, so that any fp32 program computes the same states bit for bit.  The change of p takes the approximate
@@ -25,6 +30,7 @@
 
 #include <cuda_fp8.h>
 
+#include "common.cuh"
 #include "internal.h"
 #include "rows.cuh"
 
@@ -32,8 +38,11 @@ namespace hb {
 namespace adamw {
 
 constexpr int kThreads = 256, kBlock = 256;            // kBlock: elements of a scale, a warp's
-constexpr int kChunk = 2048, kLongChunk = 8192;        // elements of a block of threads
-constexpr int64_t kLongLeast = 148 * 8 * (int64_t)kLongChunk;  // elements from which chunks are long
+constexpr int kStage = kThreads / 32 * kBlock;          // elements of a block of threads at a time
+constexpr int kRing = 3;                                // 8-bit states: stages of a block in shared memory
+// Elements of a block of threads: one stage, so that small calls take all SMs, or from kLongLeast elements on several.
+constexpr int kChunk = kStage, kLongChunk = 8192;
+constexpr int64_t kLongLeast = 148 * 8 * (int64_t)kLongChunk;
 constexpr float kLeastBy = 0x1p-63f;                   // least divisor of a change: the root of the least normal v
 constexpr int kFew = 24, kMany = 360;                  // tensors of a launch: 2 KB or 31 KB of parameters
 
@@ -330,7 +339,18 @@ __device__ __forceinline__ void advance(const Chunk<T, TS, TG>& c, uint32_t bloc
     }
 }
 
-// A warp's blocks of the chunk [from, to).
+// The stages of a block's ring: every array's piece of a stage, brought by bulk copies that need neither registers nor
+// warps while they are on their way.
+struct Ring {
+    uint64_t full[kRing], empty[kRing];
+    int abort, status;
+};
+extern __shared__ __align__(128) uint8_t ring_memory[];
+
+template <typename TS, typename TG>
+constexpr int stage_bytes() { return kStage * ((int)sizeof(TS) + (int)sizeof(TG) + 2) + 2 * (kStage / kBlock) * (int)sizeof(float); }
+
+// A block of threads' chunk [from, to).
 template <int BITS, typename T, typename TS, typename TG>
 __device__ __forceinline__ void step_chunk(const Entry& e, int64_t from, int64_t to, const Fixed& fixed, const Shared* shared) {
     constexpr uint32_t kWarps = kThreads / 32;
@@ -346,19 +366,85 @@ __device__ __forceinline__ void step_chunk(const Entry& e, int64_t from, int64_t
     c.second = static_cast<char*>(e.second) + from * (BITS / 8);
     if constexpr (BITS == 8) c.first_scale = e.first_scale + from / kBlock, c.second_scale = e.second_scale + from / kBlock;
     const uint32_t length = (uint32_t)(to - from), whole = e.aligned ? length / kBlock : 0, blocks = (length + kBlock - 1) / kBlock;
-    Lane<BITS, TS, TG> here, next;
+    Shared now;
+    auto read_shared = [&] {
+        asm volatile("griddepcontrol.wait;" ::: "memory");  // also where no block is left: not to end before the launch it overlaps
+        const volatile Shared* const written = shared;
+        now = {written->factor, written->keep, written->rate, written->over_root};
+    };
     uint32_t block = threadIdx.x >> 5;
-    if (block < whole) here.load(c, block);
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // also where no block is left: not to end before the launch it overlaps
-    const volatile Shared* const written = shared;
-    const Shared now{written->factor, written->keep, written->rate, written->over_root};
-    for (; block < whole; block += kWarps) {
-        if (block + kWarps < whole) next.load(c, block + kWarps);
-        advance<BITS, true>(c, block, kBlock, here, fixed, now);
-        here = next;
+    if constexpr (BITS == 8) {
+        const uint32_t stages = whole / kWarps;
+        __shared__ Ring ring;
+        uint8_t* const memory = ring_memory;
+        auto piece = [&](uint32_t stage) {  // the stage's arrays in shared memory
+            uint8_t* at = memory + stage % kRing * stage_bytes<TS, TG>();
+            Chunk<T, TS, TG> r = c;
+            r.source = reinterpret_cast<const TS*>(at);
+            at += kStage * sizeof(TS);
+            r.grad = reinterpret_cast<const TG*>(at);
+            at += kStage * sizeof(TG);
+            r.first = at;
+            r.second = at + kStage;
+            r.first_scale = reinterpret_cast<float*>(at + 2 * kStage);
+            r.second_scale = r.first_scale + kWarps;
+            return r;
+        };
+        auto bring = [&](uint32_t stage) {  // one thread
+            const Chunk<T, TS, TG> r = piece(stage);
+            uint64_t* const bar = &ring.full[stage % kRing];
+            const uint32_t i = stage * kStage;
+            mbar_arrive_expect_tx(bar, stage_bytes<TS, TG>());
+            bulk_load_1d(const_cast<TS*>(r.source), c.source + i, kStage * sizeof(TS), bar);
+            bulk_load_1d(const_cast<TG*>(r.grad), c.grad + i, kStage * sizeof(TG), bar);
+            bulk_load_1d(r.first, static_cast<const uint8_t*>(c.first) + i, kStage, bar);
+            bulk_load_1d(r.second, static_cast<const uint8_t*>(c.second) + i, kStage, bar);
+            bulk_load_1d(r.first_scale, c.first_scale + stage * kWarps, kWarps * sizeof(float), bar);
+            bulk_load_1d(r.second_scale, c.second_scale + stage * kWarps, kWarps * sizeof(float), bar);
+        };
+        if (stages) {
+            if (threadIdx.x == 0) {
+                for (int i = 0; i < kRing; ++i) mbar_init(&ring.full[i], 1), mbar_init(&ring.empty[i], kWarps);
+                ring.abort = ring.status = 0;
+                fence_barrier_init();
+                for (uint32_t stage = 0; stage < min(stages, (uint32_t)kRing); ++stage) bring(stage);
+            }
+            __syncthreads();
+        }
+        read_shared();
+        for (uint32_t stage = 0; stage < stages; ++stage) {
+            const uint32_t slot = stage % kRing, turn = stage / kRing & 1;
+            // a wait that gave up makes the parameters NaN
+            if (!mbar_wait(&ring.full[slot], turn, &ring.abort, &ring.status)) now.rate = __int_as_float(0x7fc00000);
+            Lane<BITS, TS, TG> here;
+            here.load(piece(stage), block);
+            __syncwarp();
+            if ((threadIdx.x & 31) == 0) mbar_arrive(&ring.empty[slot]);
+            advance<BITS, true>(c, stage * kWarps + block, kBlock, here, fixed, now);
+            // refilled a turn late, when the other warps have long read it
+            if (threadIdx.x == 0 && stage > 0 && stage - 1 + kRing < stages) {
+                const uint32_t last = stage - 1;
+                if (mbar_wait(&ring.empty[last % kRing], last / kRing & 1, &ring.abort, &ring.status)) bring(last + kRing);
+            }
+        }
+        for (block += stages * kWarps; block < whole; block += kWarps) {
+            Lane<BITS, TS, TG> here;
+            here.load(c, block);
+            advance<BITS, true>(c, block, kBlock, here, fixed, now);
+        }
+    } else {
+        Lane<BITS, TS, TG> here, next;
+        if (block < whole) here.load(c, block);
+        read_shared();
+        for (; block < whole; block += kWarps) {
+            if (block + kWarps < whole) next.load(c, block + kWarps);
+            advance<BITS, true>(c, block, kBlock, here, fixed, now);
+            here = next;
+        }
     }
     for (; block < blocks; block += kWarps) {
         const int left = (int)(length - block * kBlock) - (int)(threadIdx.x & 31) * 4;  // may be <= 0
+        Lane<BITS, TS, TG> here;
         here.load_some(c, block, left);
         advance<BITS, false>(c, block, left, here, fixed, now);
     }
@@ -442,6 +528,7 @@ int finish(cudaError_t e, const char* what) {
     return e == cudaSuccess ? HB_OK : abi_fail(HB_LAUNCH, std::string(what) + ": " + cudaGetErrorString(e));
 }
 
+constexpr int kMostStage = stage_bytes<float, float>();
 template <int BITS, int MOST>
 cudaError_t run(int64_t count, void* const* params, const void* const* grads, void* const* first, void* const* second,
                 float* const* first_scale, float* const* second_scale, float* const* master, const int64_t* sizes,
@@ -452,6 +539,7 @@ cudaError_t run(int64_t count, void* const* params, const void* const* grads, vo
     for (int64_t from = 0; from < count; from += MOST) {
         l.count = 0;
         int64_t chunks = 0;
+        int ring = 0;  // bytes of a stage
         for (int64_t i = from; i < std::min(count, from + MOST); ++i) {
             if (sizes[i] == 0) continue;
             Entry& e = l.e[l.count++];
@@ -467,7 +555,10 @@ cudaError_t run(int64_t count, void* const* params, const void* const* grads, vo
             e.type = (uint8_t)types[i];
             e.grad_type = (uint8_t)grad_types[i];
             e.aligned = ((rows::address_bits(e.param) | rows::address_bits(e.grad) | rows::address_bits(e.first) |
-                          rows::address_bits(e.second) | rows::address_bits(e.master)) & 15) == 0;
+                          rows::address_bits(e.second) | rows::address_bits(e.master) | rows::address_bits(e.first_scale) |
+                          rows::address_bits(e.second_scale)) & 15) == 0;
+            ring = std::max(ring, kStage * ((e.master ? 4 : rows::type_bytes(e.type)) + rows::type_bytes(e.grad_type) + 2) +
+                                      2 * (kStage / kBlock) * (int)sizeof(float));
             chunks += (sizes[i] + chunk - 1) / chunk;
         }
         if (l.count == 0) continue;
@@ -477,11 +568,14 @@ cudaError_t run(int64_t count, void* const* params, const void* const* grads, vo
         cudaLaunchConfig_t config{};
         config.gridDim = dim3((unsigned)chunks);
         config.blockDim = dim3(kThreads);
+        config.dynamicSmemBytes = BITS == 8 ? (size_t)kRing * ring : 0;
         config.stream = st;
         config.attrs = &attr;
         config.numAttrs = overlap ? 1 : 0;
         overlap = false;
-        const cudaError_t e = cudaLaunchKernelEx(&config, step_kernel<BITS, MOST>, l, fixed, shared);
+        cudaError_t e = cudaSuccess;
+        if (BITS == 8) e = cudaFuncSetAttribute(step_kernel<BITS, MOST>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing * kMostStage);
+        if (e == cudaSuccess) e = cudaLaunchKernelEx(&config, step_kernel<BITS, MOST>, l, fixed, shared);
         count_launches(1);
         if (e != cudaSuccess) return e;
     }
@@ -537,7 +631,7 @@ extern "C" int hb_adamw_step(int64_t count, void* const* params, const void* con
     const auto go = bits == 8 ? (count <= kFew ? run<8, kFew> : run<8, kMany>) : (count <= kFew ? run<32, kFew> : run<32, kMany>);
     if (e == cudaSuccess)
         e = go(count, params, grads, first, second, first_scale, second_scale, master, sizes, types, grad_types,
-               total >= kLongLeast ? kLongChunk : kChunk, fixed, shared, st);
+               total < kLongLeast ? kChunk : kLongChunk, fixed, shared, st);
     return finish(e, what);
 }
 
