@@ -17,7 +17,7 @@
 // The rows of an expert begin anywhere: TMA boxes may (only the innermost coordinate has to lie on 16
 // bytes), rows of the next expert that a tile's box brings along are summed and not written.  In the sum
 // over an expert's rows (dW) they have to be zeros instead, of both operands (0 * NaN): the box that holds
-// the expert's end completes on a barrier of its own CTA, the producer's warp zeroes the foreign rows and
+// the expert's end completes on a barrier of its own CTA, a warp of its own zeroes the foreign rows and
 // hands the stage on.
 #include <algorithm>
 #include <string>
@@ -30,7 +30,9 @@
 namespace hb {
 namespace experts {
 
-constexpr int BK = 64, kStages = 6, kEpiWarps = 8, kThreads = 64 + 32 * kEpiWarps;
+constexpr int BK = 64, kStages = 5, kEpiWarps = 16;
+// producer, issuer, writers, and in kWeights a warp that zeroes foreign rows
+constexpr int threads_of(int form) { return 64 + 32 * kEpiWarps + (form == kWeights ? 32 : 0); }
 constexpr int kTileBytes = 128 * BK * 2, kStageBytes = 2 * kTileBytes;
 constexpr int kBand = 8;  // row tiles that share a weight tile while it is in L2
 
@@ -50,9 +52,9 @@ struct Params {
 
 struct __align__(1024) Smem {
     uint8_t stage[kStages][kStageBytes];
-    __align__(16) uint8_t out[kEpiWarps][32 * 64];  // a warp's 32 x 32 chunk on its way out
+    __align__(16) uint8_t out[kEpiWarps][32 * 64];  // a warp's 32 rows x 64 bytes on their way out
     int start[kMostGroups + 2], tile[kMostGroups + 2];
-    uint64_t full[kStages], empty[kStages], tfull[2], tempty[2], tail;
+    uint64_t full[kStages], empty[kStages], tail[kStages], tfull[2], tempty[2];
     uint32_t tmem_base;
     int abort, status;
 };
@@ -88,6 +90,11 @@ __device__ __forceinline__ void load_4d_pair(void* dst, const CUtensorMap* map, 
     asm volatile(
         "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
         ::"r"(smem_u32(dst)), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
+}
+// Arrive on an mbarrier of the other CTA after reading TMEM (whose loads have been waited for): nothing in memory is
+// handed over, so no release either.
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // A bounded wait on a barrier that the other CTA arrives on as well.
 template <bool PAIR>
@@ -238,7 +245,7 @@ template <int FORM, bool PAIR>
 __device__ __forceinline__ void produce(const Params& p, Smem& s, int rank) {
     using S = Shape<FORM, PAIR>;
     const int lane = threadIdx.x & 31;
-    uint32_t stage = 0, phase = 0, tails = 0;
+    uint32_t stage = 0, phase = 0;
     const int units = tiles_of<FORM, PAIR>(p, s);
     const int per_segment = (p.k + BK - 1) / BK;
     for (int u = blockIdx.x / (PAIR ? 2 : 1); u < units; u += gridDim.x / (PAIR ? 2 : 1)) {
@@ -258,25 +265,10 @@ __device__ __forceinline__ void produce(const Params& p, Smem& s, int rank) {
                         columns_2d<PAIR>(a, am, &s.full[stage], full, t.row, row, p.blocked[0]);
                         columns_2d<PAIR>(b, &p.b[0], &s.full[stage], full, bcol, row, p.blocked[1]);
                     }
-                } else {  // rows of the next expert are in the box: zero them once it is there
-                    if (lane == 0) {
-                        mbar_arrive_expect_tx(&s.tail, kStageBytes);
-                        columns_2d<false>(a, am, &s.tail, 0, t.row, row, p.blocked[0]);
-                        columns_2d<false>(b, &p.b[0], &s.tail, 0, bcol, row, p.blocked[1]);
-                    }
-                    if (!warp_wait<false>(&s.tail, tails & 1, s)) return;
-                    ++tails;
-                    const int words = (BK - left) * 8;  // 16 bytes each, of every box
-                    for (int i = lane; i < words; i += 32)
-#pragma unroll
-                        for (int box = 0; box < 4; ++box)
-                            *reinterpret_cast<uint4*>(a + box * BK * 128 + left * 128 + i * 16) = make_uint4(0, 0, 0, 0);
-                    fence_async_shared();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if (PAIR) mbar_arrive_remote(full);
-                        else mbar_arrive(&s.full[stage]);
-                    }
+                } else if (lane == 0) {  // rows of the next expert are in the box: clean_tails hands the stage on
+                    mbar_arrive_expect_tx(&s.tail[stage], kStageBytes);
+                    columns_2d<false>(a, am, &s.tail[stage], 0, t.row, row, p.blocked[0]);
+                    columns_2d<false>(b, &p.b[0], &s.tail[stage], 0, bcol, row, p.blocked[1]);
                 }
             } else if (lane == 0) {
                 const int seg = FORM == kBack ? kb / per_segment : 0;
@@ -306,6 +298,36 @@ __device__ __forceinline__ void produce(const Params& p, Smem& s, int rank) {
                 }
             }
             if (++stage == kStages) stage = 0, phase ^= 1;
+        }
+    }
+}
+
+// kWeights: a warp zeroes the rows behind the end of the summed ones in the stage that holds it, of both operands, and
+// hands the stage on; the producer goes on meanwhile (one that waited for each end took twice as long where experts
+// have few rows).
+template <bool PAIR>
+__device__ __forceinline__ void clean_tails(const Params& p, Smem& s, int rank) {
+    const int lane = threadIdx.x & 31;
+    uint32_t stage = 0, phases = 0;
+    const int units = tiles_of<kWeights, PAIR>(p, s);
+    for (int u = blockIdx.x / (PAIR ? 2 : 1); u < units; u += gridDim.x / (PAIR ? 2 : 1)) {
+        const Tile t = tile_at<kWeights, PAIR>(p, s, u, rank);
+        stage = (stage + t.blocks) % kStages;
+        const int left = t.length % BK;
+        if (left == 0) continue;
+        const uint32_t last = (stage + kStages - 1) % kStages;
+        if (!warp_wait<false>(&s.tail[last], phases >> last & 1, s)) return;
+        phases ^= 1u << last;
+        const int words = (BK - left) * 8;  // 16 bytes each, of every box
+        for (int i = lane; i < words; i += 32)
+#pragma unroll
+            for (int box = 0; box < 4; ++box)
+                *reinterpret_cast<uint4*>(s.stage[last] + box * BK * 128 + left * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) {
+            if (PAIR) mbar_arrive_remote(peer_smem(&s.full[last], 0));
+            else mbar_arrive(&s.full[last]);
         }
     }
 }
@@ -347,52 +369,98 @@ __device__ __forceinline__ void multiply(const Params& p, Smem& s, uint32_t tmem
     }
 }
 
-// Writes a warp's chunk of 32 rows x 32 columns (thread: its row's 32 values) through shared memory, so that rows leave
-// in whole sectors: `out` its first element, `stride` the rows' distance, `rows` and `cols` how many there are.
-// Rows pass in pieces of 64 bytes; the swizzle keeps 8 rows' 16-byte words in different banks.
+// 16 columns of a warp's 32 rows: lane l gets row l.  Waited for by tmem_wait16.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&r)[16]) {
+    uint32_t* u = reinterpret_cast<uint32_t*>(r);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]),
+          "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait16(float (&r)[16]) {
+    uint32_t* u = reinterpret_cast<uint32_t*>(r);
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(u[0]), "+r"(u[1]), "+r"(u[2]), "+r"(u[3]), "+r"(u[4]), "+r"(u[5]), "+r"(u[6]), "+r"(u[7]),
+                   "+r"(u[8]), "+r"(u[9]), "+r"(u[10]), "+r"(u[11]), "+r"(u[12]), "+r"(u[13]), "+r"(u[14]), "+r"(u[15])
+                 ::"memory");
+}
+
+// A thread's 16 values of its row as the words of T that they round to: 32 or 64 bytes.
 template <typename T>
-__device__ __forceinline__ void write_chunk(uint8_t* buf, const float (&v)[32], T* out, int64_t stride, int rows, int cols,
-                                            bool vectors, int lane) {
-    constexpr int N = 64 / (int)sizeof(T), V = 16 / (int)sizeof(T);  // values of a piece, of a word
+union Row16 {
+    uint4 word[sizeof(T)];
+    T t[16];
+    __device__ __forceinline__ Row16() {}
+    __device__ __forceinline__ void hold(const float (&v)[16]) {
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int piece = 0; piece < 32 / N; ++piece) {
-        union {
-            uint4 raw[4];
-            T t[N];
-        } r;
+            for (int i = 0; i < 16; ++i) t[i] = v[i];
+        } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) r.t[i] = rows::from_float<T>(v[piece * N + i]);
+            for (int i = 0; i < 16; i += 2) {
+                if constexpr (std::is_same<T, __half>::value) *reinterpret_cast<__half2*>(t + i) = __floats2half2_rn(v[i], v[i + 1]);
+                else *reinterpret_cast<__nv_bfloat162*>(t + i) = __floats2bfloat162_rn(v[i], v[i + 1]);
+            }
+        }
+    }
+};
+
+// Where a warp's chunk of 32 rows goes: 64 bytes of each (COLS values of T), through shared memory, so that rows leave in
+// whole sectors.  The swizzle keeps 8 rows' 16-byte words in different banks.
+template <typename T>
+struct Writer {
+    static constexpr int COLS = 64 / (int)sizeof(T), V = 16 / (int)sizeof(T);
+    uint8_t* buf;
+    int lane, unit;  // unit: bytes (16, 4 or a value) that rows lie on
+    // Words first..first + N of this thread's row.
+    template <int N>
+    __device__ __forceinline__ void stage(const uint4 (&word)[N], int first) {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            *reinterpret_cast<uint4*>(buf + lane * 64 + (((first + j) ^ ((lane >> 1) & 3)) << 4)) = word[j];
+    }
+    // The staged chunk to `to`, `stride` values between rows; `rows` and `cols` how many there are.
+    __device__ __forceinline__ void write(T* to, int64_t stride, int rows, int cols) {
         __syncwarp();
-#pragma unroll
-        for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = r.raw[j];
-        __syncwarp();
-        T* to = out + piece * N;
-        const int left = cols - piece * N;
-        if (vectors) {
+        if (unit == 16) {
             const int j = lane & 3;
-            if (j * V < left) {
+            to += (lane >> 2) * stride + j * V;
+            if (j * V < cols) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int row = i * 8 + (lane >> 2);
                     if (row < rows)
-                        *reinterpret_cast<uint4*>(to + row * stride + j * V) =
-                            *reinterpret_cast<const uint4*>(buf + row * 64 + ((j ^ ((row >> 1) & 3)) << 4));
+                        *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(buf + row * 64 + ((j ^ ((row >> 1) & 3)) << 4));
+                    to += 8 * stride;
                 }
             }
+        } else if (unit == 4) {
+            constexpr int W = 4 / (int)sizeof(T);  // rows are even, so the end cuts no word
+            const int w = lane & 15, j = w >> 2;
+            to += (lane >> 4) * stride + w * W;
+            if (w * W < cols)
+#pragma unroll 4
+                for (int row = lane >> 4; row < rows; row += 2, to += 2 * stride)
+                    *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(buf + row * 64 + ((j ^ ((row >> 1) & 3)) << 4) + (w & 3) * 4);
         } else {
-            const int c = lane % N, j = c / V, in = c % V * (int)sizeof(T);
-            for (int row = lane / N; row < rows; row += 32 / N)
-                if (c < left) to[row * stride + c] = *reinterpret_cast<const T*>(buf + row * 64 + ((j ^ ((row >> 1) & 3)) << 4) + in);
+            const int c = lane % COLS, j = c / V, in = c % V * (int)sizeof(T);
+            to += lane / COLS * stride + c;
+            if (c < cols)
+#pragma unroll 4
+                for (int row = lane / COLS; row < rows; row += 32 / COLS, to += 32 / COLS * stride)
+                    *to = *reinterpret_cast<const T*>(buf + row * 64 + ((j ^ ((row >> 1) & 3)) << 4) + in);
         }
+        __syncwarp();
     }
-}
+};
 
-// A thread's 32 values of a row.
+// A thread's 16 values of a row.
 template <typename T>
-__device__ __forceinline__ void read_row(float (&v)[32], const T* at, int cols, bool vectors) {
+__device__ __forceinline__ void read_row(float (&v)[16], const T* at, int cols, bool vectors) {
     if (vectors) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 2; ++j) {
             rows::Vec<T, 16> w;
             if (j * 8 < cols) w.load(at + j * 8);
             else w.zero();
@@ -401,21 +469,23 @@ __device__ __forceinline__ void read_row(float (&v)[32], const T* at, int cols, 
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = i < cols ? rows::to_float(at[i]) : 0.0f;
+        for (int i = 0; i < 16; ++i) v[i] = i < cols ? rows::to_float(at[i]) : 0.0f;
     }
 }
 
-// Two warps a TMEM lane quarter, each on half of the output's columns.  A wait that gave up leaves NaN.
+// Four warps a TMEM lane quarter, each on a quarter of the output's columns.  A wait that gave up leaves NaN.
 template <int FORM, bool PAIR, typename T>
 __device__ __forceinline__ void write_out(const Params& p, Smem& s, uint32_t tmem, int rank) {
     using S = Shape<FORM, PAIR>;
-    constexpr int kSlice = S::kCols / 2;
+    constexpr int kSlice = S::kCols / 4, kChunk = kSlice < 32 ? kSlice : 32;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int quarter = warp & 3, slice = (warp - 2) >> 2;
-    uint8_t* buf = s.out[warp - 2];
     const uint32_t tempty = PAIR ? peer_smem(&s.tempty[0], 0) : 0u;
     const int width = FORM == kWeights ? p.k : p.n;
-    const bool vectors = p.out_row % 8 == 0 && ((reinterpret_cast<uintptr_t>(p.out[0]) | reinterpret_cast<uintptr_t>(p.out[1])) & 15) == 0;
+    // what all rows of the outputs lie on
+    const uint64_t grid = (uint64_t)p.out_row * 2 | reinterpret_cast<uintptr_t>(p.out[0]) | reinterpret_cast<uintptr_t>(p.out[1]);
+    Writer<T> writer{s.out[warp - 2], lane, grid % 16 == 0 ? 16 : grid % 4 == 0 ? 4 : 2};
+    Writer<float> writer32{s.out[warp - 2], lane, p.k % 4 == 0 ? 16 : 4};
     const bool dh_vectors = p.dh_row % 8 == 0 && width % 8 == 0 && (reinterpret_cast<uintptr_t>(p.dh) & 15) == 0;
     uint32_t done = 0;
     bool good = true;
@@ -438,59 +508,74 @@ __device__ __forceinline__ void write_out(const Params& p, Smem& s, uint32_t tme
         }
         const int64_t at = (int64_t)(t.row + row0) * p.out_row + col0;
         const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16) + acc * S::N + slice * kSlice;
-        for (int c = 0; c < kSlice; c += 32) {
-            const int cols = min(32, width - col0 - c);
+#pragma unroll
+        for (int c = 0; c < kSlice; c += kChunk) {
+            const int cols = min(kChunk, width - col0 - c);
             if (rows <= 0 || cols <= 0) break;  // the same for the whole warp
-            float v[32];
-            if (!summed || !good) {
+            const bool filled = summed && good;
+            float v[kChunk / 16][16], w[S::kHalves ? kChunk / 16 : 1][16];
+            Row16<T> second[FORM == kGatedGrad ? kChunk / 16 : 1];
+            if (filled) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = good ? 0.0f : __int_as_float(0x7fc00000);
-                if (FORM == kWeights && partial) {
-                    write_chunk<float>(buf, v, partial + at + c, p.k, rows, cols, p.k % 4 == 0, lane);
-                    continue;
+                for (int h = 0; h < kChunk / 16; ++h) {
+                    tmem_ld16(taddr + c + h * 16, v[h]);
+                    if constexpr (S::kHalves) tmem_ld16(taddr + S::N / 2 + c + h * 16, w[h]);
                 }
-                write_chunk<T>(buf, v, out + at + c, p.out_row, rows, cols, vectors, lane);
-                if (FORM == kGatedGrad)
-                    write_chunk<T>(buf, v, static_cast<T*>(p.out[1]) + at + c, p.out_row, rows, cols, vectors, lane);
-                continue;
             }
-            if constexpr (S::kHalves) {
-                float w[32], d[32];
-                if (FORM == kGatedGrad) {
-                    const int r = min(lane, rows - 1);
-                    read_row<T>(d, static_cast<const T*>(p.dh) + (int64_t)(t.row + row0 + r) * p.dh_row + col0 + c, cols, dh_vectors);
-                }
-                tmem_ld32(taddr + c, v);
-                tmem_ld32(taddr + S::N / 2 + c, w);
-                tmem_wait_ld(v);
-                tmem_wait_ld(w);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    float slope;
-                    const float a = activate<false, FORM == kGatedGrad>(p.activation, v[i], slope);
-                    if (FORM == kGated) {
-                        v[i] = a * w[i];
-                    } else {
-                        v[i] = d[i] * w[i] * slope;
-                        w[i] = d[i] * a;
+            for (int h = 0; h < kChunk / 16; ++h) {
+                if (!filled) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[h][i] = good ? 0.0f : __int_as_float(0x7fc00000);
+                    if constexpr (FORM == kGatedGrad) second[h].hold(v[h]);
+                } else if constexpr (S::kHalves) {
+                    float d[16];
+                    if constexpr (FORM == kGatedGrad)
+                        read_row<T>(d, static_cast<const T*>(p.dh) + (int64_t)(t.row + row0 + min(lane, rows - 1)) * p.dh_row + col0 + c + h * 16,
+                                    cols - h * 16, dh_vectors);
+                    tmem_wait16(v[h]);
+                    tmem_wait16(w[h]);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        float slope;
+                        const float a = activate<false, FORM == kGatedGrad>(p.activation, v[h][i], slope);
+                        if (FORM == kGated) {
+                            v[h][i] = a * w[h][i];
+                        } else {
+                            v[h][i] = d[i] * w[h][i] * slope;
+                            w[h][i] = d[i] * a;
+                        }
                     }
+                    if constexpr (FORM == kGatedGrad) second[h].hold(w[h]);
+                } else {
+                    tmem_wait16(v[h]);
                 }
-                write_chunk<T>(buf, v, out + at + c, p.out_row, rows, cols, vectors, lane);
-                if (FORM == kGatedGrad)
-                    write_chunk<T>(buf, w, static_cast<T*>(p.out[1]) + at + c, p.out_row, rows, cols, vectors, lane);
-            } else {
-                tmem_ld32(taddr + c, v);
-                tmem_wait_ld(v);
-                if (FORM == kWeights && partial)
-                    write_chunk<float>(buf, v, partial + at + c, p.k, rows, cols, p.k % 4 == 0, lane);
-                else
-                    write_chunk<T>(buf, v, out + at + c, p.out_row, rows, cols, vectors, lane);
+                if (FORM == kWeights && partial) {
+                    Row16<float> r;
+                    r.hold(v[h]);
+                    writer32.stage(r.word, 0);
+                    writer32.write(partial + at + c + h * 16, p.k, rows, cols - h * 16);
+                } else {
+                    Row16<T> r;
+                    r.hold(v[h]);
+                    writer.stage(r.word, 2 * h);
+                }
+            }
+            if (FORM == kWeights && partial) continue;
+            writer.write(out + at + c, p.out_row, rows, cols);
+            if constexpr (FORM == kGatedGrad) {
+#pragma unroll
+                for (int h = 0; h < kChunk / 16; ++h) writer.stage(second[h].word, 2 * h);
+                writer.write(static_cast<T*>(p.out[1]) + at + c, p.out_row, rows, cols);
             }
         }
         if (summed) {
             tc_fence_before();
-            if (PAIR && rank != 0) mbar_arrive_remote(tempty + acc * (uint32_t)sizeof(uint64_t));
-            else mbar_arrive(&s.tempty[acc]);
+            __syncwarp();
+            if (lane == 0) {
+                if (PAIR && rank != 0) arrive_cluster(tempty + acc * (uint32_t)sizeof(uint64_t));
+                else mbar_arrive(&s.tempty[acc]);
+            }
             ++done;
         }
     }
@@ -499,7 +584,7 @@ __device__ __forceinline__ void write_out(const Params& p, Smem& s, uint32_t tme
 // With pairs both CTAs allocate TMEM together, meet after the barriers are ready and before they leave; every role
 // returns to the end, after a wait that gave up too.
 template <int FORM, bool PAIR, typename T>
-__global__ void __launch_bounds__(kThreads, 1) expert_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(threads_of(FORM), 1) expert_kernel(const __grid_constant__ Params p) {
     using S = Shape<FORM, PAIR>;
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ uint8_t smem_raw[];
@@ -507,9 +592,8 @@ __global__ void __launch_bounds__(kThreads, 1) expert_kernel(const __grid_consta
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = PAIR ? (int)cluster_rank() : 0;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kStages; ++i) mbar_init(&s.full[i], PAIR ? 2 : 1), mbar_init(&s.empty[i], 1);
-        for (int i = 0; i < 2; ++i) mbar_init(&s.tfull[i], 1), mbar_init(&s.tempty[i], 32 * kEpiWarps * (PAIR ? 2 : 1));
-        mbar_init(&s.tail, 1);
+        for (int i = 0; i < kStages; ++i) mbar_init(&s.full[i], PAIR ? 2 : 1), mbar_init(&s.empty[i], 1), mbar_init(&s.tail[i], 1);
+        for (int i = 0; i < 2; ++i) mbar_init(&s.tfull[i], 1), mbar_init(&s.tempty[i], kEpiWarps * (PAIR ? 2 : 1));
         s.abort = s.status = 0;
         fence_barrier_init();
     }
@@ -528,8 +612,10 @@ __global__ void __launch_bounds__(kThreads, 1) expert_kernel(const __grid_consta
         produce<FORM, PAIR>(p, s, rank);
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) multiply<FORM, PAIR, BF16>(p, s, tmem);
-    } else {
+    } else if (warp < 2 + kEpiWarps) {
         write_out<FORM, PAIR, T>(p, s, tmem, rank);
+    } else if constexpr (FORM == kWeights) {
+        clean_tails<PAIR>(p, s, rank);
     }
     tc_fence_before();
     __syncthreads();
@@ -591,7 +677,7 @@ cudaError_t launch(const Params& p, int64_t tiles, cudaStream_t st) {
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)std::min<int64_t>(PAIR ? sms / 2 * 2 : sms, tiles * (PAIR ? 2 : 1)));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(threads_of(FORM));
     cfg.dynamicSmemBytes = kSmemBytes;
     cfg.stream = st;
     cfg.attrs = at;

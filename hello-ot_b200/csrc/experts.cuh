@@ -98,12 +98,22 @@ __device__ inline int group_of(const int* tile, int groups, int t) {
     return lo;
 }
 
-// act(g) and, with SLOPE, act'(g).  PRECISE: results that are held in 32 bits; otherwise the fast exponential and
-// quotient (2^-21 relative), 8 bits below the rounding of a 16-bit result.
+// act(g) and, with SLOPE, act'(g).  PRECISE: results that are held in 32 bits; otherwise the approximate exponential
+// and inverse ((4 + 2 |g|) 2^-23 relative), 8 bits below the rounding of a 16-bit result.
+template <bool PRECISE>
+__device__ __forceinline__ float exponential(float x) {
+    if (PRECISE) return expf(x);
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+    return r;
+}
 template <bool PRECISE>
 __device__ __forceinline__ float sigmoid(float g) {
-    if (PRECISE) return 1.0f / (1.0f + expf(-g));
-    return __fdividef(1.0f, 1.0f + __expf(-g));
+    const float below = 1.0f + exponential<PRECISE>(-g);
+    if (PRECISE) return 1.0f / below;
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(below));
+    return r;
 }
 template <bool PRECISE, bool SLOPE>
 __device__ __forceinline__ float activate(int kind, float g, float& slope) {
@@ -113,7 +123,7 @@ __device__ __forceinline__ float activate(int kind, float g, float& slope) {
         return g * s;
     }
     const float cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
-    if (SLOPE) slope = fmaf(g * 0.39894228040143268f, PRECISE ? expf(-0.5f * g * g) : __expf(-0.5f * g * g), cdf);
+    if (SLOPE) slope = fmaf(g * 0.39894228040143268f, exponential<PRECISE>(-0.5f * g * g), cdf);
     return g * cdf;
 }
 
