@@ -455,21 +455,71 @@ struct Writer {
     }
 };
 
-// A thread's 16 values of a row.
+// A chunk of 32 rows x 32 values on its way in: 8 rows' 64 bytes an instruction, held in registers until the sums are
+// there, then through the same shared memory to the thread of each row.
 template <typename T>
-__device__ __forceinline__ void read_row(float (&v)[16], const T* at, int cols, bool vectors) {
-    if (vectors) {
+struct Reader {
+    uint4 word[4];
+    bool vectors;
+    int lane;
+    __device__ __forceinline__ void load(const T* from, int64_t stride, int rows, int cols) {
+        if (!vectors) return;
+        const int j = lane & 3;
+        from += (lane >> 2) * stride + j * 8;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            rows::Vec<T, 16> w;
-            if (j * 8 < cols) w.load(at + j * 8);
-            else w.zero();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[j * 8 + i] = rows::to_float(w.v[i]);
+        for (int i = 0; i < 4; ++i) {
+            word[i] = make_uint4(0, 0, 0, 0);
+            if (i * 8 + (lane >> 2) < rows && j * 8 < cols) word[i] = __ldcs(reinterpret_cast<const uint4*>(from));
+            from += 8 * stride;
         }
-    } else {
+    }
+    __device__ __forceinline__ void stage(uint8_t* buf, const T* from, int64_t stride, int rows, int cols) const {
+        if (vectors) {
+            const int j = lane & 3;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = i < cols ? rows::to_float(at[i]) : 0.0f;
+            for (int i = 0; i < 4; ++i) {
+                const int row = i * 8 + (lane >> 2);
+                *reinterpret_cast<uint4*>(buf + row * 64 + ((j ^ ((row >> 1) & 3)) << 4)) = word[i];
+            }
+        } else {
+            const int j = lane >> 3, in = (lane & 7) * 2;
+#pragma unroll 4
+            for (int row = 0; row < 32; ++row)
+                *reinterpret_cast<T*>(buf + row * 64 + ((j ^ ((row >> 1) & 3)) << 4) + in) =
+                    row < rows && lane < cols ? from[row * stride + lane] : rows::from_float<T>(0.0f);
+        }
+        __syncwarp();
+    }
+    // This thread's row; the shared memory is free again.
+    __device__ __forceinline__ void take(const uint8_t* buf) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) word[q] = *reinterpret_cast<const uint4*>(buf + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4));
+        __syncwarp();
+    }
+    __device__ __forceinline__ void values(int h, float (&v)[16]) const {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            rows::Vec<T, 16> w;
+            w.raw = word[2 * h + q];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[q * 8 + i] = rows::to_float(w.v[i]);
+        }
+    }
+};
+
+// g and u of 16 places to the outputs: h in v, or dg in v and du in w.
+template <int FORM, int ACTIVATION>
+__device__ __forceinline__ void combine(float (&v)[16], float (&w)[16], const float (&d)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        float slope;
+        const float a = activate<false, FORM == kGatedGrad>(ACTIVATION, v[i], slope);
+        if (FORM == kGated) {
+            v[i] = a * w[i];
+        } else {
+            v[i] = d[i] * w[i] * slope;
+            w[i] = d[i] * a;
+        }
     }
 }
 
@@ -486,7 +536,9 @@ __device__ __forceinline__ void write_out(const Params& p, Smem& s, uint32_t tme
     const uint64_t grid = (uint64_t)p.out_row * 2 | reinterpret_cast<uintptr_t>(p.out[0]) | reinterpret_cast<uintptr_t>(p.out[1]);
     Writer<T> writer{s.out[warp - 2], lane, grid % 16 == 0 ? 16 : grid % 4 == 0 ? 4 : 2};
     Writer<float> writer32{s.out[warp - 2], lane, p.k % 4 == 0 ? 16 : 4};
-    const bool dh_vectors = p.dh_row % 8 == 0 && width % 8 == 0 && (reinterpret_cast<uintptr_t>(p.dh) & 15) == 0;
+    Reader<T> reader;  // kGatedGrad
+    reader.lane = lane;
+    reader.vectors = p.dh_row % 8 == 0 && width % 8 == 0 && (reinterpret_cast<uintptr_t>(p.dh) & 15) == 0;
     uint32_t done = 0;
     bool good = true;
     const int units = tiles_of<FORM, PAIR>(p, s);
@@ -494,6 +546,13 @@ __device__ __forceinline__ void write_out(const Params& p, Smem& s, uint32_t tme
         const Tile t = tile_at<FORM, PAIR>(p, s, u, rank);
         const uint32_t acc = done & 1;
         const bool summed = t.blocks != 0;
+        const T* dh = nullptr;
+        if constexpr (FORM == kGatedGrad) {  // on its way while the tile is summed
+            static_assert(kSlice == kChunk, "one chunk a warp");
+            const int64_t first = (int64_t)(t.row + quarter * 32) * p.dh_row + t.col + slice * kSlice;
+            dh = static_cast<const T*>(p.dh) + first;
+            if (summed) reader.load(dh, p.dh_row, min(32, t.rows - quarter * 32), min(kChunk, width - t.col - slice * kSlice));
+        }
         if (summed) {
             good = __all_sync(0xffffffffu, good && wait<PAIR>(&s.tfull[acc], (done >> 1) & 1, s));  // a warp goes on as one
             tc_fence_after();
@@ -515,7 +574,12 @@ __device__ __forceinline__ void write_out(const Params& p, Smem& s, uint32_t tme
             const bool filled = summed && good;
             float v[kChunk / 16][16], w[S::kHalves ? kChunk / 16 : 1][16];
             Row16<T> second[FORM == kGatedGrad ? kChunk / 16 : 1];
-            if (filled) {
+            if constexpr (FORM == kGatedGrad)
+                if (filled) {
+                    reader.stage(s.out[warp - 2], dh, p.dh_row, rows, cols);
+                    reader.take(s.out[warp - 2]);
+                }
+            if (FORM != kGatedGrad && filled) {
 #pragma unroll
                 for (int h = 0; h < kChunk / 16; ++h) {
                     tmem_ld16(taddr + c + h * 16, v[h]);
@@ -530,22 +594,15 @@ __device__ __forceinline__ void write_out(const Params& p, Smem& s, uint32_t tme
                     if constexpr (FORM == kGatedGrad) second[h].hold(v[h]);
                 } else if constexpr (S::kHalves) {
                     float d[16];
-                    if constexpr (FORM == kGatedGrad)
-                        read_row<T>(d, static_cast<const T*>(p.dh) + (int64_t)(t.row + row0 + min(lane, rows - 1)) * p.dh_row + col0 + c + h * 16,
-                                    cols - h * 16, dh_vectors);
+                    if constexpr (FORM == kGatedGrad) {  // half a chunk at a time: registers
+                        tmem_ld16(taddr + c + h * 16, v[h]);
+                        tmem_ld16(taddr + S::N / 2 + c + h * 16, w[h]);
+                        reader.values(h, d);
+                    }
                     tmem_wait16(v[h]);
                     tmem_wait16(w[h]);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        float slope;
-                        const float a = activate<false, FORM == kGatedGrad>(p.activation, v[h][i], slope);
-                        if (FORM == kGated) {
-                            v[h][i] = a * w[h][i];
-                        } else {
-                            v[h][i] = d[i] * w[h][i] * slope;
-                            w[h][i] = d[i] * a;
-                        }
-                    }
+                    if (p.activation == kSilu) combine<FORM, kSilu>(v[h], w[h], d);
+                    else combine<FORM, kGelu>(v[h], w[h], d);
                     if constexpr (FORM == kGatedGrad) second[h].hold(w[h]);
                 } else {
                     tmem_wait16(v[h]);
