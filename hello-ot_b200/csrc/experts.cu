@@ -796,11 +796,12 @@ bool use_pairs(const Job& job) {
 // kWeights: parts of the rows, where the tiles alone leave most of the device idle and experts have many stages.
 constexpr int kSlots = 148, kLeastStages = 16;
 int splits_of(const Job& job) {
-    const bool pair = job.type != HB_F32 && use_pairs(job);
-    const int64_t side = pair ? 256 : 128, slots = pair ? kSlots / 2 : kSlots;
+    const bool f32 = job.type == HB_F32, pair = !f32 && use_pairs(job);
+    const int64_t side = f32 ? f32_tile(job) : pair ? 256 : 128;
+    const int64_t slots = f32 ? kSlots * (side == 128 ? 2 : 4) : pair ? kSlots / 2 : kSlots;  // resident tiles
     const int64_t tiles = job.segments * (int64_t)job.groups * ((job.n + side - 1) / side) * ((job.k + side - 1) / side);
     const int64_t stages = (job.rows / job.groups + 63) / 64;
-    return (int)std::max<int64_t>(1, std::min(slots / tiles, stages / kLeastStages));
+    return (int)std::max<int64_t>(1, std::min(slots / tiles, stages / (f32 ? 2 : kLeastStages)));
 }
 size_t partial_bytes(const Job& job, int splits) {
     return splits > 1 ? (size_t)splits * job.segments * job.groups * job.n * job.k * sizeof(float) : 0;
@@ -832,6 +833,7 @@ int run(const Job& job, cudaStream_t st) {
 }
 
 // ---------------------------------------------------------------- checks of the C entries
+constexpr int64_t kMostWidth = 1 << 21;
 bool fits(const Operand& o, int type, int64_t cols, int64_t rows, bool weights, int64_t groups, bool grid) {
     const uint64_t size = rows::type_bytes(type), unit = grid && type != HB_F32 ? 16 : size;
     if (!o.p || rows::address_bits(o.p) % unit || o.row < 0 || o.row > INT32_MAX) return false;
@@ -849,7 +851,7 @@ int check(const hb_expert_shape* s, const int32_t* offsets, const char* what) {
     const std::string at = std::string(what) + ": ";
     if (!s) return abi_fail(HB_BAD_ARGUMENT, at + "null shape");
     if (!rows::valid_type(s->type)) return abi_fail(HB_BAD_ARGUMENT, at + "element type");
-    if (s->rows < 0 || s->rows > INT32_MAX - 1024 || s->width < 1 || s->hidden < 1 || s->width > (1 << 28) || s->hidden > (1 << 28))
+    if (s->rows < 0 || s->rows > INT32_MAX - 1024 || s->width < 1 || s->hidden < 1 || s->width > kMostWidth || s->hidden > kMostWidth)
         return abi_fail(HB_BAD_ARGUMENT, at + "rows, width or hidden out of range");
     if (s->experts < 1 || s->experts > kMostGroups || (!offsets && s->experts != 1))
         return abi_fail(HB_BAD_ARGUMENT, at + "1 to 2048 experts, and one without offsets");
@@ -947,7 +949,7 @@ Job weights_job(const hb_expert_shape* s, const int32_t* offsets, int segments) 
 }
 bool valid(const hb_expert_shape* s) {
     return s && rows::valid_type(s->type) && s->rows >= 0 && s->rows <= INT32_MAX - 1024 && s->hidden >= 1 && s->width >= 1 &&
-           s->hidden <= (1 << 28) && s->width <= (1 << 28) && s->experts >= 1 && s->experts <= kMostGroups;
+           s->hidden <= kMostWidth && s->width <= kMostWidth && s->experts >= 1 && s->experts <= kMostGroups;
 }
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 size_t held_bytes(const hb_expert_shape* s) { return round256((size_t)s->rows * padded(s->hidden) * rows::type_bytes(s->type)); }

@@ -131,6 +131,8 @@ __device__ __forceinline__ float activate(int kind, float g, float& slope) {
 constexpr int kFewRows = HB_EXPERT_FEW_ROWS;
 cudaError_t few_rows(const Job& job, cudaStream_t st);
 cudaError_t product_f32(const Job& job, cudaStream_t st);
+// The side of product_f32's tiles: 64 where tiles of 128 would leave SMs without one.
+int f32_tile(const Job& job);
 // Adds the parts of kWeights in order and rounds them once.
 cudaError_t join_parts(const Job& job, cudaStream_t st);
 

@@ -1,10 +1,12 @@
 // Products of rows sorted by expert on the CUDA cores: fp32 rows, and few rows of any type.
 //
-// fp32 (product_f32): every form of experts.cu in tiles of 128 x 128, 8 of the summed length a step, two steps in
-// shared memory; a thread holds 8 x 8 sums and adds products in pairs (fma.rn.f32x2), each rounded like the scalar
-// instruction, so the sums are plain fp32 sums.  The tensor cores would need three bf16 parts of each operand and
-// cut off the low bits of their running sums, which fp32 results do not allow.  In the gated forms a tile's
-// columns are 64 of g and the same 64 of u, and one thread holds both of a place.
+// fp32 (product_f32): every form of experts.cu in tiles of 128 x 128 or 64 x 64, 8 of the summed length a step.  Each
+// thread copies its elements straight to shared memory (asynchronous copies of 4 bytes, which take any alignment and
+// order and write zeros for what is not there), four steps ahead; it holds 8 x 8 or 4 x 4 sums and adds products in
+// pairs (fma.rn.f32x2), each rounded like the scalar instruction, so the sums are plain fp32 sums.  The tensor cores
+// would need three bf16 parts of each operand and cut off the low bits of their running sums, which fp32 results do
+// not allow.  In the gated forms half of a tile's columns are g's and half the same places of u, and one thread
+// holds both of a place.
 //
 // Few rows (few_rows, at most 16 of all experts together): one token's step of a decode batch reads the named
 // experts' weights once and is bound by that.  A warp streams the weight rows of one output column and multiplies
@@ -21,7 +23,7 @@ namespace experts {
 namespace {
 
 // ---------------------------------------------------------------- fp32 tiles
-constexpr int BM = 128, BN = 128, BK = 8, kPitch = 132, kThreads = 256;
+constexpr int BK = 8, kStages = 4, kThreads = 256;
 
 struct Params {
     const int32_t* offsets;
@@ -39,125 +41,175 @@ __device__ __forceinline__ void fma2(uint64_t& c, uint64_t a, uint64_t b) {
     asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b));
 }
 __device__ __forceinline__ float half_of(uint64_t v, int hi) { return __uint_as_float((uint32_t)(hi ? v >> 32 : v)); }
-
-// Four of an operand tile's 128 x 8 values for this thread: LONG rows run along the summed length, else across it.
-// Place i of the tile's 128 is at base + i * row (LONG) or base + i; `lim` of them and `left` of the length are there.
-template <bool LONG>
-__device__ __forceinline__ void fetch(float (&r)[4], const float* base, int64_t row, int lim, int k0, int left) {
-    const int t = threadIdx.x;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int k = LONG ? t & 7 : (t >> 7) + 2 * i, m = LONG ? (t >> 3) + 32 * i : t & 127;
-        r[i] = m < lim && k < left ? __ldg(LONG ? base + m * row + k0 + k : base + (int64_t)(k0 + k) * row + m) : 0.0f;
-    }
-}
-template <bool LONG>
-__device__ __forceinline__ void stage(float (*to)[kPitch], const float (&r)[4]) {
-    const int t = threadIdx.x;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int k = LONG ? t & 7 : (t >> 7) + 2 * i, m = LONG ? (t >> 3) + 32 * i : t & 127;
-        to[k][m] = r[i];
-    }
+// 4 bytes to shared memory, or zeros.
+__device__ __forceinline__ void copy4(uint32_t to, const float* from, bool there) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
 }
 
-template <int FORM>
-__global__ void __launch_bounds__(kThreads, 2) f32_kernel(const __grid_constant__ Params p) {
+// What a thread copies of an operand's TILE x 8 values each step.  LONG: the operand's rows run along the summed length,
+// and 8 threads take 8 neighbours of a row; else across it, and TILE threads take neighbours of one place of the length.
+template <int TILE, bool LONG>
+struct Source {
+    static constexpr int EACH = TILE * BK / kThreads, ACROSS = kThreads / TILE;  // elements of a thread; LONG: 32 rows apart
+    const float* at[LONG ? EACH : 1];
+    int64_t step;  // from one step to the next
+    int64_t row;
+    uint32_t to;   // the first element's place in a stage, bytes
+    uint32_t live; // which of the rows are there
+    int k;         // the first element's place in the summed length
+    // Place 0 of the tile at `base`, `lim` of them there; HALVES: places from TILE / 2 on at `other`, by its own stride.
+    template <bool HALVES>
+    __device__ __forceinline__ void start(const float* base, const float* other, int64_t stride, int64_t other_stride, int lim, int pitch) {
+        const int t = threadIdx.x;
+        row = stride;
+        live = 0;
+        if (LONG) {
+            const int m0 = t >> 3;
+            k = t & 7;
+            step = BK;
+            to = (k * pitch + m0) * 4;
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                const int m = m0 + 32 * i, place = HALVES ? m % (TILE / 2) : m;
+                const int there = place < lim ? place : 0;
+                at[i] = (HALVES && m >= TILE / 2 ? other + there * other_stride : base + there * stride) + k;
+                live |= (place < lim ? 1u : 0u) << i;
+            }
+        } else {
+            const int m = t % TILE;
+            k = t / TILE;
+            step = BK * stride;
+            to = (k * pitch + m) * 4;
+            at[0] = base + (m < lim ? m : 0) + (int64_t)k * stride;
+            live = m < lim ? ~0u : 0u;
+        }
+    }
+    // The next step's elements; `left` of the length are left.
+    __device__ __forceinline__ void copy(uint32_t stage, int left, int pitch) {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            if (LONG) {
+                const bool there = (live >> i & 1) && k < left;
+                copy4(stage + to + 32 * i * 4, there ? at[i] : at[0], there);
+                if (k + BK < left) at[i] += step;
+            } else {
+                const int kk = k + ACROSS * i;
+                const bool there = live && kk < left;
+                copy4(stage + to + ACROSS * i * pitch * 4, there ? at[0] + (int64_t)(ACROSS * i) * row : at[0], there);
+            }
+        }
+        if (!LONG && k + BK < left) at[0] += step;
+    }
+};
+
+template <int FORM, int TILE>
+__global__ void __launch_bounds__(kThreads, TILE == 128 ? 2 : 4) f32_kernel(const __grid_constant__ Params p) {
     constexpr bool HALVES = FORM == kGated || FORM == kGatedGrad;
     constexpr bool A_LONG = FORM != kWeights, B_LONG = FORM != kWeights && FORM != kBack;
-    constexpr int COLS = HALVES ? BN / 2 : BN;
-    __shared__ __align__(16) float as[2][BK][kPitch], bs[2][BK][kPitch];
-    __shared__ int start[kMostGroups + 2], tile[kMostGroups + 2];
-    read_groups(p.offsets, p.groups, p.rows, BM, start, tile);
+    constexpr int COLS = HALVES ? TILE / 2 : TILE, PITCH = TILE + 4;
+    constexpr int NR = TILE / 16, HR = NR / 2;  // sums of a thread: NR x NR, in four blocks of HR x HR half a tile apart
+    constexpr int STAGE = BK * PITCH;           // floats of an operand
+    union Memory {
+        float stage[kStages][2][STAGE];
+        int groups[2][kMostGroups + 2];  // until the block knows its rows
+    };
+    __shared__ __align__(16) Memory memory;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    const int col = blockIdx.x * COLS;
-    int row, lim, length, group, part = 0, split = 0;  // lim: rows of the tile that are the output's
-    const float *a0, *b0;
-    if (FORM == kWeights) {
-        part = blockIdx.z % p.segments;
-        group = blockIdx.z / p.segments;
-        split = group % p.splits;
-        group /= p.splits;
-        row = blockIdx.y * BM;
-        lim = min(BM, p.n - row);
-        int begin, end;
-        split_rows(start[group + 1] - start[group], p.splits, split, begin, end);
-        length = end - begin;
-        begin += start[group];
-        a0 = static_cast<const float*>(p.a[part].p) + begin * p.a[part].row + row;
-        b0 = static_cast<const float*>(p.b[0].p) + begin * p.b[0].row + col;
-    } else {
-        if ((int)blockIdx.y >= tile[p.groups + 1]) return;
-        group = group_of(tile, p.groups, blockIdx.y);
-        row = start[group] + ((int)blockIdx.y - tile[group]) * BM;
-        lim = min(BM, start[group + 1] - row);
-        length = group == p.groups ? 0 : p.k;
-        a0 = b0 = nullptr;
-    }
-    uint64_t acc[8][4];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = 0;
-    for (int seg = 0; seg < (FORM == kBack ? p.segments : 1) && length > 0; ++seg) {
-        int64_t arow, brow;
-        int blim = min(COLS, (FORM == kWeights ? p.k : p.n) - col);
-        const float* b1 = nullptr;
+    const int col = blockIdx.y * COLS;
+    int row, lim, length, group, part = 0, split = 0, first = 0;  // lim: rows of the tile that are the output's
+    {
+        int *start = memory.groups[0], *tile = memory.groups[1];
+        read_groups(p.offsets, p.groups, p.rows, TILE, start, tile);
         if (FORM == kWeights) {
-            arow = p.a[part].row;
-            brow = p.b[0].row;
+            part = blockIdx.z % p.segments;
+            group = blockIdx.z / p.segments;
+            split = group % p.splits;
+            group /= p.splits;
+            row = blockIdx.x * TILE;
+            lim = min(TILE, p.n - row);
+            int end;
+            split_rows(start[group + 1] - start[group], p.splits, split, first, end);
+            length = end - first;
+            first += start[group];
         } else {
-            arow = p.a[seg].row;
-            a0 = static_cast<const float*>(p.a[seg].p) + row * arow;
-            brow = p.b[seg].row;
-            b0 = static_cast<const float*>(p.b[seg].p) + group * p.b[seg].group + (B_LONG ? col * brow : col);
-            if (HALVES) b1 = static_cast<const float*>(p.b[1].p) + group * p.b[1].group + col * p.b[1].row;
+            if ((int)blockIdx.x >= tile[p.groups + 1]) return;
+            group = group_of(tile, p.groups, blockIdx.x);
+            row = start[group] + ((int)blockIdx.x - tile[group]) * TILE;
+            lim = min(TILE, start[group + 1] - row);
+            length = group == p.groups ? 0 : p.k;
         }
-        float ra[4], rb[4];
-        auto load = [&](int k0) {
-            fetch<A_LONG>(ra, a0, arow, lim, k0, length - k0);
-            if (HALVES) {  // places 0-63 of the tile are g's columns, 64-127 u's
-                const int t = threadIdx.x;
+        __syncthreads();  // the stages lie over the groups
+    }
+    const int width = FORM == kWeights ? p.k : p.n;
+    uint64_t acc[NR][NR / 2];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int k = t & 7, m = (t >> 3) + 32 * i, c = m & 63;
-                    rb[i] = c < blim && k0 + k < length ? __ldg((m < 64 ? b0 + c * brow : b1 + c * p.b[1].row) + k0 + k) : 0.0f;
-                }
+    for (int i = 0; i < NR; ++i)
+#pragma unroll
+        for (int j = 0; j < NR / 2; ++j) acc[i][j] = 0;
+    const uint32_t base = (uint32_t)__cvta_generic_to_shared(&memory.stage[0][0][0]);
+    for (int seg = 0; seg < (FORM == kBack ? p.segments : 1) && length > 0; ++seg) {
+        Source<TILE, A_LONG> a;
+        Source<TILE, B_LONG> b;
+        const int blim = min(COLS, width - col);
+        if (FORM == kWeights) {
+            const Operand &x = p.a[part], &y = p.b[0];
+            a.template start<false>(static_cast<const float*>(x.p) + first * x.row + row, nullptr, x.row, 0, lim, PITCH);
+            b.template start<false>(static_cast<const float*>(y.p) + first * y.row + col, nullptr, y.row, 0, blim, PITCH);
+        } else {
+            const Operand &x = p.a[seg], &y = p.b[seg];
+            a.template start<false>(static_cast<const float*>(x.p) + row * x.row, nullptr, x.row, 0, lim, PITCH);
+            const float* from = static_cast<const float*>(y.p) + group * y.group;
+            if (HALVES) {
+                const Operand& z = p.b[1];
+                b.template start<true>(from + col * y.row, static_cast<const float*>(z.p) + group * z.group + col * z.row, y.row, z.row, blim, PITCH);
             } else {
-                fetch<B_LONG>(rb, b0, brow, blim, k0, length - k0);
+                b.template start<false>(from + (B_LONG ? col * y.row : col), nullptr, y.row, 0, blim, PITCH);
             }
+        }
+        const int steps = (length + BK - 1) / BK;
+        auto bring = [&](int step) {
+            if (step < steps) {
+                const uint32_t to = base + step % kStages * 2 * STAGE * 4;
+                a.copy(to, length - step * BK, PITCH);
+                b.copy(to + STAGE * 4, length - step * BK, PITCH);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
         };
-        load(0);
-        stage<A_LONG>(as[0], ra);
-        stage<B_LONG>(bs[0], rb);
-        __syncthreads();
-        int buf = 0;
-        for (int k0 = 0; k0 < length; k0 += BK) {
-            const bool more = k0 + BK < length;
-            if (more) load(k0 + BK);
+        for (int step = 0; step < kStages - 1; ++step) bring(step);
+        for (int step = 0; step < steps; ++step) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+            __syncthreads();  // this step's elements are there, and the step before is read
+            bring(step + kStages - 1);
+            const float *as = memory.stage[step % kStages][0], *bs = memory.stage[step % kStages][1];
 #pragma unroll
             for (int k = 0; k < BK; ++k) {
-                const float4 a_lo = *reinterpret_cast<const float4*>(&as[buf][k][ty * 4]);
-                const float4 a_hi = *reinterpret_cast<const float4*>(&as[buf][k][64 + ty * 4]);
-                const ulonglong2 b_lo = *reinterpret_cast<const ulonglong2*>(&bs[buf][k][tx * 4]);
-                const ulonglong2 b_hi = *reinterpret_cast<const ulonglong2*>(&bs[buf][k][64 + tx * 4]);
-                const float av[8] = {a_lo.x, a_lo.y, a_lo.z, a_lo.w, a_hi.x, a_hi.y, a_hi.z, a_hi.w};
+                float av[NR];
+                uint64_t bv[NR / 2];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int h = 0; h < 2; ++h) {
+                    const float* pa = as + k * PITCH + h * (TILE / 2) + ty * HR;
+                    const float* pb = bs + k * PITCH + h * (TILE / 2) + tx * HR;
+                    if constexpr (HR == 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(pa);
+                        av[h * 4] = f.x, av[h * 4 + 1] = f.y, av[h * 4 + 2] = f.z, av[h * 4 + 3] = f.w;
+                        const ulonglong2 u = *reinterpret_cast<const ulonglong2*>(pb);
+                        bv[h * 2] = u.x, bv[h * 2 + 1] = u.y;
+                    } else {
+                        const float2 f = *reinterpret_cast<const float2*>(pa);
+                        av[h * 2] = f.x, av[h * 2 + 1] = f.y;
+                        bv[h] = *reinterpret_cast<const uint64_t*>(pb);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < NR; ++i) {
                     const uint64_t aa = pack(av[i], av[i]);
-                    fma2(acc[i][0], aa, b_lo.x);
-                    fma2(acc[i][1], aa, b_lo.y);
-                    fma2(acc[i][2], aa, b_hi.x);
-                    fma2(acc[i][3], aa, b_hi.y);
+#pragma unroll
+                    for (int j = 0; j < NR / 2; ++j) fma2(acc[i][j], aa, bv[j]);
                 }
             }
-            if (more) {
-                stage<A_LONG>(as[buf ^ 1], ra);
-                stage<B_LONG>(bs[buf ^ 1], rb);
-            }
-            __syncthreads();
-            buf ^= 1;
         }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();  // the next segment writes the stages
     }
     float* out = p.out[FORM == kWeights ? part : 0];
     int64_t out_row = p.out_row;
@@ -169,19 +221,18 @@ __global__ void __launch_bounds__(kThreads, 2) f32_kernel(const __grid_constant_
             out += (int64_t)group * p.n * out_row;
         }
     }
-    const int width = FORM == kWeights ? p.k : p.n;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int m = (i < 4 ? 0 : 60) + ty * 4 + i;
+    for (int i = 0; i < NR; ++i) {
+        const int m = i / HR * (TILE / 2) + ty * HR + i % HR;
         if (m >= lim) continue;
         const int64_t r = (int64_t)(row + m) * out_row;
 #pragma unroll
-        for (int j = 0; j < (HALVES ? 4 : 8); ++j) {
-            const int c = col + (j < 4 ? 0 : 60) + tx * 4 + j;
+        for (int j = 0; j < (HALVES ? HR : NR); ++j) {
+            const int c = col + j / HR * (TILE / 2) + tx * HR + j % HR;
             if (c >= width) continue;
             const float v = half_of(acc[i][j / 2], j & 1);
             if (HALVES) {
-                const float u = half_of(acc[i][2 + j / 2], j & 1);
+                const float u = half_of(acc[i][HR / 2 + j / 2], j & 1);
                 float slope;
                 const float act = activate<true, FORM == kGatedGrad>(p.activation, v, slope);
                 if (FORM == kGated) {
@@ -200,13 +251,12 @@ __global__ void __launch_bounds__(kThreads, 2) f32_kernel(const __grid_constant_
     }
 }
 
-template <int FORM>
+template <int FORM, int TILE>
 cudaError_t launch_f32(const Params& p, cudaStream_t st) {
-    const int width = FORM == kWeights ? p.k : p.n, cols = FORM == kGated || FORM == kGatedGrad ? BN / 2 : BN;
-    dim3 grid((width + cols - 1) / cols, FORM == kWeights ? (p.n + BM - 1) / BM : p.rows / BM + p.groups + 1,
-              FORM == kWeights ? p.splits * p.segments * p.groups : 1);
-    if (grid.y > 65535 || grid.z > 65535) return cudaErrorInvalidConfiguration;
-    f32_kernel<FORM><<<grid, kThreads, 0, st>>>(p);
+    const int width = FORM == kWeights ? p.k : p.n, cols = FORM == kGated || FORM == kGatedGrad ? TILE / 2 : TILE;
+    const dim3 grid(FORM == kWeights ? (p.n + TILE - 1) / TILE : p.rows / TILE + p.groups + 1, (width + cols - 1) / cols,
+                    FORM == kWeights ? p.splits * p.segments * p.groups : 1);
+    f32_kernel<FORM, TILE><<<grid, kThreads, 0, st>>>(p);
     count_launches(1);
     return cudaGetLastError();
 }
@@ -350,13 +400,21 @@ cudaError_t product_f32(const Job& job, cudaStream_t st) {
     p.out_row = job.out_row;
     p.partial = job.partial;
     for (int i = 0; i < 2; ++i) p.a[i] = job.a[i], p.b[i] = job.b[i], p.out[i] = static_cast<float*>(job.out[i]);
+    const bool wide = f32_tile(job) == 128;
     switch (job.form) {
-        case kProduct: return launch_f32<kProduct>(p, st);
-        case kGated: return launch_f32<kGated>(p, st);
-        case kGatedGrad: return launch_f32<kGatedGrad>(p, st);
-        case kBack: return launch_f32<kBack>(p, st);
-        default: return launch_f32<kWeights>(p, st);
+        case kProduct: return wide ? launch_f32<kProduct, 128>(p, st) : launch_f32<kProduct, 64>(p, st);
+        case kGated: return wide ? launch_f32<kGated, 128>(p, st) : launch_f32<kGated, 64>(p, st);
+        case kGatedGrad: return wide ? launch_f32<kGatedGrad, 128>(p, st) : launch_f32<kGatedGrad, 64>(p, st);
+        case kBack: return wide ? launch_f32<kBack, 128>(p, st) : launch_f32<kBack, 64>(p, st);
+        default: return wide ? launch_f32<kWeights, 128>(p, st) : launch_f32<kWeights, 64>(p, st);
     }
+}
+
+int f32_tile(const Job& job) {
+    const int64_t cols = job.form == kGated || job.form == kGatedGrad ? 64 : 128, width = job.form == kWeights ? job.k : job.n;
+    const int64_t tiles = (width + cols - 1) / cols *
+                          (job.form == kWeights ? job.segments * (int64_t)job.groups * ((job.n + 127) / 128) : job.rows / 128 + job.groups / 2);
+    return tiles * (job.form == kWeights ? std::max<int64_t>(1, job.rows / job.groups / 1024) : 1) < 2 * 148 ? 64 : 128;
 }
 
 cudaError_t join_parts(const Job& job, cudaStream_t st) {
