@@ -2,8 +2,10 @@
 //
 // fp32 (product_f32): every form of experts.cu in tiles of 128 x 128 or 64 x 64, 8 of the summed length a step.  Each
 // thread copies its elements straight to shared memory (asynchronous copies of 4 bytes, which take any alignment and
-// order and write zeros for what is not there), four steps ahead; it holds 8 x 8 or 4 x 4 sums and adds products in
-// pairs (fma.rn.f32x2), each rounded like the scalar instruction, so the sums are plain fp32 sums.  The tensor cores
+// order and write zeros for what is not there), three steps ahead; it holds 8 x 16 or 8 x 8 sums and adds products in
+// pairs (fma.rn.f32x2), each rounded like the scalar instruction, so the sums are plain fp32 sums.  Shared memory
+// returns 128 bytes a cycle, whatever the lanes share, and 8 x 8 sums want just that for 128 products a cycle: with
+// them 32768 x 2048 x 1024 ran at 47 TFLOP/s.  The tensor cores
 // would need three bf16 parts of each operand and cut off the low bits of their running sums, which fp32 results do
 // not allow.  In the gated forms half of a tile's columns are g's and half the same places of u, and one thread
 // holds both of a place.
@@ -23,7 +25,7 @@ namespace experts {
 namespace {
 
 // ---------------------------------------------------------------- fp32 tiles
-constexpr int BK = 8, kStages = 4, kThreads = 256;
+constexpr int BK = 8, kStages = 4;
 
 struct Params {
     const int32_t* offsets;
@@ -47,10 +49,10 @@ __device__ __forceinline__ void copy4(uint32_t to, const float* from, bool there
 }
 
 // What a thread copies of an operand's TILE x 8 values each step.  LONG: the operand's rows run along the summed length,
-// and 8 threads take 8 neighbours of a row; else across it, and TILE threads take neighbours of one place of the length.
+// and 8 threads take 8 neighbours of a row; else across it, and the threads take neighbours of one place of the length.
 template <int TILE, bool LONG>
 struct Source {
-    static constexpr int EACH = TILE * BK / kThreads, ACROSS = kThreads / TILE;  // elements of a thread; LONG: 32 rows apart
+    static constexpr int EACH = BK, APART = TILE / 8;  // elements of each of TILE threads; LONG: rows apart
     const float* at[LONG ? EACH : 1];
     int64_t step;  // from one step to the next
     int64_t row;
@@ -70,18 +72,17 @@ struct Source {
             to = (k * pitch + m0) * 4;
 #pragma unroll
             for (int i = 0; i < EACH; ++i) {
-                const int m = m0 + 32 * i, place = HALVES ? m % (TILE / 2) : m;
+                const int m = m0 + APART * i, place = HALVES ? m % (TILE / 2) : m;
                 const int there = place < lim ? place : 0;
                 at[i] = (HALVES && m >= TILE / 2 ? other + there * other_stride : base + there * stride) + k;
                 live |= (place < lim ? 1u : 0u) << i;
             }
         } else {
-            const int m = t % TILE;
-            k = t / TILE;
+            k = 0;
             step = BK * stride;
-            to = (k * pitch + m) * 4;
-            at[0] = base + (m < lim ? m : 0) + (int64_t)k * stride;
-            live = m < lim ? ~0u : 0u;
+            to = t * 4;
+            at[0] = base + (t < lim ? t : 0);
+            live = t < lim ? ~0u : 0u;
         }
     }
     // The next step's elements; `left` of the length are left.
@@ -90,12 +91,11 @@ struct Source {
         for (int i = 0; i < EACH; ++i) {
             if (LONG) {
                 const bool there = (live >> i & 1) && k < left;
-                copy4(stage + to + 32 * i * 4, there ? at[i] : at[0], there);
+                copy4(stage + to + APART * i * 4, there ? at[i] : at[0], there);
                 if (k + BK < left) at[i] += step;
             } else {
-                const int kk = k + ACROSS * i;
-                const bool there = live && kk < left;
-                copy4(stage + to + ACROSS * i * pitch * 4, there ? at[0] + (int64_t)(ACROSS * i) * row : at[0], there);
+                const bool there = live && i < left;
+                copy4(stage + to + i * pitch * 4, there ? at[0] + i * row : at[0], there);
             }
         }
         if (!LONG && k + BK < left) at[0] += step;
@@ -103,18 +103,18 @@ struct Source {
 };
 
 template <int FORM, int TILE>
-__global__ void __launch_bounds__(kThreads, TILE == 128 ? 2 : 4) f32_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(TILE, TILE == 128 ? 2 : 8) f32_kernel(const __grid_constant__ Params p) {
     constexpr bool HALVES = FORM == kGated || FORM == kGatedGrad;
     constexpr bool A_LONG = FORM != kWeights, B_LONG = FORM != kWeights && FORM != kBack;
     constexpr int COLS = HALVES ? TILE / 2 : TILE, PITCH = TILE + 4;
-    constexpr int NR = TILE / 16, HR = NR / 2;  // sums of a thread: NR x NR, in four blocks of HR x HR half a tile apart
+    constexpr int NR = 8, NQ = TILE / 32;       // a thread's rows, and its blocks of 4 columns, 32 apart
     constexpr int STAGE = BK * PITCH;           // floats of an operand
     union Memory {
         float stage[kStages][2][STAGE];
         int groups[2][kMostGroups + 2];  // until the block knows its rows
     };
     __shared__ __align__(16) Memory memory;
-    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    const int tid = threadIdx.x, tx = tid & 7, ty = tid >> 3;
     const int col = blockIdx.y * COLS;
     int row, lim, length, group, part = 0, split = 0, first = 0;  // lim: rows of the tile that are the output's
     {
@@ -141,11 +141,11 @@ __global__ void __launch_bounds__(kThreads, TILE == 128 ? 2 : 4) f32_kernel(cons
         __syncthreads();  // the stages lie over the groups
     }
     const int width = FORM == kWeights ? p.k : p.n;
-    uint64_t acc[NR][NR / 2];
+    uint64_t acc[NR][2 * NQ];
 #pragma unroll
     for (int i = 0; i < NR; ++i)
 #pragma unroll
-        for (int j = 0; j < NR / 2; ++j) acc[i][j] = 0;
+        for (int j = 0; j < 2 * NQ; ++j) acc[i][j] = 0;
     const uint32_t base = (uint32_t)__cvta_generic_to_shared(&memory.stage[0][0][0]);
     for (int seg = 0; seg < (FORM == kBack ? p.segments : 1) && length > 0; ++seg) {
         Source<TILE, A_LONG> a;
@@ -184,27 +184,22 @@ __global__ void __launch_bounds__(kThreads, TILE == 128 ? 2 : 4) f32_kernel(cons
 #pragma unroll
             for (int k = 0; k < BK; ++k) {
                 float av[NR];
-                uint64_t bv[NR / 2];
+                uint64_t bv[2 * NQ];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const float* pa = as + k * PITCH + h * (TILE / 2) + ty * HR;
-                    const float* pb = bs + k * PITCH + h * (TILE / 2) + tx * HR;
-                    if constexpr (HR == 4) {
-                        const float4 f = *reinterpret_cast<const float4*>(pa);
-                        av[h * 4] = f.x, av[h * 4 + 1] = f.y, av[h * 4 + 2] = f.z, av[h * 4 + 3] = f.w;
-                        const ulonglong2 u = *reinterpret_cast<const ulonglong2*>(pb);
-                        bv[h * 2] = u.x, bv[h * 2 + 1] = u.y;
-                    } else {
-                        const float2 f = *reinterpret_cast<const float2*>(pa);
-                        av[h * 2] = f.x, av[h * 2 + 1] = f.y;
-                        bv[h] = *reinterpret_cast<const uint64_t*>(pb);
-                    }
+                    const float4 f = *reinterpret_cast<const float4*>(as + k * PITCH + h * (TILE / 2) + ty * 4);
+                    av[h * 4] = f.x, av[h * 4 + 1] = f.y, av[h * 4 + 2] = f.z, av[h * 4 + 3] = f.w;
+                }
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) {
+                    const ulonglong2 u = *reinterpret_cast<const ulonglong2*>(bs + k * PITCH + q * 32 + tx * 4);
+                    bv[2 * q] = u.x, bv[2 * q + 1] = u.y;
                 }
 #pragma unroll
                 for (int i = 0; i < NR; ++i) {
                     const uint64_t aa = pack(av[i], av[i]);
 #pragma unroll
-                    for (int j = 0; j < NR / 2; ++j) fma2(acc[i][j], aa, bv[j]);
+                    for (int j = 0; j < 2 * NQ; ++j) fma2(acc[i][j], aa, bv[j]);
                 }
             }
         }
@@ -223,16 +218,16 @@ __global__ void __launch_bounds__(kThreads, TILE == 128 ? 2 : 4) f32_kernel(cons
     }
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
-        const int m = i / HR * (TILE / 2) + ty * HR + i % HR;
+        const int m = i / 4 * (TILE / 2) + ty * 4 + i % 4;
         if (m >= lim) continue;
         const int64_t r = (int64_t)(row + m) * out_row;
 #pragma unroll
-        for (int j = 0; j < (HALVES ? HR : NR); ++j) {
-            const int c = col + j / HR * (TILE / 2) + tx * HR + j % HR;
+        for (int j = 0; j < (HALVES ? 2 * NQ : 4 * NQ); ++j) {  // HALVES: the second half of the blocks is u's
+            const int c = col + j / 4 * 32 + tx * 4 + j % 4;
             if (c >= width) continue;
             const float v = half_of(acc[i][j / 2], j & 1);
             if (HALVES) {
-                const float u = half_of(acc[i][HR / 2 + j / 2], j & 1);
+                const float u = half_of(acc[i][NQ + j / 2], j & 1);
                 float slope;
                 const float act = activate<true, FORM == kGatedGrad>(p.activation, v, slope);
                 if (FORM == kGated) {
@@ -256,7 +251,7 @@ cudaError_t launch_f32(const Params& p, cudaStream_t st) {
     const int width = FORM == kWeights ? p.k : p.n, cols = FORM == kGated || FORM == kGatedGrad ? TILE / 2 : TILE;
     const dim3 grid(FORM == kWeights ? (p.n + TILE - 1) / TILE : p.rows / TILE + p.groups + 1, (width + cols - 1) / cols,
                     FORM == kWeights ? p.splits * p.segments * p.groups : 1);
-    f32_kernel<FORM, TILE><<<grid, kThreads, 0, st>>>(p);
+    f32_kernel<FORM, TILE><<<grid, TILE, 0, st>>>(p);
     count_launches(1);
     return cudaGetLastError();
 }
