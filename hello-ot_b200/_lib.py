@@ -30,7 +30,7 @@ EXPORTS = ("hb_abi_version", "hb_last_error", "hb_kernel_launch_count", "hb_set_
            "hb_clip_grad_norm", "hb_expert_product", "hb_expert_gated", "hb_expert_product_grad_workspace",
            "hb_expert_product_grad", "hb_expert_gated_grad_workspace", "hb_expert_gated_grad", "hb_rms_norm",
            "hb_rows_of_8bit", "hb_rms_norm_grad_workspace", "hb_rms_norm_grad", "hb_adamw_workspace", "hb_adamw_step",
-           "hb_adamw_moments")
+           "hb_adamw_moments", "hb_expert_any_grid", "hb_expert_copy")
 
 
 class HBError(RuntimeError):
@@ -181,6 +181,10 @@ def load_library(path: Path | str = LIB_PATH):
     lib.hb_clip_grad_norm.restype = c_int
     lib.hb_clip_grad_norm.argtypes = [c_int64, P, P, P, P, P, c_double, P, P, c_size_t, P]
     S, W = POINTER(ExpertShape), POINTER(ExpertWeight)
+    lib.hb_expert_any_grid.restype = c_int
+    lib.hb_expert_any_grid.argtypes = [S, c_int]
+    lib.hb_expert_copy.restype = c_int
+    lib.hb_expert_copy.argtypes = [c_int64] + [P] * 9
     lib.hb_expert_product.restype = c_int
     lib.hb_expert_product.argtypes = [S, P, c_int64, P, W, P, P]
     lib.hb_expert_gated.restype = c_int

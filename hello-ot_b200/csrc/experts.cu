@@ -798,7 +798,7 @@ constexpr int kSlots = 148, kLeastStages = 16;
 int splits_of(const Job& job) {
     const bool f32 = job.type == HB_F32, pair = !f32 && use_pairs(job);
     const int64_t side = f32 ? f32_tile(job) : pair ? 256 : 128;
-    const int64_t slots = f32 ? kSlots * (side == 128 ? 2 : 4) : pair ? kSlots / 2 : kSlots;  // resident tiles
+    const int64_t slots = f32 ? kSlots * (side == 128 ? 2 : 5) : pair ? kSlots / 2 : kSlots;  // resident tiles
     const int64_t tiles = job.segments * (int64_t)job.groups * ((job.n + side - 1) / side) * ((job.k + side - 1) / side);
     const int64_t stages = (job.rows / job.groups + 63) / 64;
     return (int)std::max<int64_t>(1, std::min(slots / tiles, stages / (f32 ? 2 : kLeastStages)));
@@ -815,7 +815,7 @@ int run_pairs(const Job& job, cudaStream_t st) {
 int run(const Job& job, cudaStream_t st) {
     const bool row_form = job.form == kProduct || job.form == kGated;
     cudaError_t e = cudaSuccess;
-    if (row_form && job.rows <= kFewRows) e = few_rows(job, st);
+    if (row_form && is_few(job.type, job.rows, job.groups, job.n, job.k, job.form == kGated ? 2 : 1)) e = few_rows(job, st);
     else if (job.type == HB_F32) e = product_f32(job, st);
     else {
         int rc;
@@ -889,12 +889,73 @@ Operand weight_of(const hb_expert_weight* w) { return w ? Operand{w->data, w->ro
 bool aligned_out(const void* p, int type) { return rows::address_bits(p) % rows::type_bytes(type) == 0; }
 }  // namespace
 
+extern "C" int hb_expert_any_grid(const hb_expert_shape* s, int weights) {
+    return s && (s->type == HB_F32 || is_few(s->type, s->rows, s->experts, s->hidden, s->width, weights));
+}
+
+// Up to three operands copied to rows on 16 bytes: a warp a row.
+namespace hb {
+namespace experts {
+struct Copies {
+    const uint16_t* from[3];
+    uint16_t* to[3];
+    int64_t row[3], group[3], to_row[3];
+    int64_t rows[3], first[3];  // rows of a group; first row of the operand among all
+    int width[3], count;
+};
+__global__ void __launch_bounds__(256) copy_kernel(const __grid_constant__ Copies c, int64_t total) {
+    const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (r >= total) return;
+    int i = 0;
+    while (i + 1 < c.count && r >= c.first[i + 1]) ++i;
+    const int64_t at = r - c.first[i], g = at / c.rows[i];
+    const uint16_t* from = c.from[i] + g * c.group[i] + (at - g * c.rows[i]) * c.row[i];
+    uint16_t* to = c.to[i] + at * c.to_row[i];
+#pragma unroll 4
+    for (int k = threadIdx.x & 31; k < c.width[i]; k += 32) to[k] = from[k];
+}
+}  // namespace experts
+}  // namespace hb
+
+extern "C" int hb_expert_copy(int64_t count, const void* const* from, const int64_t* groups, const int64_t* rows, const int64_t* width,
+                              const int64_t* group_stride, const int64_t* row_stride, void* const* to, const int64_t* to_stride,
+                              void* stream) {
+    if (count < 0 || count > 3 || (count > 0 && (!from || !groups || !rows || !width || !group_stride || !row_stride || !to || !to_stride)))
+        return abi_fail(HB_BAD_ARGUMENT, "hb_expert_copy: at most 3 operands, no null pointer");
+    Copies c{};
+    int64_t total = 0;
+    for (int64_t i = 0; i < count; ++i) {
+        if (groups[i] < 0 || rows[i] < 0 || width[i] < 1 || width[i] > INT32_MAX || to_stride[i] < width[i] ||
+            (groups[i] > 0 && rows[i] > INT64_MAX / 4 / groups[i]))
+            return abi_fail(HB_BAD_ARGUMENT, "hb_expert_copy: shape of an operand");
+        if (groups[i] * rows[i] == 0) continue;
+        if (!from[i] || !to[i] || rows::address_bits(from[i]) % 2 || rows::address_bits(to[i]) % 2)
+            return abi_fail(HB_BAD_ARGUMENT, "hb_expert_copy: null or misaligned pointer");
+        const int at = c.count++;
+        c.from[at] = static_cast<const uint16_t*>(from[i]);
+        c.to[at] = static_cast<uint16_t*>(to[i]);
+        c.row[at] = row_stride[i];
+        c.group[at] = group_stride[i];
+        c.to_row[at] = to_stride[i];
+        c.rows[at] = rows[i];
+        c.width[at] = (int)width[i];
+        c.first[at] = total;
+        total += groups[i] * rows[i];
+    }
+    if (total == 0) return HB_OK;
+    if ((total + 7) / 8 > INT32_MAX) return abi_fail(HB_BAD_ARGUMENT, "hb_expert_copy: too many rows");
+    copy_kernel<<<(unsigned)((total + 7) / 8), 256, 0, static_cast<cudaStream_t>(stream)>>>(c, total);
+    count_launches(1);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? HB_OK : abi_fail(HB_LAUNCH, std::string("hb_expert_copy: ") + cudaGetErrorString(e));
+}
+
 extern "C" int hb_expert_product(const hb_expert_shape* s, const void* x, int64_t x_stride, const int32_t* offsets,
                                  const hb_expert_weight* weight, void* out, void* stream) {
     const char* what = "hb_expert_product";
     if (const int rc = check(s, offsets, what)) return rc;
     if (s->rows == 0) return HB_OK;
-    const bool grid = s->rows > kFewRows;
+    const bool grid = !hb_expert_any_grid(s, 1);
     Job j = job_of(s, offsets, kProduct, s->hidden, s->width);
     j.a[0] = rows_of(x, x_stride);
     j.b[0] = weight_of(weight);
@@ -912,7 +973,7 @@ extern "C" int hb_expert_gated(const hb_expert_shape* s, const void* x, int64_t 
     const char* what = "hb_expert_gated";
     if (const int rc = check(s, offsets, what)) return rc;
     if (s->rows == 0) return HB_OK;
-    const bool grid = s->rows > kFewRows;
+    const bool grid = !hb_expert_any_grid(s, 2);
     Job j = job_of(s, offsets, kGated, s->hidden, s->width);
     j.a[0] = rows_of(x, x_stride);
     j.b[0] = weight_of(gate);

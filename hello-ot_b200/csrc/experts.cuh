@@ -122,13 +122,32 @@ __device__ __forceinline__ float activate(int kind, float g, float& slope) {
         if (SLOPE) slope = s * fmaf(g, 1.0f - s, 1.0f);
         return g * s;
     }
-    const float cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
-    if (SLOPE) slope = fmaf(g * 0.39894228040143268f, exponential<PRECISE>(-0.5f * g * g), cdf);
+    float cdf, bell = 0.0f;
+    if (PRECISE) {
+        cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
+        if (SLOPE) bell = expf(-0.5f * g * g);
+    } else {
+        // The complement of the error function after Abramowitz and Stegun 7.1.26, off by at most 1.5e-7 of 1 (the gated
+        // product of 73879 x 6 x 190 x 696 f16, bound by erff, 141 -> 97 us)
+        const float x = fabsf(g) * 0.70710678118654752f;
+        float t;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(0.3275911f, x, 1.0f)));
+        bell = exponential<false>(-x * x);
+        const float poly = fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+        const float tail = 0.5f * t * poly * bell;
+        cdf = g < 0.0f ? tail : 1.0f - tail;  // a NaN stays
+    }
+    if (SLOPE) slope = fmaf(g * 0.39894228040143268f, bell, cdf);
     return g * cdf;
 }
 
-// Up to this many rows the weights are streamed by warps (experts_simt.cu), any type.
-constexpr int kFewRows = HB_EXPERT_FEW_ROWS;
+// Whether a forward product streams the weights by warps (experts_simt.cu): few rows, or few for each expert in fp32 or where
+// there is little work.  Gated, streamed and in tiles (us): 64 x 64 x 512 x 512 f32 29 and 125, 128 x 64 41 and 126,
+// 273 x 73 x 25 x 24 f16 8.6 and 12.5; but 487 x 117 x 18 x 50 f16 18.7 and 14.7, 100 x 21 x 886 x 719 f32 above both.
+constexpr int64_t kFewRows = 16, kFewEach = 4, kFewWork = 1 << 24;  // rows, rows an expert, products
+inline bool is_few(int type, int64_t rows, int64_t experts, int64_t n, int64_t k, int weights) {
+    return rows <= kFewRows || (rows <= kFewEach * experts && (type == HB_F32 || rows * n * k * weights <= kFewWork));
+}
 cudaError_t few_rows(const Job& job, cudaStream_t st);
 cudaError_t product_f32(const Job& job, cudaStream_t st);
 // The side of product_f32's tiles: 64 where tiles of 128 would leave SMs without one.

@@ -2,7 +2,7 @@
 //
 // fp32 (product_f32): every form of experts.cu in tiles of 128 x 128 or 64 x 64, 8 of the summed length a step.  Each
 // thread copies its elements straight to shared memory (asynchronous copies of 4 bytes, which take any alignment and
-// order and write zeros for what is not there), three steps ahead; it holds 8 x 16 or 8 x 8 sums and adds products in
+// order and write zeros for what is not there), three steps ahead; it holds 8 x 16 or 8 x 4 sums and adds products in
 // pairs (fma.rn.f32x2), each rounded like the scalar instruction, so the sums are plain fp32 sums.  Shared memory
 // returns 128 bytes a cycle, whatever the lanes share, and 8 x 8 sums want just that for 128 products a cycle: with
 // them 32768 x 2048 x 1024 ran at 47 TFLOP/s.  The tensor cores
@@ -10,8 +10,7 @@
 // not allow.  In the gated forms half of a tile's columns are g's and half the same places of u, and one thread
 // holds both of a place.
 //
-// Few rows (few_rows, at most 16 of all experts together): one token's step of a decode batch reads the named
-// experts' weights once and is bound by that.  A warp streams the weight rows of one output column and multiplies
+// Few rows (few_rows): one token's step of a decode batch reads the named experts' weights once and is bound by that.  A warp streams the weight rows of one output column and multiplies
 // them with up to 8 rows of x, which stay in L1; a block of 8 warps takes 8 columns for the rows of one expert,
 // which the expert's first row finds out for itself.
 #include <algorithm>
@@ -25,7 +24,7 @@ namespace experts {
 namespace {
 
 // ---------------------------------------------------------------- fp32 tiles
-constexpr int BK = 8, kStages = 4;
+constexpr int BK = 8, kStages = 4, kThreads = 128;
 
 struct Params {
     const int32_t* offsets;
@@ -52,7 +51,7 @@ __device__ __forceinline__ void copy4(uint32_t to, const float* from, bool there
 // and 8 threads take 8 neighbours of a row; else across it, and the threads take neighbours of one place of the length.
 template <int TILE, bool LONG>
 struct Source {
-    static constexpr int EACH = BK, APART = TILE / 8;  // elements of each of TILE threads; LONG: rows apart
+    static constexpr int EACH = TILE * BK / kThreads, APART = kThreads / 8, ACROSS = kThreads / TILE;  // LONG: rows apart; else places of the length
     const float* at[LONG ? EACH : 1];
     int64_t step;  // from one step to the next
     int64_t row;
@@ -78,11 +77,12 @@ struct Source {
                 live |= (place < lim ? 1u : 0u) << i;
             }
         } else {
-            k = 0;
+            const int m = t % TILE;
+            k = t / TILE;
             step = BK * stride;
-            to = t * 4;
-            at[0] = base + (t < lim ? t : 0);
-            live = t < lim ? ~0u : 0u;
+            to = (k * pitch + m) * 4;
+            at[0] = base + (m < lim ? m : 0) + k * stride;
+            live = m < lim ? ~0u : 0u;
         }
     }
     // The next step's elements; `left` of the length are left.
@@ -94,8 +94,8 @@ struct Source {
                 copy4(stage + to + APART * i * 4, there ? at[i] : at[0], there);
                 if (k + BK < left) at[i] += step;
             } else {
-                const bool there = live && i < left;
-                copy4(stage + to + i * pitch * 4, there ? at[0] + i * row : at[0], there);
+                const bool there = live && k + ACROSS * i < left;
+                copy4(stage + to + ACROSS * i * pitch * 4, there ? at[0] + ACROSS * i * row : at[0], there);
             }
         }
         if (!LONG && k + BK < left) at[0] += step;
@@ -103,18 +103,18 @@ struct Source {
 };
 
 template <int FORM, int TILE>
-__global__ void __launch_bounds__(TILE, TILE == 128 ? 2 : 8) f32_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, TILE == 128 ? 2 : 5) f32_kernel(const __grid_constant__ Params p) {
     constexpr bool HALVES = FORM == kGated || FORM == kGatedGrad;
     constexpr bool A_LONG = FORM != kWeights, B_LONG = FORM != kWeights && FORM != kBack;
     constexpr int COLS = HALVES ? TILE / 2 : TILE, PITCH = TILE + 4;
-    constexpr int NR = 8, NQ = TILE / 32;       // a thread's rows, and its blocks of 4 columns, 32 apart
+    constexpr int NR = 8, NQ = TILE / 32, QW = TILE / 32, NP = NQ * QW / 2;  // a thread's rows, its blocks of QW columns, 32 apart, pairs
     constexpr int STAGE = BK * PITCH;           // floats of an operand
     union Memory {
         float stage[kStages][2][STAGE];
         int groups[2][kMostGroups + 2];  // until the block knows its rows
     };
     __shared__ __align__(16) Memory memory;
-    const int tid = threadIdx.x, tx = tid & 7, ty = tid >> 3;
+    const int tid = threadIdx.x, tx = tid % (32 / QW), ty = tid / (32 / QW);
     const int col = blockIdx.y * COLS;
     int row, lim, length, group, part = 0, split = 0, first = 0;  // lim: rows of the tile that are the output's
     {
@@ -141,11 +141,11 @@ __global__ void __launch_bounds__(TILE, TILE == 128 ? 2 : 8) f32_kernel(const __
         __syncthreads();  // the stages lie over the groups
     }
     const int width = FORM == kWeights ? p.k : p.n;
-    uint64_t acc[NR][2 * NQ];
+    uint64_t acc[NR][NP];
 #pragma unroll
     for (int i = 0; i < NR; ++i)
 #pragma unroll
-        for (int j = 0; j < 2 * NQ; ++j) acc[i][j] = 0;
+        for (int j = 0; j < NP; ++j) acc[i][j] = 0;
     const uint32_t base = (uint32_t)__cvta_generic_to_shared(&memory.stage[0][0][0]);
     for (int seg = 0; seg < (FORM == kBack ? p.segments : 1) && length > 0; ++seg) {
         Source<TILE, A_LONG> a;
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(TILE, TILE == 128 ? 2 : 8) f32_kernel(const __
 #pragma unroll
             for (int k = 0; k < BK; ++k) {
                 float av[NR];
-                uint64_t bv[2 * NQ];
+                uint64_t bv[NP];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const float4 f = *reinterpret_cast<const float4*>(as + k * PITCH + h * (TILE / 2) + ty * 4);
@@ -192,14 +192,19 @@ __global__ void __launch_bounds__(TILE, TILE == 128 ? 2 : 8) f32_kernel(const __
                 }
 #pragma unroll
                 for (int q = 0; q < NQ; ++q) {
-                    const ulonglong2 u = *reinterpret_cast<const ulonglong2*>(bs + k * PITCH + q * 32 + tx * 4);
-                    bv[2 * q] = u.x, bv[2 * q + 1] = u.y;
+                    const float* from = bs + k * PITCH + q * 32 + tx * QW;
+                    if constexpr (QW == 4) {
+                        const ulonglong2 u = *reinterpret_cast<const ulonglong2*>(from);
+                        bv[2 * q] = u.x, bv[2 * q + 1] = u.y;
+                    } else {
+                        bv[q] = *reinterpret_cast<const uint64_t*>(from);
+                    }
                 }
 #pragma unroll
                 for (int i = 0; i < NR; ++i) {
                     const uint64_t aa = pack(av[i], av[i]);
 #pragma unroll
-                    for (int j = 0; j < 2 * NQ; ++j) fma2(acc[i][j], aa, bv[j]);
+                    for (int j = 0; j < NP; ++j) fma2(acc[i][j], aa, bv[j]);
                 }
             }
         }
@@ -222,12 +227,12 @@ __global__ void __launch_bounds__(TILE, TILE == 128 ? 2 : 8) f32_kernel(const __
         if (m >= lim) continue;
         const int64_t r = (int64_t)(row + m) * out_row;
 #pragma unroll
-        for (int j = 0; j < (HALVES ? 2 * NQ : 4 * NQ); ++j) {  // HALVES: the second half of the blocks is u's
-            const int c = col + j / 4 * 32 + tx * 4 + j % 4;
+        for (int j = 0; j < (HALVES ? NP : 2 * NP); ++j) {  // HALVES: the second half of the blocks is u's
+            const int c = col + j / QW * 32 + tx * QW + j % QW;
             if (c >= width) continue;
             const float v = half_of(acc[i][j / 2], j & 1);
             if (HALVES) {
-                const float u = half_of(acc[i][NQ + j / 2], j & 1);
+                const float u = half_of(acc[i][NP / 2 + j / 2], j & 1);
                 float slope;
                 const float act = activate<true, FORM == kGatedGrad>(p.activation, v, slope);
                 if (FORM == kGated) {
@@ -251,7 +256,7 @@ cudaError_t launch_f32(const Params& p, cudaStream_t st) {
     const int width = FORM == kWeights ? p.k : p.n, cols = FORM == kGated || FORM == kGatedGrad ? TILE / 2 : TILE;
     const dim3 grid(FORM == kWeights ? (p.n + TILE - 1) / TILE : p.rows / TILE + p.groups + 1, (width + cols - 1) / cols,
                     FORM == kWeights ? p.splits * p.segments * p.groups : 1);
-    f32_kernel<FORM, TILE><<<grid, TILE, 0, st>>>(p);
+    f32_kernel<FORM, TILE><<<grid, kThreads, 0, st>>>(p);
     count_launches(1);
     return cudaGetLastError();
 }
@@ -292,12 +297,26 @@ __device__ __forceinline__ int expert_of(const int32_t* offsets, int groups, int
     return e;
 }
 
-template <typename T, int VB, bool GATED>
+// 16 bytes of a row from element k on, zeros behind its end; VECTORS: rows lie on 16 bytes and end there.  Either way a
+// lane has the same elements, so the sums do not depend on where the rows lie.
+template <bool VECTORS, typename T>
+__device__ __forceinline__ void load_piece(rows::Vec<T, 16>& v, const T* row, int k, int end, bool once) {
+    if (VECTORS) {
+        if (k >= end) v.zero();
+        else if (once) v.load_once(row + k);
+        else v.load(row + k);
+    } else {
+#pragma unroll
+        for (int j = 0; j < rows::Vec<T, 16>::N; ++j) v.v[j] = k + j < end ? row[k + j] : rows::from_float<T>(0.0f);
+    }
+}
+
+template <typename T, bool VECTORS, bool GATED>
 __global__ void __launch_bounds__(kFewThreads) few_kernel(const __grid_constant__ FewParams p) {
-    using V = rows::Vec<T, VB>;
+    using V = rows::Vec<T, 16>;
     __shared__ int found;
-    const int r0 = blockIdx.y, lane = threadIdx.x & 31;
-    const int col = blockIdx.x * kFewWarps + (threadIdx.x >> 5);
+    const int r0 = blockIdx.x, lane = threadIdx.x & 31;
+    const int col = blockIdx.y * kFewWarps + (threadIdx.x >> 5);
     int e = 0, count = p.rows - r0;
     if (p.offsets) {
         e = expert_of(p.offsets, p.groups, r0, &found);
@@ -320,16 +339,14 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(const __grid_constant_
         float g[kPass], u[kPass];
 #pragma unroll
         for (int i = 0; i < kPass; ++i) g[i] = u[i] = 0.0f;
-        constexpr int U = 4;  // vectors of each weight row in flight
+        constexpr int U = 4;  // pieces of each weight row in flight
         for (int k = lane * V::N; k < p.k; k += 32 * V::N * U) {
             V a[U], b[U];
 #pragma unroll
             for (int q = 0; q < U; ++q) {
                 const int at = k + q * 32 * V::N;
-                if (at < p.k) {
-                    a[q].load_once(w0 + at);
-                    if (GATED) b[q].load_once(w1 + at);
-                }
+                load_piece<VECTORS>(a[q], w0, at, p.k, true);
+                if (GATED) load_piece<VECTORS>(b[q], w1, at, p.k, true);
             }
 #pragma unroll
             for (int q = 0; q < U; ++q) {
@@ -339,7 +356,7 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(const __grid_constant_
                 for (int i = 0; i < kPass; ++i) {
                     if (i >= here) break;
                     V xv;
-                    xv.load(x + i * p.x.row + at);
+                    load_piece<VECTORS>(xv, x + i * p.x.row, at, p.k, false);
 #pragma unroll
                     for (int j = 0; j < V::N; ++j) {
                         const float xf = rows::to_float(xv.v[j]);
@@ -368,14 +385,13 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(const __grid_constant_
 
 template <typename T>
 void launch_few(const FewParams& p, bool vectors, bool gated, cudaStream_t st) {
-    const dim3 grid((p.n + kFewWarps - 1) / kFewWarps, p.rows);
-    constexpr int B = (int)sizeof(T);
+    const dim3 grid(p.rows, (p.n + kFewWarps - 1) / kFewWarps);
     if (vectors) {
-        if (gated) few_kernel<T, 16, true><<<grid, kFewThreads, 0, st>>>(p);
-        else few_kernel<T, 16, false><<<grid, kFewThreads, 0, st>>>(p);
+        if (gated) few_kernel<T, true, true><<<grid, kFewThreads, 0, st>>>(p);
+        else few_kernel<T, true, false><<<grid, kFewThreads, 0, st>>>(p);
     } else {
-        if (gated) few_kernel<T, B, true><<<grid, kFewThreads, 0, st>>>(p);
-        else few_kernel<T, B, false><<<grid, kFewThreads, 0, st>>>(p);
+        if (gated) few_kernel<T, false, true><<<grid, kFewThreads, 0, st>>>(p);
+        else few_kernel<T, false, false><<<grid, kFewThreads, 0, st>>>(p);
     }
 }
 

@@ -515,49 +515,82 @@ PyObject* clip(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 // ---------------------------------------------------------------- experts
 int64_t on_eight(int64_t width) { return (width + 7) / 8 * 8; }
-// A copy whose rows begin on 16 bytes, for 16-bit operands off that grid.
-Tensor on_grid(const Tensor& t) {
-    c10::SmallVector<int64_t, 3> shape(t.sizes().begin(), t.sizes().end());
-    const int64_t width = shape.back();
-    shape.back() = on_eight(width);
-    Tensor copy = at::empty(shape, t.options()).narrow(-1, 0, width);
-    copy.copy_(t);
-    return copy;
-}
 bool off(const void* p, size_t unit) { return reinterpret_cast<uintptr_t>(p) % unit != 0; }
 
-// Sorted rows as the products take them; grid: 16-bit rows lie on 16 bytes and apart.
-Rows expert_rows(const Tensor& given, const char* name, bool grid) {
-    Rows r = feature_rows(given, name);
-    if (!grid || r.type == HB_F32 || r.t.numel() == 0) return r;
-    const int64_t width = r.t.size(1);
-    if (off(r.t.const_data_ptr(), 16) || (r.t.size(0) > 1 && (r.stride % 8 != 0 || r.stride < width)) || r.stride > INT32_MAX) {
-        r.t = on_grid(r.t);
-        r.stride = r.t.stride(0);
+// 16-bit operands off the 16-byte grid are copied to rows that lie on it, all of a call's in one launch into one buffer.
+struct Grid {
+    static constexpr int MOST = 3;
+    int count = 0;
+    Tensor buffer, source[MOST];
+    const void** pointer[MOST];  // where the copies' addresses and distances go
+    int64_t *row_out[MOST], *group_out[MOST];
+    int64_t groups[MOST], rows[MOST], width[MOST], group[MOST], row[MOST];
+    void add(const Tensor& t, const void** at, int64_t* row_at, int64_t* group_at) {
+        const int i = count++;
+        const bool weight = t.dim() == 3;
+        source[i] = t, pointer[i] = at, row_out[i] = row_at, group_out[i] = group_at;
+        groups[i] = weight ? t.size(0) : 1, rows[i] = t.size(-2), width[i] = t.size(-1);
+        group[i] = weight ? t.stride(0) : 0, row[i] = t.stride(-2);
     }
-    return r;
+    void copy(const Launch& on) {
+        if (count == 0) return;
+        int64_t at[MOST], stride[MOST], size = 0;
+        for (int i = 0; i < count; ++i) {
+            stride[i] = on_eight(width[i]);
+            at[i] = size;
+            size += (groups[i] * rows[i] * stride[i] * 2 + 255) / 256 * 256;
+        }
+        buffer = workspace(size, source[0].device());
+        const void* from[MOST];
+        void* to[MOST];
+        for (int i = 0; i < count; ++i) {
+            from[i] = source[i].const_data_ptr();
+            to[i] = static_cast<char*>(buffer.data_ptr()) + at[i];
+            *pointer[i] = to[i];
+            *row_out[i] = stride[i];
+            if (group_out[i]) *group_out[i] = rows[i] * stride[i];
+        }
+        check(hb_expert_copy(count, from, groups, rows, width, group, row, to, stride, on.stream));
+    }
+};
+
+// Sorted rows as the products take them.
+struct Sorted {
+    Tensor t;
+    int type;
+    const void* data;
+    int64_t stride;
+};
+Sorted expert_rows(const Tensor& given, const char* name) {
+    const Rows r = feature_rows(given, name);
+    return {r.t, r.type, r.t.const_data_ptr(), r.stride};
+}
+void to_grid(Sorted& r, Grid& grid) {
+    if (r.type == HB_F32 || r.t.numel() == 0) return;
+    if (off(r.data, 16) || r.stride > INT32_MAX || (r.t.size(0) > 1 && (r.stride % 8 != 0 || r.stride < r.t.size(1))))
+        grid.add(r.t, &r.data, &r.stride, nullptr);
 }
 struct Weight {
     Tensor t;
     hb_expert_weight w;
 };
-// [experts, hidden, width], or [hidden, width] of one expert, without a copy where its rows are contiguous (and on the grid).
-Weight expert_weight(const Tensor& given, const char* name, bool grid) {
+// [experts, hidden, width], or [hidden, width] of one expert, without a copy where its rows are contiguous.
+Weight expert_weight(const Tensor& given, const char* name) {
     TORCH_CHECK_VALUE(given.dim() == 3 || given.dim() == 2, name, " must be [experts, hidden, width], or [hidden, width] of one expert, got ",
                       given.sizes());
-    const int type = type_of(given, name);
+    type_of(given, name);
     Tensor t = resolved(given.dim() == 3 ? given : given.unsqueeze(0));
     const int64_t experts = t.size(0), hidden = t.size(1), width = t.size(2);
     TORCH_CHECK_VALUE(hidden >= 1 && width >= 1 && experts >= 1, name, " must have elements, got ", given.sizes());
-    auto plain = [&](const Tensor& v) {
-        return (width == 1 || v.stride(2) == 1) && (hidden == 1 || v.stride(1) >= width) && v.stride(0) < (int64_t(1) << 38) &&
-               v.stride(1) <= INT32_MAX;
-    };
-    if (!plain(t)) t = t.contiguous();
-    if (grid && type != HB_F32 &&
-        (off(t.const_data_ptr(), 16) || (hidden > 1 && t.stride(1) % 8 != 0) || (experts > 1 && t.stride(0) % 8 != 0)))
-        t = on_grid(t);
-    return {t, {t.const_data_ptr(), hidden > 1 ? t.stride(1) : on_eight(width), t.stride(0)}};
+    const bool plain = (width == 1 || t.stride(2) == 1) && (hidden == 1 || (t.stride(1) >= width && t.stride(1) <= INT32_MAX)) &&
+                       (experts == 1 || t.stride(0) < (int64_t(1) << 38));
+    if (!plain) t = t.contiguous();
+    return {t, {t.const_data_ptr(), hidden > 1 ? t.stride(1) : on_eight(width), experts > 1 ? t.stride(0) : 0}};
+}
+void to_grid(Weight& w, Grid& grid) {
+    if (w.t.scalar_type() == at::kFloat) return;
+    if (off(w.w.data, 16) || (w.t.size(1) > 1 && w.t.stride(1) % 8 != 0) || (w.t.size(0) > 1 && w.t.stride(0) % 8 != 0))
+        grid.add(w.t, &w.w.data, &w.w.row_stride, &w.w.expert_stride);
 }
 int activation_of(PyObject* o) {
     const char* name = PyUnicode_Check(o) ? PyUnicode_AsUTF8(o) : "";
@@ -578,7 +611,7 @@ const int32_t* first_rows(const Tensor& offsets, int64_t experts, const char* wh
     return offsets.const_data_ptr<int32_t>();
 }
 // Shapes that belong together: x [rows, width], weights [experts, hidden, width], dy [rows, hidden].
-hb_expert_shape shape_of(const Rows& x, std::initializer_list<const Weight*> weights, const Rows* dy, int activation, const char* what) {
+hb_expert_shape shape_of(const Sorted& x, std::initializer_list<const Weight*> weights, const Sorted* dy, int activation, const char* what) {
     const Weight& w = **weights.begin();
     const int64_t experts = w.t.size(0), hidden = w.t.size(1), width = w.t.size(2), rows = x.t.size(0);
     for (const Weight* v : weights)
@@ -602,13 +635,14 @@ PyObject* expert_product(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return wrap(unlocked([&] {
         const c10::Device device = device_of(what, {&given, &given_weight, offsets.defined() ? &offsets : &given});
         const Launch on(device);
-        const bool grid = given.dim() == 2 && given.size(0) > HB_EXPERT_FEW_ROWS;
-        const Rows x = expert_rows(given, "x", grid);
-        const Weight w = expert_weight(given_weight, "weight", grid);
+        Sorted x = expert_rows(given, "x");
+        Weight w = expert_weight(given_weight, "weight");
         const hb_expert_shape shape = shape_of(x, {&w}, nullptr, HB_SILU, what);
         const int32_t* first = first_rows(offsets, shape.experts, what);
+        Grid grid;
+        if (!hb_expert_any_grid(&shape, 1)) to_grid(x, grid), to_grid(w, grid), grid.copy(on);
         Tensor out = at::empty({shape.rows, shape.hidden}, x.t.options());
-        check(hb_expert_product(&shape, x.t.const_data_ptr(), x.stride, first, &w.w, out.data_ptr(), on.stream));
+        check(hb_expert_product(&shape, x.data, x.stride, first, &w.w, out.data_ptr(), on.stream));
         return out;
     }));
     END_HANDLE_TH_ERRORS
@@ -625,13 +659,14 @@ PyObject* expert_gated(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return wrap(unlocked([&] {
         const c10::Device device = device_of(what, {&given, &given_gate, &given_up, offsets.defined() ? &offsets : &given});
         const Launch on(device);
-        const bool grid = given.dim() == 2 && given.size(0) > HB_EXPERT_FEW_ROWS;
-        const Rows x = expert_rows(given, "x", grid);
-        const Weight g = expert_weight(given_gate, "w_gate", grid), u = expert_weight(given_up, "w_up", grid);
+        Sorted x = expert_rows(given, "x");
+        Weight g = expert_weight(given_gate, "w_gate"), u = expert_weight(given_up, "w_up");
         const hb_expert_shape shape = shape_of(x, {&g, &u}, nullptr, activation, what);
         const int32_t* first = first_rows(offsets, shape.experts, what);
+        Grid grid;
+        if (!hb_expert_any_grid(&shape, 2)) to_grid(x, grid), to_grid(g, grid), to_grid(u, grid), grid.copy(on);
         Tensor out = at::empty({shape.rows, shape.hidden}, x.t.options());
-        check(hb_expert_gated(&shape, x.t.const_data_ptr(), x.stride, first, &g.w, &u.w, out.data_ptr(), on.stream));
+        check(hb_expert_gated(&shape, x.data, x.stride, first, &g.w, &u.w, out.data_ptr(), on.stream));
         return out;
     }));
     END_HANDLE_TH_ERRORS
@@ -658,16 +693,21 @@ PyObject* expert_product_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
     unlocked([&] {
         const c10::Device device = device_of(what, {&given, &given_dy, &given_weight, offsets.defined() ? &offsets : &given});
         const Launch on(device);
-        const Rows dy = expert_rows(given_dy, "dy", true), x = expert_rows(given, "x", need_w);
-        const Weight w = expert_weight(given_weight, "weight", need_x);
+        Sorted dy = expert_rows(given_dy, "dy"), x = expert_rows(given, "x");
+        Weight w = expert_weight(given_weight, "weight");
         const hb_expert_shape shape = shape_of(x, {&w}, &dy, HB_SILU, what);
         const int32_t* first = first_rows(offsets, shape.experts, what);
         if (need_x) dx = at::empty({shape.rows, shape.width}, x.t.options());
         if (need_w) dw = at::empty(given_weight.sizes(), x.t.options());
+        Grid grid;
+        if (need_x || need_w) to_grid(dy, grid);
+        if (need_w) to_grid(x, grid);
+        if (need_x) to_grid(w, grid);
+        grid.copy(on);
         const size_t size = need_w ? hb_expert_product_grad_workspace(&shape) : 0;
         Tensor ws;
         if (size) ws = workspace(size, device);
-        check(hb_expert_product_grad(&shape, dy.t.const_data_ptr(), dy.stride, x.t.const_data_ptr(), x.stride, first, &w.w,
+        check(hb_expert_product_grad(&shape, dy.data, dy.stride, x.data, x.stride, first, &w.w,
                                      need_x ? dx.data_ptr() : nullptr, need_w ? dw.data_ptr() : nullptr, size ? ws.data_ptr() : nullptr, size,
                                      on.stream));
     });
@@ -690,17 +730,20 @@ PyObject* expert_gated_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
     unlocked([&] {
         const c10::Device device = device_of(what, {&given, &given_dh, &given_gate, &given_up, offsets.defined() ? &offsets : &given});
         const Launch on(device);
-        const Rows dh = expert_rows(given_dh, "dh", false), x = expert_rows(given, "x", true);
-        const Weight g = expert_weight(given_gate, "w_gate", true), u = expert_weight(given_up, "w_up", true);
+        const Sorted dh = expert_rows(given_dh, "dh");
+        Sorted x = expert_rows(given, "x");
+        Weight g = expert_weight(given_gate, "w_gate"), u = expert_weight(given_up, "w_up");
         const hb_expert_shape shape = shape_of(x, {&g, &u}, &dh, activation, what);
         const int32_t* first = first_rows(offsets, shape.experts, what);
         if (need_x) dx = at::empty({shape.rows, shape.width}, x.t.options());
         if (need_g) dg = at::empty(given_gate.sizes(), x.t.options());
         if (need_u) du = at::empty(given_up.sizes(), x.t.options());
         if (!need_x && !need_g && !need_u) return;
+        Grid grid;
+        to_grid(x, grid), to_grid(g, grid), to_grid(u, grid), grid.copy(on);
         const size_t size = hb_expert_gated_grad_workspace(&shape);
         Tensor ws = workspace(size, device);
-        check(hb_expert_gated_grad(&shape, dh.t.const_data_ptr(), dh.stride, x.t.const_data_ptr(), x.stride, first, &g.w, &u.w,
+        check(hb_expert_gated_grad(&shape, dh.data, dh.stride, x.data, x.stride, first, &g.w, &u.w,
                                    need_x ? dx.data_ptr() : nullptr, need_g ? dg.data_ptr() : nullptr, need_u ? du.data_ptr() : nullptr,
                                    ws.data_ptr(), size, on.stream));
     });

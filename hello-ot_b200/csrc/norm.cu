@@ -517,10 +517,10 @@ void for_width(int64_t width, F&& f) {
 constexpr int64_t kMostHeld = 16384;  // columns of a row that for_width holds
 constexpr int kParts = 148 * 8;       // most blocks that sum dw
 
-// Blocks that sum dw: as many as are resident, each with at least 4 turns.
+// Blocks that sum dw: as many as are resident, or a row each.
 inline int parts_of(int64_t rows, int threads) {
     const int64_t side = block_of(threads) / threads, blocks = 148 * resident(threads);
-    return (int)std::max<int64_t>(1, std::min(blocks, (rows + 4 * side - 1) / (4 * side)));
+    return (int)std::max<int64_t>(1, std::min(blocks, (rows + side - 1) / side));
 }
 
 inline bool bad_rows(const void* p, int64_t stride, int type) {

@@ -433,10 +433,11 @@ int hb_clip_grad_norm(int64_t count, const void* const* grads, const int64_t* si
  *   dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x.
  * offsets (device, experts + 1): expert e's rows are offsets[e]..offsets[e+1]-1, from 0 on; it is read as its
  * running maximum within 0..rows.  Rows behind the last expert's give zero rows and are not read; null: one expert
- * has all rows.  Sums are fp32, results rounded once.  Outputs are dense; null gradients are not computed.  Above
- * HB_EXPERT_FEW_ROWS rows, and for gradients, 16-bit operands lie on 16 bytes, their rows (distances, in elements, at
- * least the row's length) and experts too, but for dh.  Experts: at most 2048.  Nothing waits and nothing is kept. */
-#define HB_EXPERT_FEW_ROWS 16
+ * has all rows.  Sums are fp32, results rounded once.  Outputs are dense; null gradients are not computed.
+ * 16-bit operands of gradients (but for dh), and those of calls for which hb_expert_any_grid (weights: 1 of the product,
+ * 2 of the gated form) is 0, lie on 16 bytes, their rows (distances, in elements, at least the row's length) and experts
+ * too; hb_expert_copy brings up to three 16-bit operands [groups][rows][width] there in one launch.
+ * Experts: at most 2048; width and hidden: at most 2^21.  Nothing waits and nothing is kept. */
 enum { HB_SILU = 0, HB_GELU = 1 }; /* g / (1 + exp(-g)); g (1 + erf(g / sqrt 2)) / 2 */
 typedef struct hb_expert_shape {
     int64_t rows, width, hidden, experts; /* sorted rows; weights [experts][hidden][width] */
@@ -446,6 +447,9 @@ typedef struct hb_expert_weight {
     const void* data;
     int64_t row_stride, expert_stride; /* elements */
 } hb_expert_weight;
+int hb_expert_any_grid(const hb_expert_shape* shape, int weights);
+int hb_expert_copy(int64_t count, const void* const* from, const int64_t* groups, const int64_t* rows, const int64_t* width,
+                   const int64_t* group_stride, const int64_t* row_stride, void* const* to, const int64_t* to_stride, void* stream);
 int hb_expert_product(const hb_expert_shape* shape, const void* x, int64_t x_stride, const int32_t* offsets,
                       const hb_expert_weight* weight, void* out, void* stream);
 int hb_expert_gated(const hb_expert_shape* shape, const void* x, int64_t x_stride, const int32_t* offsets,
