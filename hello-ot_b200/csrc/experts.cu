@@ -342,10 +342,21 @@ __device__ __forceinline__ void multiply(const Params& p, Smem& s, uint32_t tmem
         else mma_commit(bar);
     };
     uint32_t stage = 0, phase = 0, done = 0;
-    const int units = tiles_of<FORM, PAIR>(p, s);
-    for (int u = blockIdx.x / (PAIR ? 2 : 1); u < units; u += gridDim.x / (PAIR ? 2 : 1)) {
-        const int blocks = tile_at<FORM, PAIR>(p, s, u, 0).blocks;
-        if (blocks == 0) continue;
+    const int units = tiles_of<FORM, PAIR>(p, s), step = gridDim.x / (PAIR ? 2 : 1);
+    // Stages of a tile; the next tile's are looked up while this one's products are under way.
+    const int summed = FORM == kWeights ? 0 : s.tile[p.groups] * p.col_tiles, each = p.segments * ((p.k + BK - 1) / BK);
+    auto blocks_of = [&](int u) {
+        if (u >= units) return 0;
+        if constexpr (FORM == kWeights) return tile_at<FORM, PAIR>(p, s, u, 0).blocks;
+        else return u < summed ? each : 0;
+    };
+    int u = blockIdx.x / (PAIR ? 2 : 1), blocks = blocks_of(u);
+    for (; u < units; u += step) {
+        if (blocks == 0) {
+            blocks = blocks_of(u + step);
+            continue;
+        }
+        int next = 0;
         const uint32_t buf = done & 1;
         if (!wait<PAIR>(&s.tempty[buf], ((done >> 1) & 1) ^ 1, s)) return;
         tc_fence_after();
@@ -363,9 +374,11 @@ __device__ __forceinline__ void multiply(const Params& p, Smem& s, uint32_t tmem
             }
             commit(&s.empty[stage]);
             if (++stage == kStages) stage = 0, phase ^= 1;
+            if (kb == 0) next = blocks_of(u + step);
         }
         commit(&s.tfull[buf]);
         ++done;
+        blocks = next;
     }
 }
 
@@ -901,7 +914,7 @@ struct Copies {
     uint16_t* to[3];
     int64_t row[3], group[3], to_row[3];
     int64_t rows[3], first[3];  // rows of a group; first row of the operand among all
-    int width[3], count;
+    int width[3], pairs[3], count;  // pairs: the source's rows lie on 4 bytes
 };
 __global__ void __launch_bounds__(256) copy_kernel(const __grid_constant__ Copies c, int64_t total) {
     const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -911,8 +924,15 @@ __global__ void __launch_bounds__(256) copy_kernel(const __grid_constant__ Copie
     const int64_t at = r - c.first[i], g = at / c.rows[i];
     const uint16_t* from = c.from[i] + g * c.group[i] + (at - g * c.rows[i]) * c.row[i];
     uint16_t* to = c.to[i] + at * c.to_row[i];
+    int k = threadIdx.x & 31;
+    if (c.pairs[i]) {
+        const int words = c.width[i] >> 1;
 #pragma unroll 4
-    for (int k = threadIdx.x & 31; k < c.width[i]; k += 32) to[k] = from[k];
+        for (; k < words; k += 32) reinterpret_cast<uint32_t*>(to)[k] = __ldcs(reinterpret_cast<const uint32_t*>(from) + k);
+        k = words * 2 + (threadIdx.x & 31);  // an odd width's last
+    }
+#pragma unroll 4
+    for (; k < c.width[i]; k += 32) to[k] = from[k];
 }
 }  // namespace experts
 }  // namespace hb
@@ -939,6 +959,8 @@ extern "C" int hb_expert_copy(int64_t count, const void* const* from, const int6
         c.to_row[at] = to_stride[i];
         c.rows[at] = rows[i];
         c.width[at] = (int)width[i];
+        c.pairs[at] = (rows::address_bits(from[i]) | rows::address_bits(to[i]) |
+                       (uint64_t)(row_stride[i] | group_stride[i] | to_stride[i]) * 2) % 4 == 0;
         c.first[at] = total;
         total += groups[i] * rows[i];
     }
