@@ -56,9 +56,11 @@ def adamw_step(params, grads, state, *, lr, betas=(0.9, 0.999), eps: float = 1e-
 
     grads: of their parameters' types or float32, unchanged.  ``norm`` (float32 on the device, ``grad_norm``'s) with
     ``max_norm`` scales them by min(1, max_norm / (norm + 1e-6)) on the way, which saves ``clip_grad_norm``'s pass.
-    lr: a number, or one float32 value on the device that a captured step reads anew.  Every operation is rounded to
-    float32; parameters without a master are rounded to their own type.  Tensors that are written share no memory with
-    others of the call.  A norm or gradient that is not a number makes what it reaches that, states included."""
+    lr: a number, or one float32 value on the device that a captured step reads anew.  m and v are rounded to float32 at
+    every operation; the change of p is within 2^-19 of itself, and its divisor at least 2^-63; parameters without a
+    master are rounded to their own type.  eps: 0 to 1e30.  Tensors that are written share no memory with others of the
+    call.  A norm or gradient that is not a number makes what it reaches that, states included: in 8 bits the 256
+    elements that share its scale."""
     host().adamw_step(params, grads, *state[:6], lr, *betas, eps, weight_decay, norm, max_norm)
 
 

@@ -415,7 +415,7 @@ __device__ __forceinline__ void step_chunk(const Entry& e, int64_t from, int64_t
         for (uint32_t stage = 0; stage < stages; ++stage) {
             const uint32_t slot = stage % kRing, turn = stage / kRing & 1;
             // a wait that gave up makes the parameters NaN
-            if (!mbar_wait(&ring.full[slot], turn, &ring.abort, &ring.status)) now.rate = __int_as_float(0x7fc00000);
+            if (!mbar_wait_timed<false>(&ring.full[slot], turn, &ring.abort, &ring.status)) now.rate = __int_as_float(0x7fc00000);
             Lane<BITS, TS, TG> here;
             here.load(piece(stage), block);
             __syncwarp();
@@ -424,7 +424,7 @@ __device__ __forceinline__ void step_chunk(const Entry& e, int64_t from, int64_t
             // refilled a turn late, when the other warps have long read it
             if (threadIdx.x == 0 && stage > 0 && stage - 1 + kRing < stages) {
                 const uint32_t last = stage - 1;
-                if (mbar_wait(&ring.empty[last % kRing], last / kRing & 1, &ring.abort, &ring.status)) bring(last + kRing);
+                if (mbar_wait_timed<false>(&ring.empty[last % kRing], last / kRing & 1, &ring.abort, &ring.status)) bring(last + kRing);
             }
         }
         for (block += stages * kWarps; block < whole; block += kWarps) {

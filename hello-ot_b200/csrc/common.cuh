@@ -105,6 +105,36 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
     return false;
 }
 
+// A wait that ends after 10 seconds, or once another thread raised *abort: for waits as long as a tile's whole sum, which
+// a count of tries does not bound (a try may end long before the time that it was given).  CLUSTER: another CTA of
+// the cluster arrives on the barrier too.
+template <bool CLUSTER>
+__device__ __forceinline__ bool mbar_wait_timed(uint64_t* bar, uint32_t parity, volatile int* abort, int* status) {
+    uint64_t start = 0;
+    for (uint32_t it = 0; it < 0xffffffffu; ++it) {
+        uint32_t ok;
+        if constexpr (CLUSTER)
+            asm volatile(
+                "{\n\t.reg .pred p;\n\t"
+                "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+                "selp.b32 %0, 1, 0, p;\n\t}"
+                : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u) : "memory");
+        else
+            ok = mbar_try_wait(bar, parity);
+        if (ok) return true;
+        if (*abort) return false;
+        if ((it & 63) == 63) {
+            uint64_t now;
+            asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+            if (start == 0) start = now;
+            else if (now - start > 10000000000ull) break;
+        }
+    }
+    *abort = 1;
+    atomicOr(status, kErrWaitTimeout);
+    return false;
+}
+
 // ---------------------------------------------------------------- TMA
 __device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
     asm volatile(

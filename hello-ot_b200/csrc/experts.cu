@@ -5,14 +5,22 @@
 //   backward  dx[r] = dy[r] W[e],  dW[e] = sum over the expert's rows of dy[r]^T x[r]; of the gated form
 //             dg = dh u act'(g), du = dh act(g), dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x
 //
-// One persistent kernel per product: a TMA producer, one thread that issues tcgen05.mma, eight warps that
+// One persistent kernel per product: a TMA producer, one thread that issues tcgen05.mma, 16 warps that
 // read the accumulators.  A CTA pair (cta_group::2) takes a tile of 256 x 256 of the output, each CTA with
-// its own 128 rows of one operand and 128 of the other's 256, 64 of the summed length a stage, six stages;
-// the accumulators are fp32 in TMEM, twice, so that a tile is written while the next one is summed.  In the
-// gated forms the even CTA brings 128 rows of Wg and the odd one the same rows of Wu: columns 0-127 of the
-// accumulator are g, 128-255 are u, and one thread holds both of a place, so g and u never leave the chip.
-// The gradients compute g and u again: it costs 2 of 6 products, and saves two arrays of rows x hidden that,
-// kept in 16 bits, would put two more roundings into every gradient.
+// its own 128 rows of one operand and 128 of the other's 256, 64 of the summed length a stage, five stages;
+// the accumulators are fp32 in TMEM, twice, so that a tile is written while the next one is summed.  Experts
+// of up to 128 rows on average take single CTAs and tiles of 128 x 128, where half of a pair's rows
+// would be foreign (64 x 128 rows x 2048 x 1024 gated: 101 us, in pairs 119; 64 x 256 rows in pairs 121).
+// In the gated forms the even CTA brings 128 rows of Wg and the odd one the same rows of Wu: columns 0-127 of
+// the accumulator are g, 128-255 are u, and one thread holds both of a place, so g and u never leave the
+// chip.  The gradients compute g and u again: it costs 2 of 6 products, and saves two arrays of rows x hidden
+// that, kept in 16 bits, would put two more roundings into every gradient.
+//
+// Bound by the tensor cores from some hundred rows an expert on: 65536 rows of 32 experts, 2048 x 1024 bf16,
+// measured alone: product 199 us (1383 TFLOP/s), gated 385 (1428), gradients 240 (1147) and 221 (1245);
+// 16384 x 8192 x 8192 product 1445 us (1522).  With fewer rows the weights' bytes: 64 x 128 rows 101 us for
+// 537 MB.  What one product writes comes out of the same SM that sums the next, so short sums
+// (the gradients', 1024) stay further from the rate.
 //
 // The rows of an expert begin anywhere: TMA boxes may (only the innermost coordinate has to lie on 16
 // bytes), rows of the next expert that a tile's box brings along are summed and not written.  In the sum
@@ -96,23 +104,9 @@ __device__ __forceinline__ void load_4d_pair(void* dst, const CUtensorMap* map, 
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// A bounded wait on a barrier that the other CTA arrives on as well.
 template <bool PAIR>
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Smem& s) {
-    if constexpr (!PAIR) return mbar_wait(bar, parity, &s.abort, &s.status);
-    else for (int it = 0; it < 4000; ++it) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
-            "selp.b32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u) : "memory");
-        if (ok) return true;
-        if (*(volatile int*)&s.abort) return false;
-    }
-    s.abort = 1;
-    atomicOr(&s.status, kErrWaitTimeout);
-    return false;
+    return mbar_wait_timed<PAIR>(bar, parity, &s.abort, &s.status);
 }
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -846,7 +840,7 @@ int run(const Job& job, cudaStream_t st) {
 }
 
 // ---------------------------------------------------------------- checks of the C entries
-constexpr int64_t kMostWidth = 1 << 21;
+constexpr int64_t kMostWidth = 1 << 20;
 bool fits(const Operand& o, int type, int64_t cols, int64_t rows, bool weights, int64_t groups, bool grid) {
     const uint64_t size = rows::type_bytes(type), unit = grid && type != HB_F32 ? 16 : size;
     if (!o.p || rows::address_bits(o.p) % unit || o.row < 0 || o.row > INT32_MAX) return false;

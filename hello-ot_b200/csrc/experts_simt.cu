@@ -315,8 +315,8 @@ template <typename T, bool VECTORS, bool GATED>
 __global__ void __launch_bounds__(kFewThreads) few_kernel(const __grid_constant__ FewParams p) {
     using V = rows::Vec<T, 16>;
     __shared__ int found;
-    const int r0 = blockIdx.x, lane = threadIdx.x & 31;
-    const int col = blockIdx.y * kFewWarps + (threadIdx.x >> 5);
+    const int r0 = blockIdx.y, lane = threadIdx.x & 31;
+    const int col = blockIdx.x * kFewWarps + (threadIdx.x >> 5);
     int e = 0, count = p.rows - r0;
     if (p.offsets) {
         e = expert_of(p.offsets, p.groups, r0, &found);
@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(const __grid_constant_
 
 template <typename T>
 void launch_few(const FewParams& p, bool vectors, bool gated, cudaStream_t st) {
-    const dim3 grid(p.rows, (p.n + kFewWarps - 1) / kFewWarps);
+    const dim3 grid((p.n + kFewWarps - 1) / kFewWarps, p.rows);  // rows: at most 4 an expert, 8192
     if (vectors) {
         if (gated) few_kernel<T, true, true><<<grid, kFewThreads, 0, st>>>(p);
         else few_kernel<T, true, false><<<grid, kFewThreads, 0, st>>>(p);

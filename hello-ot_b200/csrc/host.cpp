@@ -700,7 +700,8 @@ PyObject* expert_product_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (need_x) dx = at::empty({shape.rows, shape.width}, x.t.options());
         if (need_w) dw = at::empty(given_weight.sizes(), x.t.options());
         Grid grid;
-        if (need_x || need_w) to_grid(dy, grid);
+        if (!need_x && !need_w) return;
+        to_grid(dy, grid);
         if (need_w) to_grid(x, grid);
         if (need_x) to_grid(w, grid);
         grid.copy(on);
@@ -928,6 +929,7 @@ std::vector<float*> scales_of(Step& s, PyObject* o, const char* name, bool write
 const float* device_number(Step& s, PyObject* o, const char* name) {
     const Tensor& t = s.on_device(o, name);
     TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat && t.numel() == 1, s.what, ": ", name, " on the device must be one float32 value");
+    TORCH_CHECK_VALUE(!(t.requires_grad() && c10::GradMode::is_enabled()), s.what, ": ", name, " is a number, not a tensor that takes a derivative");
     s.span(t, s.read);
     return static_cast<const float*>(t.const_data_ptr());
 }

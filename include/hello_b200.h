@@ -437,7 +437,7 @@ int hb_clip_grad_norm(int64_t count, const void* const* grads, const int64_t* si
  * 16-bit operands of gradients (but for dh), and those of calls for which hb_expert_any_grid (weights: 1 of the product,
  * 2 of the gated form) is 0, lie on 16 bytes, their rows (distances, in elements, at least the row's length) and experts
  * too; hb_expert_copy brings up to three 16-bit operands [groups][rows][width] there in one launch.
- * Experts: at most 2048; width and hidden: at most 2^21.  Nothing waits and nothing is kept. */
+ * Experts: at most 2048; width and hidden: at most 2^20.  Nothing waits and nothing is kept. */
 enum { HB_SILU = 0, HB_GELU = 1 }; /* g / (1 + exp(-g)); g (1 + erf(g / sqrt 2)) / 2 */
 typedef struct hb_expert_shape {
     int64_t rows, width, hidden, experts; /* sorted rows; weights [experts][hidden][width] */
@@ -481,7 +481,8 @@ int hb_rms_norm_grad(int type, const void* dy, int64_t dy_stride, const void* x,
 /* One AdamW step over `count` tensors (host arrays of device pointers, element counts and types):
  *   g' = f g, f = min(1, max_norm / (norm + 1e-6)) (norm, device, null: f = 1);  m = b1 m + (1 - b1) g';
  *   v = b2 v + (1 - b2) g'^2;  p = p (1 - lr decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
- * with every operation rounded to fp32, t = ++*step (device), and lr read from the device where rate is not null.
+ * with the moments rounded to fp32 at every operation, the change of p within 2^-19 of itself (a divisor below 2^-63
+ * counts as that), t = ++*step (device), and lr read from the device where rate is not null.
  * master (null: none) holds fp32 parameters, of which params receive the rounded values.  grads are of their
  * parameter's type or fp32.  bits 32: first and second hold m and v in fp32; bits 8: e4m3 codes of m and of sqrt(v),
  * each 256 elements with a scale of their own (first_scale, second_scale: fp32, largest magnitude / 448); a v above 0
