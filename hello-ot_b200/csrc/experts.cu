@@ -821,7 +821,11 @@ int run_pairs(const Job& job, cudaStream_t st) {
 
 int run(const Job& job, cudaStream_t st) {
     const bool row_form = job.form == kProduct || job.form == kGated;
-    cudaError_t e = cudaSuccess;
+    // a thread that has not used the device yet has no current context, which encoding a tensor map needs
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess) e = cudaSetDevice(device);
+    if (e != cudaSuccess) return abi_fail(HB_CUDA, std::string("expert product: ") + cudaGetErrorString(e));
     if (row_form && is_few(job.type, job.rows, job.groups, job.n, job.k, job.form == kGated ? 2 : 1)) e = few_rows(job, st);
     else if (job.type == HB_F32) e = product_f32(job, st);
     else {

@@ -141,6 +141,31 @@ def test_two_threads(hb, cuda):
     assert not failed
 
 
+def test_first_call_of_a_thread(hb, cuda):
+    """A thread that has not used the device before, as autograd's may be: every call finds it."""
+    x, gain, gate, up, down, first = _layer(hb, cuda, 400)
+    dy = torch.ones((400, 128), dtype=torch.bfloat16, device=cuda)
+    state = hb.adamw_state([gain.clone()], bits=8)
+    torch.cuda.synchronize()
+    calls = (lambda: hb.expert_product(x, gate, first), lambda: hb.expert_gated_grad(dy, x, gate, up, first), lambda: hb.rms_norm(x, gain),
+             lambda: hb.expert_product_grad(dy, x, gate, first), lambda: hb.rms_norm_grad(x, x, gain),
+             lambda: hb.adamw_step([gain.clone()], [gain], state, lr=0.1))
+    failed = []
+
+    def work(call):
+        try:
+            call()
+        except Exception as e:  # noqa: BLE001
+            failed.append(repr(e))
+
+    for call in calls:
+        t = threading.Thread(target=work, args=(call,))
+        t.start()
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+
+
 def test_tangents_and_traces(hb, cuda):
     """Forward mode is refused, nothing is dropped silently; a trace holds the calls that have an autograd function."""
     x, gain, gate, up, down, first = _layer(hb, cuda, 40, torch.float32)
