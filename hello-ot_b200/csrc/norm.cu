@@ -34,7 +34,7 @@ __device__ __forceinline__ int scale_byte(uint32_t bits) {
     return max(e, 1);  // 2^-126: no subnormal scale
 }
 __device__ __forceinline__ float scale_value(int byte) {
-    return byte == 255 ? __int_as_float(0x7fc00000) : byte == 0 ? 0.0f : __uint_as_float((uint32_t)byte << 23);
+    return byte == 255 ? __int_as_float(0x7fc00000) : byte == 0 ? 0x1p-127f : __uint_as_float((uint32_t)byte << 23);
 }
 __device__ __forceinline__ uint8_t to_code(float v) { return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3); }
 __device__ __forceinline__ float of_code(uint8_t c) {
@@ -106,8 +106,8 @@ __device__ __forceinline__ void write_8bit(const Forward& p, int64_t r, int c, c
     }
     if (!there) return;
     const int byte = scale_byte(most);
-    const float inverse = byte == 0 ? 0.0f : byte == 255 ? __int_as_float(0x7fc00000)
-                          : byte == 254 ? 0x1p-127f : __uint_as_float((uint32_t)(254 - byte) << 23);
+    // 2^(127 - byte); the largest byte of finite magnitudes is 247
+    const float inverse = byte == 0 ? 0.0f : byte == 255 ? __int_as_float(0x7fc00000) : __uint_as_float((uint32_t)(254 - byte) << 23);
     rows::Vec<uint8_t, N> code;
 #pragma unroll
     for (int j = 0; j < N; ++j) code.v[j] = to_code(y[j] * inverse);

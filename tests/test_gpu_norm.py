@@ -162,6 +162,18 @@ def test_extremes(hb, cuda):
         assert float(got.scales.float()[0, 0]) == scale and float(got.scales.float()[0, 1]) in (0.0, 2.0 ** -127)
 
 
+def test_every_code_and_scale(hb, cuda):
+    """Rows from elsewhere: each of the 256 codes with each of the 256 scales reads as the numbers that they are."""
+    codes = torch.arange(256, dtype=torch.int32, device=cuda).to(torch.uint8).repeat(256, 1)
+    scales = torch.arange(256, dtype=torch.int32, device=cuda).to(torch.uint8).view(256, 1).repeat(1, 8)
+    want = codes.view(torch.float8_e4m3fn).double() * torch.where(scales == 255, torch.nan, 2.0 ** (scales.double() - 127)).repeat_interleave(32, 1)
+    for out_type in ref.DTYPES:
+        for width in (256, 237):
+            values = codes[:, :width].contiguous().view(torch.float8_e4m3fn)
+            got = hb.rows_of_8bit((values, scales.view(torch.float8_e8m0fnu)), dtype=out_type)
+            assert torch.equal(got.nan_to_num(7.5), want[:, :width].float().to(out_type).nan_to_num(7.5))
+
+
 def test_graph_and_refusals(hb, cuda):
     x, r, w, dy, dsum = _data(cuda, 300, 256, torch.bfloat16, torch.float32)
     graph = torch.cuda.CUDAGraph()
