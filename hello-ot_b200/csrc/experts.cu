@@ -42,7 +42,7 @@ constexpr int BK = 64, kStages = 5, kEpiWarps = 16;
 // producer, issuer, writers, and in kWeights a warp that zeroes foreign rows
 constexpr int threads_of(int form) { return 64 + 32 * kEpiWarps + (form == kWeights ? 32 : 0); }
 constexpr int kTileBytes = 128 * BK * 2, kStageBytes = 2 * kTileBytes;
-constexpr int kBand = 8;  // row tiles that share a weight tile while it is in L2
+constexpr int kBand = 8;  // row tiles that share a weight tile while it is in L2 (16384 x 8192 x 8192 1445 us, with 4 1480, with 16 1460)
 
 struct Params {
     CUtensorMap a[2], b[2];
@@ -796,11 +796,14 @@ int run_form(const Job& job, cudaStream_t st) {
     return e == cudaSuccess ? HB_OK : abi_fail(HB_LAUNCH, std::string("expert product: ") + cudaGetErrorString(e));
 }
 
-// CTA pairs where their tiles are filled: by an expert's rows, or by the weight's two sides.
+// CTA pairs where their tiles are filled: by an expert's rows (both sides measured above), or by the weight's two sides.
 bool use_pairs(const Job& job) {
     return job.form == kWeights ? job.n > 128 && job.k > 128 : job.rows > 128 * (int64_t)job.groups;
 }
-// kWeights: parts of the rows, where the tiles alone leave most of the device idle and experts have many stages.
+// kWeights: parts of the rows, where the tiles alone leave most of the device idle and experts have many stages.  Parts
+// against none (us): 20000 x 1 x 48 x 142 bf16 25 and 134, 131072 x 1 x 2048 x 1024 422 and 658, 8198 x 8 x 257 x 129 f32
+// 35 and 45.  Parts of at least 4 stages instead of 16: 2000 x 1 x 512 x 512 bf16 19 (none: 21), but 3056 x 6 x 376 x 429
+// 27 and 21.
 constexpr int kSlots = 148, kLeastStages = 16;
 int splits_of(const Job& job) {
     const bool f32 = job.type == HB_F32, pair = !f32 && use_pairs(job);

@@ -128,7 +128,7 @@ __device__ __forceinline__ float activate(int kind, float g, float& slope) {
         if (SLOPE) bell = expf(-0.5f * g * g);
     } else {
         // The complement of the error function after Abramowitz and Stegun 7.1.26, off by at most 1.5e-7 of 1 (the gated
-        // product of 73879 x 6 x 190 x 696 f16, bound by erff, 141 -> 97 us)
+        // product of 73879 x 6 x 190 x 696 f16, which erff bound, 141 -> 105 us)
         const float x = fabsf(g) * 0.70710678118654752f;
         float t;
         asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(0.3275911f, x, 1.0f)));
@@ -143,14 +143,15 @@ __device__ __forceinline__ float activate(int kind, float g, float& slope) {
 
 // Whether a forward product streams the weights by warps (experts_simt.cu): few rows, or few for each expert in fp32 or where
 // there is little work.  Gated, streamed and in tiles (us): 64 x 64 x 512 x 512 f32 29 and 125, 128 x 64 41 and 126,
-// 273 x 73 x 25 x 24 f16 8.6 and 12.5; but 487 x 117 x 18 x 50 f16 18.7 and 14.7, 100 x 21 x 886 x 719 f32 above both.
+// 273 x 73 x 25 x 24 f16 8.6 and 12.5; but 487 x 117 x 18 x 50 f16 18.7 and 14.7, 200 x 4 x 128 x 128 f16 29 and 8.
 constexpr int64_t kFewRows = 16, kFewEach = 4, kFewWork = 1 << 24;  // rows, rows an expert, products
 inline bool is_few(int type, int64_t rows, int64_t experts, int64_t n, int64_t k, int weights) {
     return rows <= kFewRows || (rows <= kFewEach * experts && (type == HB_F32 || rows * n * k * weights <= kFewWork));
 }
 cudaError_t few_rows(const Job& job, cudaStream_t st);
 cudaError_t product_f32(const Job& job, cudaStream_t st);
-// The side of product_f32's tiles: 64 where tiles of 128 would leave SMs without one.
+// The side of product_f32's tiles: 64 where those of 128 would be fewer than 1.5 an SM.  Product, with 64 and 128 (us):
+// 8198 x 8 x 257 x 129 (136 tiles of 128) 31 and 37, 8192 x 8 x 512 x 512 (272 tiles) 117 and 103.
 int f32_tile(const Job& job);
 // Adds the parts of kWeights in order and rounds them once.
 cudaError_t join_parts(const Job& job, cudaStream_t st);

@@ -429,7 +429,7 @@ int f32_tile(const Job& job) {
     const int64_t cols = job.form == kGated || job.form == kGatedGrad ? 64 : 128, width = job.form == kWeights ? job.k : job.n;
     const int64_t tiles = (width + cols - 1) / cols *
                           (job.form == kWeights ? job.segments * (int64_t)job.groups * ((job.n + 127) / 128) : job.rows / 128 + job.groups / 2);
-    return tiles * (job.form == kWeights ? std::max<int64_t>(1, job.rows / job.groups / 1024) : 1) < 2 * 148 ? 64 : 128;
+    return tiles * (job.form == kWeights ? std::max<int64_t>(1, job.rows / job.groups / 1024) : 1) < 222 ? 64 : 128;
 }
 
 cudaError_t join_parts(const Job& job, cudaStream_t st) {
