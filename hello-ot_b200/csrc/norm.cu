@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(block_of(THREADS)) forward_kernel(const __grid
         const int64_t next = r + step;
         a.load(x + next * p.x_row, p.width, next < end);
         if (ADD) b.load(residual + next * p.residual_row, p.width, next < end);
-        if (ADD && p.total && there) {
+        if (p.total && there) {
 #pragma unroll
             for (int i = 0; i < R::HELD; ++i) {
                 const int c = (i * THREADS + t) * V::N;
