@@ -357,8 +357,9 @@ __device__ __forceinline__ void step_chunk(const Entry& e, int64_t from, int64_t
     T* const param = static_cast<T*>(e.param) + from;
     float* const master = e.master ? e.master + from : nullptr;
     Chunk<T, TS, TG> c{};
-    if constexpr (std::is_same<T, TS>::value) c.source = param;
-    else c.source = master;
+    if constexpr (!std::is_same<T, TS>::value) c.source = master;
+    else if constexpr (std::is_same<T, float>::value) c.source = master ? master : param;  // an fp32 parameter may have one too
+    else c.source = param;
     c.param = param;
     c.master = master;
     c.grad = static_cast<const TG*>(e.grad) + from;
