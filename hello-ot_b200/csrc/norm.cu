@@ -321,6 +321,10 @@ __device__ __forceinline__ float2 row_sums(float a, float b, float2* shared) {
     return s;
 }
 
+// r^3 mean(w dy x), one factor at a time: the mean grows as the row does, while r^3 alone leaves fp32's normal numbers from
+// rows of some 10^13 and 10^-13 on, whose squares it still sums.
+__device__ __forceinline__ float row_pull(float inverse, float mean) { return inverse * (inverse * (inverse * mean)); }
+
 // Resident blocks an SM: what the registers of a thread's columns leave (128 a thread, 80 with 8 columns).
 constexpr int resident(int threads, int columns) {
     return (columns <= 8 ? 768 : 512) / block_of(threads) > 1 ? (columns <= 8 ? 768 : 512) / block_of(threads) : 1;
@@ -380,7 +384,7 @@ __global__ void __launch_bounds__(block_of(THREADS), resident(THREADS, COLUMNS))
         }
         const float2 sums = row_sums<THREADS>(along, squares, shared);
         const float inverse = 1.0f / sqrtf(sums.y / (float)p.width + p.eps);
-        const float back = inverse * inverse * inverse * (sums.x / (float)p.width);
+        const float back = row_pull(inverse, sums.x / (float)p.width);
         if (r < p.rows) {
 #pragma unroll
             for (int i = 0; i < HELD; ++i) {
@@ -455,7 +459,7 @@ __global__ void __launch_bounds__(512) wide_sums_kernel(const __grid_constant__ 
     if (threadIdx.x == 0) {
         const float inverse = 1.0f / sqrtf(sums.x / (float)p.width + p.eps);
         p.stats[2 * r] = inverse;
-        p.stats[2 * r + 1] = inverse * inverse * inverse * (sums.y / (float)p.width);
+        p.stats[2 * r + 1] = row_pull(inverse, sums.y / (float)p.width);
     }
 }
 template <typename T, int VB>

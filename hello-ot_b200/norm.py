@@ -1,8 +1,9 @@
 """Root-mean-square norm of rows with the residual's addition, its output in 8 bits, and its gradients.
 
 Rows are the last dimension of tensors of any shape.  Sums are fp32, whatever the
-type, and results are rounded once.  Calls enqueue work on the current stream and
-never wait for the device.
+type, and results are rounded once; so a row's squares have to sum to an fp32 number
+(values of some 1e18 at most, and with eps 0 of some 1e-18 at least).  Calls enqueue
+work on the current stream and never wait for the device.
 """
 from __future__ import annotations
 

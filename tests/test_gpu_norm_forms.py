@@ -1,4 +1,4 @@
-"""The row norm where its forms differ: the sum without a residual."""
+"""The row norm where its forms differ: the sum without a residual, gradients of rows of very large and very small values."""
 import pytest
 import torch
 
@@ -29,3 +29,24 @@ def test_sum_without_a_residual(hb, cuda, width, dtype):
             assert torch.equal(codes, want.values.view(torch.uint8)) and torch.equal(scales, want.scales.view(torch.uint8))
         else:
             assert torch.equal(y, hb.rms_norm(x, w, eps=base.EPS))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("width", [7, 64, 2048, 16400])
+@pytest.mark.parametrize("size,eps", [(1e15, 1e-6), (1e17, 1e-6), (1e-14, 0.0), (1e-17, 0.0)])
+def test_gradients_of_large_and_small_rows(hb, cuda, size, eps, width, dtype):
+    """The row's length enters dx to the third power, which fp32 does not hold where it holds the squares' sum.  Bounds as in
+    test_gradients: the same sums, and fewer than 12 roundings beside them.  dy lies along x, so that the term counts."""
+    x, _, w, noise, _ = base._data(cuda, 3, width, dtype, torch.float32, scale=size)
+    dy = (x.double() / size + 0.25 * noise.double()).to(dtype)
+    x64, w64, g64 = x.double(), w.double(), dy.double()
+    inverse = (x64.square().mean(1, keepdim=True) + eps).rsqrt()
+    pull = (w64 * g64 * x64).mean(1, keepdim=True)
+    want = inverse * w64 * g64 - x64 * inverse ** 3 * pull
+    each, u = (width + 12) * ref.E32, ref.U[dtype]
+    mag = inverse * (w64 * g64).abs() + x64.abs() * inverse ** 3 * (w64 * g64 * x64).abs().mean(1, keepdim=True)
+    bound = 3 * each * mag + 2 * ref.E32 * want.abs()
+    dx, dw = hb.rms_norm_grad(dy, x, w, eps=eps)
+    close(dx, want, bound * (1 + u) + u * want.abs() + ref.FLOOR[dtype], "dx")
+    terms = g64 * x64 * inverse
+    close(dw, terms.sum(0), (3 + width / 2 + 12) * ref.E32 * terms.abs().sum(0) + ref.E32 * terms.sum(0).abs(), "dw")
