@@ -38,3 +38,28 @@ def test_gelu_of_far_values_in_32_bits(hb, cuda, rows):
     dx, dgate, dup = hb.expert_gated_grad(torch.ones((rows, 1), device=cuda), x, gate, up, activation="gelu")
     er.close(dx[:, 1], value, bound, "du")
     er.close(dx[:, 0], slope, 5 * e23 * cdf + (g.double().square() / 4 + 4) * e23 * bell + e23 * slope.abs(), "dg")
+
+
+@pytest.mark.parametrize("name", ["gelu", "silu"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows", [16, 4000])
+def test_activations_of_far_values_in_16_bits(hb, cuda, rows, dtype, name):
+    """Relative to the value: the approximations are within 2^-18 and the exponential's argument within 2 g^2 2^-24 (silu:
+    2 |g| 2^-23), the result is rounded once.  u lifts what fp16 would hold in fewer bits."""
+    left = -9.0 if dtype == torch.float16 else -12.5
+    g = torch.linspace(left, -0.001, rows, device=cuda).to(dtype).float()
+    lift = 2.0 ** 15
+    x, gate, up = _alone(cuda, g, dtype, lift)
+    value, slope, cdf, bell = _gelu(g)
+    if name == "silu":
+        value, slope = er.activation(g.double(), "silu")
+        cdf, bell = torch.sigmoid(g.double()), (g.double() * torch.sigmoid(g.double())).abs()
+    u, floor = ref.U[dtype], ref.FLOOR[dtype]
+    near = 2.0 ** -18 + 2 * g.double().square() * 2.0 ** -24 + 2 * g.double().abs() * er.E23
+    bound = lift * value.abs() * (near * (1 + u) + u) + floor
+    er.close(hb.expert_gated(x, gate, up, activation=name)[:, 0], lift * value, bound, name)
+    x[:, 1] = 1.0
+    dx, _, _ = hb.expert_gated_grad(torch.full((rows, 1), lift, device=cuda).to(dtype), x, gate, up, activation=name)
+    er.close(dx[:, 1], lift * value, bound, "du")
+    # dg passes on in dtype and its product is exact: rounded once
+    er.close(dx[:, 0], lift * slope, lift * (near * (cdf + bell) * (1 + u) + u * slope.abs()) + floor, "dg")
