@@ -562,12 +562,13 @@ struct Sorted {
     int64_t stride;
 };
 Sorted expert_rows(const Tensor& given, const char* name) {
-    const Rows r = feature_rows(given, name);
+    Rows r = feature_rows(given, name);
+    if (r.stride > INT32_MAX) r.t = r.t.contiguous(), r.stride = r.t.size(1);  // farther apart than the kernels step
     return {r.t, r.type, r.t.const_data_ptr(), r.stride};
 }
 void to_grid(Sorted& r, Grid& grid) {
     if (r.type == HB_F32 || r.t.numel() == 0) return;
-    if (off(r.data, 16) || r.stride > INT32_MAX || (r.t.size(0) > 1 && (r.stride % 8 != 0 || r.stride < r.t.size(1))))
+    if (off(r.data, 16) || (r.t.size(0) > 1 && (r.stride % 8 != 0 || r.stride < r.t.size(1))))
         grid.add(r.t, &r.data, &r.stride, nullptr);
 }
 struct Weight {

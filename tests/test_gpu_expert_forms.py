@@ -1,4 +1,4 @@
-"""The experts' products where their forms differ: activations of far values."""
+"""The experts' products where their forms differ: activations of far values, rows that lie far apart."""
 import math
 
 import pytest
@@ -63,3 +63,21 @@ def test_activations_of_far_values_in_16_bits(hb, cuda, rows, dtype, name):
     er.close(dx[:, 1], lift * value, bound, "du")
     # dg passes on in dtype and its product is exact: rounded once
     er.close(dx[:, 0], lift * slope, lift * (near * (cdf + bell) * (1 + u) + u * slope.abs()) + floor, "dg")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_far_apart(hb, cuda, dtype):
+    """Rows more than 2^31 elements apart are taken like any others."""
+    gen = torch.Generator(device=cuda).manual_seed(6)
+    apart, width = 2 ** 31 + 8, 24
+    room = torch.empty(apart + width, dtype=dtype, device=cuda)
+    far = room.as_strided((2, width), (apart, 1))
+    far.copy_(torch.randn((2, width), generator=gen, device=cuda))
+    near = far.contiguous()
+    gate, up = (torch.randn((2, width, width), generator=gen, device=cuda).to(dtype) for _ in range(2))
+    first = torch.tensor([0, 1, 2], dtype=torch.int32, device=cuda)
+    assert torch.equal(hb.expert_product(far, gate, first), hb.expert_product(near, gate, first))
+    assert torch.equal(hb.expert_gated(far, gate, up, first), hb.expert_gated(near, gate, up, first))
+    for got, want in ((hb.expert_product_grad(far, far, gate, first), hb.expert_product_grad(near, near, gate, first)),
+                      (hb.expert_gated_grad(far, far, gate, up, first), hb.expert_gated_grad(near, near, gate, up, first))):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
