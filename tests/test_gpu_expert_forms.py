@@ -1,4 +1,5 @@
-"""The experts' products where their forms differ: activations of far values, rows that lie far apart."""
+"""The experts' products where their forms differ: activations of far values, rows that lie far apart, tiles past the
+first band, parts of sums over pairs of blocks."""
 import math
 
 import pytest
@@ -81,3 +82,45 @@ def test_rows_far_apart(hb, cuda, dtype):
     for got, want in ((hb.expert_product_grad(far, far, gate, first), hb.expert_product_grad(near, near, gate, first)),
                       (hb.expert_gated_grad(far, far, gate, up, first), hb.expert_gated_grad(near, near, gate, up, first))):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# counts, rows behind the last, width, hidden.  Tiles of an expert come in bands of 8: several bands and a partial one with several
+# tiles of columns, in pairs of blocks and by single ones (few rows an expert on average); sums over rows cut into parts over
+# pairs; weights with more than one band of their own.
+BANDS = {
+    "bands of pairs": ([4500, 2300], 300, 264, 520),
+    "bands of single blocks": ([1300] + [0] * 9 + [60, 7], 20, 264, 392),
+    "parts over pairs": ([6000], 0, 264, 520),
+    "parts over pairs, uneven": ([9000, 17, 0, 3300], 5, 136, 200),
+    "bands of weights": ([200, 130], 0, 300, 2600),
+    "bands of wide rows": ([150, 300], 9, 2600, 264),
+}
+
+
+@pytest.mark.parametrize("dtype", ref.DTYPES)
+@pytest.mark.parametrize("shape", BANDS)
+def test_bands_and_parts(hb, cuda, shape, dtype):
+    counts, behind, width, hidden = BANDS[shape]
+    gen = torch.Generator(device=cuda).manual_seed(len(shape))
+    offsets, rows = er.groups(counts, behind)
+    first = torch.tensor(offsets, dtype=torch.int32, device=cuda)
+
+    def normal(*size, scale=1.0):
+        return (torch.randn(size, generator=gen, device=cuda) * scale).to(dtype)
+
+    x, dy = normal(rows, width), normal(rows, hidden)
+    gate, up = (normal(len(counts), hidden, width, scale=width ** -0.5) for _ in range(2))
+    x[offsets[-1]:], dy[offsets[-1]:] = float("nan"), float("inf")
+    x64, dy64 = x.double(), dy.double()
+    x64[offsets[-1]:], dy64[offsets[-1]:] = 0, 0
+    y = hb.expert_product(x, gate, first)
+    er.close(y, *er.product(x64, gate.double(), offsets, dtype), "product")
+    h = hb.expert_gated(x, gate, up, first)
+    er.close(h, *er.gated(x64, gate.double(), up.double(), offsets, "silu", dtype), "gated")
+    got = [*hb.expert_product_grad(dy, x, gate, first), *hb.expert_gated_grad(dy, x, gate, up, first)]
+    wants = [*er.product_grad(dy64, x64, gate.double(), offsets, dtype),
+             *er.gated_grad(dy64, x64, gate.double(), up.double(), offsets, "silu", dtype)]
+    for name, g, (want, bound) in zip(("dx", "dw", "gated dx", "dgate", "dup"), got, wants):
+        er.close(g, want, bound, name)
+    again = [*hb.expert_product_grad(dy, x, gate, first), *hb.expert_gated_grad(dy, x, gate, up, first)]
+    assert all(torch.equal(a, b) for a, b in zip(got, again)) and torch.equal(y, hb.expert_product(x, gate, first))
