@@ -1,4 +1,5 @@
-"""The row norm where its forms differ: the sum without a residual, gradients of rows of very large and very small values."""
+"""The row norm where its forms differ: the sum without a residual, gradients of rows of very large and very small values,
+every width that has a kernel of its own, views in 8 bits."""
 import pytest
 import torch
 
@@ -50,3 +51,41 @@ def test_gradients_of_large_and_small_rows(hb, cuda, size, eps, width, dtype):
     close(dx, want, bound * (1 + u) + u * want.abs() + ref.FLOOR[dtype], "dx")
     terms = g64 * x64 * inverse
     close(dw, terms.sum(0), (3 + width / 2 + 12) * ref.E32 * terms.abs().sum(0) + ref.E32 * terms.sum(0).abs(), "dw")
+
+
+# widths of each kernel's own: 2049 to 4096, 4097 to 8192 and 8193 to 16384 columns on and off the 16-byte grid, rows enough for
+# several of a block, in order (forward) and strided (gradients)
+FORMS = [(5, 4096), (5, 8192), (7, 1090), (7, 1091), (5, 3333), (5, 6002), (4, 12001), (40003, 64), (3001, 2048)]
+
+
+@pytest.mark.parametrize("dtype", ref.DTYPES)
+@pytest.mark.parametrize("rows,width", FORMS)
+def test_forms(hb, cuda, rows, width, dtype):
+    base.test_forward(hb, cuda, rows, width, dtype)
+    base.test_gradients(hb, cuda, rows, width, dtype)
+
+
+@pytest.mark.parametrize("dtype", ref.DTYPES)
+@pytest.mark.parametrize("width", [128, 101, 1090, 4500])
+def test_strides_in_8_bits(hb, cuda, width, dtype):
+    """Rows apart, off the grid, in another order, the same one again: the values that the codes stand for, within the
+    bounds of test_forward, and scales from both sides."""
+    x, r, w, _, _ = base._data(cuda, 40, width + 4, dtype, dtype)
+    for view in (lambda v: v[:, :width], lambda v: v[:, 2:width + 2], lambda v: v[:, 1:width + 1], lambda v: v.t().contiguous().t()[:, :width],
+                 lambda v: v[:1, :width].expand(40, width), lambda v: v[::2, :width]):
+        a, b, k = view(x), view(r), w[:width]
+        t = a.double() + b.double()
+        want = base._norm(t, k.double())
+        rows8, total = hb.rms_norm_8bit(a, k, b, eps=base.EPS)
+        close(total, t, ref.E32 * t.abs() + ref.U[dtype] * t.abs() * (1 + ref.E32) + ref.FLOOR[dtype], "sum")
+        most = torch.nn.functional.pad(want.abs(), (0, -width % 32)).view(len(want), -1, 32).amax(-1)
+        off = 1 + (width / 2 + 8) * ref.E32
+        floor = (2 * most * off / 448 * 2.0 ** -10).repeat_interleave(32, 1)[:, :width]
+        close(hb.rows_of_8bit(rows8), want, 2.0 ** -4 * want.abs() * off + floor + (width / 2 + 8) * ref.E32 * want.abs(), "8 bits")
+        scale = rows8.scales.float()
+        assert bool((scale >= most / 448 * (2 - off)).all()) and bool((scale < 2 * most / 448 * off).all())
+    # codes and scales that lie apart are read as their dense copies
+    wide = hb.rms_norm_8bit(x, w, r, eps=base.EPS)[0]
+    apart = (wide.values.view(torch.uint8).repeat(1, 2)[:, :width + 4].view(torch.float8_e4m3fn),
+             wide.scales.view(torch.uint8).repeat(1, 2)[:, :wide.scales.shape[1]].view(torch.float8_e8m0fnu))
+    assert not apart[0].is_contiguous() and torch.equal(hb.rows_of_8bit(apart), hb.rows_of_8bit(wide))
