@@ -7,7 +7,7 @@
 // all elements share (in fp64: t, the bias corrections, f), then a warp takes a block of 256 elements, 8 a lane.
 // The second launch starts while the first runs and waits for it when its first loads are on their way
 // (programmatic dependent launch).  Bound by HBM: every array passes once.  On a B200 400 million bf16 parameters with
-// masters and 8-bit states take 981 us (6.5 TB/s), 200 million in fp32 with fp32 states 818 us (6.8 TB/s).
+// masters and 8-bit states take 992 us (6.5 TB/s), 200 million in fp32 with fp32 states 818 us (6.8 TB/s).
 //
 // 8 bits: e4m3 codes of m and of sqrt(v) with a scale for each 256 elements (largest magnitude / 448).  The root
 // halves v's range of exponents, so e4m3's 2^17 between the largest and the smallest code are 2^34 of v; a v above

@@ -10,17 +10,18 @@
 // its own 128 rows of one operand and 128 of the other's 256, 64 of the summed length a stage, five stages;
 // the accumulators are fp32 in TMEM, twice, so that a tile is written while the next one is summed.  Experts
 // of up to 128 rows on average take single CTAs and tiles of 128 x 128, where half of a pair's rows
-// would be foreign (64 x 128 rows x 2048 x 1024 gated: 101 us, in pairs 119; 64 x 256 rows in pairs 121).
+// would be foreign (64 x 128 rows x 2048 x 1024 gated: 105 us, in pairs 120; 64 x 256 rows in pairs 124).
 // In the gated forms the even CTA brings 128 rows of Wg and the odd one the same rows of Wu: columns 0-127 of
 // the accumulator are g, 128-255 are u, and one thread holds both of a place, so g and u never leave the
 // chip.  The gradients compute g and u again: it costs 2 of 6 products, and saves two arrays of rows x hidden
-// that, kept in 16 bits, would put two more roundings into every gradient.
+// that, kept in 16 bits, would put two more roundings into every gradient.  dg and du do go through memory in
+// 16 bits, as operands of kind::f16 have to be: one rounding more, and a bf16 gradient's error from 0.0017 to 0.0023.
 //
 // Bound by the tensor cores from some hundred rows an expert on: 65536 rows of 32 experts, 2048 x 1024 bf16,
-// measured alone: product 199 us (1383 TFLOP/s), gated 385 (1428), gradients 240 (1147) and 221 (1245);
-// 16384 x 8192 x 8192 product 1445 us (1522).  With fewer rows the weights' bytes: 64 x 128 rows 101 us for
-// 537 MB.  What one product writes comes out of the same SM that sums the next, so short sums
-// (the gradients', 1024) stay further from the rate.
+// calls one after the other on three sets of inputs: product 206 us (1334 TFLOP/s), gated 396 (1388), dx 280 to 350
+// (982 to 785), dW 222 (1238); 16384 x 8192 x 8192 product 1445 us (1522).  With fewer rows the weights' bytes: 64 x 128
+// rows gated 105 us for 537 MB.  What one product writes comes out of the same SM that sums the next, so short
+// sums (dx's, 1024) stay further from the rate.
 //
 // The rows of an expert begin anywhere: TMA boxes may (only the innermost coordinate has to lie on 16
 // bytes), rows of the next expert that a tile's box brings along are summed and not written.  In the sum

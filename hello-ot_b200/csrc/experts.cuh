@@ -150,6 +150,8 @@ __device__ __forceinline__ float activate(int kind, float g, float& slope) {
 // Whether a forward product streams the weights by warps (experts_simt.cu): few rows, or few for each expert in fp32 or where
 // there is little work.  Gated, streamed and in tiles (us): 64 x 64 x 512 x 512 f32 29 and 125, 128 x 64 41 and 126,
 // 273 x 73 x 25 x 24 f16 8.6 and 12.5; but 487 x 117 x 18 x 50 f16 18.7 and 14.7, 200 x 4 x 128 x 128 f16 29 and 8.
+// The counts lie on the device, so the rule goes by their average: where one of 128 experts has all of 512 rows, 1024 x 1024
+// f32 takes 860 us, and 210 in tiles.
 constexpr int64_t kFewRows = 16, kFewEach = 4, kFewWork = 1 << 24;  // rows, rows an expert, products
 inline bool is_few(int type, int64_t rows, int64_t experts, int64_t n, int64_t k, int weights) {
     return rows <= kFewRows || (rows <= kFewEach * experts && (type == HB_F32 || rows * n * k * weights <= kFewWork));

@@ -5,14 +5,15 @@
 // order and write zeros for what is not there), three steps ahead; it holds 8 x 16 or 8 x 4 sums and adds products in
 // pairs (fma.rn.f32x2), each rounded like the scalar instruction, so the sums are plain fp32 sums.  Shared memory
 // returns 128 bytes a cycle, whatever the lanes share, and 8 x 8 sums want just that for 128 products a cycle: with
-// them 32768 x 2048 x 1024 ran at 47 TFLOP/s.  The tensor cores
+// them 32768 x 2048 x 1024 ran at 47 TFLOP/s, now at 53 (2603 us).  The tensor cores
 // would need three bf16 parts of each operand and cut off the low bits of their running sums, which fp32 results do
 // not allow.  In the gated forms half of a tile's columns are g's and half the same places of u, and one thread
 // holds both of a place.
 //
-// Few rows (few_rows): one token's step of a decode batch reads the named experts' weights once and is bound by that.  A warp streams the weight rows of one output column and multiplies
-// them with up to 8 rows of x, which stay in L1; a block of 8 warps takes 8 columns for the rows of one expert,
-// which the expert's first row finds out for itself.
+// Few rows (few_rows): one token's step of a decode batch reads the named experts' weights once and is bound by that.
+// A warp streams the weight rows of one output column and multiplies them with up to 8 rows of x, which
+// stay in L1; a block of 8 warps takes 8 columns for the rows of one expert, which the expert's first row finds out for
+// itself.
 #include <algorithm>
 #include <string>
 
@@ -313,8 +314,8 @@ __device__ __forceinline__ void load_piece(rows::Vec<T, 16>& v, const T* row, in
     }
 }
 
-// Four blocks an SM and two pieces of a row in flight; two blocks with four pieces took 33 us where this takes 25 (16 rows of
-// 16 experts, 2048 x 1024 bf16).
+// Four blocks an SM and two pieces of a row in flight; two blocks with four pieces took 33 us where this takes 25, and 51 where
+// it takes 37 (16 rows of 16 experts, 2048 x 1024 bf16, on two machines).
 template <typename T, bool VECTORS, bool GATED>
 __global__ void __launch_bounds__(kFewThreads, 4) few_kernel(const __grid_constant__ FewParams p) {
     using V = rows::Vec<T, 16>;

@@ -437,7 +437,7 @@ int hb_clip_grad_norm(int64_t count, const void* const* grads, const int64_t* si
  * 16-bit operands of gradients (but for dh), and those of calls for which hb_expert_any_grid (weights: 1 of the product,
  * 2 of the gated form) is 0, lie on 16 bytes, their rows (distances, in elements, at least the row's length) and experts
  * too; hb_expert_copy brings up to three 16-bit operands [groups][rows][width] there in one launch.
- * Experts: at most 2048; width and hidden: at most 2^20.  Nothing waits and nothing is kept. */
+ * Experts: at most 2048; width and hidden: at most 2^20; rows less than 2^31 elements apart.  Nothing waits and nothing is kept. */
 enum { HB_SILU = 0, HB_GELU = 1 }; /* g / (1 + exp(-g)); g (1 + erf(g / sqrt 2)) / 2 */
 typedef struct hb_expert_shape {
     int64_t rows, width, hidden, experts; /* sorted rows; weights [experts][hidden][width] */
